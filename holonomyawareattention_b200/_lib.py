@@ -16,9 +16,10 @@ HOA_F32, HOA_BF16 = 0, 1
 HOA_GEN_BANKED = 0x100        # generator layout flag OR'ed into a_dtype
 # status codes (include/hoa.h)
 (HOA_OK, HOA_ERR_INVALID_ARG, HOA_ERR_UNSUPPORTED, HOA_ERR_LAUNCH, HOA_ERR_WORKSPACE, HOA_ERR_TIMEOUT,
- HOA_ERR_BOUNDS) = range(7)
+ HOA_ERR_BOUNDS, HOA_ERR_PAGES) = range(8)
 
 c_int, c_float, c_size_t, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_ll = ctypes.c_longlong
 
 # name -> (restype, argtypes); mirrors include/hoa.h
 SIGNATURES = {
@@ -64,6 +65,23 @@ SIGNATURES = {
                                      c_void_p]),
     "hoa_edge_gemm_fp8_acc": (c_int, [c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_void_p,
                                       c_size_t, c_void_p]),
+    "hoa_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "hoa_pages_reserve": (c_int, [c_void_p] * 7 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hoa_pages_fork": (c_int, [c_void_p] * 5 + [c_int] + [c_void_p] * 3 + [c_int] * 4 + [c_void_p] * 3 + [c_int]
+                       + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hoa_pages_free": (c_int, [c_void_p] * 4 + [c_int] + [c_void_p] * 3 + [c_int] * 4 + [c_void_p] * 2),
+    "hoa_pages_compact": (c_int, [c_void_p] * 5 + [c_int] * 3 + [c_void_p] * 3 + [c_int]
+                          + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hoa_pages_copy": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 2 + [c_void_p] * 2),
+    "hoa_pages_write": (c_int, [c_void_p] * 2 + [c_int] + [c_void_p] * 4 + [c_int, c_void_p, c_void_p, c_ll, c_void_p]
+                        + [c_int] * 7 + [c_void_p] * 2),
+    "hoa_paged_attn_workspace_bytes": (c_size_t, [c_int] * 9),
+    "hoa_paged_attn_fwd": (c_int, [c_void_p] * 5 + [c_int, c_void_p, c_int, c_void_p, c_ll, c_int, c_void_p, c_void_p,
+                                   c_void_p, c_int, c_void_p, c_float] + [c_int] * 8
+                           + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "hoa_path_step": (c_int, [c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int, c_ll, c_void_p,
+                              c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_int, c_void_p] + [c_int] * 5
+                      + [c_void_p] * 2),
 }
 
 _lock = threading.Lock()

@@ -985,6 +985,7 @@ extern "C" const char* hoa_status_string(int st) {
     case HOA_ERR_WORKSPACE: return "workspace too small";
     case HOA_ERR_TIMEOUT: return "device-side wait timed out";
     case HOA_ERR_BOUNDS: return "device-side index check failed (debug build)";
+    case HOA_ERR_PAGES: return "no free page, or a row or page outside the cache";
     default: return "unknown status";
   }
 }

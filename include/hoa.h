@@ -52,7 +52,8 @@ typedef enum {
   HOA_ERR_LAUNCH = 3,        /* CUDA launch failed (cudaGetLastError)       */
   HOA_ERR_WORKSPACE = 4,     /* workspace too small                          */
   HOA_ERR_TIMEOUT = 5,       /* a bounded device-side wait gave up           */
-  HOA_ERR_BOUNDS = 6         /* debug build: a device-side index check failed */
+  HOA_ERR_BOUNDS = 6,        /* debug build: a device-side index check failed */
+  HOA_ERR_PAGES = 7          /* cache: no free page, or a row or page outside it */
 } hoa_status;
 
 typedef enum { HOA_F32 = 0, HOA_BF16 = 1 } hoa_dtype;
@@ -336,6 +337,105 @@ int hoa_edge_gelu_split8(const float* h, void* hi, void* lo, long long rows, int
                          void* stream);
 int hoa_edge_gemm_fp8_acc(const void* lo, const void* w, float* out, float alpha, int M, int N, int K,
                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * Generation: pages of a cache, attention over them, and the path step of one
+ * token.  No counterpart in the reference, which recomputes the whole sequence:
+ * k^_t = P_t^T k_t and v^_t = P_t^T v_t are in the gauge of their sequence's
+ * origin, so a token's k^ and v^ never change as the sequence grows, and
+ * sequences with a common beginning share them.
+ *
+ * A pool holds pages (n_pages, H, page, d) of fp32 or bf16, innermost dimension
+ * contiguous; k and v pools of a call have the same `page_strides` (elements:
+ * page, head, token).  Bookkeeping is int32 on the device: table (S, W) the page
+ * ids of each row in order, -1 beyond its last; lens (S) its tokens; refs
+ * (n_pages) the rows that hold a page (0: free).  Row s uses ceil(lens[s] / page)
+ * entries.  Page ids and rows read from device memory are checked by the kernels:
+ * one outside the cache is not followed, and sets HOA_ERR_PAGES in `status`
+ * (nullable; device or mapped host int, only ever set; known once the stream has
+ * completed).
+ * ---------------------------------------------------------------------------
+ *
+ * The bookkeeping entry points read one state and write the next one to other
+ * buffers (same shapes), in one launch; free pages are taken lowest index first
+ * and requests served in list order, so results are reproducible.
+ *   reserve  row s grows by counts[s] tokens.
+ *   fork     row dst[i] (empty) becomes a copy of row src[i], i < n: full pages
+ *            are shared, a last page that is not full is copied in every pool.
+ *   free     the rows end; pages that no row holds any more are free.
+ *   compact  the *live pages move to 0 .. live-1 in every pool and the table
+ *            follows, so that the pool's tail can be given up.
+ * reserve and fork are all or nothing: with too few free pages or an invalid
+ * request (a row outside the table, a dst that is not empty or listed twice, a
+ * row longer than W pages) the new state equals the old one, no payload moves,
+ * and `status` is set.  S <= 65536 and S * W < 2^31.
+ * pools / strides / bytes: n_pools base pointers, bytes between pages and bytes
+ * of a page; host arrays, read during the call.  Payload moves only into pages
+ * that are free in the old state.
+ *   hoa_pages_copy   page to[i] = page from[i] in every pool, i < n (device
+ *            lists; both -1: skipped); no page is both read and written.
+ *   hoa_pages_write  k, v (B, T, H, d) (strides of row, token, head) become the
+ *            last T tokens of each row: token t goes to position lens[b] - T + t
+ *            (not written where that is negative).
+ */
+size_t hoa_pages_workspace_bytes(int n, int n_pages);
+int hoa_pages_reserve(const int* table, const int* lens, const int* refs, const int* counts, int* table_out,
+                      int* lens_out, int* refs_out, int S, int W, int n_pages, int page, void* workspace,
+                      size_t workspace_bytes, int* status, void* stream);
+int hoa_pages_fork(const int* table, const int* lens, const int* refs, const int* src, const int* dst, int n,
+                   int* table_out, int* lens_out, int* refs_out, int S, int W, int n_pages, int page,
+                   void* const* pools, const long long* strides, const long long* bytes, int n_pools,
+                   void* workspace, size_t workspace_bytes, int* status, void* stream);
+int hoa_pages_free(const int* table, const int* lens, const int* refs, const int* rows, int n, int* table_out,
+                   int* lens_out, int* refs_out, int S, int W, int n_pages, int page, int* status, void* stream);
+int hoa_pages_compact(const int* table, const int* refs, int* table_out, int* refs_out, int* live, int S, int W,
+                      int n_pages, void* const* pools, const long long* strides, const long long* bytes, int n_pools,
+                      void* workspace, size_t workspace_bytes, int* status, void* stream);
+int hoa_pages_copy(void* const* pools, const long long* strides, const long long* bytes, int n_pools,
+                   const int* from, const int* to, int n, int n_pages, int* status, void* stream);
+int hoa_pages_write(const void* k, const void* v, int src_dtype, const long long* k_strides,
+                    const long long* v_strides, void* k_pages, void* v_pages, int dtype,
+                    const long long* page_strides, const int* table, long long table_stride, const int* lens,
+                    int B, int T, int H, int d, int page, int W, int n_pages, int* status, void* stream);
+
+/*
+ * Attention of B rows over the cache.  q (B, Tq, H, d) (strides of row, token,
+ * head), H a multiple of the pools' Hk heads: query head h reads kv head
+ * h / (H / Hk).  The first n_shared pages of every row are `shared` (their keys
+ * are read once for the whole batch); `table` (B, W) holds the pages after them.
+ * lens[b] counts all keys of row b, the shared ones and its Tq newest included:
+ * query t sees keys 0 .. lens[b] - Tq + t.  A row may end inside the shared
+ * pages, have fewer keys than queries, or none.
+ *   out (B, Tq, H, d) = softmax(q k^T * scale) v, 0 where a query sees no key;
+ *   lse (B, Tq, H) = the log of the softmax's sum, -inf there.
+ * paths (nullable, Tq = 1): (B, H, d, d) fp32, then out = P o, the inverse
+ * transport (core/attention_fast_chunked.py:171).  q and the pools share `dtype`;
+ * d <= 128.  Slots that no query sees may hold anything, NaN included.
+ */
+size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms);
+int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
+                       const long long* page_strides, int dtype, const int* shared, int n_shared,
+                       const int* table, long long table_stride, int W, const int* lens, const float* paths,
+                       void* out, int out_dtype, float* lse, float softmax_scale, int B, int Tq, int H, int Hk,
+                       int d, int page, int n_pages, int num_sms, void* workspace, size_t workspace_bytes,
+                       int* status, void* stream);
+
+/*
+ * One generated token of every row: kernels (1) and (2) in their single-token form
+ * (core/attention_fast_chunked.py:86-94, 108-110).
+ *   P_out = expm(skew(edge_scale * (a + a_bias))) P     (B, H, d, d) fp32
+ *   q^ = P_out^T q -> qh (B, H, d); k^, v^ likewise -> slot lens[b] - 1 of the row
+ * a (B, H * stride) fp32: the generators of the edge from the row's previous token
+ * to this one (a_dtype HOA_F32, with or without HOA_GEN_BANKED); qkv (B, H, 3d)
+ * rows `qkv_stride` elements apart.  lens[b] counts the token itself: at lens 1
+ * there is no edge and P_out = I; at lens 0 P_out = P, q^ = 0 and nothing is
+ * written.  P_out may be P.  qh and the pools share `dtype`; 2 <= d <= 120.
+ */
+int hoa_path_step(const float* a, int a_dtype, const float* a_bias, float edge_scale, const float* P, float* P_out,
+                  const void* qkv, int qkv_dtype, long long qkv_stride, void* qh, void* k_pages, void* v_pages,
+                  int dtype, const long long* page_strides, const int* table, long long table_stride, int W,
+                  const int* lens, int B, int H, int d, int page, int n_pages, int* status, void* stream);
 
 /*
  * hoa_selftest_wait — no counterpart in the reference.  Diagnostic for the
