@@ -22,14 +22,14 @@ namespace hoa {
 // ---------------------------------------------------------------------------
 constexpr int kPsRows = 16, kPsKeys = 64, kPsThreads = 128;
 
-__global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __grid_constant__ PaArgs p) {
+__global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   extern __shared__ float sm[];
   const int d = p.d, ld = d | 1;                       // odd row stride: rows fall on different banks
   float* Qs = sm;                                      // [16][ld]
   float* Ks = Qs + kPsRows * ld;                       // [64][ld]
   float* Vs = Ks + kPsKeys * ld;                       // [64][ld]
   float* Ps = Vs + kPsKeys * ld;                       // [16][64]
-  const PaItem it = pa_item(p, blockIdx.x, kPsRows, kPsKeys);
+  PaItem it = pa_item(p, first + blockIdx.x, kPsRows, kPsKeys);
   const int tid = threadIdx.x, row = tid >> 3, kg = tid & 7;
   const PaRow my = pa_row(p, it, it.row0 + row);
   for (int i = tid; i < kPsRows * d; i += kPsThreads) {
@@ -37,7 +37,13 @@ __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __gri
     const PaRow q = pa_row(p, it, it.row0 + r);
     Qs[r * ld + c] = q.ok ? load_elem(p.q, q.b * p.qsb + q.t * p.qst + q.h * p.qsh + c, p.dtype) : 0.f;
   }
-  const int seen = min(my.seen - it.key_base, it.k1);  // keys of this part that the row sees, and the range ends
+  const int seen = my.ok ? min(my.seen - it.key_base, it.k1) : 0;   // keys of this part that the row sees
+  __shared__ int s_top;                                // no key past the last one that a row sees is read
+  if (tid == 0) s_top = 0;
+  __syncthreads();
+  if (kg == 0) atomicMax(&s_top, seen);
+  __syncthreads();
+  it.k1 = min(it.k1, s_top);
   float o[16], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.f;
@@ -144,13 +150,35 @@ __global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_const
 
 using namespace hoa;
 
+static bool pa_shape_ok(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms) {
+  return B >= 1 && Tq >= 1 && Hk >= 1 && H >= Hk && H % Hk == 0 && d >= 1 && page >= 1 && n_shared >= 0 && W >= 0 &&
+         num_sms >= 1;
+}
+
+static size_t pa_bytes(const PaPlan& pl, int B, int Tq, int H, int d) {
+  return ((size_t)pl.ns1 + pl.ns2) * B * Tq * H * (8 + 4 * (size_t)d) + 256;
+}
+
 extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W,
                                                  int num_sms) {
-  if (B < 1 || Tq < 1 || Hk < 1 || H < Hk || H % Hk != 0 || d < 1 || page < 1 || n_shared < 0 || W < 0 || num_sms < 1)
-    return 0;
-  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms);
-  const size_t rows = (size_t)B * Tq * H, slots = (size_t)pl.ns1 + pl.ns2;
-  return slots * rows * (8 + 4 * (size_t)d) + 256;
+  if (!pa_shape_ok(B, Tq, H, Hk, d, page, n_shared, W, num_sms)) return 0;
+  size_t most = 0;                                 // enough for whichever kernels take the call
+  for (int k = 0; k < 3; ++k) {
+    const size_t n = pa_bytes(pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, k > 0, k > 1), B, Tq, H, d);
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+static int run_items(int kind, const PaArgs& a, long long first, long long items, cudaStream_t s) {
+  if (items == 0) return HOA_OK;
+  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, s);
+  if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, s);
+  const size_t smem = ((kPsRows + 2 * kPsKeys) * (size_t)(a.d | 1) + kPsRows * kPsKeys) * sizeof(float);
+  if (cudaFuncSetAttribute(paged_attn_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return HOA_ERR_LAUNCH;
+  paged_attn_simt_kernel<<<(unsigned)items, kPsThreads, smem, s>>>(a, (unsigned)first);
+  return launch_status();
 }
 
 extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -159,17 +187,21 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
                                   void* out, int out_dtype, float* lse, float softmax_scale, int B, int Tq, int H, int Hk,
                                   int d, int page, int n_pages, int num_sms, void* workspace, size_t workspace_bytes,
                                   int* status, void* stream) {
-  if (!q || !q_strides || !k_pages || !v_pages || !page_strides || !lens || !out || !lse || !workspace || B < 1 ||
-      Tq < 1 || Hk < 1 || H < Hk || H % Hk != 0 || d < 1 || page < 1 || n_pages < 1 || n_shared < 0 || W < 0 ||
-      num_sms < 1 || (n_shared > 0 && !shared) || (W > 0 && !table) || (paths && Tq != 1))
+  if (!q || !q_strides || !k_pages || !v_pages || !page_strides || !lens || !out || !lse || !workspace ||
+      !pa_shape_ok(B, Tq, H, Hk, d, page, n_shared, W, num_sms) || n_pages < 1 || (n_shared > 0 && !shared) ||
+      (W > 0 && !table) || (paths && Tq != 1))
     return HOA_ERR_INVALID_ARG;
   if ((dtype != HOA_F32 && dtype != HOA_BF16) || (out_dtype != HOA_F32 && out_dtype != HOA_BF16) || d > 128)
     return HOA_ERR_UNSUPPORTED;
-  // key positions are ints
+  // key positions and item numbers are ints
   if ((long long)(n_shared + (long long)W) * page > 0x7fff0000ll) return HOA_ERR_UNSUPPORTED;
-  const size_t need = hoa_paged_attn_workspace_bytes(B, Tq, H, Hk, d, page, n_shared, W, num_sms);
-  if (workspace_bytes < need) return HOA_ERR_WORKSPACE;
-  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms);
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
+                         (uintptr_t)(page_strides[0] * 2) | (uintptr_t)(page_strides[1] * 2) | (uintptr_t)(page_strides[2] * 2);
+  const bool tensor = dtype == HOA_BF16 && d % 8 == 0 && (bits & 15) == 0;
+  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, tensor, tensor && softmax_scale > 0.f);
+  if (workspace_bytes < pa_bytes(pl, B, Tq, H, d)) return HOA_ERR_WORKSPACE;
+  const long long items1 = (long long)pl.tiles1 * Hk * pl.ns1, items2 = (long long)B * Hk * pl.tiles2 * pl.ns2;
+  if (items1 + items2 > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;
   PaArgs a{};
   a.q = q; a.qsb = q_strides[0]; a.qst = q_strides[1]; a.qsh = q_strides[2];
   a.kp = k_pages; a.vp = v_pages; a.ps = page_strides[0]; a.hs = page_strides[1]; a.ts = page_strides[2];
@@ -183,17 +215,14 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)(pl.ns1 + pl.ns2) * a.rows * d);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const int ld = d | 1;
-  const size_t smem = ((kPsRows + 2 * kPsKeys) * (size_t)ld + kPsRows * kPsKeys) * sizeof(float);
-  if (cudaFuncSetAttribute(paged_attn_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
-  const long long items = (long long)pl.tiles1 * Hk * pl.ns1 + (long long)B * Hk * pl.tiles2 * pl.ns2;
-  if (items > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;
-  if (items > 0) {
-    paged_attn_simt_kernel<<<(unsigned)items, kPsThreads, smem, s>>>(a);
-    const int st = launch_status();
-    if (st != HOA_OK) return st;
+  int st;
+  if (pl.kind1 == pl.kind2) {                      // one launch for both parts
+    st = run_items(pl.kind1, a, 0, items1 + items2, s);
+  } else {
+    st = run_items(pl.kind1, a, 0, items1, s);
+    if (st == HOA_OK) st = run_items(pl.kind2, a, items1, items2, s);
   }
+  if (st != HOA_OK) return st;
   paged_attn_join_kernel<<<(unsigned)(a.rows < 148 * 64 ? a.rows : 148 * 64), 128, 0, s>>>(a);
   return launch_status();
 }

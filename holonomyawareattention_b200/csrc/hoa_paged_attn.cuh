@@ -33,30 +33,68 @@ struct PaItem {
 
 struct PaRow { bool ok; int b, t, h, seen; long long grow; };
 
-struct PaPlan { int tiles1, ns1, tiles2, ns2; };
-
 HOA_DEVICE void pa_fail(int* status) {
   if (status != nullptr) *reinterpret_cast<volatile int*>(status) = HOA_ERR_PAGES;
 }
 
-// rows of a tile: see paged_attn_simt_kernel
-inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int W, int num_sms) {
+// Keys of a tensor-core tile: whole pages, or whole tiles of a page, of at most 128 keys in
+// multiples of 16 (a product's k-step); 0 where no such tile exists (pages of 25, say).
+inline int pa_tile_keys(int page) {
+  if (page % 8 != 0) return 0;                     // the swizzle pattern repeats every 8 rows
+  if (page <= 128) {
+    int kt = 128 / page * page;
+    while (kt > 0 && kt % 16 != 0) kt -= page;
+    return kt;
+  }
+  for (int kt = 128; kt > 0; kt -= 16)
+    if (page % kt == 0) return kt;
+  return 0;
+}
+
+// Which kernel takes a part.
+//   simt: fp32, head dims or strides that the copies do not take; 16 rows a tile.
+//   mma:  bf16, 16 rows a tile, any page size.
+//   tc:   bf16, 256 rows a tile, pages that tile (pa_tile_keys).
+enum PaKind { kPaSimt = 0, kPaMma = 1, kPaTc = 2 };
+
+// Rows of a head from which tcgen05 takes a part: up to 16 one mma item reads the keys once.
+constexpr int kPaTcRows = 17;
+
+struct PaPlan { int kind1, tiles1, ns1, kind2, tiles2, ns2; };
+
+// `tensor`: bf16 with d % 8 == 0 and 16-byte strides, `tc`: tcgen05 takes the call (tensor, scale > 0).
+inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int W, int num_sms, bool tensor, bool tc) {
   PaPlan pl{};
-  const int G = H / Hk;
-  if (n_shared > 0) {
-    pl.tiles1 = ceil_div((long long)B * Tq * G, 16);
-    const long long units = (long long)pl.tiles1 * Hk, tiles = ceil_div((long long)n_shared * page, 64);
-    long long ns = (2 * num_sms + units - 1) / units;
-    if (ns > tiles) ns = tiles;
-    pl.ns1 = (int)(ns < 1 ? 1 : ns);
-  }
-  if (W > 0) {
-    pl.tiles2 = ceil_div((long long)Tq * G, 16);
-    const long long units = (long long)B * Hk * pl.tiles2, tiles = ceil_div((long long)W * page, 64);
-    long long ns = (2 * num_sms + units - 1) / units;
-    if (ns > tiles) ns = tiles;
-    pl.ns2 = (int)(ns < 1 ? 1 : ns);
-  }
+  const long long G = H / Hk, keys1 = (long long)n_shared * page, keys2 = (long long)W * page;
+  const long long rows1 = B * (long long)Tq * G, rows2 = Tq * G;
+  const int kt = pa_tile_keys(page);
+  tc = tc && kt > 0;
+  pl.kind1 = tc && rows1 >= kPaTcRows ? kPaTc : tensor ? kPaMma : kPaSimt;
+  pl.kind2 = tc && rows2 >= kPaTcRows ? kPaTc : tensor ? kPaMma : kPaSimt;
+  const long long t1 = keys1 > 0 ? (rows1 + (pl.kind1 == kPaTc ? 255 : 15)) / (pl.kind1 == kPaTc ? 256 : 16) : 0;
+  const long long t2 = keys2 > 0 ? (rows2 + (pl.kind2 == kPaTc ? 255 : 15)) / (pl.kind2 == kPaTc ? 256 : 16) : 0;
+  const long long u1 = t1 * Hk, u2 = t2 * Hk * B;
+  // mma and simt items: a range of keys such that all of them make about two waves of 4 CTAs an SM
+  // (of the room that the rows have; the shorter ones split their own range as finely)
+  const long long all = (pl.kind1 != kPaTc ? u1 * keys1 : 0) + (pl.kind2 != kPaTc ? u2 * keys2 : 0);
+  long long range = all / (8ll * num_sms);
+  range = range < 128 ? 128 : range;
+  auto splits = [&](int kind, long long units, long long keys) -> int {
+    if (units == 0) return 0;
+    long long ns;
+    if (kind == kPaTc) {                           // one CTA an SM: split only what leaves SMs without one
+      ns = num_sms / units;
+      const long long most = (keys + kt - 1) / kt;
+      ns = ns > most ? most : ns;
+    } else {
+      ns = (keys + range - 1) / range;
+    }
+    return (int)(ns < 1 ? 1 : ns > 4096 ? 4096 : ns);
+  };
+  pl.tiles1 = (int)t1;
+  pl.tiles2 = (int)t2;
+  pl.ns1 = splits(pl.kind1, u1, keys1);
+  pl.ns2 = splits(pl.kind2, u2, keys2);
   return pl;
 }
 
@@ -126,5 +164,9 @@ HOA_DEVICE long long pa_key(const PaArgs& p, const PaItem& it, int j) {
   }
   return id * p.ps + it.kvh * p.hs + (long long)(j - pg * p.page) * p.ts;
 }
+
+// items first .. first + items - 1
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
+int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
 
 }  // namespace hoa

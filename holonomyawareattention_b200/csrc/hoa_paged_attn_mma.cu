@@ -1,0 +1,294 @@
+// Paged attention for few query rows (bf16): every warp streams its own keys.
+//
+// An item is at most 16 query rows against a range of keys; its 4 warps take the
+// range's 16-key chunks in turn.  A warp copies a chunk of K and V to its own two
+// shared-memory stages (16-byte asynchronous copies, a key's page looked up by one
+// lane one chunk ahead), and runs
+//   S (16 x 16) = Q K^T, online softmax, O (16 x d) += P V
+// on m16n8k16 products whose accumulators and P stay in registers.  No barrier in
+// the loop: warps meet once at the end, to join their (m, l, O).
+//
+// What bounds it is HBM: a key costs 4 d bytes (23.6 bytes an SM cycle at the
+// measured copy rate, so 16 keys of d = 96 take 260 SM cycles) against about 150
+// issue slots a chunk over four schedulers.  16 warps an SM with a chunk of 6 KB
+// each in flight keep 96 KB under way, twice what the latency needs.  The tensor
+// cores' tcgen05 form (hoa_paged_attn_tc.cu) takes over where the rows of a head
+// fill more of its 128-row tile.
+#include "hoa_paged_attn.cuh"
+#include "hoa_sm100.cuh"
+
+namespace hoa {
+
+constexpr int kPmWarps = 4, kPmKeys = 16, kPmStages = 2;
+
+template <int D8>
+struct PmCfg {
+  static constexpr int d = 8 * D8, KS = (D8 + 1) / 2;      // k-steps of 16 over the head dim
+  static constexpr int kRow = KS * 32 + 16;                // bytes of a key's row: an odd number of 16-byte chunks, so that
+                                                           // the 8 rows of a matrix load fall on different banks
+  static constexpr int kTile = kPmKeys * kRow;             // K or V chunk
+  static constexpr int kStage = 2 * kTile;
+  static constexpr int kWarp = kPmStages * kStage;
+  static constexpr int kRing = kPmWarps * kWarp;
+  static constexpr int kJoinRow = d + 4;                   // floats of a row of the join
+  static constexpr int kJoin = kPmWarps * 16 * kJoinRow * 4;
+  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kMinBlocks = D8 <= 12 ? 4 : 3;
+};
+
+HOA_DEVICE void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+HOA_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+HOA_DEVICE void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+HOA_DEVICE void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+HOA_DEVICE void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+HOA_DEVICE void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+HOA_DEVICE uint32_t pm_pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int D8>
+__global__ void __launch_bounds__(kPmWarps * 32, PmCfg<D8>::kMinBlocks)
+paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
+  using C = PmCfg<D8>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  PaItem it = pa_item(p, first + blockIdx.x, 16, kPmKeys);
+  const int tid = threadIdx.x, w = tid >> 5, lid = tid & 31, r0 = lid >> 2, q2 = (lid & 3) * 2;
+  const uint32_t ring = sm100::smem_u32(smem) + w * C::kWarp;
+
+  // the pad chunk of a head dim that is 8 mod 16 enters the products: zero, once
+  if (D8 & 1) {
+    for (int i = lid; i < kPmStages * 2 * kPmKeys; i += 32)
+      *reinterpret_cast<uint4*>(smem + w * C::kWarp + i * C::kRow + D8 * 16) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
+
+  // no key past the last one that a row of the item sees is read: its slot may hold anything
+  {
+    const PaRow row = pa_row(p, it, it.row0 + (lid & 15));
+    it.k1 = min(it.k1, __reduce_max_sync(0xffffffffu, row.ok ? row.seen - it.key_base : 0));
+  }
+  const int chunks = it.k1 > it.k0 ? (it.k1 - it.k0 + kPmKeys - 1) / kPmKeys : 0;
+  // element offset of this lane's key (lanes 0-15) of a chunk, -1: none
+  auto key_of = [&](int c) -> long long {
+    const int j = it.k0 + c * kPmKeys + (lid & 15);
+    return c < chunks && j < it.k1 ? pa_key(p, it, j) : -1;
+  };
+  const uint8_t* kp = reinterpret_cast<const uint8_t*>(p.kp);
+  const uint8_t* vp = reinterpret_cast<const uint8_t*>(p.vp);
+  auto issue = [&](int stage, long long off) {
+    const uint32_t base = ring + stage * C::kStage;
+#pragma unroll
+    for (int i = 0; i < (kPmKeys * D8 + 31) / 32; ++i) {
+      const int x = lid + 32 * i, key = x / D8, ch = x % D8;
+      const long long o = __shfl_sync(0xffffffffu, off, key & 15);
+      if (kPmKeys * D8 % 32 == 0 || x < kPmKeys * D8) {
+        const uint32_t n = o >= 0 ? 16u : 0u;           // 0: filled with zeros (a masked V row must not hold NaN)
+        const long long at = (o >= 0 ? o : 0) * 2 + ch * 16;
+        cp_async16(base + key * C::kRow + ch * 16, kp + at, n);
+        cp_async16(base + C::kTile + key * C::kRow + ch * 16, vp + at, n);
+      }
+    }
+  };
+
+  long long off = key_of(w);
+#pragma unroll
+  for (int s = 0; s < kPmStages; ++s) {
+    if (w + s * kPmWarps < chunks) issue(s, off);
+    cp_commit();
+    off = key_of(w + (s + 1) * kPmWarps);
+  }
+
+  // Q as A fragments: rows r0 and r0 + 8, columns 16 ks + q2 + {0, 1} and + 8
+  const PaRow ra = pa_row(p, it, it.row0 + r0), rb = pa_row(p, it, it.row0 + r0 + 8);
+  uint32_t qf[C::KS][4];
+  {
+    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
+    const __nv_bfloat16* qa = q + ra.b * p.qsb + ra.t * p.qst + ra.h * p.qsh;
+    const __nv_bfloat16* qb = q + rb.b * p.qsb + rb.t * p.qst + rb.h * p.qsh;
+    auto pair = [&](const __nv_bfloat16* r, bool ok, int c) -> uint32_t {
+      if (!ok || c >= C::d) return 0u;
+      const uint32_t lo = *reinterpret_cast<const uint16_t*>(r + c), hi = *reinterpret_cast<const uint16_t*>(r + c + 1);
+      return lo | hi << 16;
+    };
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      qf[ks][0] = pair(qa, ra.ok, 16 * ks + q2);
+      qf[ks][1] = pair(qb, rb.ok, 16 * ks + q2);
+      qf[ks][2] = pair(qa, ra.ok, 16 * ks + q2 + 8);
+      qf[ks][3] = pair(qb, rb.ok, 16 * ks + q2 + 8);
+    }
+  }
+  const int seen_a = ra.ok ? ra.seen - it.key_base : 0, seen_b = rb.ok ? rb.seen - it.key_base : 0;
+
+  float o[D8][4];
+#pragma unroll
+  for (int n = 0; n < D8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  // matrix loads: lane l gives row l % 8 of matrix l / 8
+  const uint32_t k_at = ((lid >> 4) * 8 + (lid & 7)) * C::kRow + ((lid >> 3) & 1) * 16;   // matrices: keys 0-7 (k, k+8), keys 8-15
+  const uint32_t v_at = C::kTile + (((lid >> 3) & 1) * 8 + (lid & 7)) * C::kRow + (lid >> 4) * 16;
+
+  int stage = 0;
+  for (int c = w; c < chunks; c += kPmWarps) {
+    cp_wait<kPmStages - 1>();
+    __syncwarp();
+    const uint32_t base = ring + stage * C::kStage;
+    float s[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      uint32_t b[4];
+      ldsm4(base + k_at + ks * 32, b);
+      mma_16816(s[0], qf[ks], b[0], b[1]);
+      mma_16816(s[1], qf[ks], b[2], b[3]);
+    }
+    const int j0 = it.k0 + c * kPmKeys + q2;
+    const int na = min(seen_a, it.k1) - j0, nb = min(seen_b, it.k1) - j0;   // keys of the chunk from q2 on that the rows see
+    float xa = -INFINITY, xb = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 8 * n + e;
+        s[n][e] = j < na ? s[n][e] * p.scale_log2 : -INFINITY;
+        s[n][2 + e] = j < nb ? s[n][2 + e] * p.scale_log2 : -INFINITY;
+        xa = fmaxf(xa, s[n][e]);
+        xb = fmaxf(xb, s[n][2 + e]);
+      }
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, x));
+      xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, x));
+    }
+    if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
+      const float na2 = fmaxf(ma, xa), nb2 = fmaxf(mb, xb);
+      const float ca = na2 == -INFINITY ? 1.f : exp2f(ma - na2), cb = nb2 == -INFINITY ? 1.f : exp2f(mb - nb2);
+      ma = na2;
+      mb = nb2;
+      la *= ca;
+      lb *= cb;
+#pragma unroll
+      for (int n = 0; n < D8; ++n) {
+        o[n][0] *= ca; o[n][1] *= ca; o[n][2] *= cb; o[n][3] *= cb;
+      }
+    }
+    const float fa = ma == -INFINITY ? 0.f : ma, fb = mb == -INFINITY ? 0.f : mb;   // no key seen yet: weights 0
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[n][e] = exp2f(s[n][e] - fa);
+        s[n][2 + e] = exp2f(s[n][2 + e] - fb);
+        la += s[n][e];
+        lb += s[n][2 + e];
+      }
+    // the weights are rounded to bf16 for the product only (2^-9 relative, as the output's own rounding); l sums them unrounded
+    const uint32_t pf[4] = {pm_pack(s[0][0], s[0][1]), pm_pack(s[0][2], s[0][3]), pm_pack(s[1][0], s[1][1]), pm_pack(s[1][2], s[1][3])};
+#pragma unroll
+    for (int n = 0; n < C::KS; ++n) {
+      uint32_t b[4];
+      ldsm4_t(base + v_at + n * 32, b);
+      mma_16816(o[2 * n], pf, b[0], b[1]);
+      if (2 * n + 1 < D8) mma_16816(o[2 * n + 1 < D8 ? 2 * n + 1 : 0], pf, b[2], b[3]);
+    }
+    __syncwarp();                                       // all lanes have read the stage
+    if (c + kPmStages * kPmWarps < chunks) issue(stage, off);
+    cp_commit();
+    off = key_of(c + (kPmStages + 1) * kPmWarps);
+    stage ^= 1;
+  }
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) {
+    la += __shfl_xor_sync(0xffffffffu, la, x);
+    lb += __shfl_xor_sync(0xffffffffu, lb, x);
+  }
+
+  // ---- join the warps
+  cp_wait<0>();
+  __syncthreads();
+  float* jn = reinterpret_cast<float*>(smem);
+  {
+    float* a = jn + (w * 16 + r0) * C::kJoinRow;
+    float* b = a + 8 * C::kJoinRow;
+    if (q2 == 0) {
+      a[C::d] = ma; a[C::d + 1] = la;
+      b[C::d] = mb; b[C::d + 1] = lb;
+    }
+#pragma unroll
+    for (int n = 0; n < D8; ++n) {
+      *reinterpret_cast<float2*>(a + 8 * n + q2) = make_float2(o[n][0], o[n][1]);
+      *reinterpret_cast<float2*>(b + 8 * n + q2) = make_float2(o[n][2], o[n][3]);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < 16 * C::d; i += kPmWarps * 32) {
+    const int r = i / C::d, c = i % C::d;
+    const PaRow row = pa_row(p, it, it.row0 + r);
+    if (!row.ok) break;                                 // rows are in order: none after this one either
+    float m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kPmWarps; ++x) m = fmaxf(m, jn[(x * 16 + r) * C::kJoinRow + C::d]);
+    float l = 0.f, y = 0.f;
+    if (m != -INFINITY) {
+#pragma unroll
+      for (int x = 0; x < kPmWarps; ++x) {
+        const float* a = jn + (x * 16 + r) * C::kJoinRow;
+        const float f = exp2f(a[C::d] - m);
+        l = fmaf(f, a[C::d + 1], l);
+        y = fmaf(f, a[c], y);
+      }
+    }
+    const long long part = (long long)it.slot * p.rows + row.grow;
+    if (c == 0) p.part_ml[part] = make_float2(m, l);
+    if (l > 0.f) p.part_o[part * C::d + c] = y;
+  }
+}
+
+template <int D8>
+static int launch_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+  using C = PmCfg<D8>;
+  if (cudaFuncSetAttribute(paged_attn_mma_kernel<D8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+    return HOA_ERR_LAUNCH;
+  paged_attn_mma_kernel<D8><<<items, kPmWarps * 32, C::kSmem, s>>>(a, first);
+  return launch_status();
+}
+
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+  switch (a.d / 8) {
+    case 1: return launch_mma<1>(a, first, items, s);
+    case 2: return launch_mma<2>(a, first, items, s);
+    case 3: return launch_mma<3>(a, first, items, s);
+    case 4: return launch_mma<4>(a, first, items, s);
+    case 5: return launch_mma<5>(a, first, items, s);
+    case 6: return launch_mma<6>(a, first, items, s);
+    case 7: return launch_mma<7>(a, first, items, s);
+    case 8: return launch_mma<8>(a, first, items, s);
+    case 9: return launch_mma<9>(a, first, items, s);
+    case 10: return launch_mma<10>(a, first, items, s);
+    case 11: return launch_mma<11>(a, first, items, s);
+    case 12: return launch_mma<12>(a, first, items, s);
+    case 13: return launch_mma<13>(a, first, items, s);
+    case 14: return launch_mma<14>(a, first, items, s);
+    case 15: return launch_mma<15>(a, first, items, s);
+    case 16: return launch_mma<16>(a, first, items, s);
+    default: return HOA_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace hoa
