@@ -72,78 +72,111 @@ struct StLayout {
   static constexpr int kMat = NKB * kSlab;               // one f16 matrix
   static constexpr int kLd = DP + 4;                     // floats of a row of E P: rows of a warp on different banks
   static constexpr int kRight = 2 * kMat + (128 - DP) * 128;   // hi, lo; P1 reads 128 rows as its left factor
-  static constexpr int kDelta = DP * kLd * 4;
-  static constexpr int offVec = ((kRight > kDelta ? kRight : kDelta) + 127) / 128 * 128;
-  static constexpr int offSum = offVec + 3 * DP * 4;     // row sums (2 x 128), later the partial q^, k^, v^
-  static constexpr int offMax = offSum + 3 * 128 * 4;
+  static constexpr int kDim = DP < 120 ? DP : 120;       // the largest head dim
+  static constexpr int kDelta = kDim * kLd * 4;
+  static constexpr int kDeltaEnd = kDelta + 256 * 12 * 4;      // + the partial sums of q^, k^, v^ (12 a thread)
+  static constexpr int offGen = ((kRight > kDeltaEnd ? kRight : kDeltaEnd) + 127) / 128 * 128;   // the next row's generators
+  static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2) * 4;   // (either layout: banked has d / 2 unused slots)
+  static constexpr int offVec = offGen + (kGen + 127) / 128 * 128;
+  static constexpr int offSum = offVec + 3 * DP * 4;           // row sums (2 x 128)
+  static constexpr int offMax = offSum + 2 * 128 * 4;
   static constexpr int offBar = offMax + 32;
   static constexpr int kAlloc = offBar + 32 + 1024;
   static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
   static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
 };
 
-HOA_DEVICE void st_split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
+// Pairs of fp32 values: the packed forms of sm_100 (fma.rn.f32x2) halve the element
+// work's instructions, which is what a row's time goes into beside the products.
+using F2 = unsigned long long;
+HOA_DEVICE F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+HOA_DEVICE F2 f2(float x) { return f2(x, x); }
+HOA_DEVICE float2 f2_get(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+HOA_DEVICE F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+HOA_DEVICE F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+HOA_DEVICE F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// x = hi + lo to 2^-22, two f16 each
+HOA_DEVICE void st_split2(F2 x, uint32_t& hi, uint32_t& lo) {
+  const float2 v = f2_get(x);
+  const __half2 h = __floats2half2_rn(v.x, v.y);
   const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  const float2 r = f2_get(f2_fma(f2(f.x, f.y), f2(-1.f), x));
+  const __half2 l = __floats2half2_rn(r.x, r.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-HOA_DEVICE float2 st_join2(uint32_t hi, uint32_t lo) {
+HOA_DEVICE F2 st_join2(uint32_t hi, uint32_t lo) {
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-  return make_float2(h.x + l.x, h.y + l.y);
+  return f2_add(f2(h.x, h.y), f2(l.x, l.y));
 }
 
+// What a thread owns of the matrices: a row (= TMEM lane), and every other 16 columns.
 template <int DP>
 struct StUnit {
   using L = StLayout<DP>;
   uint8_t* sm;
   uint32_t tmem;           // + this warp's lanes
-  int row, half;           // the thread's row (= TMEM lane), which of every two 16-column chunks
+  int row, half;
 
-  // 16 columns of chunk c of the right factor (this thread's row) / of the left factor
-  HOA_DEVICE uint32_t* right(int part, int c, int q) const {   // q: which 8 columns
-    const int ch = 2 * c + q;
-    return reinterpret_cast<uint32_t*>(sm + part * L::kMat + (ch >> 3) * L::kSlab + sw128_offset(row, ch & 7));
-  }
-  HOA_DEVICE void put_right(int c, const float (&v)[16], float s) const {
+  // 16 columns (chunk c) of this thread's row of the right factor
+  HOA_DEVICE void put_right(int c, const F2 (&v)[8]) const {
     if (row >= DP) return;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       uint4 h, l;
-      st_split2(v[8 * q] * s, v[8 * q + 1] * s, h.x, l.x);
-      st_split2(v[8 * q + 2] * s, v[8 * q + 3] * s, h.y, l.y);
-      st_split2(v[8 * q + 4] * s, v[8 * q + 5] * s, h.z, l.z);
-      st_split2(v[8 * q + 6] * s, v[8 * q + 7] * s, h.w, l.w);
-      *reinterpret_cast<uint4*>(right(0, c, q)) = h;
-      *reinterpret_cast<uint4*>(right(1, c, q)) = l;
+      st_split2(v[4 * q], h.x, l.x);
+      st_split2(v[4 * q + 1], h.y, l.y);
+      st_split2(v[4 * q + 2], h.z, l.z);
+      st_split2(v[4 * q + 3], h.w, l.w);
+      const int ch = 2 * c + q;
+      uint8_t* at = sm + (ch >> 3) * L::kSlab + sw128_offset(row, ch & 7);
+      *reinterpret_cast<uint4*>(at) = h;
+      *reinterpret_cast<uint4*>(at + L::kMat) = l;
     }
   }
-  HOA_DEVICE void get_right(int c, float (&v)[16], float s) const {   // s: 1 / the factor's scale
+  HOA_DEVICE void get_right(int c, F2 (&v)[8]) const {
+    const int r = row < DP ? row : 0;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int r = row < DP ? row : 0;
       const int ch = 2 * c + q;
       const uint8_t* at = sm + (ch >> 3) * L::kSlab + sw128_offset(r, ch & 7);
       const uint4 h = *reinterpret_cast<const uint4*>(at), l = *reinterpret_cast<const uint4*>(at + L::kMat);
-      const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = st_join2(hh[e], ll[e]);
-        v[8 * q + 2 * e] = f.x * s;
-        v[8 * q + 2 * e + 1] = f.y * s;
-      }
+      v[4 * q] = st_join2(h.x, l.x);
+      v[4 * q + 1] = st_join2(h.y, l.y);
+      v[4 * q + 2] = st_join2(h.z, l.z);
+      v[4 * q + 3] = st_join2(h.w, l.w);
     }
   }
-  // (TMEM accesses are warp-collective: every lane of the warp calls these)
-  HOA_DEVICE void put_left(int c, const float (&v)[16], float s) const {
+  // the same of the left factor (TMEM accesses are warp-collective: every lane calls these)
+  HOA_DEVICE void put_left(int c, const F2 (&v)[8]) const {
     float h[8], l[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       uint32_t hi, lo;
-      st_split2(v[2 * e] * s, v[2 * e + 1] * s, hi, lo);
+      st_split2(v[e], hi, lo);
       h[e] = __uint_as_float(hi);
       l[e] = __uint_as_float(lo);
     }
@@ -154,17 +187,18 @@ struct StUnit {
     tmem_ld8(tmem + L::colHi + 8 * c, h);
     tmem_ld8(tmem + L::colLo + 8 * c, l);
   }
-  HOA_DEVICE static void join_left(float (&h)[8], float (&l)[8], float (&v)[16], float s) {
+  HOA_DEVICE static void join_left(float (&h)[8], float (&l)[8], F2 (&v)[8]) {   // after tmem_wait_ld
     tmem_touch(h);
     tmem_touch(l);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 f = st_join2(__float_as_uint(h[e]), __float_as_uint(l[e]));
-      v[2 * e] = f.x * s;
-      v[2 * e + 1] = f.y * s;
-    }
+    for (int e = 0; e < 8; ++e) v[e] = st_join2(__float_as_uint(h[e]), __float_as_uint(l[e]));
   }
 };
+
+HOA_DEVICE void cp_async(uint32_t dst, const float* src, bool wide) {
+  if (wide) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 
 // the three products of one fp32-accurate product, by one thread: D (+)= X Y
 template <int DP, bool kSmemLeft>
@@ -189,17 +223,20 @@ HOA_DEVICE void st_product(uint8_t* sm, uint32_t tmem, bool accumulate, uint64_t
   tc_commit(done);
 }
 
-template <int DP>
+// V: floats of a global access to P (4 where d % 4 == 0, else 1).
+template <int DP, int V>
 __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_constant__ StepArgs p) {
   using L = StLayout<DP>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* gen = reinterpret_cast<float*>(sm + L::offGen);
   float* vec = reinterpret_cast<float*>(sm + L::offVec);
   float* sum = reinterpret_cast<float*>(sm + L::offSum);
   float* s_max = reinterpret_cast<float*>(sm + L::offMax);     // one per warp
   uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   float* delta = reinterpret_cast<float*>(sm);
+  float* part = reinterpret_cast<float*>(sm + L::kDelta);
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int d = p.d, dd = d * d;
   if (tid == 0) {
@@ -214,14 +251,54 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  StUnit<DP> un{sm, tmem + ((uint32_t)(warp & 3) << 21), (warp & 3) * 32 + lid, warp >> 2};
+  const StUnit<DP> un{sm, tmem + ((uint32_t)(warp & 3) << 21), (warp & 3) * 32 + lid, warp >> 2};
   const int row = un.row;
   uint32_t phase = 0;
   bool bad = false;
-  constexpr int CH = (L::NC + 1) / 2;                          // 16-column chunks of a thread, at most
 
-  // shared-memory and TMEM writes of every thread -> the tensor core; thread 0 issues; all wait
-  auto product = [&](auto smem_left, bool accumulate) {
+  // V columns of P a thread, rows pr, pr + RG, ...: a pass over P is contiguous
+  const int n4 = d / V, RG = kStThreads / n4, pc = (tid % n4) * V;
+  int pr = tid / n4;
+  constexpr int kRows = (DP + (kStThreads * V / DP) - 1) / (kStThreads * V / DP);
+  float pv[kRows][V];
+  auto load_P = [&](const float* P) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = pr + k * RG;
+      const bool in = r < d && pr < RG;
+      if (V == 4) {
+        const float4 v = in ? *reinterpret_cast<const float4*>(P + r * d + pc) : make_float4(0.f, 0.f, 0.f, 0.f);
+        pv[k][0] = v.x; pv[k][V > 1 ? 1 : 0] = v.y; pv[k][V > 2 ? 2 : 0] = v.z; pv[k][V > 3 ? 3 : 0] = v.w;
+      } else {
+        pv[k][0] = in ? P[r * d + pc] : 0.f;
+      }
+    }
+  };
+  // P as the right factor; its pad rows and columns are zero already (every right factor's are)
+  auto put_P = [&]() {
+    asm volatile("" : "+r"(pr));
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = pr + k * RG;
+      if (r >= d || pr >= RG) break;
+      uint8_t* at = sm + (pc >> 6) * L::kSlab + sw128_offset(r, (pc & 63) >> 3) + (pc & 7) * 2;
+      if (V == 4) {
+        uint2 hi, lo;
+        st_split2(f2_mul(f2(pv[k][0], pv[k][V > 1 ? 1 : 0]), f2(kSP)), hi.x, lo.x);
+        st_split2(f2_mul(f2(pv[k][V > 2 ? 2 : 0], pv[k][V > 3 ? 3 : 0]), f2(kSP)), hi.y, lo.y);
+        *reinterpret_cast<uint2*>(at) = hi;
+        *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+      } else {
+        const float v = pv[k][0] * kSP;
+        const __half hi = __float2half_rn(v);
+        *reinterpret_cast<__half*>(at) = hi;
+        *reinterpret_cast<__half*>(at + L::kMat) = __float2half_rn(v - __half2float(hi));
+      }
+    }
+  };
+
+  // shared-memory and TMEM writes of every thread -> the tensor core; thread 0 issues
+  auto issue = [&](auto smem_left, bool accumulate) {
     tmem_wait_st();
     fence_proxy_async_smem();
     tc_fence_before();
@@ -230,6 +307,8 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       tc_fence_after();
       st_product<DP, decltype(smem_left)::value>(sm, tmem, accumulate, done);
     }
+  };
+  auto wait = [&]() {
     bad |= !mbar_wait(done, phase);
     phase ^= 1;
     tc_fence_after();
@@ -237,7 +316,20 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   using Yes = std::true_type;
   using No = std::false_type;
 
+  // a row's generators -> shared memory, one row ahead
+  const bool wide = ((reinterpret_cast<uintptr_t>(p.a) | (uintptr_t)(p.stride * 4)) & 15) == 0;
   const int units = p.B * p.H;
+  auto fetch = [&](int u) {
+    if (u < units) {
+      const float* g = p.a + (long long)u * p.stride;
+      const uint32_t dst = smem_u32(gen);
+      const int n = wide ? p.stride / 4 : p.stride;
+      for (int i = tid; i < n; i += kStThreads) cp_async(dst + i * (wide ? 16 : 4), g + i * (wide ? 4 : 1), wide);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(blockIdx.x);
+
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const int b = u / p.H, h = u % p.H;
     const int len = p.lens[b];
@@ -246,41 +338,60 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
     if (len <= 0) {                                            // (block-uniform)
       for (int i = tid; i < dd; i += kStThreads) Po[i] = P[i];
       for (int i = tid; i < d; i += kStThreads) store_elem(p.qh, (long long)u * d + i, p.dtype, 0.f);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fetch(u + gridDim.x);
       continue;
     }
-    for (int i = tid; i < 3 * d; i += kStThreads)
-      vec[i] = load_elem(p.qkv, b * p.qkv_stride + (long long)h * 3 * d + i, p.qkv_dtype);
+    asm volatile("" : "+r"(pr));                               // (as q0 below)
+    // this token's vectors and its slot: read now, used at the end
+    float qv[(3 * DP + kStThreads - 1) / kStThreads];
+#pragma unroll
+    for (int k = 0; k < (3 * DP + kStThreads - 1) / kStThreads; ++k) {
+      const int i = tid + k * kStThreads;
+      qv[k] = i < 3 * d ? load_elem(p.qkv, b * p.qkv_stride + (long long)h * 3 * d + i, p.qkv_dtype) : 0.f;
+    }
+    const int pg = (len - 1) / p.page;
+    const int id = pg < p.W ? p.table[b * p.tstride + pg] : -1;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();                                           // the staged generators are in; the last row's sums were read
+#pragma unroll
+    for (int k = 0; k < (3 * DP + kStThreads - 1) / kStThreads; ++k)
+      if (tid + k * kStThreads < 3 * d) vec[tid + k * kStThreads] = qv[k];
     if (len > 1) {
-      // ---- A: rows q and d-2-q of the strict upper triangle together have d entries; a warp takes
-      // every eighth such pair, a lane every 32nd entry
-      constexpr int QW = (DP / 2 + 7) / 8, EW = (DP + 31) / 32;
-      float av[QW][EW];
-      const float* g = p.a + (long long)u * p.stride;
-      const float* bias = p.a_bias ? p.a_bias + (long long)h * p.stride : nullptr;
-      const int nq = d / 2;                                    // pairs (the middle row alone when d is even)
-      auto entry = [&](int x, int y, int& i, int& j) -> bool {
-        const int q = warp + 8 * x, e = lid + 32 * y;
-        const int first = d - 1 - q;
-        i = e < first ? q : d - 2 - q;
-        j = e < first ? q + 1 + e : i + 1 + (e - first);
-        return q < nq && e < d && (e < first || i != q);
+      // ---- A, row by row: entry (r, c) is +-the generator of {r, c}
+      if (p.a_bias) {
+        const float* bias = p.a_bias + (long long)h * p.stride;
+        for (int i = tid; i < p.stride; i += kStThreads) gen[i] += bias[i];
+        __syncthreads();
+      }
+      int rr = row;                                            // (opaque: not worked out ahead for every column and spilled)
+      asm volatile("" : "+r"(rr));
+      const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1;   // packed: {r, c}, r < c, lies at base_r + c
+      auto chunk = [&](int c0, float (&v)[16]) {
+        if (p.banked) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = c0 + e;
+            v[e] = rr < d && c < d && c != rr ? gen[gen_banked_slot(rr, c, d)] : 0.f;
+          }
+        } else {
+          int base_c = c0 * (2 * d - c0 - 1) / 2 - c0 - 1;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int c = c0 + e;
+            v[e] = rr < d && c < d && c != rr ? gen[c > rr ? base_r + c : base_c + rr] : 0.f;
+            base_c += d - c - 2;
+          }
+        }
       };
       float mx = 0.f;
+#pragma unroll 1
+      for (int c = un.half; c < L::NC; c += 2) {
+        float v[16];
+        chunk(16 * c, v);
 #pragma unroll
-      for (int x = 0; x < QW; ++x)
-#pragma unroll
-        for (int y = 0; y < EW; ++y) {
-          int i, j;
-          av[x][y] = 0.f;
-          if (entry(x, y, i, j)) {
-            const int at = p.banked ? gen_banked_slot(i, j, d) : i * (2 * d - i - 1) / 2 + j - i - 1;
-            av[x][y] = g[at];
-            if (bias) av[x][y] += bias[at];
-            av[x][y] *= p.edge_scale;
-          }
-          mx = fmaxf(mx, fabsf(av[x][y]));
-        }
-      for (int i = tid; i < (2 * L::kMat) / 16; i += kStThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0, 0, 0, 0);
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(v[e]));
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       if (lid == 0) s_max[warp] = mx;
@@ -289,40 +400,34 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
 #pragma unroll
       for (int w = 1; w < 8; ++w) mx = fmaxf(mx, s_max[w]);
       // s = 2^(10 - exponent): entries of A s below 2^10
+      mx *= fabsf(p.edge_scale);
       int ex = 0;
       frexpf(mx, &ex);
       ex = mx > 0.f ? min(max(ex, -60), 60) : 0;
-      const float sA = ldexpf(1.f, 10 - ex), iA = ldexpf(1.f, ex - 10);
+      const float sA = p.edge_scale * ldexpf(1.f, 10 - ex), iA = ldexpf(1.f, ex - 10);
+#pragma unroll 1
+      for (int c = un.half; c < L::NC; c += 2) {
+        float a[16];
+        chunk(16 * c, a);
+        F2 v[8];
 #pragma unroll
-      for (int x = 0; x < QW; ++x)
-#pragma unroll
-        for (int y = 0; y < EW; ++y) {
-          int i, j;
-          if (entry(x, y, i, j)) {
-            const float v = av[x][y] * sA;
-            const __half hi = __float2half_rn(v), lo = __float2half_rn(v - __half2float(hi));
-            uint8_t* up = sm + (j >> 6) * L::kSlab + sw128_offset(i, (j & 63) >> 3) + (j & 7) * 2;
-            uint8_t* dn = sm + (i >> 6) * L::kSlab + sw128_offset(j, (i & 63) >> 3) + (i & 7) * 2;
-            *reinterpret_cast<__half*>(up) = hi;
-            *reinterpret_cast<__half*>(up + L::kMat) = lo;
-            *reinterpret_cast<__half*>(dn) = __hneg(hi);
-            *reinterpret_cast<__half*>(dn + L::kMat) = __hneg(lo);
-          }
-        }
+        for (int e = 0; e < 16; e += 2)
+          v[e / 2] = f2_mul(f2(a[e], a[e + 1]), f2(16 * c + e > rr ? sA : -sA, 16 * c + e + 1 > rr ? sA : -sA));
+        un.put_right(c, v);
+      }
       // ---- P1: A2, and the scaling: ||A2||_1 (A2 is symmetric: row sums) bounds ||A||_2^2
-      product(Yes{}, false);
+      issue(Yes{}, false);
+      fetch(u + gridDim.x);                                    // (the staged row has been read)
+      wait();
       float rs = 0.f;
+#pragma unroll 1
+      for (int c = un.half; c < L::NC; c += 2) {
+        float v[16];
+        tmem_ld16(un.tmem + L::colD + 16 * c, v);
+        tmem_wait_ld();
+        tmem_touch(v);
 #pragma unroll
-      for (int x = 0; x < CH; ++x) {
-        const int c = 2 * x + un.half;
-        if (c < L::NC) {
-          float v[16];
-          tmem_ld16(un.tmem + L::colD + 16 * c, v);
-          tmem_wait_ld();
-          tmem_touch(v);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) rs += fabsf(v[e]);
-        }
+        for (int e = 0; e < 16; ++e) rs += fabsf(v[e]);
       }
       sum[un.half * 128 + row] = rs;
       __syncthreads();
@@ -339,106 +444,103 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       while (theta > kStTheta && nsq < 64) { theta *= 0.5f; ++nsq; }
       const float sa = ldexpf(iA, -nsq), sa2 = sa * sa;        // A = (hi + lo) sa, A2 = D sa2 once scaled
       // ---- P2: A4 = A2 T
+      {
+        const F2 ca = f2(kStX1 * kST * sa), ca2 = f2(kStX2 * kST / kSA2), cl = f2(kSA2 * sa2);
+#pragma unroll 1
+        for (int c = un.half; c < L::NC; c += 2) {
+          {
+            float v[16];
+            F2 a[8], a2[8];
+            tmem_ld16(un.tmem + L::colD + 16 * c, v);
+            un.get_right(c, a);
+            tmem_wait_ld();
+            tmem_touch(v);
 #pragma unroll
-      for (int x = 0; x < CH; ++x) {
-        const int c = 2 * x + un.half;
-        if (c < L::NC) {
-          float a[16], a2[16];
-          tmem_ld16(un.tmem + L::colD + 16 * c, a2);
-          un.get_right(c, a, sa);
-          tmem_wait_ld();
-          tmem_touch(a2);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            a2[e] *= sa2;
-            a[e] = kStX1 * a[e] + kStX2 * a2[e];
+            for (int e = 0; e < 8; ++e) {
+              a2[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), cl);
+              a[e] = f2_fma(a[e], ca, f2_mul(a2[e], ca2));
+            }
+            un.put_left(c, a2);
+            un.put_right(c, a);
           }
-          un.put_left(c, a2, kSA2);
-          un.put_right(c, a, kST);
         }
       }
-      product(No{}, false);
-      // ---- P3: E = E0 + L R
+      issue(No{}, false);
+      wait();
+      // ---- P3: E = E0 + L R, in units of 1 / (kSL kSR)
+      {
+        const F2 ct = f2(1.f / (kST * kStX1)), cta = f2(-kStX2 / (kStX1 * kSA2)), cq = f2(1.f / (kSA2 * kST));
+        const F2 l2 = f2(kStX3 * kSL / kSA2), lq = f2(kSL), r1 = f2(kStX5 * kSR), r2 = f2(kStX6 * kSR / kSA2),
+                 rq = f2(kStX7 * kSR), e1 = f2(kSL * kSR), e2 = f2(kStY2 * kSL * kSR / kSA2), el = f2(kSR);
+#pragma unroll 1
+        for (int c = un.half; c < L::NC; c += 2) {
+          {
+            float v[16], hh[8], ll[8];
+            F2 t[8], a2[8];
+            tmem_ld16(un.tmem + L::colD + 16 * c, v);
+            un.load_left(c, hh, ll);
+            un.get_right(c, t);
+            tmem_wait_ld();
+            tmem_touch(v);
+            un.join_left(hh, ll, a2);
 #pragma unroll
-      for (int x = 0; x < CH; ++x) {
-        const int c = 2 * x + un.half;
-        if (c < L::NC) {
-          float a4[16], t[16], a2[16], hh[8], ll[8];
-          tmem_ld16(un.tmem + L::colD + 16 * c, a4);
-          un.load_left(c, hh, ll);
-          un.get_right(c, t, 1.f / kST);
-          tmem_wait_ld();
-          tmem_touch(a4);
-          un.join_left(hh, ll, a2, 1.f / kSA2);
-          float r[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = (t[e] - kStX2 * a2[e]) * (1.f / kStX1), q = a4[e] * (1.f / (kSA2 * kST));
-            const float l = kStX3 * a2[e] + q;
-            r[e] = kStX5 * a + kStX6 * a2[e] + kStX7 * q;
-            a4[e] = l;
-            t[e] = (a + kStY2 * a2[e] + l) * (kSL * kSR);
+            for (int e = 0; e < 8; ++e) {
+              const F2 a = f2_fma(t[e], ct, f2_mul(a2[e], cta));               // A = (T - x2 A2) / x1
+              const F2 q = f2_mul(f2(v[2 * e], v[2 * e + 1]), cq);             // A4
+              const F2 l = f2_fma(q, lq, f2_mul(a2[e], l2));
+              const float2 e0 = f2_get(f2_fma(a, e1, f2_fma(a2[e], e2, f2_mul(l, el))));
+              t[e] = f2_fma(a, r1, f2_fma(a2[e], r2, f2_mul(q, rq)));
+              a2[e] = l;
+              v[2 * e] = e0.x;
+              v[2 * e + 1] = e0.y;
+            }
+            un.put_left(c, a2);
+            un.put_right(c, t);
+            tmem_st16(un.tmem + L::colD + 16 * c, v);
           }
-          un.put_left(c, a4, kSL);
-          un.put_right(c, r, kSR);
-          tmem_st16(un.tmem + L::colD + 16 * c, t);
         }
       }
-      product(No{}, true);
+      issue(No{}, true);
+      load_P(P);
+      wait();
       // ---- E, squared nsq times: (I + E)^2 = I + (2 E + E E)
+      if (nsq == 0) put_P();
       for (int s = 0;; ++s) {
-#pragma unroll
-        for (int x = 0; x < CH; ++x) {
-          const int c = 2 * x + un.half;
-          if (c < L::NC) {
-            float e1[16], e0[16], hh[8], ll[8];
-            tmem_ld16(un.tmem + L::colD + 16 * c, e1);
+        const F2 ce = s > 0 ? f2(1.f / kSE) : f2(kSE / (kSL * kSR));
+#pragma unroll 1
+        for (int c = un.half; c < L::NC; c += 2) {
+          {
+            float v[16], hh[8], ll[8];
+            F2 e1[8];
+            tmem_ld16(un.tmem + L::colD + 16 * c, v);
             if (s > 0) un.load_left(c, hh, ll);
             tmem_wait_ld();
-            tmem_touch(e1);
-            if (s > 0) {
-              un.join_left(hh, ll, e0, 2.f / kSE);
+            tmem_touch(v);
+            if (s > 0) un.join_left(hh, ll, e1);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) e1[e] = fmaf(e1[e], 1.f / (kSE * kSE), e0[e]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) e1[e] *= 1.f / (kSL * kSR);
+            for (int e = 0; e < 8; ++e) {
+              const F2 y = f2_mul(f2(v[2 * e], v[2 * e + 1]), ce);
+              e1[e] = s > 0 ? f2_fma(e1[e], f2(2.f), y) : y;
             }
-            un.put_left(c, e1, kSE);
-            if (s < nsq) un.put_right(c, e1, kSE);
+            un.put_left(c, e1);
+            if (s < nsq) un.put_right(c, e1);
           }
         }
         if (s >= nsq) break;
-        product(No{}, false);
+        issue(No{}, false);
+        wait();
       }
-      // ---- P4: E P.  Pad rows and columns of the right factor are zero already.
-      if (d % 4 == 0) {
-        const int n4 = d / 4;
-        for (int i = tid; i < dd / 4; i += kStThreads) {
-          const int r = i / n4, c = (i % n4) * 4;
-          const float4 v = reinterpret_cast<const float4*>(P)[i];
-          uint2 hi, lo;
-          st_split2(v.x * kSP, v.y * kSP, hi.x, lo.x);
-          st_split2(v.z * kSP, v.w * kSP, hi.y, lo.y);
-          uint8_t* at = sm + (c >> 6) * L::kSlab + sw128_offset(r, (c & 63) >> 3) + (c & 7) * 2;
-          *reinterpret_cast<uint2*>(at) = hi;
-          *reinterpret_cast<uint2*>(at + L::kMat) = lo;
-        }
-      } else {
-        for (int i = tid; i < dd; i += kStThreads) {
-          const int r = i / d, c = i % d;
-          const float v = P[i] * kSP;
-          const __half hi = __float2half_rn(v), lo = __float2half_rn(v - __half2float(hi));
-          uint8_t* at = sm + (c >> 6) * L::kSlab + sw128_offset(r, (c & 63) >> 3) + (c & 7) * 2;
-          *reinterpret_cast<__half*>(at) = hi;
-          *reinterpret_cast<__half*>(at + L::kMat) = lo;
-        }
+      if (nsq > 0) {
+        load_P(P);
+        put_P();
       }
-      product(No{}, false);
-#pragma unroll
-      for (int x = 0; x < CH; ++x) {
-        const int c = 2 * x + un.half;
-        if (c < L::NC) {
+      // ---- P4: E P
+      issue(No{}, false);
+      load_P(P);                                               // again, for P + E P (from L2)
+      wait();
+#pragma unroll 1
+      for (int c = un.half; c < L::NC; c += 2) {
+        {
           float v[16];
           tmem_ld16(un.tmem + L::colD + 16 * c, v);
           tmem_wait_ld();
@@ -446,74 +548,85 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
           if (row < d) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(delta + row * L::kLd + 16 * c + e) =
-                  make_float4(v[e] * (1.f / (kSE * kSP)), v[e + 1] * (1.f / (kSE * kSP)), v[e + 2] * (1.f / (kSE * kSP)),
-                              v[e + 3] * (1.f / (kSE * kSP)));
+              *reinterpret_cast<float4*>(delta + row * L::kLd + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           }
         }
       }
+    } else {
+      fetch(u + gridDim.x);                                    // (P' = I: the staged row goes unused)
     }
     if (__syncthreads_or(bad)) break;
-    // ---- P' = P + E P, to global memory and in place of E P
-    if (len > 1 && d % 4 == 0) {
-      const int n4 = d / 4;
-      for (int i = tid; i < dd / 4; i += kStThreads) {
-        float4* at = reinterpret_cast<float4*>(delta + (i / n4) * L::kLd + (i % n4) * 4);
-        const float4 v = reinterpret_cast<const float4*>(P)[i], e = *at;
-        const float4 y = make_float4(v.x + e.x, v.y + e.y, v.z + e.z, v.w + e.w);
-        reinterpret_cast<float4*>(Po)[i] = y;
-        *at = y;
-      }
-    } else {
-      for (int i = tid; i < dd; i += kStThreads) {
-        const int r = i / d, c = i % d;
-        const float y = len > 1 ? P[i] + delta[r * L::kLd + c] : (r == c ? 1.f : 0.f);
-        Po[i] = y;
-        delta[r * L::kLd + c] = y;
+    asm volatile("" : "+r"(pr));
+    // ---- P' = P + E P to global memory, and this thread's part of q^, k^, v^ = P'^T q, ...
+    float y[3][V];
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[w][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = pr + k * RG;
+      if (r < d && pr < RG) {
+        float x[V];
+        if (V == 4) {
+          const float4 e = *reinterpret_cast<const float4*>(delta + r * L::kLd + pc);
+          x[0] = e.x; x[V > 1 ? 1 : 0] = e.y; x[V > 2 ? 2 : 0] = e.z; x[V > 3 ? 3 : 0] = e.w;
+        } else {
+          x[0] = delta[r * L::kLd + pc];
+        }
+        const float q = vec[r], kk = vec[d + r], vv = vec[2 * d + r];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          x[e] = len > 1 ? fmaf(x[e], 1.f / (kSE * kSP), pv[k][e]) : (r == pc + e ? 1.f : 0.f);
+          y[0][e] = fmaf(x[e], q, y[0][e]);
+          y[1][e] = fmaf(x[e], kk, y[1][e]);
+          y[2][e] = fmaf(x[e], vv, y[2][e]);
+        }
+        if (V == 4) *reinterpret_cast<float4*>(Po + r * d + pc) = make_float4(x[0], x[V > 1 ? 1 : 0], x[V > 2 ? 2 : 0], x[V > 3 ? 3 : 0]);
+        else Po[r * d + pc] = x[0];
       }
     }
-    __syncthreads();
-    // ---- q^, k^, v^ = P'^T q, ...: a thread per column and half of the rows
-    const int c = tid & 127, part = tid >> 7;
-    float y0 = 0.f, y1 = 0.f, y2 = 0.f;
-    if (c < d) {
-#pragma unroll 4
-      for (int r = part; r < d; r += 2) {
-        const float x = delta[r * L::kLd + c];
-        y0 = fmaf(x, vec[r], y0);
-        y1 = fmaf(x, vec[d + r], y1);
-        y2 = fmaf(x, vec[2 * d + r], y2);
-      }
-      if (part) { sum[c] = y0; sum[128 + c] = y1; sum[256 + c] = y2; }
+    if (pr < RG) {
+#pragma unroll
+      for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int e = 0; e < V; ++e) part[(pr * 3 + w) * d + pc + e] = y[w][e];
     }
     __syncthreads();
-    if (c < d && part == 0) {
-      const int pos = len - 1, pg = pos / p.page;
-      const int id = pg < p.W ? p.table[b * p.tstride + pg] : -1;
-      store_elem(p.qh, (long long)u * d + c, p.dtype, y0 + sum[c]);
-      if (id >= 0 && id < p.n_pages) {
-        const long long at = id * p.ps + h * p.hs + (long long)(pos % p.page) * p.ts + c;
-        store_elem(p.kp, at, p.dtype, y1 + sum[128 + c]);
-        store_elem(p.vp, at, p.dtype, y2 + sum[256 + c]);
+    for (int i = tid; i < 3 * d; i += kStThreads) {
+      float t = 0.f;
+      for (int g = 0; g < RG; ++g) t += part[g * 3 * d + i];
+      const int w = i / d, c = i - w * d;
+      if (w == 0) {
+        store_elem(p.qh, (long long)u * d + c, p.dtype, t);
+      } else if (id >= 0 && id < p.n_pages) {
+        const long long at = id * p.ps + h * p.hs + (long long)((len - 1) % p.page) * p.ts + c;
+        store_elem(w == 1 ? p.kp : p.vp, at, p.dtype, t);
       } else if (c == 0) {
         st_fail(p.status);
       }
     }
-    __syncthreads();                                           // the next row overwrites shared memory
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (__syncthreads_or(bad) && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, L::kCols);
 }
 
-template <int DP>
-static int launch_step(const StepArgs& s, int num_sms, cudaStream_t stream) {
+template <int DP, int V>
+static int launch_step_v(const StepArgs& s, int num_sms, cudaStream_t stream) {
   using L = StLayout<DP>;
-  if (cudaFuncSetAttribute(path_step_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
+  if (cudaFuncSetAttribute(path_step_kernel<DP, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
     return HOA_ERR_LAUNCH;
   const int units = s.B * s.H;
-  path_step_kernel<DP><<<(unsigned)(units < 2 * num_sms ? units : 2 * num_sms), kStThreads, L::kAlloc, stream>>>(s);
+  path_step_kernel<DP, V><<<(unsigned)(units < 2 * num_sms ? units : 2 * num_sms), kStThreads, L::kAlloc, stream>>>(s);
   return launch_status();
+}
+
+template <int DP>
+static int launch_step(const StepArgs& s, int num_sms, cudaStream_t stream) {
+  const bool v4 = s.d % 4 == 0 && ((reinterpret_cast<uintptr_t>(s.P) | reinterpret_cast<uintptr_t>(s.P_out)) & 15) == 0;
+  return v4 ? launch_step_v<DP, 4>(s, num_sms, stream) : launch_step_v<DP, 1>(s, num_sms, stream);
 }
 
 }  // namespace hoa
