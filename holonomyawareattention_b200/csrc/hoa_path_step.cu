@@ -62,7 +62,7 @@ HOA_DEVICE void st_fail(int* status) {
 // ---------------------------------------------------------------------------
 using namespace sm100;
 
-constexpr int kStThreads = 256;
+constexpr int kStGroups = 2, kStThreads = 128 * kStGroups;     // warpgroups: each has all 128 rows and every kStGroups-th chunk
 constexpr float kSA2 = 2048.f, kST = 16384.f, kSL = 4096.f, kSR = 4096.f, kSE = 512.f, kSP = 256.f;
 
 template <int DP>
@@ -74,13 +74,14 @@ struct StLayout {
   static constexpr int kRight = 2 * kMat + (128 - DP) * 128;   // hi, lo; P1 reads 128 rows as its left factor
   static constexpr int kDim = DP < 120 ? DP : 120;       // the largest head dim
   static constexpr int kDelta = kDim * kLd * 4;
-  static constexpr int kDeltaEnd = kDelta + 256 * 12 * 4;      // + the partial sums of q^, k^, v^ (12 a thread)
-  static constexpr int offGen = ((kRight > kDeltaEnd ? kRight : kDeltaEnd) + 127) / 128 * 128;   // the next row's generators
+  static constexpr int kPart = kStThreads * 12 * 4;            // partial sums of q^, k^, v^, in place of E P
+  static constexpr int kWork = kRight > kDelta ? kRight : kDelta;
+  static constexpr int offGen = ((kWork > kPart ? kWork : kPart) + 127) / 128 * 128;   // the next row's generators
   static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2) * 4;   // (either layout: banked has d / 2 unused slots)
   static constexpr int offVec = offGen + (kGen + 127) / 128 * 128;
-  static constexpr int offSum = offVec + 3 * DP * 4;           // row sums (2 x 128)
-  static constexpr int offMax = offSum + 2 * 128 * 4;
-  static constexpr int offBar = offMax + 32;
+  static constexpr int offSum = offVec + 3 * DP * 4;           // row sums, of each group
+  static constexpr int offMax = offSum + kStThreads * 4;
+  static constexpr int offBar = offMax + 64;
   static constexpr int kAlloc = offBar + 32 + 1024;
   static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
   static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
@@ -133,13 +134,13 @@ HOA_DEVICE F2 st_join2(uint32_t hi, uint32_t lo) {
   return f2_add(f2(h.x, h.y), f2(l.x, l.y));
 }
 
-// What a thread owns of the matrices: a row (= TMEM lane), and every other 16 columns.
+// What a thread owns of the matrices: a row (= TMEM lane), and every kStGroups-th 16 columns.
 template <int DP>
 struct StUnit {
   using L = StLayout<DP>;
   uint8_t* sm;
   uint32_t tmem;           // + this warp's lanes
-  int row, half;
+  int row, group;
 
   // 16 columns (chunk c) of this thread's row of the right factor
   HOA_DEVICE void put_right(int c, const F2 (&v)[8]) const {
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   float* delta = reinterpret_cast<float*>(sm);
-  float* part = reinterpret_cast<float*>(sm + L::kDelta);
+  float* part = reinterpret_cast<float*>(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int d = p.d, dd = d * d;
   if (tid == 0) {
@@ -364,33 +365,13 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
         for (int i = tid; i < p.stride; i += kStThreads) gen[i] += bias[i];
         __syncthreads();
       }
-      int rr = row;                                            // (opaque: not worked out ahead for every column and spilled)
-      asm volatile("" : "+r"(rr));
-      const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1;   // packed: {r, c}, r < c, lies at base_r + c
-      auto chunk = [&](int c0, float (&v)[16]) {
-        if (p.banked) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = c0 + e;
-            v[e] = rr < d && c < d && c != rr ? gen[gen_banked_slot(rr, c, d)] : 0.f;
-          }
-        } else {
-          int base_c = c0 * (2 * d - c0 - 1) / 2 - c0 - 1;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int c = c0 + e;
-            v[e] = rr < d && c < d && c != rr ? gen[c > rr ? base_r + c : base_c + rr] : 0.f;
-            base_c += d - c - 2;
-          }
-        }
-      };
       float mx = 0.f;
-#pragma unroll 1
-      for (int c = un.half; c < L::NC; c += 2) {
-        float v[16];
-        chunk(16 * c, v);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fabsf(v[e]));
+      const int diag = p.banked ? (d / 32) * (d / 32 - 1) * 512 : p.stride;   // banked: where the diagonal blocks begin
+#pragma unroll 4
+      for (int i = tid; i < p.stride; i += kStThreads) {
+        const int o = i - diag;
+        const bool unused = o >= 0 && (o & 0x1e1) == 0x1e0;    // their slots that hold no generator may hold anything
+        mx = fmaxf(mx, unused ? 0.f : fabsf(gen[i]));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -398,22 +379,72 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       __syncthreads();
       mx = s_max[0];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) mx = fmaxf(mx, s_max[w]);
+      for (int w = 1; w < 4 * kStGroups; ++w) mx = fmaxf(mx, s_max[w]);
       // s = 2^(10 - exponent): entries of A s below 2^10
       mx *= fabsf(p.edge_scale);
       int ex = 0;
       frexpf(mx, &ex);
       ex = mx > 0.f ? min(max(ex, -60), 60) : 0;
       const float sA = p.edge_scale * ldexpf(1.f, 10 - ex), iA = ldexpf(1.f, ex - 10);
+      // Row r of A, 16 columns at a time: entry (r, c) is +gen{r, c} right of the diagonal, -gen{c, r} left of
+      // it.  A chunk that the diagonal misses in all 32 rows of the warp has one rule for all of them.
+      const int w0 = row & ~31, rr = min(row, d - 1);          // (rows past the matrix read its last row and get 0)
+      const float sr = row < d ? sA : 0.f;
+      const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1;   // packed: {r, c}, r < c, lies at base_r + c
+      if (w0 < DP) {
 #pragma unroll 1
-      for (int c = un.half; c < L::NC; c += 2) {
-        float a[16];
-        chunk(16 * c, a);
-        F2 v[8];
+        for (int c = un.group; c < L::NC; c += kStGroups) {
+          const int c0 = 16 * c;
+          float v[16];
+          float sg = sr;
+          if (p.banked) {                                      // gen_banked_slot, 32 x 32 block by block
+            const int nb = d >> 5, ba = w0 >> 5, bb = c0 >> 5, v0 = c0 & 31, lo = min(ba, bb), hi = max(ba, bb);
+            const float* blk = gen + (lo * nb - lo * (lo + 1) / 2 + hi - lo - 1) * 1024;
+            if (ba < bb) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2)
-          v[e / 2] = f2_mul(f2(a[e], a[e + 1]), f2(16 * c + e > rr ? sA : -sA, 16 * c + e + 1 > rr ? sA : -sA));
-        un.put_right(c, v);
+              for (int e = 0; e < 16; ++e) v[e] = blk[lid * 32 + ((v0 + e) ^ (4 * (lid & 7)))];
+            } else if (ba > bb) {
+              sg = -sr;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) v[e] = blk[(v0 + e) * 32 + (lid ^ (4 * ((v0 + e) & 7)))];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int cc = c0 + e;
+                const float g = gen[cc != rr ? gen_banked_slot(rr, cc, d) : 0];
+                v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
+              }
+            }
+          } else if (c0 > w0 + 31) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = gen[base_r + c0 + e];
+          } else {
+            int base_c = c0 * (2 * d - c0 - 1) / 2 - c0 - 1;
+            if (c0 + 15 < w0) {
+              sg = -sr;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                v[e] = gen[base_c + rr];
+                base_c += d - c0 - e - 2;
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int cc = c0 + e;
+                const float g = gen[max(0, min(cc > rr ? base_r + cc : base_c + rr, p.stride - 1))];
+                v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
+                base_c += d - cc - 2;
+              }
+            }
+          }
+          if (c0 + 16 > d)                                     // pad columns
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = c0 + e < d ? v[e] : 0.f;
+          F2 y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), f2(sg));
+          un.put_right(c, y);
+        }
       }
       // ---- P1: A2, and the scaling: ||A2||_1 (A2 is symmetric: row sums) bounds ||A||_2^2
       issue(Yes{}, false);
@@ -421,7 +452,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       wait();
       float rs = 0.f;
 #pragma unroll 1
-      for (int c = un.half; c < L::NC; c += 2) {
+      for (int c = un.group; c < L::NC; c += kStGroups) {
         float v[16];
         tmem_ld16(un.tmem + L::colD + 16 * c, v);
         tmem_wait_ld();
@@ -429,13 +460,16 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 16; ++e) rs += fabsf(v[e]);
       }
-      sum[un.half * 128 + row] = rs;
+      sum[un.group * 128 + row] = rs;
       __syncthreads();
       float top = 0.f;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int r = lid + 32 * x;
-        if (r < d) top = fmaxf(top, sum[r] + sum[128 + r]);
+        float t = 0.f;
+#pragma unroll
+        for (int g = 0; g < kStGroups; ++g) t += sum[g * 128 + r];
+        if (r < d) top = fmaxf(top, t);
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -447,7 +481,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       {
         const F2 ca = f2(kStX1 * kST * sa), ca2 = f2(kStX2 * kST / kSA2), cl = f2(kSA2 * sa2);
 #pragma unroll 1
-        for (int c = un.half; c < L::NC; c += 2) {
+        for (int c = un.group; c < L::NC; c += kStGroups) {
           {
             float v[16];
             F2 a[8], a2[8];
@@ -469,11 +503,14 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       wait();
       // ---- P3: E = E0 + L R, in units of 1 / (kSL kSR)
       {
-        const F2 ct = f2(1.f / (kST * kStX1)), cta = f2(-kStX2 / (kStX1 * kSA2)), cq = f2(1.f / (kSA2 * kST));
-        const F2 l2 = f2(kStX3 * kSL / kSA2), lq = f2(kSL), r1 = f2(kStX5 * kSR), r2 = f2(kStX6 * kSR / kSA2),
-                 rq = f2(kStX7 * kSR), e1 = f2(kSL * kSR), e2 = f2(kStY2 * kSL * kSR / kSA2), el = f2(kSR);
+        // with t = T kST, a = A2 kSA2, q = A4 kSA2 kST and A = (T - x2 A2) / x1:
+        //   l = L kSL,  r = R kSR,  e = E0 kSL kSR
+        const F2 la = f2(kStX3 * kSL / kSA2), lq = f2(kSL / (kSA2 * kST));
+        const F2 rt = f2(kStX5 / kStX1 * kSR / kST), ra = f2((kStX6 - kStX5 * kStX2 / kStX1) * kSR / kSA2),
+                 rq = f2(kStX7 * kSR / (kSA2 * kST));
+        const F2 et = f2(kSL * kSR / (kStX1 * kST)), ea = f2((kStY2 - kStX2 / kStX1) * kSL * kSR / kSA2), el = f2(kSR);
 #pragma unroll 1
-        for (int c = un.half; c < L::NC; c += 2) {
+        for (int c = un.group; c < L::NC; c += kStGroups) {
           {
             float v[16], hh[8], ll[8];
             F2 t[8], a2[8];
@@ -485,11 +522,10 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
             un.join_left(hh, ll, a2);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const F2 a = f2_fma(t[e], ct, f2_mul(a2[e], cta));               // A = (T - x2 A2) / x1
-              const F2 q = f2_mul(f2(v[2 * e], v[2 * e + 1]), cq);             // A4
-              const F2 l = f2_fma(q, lq, f2_mul(a2[e], l2));
-              const float2 e0 = f2_get(f2_fma(a, e1, f2_fma(a2[e], e2, f2_mul(l, el))));
-              t[e] = f2_fma(a, r1, f2_fma(a2[e], r2, f2_mul(q, rq)));
+              const F2 q = f2(v[2 * e], v[2 * e + 1]);
+              const F2 l = f2_fma(q, lq, f2_mul(a2[e], la));
+              const float2 e0 = f2_get(f2_fma(l, el, f2_fma(a2[e], ea, f2_mul(t[e], et))));
+              t[e] = f2_fma(q, rq, f2_fma(a2[e], ra, f2_mul(t[e], rt)));
               a2[e] = l;
               v[2 * e] = e0.x;
               v[2 * e + 1] = e0.y;
@@ -508,7 +544,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       for (int s = 0;; ++s) {
         const F2 ce = s > 0 ? f2(1.f / kSE) : f2(kSE / (kSL * kSR));
 #pragma unroll 1
-        for (int c = un.half; c < L::NC; c += 2) {
+        for (int c = un.group; c < L::NC; c += kStGroups) {
           {
             float v[16], hh[8], ll[8];
             F2 e1[8];
@@ -539,7 +575,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       load_P(P);                                               // again, for P + E P (from L2)
       wait();
 #pragma unroll 1
-      for (int c = un.half; c < L::NC; c += 2) {
+      for (int c = un.group; c < L::NC; c += kStGroups) {
         {
           float v[16];
           tmem_ld16(un.tmem + L::colD + 16 * c, v);
@@ -586,6 +622,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
         else Po[r * d + pc] = x[0];
       }
     }
+    __syncthreads();                                           // E P has been read
     if (pr < RG) {
 #pragma unroll
       for (int w = 0; w < 3; ++w)
