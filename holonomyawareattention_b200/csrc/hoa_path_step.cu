@@ -41,7 +41,8 @@ HOA_DEVICE void st_fail(int* status) {
 // tensor-core products hi hi + hi lo + lo hi with fp32 accumulation; lo lo, 2^-22 of
 // it, is left out.  f16 runs at twice the rate of tf32 and has its 11 bits; its
 // short exponent is no loss, because the bounds are known: theta <= 0.6 after
-// scaling, |P| <= 1.
+// scaling, |P| <= 1.  (A itself is split at 16 A: entries up to 4094 fit, and what
+// f16 drops of small ones, 2^-29, is below fp32's rounding of P'.)
 //
 //   P1  A2 = A A                                  scale 2^-s from ||A2||_1 >= ||A||_2^2
 //   P2  A4 = A2 T,        T = x1 A + x2 A2
@@ -63,7 +64,7 @@ HOA_DEVICE void st_fail(int* status) {
 using namespace sm100;
 
 constexpr int kStGroups = 2, kStThreads = 128 * kStGroups;     // warpgroups: each has all 128 rows and every kStGroups-th chunk
-constexpr float kSA2 = 2048.f, kST = 16384.f, kSL = 4096.f, kSR = 4096.f, kSE = 512.f, kSP = 256.f;
+constexpr float kSA = 16.f, kSA2 = 2048.f, kST = 16384.f, kSL = 4096.f, kSR = 4096.f, kSE = 512.f, kSP = 256.f;
 
 template <int DP>
 struct StLayout {
@@ -80,8 +81,7 @@ struct StLayout {
   static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2) * 4;   // (either layout: banked has d / 2 unused slots)
   static constexpr int offVec = offGen + (kGen + 127) / 128 * 128;
   static constexpr int offSum = offVec + 3 * DP * 4;           // row sums, of each group
-  static constexpr int offMax = offSum + kStThreads * 4;
-  static constexpr int offBar = offMax + 64;
+  static constexpr int offBar = offSum + kStThreads * 4;
   static constexpr int kAlloc = offBar + 32 + 1024;
   static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
   static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
@@ -188,9 +188,7 @@ struct StUnit {
     tmem_ld8(tmem + L::colHi + 8 * c, h);
     tmem_ld8(tmem + L::colLo + 8 * c, l);
   }
-  HOA_DEVICE static void join_left(float (&h)[8], float (&l)[8], F2 (&v)[8]) {   // after tmem_wait_ld
-    tmem_touch(h);
-    tmem_touch(l);
+  HOA_DEVICE static void join_left(float (&h)[8], float (&l)[8], F2 (&v)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = st_join2(__float_as_uint(h[e]), __float_as_uint(l[e]));
   }
@@ -233,7 +231,6 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   float* gen = reinterpret_cast<float*>(sm + L::offGen);
   float* vec = reinterpret_cast<float*>(sm + L::offVec);
   float* sum = reinterpret_cast<float*>(sm + L::offSum);
-  float* s_max = reinterpret_cast<float*>(sm + L::offMax);     // one per warp
   uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   float* delta = reinterpret_cast<float*>(sm);
@@ -257,44 +254,87 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   uint32_t phase = 0;
   bool bad = false;
 
-  // V columns of P a thread, rows pr, pr + RG, ...: a pass over P is contiguous
-  const int n4 = d / V, RG = kStThreads / n4, pc = (tid % n4) * V;
+  // f(c, x) for this thread's chunks c, x the values there; the next chunk's are on their way meanwhile
+  auto chunks = [&](auto load, auto f) {
+    int c = un.group;
+    if (c >= L::NC) return;
+    auto x = load(c), y = x;
+    tmem_wait_ld();
+    x.touch();
+#pragma unroll 1
+    while (true) {
+      const int n = c + kStGroups;
+      if (n < L::NC) y = load(n);
+      f(c, x);
+      if (n >= L::NC) break;
+      tmem_wait_ld();
+      y.touch();
+      x = y;
+      c = n;
+    }
+  };
+  struct Acc {
+    float v[16];
+    HOA_DEVICE void touch() { tmem_touch(v); }
+  };
+  struct AccLeft {
+    float v[16], h[8], l[8];
+    HOA_DEVICE void touch() { tmem_touch(v); tmem_touch(h); tmem_touch(l); }
+  };
+  auto load_acc = [&](int c) {
+    Acc x;
+    tmem_ld16(un.tmem + L::colD + 16 * c, x.v);
+    return x;
+  };
+  auto load_left = [&](int c) {
+    AccLeft x;
+    tmem_ld16(un.tmem + L::colD + 16 * c, x.v);
+    un.load_left(c, x.h, x.l);
+    return x;
+  };
+
+  // V columns of P a thread, rows pr, pr + RG, ... (pn of them): a pass over P is contiguous
+  const int n4 = d / V, RG = kStThreads / n4, pc = (tid % n4) * V, step = RG * d;
   int pr = tid / n4;
+  const int pn = pr < RG && pr < d ? (d - pr + RG - 1) / RG : 0;
   constexpr int kRows = (DP + (kStThreads * V / DP) - 1) / (kStThreads * V / DP);
-  float pv[kRows][V];
+  using PV = typename std::conditional<V == 4, float4, float>::type;
+  PV pv[kRows];
   auto load_P = [&](const float* P) {
+    const float* at = P + pr * d + pc;
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int r = pr + k * RG;
-      const bool in = r < d && pr < RG;
-      if (V == 4) {
-        const float4 v = in ? *reinterpret_cast<const float4*>(P + r * d + pc) : make_float4(0.f, 0.f, 0.f, 0.f);
-        pv[k][0] = v.x; pv[k][V > 1 ? 1 : 0] = v.y; pv[k][V > 2 ? 2 : 0] = v.z; pv[k][V > 3 ? 3 : 0] = v.w;
-      } else {
-        pv[k][0] = in ? P[r * d + pc] : 0.f;
-      }
+      pv[k] = PV{};
+      if (k < pn) pv[k] = *reinterpret_cast<const PV*>(at);
+      at += step;
     }
   };
   // P as the right factor; its pad rows and columns are zero already (every right factor's are)
   auto put_P = [&]() {
     asm volatile("" : "+r"(pr));
+    uint8_t* slab = sm + (pc >> 6) * L::kSlab + (pc & 7) * 2;
+    const uint32_t ch = (pc & 63) >> 3;
+    int r = pr;
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int r = pr + k * RG;
-      if (r >= d || pr >= RG) break;
-      uint8_t* at = sm + (pc >> 6) * L::kSlab + sw128_offset(r, (pc & 63) >> 3) + (pc & 7) * 2;
-      if (V == 4) {
+      uint8_t* at = slab + sw128_offset(r, ch);
+      if constexpr (V == 4) {
         uint2 hi, lo;
-        st_split2(f2_mul(f2(pv[k][0], pv[k][V > 1 ? 1 : 0]), f2(kSP)), hi.x, lo.x);
-        st_split2(f2_mul(f2(pv[k][V > 2 ? 2 : 0], pv[k][V > 3 ? 3 : 0]), f2(kSP)), hi.y, lo.y);
-        *reinterpret_cast<uint2*>(at) = hi;
-        *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+        st_split2(f2_mul(f2(pv[k].x, pv[k].y), f2(kSP)), hi.x, lo.x);
+        st_split2(f2_mul(f2(pv[k].z, pv[k].w), f2(kSP)), hi.y, lo.y);
+        if (k < pn) {
+          *reinterpret_cast<uint2*>(at) = hi;
+          *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+        }
       } else {
-        const float v = pv[k][0] * kSP;
-        const __half hi = __float2half_rn(v);
-        *reinterpret_cast<__half*>(at) = hi;
-        *reinterpret_cast<__half*>(at + L::kMat) = __float2half_rn(v - __half2float(hi));
+        const float v = pv[k] * kSP;
+        const __half hi = __float2half_rn(v), lo = __float2half_rn(v - __half2float(hi));
+        if (k < pn) {
+          *reinterpret_cast<__half*>(at) = hi;
+          *reinterpret_cast<__half*>(at + L::kMat) = lo;
+        }
       }
+      r += RG;
     }
   };
 
@@ -331,9 +371,27 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   };
   fetch(blockIdx.x);
 
-  for (int u = blockIdx.x; u < units; u += gridDim.x) {
-    const int b = u / p.H, h = u % p.H;
-    const int len = p.lens[b];
+  // the token's vectors and its page, read one row ahead too
+  constexpr int kQ = (3 * DP + kStThreads - 1) / kStThreads;
+  float qv[kQ];
+  int len = 0, id = -1;
+  auto peek_len = [&](int u) { return u < units ? p.lens[u / p.H] : 0; };
+  auto peek = [&](int u, int n) {
+    if (n <= 0) return;
+    const int b = u / p.H, h = u - b * p.H, pg = (n - 1) / p.page;
+#pragma unroll
+    for (int k = 0; k < kQ; ++k) {
+      const int i = tid + k * kStThreads;
+      qv[k] = i < 3 * d ? load_elem(p.qkv, b * p.qkv_stride + (long long)h * 3 * d + i, p.qkv_dtype) : 0.f;
+    }
+    id = pg < p.W ? p.table[b * p.tstride + pg] : -1;
+  };
+  len = peek_len(blockIdx.x);
+  peek(blockIdx.x, len);
+
+  for (int u = blockIdx.x, next = 0; u < units; u += gridDim.x, len = next) {
+    const int h = u % p.H;
+    next = peek_len(u + gridDim.x);
     const float* P = p.P + (long long)u * dd;
     float* Po = p.P_out + (long long)u * dd;
     if (len <= 0) {                                            // (block-uniform)
@@ -341,23 +399,17 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       for (int i = tid; i < d; i += kStThreads) store_elem(p.qh, (long long)u * d + i, p.dtype, 0.f);
       asm volatile("cp.async.wait_all;" ::: "memory");
       fetch(u + gridDim.x);
+      peek(u + gridDim.x, next);
       continue;
     }
-    asm volatile("" : "+r"(pr));                               // (as q0 below)
-    // this token's vectors and its slot: read now, used at the end
-    float qv[(3 * DP + kStThreads - 1) / kStThreads];
-#pragma unroll
-    for (int k = 0; k < (3 * DP + kStThreads - 1) / kStThreads; ++k) {
-      const int i = tid + k * kStThreads;
-      qv[k] = i < 3 * d ? load_elem(p.qkv, b * p.qkv_stride + (long long)h * 3 * d + i, p.qkv_dtype) : 0.f;
-    }
-    const int pg = (len - 1) / p.page;
-    const int id = pg < p.W ? p.table[b * p.tstride + pg] : -1;
+    asm volatile("" : "+r"(pr));                               // (as rr below)
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                           // the staged generators are in; the last row's sums were read
 #pragma unroll
-    for (int k = 0; k < (3 * DP + kStThreads - 1) / kStThreads; ++k)
+    for (int k = 0; k < kQ; ++k)
       if (tid + k * kStThreads < 3 * d) vec[tid + k * kStThreads] = qv[k];
+    const int at_page = id;
+    peek(u + gridDim.x, next);
     if (len > 1) {
       // ---- A, row by row: entry (r, c) is +-the generator of {r, c}
       if (p.a_bias) {
@@ -365,31 +417,10 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
         for (int i = tid; i < p.stride; i += kStThreads) gen[i] += bias[i];
         __syncthreads();
       }
-      float mx = 0.f;
-      const int diag = p.banked ? (d / 32) * (d / 32 - 1) * 512 : p.stride;   // banked: where the diagonal blocks begin
-#pragma unroll 4
-      for (int i = tid; i < p.stride; i += kStThreads) {
-        const int o = i - diag;
-        const bool unused = o >= 0 && (o & 0x1e1) == 0x1e0;    // their slots that hold no generator may hold anything
-        mx = fmaxf(mx, unused ? 0.f : fabsf(gen[i]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (lid == 0) s_max[warp] = mx;
-      __syncthreads();
-      mx = s_max[0];
-#pragma unroll
-      for (int w = 1; w < 4 * kStGroups; ++w) mx = fmaxf(mx, s_max[w]);
-      // s = 2^(10 - exponent): entries of A s below 2^10
-      mx *= fabsf(p.edge_scale);
-      int ex = 0;
-      frexpf(mx, &ex);
-      ex = mx > 0.f ? min(max(ex, -60), 60) : 0;
-      const float sA = p.edge_scale * ldexpf(1.f, 10 - ex), iA = ldexpf(1.f, ex - 10);
       // Row r of A, 16 columns at a time: entry (r, c) is +gen{r, c} right of the diagonal, -gen{c, r} left of
       // it.  A chunk that the diagonal misses in all 32 rows of the warp has one rule for all of them.
       const int w0 = row & ~31, rr = min(row, d - 1);          // (rows past the matrix read its last row and get 0)
-      const float sr = row < d ? sA : 0.f;
+      const float sr = row < d ? p.edge_scale * kSA : 0.f;
       const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1;   // packed: {r, c}, r < c, lies at base_r + c
       if (w0 < DP) {
 #pragma unroll 1
@@ -451,15 +482,10 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       fetch(u + gridDim.x);                                    // (the staged row has been read)
       wait();
       float rs = 0.f;
-#pragma unroll 1
-      for (int c = un.group; c < L::NC; c += kStGroups) {
-        float v[16];
-        tmem_ld16(un.tmem + L::colD + 16 * c, v);
-        tmem_wait_ld();
-        tmem_touch(v);
+      chunks(load_acc, [&](int, Acc& x) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) rs += fabsf(v[e]);
-      }
+        for (int e = 0; e < 16; ++e) rs += fabsf(x.v[e]);
+      });
       sum[un.group * 128 + row] = rs;
       __syncthreads();
       float top = 0.f;
@@ -473,31 +499,24 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float theta = sqrtf(top) * iA;
+      float theta = sqrtf(top) * (1.f / kSA);
       int nsq = 0;
       while (theta > kStTheta && nsq < 64) { theta *= 0.5f; ++nsq; }
-      const float sa = ldexpf(iA, -nsq), sa2 = sa * sa;        // A = (hi + lo) sa, A2 = D sa2 once scaled
+      const float sa = ldexpf(1.f / kSA, -nsq), sa2 = sa * sa;        // A = (hi + lo) sa, A2 = D sa2 once scaled
       // ---- P2: A4 = A2 T
       {
         const F2 ca = f2(kStX1 * kST * sa), ca2 = f2(kStX2 * kST / kSA2), cl = f2(kSA2 * sa2);
-#pragma unroll 1
-        for (int c = un.group; c < L::NC; c += kStGroups) {
-          {
-            float v[16];
-            F2 a[8], a2[8];
-            tmem_ld16(un.tmem + L::colD + 16 * c, v);
-            un.get_right(c, a);
-            tmem_wait_ld();
-            tmem_touch(v);
+        chunks(load_acc, [&](int c, Acc& x) {
+          F2 a[8], a2[8];
+          un.get_right(c, a);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              a2[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), cl);
-              a[e] = f2_fma(a[e], ca, f2_mul(a2[e], ca2));
-            }
-            un.put_left(c, a2);
-            un.put_right(c, a);
+          for (int e = 0; e < 8; ++e) {
+            a2[e] = f2_mul(f2(x.v[2 * e], x.v[2 * e + 1]), cl);
+            a[e] = f2_fma(a[e], ca, f2_mul(a2[e], ca2));
           }
-        }
+          un.put_left(c, a2);
+          un.put_right(c, a);
+        });
       }
       issue(No{}, false);
       wait();
@@ -509,62 +528,50 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
         const F2 rt = f2(kStX5 / kStX1 * kSR / kST), ra = f2((kStX6 - kStX5 * kStX2 / kStX1) * kSR / kSA2),
                  rq = f2(kStX7 * kSR / (kSA2 * kST));
         const F2 et = f2(kSL * kSR / (kStX1 * kST)), ea = f2((kStY2 - kStX2 / kStX1) * kSL * kSR / kSA2), el = f2(kSR);
-#pragma unroll 1
-        for (int c = un.group; c < L::NC; c += kStGroups) {
-          {
-            float v[16], hh[8], ll[8];
-            F2 t[8], a2[8];
-            tmem_ld16(un.tmem + L::colD + 16 * c, v);
-            un.load_left(c, hh, ll);
-            un.get_right(c, t);
-            tmem_wait_ld();
-            tmem_touch(v);
-            un.join_left(hh, ll, a2);
+        chunks(load_left, [&](int c, AccLeft& x) {
+          F2 t[8], a2[8];
+          un.get_right(c, t);
+          un.join_left(x.h, x.l, a2);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const F2 q = f2(v[2 * e], v[2 * e + 1]);
-              const F2 l = f2_fma(q, lq, f2_mul(a2[e], la));
-              const float2 e0 = f2_get(f2_fma(l, el, f2_fma(a2[e], ea, f2_mul(t[e], et))));
-              t[e] = f2_fma(q, rq, f2_fma(a2[e], ra, f2_mul(t[e], rt)));
-              a2[e] = l;
-              v[2 * e] = e0.x;
-              v[2 * e + 1] = e0.y;
-            }
-            un.put_left(c, a2);
-            un.put_right(c, t);
-            tmem_st16(un.tmem + L::colD + 16 * c, v);
+          for (int e = 0; e < 8; ++e) {
+            const F2 q = f2(x.v[2 * e], x.v[2 * e + 1]);
+            const F2 l = f2_fma(q, lq, f2_mul(a2[e], la));
+            const float2 e0 = f2_get(f2_fma(l, el, f2_fma(a2[e], ea, f2_mul(t[e], et))));
+            t[e] = f2_fma(q, rq, f2_fma(a2[e], ra, f2_mul(t[e], rt)));
+            a2[e] = l;
+            x.v[2 * e] = e0.x;
+            x.v[2 * e + 1] = e0.y;
           }
-        }
+          un.put_left(c, a2);
+          un.put_right(c, t);
+          tmem_st16(un.tmem + L::colD + 16 * c, x.v);
+        });
       }
       issue(No{}, true);
       load_P(P);
       wait();
       // ---- E, squared nsq times: (I + E)^2 = I + (2 E + E E)
       if (nsq == 0) put_P();
-      for (int s = 0;; ++s) {
-        const F2 ce = s > 0 ? f2(1.f / kSE) : f2(kSE / (kSL * kSR));
-#pragma unroll 1
-        for (int c = un.group; c < L::NC; c += kStGroups) {
-          {
-            float v[16], hh[8], ll[8];
-            F2 e1[8];
-            tmem_ld16(un.tmem + L::colD + 16 * c, v);
-            if (s > 0) un.load_left(c, hh, ll);
-            tmem_wait_ld();
-            tmem_touch(v);
-            if (s > 0) un.join_left(hh, ll, e1);
+      chunks(load_acc, [&](int c, Acc& x) {
+        F2 e1[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const F2 y = f2_mul(f2(v[2 * e], v[2 * e + 1]), ce);
-              e1[e] = s > 0 ? f2_fma(e1[e], f2(2.f), y) : y;
-            }
-            un.put_left(c, e1);
-            if (s < nsq) un.put_right(c, e1);
-          }
-        }
-        if (s >= nsq) break;
+        for (int e = 0; e < 8; ++e) e1[e] = f2_mul(f2(x.v[2 * e], x.v[2 * e + 1]), f2(kSE / (kSL * kSR)));
+        un.put_left(c, e1);
+        if (nsq > 0) un.put_right(c, e1);
+      });
+#pragma unroll 1
+      for (int s = 1; s <= nsq; ++s) {
         issue(No{}, false);
         wait();
+        chunks(load_left, [&](int c, AccLeft& x) {
+          F2 e1[8];
+          un.join_left(x.h, x.l, e1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            e1[e] = f2_fma(e1[e], f2(2.f), f2_mul(f2(x.v[2 * e], x.v[2 * e + 1]), f2(1.f / kSE)));
+          un.put_left(c, e1);
+          if (s < nsq) un.put_right(c, e1);
+        });
       }
       if (nsq > 0) {
         load_P(P);
@@ -574,20 +581,13 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       issue(No{}, false);
       load_P(P);                                               // again, for P + E P (from L2)
       wait();
-#pragma unroll 1
-      for (int c = un.group; c < L::NC; c += kStGroups) {
-        {
-          float v[16];
-          tmem_ld16(un.tmem + L::colD + 16 * c, v);
-          tmem_wait_ld();
-          tmem_touch(v);
-          if (row < d) {
+      chunks(load_acc, [&](int c, Acc& x) {
+        if (row < d) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              *reinterpret_cast<float4*>(delta + row * L::kLd + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          }
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(delta + row * L::kLd + 16 * c + e) = make_float4(x.v[e], x.v[e + 1], x.v[e + 2], x.v[e + 3]);
         }
-      }
+      });
     } else {
       fetch(u + gridDim.x);                                    // (P' = I: the staged row goes unused)
     }
@@ -599,27 +599,56 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
     for (int w = 0; w < 3; ++w)
 #pragma unroll
       for (int e = 0; e < V; ++e) y[w][e] = 0.f;
+    if (len <= 1) {
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const int r = pr + k * RG;
-      if (r < d && pr < RG) {
-        float x[V];
-        if (V == 4) {
-          const float4 e = *reinterpret_cast<const float4*>(delta + r * L::kLd + pc);
-          x[0] = e.x; x[V > 1 ? 1 : 0] = e.y; x[V > 2 ? 2 : 0] = e.z; x[V > 3 ? 3 : 0] = e.w;
-        } else {
-          x[0] = delta[r * L::kLd + pc];
-        }
-        const float q = vec[r], kk = vec[d + r], vv = vec[2 * d + r];
+      for (int k = 0; k < kRows; ++k) pv[k] = PV{};
+    }
+    {
+      // four rows' shared-memory reads at a time; a row past the last one reads the last one and counts as zero
+      constexpr int kB = 4;
+      const float es = len > 1 ? 1.f / (kSE * kSP) : 0.f;
+      float* op = Po + pr * d + pc;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          x[e] = len > 1 ? fmaf(x[e], 1.f / (kSE * kSP), pv[k][e]) : (r == pc + e ? 1.f : 0.f);
-          y[0][e] = fmaf(x[e], q, y[0][e]);
-          y[1][e] = fmaf(x[e], kk, y[1][e]);
-          y[2][e] = fmaf(x[e], vv, y[2][e]);
+      for (int k0 = 0; k0 < kRows; k0 += kB) {
+        PV dv[kB];
+        float q[kB][3];
+#pragma unroll
+        for (int k = 0; k < kB; ++k) {
+          const int r = min(pr + (k0 + k) * RG, d - 1);
+          dv[k] = *reinterpret_cast<const PV*>(delta + r * L::kLd + pc);
+          q[k][0] = vec[r];
+          q[k][1] = vec[d + r];
+          q[k][2] = vec[2 * d + r];
         }
-        if (V == 4) *reinterpret_cast<float4*>(Po + r * d + pc) = make_float4(x[0], x[V > 1 ? 1 : 0], x[V > 2 ? 2 : 0], x[V > 3 ? 3 : 0]);
-        else Po[r * d + pc] = x[0];
+#pragma unroll
+        for (int k = 0; k < kB; ++k) {
+          if (k0 + k >= kRows) break;
+          const bool in = k0 + k < pn;
+          float x[V];
+          if constexpr (V == 4) {
+            x[0] = fmaf(dv[k].x, es, pv[k0 + k].x);
+            x[1] = fmaf(dv[k].y, es, pv[k0 + k].y);
+            x[2] = fmaf(dv[k].z, es, pv[k0 + k].z);
+            x[3] = fmaf(dv[k].w, es, pv[k0 + k].w);
+          } else {
+            x[0] = fmaf(dv[k], es, pv[k0 + k]);
+          }
+          if (len <= 1)
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = pr + (k0 + k) * RG == pc + e ? 1.f : 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            x[e] = in ? x[e] : 0.f;
+            y[0][e] = fmaf(x[e], q[k][0], y[0][e]);
+            y[1][e] = fmaf(x[e], q[k][1], y[1][e]);
+            y[2][e] = fmaf(x[e], q[k][2], y[2][e]);
+          }
+          if (in) {
+            if constexpr (V == 4) *reinterpret_cast<float4*>(op) = make_float4(x[0], x[1], x[2], x[3]);
+            else *op = x[0];
+          }
+          op += step;
+        }
       }
     }
     __syncthreads();                                           // E P has been read
@@ -636,8 +665,8 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       const int w = i / d, c = i - w * d;
       if (w == 0) {
         store_elem(p.qh, (long long)u * d + c, p.dtype, t);
-      } else if (id >= 0 && id < p.n_pages) {
-        const long long at = id * p.ps + h * p.hs + (long long)((len - 1) % p.page) * p.ts + c;
+      } else if (at_page >= 0 && at_page < p.n_pages) {
+        const long long at = at_page * p.ps + h * p.hs + (long long)((len - 1) % p.page) * p.ts + c;
         store_elem(w == 1 ? p.kp : p.vp, at, p.dtype, t);
       } else if (c == 0) {
         st_fail(p.status);
