@@ -24,6 +24,7 @@ constexpr int kPsRows = 16, kPsKeys = 64, kPsThreads = 128;
 
 __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   extern __shared__ float sm[];
+  pa_let_next_start();
   const int d = p.d, ld = d | 1;                       // odd row stride: rows fall on different banks
   float* Qs = sm;                                      // [16][ld]
   float* Ks = Qs + kPsRows * ld;                       // [64][ld]
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __gri
         if (kg + 8 * i < d) o[i] = fmaf(e, Vs[k * ld + kg + 8 * i], o[i]);
     }
   }
+  pa_end_after_previous();
   if (!my.ok) return;
   const long long part = (long long)it.slot * p.rows + my.grow;
   if (kg == 0) p.part_ml[part] = make_float2(m, l);
@@ -109,41 +111,151 @@ __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __gri
 // ---------------------------------------------------------------------------
 // join the parts of each (row, query, head); optionally out = P o
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(128) paged_attn_join_kernel(const __grid_constant__ PaArgs p) {
-  __shared__ float s_o[128];
-  const int d = p.d, c = threadIdx.x, slots = p.ns1 + p.ns2;
-  for (long long g = blockIdx.x; g < p.rows; g += gridDim.x) {
-    float m = -INFINITY;
-    for (int s = 0; s < slots; ++s) {
+// kWpr warps share an output row: one where rows are many, eight (a CTA a row) where
+// the parts or P are most of the bytes.  A lane holds four columns (V = 4, d % 4 == 0)
+// or up to four that are 32 apart.  Launched while the items still run: P, which does
+// not depend on them, is read before the wait (8 lanes a row of P, 32 rows a pass,
+// all passes' loads at once), so that its bytes - most of a decode step's, 4 d^2 a
+// head - are under way when the parts arrive.
+constexpr int kPjThreads = 256;
+
+template <int V, int kWpr, bool kPaths>
+__global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __grid_constant__ PaArgs p) {
+  static_assert(!kPaths || kWpr == 8, "P takes the whole CTA");
+  __shared__ float4 s_o[8][32];
+  __shared__ float s_l[8];
+  const int d = p.d, slots = p.ns1 + p.ns2, warp = threadIdx.x >> 5, lid = threadIdx.x & 31;
+  const int w = warp % kWpr;
+  const long long g = (long long)blockIdx.x * (8 / kWpr) + warp / kWpr;
+  const bool ok = g < p.rows;                          // (uniform in the warps that share a row)
+  float4 P[4][4];                                      // pass, chunk of 4 columns
+  const int pr = threadIdx.x >> 3, pq = threadIdx.x & 7;
+  if constexpr (kPaths) {
+    const float* Pg = p.paths + g * d * d;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int r = pr + 32 * x, c = 4 * (pq + 8 * y);
+        P[x][y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < d) {
+          if (V == 4) {
+            if (c < d) P[x][y] = *reinterpret_cast<const float4*>(Pg + r * d + c);
+          } else {
+            const float* at = Pg + r * d + c;
+            if (c < d) P[x][y].x = at[0];
+            if (c + 1 < d) P[x][y].y = at[1];
+            if (c + 2 < d) P[x][y].z = at[2];
+            if (c + 3 < d) P[x][y].w = at[3];
+          }
+        }
+      }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float m = -INFINITY;
+  if (ok)
+    for (int s = lid; s < slots; s += 32) {
       const float2 ml = p.part_ml[s * p.rows + g];
       if (ml.y > 0.f) m = fmaxf(m, ml.x);
     }
-    float l = 0.f, o = 0.f;
-    for (int s = 0; s < slots; ++s) {
-      const float2 ml = p.part_ml[s * p.rows + g];
-      if (!(ml.y > 0.f)) continue;
-      const float w = exp2f(ml.x - m);
-      l = fmaf(w, ml.y, l);
-      if (c < d) o = fmaf(w, p.part_o[(s * p.rows + g) * d + c], o);
-    }
-    o = l > 0.f ? o / l : 0.f;
-    if (c == 0) p.lse[g] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
-    if (p.paths == nullptr) {
-      if (c < d) store_elem(p.out, g * d + c, p.out_dtype, o);
-      continue;
-    }
-    __syncthreads();
-    s_o[c] = c < d ? o : 0.f;
-    __syncthreads();
-    const float* P = p.paths + g * d * d;
-    for (int i = c >> 5; i < d; i += 4) {
-      float y = 0.f;
-      for (int j = c & 31; j < d; j += 32) y = fmaf(P[i * d + j], s_o[j], y);
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
-      if ((c & 31) == 0) store_elem(p.out, g * d + i, p.out_dtype, y);
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  if (ok && m != -INFINITY) {
+#pragma unroll 4
+    for (int s = w; s < slots; s += kWpr) {
+      const float2 ml = p.part_ml[s * p.rows + g];
+      const float f = ml.y > 0.f ? exp2f(ml.x - m) : 0.f;
+      l = fmaf(f, ml.y, l);
+      const float* at = p.part_o + (s * p.rows + g) * d;
+      if (V == 4) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (4 * lid < d && ml.y > 0.f) v = *reinterpret_cast<const float4*>(at + 4 * lid);   // (a part without a key wrote no O)
+        o[0] = fmaf(f, v.x, o[0]); o[1] = fmaf(f, v.y, o[1]); o[2] = fmaf(f, v.z, o[2]); o[3] = fmaf(f, v.w, o[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (lid + 32 * e < d && ml.y > 0.f) o[e] = fmaf(f, at[lid + 32 * e], o[e]);
+      }
     }
   }
+  if constexpr (kWpr > 1) {
+    s_o[w][lid] = make_float4(o[0], o[1], o[2], o[3]);
+    if (lid == 0) s_l[w] = l;
+    __syncthreads();
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    l = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWpr; ++x) {
+      const float4 v = s_o[x][lid];
+      t[0] += v.x; t[1] += v.y; t[2] += v.z; t[3] += v.w;
+      l += s_l[x];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = t[e];
+  }
+  if (!ok) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  if (w == 0 && lid == 0) p.lse[g] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  if constexpr (kPaths) {
+    float* so = reinterpret_cast<float*>(s_o);         // o in column order, zero past d
+    __syncthreads();
+    if (w == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = V == 4 ? 4 * lid + e : lid + 32 * e;
+        so[c] = c < d ? o[e] : 0.f;
+      }
+    }
+    __syncthreads();
+    float4 q[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) q[y] = *reinterpret_cast<const float4*>(so + 4 * (pq + 8 * y));
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      float y = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        y = fmaf(P[x][k].x, q[k].x, fmaf(P[x][k].y, q[k].y, fmaf(P[x][k].z, q[k].z, fmaf(P[x][k].w, q[k].w, y))));
+#pragma unroll
+      for (int k = 1; k < 8; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
+      const int r = pr + 32 * x;
+      if (pq == 0 && r < d) store_elem(p.out, g * d + r, p.out_dtype, y);
+    }
+  } else if (w == 0) {
+    if (V == 4 && 4 * lid < d) {
+      if (p.out_dtype == HOA_BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(o[0], o[1]), b = __floats2bfloat162_rn(o[2], o[3]);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + g * d + 4 * lid) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      } else {
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + g * d + 4 * lid) = make_float4(o[0], o[1], o[2], o[3]);
+      }
+    } else if (V == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lid + 32 * e < d) store_elem(p.out, g * d + lid + 32 * e, p.out_dtype, o[e]);
+    }
+  }
+}
+
+template <int V, int kWpr, bool kPaths>
+static int launch_join(const PaArgs& a, bool early, cudaStream_t s) {
+  const long long blocks = (a.rows + 8 / kWpr - 1) / (8 / kWpr);
+  if (blocks > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;
+  return pa_launch(paged_attn_join_kernel<V, kWpr, kPaths>, (unsigned)blocks, kPjThreads, 0, s, early, a);
+}
+
+static int join(const PaArgs& a, bool early, cudaStream_t s) {
+  // 16-byte accesses: four columns a lane of o, the parts and P
+  const bool v4 = a.d % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.paths) |
+                                    reinterpret_cast<uintptr_t>(a.part_o)) & 15) == 0;
+  if (a.paths) return v4 ? launch_join<4, 8, true>(a, early, s) : launch_join<1, 8, true>(a, early, s);
+  // eight warps a row where one a row would leave SMs without work and there are parts to share
+  if (a.rows < 148 * 16 && a.ns1 + a.ns2 > 4) return v4 ? launch_join<4, 8, false>(a, early, s) : launch_join<1, 8, false>(a, early, s);
+  return v4 ? launch_join<4, 1, false>(a, early, s) : launch_join<1, 1, false>(a, early, s);
 }
 
 }  // namespace hoa
@@ -170,15 +282,15 @@ extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, i
   return most;
 }
 
-static int run_items(int kind, const PaArgs& a, long long first, long long items, cudaStream_t s) {
+// `early`: may start while the launch before it (the other part's items) still runs
+static int run_items(int kind, const PaArgs& a, long long first, long long items, bool early, cudaStream_t s) {
   if (items == 0) return HOA_OK;
-  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, s);
-  if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, s);
+  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, early, s);
+  if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, early, s);
   const size_t smem = ((kPsRows + 2 * kPsKeys) * (size_t)(a.d | 1) + kPsRows * kPsKeys) * sizeof(float);
   if (cudaFuncSetAttribute(paged_attn_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return HOA_ERR_LAUNCH;
-  paged_attn_simt_kernel<<<(unsigned)items, kPsThreads, smem, s>>>(a, (unsigned)first);
-  return launch_status();
+  return pa_launch(paged_attn_simt_kernel, (unsigned)items, kPsThreads, smem, s, early, a, (unsigned)first);
 }
 
 extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -217,12 +329,11 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int st;
   if (pl.kind1 == pl.kind2) {                      // one launch for both parts
-    st = run_items(pl.kind1, a, 0, items1 + items2, s);
+    st = run_items(pl.kind1, a, 0, items1 + items2, false, s);
   } else {
-    st = run_items(pl.kind1, a, 0, items1, s);
-    if (st == HOA_OK) st = run_items(pl.kind2, a, items1, items2, s);
+    st = run_items(pl.kind1, a, 0, items1, false, s);
+    if (st == HOA_OK) st = run_items(pl.kind2, a, items1, items2, items1 > 0, s);
   }
   if (st != HOA_OK) return st;
-  paged_attn_join_kernel<<<(unsigned)(a.rows < 148 * 64 ? a.rows : 148 * 64), 128, 0, s>>>(a);
-  return launch_status();
+  return join(a, items1 + items2 > 0, s);
 }

@@ -165,8 +165,31 @@ HOA_DEVICE long long pa_key(const PaArgs& p, const PaItem& it, int j) {
   return id * p.ps + it.kvh * p.hs + (long long)(j - pg * p.page) * p.ts;
 }
 
+// The launches of a call overlap (programmatic dependent launch): the items of part 2 may run beside those of
+// part 1, and the join comes up while the last items run.  Every kernel lets the next one start at once, and waits
+// for the one before it at its own end at the latest, so that a kernel has completed only after all before it have:
+// the join's wait then covers both.  The first launch of a call is an ordinary one.
+HOA_DEVICE void pa_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+HOA_DEVICE void pa_end_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class K, class... A>
+static int pa_launch(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t s, bool early, const A&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = early ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  return e == cudaSuccess ? launch_status() : (cudaGetLastError(), (int)HOA_ERR_LAUNCH);
+}
+
 // items first .. first + items - 1
-int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s);
+int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s);
 
 }  // namespace hoa

@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kPmWarps * 32, PmCfg<D8>::kMinBlocks)
 paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   using C = PmCfg<D8>;
   extern __shared__ __align__(16) uint8_t smem[];
+  pa_let_next_start();
   PaItem it = pa_item(p, first + blockIdx.x, 16, kPmKeys);
   const int tid = threadIdx.x, w = tid >> 5, lid = tid & 31, r0 = lid >> 2, q2 = (lid & 3) * 2;
   const uint32_t ring = sm100::smem_u32(smem) + w * C::kWarp;
@@ -220,6 +221,7 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   }
 
   // ---- join the warps
+  pa_end_after_previous();
   cp_wait<0>();
   __syncthreads();
   float* jn = reinterpret_cast<float*>(smem);
@@ -261,32 +263,31 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
 }
 
 template <int D8>
-static int launch_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+static int launch_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
   using C = PmCfg<D8>;
   if (cudaFuncSetAttribute(paged_attn_mma_kernel<D8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return HOA_ERR_LAUNCH;
-  paged_attn_mma_kernel<D8><<<items, kPmWarps * 32, C::kSmem, s>>>(a, first);
-  return launch_status();
+  return pa_launch(paged_attn_mma_kernel<D8>, items, kPmWarps * 32, C::kSmem, s, early, a, first);
 }
 
-int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
   switch (a.d / 8) {
-    case 1: return launch_mma<1>(a, first, items, s);
-    case 2: return launch_mma<2>(a, first, items, s);
-    case 3: return launch_mma<3>(a, first, items, s);
-    case 4: return launch_mma<4>(a, first, items, s);
-    case 5: return launch_mma<5>(a, first, items, s);
-    case 6: return launch_mma<6>(a, first, items, s);
-    case 7: return launch_mma<7>(a, first, items, s);
-    case 8: return launch_mma<8>(a, first, items, s);
-    case 9: return launch_mma<9>(a, first, items, s);
-    case 10: return launch_mma<10>(a, first, items, s);
-    case 11: return launch_mma<11>(a, first, items, s);
-    case 12: return launch_mma<12>(a, first, items, s);
-    case 13: return launch_mma<13>(a, first, items, s);
-    case 14: return launch_mma<14>(a, first, items, s);
-    case 15: return launch_mma<15>(a, first, items, s);
-    case 16: return launch_mma<16>(a, first, items, s);
+    case 1: return launch_mma<1>(a, first, items, early, s);
+    case 2: return launch_mma<2>(a, first, items, early, s);
+    case 3: return launch_mma<3>(a, first, items, early, s);
+    case 4: return launch_mma<4>(a, first, items, early, s);
+    case 5: return launch_mma<5>(a, first, items, early, s);
+    case 6: return launch_mma<6>(a, first, items, early, s);
+    case 7: return launch_mma<7>(a, first, items, early, s);
+    case 8: return launch_mma<8>(a, first, items, early, s);
+    case 9: return launch_mma<9>(a, first, items, early, s);
+    case 10: return launch_mma<10>(a, first, items, early, s);
+    case 11: return launch_mma<11>(a, first, items, early, s);
+    case 12: return launch_mma<12>(a, first, items, early, s);
+    case 13: return launch_mma<13>(a, first, items, early, s);
+    case 14: return launch_mma<14>(a, first, items, early, s);
+    case 15: return launch_mma<15>(a, first, items, early, s);
+    case 16: return launch_mma<16>(a, first, items, early, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
 }

@@ -87,6 +87,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
   volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 17);
   int* s_seen = reinterpret_cast<int*>(bars + 18);   // [2] the last key that a row of the tile sees, + 1
 
+  pa_let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int KT = pt.kt;
   const PaItem it = pa_item(p, first + blockIdx.x, 256, KT);
@@ -180,23 +181,32 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       const uint32_t colS[2] = {tmem + L::colS0, tmem + L::colS1};
       const uint32_t colO[2] = {tmem + L::colO0, tmem + L::colO1};
       bool ok = mbar_wait_abortable(q_full, 0, s_abort, pt.max_wait);
+      // Order: S0 S1 | PV0 S0' PV1 S1' | ...: a query tile's next scores are computed as soon as its own weights are
+      // taken, so that the two softmax warpgroups run out of step and the products of one hide behind the other's
+      // exponentials (with S0 S1 PV0 PV1 both waited for all four).
+      int have = 0;                                  // key tiles known to have landed
+      auto scores = [&](int i, int j) {
+        const int s = j % L::NS;
+        if (j >= have) {
+          ok = mbar_wait_abortable(&kv_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+          if (!ok) return;
+          have = j + 1;
+        }
+        tc_fence_after();
+        const uint64_t dK = desc_sw128(smem_u32(sm + L::offStage + s * L::kStage));
+#pragma unroll
+        for (int kk = 0; kk < KSTEPS; ++kk) {
+          const uint64_t off = (uint64_t)(((kk >> 2) * L::kBlk + (kk & 3) * 32) >> 4);
+          mma_bf16(colS[i], dQ[i] + off, dK + off, idS, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[i]);
+      };
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (ok && n_t[i] > 0) scores(i, 0);
       for (int j = 0; j < nkt && ok; ++j) {
         const int s = j % L::NS;
-        ok = mbar_wait_abortable(&kv_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t st = smem_u32(sm + L::offStage + s * L::kStage);
-        const uint64_t dK = desc_sw128(st), dV = desc_sw128_mn(st + L::kQ, L::kBlk);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (j >= n_t[i]) continue;
-#pragma unroll
-          for (int kk = 0; kk < KSTEPS; ++kk) {
-            const uint64_t off = (uint64_t)(((kk >> 2) * L::kBlk + (kk & 3) * 32) >> 4);
-            mma_bf16(colS[i], dQ[i] + off, dK + off, idS, kk > 0 ? 1u : 0u);
-          }
-          tc_commit(&s_full[i]);
-        }
+        const uint64_t dV = desc_sw128_mn(smem_u32(sm + L::offStage + s * L::kStage) + L::kQ, L::kBlk);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (j >= n_t[i] || !ok) continue;
@@ -206,6 +216,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
           for (int kk = 0; kk < KT / 16; ++kk)         // 16 keys: 16 rows of 128 bytes of every V slab
             mma_bf16_ts(colO[i], colS[i] + kk * 8, dV + (uint64_t)(kk * 2048 >> 4), idO, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit(&pv_done[i]);
+          if (j + 1 < n_t[i]) scores(i, j + 1);
         }
         tc_commit(&kv_empty[s]);
       }
@@ -346,6 +357,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     }
   }
 
+  pa_end_after_previous();
   bad = __syncthreads_or(bad || *s_abort != 0);
   if (bad && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
@@ -385,15 +397,14 @@ static bool page_map(CUtensorMap* m, const void* base, const PaArgs& a, int box)
 
 template <int DP16>
 static int launch_ptc(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, unsigned first,
-                      unsigned items, cudaStream_t s) {
+                      unsigned items, bool early, cudaStream_t s) {
   using L = PtLayout<DP16>;
   if (cudaFuncSetAttribute(paged_attn_tc_kernel<DP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
     return HOA_ERR_LAUNCH;
-  paged_attn_tc_kernel<DP16><<<items, kPtThreads, L::kAlloc, s>>>(mk, mv, a, t, first);
-  return launch_status();
+  return pa_launch(paged_attn_tc_kernel<DP16>, items, kPtThreads, L::kAlloc, s, early, mk, mv, a, t, first);
 }
 
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
   PtArgs t;
   t.kt = pa_tile_keys(a.page);
   t.box = a.page < t.kt ? a.page : t.kt;
@@ -402,14 +413,14 @@ int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t 
   CUtensorMap mk, mv;
   if (t.kt == 0 || !page_map(&mk, a.kp, a, t.box) || !page_map(&mv, a.vp, a, t.box)) return HOA_ERR_INVALID_ARG;
   switch ((a.d + 15) / 16) {
-    case 1: return launch_ptc<16>(mk, mv, a, t, first, items, s);
-    case 2: return launch_ptc<32>(mk, mv, a, t, first, items, s);
-    case 3: return launch_ptc<48>(mk, mv, a, t, first, items, s);
-    case 4: return launch_ptc<64>(mk, mv, a, t, first, items, s);
-    case 5: return launch_ptc<80>(mk, mv, a, t, first, items, s);
-    case 6: return launch_ptc<96>(mk, mv, a, t, first, items, s);
-    case 7: return launch_ptc<112>(mk, mv, a, t, first, items, s);
-    case 8: return launch_ptc<128>(mk, mv, a, t, first, items, s);
+    case 1: return launch_ptc<16>(mk, mv, a, t, first, items, early, s);
+    case 2: return launch_ptc<32>(mk, mv, a, t, first, items, early, s);
+    case 3: return launch_ptc<48>(mk, mv, a, t, first, items, early, s);
+    case 4: return launch_ptc<64>(mk, mv, a, t, first, items, early, s);
+    case 5: return launch_ptc<80>(mk, mv, a, t, first, items, early, s);
+    case 6: return launch_ptc<96>(mk, mv, a, t, first, items, early, s);
+    case 7: return launch_ptc<112>(mk, mv, a, t, first, items, early, s);
+    case 8: return launch_ptc<128>(mk, mv, a, t, first, items, early, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
 }
