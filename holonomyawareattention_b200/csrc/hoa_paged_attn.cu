@@ -322,6 +322,11 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.B = B; a.Tq = Tq; a.H = H; a.Hk = Hk; a.G = H / Hk; a.d = d; a.page = page; a.n_pages = n_pages;
   a.rows = (long long)B * Tq * H;
+  // with 2^s >= page > 2^(s-1): ceil(2^(31+s) / page) < 2^32, exact for j < 2^31
+  int sh = 0;
+  while ((1ll << sh) < page) ++sh;
+  a.page_mul = page > 1 ? (unsigned)(((1ull << (31 + sh)) + page - 1) / page) : 0u;
+  a.page_shift = sh - 1;
   a.ns1 = pl.ns1; a.ns2 = pl.ns2; a.tiles1 = pl.tiles1; a.tiles2 = pl.tiles2;
   a.status = status;
   a.part_o = static_cast<float*>(workspace);

@@ -21,6 +21,7 @@ struct PaArgs {
   long long rows;                                  // B * Tq * H
   float scale_log2;
   int dtype, B, Tq, H, Hk, G, d, page, n_pages;
+  unsigned page_mul; int page_shift;               // j / page = umulhi(j, page_mul) >> page_shift for 0 <= j < 2^31 (page > 1)
   int tiles1, ns1, tiles2, ns2;
   int* status;
 };
@@ -32,6 +33,12 @@ struct PaItem {
 };
 
 struct PaRow { bool ok; int b, t, h, seen; long long grow; };
+
+HOA_DEVICE float pa_ex2(float x) {     // 2^x, results below 2^-126 flushed to 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 HOA_DEVICE void pa_fail(int* status) {
   if (status != nullptr) *reinterpret_cast<volatile int*>(status) = HOA_ERR_PAGES;
@@ -74,12 +81,11 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   const long long t1 = keys1 > 0 ? (rows1 + (pl.kind1 == kPaTc ? 255 : 15)) / (pl.kind1 == kPaTc ? 256 : 16) : 0;
   const long long t2 = keys2 > 0 ? (rows2 + (pl.kind2 == kPaTc ? 255 : 15)) / (pl.kind2 == kPaTc ? 256 : 16) : 0;
   const long long u1 = t1 * Hk, u2 = t2 * Hk * B;
-  // mma and simt items: a range of keys such that all of them make about two waves of 4 CTAs an SM
-  // (of the room that the rows have; the shorter ones split their own range as finely)
-  const long long all = (pl.kind1 != kPaTc ? u1 * keys1 : 0) + (pl.kind2 != kPaTc ? u2 * keys2 : 0);
-  long long range = all / (8ll * num_sms);
-  range = range < 128 ? 128 : range;
-  auto splits = [&](int kind, long long units, long long keys) -> int {
+  // mma and simt items take a range of keys each, the same for both parts: the shortest one with which all items run
+  // at once (4 CTAs an SM; of the room that the rows have - shorter rows split what they have as finely).  Measured at
+  // 65536 shared tokens and 8 rows: one wave 96 us, two 103, three 107; a range as short as 64 keys for small calls,
+  // where the time is one item's latency.
+  auto splits = [&](int kind, long long units, long long keys, long long range) -> long long {
     if (units == 0) return 0;
     long long ns;
     if (kind == kPaTc) {                           // one CTA an SM: split only what leaves SMs without one
@@ -89,12 +95,19 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
     } else {
       ns = (keys + range - 1) / range;
     }
-    return (int)(ns < 1 ? 1 : ns > 4096 ? 4096 : ns);
+    return ns < 1 ? 1 : ns > 4096 ? 4096 : ns;
   };
+  long long range = 64;
+  const long long longest = (pl.kind1 != kPaTc ? keys1 : 0) + (pl.kind2 != kPaTc ? keys2 : 0);
+  for (; range < longest; range += range / 8) {
+    const long long items = (pl.kind1 != kPaTc ? u1 * splits(pl.kind1, u1, keys1, range) : 0) +
+                            (pl.kind2 != kPaTc ? u2 * splits(pl.kind2, u2, keys2, range) : 0);
+    if (items <= 4ll * num_sms) break;
+  }
   pl.tiles1 = (int)t1;
   pl.tiles2 = (int)t2;
-  pl.ns1 = splits(pl.kind1, u1, keys1);
-  pl.ns2 = splits(pl.kind2, u2, keys2);
+  pl.ns1 = (int)splits(pl.kind1, u1, keys1, range);
+  pl.ns2 = (int)splits(pl.kind2, u2, keys2, range);
   return pl;
 }
 
@@ -154,9 +167,11 @@ HOA_DEVICE PaRow pa_row(const PaArgs& p, const PaItem& it, int r) {
   return w;
 }
 
+HOA_DEVICE int pa_page(const PaArgs& p, int j) { return p.page > 1 ? (int)(__umulhi((unsigned)j, p.page_mul) >> p.page_shift) : j; }
+
 // element offset of key j of the item's part in k_pages / v_pages, or -1 for a page outside the pool
 HOA_DEVICE long long pa_key(const PaArgs& p, const PaItem& it, int j) {
-  const int pg = j / p.page;
+  const int pg = pa_page(p, j);
   const int id = it.part == 1 ? p.shared[pg] : p.table[it.b * p.tstride + pg];
   if (id < 0 || id >= p.n_pages) {
     pa_fail(p.status);

@@ -9,9 +9,12 @@
 // the loop: warps meet once at the end, to join their (m, l, O).
 //
 // What bounds it is HBM: a key costs 4 d bytes (23.6 bytes an SM cycle at the
-// measured copy rate, so 16 keys of d = 96 take 260 SM cycles) against about 150
-// issue slots a chunk over four schedulers.  16 warps an SM with a chunk of 6 KB
-// each in flight keep 96 KB under way, twice what the latency needs.  The tensor
+// measured copy rate, so 16 keys of d = 96 take 260 SM cycles): 16 warps an SM with a
+// chunk of 6 KB each in flight keep 96 KB under way, twice what the latency needs -
+// as long as a warp's own chain through a chunk stays short.  So, where pages hold
+// whole chunks of adjacent tokens, a chunk's copies go to fixed offsets from one base;
+// masks are applied only where a chunk has keys that some row does not see; and up to
+// 8 query rows leave the lower half of the 16-row tile out of the softmax.  The tensor
 // cores' tcgen05 form (hoa_paged_attn_tc.cu) takes over where the rows of a head
 // fill more of its 128-row tile.
 #include "hoa_paged_attn.cuh"
@@ -32,7 +35,8 @@ struct PmCfg {
   static constexpr int kRing = kPmWarps * kWarp;
   static constexpr int kJoinRow = d + 4;                   // floats of a row of the join
   static constexpr int kJoin = kPmWarps * 16 * kJoinRow * 4;
-  static constexpr int kSmem = kRing > kJoin ? kRing : kJoin;
+  static constexpr int offRow = kRing > kJoin ? kRing : kJoin;   // per row: its place in the outputs, the warps' factors
+  static constexpr int kSmem = offRow + 16 * 8 + 16 * 4 * 4;
   static constexpr int kMinBlocks = D8 <= 12 ? 4 : 3;
 };
 
@@ -61,7 +65,8 @@ HOA_DEVICE uint32_t pm_pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <int D8>
+// kHalf: at most 8 rows an item.
+template <int D8, bool kHalf>
 __global__ void __launch_bounds__(kPmWarps * 32, PmCfg<D8>::kMinBlocks)
 paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   using C = PmCfg<D8>;
@@ -78,28 +83,54 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
     __syncwarp();
   }
 
-  // no key past the last one that a row of the item sees is read: its slot may hold anything
+  // no key past the last one that a row of the item sees is read: its slot may hold anything; keys before the last
+  // one that every row sees need no mask
+  // (lane l has row l % 16 of the item: where its q lies, and how many keys of the part it sees)
+  int all_see, my_seen;
+  long long my_q;
   {
     const PaRow row = pa_row(p, it, it.row0 + (lid & 15));
-    it.k1 = min(it.k1, __reduce_max_sync(0xffffffffu, row.ok ? row.seen - it.key_base : 0));
+    my_seen = row.ok ? row.seen - it.key_base : 0;
+    my_q = row.ok ? row.b * p.qsb + row.t * p.qst + row.h * p.qsh : -1;
+    it.k1 = min(it.k1, __reduce_max_sync(0xffffffffu, my_seen));
+    all_see = min(it.k1, __reduce_min_sync(0xffffffffu, row.ok ? my_seen : 0x7fffffff));
+    if (tid < 16) reinterpret_cast<long long*>(smem + C::offRow)[tid] = row.ok ? row.grow : -1;
   }
   const int chunks = it.k1 > it.k0 ? (it.k1 - it.k0 + kPmKeys - 1) / kPmKeys : 0;
-  // element offset of this lane's key (lanes 0-15) of a chunk, -1: none
-  auto key_of = [&](int c) -> long long {
-    const int j = it.k0 + c * kPmKeys + (lid & 15);
-    return c < chunks && j < it.k1 ? pa_key(p, it, j) : -1;
-  };
   const uint8_t* kp = reinterpret_cast<const uint8_t*>(p.kp);
   const uint8_t* vp = reinterpret_cast<const uint8_t*>(p.vp);
-  auto issue = [&](int stage, long long off) {
+  constexpr int NP = (kPmKeys * D8 + 31) / 32;          // 16-byte pieces of a lane
+  // whole chunks of adjacent tokens: one offset a chunk (pieces 16 bytes apart); else one a key, on lanes 0-15
+  const bool whole = p.page % kPmKeys == 0 && p.ts == C::d;
+  auto key_of = [&](int c) -> long long {
+    const int j = it.k0 + c * kPmKeys + (whole ? 0 : lid & 15);
+    return c < chunks && j < it.k1 ? pa_key(p, it, j) : -1;
+  };
+  auto issue = [&](int stage, long long off, int c) {
     const uint32_t base = ring + stage * C::kStage;
+    const int valid = it.k1 - it.k0 - c * kPmKeys;      // keys of the chunk that exist
+    if (whole && valid >= kPmKeys && off >= 0) {
+      const uint8_t* ks = kp + off * 2 + lid * 16;
+      const uint8_t* vs = vp + off * 2 + lid * 16;
 #pragma unroll
-    for (int i = 0; i < (kPmKeys * D8 + 31) / 32; ++i) {
+      for (int i = 0; i < NP; ++i) {
+        const int x = lid + 32 * i, key = x / D8, ch = x % D8;
+        if (kPmKeys * D8 % 32 == 0 || x < kPmKeys * D8) {
+          const uint32_t dst = base + key * C::kRow + ch * 16;
+          cp_async16(dst, ks + i * 512, 16);
+          cp_async16(dst + C::kTile, vs + i * 512, 16);
+        }
+      }
+      return;
+    }
+#pragma unroll 1
+    for (int i = 0; i < NP; ++i) {
       const int x = lid + 32 * i, key = x / D8, ch = x % D8;
-      const long long o = __shfl_sync(0xffffffffu, off, key & 15);
-      if (kPmKeys * D8 % 32 == 0 || x < kPmKeys * D8) {
-        const uint32_t n = o >= 0 ? 16u : 0u;           // 0: filled with zeros (a masked V row must not hold NaN)
-        const long long at = (o >= 0 ? o : 0) * 2 + ch * 16;
+      long long o = __shfl_sync(0xffffffffu, off, key & 15);
+      if (whole && o >= 0) o += key * C::d;
+      if (x < kPmKeys * D8) {
+        const uint32_t n = o >= 0 && key < valid ? 16u : 0u;   // 0: filled with zeros (a masked V row must not hold NaN)
+        const long long at = (n ? o : 0) * 2 + ch * 16;
         cp_async16(base + key * C::kRow + ch * 16, kp + at, n);
         cp_async16(base + C::kTile + key * C::kRow + ch * 16, vp + at, n);
       }
@@ -109,44 +140,46 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   long long off = key_of(w);
 #pragma unroll
   for (int s = 0; s < kPmStages; ++s) {
-    if (w + s * kPmWarps < chunks) issue(s, off);
+    if (w + s * kPmWarps < chunks) issue(s, off, w + s * kPmWarps);
     cp_commit();
     off = key_of(w + (s + 1) * kPmWarps);
   }
 
   // Q as A fragments: rows r0 and r0 + 8, columns 16 ks + q2 + {0, 1} and + 8
-  const PaRow ra = pa_row(p, it, it.row0 + r0), rb = pa_row(p, it, it.row0 + r0 + 8);
   uint32_t qf[C::KS][4];
   {
+    const long long oa = __shfl_sync(0xffffffffu, my_q, r0), ob = __shfl_sync(0xffffffffu, my_q, r0 + 8);
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q);
-    const __nv_bfloat16* qa = q + ra.b * p.qsb + ra.t * p.qst + ra.h * p.qsh;
-    const __nv_bfloat16* qb = q + rb.b * p.qsb + rb.t * p.qst + rb.h * p.qsh;
-    auto pair = [&](const __nv_bfloat16* r, bool ok, int c) -> uint32_t {
-      if (!ok || c >= C::d) return 0u;
-      const uint32_t lo = *reinterpret_cast<const uint16_t*>(r + c), hi = *reinterpret_cast<const uint16_t*>(r + c + 1);
-      return lo | hi << 16;
+    const bool even = ((reinterpret_cast<uintptr_t>(p.q) & 3) | ((p.qsb | p.qst | p.qsh) & 1)) == 0;   // rows 4-byte aligned
+    auto pair = [&](long long o, int c) -> uint32_t {
+      if (o < 0 || c >= C::d) return 0u;
+      const uint16_t* at = reinterpret_cast<const uint16_t*>(q + o + c);
+      if (even) return *reinterpret_cast<const uint32_t*>(at);
+      return at[0] | (uint32_t)at[1] << 16;
     };
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
-      qf[ks][0] = pair(qa, ra.ok, 16 * ks + q2);
-      qf[ks][1] = pair(qb, rb.ok, 16 * ks + q2);
-      qf[ks][2] = pair(qa, ra.ok, 16 * ks + q2 + 8);
-      qf[ks][3] = pair(qb, rb.ok, 16 * ks + q2 + 8);
+      qf[ks][0] = pair(oa, 16 * ks + q2);
+      qf[ks][1] = kHalf ? 0u : pair(ob, 16 * ks + q2);
+      qf[ks][2] = pair(oa, 16 * ks + q2 + 8);
+      qf[ks][3] = kHalf ? 0u : pair(ob, 16 * ks + q2 + 8);
     }
   }
-  const int seen_a = ra.ok ? ra.seen - it.key_base : 0, seen_b = rb.ok ? rb.seen - it.key_base : 0;
+  const int seen_a = __shfl_sync(0xffffffffu, my_seen, r0), seen_b = __shfl_sync(0xffffffffu, my_seen, r0 + 8);
+  constexpr int NE = kHalf ? 2 : 4;                     // accumulator elements of a tile in use: row r0 (, row r0 + 8)
 
   float o[D8][4];
 #pragma unroll
   for (int n = 0; n < D8; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   // matrix loads: lane l gives row l % 8 of matrix l / 8
   const uint32_t k_at = ((lid >> 4) * 8 + (lid & 7)) * C::kRow + ((lid >> 3) & 1) * 16;   // matrices: keys 0-7 (k, k+8), keys 8-15
   const uint32_t v_at = C::kTile + (((lid >> 3) & 1) * 8 + (lid & 7)) * C::kRow + (lid >> 4) * 16;
 
   int stage = 0;
+#pragma unroll 1
   for (int c = w; c < chunks; c += kPmWarps) {
     cp_wait<kPmStages - 1>();
     __syncwarp();
@@ -159,48 +192,55 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
       mma_16816(s[0], qf[ks], b[0], b[1]);
       mma_16816(s[1], qf[ks], b[2], b[3]);
     }
-    const int j0 = it.k0 + c * kPmKeys + q2;
-    const int na = min(seen_a, it.k1) - j0, nb = min(seen_b, it.k1) - j0;   // keys of the chunk from q2 on that the rows see
-    float xa = -INFINITY, xb = -INFINITY;
+    const int j0 = it.k0 + c * kPmKeys;
+    float x[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int j = 8 * n + e;
-        s[n][e] = j < na ? s[n][e] * p.scale_log2 : -INFINITY;
-        s[n][2 + e] = j < nb ? s[n][2 + e] * p.scale_log2 : -INFINITY;
-        xa = fmaxf(xa, s[n][e]);
-        xb = fmaxf(xb, s[n][2 + e]);
-      }
+      for (int e = 0; e < NE; ++e) s[n][e] *= p.scale_log2;
+    if (j0 + kPmKeys > all_see) {
+      const int na = min(seen_a, it.k1) - j0 - q2, nb = min(seen_b, it.k1) - j0 - q2;   // keys from q2 on that the rows see
 #pragma unroll
-    for (int x = 1; x < 4; x <<= 1) {
-      xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, x));
-      xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, x));
-    }
-    if (__any_sync(0xffffffffu, xa > ma || xb > mb)) {
-      const float na2 = fmaxf(ma, xa), nb2 = fmaxf(mb, xb);
-      const float ca = na2 == -INFINITY ? 1.f : exp2f(ma - na2), cb = nb2 == -INFINITY ? 1.f : exp2f(mb - nb2);
-      ma = na2;
-      mb = nb2;
-      la *= ca;
-      lb *= cb;
+      for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int n = 0; n < D8; ++n) {
-        o[n][0] *= ca; o[n][1] *= ca; o[n][2] *= cb; o[n][3] *= cb;
-      }
+        for (int e = 0; e < NE; ++e)
+          if (8 * n + (e & 1) >= (e < 2 ? na : nb)) s[n][e] = -INFINITY;
     }
-    const float fa = ma == -INFINITY ? 0.f : ma, fb = mb == -INFINITY ? 0.f : mb;   // no key seen yet: weights 0
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[n][e] = exp2f(s[n][e] - fa);
-        s[n][2 + e] = exp2f(s[n][2 + e] - fb);
-        la += s[n][e];
-        lb += s[n][2 + e];
+      for (int e = 0; e < NE; ++e) x[e >> 1] = fmaxf(x[e >> 1], s[n][e]);
+#pragma unroll
+    for (int k = 1; k < 4; k <<= 1)
+#pragma unroll
+      for (int h = 0; h < NE / 2; ++h) x[h] = fmaxf(x[h], __shfl_xor_sync(0xffffffffu, x[h], k));
+    if (__any_sync(0xffffffffu, x[0] > m[0] || (!kHalf && x[1] > m[1]))) {
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < NE / 2; ++h) {
+        const float mn = fmaxf(m[h], x[h]);
+        f[h] = mn == -INFINITY ? 1.f : exp2f(m[h] - mn);
+        m[h] = mn;
+        l[h] *= f[h];
+      }
+#pragma unroll
+      for (int n = 0; n < D8; ++n)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[n][e] *= f[e >> 1];
+    }
+    float ref[2];
+#pragma unroll
+    for (int h = 0; h < NE / 2; ++h) ref[h] = m[h] == -INFINITY ? 0.f : m[h];   // no key seen yet: weights 0
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        s[n][e] = pa_ex2(s[n][e] - ref[e >> 1]);
+        l[e >> 1] += s[n][e];
       }
     // the weights are rounded to bf16 for the product only (2^-9 relative, as the output's own rounding); l sums them unrounded
-    const uint32_t pf[4] = {pm_pack(s[0][0], s[0][1]), pm_pack(s[0][2], s[0][3]), pm_pack(s[1][0], s[1][1]), pm_pack(s[1][2], s[1][3])};
+    const uint32_t pf[4] = {pm_pack(s[0][0], s[0][1]), kHalf ? 0u : pm_pack(s[0][2], s[0][3]), pm_pack(s[1][0], s[1][1]),
+                            kHalf ? 0u : pm_pack(s[1][2], s[1][3])};
 #pragma unroll
     for (int n = 0; n < C::KS; ++n) {
       uint32_t b[4];
@@ -209,16 +249,15 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
       if (2 * n + 1 < D8) mma_16816(o[2 * n + 1 < D8 ? 2 * n + 1 : 0], pf, b[2], b[3]);
     }
     __syncwarp();                                       // all lanes have read the stage
-    if (c + kPmStages * kPmWarps < chunks) issue(stage, off);
+    if (c + kPmStages * kPmWarps < chunks) issue(stage, off, c + kPmStages * kPmWarps);
     cp_commit();
     off = key_of(c + (kPmStages + 1) * kPmWarps);
     stage ^= 1;
   }
 #pragma unroll
-  for (int x = 1; x < 4; x <<= 1) {
-    la += __shfl_xor_sync(0xffffffffu, la, x);
-    lb += __shfl_xor_sync(0xffffffffu, lb, x);
-  }
+  for (int k = 1; k < 4; k <<= 1)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], k);
 
   // ---- join the warps
   pa_end_after_previous();
@@ -229,8 +268,8 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
     float* a = jn + (w * 16 + r0) * C::kJoinRow;
     float* b = a + 8 * C::kJoinRow;
     if (q2 == 0) {
-      a[C::d] = ma; a[C::d + 1] = la;
-      b[C::d] = mb; b[C::d + 1] = lb;
+      a[C::d] = m[0]; a[C::d + 1] = l[0];
+      b[C::d] = m[1]; b[C::d + 1] = l[1];
     }
 #pragma unroll
     for (int n = 0; n < D8; ++n) {
@@ -239,35 +278,51 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < 16 * C::d; i += kPmWarps * 32) {
-    const int r = i / C::d, c = i % C::d;
-    const PaRow row = pa_row(p, it, it.row0 + r);
-    if (!row.ok) break;                                 // rows are in order: none after this one either
-    float m = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < kPmWarps; ++x) m = fmaxf(m, jn[(x * 16 + r) * C::kJoinRow + C::d]);
-    float l = 0.f, y = 0.f;
-    if (m != -INFINITY) {
-#pragma unroll
-      for (int x = 0; x < kPmWarps; ++x) {
-        const float* a = jn + (x * 16 + r) * C::kJoinRow;
-        const float f = exp2f(a[C::d] - m);
-        l = fmaf(f, a[C::d + 1], l);
-        y = fmaf(f, a[c], y);
-      }
-    }
-    const long long part = (long long)it.slot * p.rows + row.grow;
-    if (c == 0) p.part_ml[part] = make_float2(m, l);
-    if (l > 0.f) p.part_o[part * C::d + c] = y;
+  const long long* s_row = reinterpret_cast<const long long*>(smem + C::offRow);
+  float4* s_f = reinterpret_cast<float4*>(smem + C::offRow + 16 * 8);   // the warps' factors of a row
+  constexpr int NR = kHalf ? 8 : 16;
+  if (tid < NR && s_row[tid] >= 0) {
+    const float* a = jn + tid * C::kJoinRow + C::d;
+    constexpr int ws = 16 * C::kJoinRow;
+    const float m0 = a[0], m1 = a[ws], m2 = a[2 * ws], m3 = a[3 * ws];
+    const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)), ref = mx == -INFINITY ? 0.f : mx;
+    const float4 f = make_float4(pa_ex2(m0 - ref), pa_ex2(m1 - ref), pa_ex2(m2 - ref), pa_ex2(m3 - ref));
+    s_f[tid] = f;
+    const float sum = fmaf(f.x, a[1], fmaf(f.y, a[ws + 1], fmaf(f.z, a[2 * ws + 1], f.w * a[3 * ws + 1])));
+    p.part_ml[(long long)it.slot * p.rows + s_row[tid]] = make_float2(mx, sum);
   }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < NR * (C::d / 4); i += kPmWarps * 32) {
+    const int r = i / (C::d / 4), c = (i % (C::d / 4)) * 4;
+    const long long row = s_row[r];
+    if (row < 0) break;                                 // rows are in order: none after this one either
+    const float4 f = s_f[r];
+    const float ff[4] = {f.x, f.y, f.z, f.w};
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < kPmWarps; ++x) {
+      const float4 v = *reinterpret_cast<const float4*>(jn + (x * 16 + r) * C::kJoinRow + c);
+      y.x = fmaf(ff[x], v.x, y.x); y.y = fmaf(ff[x], v.y, y.y); y.z = fmaf(ff[x], v.z, y.z); y.w = fmaf(ff[x], v.w, y.w);
+    }
+    *reinterpret_cast<float4*>(p.part_o + ((long long)it.slot * p.rows + row) * C::d + c) = y;
+  }
+}
+
+template <int D8, bool kHalf>
+static int launch_mma_h(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+  using C = PmCfg<D8>;
+  if (cudaFuncSetAttribute(paged_attn_mma_kernel<D8, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+    return HOA_ERR_LAUNCH;
+  return pa_launch(paged_attn_mma_kernel<D8, kHalf>, items, kPmWarps * 32, C::kSmem, s, early, a, first);
 }
 
 template <int D8>
 static int launch_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
-  using C = PmCfg<D8>;
-  if (cudaFuncSetAttribute(paged_attn_mma_kernel<D8>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
-  return pa_launch(paged_attn_mma_kernel<D8>, items, kPmWarps * 32, C::kSmem, s, early, a, first);
+  // the rows of an item: of the whole batch where the launch has items of part 1
+  const bool part1 = first < (unsigned)a.tiles1 * a.Hk * a.ns1;
+  const long long rows = (part1 ? a.B : 1) * (long long)a.Tq * a.G;
+  return rows <= 8 ? launch_mma_h<D8, true>(a, first, items, early, s) : launch_mma_h<D8, false>(a, first, items, early, s);
 }
 
 int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {

@@ -50,12 +50,6 @@ HOA_DEVICE void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, in
       : "memory");
 }
 
-HOA_DEVICE float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 HOA_DEVICE uint32_t pt_pack(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -293,7 +287,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
         const float m_cand = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;   // (c > 0)
         const bool move = m_cand > m_ref + (float)kPtRescaleLog2;    // also the first key seen (m_ref = -inf)
         const float m_new = move ? m_cand : m_ref;
-        const float corr = move ? ex2(m_ref - m_new) : 1.f;          // 0 at the first key seen
+        const float corr = move ? pa_ex2(m_ref - m_new) : 1.f;          // 0 at the first key seen
         if (__any_sync(0xffffffffu, move) && j > 0) {
           // rescale this warp's rows of O once the previous P V has completed
           bad |= !mbar_wait_abortable(&pv_done[i], (j - 1) & 1, s_abort, pt.max_wait);
@@ -318,8 +312,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
           float pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = ex2(fmaf(sv[h][2 * e], c, -ref));
-            const float p1 = ex2(fmaf(sv[h][2 * e + 1], c, -ref));
+            const float p0 = pa_ex2(fmaf(sv[h][2 * e], c, -ref));
+            const float p1 = pa_ex2(fmaf(sv[h][2 * e + 1], c, -ref));
             ps[(2 * e) & 7] += p0;
             ps[(2 * e + 1) & 7] += p1;
             // the weights are rounded to bf16 for the product only; l sums them unrounded
