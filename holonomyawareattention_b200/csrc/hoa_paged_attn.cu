@@ -18,94 +18,200 @@
 namespace hoa {
 
 // ---------------------------------------------------------------------------
-// any head dim and alignment, fp32 products on the CUDA cores
+// any head dim, type and alignment, fp32 products on the CUDA cores
 // ---------------------------------------------------------------------------
-constexpr int kPsRows = 16, kPsKeys = 64, kPsThreads = 128;
+// RT = 8 R query rows against 64 keys at a time; 128 threads as 8 x 16: thread (ty, tx) has rows
+// ty R .. + R - 1 and keys tx + 16 j of the scores, columns 4 tx + 64 k of the output.  Rows of K and V
+// are padded to an odd number of 16-byte chunks, so that the 16 keys of a warp's read fall on different
+// banks.  Few rows (R = 2) are bound by the loads, 8 d bytes a key; many (R = 4) by the FMAs, 4 d a key
+// and row: 32 rows halve the shared-memory reads an FMA needs.
+constexpr int kPsKeys = 64, kPsThreads = 128;
 
+HOA_DEVICE int ps_ld(int d) { return ((d + 3) / 4 | 1) * 4; }    // floats of a padded row
+
+// V4: fp32 with d % 4 == 0 and 16-byte aligned rows
+template <int R, bool V4>
 __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __grid_constant__ PaArgs p, unsigned first) {
+  constexpr int RT = 8 * R;
   extern __shared__ float sm[];
   pa_let_next_start();
-  const int d = p.d, ld = d | 1;                       // odd row stride: rows fall on different banks
-  float* Qs = sm;                                      // [16][ld]
-  float* Ks = Qs + kPsRows * ld;                       // [64][ld]
+  const int d = p.d, ld = ps_ld(d), d4 = (d + 3) / 4;
+  float* Qs = sm;                                      // [RT][ld]
+  float* Ks = Qs + RT * ld;                            // [64][ld]
   float* Vs = Ks + kPsKeys * ld;                       // [64][ld]
-  float* Ps = Vs + kPsKeys * ld;                       // [16][64]
-  PaItem it = pa_item(p, first + blockIdx.x, kPsRows, kPsKeys);
-  const int tid = threadIdx.x, row = tid >> 3, kg = tid & 7;
-  const PaRow my = pa_row(p, it, it.row0 + row);
-  for (int i = tid; i < kPsRows * d; i += kPsThreads) {
-    const int r = i / d, c = i % d;
-    const PaRow q = pa_row(p, it, it.row0 + r);
-    Qs[r * ld + c] = q.ok ? load_elem(p.q, q.b * p.qsb + q.t * p.qst + q.h * p.qsh + c, p.dtype) : 0.f;
+  float* Ps = Vs + kPsKeys * ld;                       // [RT][68] weights
+  __shared__ int s_top;
+  __shared__ long long s_key[kPsKeys];
+  PaItem it = pa_item(p, first + blockIdx.x, RT, kPsKeys);
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15, warp = tid >> 5, lid = tid & 31;
+  PaRow my[R];
+  int seen[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    my[i] = pa_row(p, it, it.row0 + ty * R + i);
+    seen[i] = my[i].ok ? min(my[i].seen - it.key_base, it.k1) : 0;   // keys of this part that the row sees
   }
-  const int seen = my.ok ? min(my.seen - it.key_base, it.k1) : 0;   // keys of this part that the row sees
-  __shared__ int s_top;                                // no key past the last one that a row sees is read
   if (tid == 0) s_top = 0;
   __syncthreads();
-  if (kg == 0) atomicMax(&s_top, seen);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (tx == 0) atomicMax(&s_top, seen[i]);
+#pragma unroll
+  for (int i = 0; i < R; ++i)                          // the 16 threads of a row read it
+    for (int c = tx; c < ld; c += 16)
+      Qs[(ty * R + i) * ld + c] =
+          my[i].ok && c < d ? load_elem(p.q, my[i].b * p.qsb + my[i].t * p.qst + my[i].h * p.qsh + c, p.dtype) : 0.f;
   __syncthreads();
-  it.k1 = min(it.k1, s_top);
-  float o[16], m = -INFINITY, l = 0.f;
+  it.k1 = min(it.k1, s_top);                           // no key past the last one that a row sees is read
+  float4 o[R][2];
+  float m[R], l[R];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+  for (int i = 0; i < R; ++i) {
+    o[i][0] = o[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
   for (int k0 = it.k0; k0 < it.k1; k0 += kPsKeys) {
+    __syncthreads();                                   // the last tile has been read
+    if (tid < kPsKeys) s_key[tid] = k0 + tid < it.k1 ? pa_key(p, it, k0 + tid) : -1;
     __syncthreads();
-    for (int i = tid; i < kPsKeys * d; i += kPsThreads) {
-      const int j = i / d, c = i % d;
-      const long long at = k0 + j < it.k1 ? pa_key(p, it, k0 + j) : -1;
-      Ks[j * ld + c] = at >= 0 ? load_elem(p.kp, at + c, p.dtype) : 0.f;
-      Vs[j * ld + c] = at >= 0 ? load_elem(p.vp, at + c, p.dtype) : 0.f;
+    if (V4) {
+#pragma unroll 8
+      for (int j = warp; j < kPsKeys; j += 4) {        // a warp a key, a lane 16 bytes of it
+        const long long at = s_key[j];
+        float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+        if (lid < d4) {
+          if (at >= 0) {
+            k = *reinterpret_cast<const float4*>(static_cast<const float*>(p.kp) + at + 4 * lid);
+            v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.vp) + at + 4 * lid);
+          }
+          *reinterpret_cast<float4*>(Ks + j * ld + 4 * lid) = k;
+          *reinterpret_cast<float4*>(Vs + j * ld + 4 * lid) = v;
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int j = warp; j < kPsKeys; j += 4) {
+        const long long at = s_key[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = lid + 32 * e;
+          if (c < 4 * d4) {
+            const bool in = at >= 0 && c < d;
+            Ks[j * ld + c] = in ? load_elem(p.kp, at + c, p.dtype) : 0.f;
+            Vs[j * ld + c] = in ? load_elem(p.vp, at + c, p.dtype) : 0.f;
+          }
+        }
+      }
     }
     __syncthreads();
-    float s[8];
+    float s[R][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = 0.f;
-    for (int c = 0; c < d; ++c) {
-      const float qv = Qs[row * ld + c];
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = fmaf(qv, Ks[(kg + 8 * j) * ld + c], s[j]);
-    }
-    float mx = -INFINITY;
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 2
+    for (int c = 0; c < d4; ++c) {
+      float4 q[R], k[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[j] = k0 + kg + 8 * j < seen ? s[j] * p.scale_log2 : -INFINITY;
-      mx = fmaxf(mx, s[j]);
-    }
+      for (int i = 0; i < R; ++i) q[i] = *reinterpret_cast<const float4*>(Qs + (ty * R + i) * ld + 4 * c);
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float mn = fmaxf(m, mx);
-    const float ref = mn == -INFINITY ? 0.f : mn;      // a row that has seen no key yet
-    const float corr = exp2f(m - ref);
-    float ps = 0.f;
+      for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(Ks + (tx + 16 * j) * ld + 4 * c);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e = exp2f(s[j] - ref);
-      Ps[row * kPsKeys + kg + 8 * j] = e;
-      ps += e;
+      for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[i][j] = fmaf(q[i].x, k[j].x, fmaf(q[i].y, k[j].y, fmaf(q[i].z, k[j].z, fmaf(q[i].w, k[j].w, s[i][j]))));
     }
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) ps += __shfl_xor_sync(0xffffffffu, ps, x);
-    l = l * corr + ps;
-    m = mn;
+    for (int i = 0; i < R; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = k0 + tx + 16 * j < seen[i] ? s[i][j] * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 1; x < 16; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float mn = fmaxf(m[i], mx), ref = mn == -INFINITY ? 0.f : mn;   // (a row that has seen no key yet)
+      const float corr = exp2f(m[i] - ref);
+      m[i] = mn;
+      float ps = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(s[i][j] - ref);
+        Ps[(ty * R + i) * 68 + tx + 16 * j] = e;
+        ps += e;
+      }
+      l[i] = l[i] * corr + ps;                         // this thread's keys only; joined at the end
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        o[i][k].x *= corr; o[i][k].y *= corr; o[i][k].z *= corr; o[i][k].w *= corr;
+      }
+    }
     __syncwarp();                                      // a row's weights come from its own warp
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] *= corr;
-    for (int k = 0; k < kPsKeys; ++k) {
-      const float e = Ps[row * kPsKeys + k];
+    for (int g = 0; g < 2; ++g) {
+      if (4 * tx + 64 * g >= d) break;
+#pragma unroll 4
+      for (int k = 0; k < kPsKeys; k += 4) {
+        float4 w[R];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (kg + 8 * i < d) o[i] = fmaf(e, Vs[k * ld + kg + 8 * i], o[i]);
+        for (int i = 0; i < R; ++i) w[i] = *reinterpret_cast<const float4*>(Ps + (ty * R + i) * 68 + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 v = *reinterpret_cast<const float4*>(Vs + (k + e) * ld + 4 * tx + 64 * g);
+#pragma unroll
+          for (int i = 0; i < R; ++i) {
+            const float f = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+            o[i][g].x = fmaf(f, v.x, o[i][g].x); o[i][g].y = fmaf(f, v.y, o[i][g].y);
+            o[i][g].z = fmaf(f, v.z, o[i][g].z); o[i][g].w = fmaf(f, v.w, o[i][g].w);
+          }
+        }
+      }
     }
   }
-  pa_end_after_previous();
-  if (!my.ok) return;
-  const long long part = (long long)it.slot * p.rows + my.grow;
-  if (kg == 0) p.part_ml[part] = make_float2(m, l);
-  if (l > 0.f) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (kg + 8 * i < d) p.part_o[part * d + kg + 8 * i] = o[i];
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+  pa_end_after_previous();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (!my[i].ok) continue;
+    const long long part = (long long)it.slot * p.rows + my[i].grow;
+    if (tx == 0) p.part_ml[part] = make_float2(m[i], l[i]);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int c = 4 * tx + 64 * g;
+      float* at = p.part_o + part * d + c;
+      const float v[4] = {o[i][g].x, o[i][g].y, o[i][g].z, o[i][g].w};
+      if (V4) {
+        if (c < d) *reinterpret_cast<float4*>(at) = o[i][g];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < d) at[e] = v[e];
+      }
+    }
   }
+}
+
+template <int R, bool V4>
+static int launch_simt(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+  const int ld = ((a.d + 3) / 4 | 1) * 4;
+  const size_t smem = ((8 * R + 2 * kPsKeys) * (size_t)ld + 8 * R * 68) * sizeof(float);
+  if (cudaFuncSetAttribute(paged_attn_simt_kernel<R, V4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return HOA_ERR_LAUNCH;
+  return pa_launch(paged_attn_simt_kernel<R, V4>, items, kPsThreads, smem, s, early, a, first);
+}
+
+static int paged_attn_simt(const PaArgs& a, int tile_rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
+  const bool v4 = a.dtype == HOA_F32 && a.d % 4 == 0 &&
+                  ((reinterpret_cast<uintptr_t>(a.kp) | reinterpret_cast<uintptr_t>(a.vp) | (uintptr_t)(a.ps * 4) |
+                    (uintptr_t)(a.hs * 4) | (uintptr_t)(a.ts * 4)) & 15) == 0;
+  if (tile_rows == 32) return v4 ? launch_simt<4, true>(a, first, items, early, s) : launch_simt<4, false>(a, first, items, early, s);
+  return v4 ? launch_simt<2, true>(a, first, items, early, s) : launch_simt<2, false>(a, first, items, early, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -287,10 +393,7 @@ static int run_items(int kind, const PaArgs& a, long long first, long long items
   if (items == 0) return HOA_OK;
   if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, early, s);
   if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, early, s);
-  const size_t smem = ((kPsRows + 2 * kPsKeys) * (size_t)(a.d | 1) + kPsRows * kPsKeys) * sizeof(float);
-  if (cudaFuncSetAttribute(paged_attn_simt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
-  return pa_launch(paged_attn_simt_kernel, (unsigned)items, kPsThreads, smem, s, early, a, (unsigned)first);
+  return paged_attn_simt(a, kind == kPaSimt32 ? 32 : 16, (unsigned)first, (unsigned)items, early, s);
 }
 
 extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -300,6 +403,7 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
                                   int d, int page, int n_pages, int num_sms, void* workspace, size_t workspace_bytes,
                                   int* status, void* stream) {
   if (!q || !q_strides || !k_pages || !v_pages || !page_strides || !lens || !out || !lse || !workspace ||
+      (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
       !pa_shape_ok(B, Tq, H, Hk, d, page, n_shared, W, num_sms) || n_pages < 1 || (n_shared > 0 && !shared) ||
       (W > 0 && !table) || (paths && Tq != 1))
     return HOA_ERR_INVALID_ARG;

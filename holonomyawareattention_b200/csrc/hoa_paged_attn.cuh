@@ -59,10 +59,11 @@ inline int pa_tile_keys(int page) {
 }
 
 // Which kernel takes a part.
-//   simt: fp32, head dims or strides that the copies do not take; 16 rows a tile.
+//   simt: fp32, head dims or strides that the copies do not take; 16 rows a tile, 32 where there are more.
 //   mma:  bf16, 16 rows a tile, any page size.
 //   tc:   bf16, 256 rows a tile, pages that tile (pa_tile_keys).
-enum PaKind { kPaSimt = 0, kPaMma = 1, kPaTc = 2 };
+enum PaKind { kPaSimt = 0, kPaSimt32 = 1, kPaMma = 2, kPaTc = 3 };
+inline int pa_tile_rows(int kind) { return kind == kPaTc ? 256 : kind == kPaSimt32 ? 32 : 16; }
 
 // Rows of a head from which tcgen05 takes a part: up to 16 one mma item reads the keys once.
 constexpr int kPaTcRows = 17;
@@ -76,10 +77,13 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   const long long rows1 = B * (long long)Tq * G, rows2 = Tq * G;
   const int kt = pa_tile_keys(page);
   tc = tc && kt > 0;
-  pl.kind1 = tc && rows1 >= kPaTcRows ? kPaTc : tensor ? kPaMma : kPaSimt;
-  pl.kind2 = tc && rows2 >= kPaTcRows ? kPaTc : tensor ? kPaMma : kPaSimt;
-  const long long t1 = keys1 > 0 ? (rows1 + (pl.kind1 == kPaTc ? 255 : 15)) / (pl.kind1 == kPaTc ? 256 : 16) : 0;
-  const long long t2 = keys2 > 0 ? (rows2 + (pl.kind2 == kPaTc ? 255 : 15)) / (pl.kind2 == kPaTc ? 256 : 16) : 0;
+  auto kind_of = [&](long long rows) -> int {
+    return tc && rows >= kPaTcRows ? kPaTc : tensor ? kPaMma : rows > 16 ? kPaSimt32 : kPaSimt;
+  };
+  pl.kind1 = kind_of(rows1);
+  pl.kind2 = kind_of(rows2);
+  const long long r1 = pa_tile_rows(pl.kind1), r2 = pa_tile_rows(pl.kind2);
+  const long long t1 = keys1 > 0 ? (rows1 + r1 - 1) / r1 : 0, t2 = keys2 > 0 ? (rows2 + r2 - 1) / r2 : 0;
   const long long u1 = t1 * Hk, u2 = t2 * Hk * B;
   // mma and simt items take a range of keys each, the same for both parts: the shortest one with which all items run
   // at once (4 CTAs an SM; of the room that the rows have - shorter rows split what they have as finely).  Measured at
