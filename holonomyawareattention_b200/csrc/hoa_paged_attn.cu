@@ -215,6 +215,147 @@ static int paged_attn_simt(const PaArgs& a, int tile_rows, unsigned first, unsig
 }
 
 // ---------------------------------------------------------------------------
+// fp32, up to 4 query rows: bound by the loads alone
+// ---------------------------------------------------------------------------
+// Eight lanes share a key (CH chunks of 4 columns each), a warp has four keys at a time and takes two
+// such steps an iteration, straight from global memory to registers.  Every group of eight lanes keeps
+// its own (m, l, O): a step needs three shuffles a row and no barrier; groups and warps join at the end.
+constexpr int kPvThreads = 128;
+
+template <int CH, int NR>
+__global__ void __launch_bounds__(kPvThreads) paged_attn_vec_kernel(const __grid_constant__ PaArgs p, unsigned first) {
+  __shared__ float s_o[4][NR][32 * CH];
+  __shared__ float2 s_ml[4][NR];
+  pa_let_next_start();
+  const PaItem it = pa_item(p, first + blockIdx.x, NR, 16);
+  const int warp = threadIdx.x >> 5, lid = threadIdx.x & 31, gl = lid & 7, g = lid >> 3, d = p.d;
+  const float* q = static_cast<const float*>(p.q);
+  float4 qv[NR][CH], o[NR][CH];
+  float m[NR], l[NR];
+  int seen[NR], top = 0;
+  long long grow[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const PaRow row = pa_row(p, it, it.row0 + r);
+    const float* at = q + row.b * p.qsb + row.t * p.qst + row.h * p.qsh;
+    seen[r] = row.ok ? min(row.seen - it.key_base, it.k1) : 0;
+    top = max(top, seen[r]);
+    grow[r] = row.ok ? row.grow : -1;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int c = 4 * (gl + 8 * i);
+      o[r][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      qv[r][i] = o[r][i];
+      if (row.ok && c < d)
+        qv[r][i] = make_float4(at[c] * p.scale_log2, at[c + 1] * p.scale_log2, at[c + 2] * p.scale_log2, at[c + 3] * p.scale_log2);
+    }
+  }
+  const int k1 = min(it.k1, top);                      // no key past the last one that a row sees is read
+  for (int k0 = it.k0 + warp * 8; k0 < k1; k0 += 32) {
+    float4 k[2][CH], v[2][CH];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = k0 + 4 * u + g;
+      const long long at = j < k1 ? pa_key(p, it, j) : -1;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int c = 4 * (gl + 8 * i);
+        k[u][i] = v[u][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (at >= 0 && c < d) {
+          k[u][i] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.kp) + at + c);
+          v[u][i] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.vp) + at + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+          s[u] = fmaf(qv[r][i].x, k[u][i].x, fmaf(qv[r][i].y, k[u][i].y, fmaf(qv[r][i].z, k[u][i].z, fmaf(qv[r][i].w, k[u][i].w, s[u]))));
+      }
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], x);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[u] = k0 + 4 * u + g < seen[r] ? s[u] : -INFINITY;
+      const float mn = fmaxf(m[r], fmaxf(s[0], s[1])), ref = mn == -INFINITY ? 0.f : mn;   // (no key seen yet: weights 0)
+      const float f = pa_ex2(m[r] - ref), p0 = pa_ex2(s[0] - ref), p1 = pa_ex2(s[1] - ref);
+      m[r] = mn;
+      l[r] = fmaf(l[r], f, p0 + p1);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        o[r][i].x = fmaf(p1, v[1][i].x, fmaf(p0, v[0][i].x, o[r][i].x * f));
+        o[r][i].y = fmaf(p1, v[1][i].y, fmaf(p0, v[0][i].y, o[r][i].y * f));
+        o[r][i].z = fmaf(p1, v[1][i].z, fmaf(p0, v[0][i].z, o[r][i].z * f));
+        o[r][i].w = fmaf(p1, v[1][i].w, fmaf(p0, v[0][i].w, o[r][i].w * f));
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    float mx = m[r];
+#pragma unroll
+    for (int x = 8; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    const float f = pa_ex2(m[r] - (mx == -INFINITY ? 0.f : mx));
+    l[r] *= f;
+#pragma unroll
+    for (int x = 8; x < 32; x <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], x);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      float4 y = make_float4(o[r][i].x * f, o[r][i].y * f, o[r][i].z * f, o[r][i].w * f);
+#pragma unroll
+      for (int x = 8; x < 32; x <<= 1) {
+        y.x += __shfl_xor_sync(0xffffffffu, y.x, x); y.y += __shfl_xor_sync(0xffffffffu, y.y, x);
+        y.z += __shfl_xor_sync(0xffffffffu, y.z, x); y.w += __shfl_xor_sync(0xffffffffu, y.w, x);
+      }
+      if (g == 0) *reinterpret_cast<float4*>(&s_o[warp][r][4 * (gl + 8 * i)]) = y;
+    }
+    if (lid == 0) s_ml[warp][r] = make_float2(mx, l[r]);
+  }
+  pa_end_after_previous();
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    if (grow[r] < 0) continue;
+    float mx = -INFINITY, sum = 0.f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, s_ml[w][r].x);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = pa_ex2(s_ml[w][r].x - (mx == -INFINITY ? 0.f : mx));
+      sum = fmaf(f[w], s_ml[w][r].y, sum);
+    }
+    const long long part = (long long)it.slot * p.rows + grow[r];
+    const int c = threadIdx.x;
+    if (c == 0) p.part_ml[part] = make_float2(mx, sum);
+    if (c < d) p.part_o[part * d + c] = fmaf(f[0], s_o[0][r][c], fmaf(f[1], s_o[1][r][c], fmaf(f[2], s_o[2][r][c], f[3] * s_o[3][r][c])));
+  }
+}
+
+template <int CH>
+static int launch_vec(const PaArgs& a, int rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
+  if (rows == 1) return pa_launch(paged_attn_vec_kernel<CH, 1>, items, kPvThreads, 0, s, early, a, first);
+  if (rows == 2) return pa_launch(paged_attn_vec_kernel<CH, 2>, items, kPvThreads, 0, s, early, a, first);
+  return pa_launch(paged_attn_vec_kernel<CH, 4>, items, kPvThreads, 0, s, early, a, first);
+}
+
+static int paged_attn_vec(const PaArgs& a, int rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
+  switch ((a.d + 31) / 32) {
+    case 1: return launch_vec<1>(a, rows, first, items, early, s);
+    case 2: return launch_vec<2>(a, rows, first, items, early, s);
+    case 3: return launch_vec<3>(a, rows, first, items, early, s);
+    default: return launch_vec<4>(a, rows, first, items, early, s);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // join the parts of each (row, query, head); optionally out = P o
 // ---------------------------------------------------------------------------
 // kWpr warps share an output row: one where rows are many, eight (a CTA a row) where
@@ -381,8 +522,8 @@ extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, i
                                                  int num_sms) {
   if (!pa_shape_ok(B, Tq, H, Hk, d, page, n_shared, W, num_sms)) return 0;
   size_t most = 0;                                 // enough for whichever kernels take the call
-  for (int k = 0; k < 3; ++k) {
-    const size_t n = pa_bytes(pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, k > 0, k > 1), B, Tq, H, d);
+  for (int k = 0; k < 4; ++k) {
+    const size_t n = pa_bytes(pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, k == 1, k > 1, k > 2), B, Tq, H, d);
     most = n > most ? n : most;
   }
   return most;
@@ -393,7 +534,8 @@ static int run_items(int kind, const PaArgs& a, long long first, long long items
   if (items == 0) return HOA_OK;
   if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, early, s);
   if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, early, s);
-  return paged_attn_simt(a, kind == kPaSimt32 ? 32 : 16, (unsigned)first, (unsigned)items, early, s);
+  if (kind < kPaSimt) return paged_attn_vec(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, early, s);
+  return paged_attn_simt(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, early, s);
 }
 
 extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -411,10 +553,13 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
     return HOA_ERR_UNSUPPORTED;
   // key positions and item numbers are ints
   if ((long long)(n_shared + (long long)W) * page > 0x7fff0000ll) return HOA_ERR_UNSUPPORTED;
+  const int e = dtype == HOA_BF16 ? 2 : 4;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
-                         (uintptr_t)(page_strides[0] * 2) | (uintptr_t)(page_strides[1] * 2) | (uintptr_t)(page_strides[2] * 2);
-  const bool tensor = dtype == HOA_BF16 && d % 8 == 0 && (bits & 15) == 0;
-  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, tensor, tensor && softmax_scale > 0.f);
+                         (uintptr_t)(page_strides[0] * e) | (uintptr_t)(page_strides[1] * e) | (uintptr_t)(page_strides[2] * e);
+  const bool rows16 = (bits & 15) == 0;              // every token's row is 16-byte aligned
+  const bool tensor = dtype == HOA_BF16 && d % 8 == 0 && rows16;
+  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, dtype == HOA_F32 && d % 4 == 0 && rows16, tensor,
+                            tensor && softmax_scale > 0.f);
   if (workspace_bytes < pa_bytes(pl, B, Tq, H, d)) return HOA_ERR_WORKSPACE;
   const long long items1 = (long long)pl.tiles1 * Hk * pl.ns1, items2 = (long long)B * Hk * pl.tiles2 * pl.ns2;
   if (items1 + items2 > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;

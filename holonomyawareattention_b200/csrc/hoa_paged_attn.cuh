@@ -59,25 +59,32 @@ inline int pa_tile_keys(int page) {
 }
 
 // Which kernel takes a part.
+//   vec:  fp32 with 16-byte rows, up to 4 rows a head (1, 2 or 4 a tile).
 //   simt: fp32, head dims or strides that the copies do not take; 16 rows a tile, 32 where there are more.
 //   mma:  bf16, 16 rows a tile, any page size.
 //   tc:   bf16, 256 rows a tile, pages that tile (pa_tile_keys).
-enum PaKind { kPaSimt = 0, kPaSimt32 = 1, kPaMma = 2, kPaTc = 3 };
-inline int pa_tile_rows(int kind) { return kind == kPaTc ? 256 : kind == kPaSimt32 ? 32 : 16; }
+enum PaKind { kPaVec1, kPaVec2, kPaVec4, kPaSimt, kPaSimt32, kPaMma, kPaTc };
+inline int pa_tile_rows(int kind) {
+  const int rows[] = {1, 2, 4, 16, 32, 16, 256};
+  return rows[kind];
+}
 
 // Rows of a head from which tcgen05 takes a part: up to 16 one mma item reads the keys once.
 constexpr int kPaTcRows = 17;
 
 struct PaPlan { int kind1, tiles1, ns1, kind2, tiles2, ns2; };
 
-// `tensor`: bf16 with d % 8 == 0 and 16-byte strides, `tc`: tcgen05 takes the call (tensor, scale > 0).
-inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int W, int num_sms, bool tensor, bool tc) {
+// `vec`: fp32 with d % 4 == 0 and 16-byte strides, `tensor`: bf16 with d % 8 == 0 and 16-byte strides, `tc`: tcgen05
+// takes the call (tensor, scale > 0).
+inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int W, int num_sms, bool vec, bool tensor,
+                      bool tc) {
   PaPlan pl{};
   const long long G = H / Hk, keys1 = (long long)n_shared * page, keys2 = (long long)W * page;
   const long long rows1 = B * (long long)Tq * G, rows2 = Tq * G;
   const int kt = pa_tile_keys(page);
   tc = tc && kt > 0;
   auto kind_of = [&](long long rows) -> int {
+    if (vec && rows <= 4) return rows == 1 ? kPaVec1 : rows == 2 ? kPaVec2 : kPaVec4;
     return tc && rows >= kPaTcRows ? kPaTc : tensor ? kPaMma : rows > 16 ? kPaSimt32 : kPaSimt;
   };
   pl.kind1 = kind_of(rows1);
