@@ -92,33 +92,34 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   const long long r1 = pa_tile_rows(pl.kind1), r2 = pa_tile_rows(pl.kind2);
   const long long t1 = keys1 > 0 ? (rows1 + r1 - 1) / r1 : 0, t2 = keys2 > 0 ? (rows2 + r2 - 1) / r2 : 0;
   const long long u1 = t1 * Hk, u2 = t2 * Hk * B;
-  // mma and simt items take a range of keys each, the same for both parts: the shortest one with which all items run
-  // at once (4 CTAs an SM; of the room that the rows have - shorter rows split what they have as finely).  Measured at
-  // 65536 shared tokens and 8 rows: one wave 96 us, two 103, three 107; a range as short as 64 keys for small calls,
-  // where the time is one item's latency.
-  auto splits = [&](int kind, long long units, long long keys, long long range) -> long long {
+  // An item's range of keys: all the keys that the launch reads, over 4 CTAs an SM - one wave of equal items, whatever
+  // their part (of the room that the rows have: shorter rows split what they have as finely).  Measured at 65536
+  // shared tokens and 8 rows: one wave 96 us, two 103, three 107.  A simt item spends about four times as long on a key
+  // as the others, which only read it.  At least 64 keys: there an item's time is its latency.
+  auto range_of = [&](long long cost) -> long long {
+    const long long r = (cost + 4ll * num_sms - 1) / (4ll * num_sms);
+    return r < 64 ? 64 : r;
+  };
+  auto weight = [](int kind) -> long long { return kind == kPaSimt || kind == kPaSimt32 ? 4 : 1; };
+  const long long cost1 = u1 * keys1 * weight(pl.kind1), cost2 = u2 * keys2 * weight(pl.kind2);
+  auto splits = [&](int kind, long long units, long long keys, long long cost) -> int {
     if (units == 0) return 0;
-    long long ns;
+    long long ns, most;
     if (kind == kPaTc) {                           // one CTA an SM: split only what leaves SMs without one
       ns = num_sms / units;
-      const long long most = (keys + kt - 1) / kt;
-      ns = ns > most ? most : ns;
+      most = (keys + kt - 1) / kt;
     } else {
-      ns = (keys + range - 1) / range;
+      ns = (keys * weight(kind) + range_of(cost) - 1) / range_of(cost);
+      most = (keys + 63) / 64;
     }
-    return ns < 1 ? 1 : ns > 4096 ? 4096 : ns;
+    ns = ns > most ? most : ns;
+    return (int)(ns < 1 ? 1 : ns > 4096 ? 4096 : ns);
   };
-  long long range = 64;
-  const long long longest = (pl.kind1 != kPaTc ? keys1 : 0) + (pl.kind2 != kPaTc ? keys2 : 0);
-  for (; range < longest; range += range / 8) {
-    const long long items = (pl.kind1 != kPaTc ? u1 * splits(pl.kind1, u1, keys1, range) : 0) +
-                            (pl.kind2 != kPaTc ? u2 * splits(pl.kind2, u2, keys2, range) : 0);
-    if (items <= 4ll * num_sms) break;
-  }
+  const bool same = pl.kind1 == pl.kind2;          // one launch
+  pl.ns1 = splits(pl.kind1, u1, keys1, cost1 + (same ? cost2 : 0));
+  pl.ns2 = splits(pl.kind2, u2, keys2, cost2 + (same ? cost1 : 0));
   pl.tiles1 = (int)t1;
   pl.tiles2 = (int)t2;
-  pl.ns1 = (int)splits(pl.kind1, u1, keys1, range);
-  pl.ns2 = (int)splits(pl.kind2, u2, keys2, range);
   return pl;
 }
 
