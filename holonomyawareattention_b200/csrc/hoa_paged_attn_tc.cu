@@ -17,6 +17,7 @@
 // weights are 0, and the V rows are zeroed in shared memory before the product.
 #include <cudaTypedefs.h>
 
+#include "hoa_f32x2.cuh"
 #include "hoa_paged_attn.cuh"
 #include "hoa_sm100.cuh"
 
@@ -306,22 +307,23 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
         l_run *= corr;
         m_ref = m_new;
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;          // no key seen yet: weights 0
-        float ps[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const F2 c2 = f2(c), r2 = f2(-ref);
+        F2 ps[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int h = 0; h < 4; ++h) {                // 32 keys -> 16 packed columns
           float pk[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = pa_ex2(fmaf(sv[h][2 * e], c, -ref));
-            const float p1 = pa_ex2(fmaf(sv[h][2 * e + 1], c, -ref));
-            ps[(2 * e) & 7] += p0;
-            ps[(2 * e + 1) & 7] += p1;
+            const float2 x = f2_get(f2_fma(f2(sv[h][2 * e], sv[h][2 * e + 1]), c2, r2));
+            const float p0 = pa_ex2(x.x), p1 = pa_ex2(x.y);
+            ps[e & 3] = f2_add(ps[e & 3], f2(p0, p1));
             // the weights are rounded to bf16 for the product only; l sums them unrounded
             pk[e] = __uint_as_float(pt_pack(p0, p1));
           }
           tmem_st16(cS + 16 * h, pk);
         }
-        l_run += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+        const float2 sum = f2_get(f2_add(f2_add(ps[0], ps[1]), f2_add(ps[2], ps[3])));
+        l_run += sum.x + sum.y;
         tmem_wait_st();
       }
       tc_fence_before();

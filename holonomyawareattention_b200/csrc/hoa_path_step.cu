@@ -9,6 +9,7 @@
 
 #include <type_traits>
 
+#include "hoa_f32x2.cuh"
 #include "hoa_sm100.cuh"
 
 namespace hoa {
@@ -86,36 +87,6 @@ struct StLayout {
   static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
   static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
 };
-
-// Pairs of fp32 values: the packed forms of sm_100 (fma.rn.f32x2) halve the element
-// work's instructions, which is what a row's time goes into beside the products.
-using F2 = unsigned long long;
-HOA_DEVICE F2 f2(float x, float y) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-HOA_DEVICE F2 f2(float x) { return f2(x, x); }
-HOA_DEVICE float2 f2_get(F2 x) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-  return r;
-}
-HOA_DEVICE F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-HOA_DEVICE F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-HOA_DEVICE F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // x = hi + lo to 2^-22, two f16 each
 HOA_DEVICE void st_split2(F2 x, uint32_t& hi, uint32_t& lo) {
