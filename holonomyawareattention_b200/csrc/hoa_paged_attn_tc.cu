@@ -76,11 +76,14 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
   uint64_t* p_full = bars + 3;       // [2] per Q tile
   uint64_t* pv_done = bars + 5;      // [2] per Q tile
   uint64_t* fin = bars + 7;
-  uint64_t* kv_full = bars + 8;      // [NS]
-  uint64_t* kv_empty = bars + 12;    // [NS]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 17);
-  int* s_seen = reinterpret_cast<int*>(bars + 18);   // [2] the last key that a row of the tile sees, + 1
+  // K and V of a stage are handed over apart: K is free again once the last scores are computed, a round before V
+  uint64_t* k_full = bars + 8;       // [NS]
+  uint64_t* v_full = bars + 12;      // [NS]
+  uint64_t* k_empty = bars + 16;     // [NS]
+  uint64_t* v_empty = bars + 20;     // [NS]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 25);
+  int* s_seen = reinterpret_cast<int*>(bars + 26);   // [2] the last key that a row of the tile sees, + 1
 
   pa_let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
@@ -95,8 +98,10 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     }
     mbar_init(fin, 1);
     for (int i = 0; i < L::NS; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
     *s_abort = 0;
     s_seen[0] = s_seen[1] = 0;
@@ -142,29 +147,32 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       return -1;
     };
     int id = page_of(0);
-    int issued = 0;
-    for (int j = 0; j < nkt; ++j) {
+    int issued[2] = {0, 0};                          // K, V tiles
+    for (int j = 0; j < nkt && !bad; ++j) {
       const int s = j % L::NS, round = j / L::NS;
-      bool ok = true;
-      if (lid == 0 && round > 0) ok = mbar_wait_abortable(&kv_empty[s], (round - 1) & 1, s_abort, pt.max_wait);
-      if (!__all_sync(0xffffffffu, ok)) { bad = true; break; }
-      const uint32_t n = __popc(__ballot_sync(0xffffffffu, id >= 0));
-      if (lid == 0) mbar_arrive_expect_tx(&kv_full[s], n * (uint32_t)(pt.box * 128 * 2 * L::NKB));
-      __syncwarp();
-      if (id >= 0) {
-        uint8_t* st = sm + L::offStage + s * L::kStage + lid * pt.box * 128;
-        const int y = (it.k0 + j * KT + lid * pt.box) % p.page;
-        for (int kb = 0; kb < L::NKB; ++kb) {
-          tma_load_4d(st + kb * L::kBlk, &tk, &kv_full[s], kb * 64, y, it.kvh, id);
-          tma_load_4d(st + L::kQ + kb * L::kBlk, &tv, &kv_full[s], kb * 64, y, it.kvh, id);
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, id >= 0)) * (uint32_t)(pt.box * 128 * L::NKB);
+      const int y = (it.k0 + j * KT + lid * pt.box) % p.page;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        uint64_t* full = (kv ? v_full : k_full) + s;
+        bool ok = true;
+        if (lid == 0 && round > 0) ok = mbar_wait_abortable((kv ? v_empty : k_empty) + s, (round - 1) & 1, s_abort, pt.max_wait);
+        if (!__all_sync(0xffffffffu, ok)) { bad = true; break; }
+        if (lid == 0) mbar_arrive_expect_tx(full, bytes);
+        __syncwarp();
+        if (id >= 0) {
+          uint8_t* st = sm + L::offStage + s * L::kStage + kv * L::kQ + lid * pt.box * 128;
+          for (int kb = 0; kb < L::NKB; ++kb) tma_load_4d(st + kb * L::kBlk, kv ? &tv : &tk, full, kb * 64, y, it.kvh, id);
         }
+        issued[kv] = j + 1;
       }
-      issued = j + 1;
       id = page_of(j + 1);
     }
     // copies in flight land before the CTA exits (the last fill of each stage)
     if (lid == 0)
-      for (int j = max(0, issued - L::NS); j < issued; ++j) bad |= !mbar_wait(&kv_full[j % L::NS], (j / L::NS) & 1);
+      for (int kv = 0; kv < 2; ++kv)
+        for (int j = max(0, issued[kv] - L::NS); j < issued[kv]; ++j)
+          bad |= !mbar_wait((kv ? v_full : k_full) + j % L::NS, (j / L::NS) & 1);
     __syncwarp();
   } else if (warp == 8) {
     // ------------------------------------------------------------------ MMA
@@ -179,11 +187,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       // Order: S0 S1 | PV0 S0' PV1 S1' | ...: a query tile's next scores are computed as soon as its own weights are
       // taken, so that the two softmax warpgroups run out of step and the products of one hide behind the other's
       // exponentials (with S0 S1 PV0 PV1 both waited for all four).
-      int have = 0;                                  // key tiles known to have landed
+      int have = 0, v_have = 0;                      // K and V tiles known to have landed
       auto scores = [&](int i, int j) {
         const int s = j % L::NS;
         if (j >= have) {
-          ok = mbar_wait_abortable(&kv_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+          ok = mbar_wait_abortable(&k_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
           if (!ok) return;
           have = j + 1;
         }
@@ -195,6 +203,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
           mma_bf16(colS[i], dQ[i] + off, dK + off, idS, kk > 0 ? 1u : 0u);
         }
         tc_commit(&s_full[i]);
+        if (i == 1 || j >= n_t[1]) tc_commit(&k_empty[s]);     // the tile's last scores
       };
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -207,13 +216,18 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
           if (j >= n_t[i] || !ok) continue;
           ok = mbar_wait_abortable(&p_full[i], j & 1, s_abort, pt.max_wait);
           if (!ok) break;
+          if (v_have <= j) {
+            ok = mbar_wait_abortable(&v_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+            if (!ok) break;
+            v_have = j + 1;
+          }
           tc_fence_after();
           for (int kk = 0; kk < KT / 16; ++kk)         // 16 keys: 16 rows of 128 bytes of every V slab
             mma_bf16_ts(colO[i], colS[i] + kk * 8, dV + (uint64_t)(kk * 2048 >> 4), idO, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit(&pv_done[i]);
           if (j + 1 < n_t[i]) scores(i, j + 1);
         }
-        tc_commit(&kv_empty[s]);
+        tc_commit(&v_empty[s]);
       }
       if (!ok) bad = true;
       tc_commit(fin);
@@ -259,7 +273,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       if (j == nkt - 1 && kmax - k0 < KT) {
         // V rows past the last key that is seen: zero (each warpgroup that runs this tile)
         const int s = j % L::NS;
-        bad |= !mbar_wait_abortable(&kv_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+        bad |= !mbar_wait_abortable(&v_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
         uint8_t* v = sm + L::offStage + s * L::kStage + L::kQ;
         if (r >= kmax - k0 && r < KT)
 #pragma unroll
