@@ -640,76 +640,115 @@ def core_stages(a_all, qkv, n_heads, edge_scale, softmax_scale, out_dtype, hat_d
 # Page ids and rows that come from device memory are checked by the kernels; what
 # they find (HOA_ERR_PAGES) is raised by poll_status() / check_status().
 # ---------------------------------------------------------------------------
+# These calls take a few microseconds on the GPU, so the host side is kept short: one
+# pass of checks by device index, library functions and workspace sizes looked up once.
 _INT = torch.int32
-_WORKSPACE = {}                 # (op, sizes) -> bytes; the library computes them from the sizes alone
-_SMS = {}
+_SIZES = {}                     # (op, sizes) -> workspace bytes; the library computes them from the sizes alone
+_DEVICES = {}                   # device index -> (SM count, address of the mapped status word)
+_FN = {}                        # library functions by name
+_ARRAYS = {}                    # ctypes array types by length
 
 
-def _sms(dev: torch.device) -> int:
-    n = _SMS.get(dev)
-    if n is None:
-        n = _SMS[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
-    return n
+def _fn(name: str):
+    f = _FN.get(name)
+    if f is None:
+        f = _FN[name] = getattr(_lib.load(), name)
+    return f
+
+
+def _device(idx: int):
+    v = _DEVICES.get(idx)
+    if v is None:
+        v = _DEVICES[idx] = (torch.cuda.get_device_properties(idx).multi_processor_count,
+                             _watch(torch.device("cuda", idx)).mapped_ptr)
+    return v
+
+
+def _index(t) -> int:
+    i = t.get_device()
+    if i < 0:
+        raise NotImplementedError("the B200 kernels need CUDA tensors (there is no CPU path)")
+    return i
 
 
 def _bytes_of(fn: str, *sizes) -> int:
     key = (fn, sizes)
-    n = _WORKSPACE.get(key)
+    n = _SIZES.get(key)
     if n is None:
-        if len(_WORKSPACE) > 4096:
-            _WORKSPACE.clear()
-        n = _WORKSPACE[key] = int(getattr(_lib.load(), fn)(*sizes))
+        if len(_SIZES) > 4096:
+            _SIZES.clear()
+        n = _SIZES[key] = int(_fn(fn)(*sizes))
     return n
 
 
-def _on(dev: torch.device, fn: str, *args) -> None:
-    """Call ``fn`` with ``dev`` current, on dev's current stream (the last argument)."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(fn, *args, _stream(dev))
+def _run(idx: int, name: str, *args) -> None:
+    """Call ``name`` with device ``idx`` current, its status word and its current stream as the last arguments."""
+    if torch.cuda.current_device() == idx:
+        st = _fn(name)(*args, _device(idx)[1], torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(dev):
-            _lib.call(fn, *args, _stream(dev))
+        with torch.cuda.device(idx):
+            st = _fn(name)(*args, _device(idx)[1], torch._C._cuda_getCurrentRawStream(idx))
+    if st != 0:
+        _lib.check(name, st)
 
 
-def _ints(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
-    if t.dtype != _INT or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{name} must be a contiguous int32 {shape} tensor on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+def _longs(*values):
+    """A host array of 64-bit integers (strides, addresses) for a call."""
+    n = len(values)
+    t = _ARRAYS.get(n)
+    if t is None:
+        t = _ARRAYS[n] = ctypes.c_longlong * n
+    return t(*values)
+
+
+def _bad_ints(t, name, shape, idx):
+    _index(t)
+    raise ValueError(f"{name} must be a contiguous int32 {shape} tensor on cuda:{idx}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _ints(t, name, shape, idx) -> None:
+    if t.dtype is not _INT or t.shape != shape or t.get_device() != idx or not t.is_contiguous():
+        _bad_ints(t, name, shape, idx)
 
 
 def _books(table, lens, refs, page):
-    """(S, W, n_pages) of a bookkeeping state, checked."""
-    _need_cuda(table, lens, refs)
+    """(device index, S, W, n_pages) of a bookkeeping state, checked."""
+    idx = _index(table)
     if table.dim() != 2 or refs.dim() != 1 or table.numel() == 0 or refs.numel() == 0:
         raise ValueError("table must be (S, W) and refs (n_pages,), neither empty")
     S, W = table.shape
-    _ints(table, "table", (S, W), table.device)
+    n_pages = refs.shape[0]
+    _ints(table, "table", (S, W), idx)
     if lens is not None:
-        _ints(lens, "lens", (S,), table.device)
-    _ints(refs, "refs", (refs.shape[0],), table.device)
+        _ints(lens, "lens", (S,), idx)
+    _ints(refs, "refs", (n_pages,), idx)
     if page < 1:
         raise ValueError("page must be at least 1")
-    return S, W, refs.shape[0]
+    return idx, S, W, n_pages
 
 
-def _pool_args(pools, n_pages, dev):
-    """ctypes arrays (base pointers, bytes between pages, bytes of a page) of a list of pools."""
+def _pool_args(pools, n_pages, idx):
+    """(keep-alive, base pointers, bytes between pages, bytes of a page, count) of a list of pools."""
     n = len(pools)
-    base, stride, size = (ctypes.c_void_p * n)(), (ctypes.c_longlong * n)(), (ctypes.c_longlong * n)()
-    for i, t in enumerate(pools):
-        if not t.is_cuda or t.device != dev or t.dim() < 2 or t.shape[0] != n_pages:
-            raise ValueError(f"pools must be ({n_pages}, ...) tensors on {dev}")
+    base, stride, size = [], [], []
+    for t in pools:
+        if t.dim() < 2 or t.shape[0] != n_pages or t.get_device() != idx:
+            _index(t)
+            raise ValueError(f"pools must be ({n_pages}, ...) tensors on cuda:{idx}")
         e = t.element_size()
-        stride[i] = t.stride(0) * e
+        st = t.stride(0) * e
         if t.is_contiguous():
-            size[i] = stride[i]
+            size.append(st)
         else:
             p = t[0]
             if not p.is_contiguous() or t.stride(0) < p.numel():
                 raise ValueError("the pages of a pool must be contiguous, one after another")
-            size[i] = p.numel() * e
-        base[i] = t.data_ptr()
-    return base, stride, size, n
+            size.append(p.numel() * e)
+        base.append(t.data_ptr())
+        stride.append(st)
+    a = _longs(*base, *stride, *size)
+    at = ctypes.addressof(a)
+    return a, at, at + 8 * n, at + 16 * n, n
 
 
 def pages_reserve(table, lens, refs, counts, page: int):
@@ -718,15 +757,13 @@ def pages_reserve(table, lens, refs, counts, page: int):
     table (S, W), lens (S,), refs (n_pages,), counts (S,): int32.  Free pages (refs == 0) are taken
     lowest index first, rows in order.  Without enough of them, or where a row would pass W pages, the
     state comes back unchanged and HOA_ERR_PAGES is reported (hoa_pages_reserve)."""
-    S, W, n_pages = _books(table, lens, refs, page)
-    dev = table.device
-    _need_cuda(counts)
-    _ints(counts, "counts", (S,), dev)
+    idx, S, W, n_pages = _books(table, lens, refs, page)
+    _ints(counts, "counts", (S,), idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
     n = _bytes_of("hoa_pages_workspace_bytes", S, n_pages)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _on(dev, "hoa_pages_reserve", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), out[0].data_ptr(),
-        out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, ws.data_ptr(), n, _watch(dev).mapped_ptr)
+    ws = torch.empty(n, dtype=torch.uint8, device=table.device)
+    _run(idx, "hoa_pages_reserve", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), out[0].data_ptr(),
+         out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, ws.data_ptr(), n)
     return out
 
 
@@ -736,35 +773,30 @@ def pages_fork(pools, table, lens, refs, src, dst, page: int):
     src, dst (n,) int32; the dst rows are empty and differ.  Full pages are shared; a last page that
     is not full is copied, in every pool (n_pages, ...) of ``pools``, to a page of its own.  All or
     nothing, as pages_reserve (hoa_pages_fork)."""
-    S, W, n_pages = _books(table, lens, refs, page)
-    dev = table.device
-    _need_cuda(src, dst)
+    idx, S, W, n_pages = _books(table, lens, refs, page)
     n = src.numel()
-    _ints(src, "src", (n,), dev)
-    _ints(dst, "dst", (n,), dev)
+    _ints(src, "src", (n,), idx)
+    _ints(dst, "dst", (n,), idx)
     if n > S:
         raise ValueError("more forks than rows")
-    base, stride, size, np_ = _pool_args(pools, n_pages, dev)
+    _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
     nb = _bytes_of("hoa_pages_workspace_bytes", n, n_pages)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _on(dev, "hoa_pages_fork", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
-        out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, base, stride, size, np_, ws.data_ptr(),
-        nb, _watch(dev).mapped_ptr)
+    ws = torch.empty(nb, dtype=torch.uint8, device=table.device)
+    _run(idx, "hoa_pages_fork", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
+         out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, base, stride, size, np_, ws.data_ptr(), nb)
     return out
 
 
 def pages_free(table, lens, refs, rows, page: int):
     """The rows (n,) int32 end: (table, lens, refs); a page that no row holds any more is free
     (hoa_pages_free)."""
-    S, W, n_pages = _books(table, lens, refs, page)
-    dev = table.device
-    _need_cuda(rows)
+    idx, S, W, n_pages = _books(table, lens, refs, page)
     n = rows.numel()
-    _ints(rows, "rows", (n,), dev)
+    _ints(rows, "rows", (n,), idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
-    _on(dev, "hoa_pages_free", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), rows.data_ptr(), n, out[0].data_ptr(),
-        out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, _watch(dev).mapped_ptr)
+    _run(idx, "hoa_pages_free", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), rows.data_ptr(), n, out[0].data_ptr(),
+         out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page)
     return out
 
 
@@ -772,72 +804,71 @@ def pages_compact(pools, table, refs):
     """The live pages move to 0 .. live-1 in every pool: (table, refs, live (1,)).
 
     The i-th free page below ``live`` receives the i-th live page at or above it (hoa_pages_compact)."""
-    S, W, n_pages = _books(table, None, refs, 1)
-    dev = table.device
-    base, stride, size, np_ = _pool_args(pools, n_pages, dev)
+    idx, S, W, n_pages = _books(table, None, refs, 1)
+    _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
     table2, refs2 = torch.empty_like(table), torch.empty_like(refs)
-    live = torch.empty(1, dtype=_INT, device=dev)
+    live = torch.empty(1, dtype=_INT, device=table.device)
     nb = _bytes_of("hoa_pages_workspace_bytes", 0, n_pages)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _on(dev, "hoa_pages_compact", table.data_ptr(), refs.data_ptr(), table2.data_ptr(), refs2.data_ptr(), live.data_ptr(),
-        S, W, n_pages, base, stride, size, np_, ws.data_ptr(), nb, _watch(dev).mapped_ptr)
+    ws = torch.empty(nb, dtype=torch.uint8, device=table.device)
+    _run(idx, "hoa_pages_compact", table.data_ptr(), refs.data_ptr(), table2.data_ptr(), refs2.data_ptr(), live.data_ptr(),
+         S, W, n_pages, base, stride, size, np_, ws.data_ptr(), nb)
     return table2, refs2, live
 
 
 def pages_copy(pools, src, dst) -> None:
     """Page dst[i] = page src[i] in every pool (n_pages, ...), in place; no page is both (hoa_pages_copy)."""
-    _need_cuda(src, dst, *pools)
+    idx = _index(src)
     if not pools:
         return
-    dev = src.device
     n = src.numel()
-    _ints(src, "src", (n,), dev)
-    _ints(dst, "dst", (n,), dev)
+    _ints(src, "src", (n,), idx)
+    _ints(dst, "dst", (n,), idx)
     n_pages = pools[0].shape[0]
-    base, stride, size, np_ = _pool_args(pools, n_pages, dev)
-    _on(dev, "hoa_pages_copy", base, stride, size, np_, src.data_ptr(), dst.data_ptr(), n, n_pages, _watch(dev).mapped_ptr)
+    _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
+    _run(idx, "hoa_pages_copy", base, stride, size, np_, src.data_ptr(), dst.data_ptr(), n, n_pages)
 
 
-def _cache(k_pages, v_pages, dev):
+def _cache(k_pages, v_pages, idx):
     """(n_pages, Hk, page, d, dtype code, strides) of a k and a v pool that go together."""
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or k_pages.numel() == 0:
         raise ValueError("k_pages and v_pages must be (n_pages, H, page, d), of one shape and type, not empty")
     st = k_pages.stride()
     if v_pages.stride() != st or (st[3] != 1 and k_pages.shape[3] != 1):
         raise ValueError("k_pages and v_pages must have the same strides, the innermost 1")
-    if k_pages.device != dev or v_pages.device != dev:
-        raise ValueError(f"k_pages and v_pages must be on {dev}")
-    return (*k_pages.shape, _dtype_code(k_pages.dtype), (ctypes.c_longlong * 3)(*st[:3]))
+    if k_pages.get_device() != idx or v_pages.get_device() != idx:
+        _index(k_pages), _index(v_pages)
+        raise ValueError(f"k_pages and v_pages must be on cuda:{idx}")
+    return (*k_pages.shape, _dtype_code(k_pages.dtype), _longs(*st[:3]))
 
 
-def _row_table(table, B, dev):
+def _row_table(table, B, idx):
     """(W, row stride) of a (B, W) table; rows may be strided (a view of a wider table)."""
-    if table.dtype != _INT or table.dim() != 2 or table.shape[0] != B or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"table must be int32 ({B}, W) on {dev}, contiguous within a row")
+    if table.dtype is not _INT or table.dim() != 2 or table.shape[0] != B or table.get_device() != idx or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        _index(table)
+        raise ValueError(f"table must be int32 ({B}, W) on cuda:{idx}, contiguous within a row")
     return table.shape[1], table.stride(0)
 
 
 def _strides3(t):
-    return (ctypes.c_longlong * 3)(*t.stride()[:3])
+    return _longs(*t.stride()[:3])
 
 
 def pages_write(k, v, k_pages, v_pages, table, lens) -> None:
     """k, v (B, T, H, d) become the last T tokens of each row, in place: token t goes to position
     lens[b] - T + t (lens counts them; the pages are reserved).  hoa_pages_write."""
-    _need_cuda(k, v, k_pages, v_pages, table, lens)
-    dev = k.device
-    n_pages, H, page, d, code, ps = _cache(k_pages, v_pages, dev)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.shape[2:] != (H, d) or v.device != dev or \
+    idx = _index(k)
+    n_pages, H, page, d, code, ps = _cache(k_pages, v_pages, idx)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.shape[2:] != (H, d) or v.get_device() != idx or \
             (d > 1 and (k.stride(3) != 1 or v.stride(3) != 1)):
         raise ValueError(f"k and v must be (B, T, {H}, {d}) of one type, the innermost stride 1")
     B, T = k.shape[:2]
     if B == 0 or T == 0:
         return
-    W, tw = _row_table(table, B, dev)
-    _ints(lens, "lens", (B,), dev)
-    _on(dev, "hoa_pages_write", k.data_ptr(), v.data_ptr(), _dtype_code(k.dtype), _strides3(k), _strides3(v),
-        k_pages.data_ptr(), v_pages.data_ptr(), code, ps, table.data_ptr(), tw, lens.data_ptr(), B, T, H, d, page, W, n_pages,
-        _watch(dev).mapped_ptr)
+    W, tw = _row_table(table, B, idx)
+    _ints(lens, "lens", (B,), idx)
+    _run(idx, "hoa_pages_write", k.data_ptr(), v.data_ptr(), _dtype_code(k.dtype), _strides3(k), _strides3(v),
+         k_pages.data_ptr(), v_pages.data_ptr(), code, ps, table.data_ptr(), tw, lens.data_ptr(), B, T, H, d, page, W, n_pages)
 
 
 def paged_attn_fwd(q, k_pages, v_pages, table, lens, softmax_scale: float, shared=None, paths=None, out_dtype=None):
@@ -849,38 +880,44 @@ def paged_attn_fwd(q, k_pages, v_pages, table, lens, softmax_scale: float, share
     all keys of a row, the shared ones and its Tq newest included.  Query t sees the keys at positions
     0 .. lens[b] - Tq + t; one that sees none gives 0 and lse -inf.  ``paths`` (B, H, d, d) fp32 with
     Tq = 1: out = P o.  hoa_paged_attn_fwd."""
-    _need_cuda(q, k_pages, v_pages, table, lens, shared, paths)
+    idx = _index(q)
     if q.dim() != 4 or q.numel() == 0:
         raise ValueError("q must be (B, Tq, H, d), not empty")
     B, Tq, H, d = q.shape
-    dev = q.device
-    n_pages, Hk, page, dk, code, ps = _cache(k_pages, v_pages, dev)
-    if dk != d or q.dtype != k_pages.dtype or H % Hk != 0 or (d > 1 and q.stride(3) != 1):
+    n_pages, Hk, page, dk, code, ps = _cache(k_pages, v_pages, idx)
+    qs = q.stride()
+    if dk != d or q.dtype != k_pages.dtype or H % Hk != 0 or (d > 1 and qs[3] != 1):
         raise ValueError(f"q must be (B, Tq, H, {dk}) {k_pages.dtype} with H a multiple of {Hk}, the innermost stride 1")
     if d > 128:
         raise NotImplementedError(f"head dim {d} > 128")
-    W, tw = _row_table(table, B, dev)
-    _ints(lens, "lens", (B,), dev)
+    W, tw = _row_table(table, B, idx)
+    _ints(lens, "lens", (B,), idx)
     n_shared = 0
     if shared is not None:
         n_shared = shared.numel()
-        _ints(shared, "shared", (n_shared,), dev)
+        _ints(shared, "shared", (n_shared,), idx)
     if paths is not None:
         if Tq != 1:
             raise ValueError("paths go with one query token a row")
-        if paths.dtype != torch.float32 or tuple(paths.shape) != (B, H, d, d) or not paths.is_contiguous() or paths.device != dev:
-            raise ValueError(f"paths must be a contiguous fp32 {(B, H, d, d)} tensor on {dev}")
+        _path(paths, "paths", (B, H, d, d), idx)
     out_dtype = out_dtype or q.dtype
-    sms = _sms(dev)
+    sms = _device(idx)[0]
     nb = _bytes_of("hoa_paged_attn_workspace_bytes", B, Tq, H, Hk, d, page, n_shared, W, sms)
+    dev = q.device
     ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    out = torch.empty(B, Tq, H, d, dtype=out_dtype, device=dev)
-    lse = torch.empty(B, Tq, H, dtype=torch.float32, device=dev)
-    _on(dev, "hoa_paged_attn_fwd", q.data_ptr(), _strides3(q), k_pages.data_ptr(), v_pages.data_ptr(), ps, code,
-        shared.data_ptr() if n_shared else None, n_shared, table.data_ptr(), tw, W, lens.data_ptr(), _ptr(paths),
-        out.data_ptr(), _dtype_code(out_dtype), lse.data_ptr(), softmax_scale, B, Tq, H, Hk, d, page, n_pages, sms,
-        ws.data_ptr(), nb, _watch(dev).mapped_ptr)
+    out = torch.empty((B, Tq, H, d), dtype=out_dtype, device=dev)
+    lse = torch.empty((B, Tq, H), dtype=torch.float32, device=dev)
+    _run(idx, "hoa_paged_attn_fwd", q.data_ptr(), _longs(*qs[:3]), k_pages.data_ptr(), v_pages.data_ptr(), ps, code,
+         shared.data_ptr() if n_shared else None, n_shared, table.data_ptr(), tw, W, lens.data_ptr(),
+         paths.data_ptr() if paths is not None else None, out.data_ptr(), _dtype_code(out_dtype), lse.data_ptr(),
+         softmax_scale, B, Tq, H, Hk, d, page, n_pages, sms, ws.data_ptr(), nb)
     return out, lse
+
+
+def _path(t, name, shape, idx) -> None:
+    if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != idx or not t.is_contiguous():
+        _index(t)
+        raise ValueError(f"{name} must be a contiguous fp32 {shape} tensor on cuda:{idx}")
 
 
 def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, table, lens, a_bias=None,
@@ -892,10 +929,9 @@ def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, tabl
     lens[b] - 1 of the row's pages (table (B, W), lens (B,) with the token counted; reserve it first).
     qkv (B, 3D) holds [q | k | v] per head.  lens 1: no edge, P' = I.  lens 0: P' = P, q^ = 0, nothing
     written.  ``P_out`` may be P.  hoa_path_step."""
-    _need_cuda(a, P, qkv, k_pages, v_pages, table, lens, a_bias, P_out)
-    dev = qkv.device
+    idx = _index(qkv)
     H = n_heads
-    n_pages, Hk, page, d, code, ps = _cache(k_pages, v_pages, dev)
+    n_pages, Hk, page, d, code, ps = _cache(k_pages, v_pages, idx)
     if Hk != H:
         raise ValueError(f"the pools must have n_heads = {H} heads, got {Hk}")
     if qkv.dim() != 2 or qkv.shape[1] != 3 * H * d or qkv.stride(1) != 1 or qkv.shape[0] == 0:
@@ -903,24 +939,32 @@ def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, tabl
     if d < 2 or d > 120:
         raise NotImplementedError(f"head dim {d} (2 to 120)")
     B = qkv.shape[0]
-    if a.dtype != torch.float32:
+    if a.dtype is not torch.float32:
         raise NotImplementedError("the path step takes fp32 generators")
-    a_code = _gen_code(a, gen_layout)
-    width = _gen_width(H, d, gen_layout)
-    if tuple(a.shape) != (B, width) or not a.is_contiguous() or a.device != dev:
-        raise ValueError(f"a must be a contiguous ({B}, {width}) tensor on {dev} for the {gen_layout} layout")
-    _check_bias(a_bias, width)
+    if gen_layout == "packed":
+        a_code, width = _lib.HOA_F32, H * (d * (d - 1) // 2)
+    else:
+        a_code, width = _gen_code(a, gen_layout), _gen_width(H, d, gen_layout)
+    if a.shape != (B, width) or not a.is_contiguous() or a.get_device() != idx:
+        _index(a)
+        raise ValueError(f"a must be a contiguous ({B}, {width}) tensor on cuda:{idx} for the {gen_layout} layout")
+    if a_bias is not None:
+        _check_bias(a_bias, width)
+        if a_bias.get_device() != idx:
+            _index(a_bias)
+            raise ValueError(f"a_bias must be on cuda:{idx}")
+    shape = (B, H, d, d)
     if P_out is None:
-        P_out = torch.empty(B, H, d, d, dtype=torch.float32, device=dev)
-    for t, nm in ((P, "P"), (P_out, "P_out")):
-        if t.dtype != torch.float32 or tuple(t.shape) != (B, H, d, d) or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"{nm} must be a contiguous fp32 {(B, H, d, d)} tensor on {dev}")
-    W, tw = _row_table(table, B, dev)
+        P_out = torch.empty(shape, dtype=torch.float32, device=qkv.device)
+    else:
+        _path(P_out, "P_out", shape, idx)
+    _path(P, "P", shape, idx)
+    W, tw = _row_table(table, B, idx)
     if W == 0:
         raise ValueError("table must have at least one page a row")
-    _ints(lens, "lens", (B,), dev)
-    qh = torch.empty(B, H, d, dtype=k_pages.dtype, device=dev)
-    _on(dev, "hoa_path_step", a.data_ptr(), a_code, _ptr(a_bias), edge_scale, P.data_ptr(), P_out.data_ptr(), qkv.data_ptr(),
-        _dtype_code(qkv.dtype), qkv.stride(0), qh.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), code, ps,
-        table.data_ptr(), tw, W, lens.data_ptr(), B, H, d, page, n_pages, _watch(dev).mapped_ptr)
+    _ints(lens, "lens", (B,), idx)
+    qh = torch.empty((B, H, d), dtype=k_pages.dtype, device=qkv.device)
+    _run(idx, "hoa_path_step", a.data_ptr(), a_code, a_bias.data_ptr() if a_bias is not None else None, edge_scale,
+         P.data_ptr(), P_out.data_ptr(), qkv.data_ptr(), _dtype_code(qkv.dtype), qkv.stride(0), qh.data_ptr(),
+         k_pages.data_ptr(), v_pages.data_ptr(), code, ps, table.data_ptr(), tw, W, lens.data_ptr(), B, H, d, page, n_pages)
     return P_out, qh
