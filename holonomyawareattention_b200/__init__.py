@@ -7,5 +7,6 @@ CUDA kernels behind the C ABI of libhoa.so (include/hoa.h).
 """
 from .attention import PathOrderedGeometricMHA
 from . import ops
+from .cache import PathCache, decode, prefill
 
-__all__ = ["PathOrderedGeometricMHA", "ops"]
+__all__ = ["PathOrderedGeometricMHA", "PathCache", "prefill", "decode", "ops"]

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/hoa.h"
 
 #define HOA_DEVICE __device__ __forceinline__
@@ -73,6 +75,19 @@ long long wait_bound_cycles();
 inline int launch_status() {
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? HOA_OK : HOA_ERR_LAUNCH;
+}
+
+// Let `kernel` use `bytes` of dynamic shared memory on the current device: asked of the driver once a device (`done`:
+// one bit each, one variable a kernel), which a call of a few microseconds would otherwise spend a tenth of its time on.
+template <class K>
+inline bool allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 // Smallest supported padded head dimension >= d, or 0.

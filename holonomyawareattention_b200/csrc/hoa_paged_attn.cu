@@ -201,8 +201,9 @@ template <int R, bool V4>
 static int launch_simt(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
   const int ld = ((a.d + 3) / 4 | 1) * 4;
   const size_t smem = ((8 * R + 2 * kPsKeys) * (size_t)ld + 8 * R * 68) * sizeof(float);
-  if (cudaFuncSetAttribute(paged_attn_simt_kernel<R, V4>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
+  static std::atomic<unsigned long long> done{0};
+  const size_t most = ((8 * R + 2 * kPsKeys) * (size_t)132 + 8 * R * 68) * sizeof(float);   // at d = 128
+  if (!allow_smem(paged_attn_simt_kernel<R, V4>, most, done)) return HOA_ERR_LAUNCH;
   return pa_launch(paged_attn_simt_kernel<R, V4>, items, kPsThreads, smem, s, early, a, first);
 }
 

@@ -312,8 +312,8 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
 template <int D8, bool kHalf>
 static int launch_mma_h(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
   using C = PmCfg<D8>;
-  if (cudaFuncSetAttribute(paged_attn_mma_kernel<D8, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(paged_attn_mma_kernel<D8, kHalf>, C::kSmem, done)) return HOA_ERR_LAUNCH;
   return pa_launch(paged_attn_mma_kernel<D8, kHalf>, items, kPmWarps * 32, C::kSmem, s, early, a, first);
 }
 

@@ -409,8 +409,8 @@ template <int DP16>
 static int launch_ptc(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, unsigned first,
                       unsigned items, bool early, cudaStream_t s) {
   using L = PtLayout<DP16>;
-  if (cudaFuncSetAttribute(paged_attn_tc_kernel<DP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(paged_attn_tc_kernel<DP16>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
   return pa_launch(paged_attn_tc_kernel<DP16>, items, kPtThreads, L::kAlloc, s, early, mk, mv, a, t, first);
 }
 

@@ -109,6 +109,56 @@ HOA_DEVICE void pg_list(PgSlice s, Pred pred, int base, int limit, int* out, int
 }
 
 // ---------------------------------------------------------------------------
+// payload: page to[i] of every pool = page from[i]
+// ---------------------------------------------------------------------------
+constexpr int kCpThreads = 256, kCpVecs = 8;       // 16-byte vectors a thread has in flight
+constexpr int kMaxPools = 32;
+
+struct PgCopyArgs {
+  uint8_t* base[kMaxPools];
+  long long stride[kMaxPools];   // bytes between pages
+  long long bytes[kMaxPools];    // bytes of a page
+  const int* from; const int* to;
+  const int* count;              // device count of pairs (nullptr: n)
+  int n, n_pages, pools, chunks; // chunks: of the largest page
+  int* status;
+};
+
+// One unit: kThreads * kCpVecs vectors of one page of one pool, by kThreads threads of which this is number t.
+template <class V, int kThreads>
+HOA_DEVICE void pg_copy_unit(const PgCopyArgs& p, long long u, int t) {
+  const int c = (int)(u % p.chunks);
+  const long long r = u / p.chunks;
+  const int pool = (int)(r % p.pools), i = (int)(r / p.pools);
+  const int a = p.from[i], b = p.to[i];
+  if (a < 0 && b < 0) return;                      // no copy for this pair
+  if (a < 0 || b < 0 || a >= p.n_pages || b >= p.n_pages) {
+    if (t == 0) pg_fail(p.status);
+    return;
+  }
+  const V* src = reinterpret_cast<const V*>(p.base[pool] + a * p.stride[pool]);
+  V* dst = reinterpret_cast<V*>(p.base[pool] + b * p.stride[pool]);
+  const long long nv = p.bytes[pool] / (long long)sizeof(V);
+  const long long v0 = (long long)c * (kThreads * kCpVecs) + t;
+  V buf[kCpVecs];
+#pragma unroll
+  for (int k = 0; k < kCpVecs; ++k)
+    if (v0 + k * kThreads < nv) buf[k] = src[v0 + k * kThreads];
+#pragma unroll
+  for (int k = 0; k < kCpVecs; ++k)
+    if (v0 + k * kThreads < nv) dst[v0 + k * kThreads] = buf[k];
+}
+
+// A payload of up to kCpInline bytes is copied by the bookkeeping cluster itself (16-byte vectors, a warp a 4 KB
+// unit), which spares the second launch: a fork with four pages of 12 KB in two pools takes 20 us with its host side
+// against 23.  Beyond a megabyte eight CTAs take longer than the launch that they spare.
+constexpr long long kCpInline = 1 << 20;
+HOA_DEVICE void pg_copy_inline(const PgCopyArgs& p, int n, int warp, int warps) {
+  const long long units = (long long)n * p.pools * p.chunks;
+  for (long long u = warp; u < units; u += warps) pg_copy_unit<uint4, 32>(p, u, threadIdx.x & 31);
+}
+
+// ---------------------------------------------------------------------------
 // reserve: row s grows by counts[s] tokens (new pages where they cross one);
 // fork: row dst[i] becomes a copy of row src[i] that shares its full pages and
 // has its own copy of a last page that is not full.
@@ -128,7 +178,7 @@ struct PgTakeArgs {
 
 template <bool kFork>
 __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
-pages_take_kernel(PgTakeArgs p) {
+pages_take_kernel(PgTakeArgs p, const __grid_constant__ PgCopyArgs cp) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ int s_warp[kPgWarps];
   __shared__ int s_free, s_need, s_bad;
@@ -239,6 +289,10 @@ pages_take_kernel(PgTakeArgs p) {
       if (lid == 0) st.lens_out[i] = len + c;
     }
   }
+  if (kFork && cp.n > 0) {                 // a small payload
+    cl.sync();
+    pg_copy_inline(cp, cp.n, gt >> 5, kPgCluster * kPgWarps);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -292,7 +346,8 @@ struct PgCompactArgs {
   int* status;
 };
 
-__global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads) pages_compact_kernel(PgCompactArgs p) {
+__global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
+pages_compact_kernel(PgCompactArgs p, const __grid_constant__ PgCopyArgs cp) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ int s_warp[kPgWarps];
   __shared__ int s_live, s_hole, s_move;
@@ -342,51 +397,15 @@ __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
     }
     st.table_out[i] = id;
   }
+  if (cp.n > 0) pg_copy_inline(cp, min(moves, cp.n), gt >> 5, kPgCluster * kPgWarps);   // a small payload
 }
 
-// ---------------------------------------------------------------------------
-// payload: page to[i] of every pool = page from[i]
-// ---------------------------------------------------------------------------
-constexpr int kCpThreads = 256, kCpVecs = 8;       // 16-byte vectors a thread has in flight
-constexpr int kMaxPools = 32;
-
-struct PgCopyArgs {
-  uint8_t* base[kMaxPools];
-  long long stride[kMaxPools];   // bytes between pages
-  long long bytes[kMaxPools];    // bytes of a page
-  const int* from; const int* to;
-  const int* count;              // device count of pairs (nullptr: n)
-  int n, n_pages, pools, chunks; // chunks: of the largest page
-  int* status;
-};
-
+// The copy as a launch of its own, bound by HBM.
 template <class V>
 __global__ void __launch_bounds__(kCpThreads) pages_copy_kernel(const __grid_constant__ PgCopyArgs p) {
-  constexpr int kChunk = kCpThreads * kCpVecs;     // vectors a unit copies
   const int n = p.count != nullptr ? min(*p.count, p.n) : p.n;
   const long long units = (long long)n * p.pools * p.chunks;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const int c = (int)(u % p.chunks);
-    const long long r = u / p.chunks;
-    const int pool = (int)(r % p.pools), i = (int)(r / p.pools);
-    const int a = p.from[i], b = p.to[i];
-    if (a < 0 && b < 0) continue;                  // no copy for this pair
-    if (a < 0 || b < 0 || a >= p.n_pages || b >= p.n_pages) {
-      if (threadIdx.x == 0) pg_fail(p.status);
-      continue;
-    }
-    const V* src = reinterpret_cast<const V*>(p.base[pool] + a * p.stride[pool]);
-    V* dst = reinterpret_cast<V*>(p.base[pool] + b * p.stride[pool]);
-    const long long nv = p.bytes[pool] / (long long)sizeof(V);
-    const long long v0 = (long long)c * kChunk + threadIdx.x;
-    V buf[kCpVecs];
-#pragma unroll
-    for (int k = 0; k < kCpVecs; ++k)
-      if (v0 + k * kCpThreads < nv) buf[k] = src[v0 + k * kCpThreads];
-#pragma unroll
-    for (int k = 0; k < kCpVecs; ++k)
-      if (v0 + k * kCpThreads < nv) dst[v0 + k * kCpThreads] = buf[k];
-  }
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) pg_copy_unit<V, kCpThreads>(p, u, threadIdx.x);
 }
 
 template <class V>
@@ -398,24 +417,47 @@ static int launch_copy(PgCopyArgs a, long long most, cudaStream_t s) {
   return launch_status();
 }
 
-static int copy_pools(void* const* pools, const long long* strides, const long long* bytes, int n_pools,
-                      const int* from, const int* to, const int* count, int n, int n_pages, int* status,
+struct PgPools { void* const* base; const long long* stride; const long long* bytes; int n; };
+
+// The copy of up to kMaxPools pools from number k0 on; `bits`: alignment of everything it touches, `most`: bytes of its
+// largest page.
+static PgCopyArgs copy_args(const PgPools& q, int k0, const int* from, const int* to, const int* count, int n, int n_pages,
+                            int* status, unsigned long long* bits, long long* most) {
+  PgCopyArgs a{};
+  a.pools = q.n - k0 < kMaxPools ? q.n - k0 : kMaxPools;
+  a.from = from; a.to = to; a.count = count; a.n = n; a.n_pages = n_pages; a.status = status;
+  *bits = 0;
+  *most = 0;
+  for (int k = 0; k < a.pools; ++k) {
+    a.base[k] = static_cast<uint8_t*>(q.base[k0 + k]);
+    a.stride[k] = q.stride[k0 + k];
+    a.bytes[k] = q.bytes[k0 + k];
+    *bits |= (unsigned long long)reinterpret_cast<uintptr_t>(a.base[k]) | (unsigned long long)a.stride[k] |
+             (unsigned long long)a.bytes[k];
+    if (a.bytes[k] > *most) *most = a.bytes[k];
+  }
+  return a;
+}
+
+// The copy for the bookkeeping kernel itself, or one with n = 0: small, in 16-byte vectors, one set of pools.
+static PgCopyArgs inline_copy(const PgPools& q, const int* from, const int* to, int n, int n_pages, int* status) {
+  unsigned long long bits;
+  long long most, all = 0;
+  if (q.n == 0 || q.n > kMaxPools || n == 0) return PgCopyArgs{};
+  PgCopyArgs a = copy_args(q, 0, from, to, nullptr, n, n_pages, status, &bits, &most);
+  for (int k = 0; k < a.pools; ++k) all += a.bytes[k] * n;
+  if ((bits & 15) != 0 || all > kCpInline) return PgCopyArgs{};
+  a.chunks = (int)((most / 16 + 32 * kCpVecs - 1) / (32 * kCpVecs));
+  return a;
+}
+
+static int copy_pools(const PgPools& q, const int* from, const int* to, const int* count, int n, int n_pages, int* status,
                       cudaStream_t s) {
   if (n == 0) return HOA_OK;
-  for (int k0 = 0; k0 < n_pools; k0 += kMaxPools) {
-    PgCopyArgs a{};
-    a.pools = n_pools - k0 < kMaxPools ? n_pools - k0 : kMaxPools;
-    a.from = from; a.to = to; a.count = count; a.n = n; a.n_pages = n_pages; a.status = status;
-    unsigned long long bits = 0;                   // alignment of everything a copy touches
-    long long most = 0;
-    for (int k = 0; k < a.pools; ++k) {
-      a.base[k] = static_cast<uint8_t*>(pools[k0 + k]);
-      a.stride[k] = strides[k0 + k];
-      a.bytes[k] = bytes[k0 + k];
-      bits |= (unsigned long long)reinterpret_cast<uintptr_t>(pools[k0 + k]) | (unsigned long long)a.stride[k] |
-              (unsigned long long)a.bytes[k];
-      if (a.bytes[k] > most) most = a.bytes[k];
-    }
+  for (int k0 = 0; k0 < q.n; k0 += kMaxPools) {
+    unsigned long long bits;
+    long long most;
+    const PgCopyArgs a = copy_args(q, k0, from, to, count, n, n_pages, status, &bits, &most);
     const int st = (bits & 15) == 0 ? launch_copy<uint4>(a, most, s)
                  : (bits & 3) == 0 ? launch_copy<uint32_t>(a, most, s)
                  : (bits & 1) == 0 ? launch_copy<uint16_t>(a, most, s) : launch_copy<uint8_t>(a, most, s);
@@ -486,7 +528,7 @@ extern "C" int hoa_pages_reserve(const int* table, const int* lens, const int* r
   int* ws = static_cast<int*>(workspace);
   PgTakeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page},
                counts, nullptr, S, ws, ws + S, nullptr, nullptr, status};
-  pages_take_kernel<false><<<kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+  pages_take_kernel<false><<<kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, PgCopyArgs{});
   return launch_status();
 }
 
@@ -504,10 +546,12 @@ extern "C" int hoa_pages_fork(const int* table, const int* lens, const int* refs
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   PgTakeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page},
                src, dst, n, ws, ws + 3 * (size_t)n, from, to, status};
-  pages_take_kernel<true><<<kPgCluster, kPgThreads, 0, s>>>(a);
+  const PgPools q{pools, strides, bytes, n_pools};
+  const PgCopyArgs cp = inline_copy(q, from, to, n, n_pages, status);
+  pages_take_kernel<true><<<kPgCluster, kPgThreads, 0, s>>>(a, cp);
   const int st = launch_status();
-  if (st != HOA_OK) return st;
-  return copy_pools(pools, strides, bytes, n_pools, from, to, nullptr, n, n_pages, status, s);
+  if (st != HOA_OK || cp.n > 0) return st;
+  return copy_pools(q, from, to, nullptr, n, n_pages, status, s);
 }
 
 extern "C" int hoa_pages_free(const int* table, const int* lens, const int* refs, const int* rows, int n, int* table_out,
@@ -533,18 +577,20 @@ extern "C" int hoa_pages_compact(const int* table, const int* refs, int* table_o
   int *from = ws, *to = ws + n_pages, *remap = ws + 2 * (size_t)n_pages, *moves = ws + 3 * (size_t)n_pages;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   PgCompactArgs a{{table, nullptr, refs, table_out, nullptr, refs_out, S, W, n_pages, 1}, live, remap, from, to, moves, status};
-  pages_compact_kernel<<<kPgCluster, kPgThreads, 0, s>>>(a);
-  const int st = launch_status();
-  if (st != HOA_OK) return st;
   // at most half of the pages move: a mover needs a hole below it
-  return copy_pools(pools, strides, bytes, n_pools, from, to, moves, n_pages / 2, n_pages, status, s);
+  const PgPools q{pools, strides, bytes, n_pools};
+  const PgCopyArgs cp = inline_copy(q, from, to, n_pages / 2, n_pages, status);
+  pages_compact_kernel<<<kPgCluster, kPgThreads, 0, s>>>(a, cp);
+  const int st = launch_status();
+  if (st != HOA_OK || cp.n > 0) return st;
+  return copy_pools(q, from, to, moves, n_pages / 2, n_pages, status, s);
 }
 
 extern "C" int hoa_pages_copy(void* const* pools, const long long* strides, const long long* bytes, int n_pools,
                               const int* from, const int* to, int n, int n_pages, int* status, void* stream) {
   if (n < 0 || n_pools < 0 || n_pages < 1 || (n > 0 && (!from || !to)) || (n_pools > 0 && (!pools || !strides || !bytes)))
     return HOA_ERR_INVALID_ARG;
-  return copy_pools(pools, strides, bytes, n_pools, from, to, nullptr, n, n_pages, status,
+  return copy_pools(PgPools{pools, strides, bytes, n_pools}, from, to, nullptr, n, n_pages, status,
                     reinterpret_cast<cudaStream_t>(stream));
 }
 

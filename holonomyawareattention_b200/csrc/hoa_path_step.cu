@@ -653,8 +653,8 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
 template <int DP, int V>
 static int launch_step_v(const StepArgs& s, int num_sms, cudaStream_t stream) {
   using L = StLayout<DP>;
-  if (cudaFuncSetAttribute(path_step_kernel<DP, V>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc) != cudaSuccess)
-    return HOA_ERR_LAUNCH;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(path_step_kernel<DP, V>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
   const int units = s.B * s.H;
   path_step_kernel<DP, V><<<(unsigned)(units < 2 * num_sms ? units : 2 * num_sms), kStThreads, L::kAlloc, stream>>>(s);
   return launch_status();
