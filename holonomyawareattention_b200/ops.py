@@ -692,6 +692,27 @@ def _run(idx: int, name: str, *args) -> None:
         _lib.check(name, st)
 
 
+# Scratch of these calls, one buffer a device and stream: calls on a stream run in order, so they can share
+# it.  Large ones, and calls under graph capture (whose memory belongs to the graph), allocate their own.
+_SCRATCH = {}
+_SCRATCH_MOST = 32 << 20
+
+
+def _scratch(idx: int, n: int):
+    """(address of n bytes of scratch on device idx's current stream, what keeps them alive)."""
+    if n <= _SCRATCH_MOST and not torch._C._cuda_isCurrentStreamCapturing():
+        key = idx, torch._C._cuda_getCurrentRawStream(idx)
+        v = _SCRATCH.get(key)
+        if v is None or v[2] < n:
+            # the old buffer may still be in use on its stream: the allocator hands it out again in stream order
+            with torch.inference_mode(False):
+                t = torch.empty(max(n, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", idx))
+            v = _SCRATCH[key] = (t.data_ptr(), t, t.numel())
+        return v
+    t = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", idx))
+    return t.data_ptr(), t, n
+
+
 def _longs(*values):
     """A host array of 64-bit integers (strides, addresses) for a call."""
     n = len(values)
@@ -761,9 +782,9 @@ def pages_reserve(table, lens, refs, counts, page: int):
     _ints(counts, "counts", (S,), idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
     n = _bytes_of("hoa_pages_workspace_bytes", S, n_pages)
-    ws = torch.empty(n, dtype=torch.uint8, device=table.device)
+    ws = _scratch(idx, n)
     _run(idx, "hoa_pages_reserve", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), counts.data_ptr(), out[0].data_ptr(),
-         out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, ws.data_ptr(), n)
+         out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, ws[0], n)
     return out
 
 
@@ -782,9 +803,9 @@ def pages_fork(pools, table, lens, refs, src, dst, page: int):
     _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
     nb = _bytes_of("hoa_pages_workspace_bytes", n, n_pages)
-    ws = torch.empty(nb, dtype=torch.uint8, device=table.device)
+    ws = _scratch(idx, nb)
     _run(idx, "hoa_pages_fork", table.data_ptr(), lens.data_ptr(), refs.data_ptr(), src.data_ptr(), dst.data_ptr(), n,
-         out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, base, stride, size, np_, ws.data_ptr(), nb)
+         out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), S, W, n_pages, page, base, stride, size, np_, ws[0], nb)
     return out
 
 
@@ -807,11 +828,11 @@ def pages_compact(pools, table, refs):
     idx, S, W, n_pages = _books(table, None, refs, 1)
     _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
     table2, refs2 = torch.empty_like(table), torch.empty_like(refs)
-    live = torch.empty(1, dtype=_INT, device=table.device)
+    live = refs.new_empty(1)
     nb = _bytes_of("hoa_pages_workspace_bytes", 0, n_pages)
-    ws = torch.empty(nb, dtype=torch.uint8, device=table.device)
+    ws = _scratch(idx, nb)
     _run(idx, "hoa_pages_compact", table.data_ptr(), refs.data_ptr(), table2.data_ptr(), refs2.data_ptr(), live.data_ptr(),
-         S, W, n_pages, base, stride, size, np_, ws.data_ptr(), nb)
+         S, W, n_pages, base, stride, size, np_, ws[0], nb)
     return table2, refs2, live
 
 
@@ -903,14 +924,16 @@ def paged_attn_fwd(q, k_pages, v_pages, table, lens, softmax_scale: float, share
     out_dtype = out_dtype or q.dtype
     sms = _device(idx)[0]
     nb = _bytes_of("hoa_paged_attn_workspace_bytes", B, Tq, H, Hk, d, page, n_shared, W, sms)
-    dev = q.device
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    out = torch.empty((B, Tq, H, d), dtype=out_dtype, device=dev)
-    lse = torch.empty((B, Tq, H), dtype=torch.float32, device=dev)
+    ws = _scratch(idx, nb)
+    if out_dtype is q.dtype:
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, Tq, H, d))
+    else:
+        out = q.new_empty((B, Tq, H, d), dtype=out_dtype)
+    lse = q.new_empty((B, Tq, H), dtype=torch.float32)
     _run(idx, "hoa_paged_attn_fwd", q.data_ptr(), _longs(*qs[:3]), k_pages.data_ptr(), v_pages.data_ptr(), ps, code,
          shared.data_ptr() if n_shared else None, n_shared, table.data_ptr(), tw, W, lens.data_ptr(),
          paths.data_ptr() if paths is not None else None, out.data_ptr(), _dtype_code(out_dtype), lse.data_ptr(),
-         softmax_scale, B, Tq, H, Hk, d, page, n_pages, sms, ws.data_ptr(), nb)
+         softmax_scale, B, Tq, H, Hk, d, page, n_pages, sms, ws[0], nb)
     return out, lse
 
 
@@ -954,16 +977,16 @@ def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, tabl
             _index(a_bias)
             raise ValueError(f"a_bias must be on cuda:{idx}")
     shape = (B, H, d, d)
+    _path(P, "P", shape, idx)
     if P_out is None:
-        P_out = torch.empty(shape, dtype=torch.float32, device=qkv.device)
+        P_out = torch.empty_like(P)
     else:
         _path(P_out, "P_out", shape, idx)
-    _path(P, "P", shape, idx)
     W, tw = _row_table(table, B, idx)
     if W == 0:
         raise ValueError("table must have at least one page a row")
     _ints(lens, "lens", (B,), idx)
-    qh = torch.empty((B, H, d), dtype=k_pages.dtype, device=qkv.device)
+    qh = k_pages.new_empty((B, H, d))
     _run(idx, "hoa_path_step", a.data_ptr(), a_code, a_bias.data_ptr() if a_bias is not None else None, edge_scale,
          P.data_ptr(), P_out.data_ptr(), qkv.data_ptr(), _dtype_code(qkv.dtype), qkv.stride(0), qh.data_ptr(),
          k_pages.data_ptr(), v_pages.data_ptr(), code, ps, table.data_ptr(), tw, W, lens.data_ptr(), B, H, d, page, n_pages)
