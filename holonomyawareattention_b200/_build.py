@@ -8,7 +8,9 @@ ranges of its global accesses and records HOA_ERR_BOUNDS (read through
 hoa_debug_bounds) for a range outside its buffer, skipping that access.
 
 The library exposes only the C ABI declared in include/hoa.h (no torch types),
-so it can be bound from ctypes, cgo, JNI or C/C++ alike.
+so it can be bound from ctypes, cgo, JNI or C/C++ alike.  Beside it, the host
+compiler makes _hoa_torch.so (csrc/hoa_torch.cpp): the ordinary case of the
+generation operators' Python side, in C++ against torch's headers.
 """
 from __future__ import annotations
 
@@ -25,6 +27,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhoa.so")
 BUILD_DIR = os.path.join(PKG, "_build")
+LIB_TORCH = os.path.join(PKG, "_hoa_torch.so")
 LIB_DEBUG = os.path.join(PKG, "libhoa_debug.so")
 BUILD_DIR_DEBUG = os.path.join(PKG, "_build", "debug_bounds")
 
@@ -62,6 +65,8 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), debug_boun
     build_dir = BUILD_DIR_DEBUG if debug_bounds else BUILD_DIR
     if debug_bounds:
         extra_flags = (*extra_flags, "-DHOA_DEBUG_BOUNDS")
+    if not debug_bounds:
+        build_torch(force)
     if not force and up_to_date(lib):
         return lib
     nvcc = nvcc_path()
@@ -91,6 +96,31 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), debug_boun
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, lib)
     return lib
+
+
+def build_torch(force: bool = False) -> str:
+    """_hoa_torch.so, against the torch that is importable here."""
+    src = os.path.join(CSRC, "hoa_torch.cpp")
+    if not force and os.path.exists(LIB_TORCH) and \
+            all(os.path.getmtime(p) <= os.path.getmtime(LIB_TORCH) for p in (src, os.path.join(INCLUDE, "hoa.h"))):
+        return LIB_TORCH
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = os.path.join(root, "include")
+    cuda_inc = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    tmp = LIB_TORCH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"), "-isystem", cuda_inc,
+           "-isystem", sysconfig.get_paths()["include"], src, "-o", tmp, "-L", os.path.join(root, "lib"), "-ltorch", "-ltorch_cpu",
+           "-ltorch_python", "-lc10", "-lc10_cuda", f"-Wl,-rpath,{os.path.join(root, 'lib')}",
+           "-L", os.path.join(os.path.dirname(cuda_inc), "lib64"), "-lcudart", f"-Wl,-rpath,{os.path.join(os.path.dirname(cuda_inc), 'lib64')}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the host compiler failed on {src}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, LIB_TORCH)
+    return LIB_TORCH
 
 
 def main(argv=None):

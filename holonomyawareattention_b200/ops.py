@@ -656,11 +656,39 @@ def _fn(name: str):
     return f
 
 
+# The ordinary case of these functions in C++ (csrc/hoa_torch.cpp): each tries it first; None means that
+# the call is not ordinary (another device, an option, a mistake) and that the code below takes it.
+_HOST = None
+_HOST_FNS = ("hoa_pages_workspace_bytes", "hoa_pages_reserve", "hoa_pages_fork", "hoa_pages_free", "hoa_pages_compact",
+             "hoa_paged_attn_workspace_bytes", "hoa_paged_attn_fwd", "hoa_path_step")
+
+
+def _host():
+    global _HOST
+    if _HOST is None:
+        try:
+            from . import _hoa_torch as m
+        except ImportError as e:
+            raise RuntimeError(f"_hoa_torch.so cannot be loaded ({e}): build it with "
+                               "`python -m holonomyawareattention_b200._build`") from None
+        m.bind(*(ctypes.cast(_fn(n), ctypes.c_void_p).value for n in _HOST_FNS))
+        _HOST = m
+    return _HOST
+
+
+def _done(name: str, r):
+    """What the C++ side returned: the outputs, or a status to raise."""
+    if type(r) is int:
+        _lib.check(name, r)
+    return r
+
+
 def _device(idx: int):
     v = _DEVICES.get(idx)
     if v is None:
         v = _DEVICES[idx] = (torch.cuda.get_device_properties(idx).multi_processor_count,
                              _watch(torch.device("cuda", idx)).mapped_ptr)
+        _host().device(idx, *v)
     return v
 
 
@@ -778,6 +806,9 @@ def pages_reserve(table, lens, refs, counts, page: int):
     table (S, W), lens (S,), refs (n_pages,), counts (S,): int32.  Free pages (refs == 0) are taken
     lowest index first, rows in order.  Without enough of them, or where a row would pass W pages, the
     state comes back unchanged and HOA_ERR_PAGES is reported (hoa_pages_reserve)."""
+    r = (_HOST or _host()).pages_reserve(table, lens, refs, counts, page)
+    if r is not None:
+        return _done("hoa_pages_reserve", r)
     idx, S, W, n_pages = _books(table, lens, refs, page)
     _ints(counts, "counts", (S,), idx)
     out = torch.empty_like(table), torch.empty_like(lens), torch.empty_like(refs)
@@ -794,6 +825,9 @@ def pages_fork(pools, table, lens, refs, src, dst, page: int):
     src, dst (n,) int32; the dst rows are empty and differ.  Full pages are shared; a last page that
     is not full is copied, in every pool (n_pages, ...) of ``pools``, to a page of its own.  All or
     nothing, as pages_reserve (hoa_pages_fork)."""
+    r = (_HOST or _host()).pages_fork(pools, table, lens, refs, src, dst, page)
+    if r is not None:
+        return _done("hoa_pages_fork", r)
     idx, S, W, n_pages = _books(table, lens, refs, page)
     n = src.numel()
     _ints(src, "src", (n,), idx)
@@ -812,6 +846,9 @@ def pages_fork(pools, table, lens, refs, src, dst, page: int):
 def pages_free(table, lens, refs, rows, page: int):
     """The rows (n,) int32 end: (table, lens, refs); a page that no row holds any more is free
     (hoa_pages_free)."""
+    r = (_HOST or _host()).pages_free(table, lens, refs, rows, page)
+    if r is not None:
+        return _done("hoa_pages_free", r)
     idx, S, W, n_pages = _books(table, lens, refs, page)
     n = rows.numel()
     _ints(rows, "rows", (n,), idx)
@@ -825,6 +862,9 @@ def pages_compact(pools, table, refs):
     """The live pages move to 0 .. live-1 in every pool: (table, refs, live (1,)).
 
     The i-th free page below ``live`` receives the i-th live page at or above it (hoa_pages_compact)."""
+    r = (_HOST or _host()).pages_compact(pools, table, refs)
+    if r is not None:
+        return _done("hoa_pages_compact", r)
     idx, S, W, n_pages = _books(table, None, refs, 1)
     _keep, base, stride, size, np_ = _pool_args(pools, n_pages, idx)
     table2, refs2 = torch.empty_like(table), torch.empty_like(refs)
@@ -901,6 +941,10 @@ def paged_attn_fwd(q, k_pages, v_pages, table, lens, softmax_scale: float, share
     all keys of a row, the shared ones and its Tq newest included.  Query t sees the keys at positions
     0 .. lens[b] - Tq + t; one that sees none gives 0 and lse -inf.  ``paths`` (B, H, d, d) fp32 with
     Tq = 1: out = P o.  hoa_paged_attn_fwd."""
+    if out_dtype is None or out_dtype is q.dtype:
+        r = (_HOST or _host()).paged_attn_fwd(q, k_pages, v_pages, table, lens, softmax_scale, shared, paths)
+        if r is not None:
+            return _done("hoa_paged_attn_fwd", r)
     idx = _index(q)
     if q.dim() != 4 or q.numel() == 0:
         raise ValueError("q must be (B, Tq, H, d), not empty")
@@ -952,6 +996,10 @@ def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, tabl
     lens[b] - 1 of the row's pages (table (B, W), lens (B,) with the token counted; reserve it first).
     qkv (B, 3D) holds [q | k | v] per head.  lens 1: no edge, P' = I.  lens 0: P' = P, q^ = 0, nothing
     written.  ``P_out`` may be P.  hoa_path_step."""
+    if a_bias is None and gen_layout == "packed":
+        r = (_HOST or _host()).path_step(a, P, qkv, n_heads, edge_scale, k_pages, v_pages, table, lens, P_out)
+        if r is not None:
+            return _done("hoa_path_step", r)
     idx = _index(qkv)
     H = n_heads
     n_pages, Hk, page, d, code, ps = _cache(k_pages, v_pages, idx)
