@@ -90,6 +90,34 @@ inline bool allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& 
   return true;
 }
 
+// Programmatic dependent launch.  A kernel launched with launch_early may come up while the one before it in the
+// stream drains: its CTAs are placed and set themselves up, and wait_previous() returns once all work before it has
+// completed and is visible.  Every such kernel waits before it touches global memory, so nothing but its start moves;
+// back to back, small kernels otherwise leave about two microseconds between them.  let_next_start() (after the wait)
+// lets the next launch of the same call come up at once.
+HOA_DEVICE void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+HOA_DEVICE void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class K, class... A>
+inline int launch_early(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t smem, cudaStream_t s,
+                        const A&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(grid);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = s;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
+  return e == cudaSuccess ? launch_status() : (cudaGetLastError(), (int)HOA_ERR_LAUNCH);
+}
+
 // Smallest supported padded head dimension >= d, or 0.
 inline int padded_dim(int d) {
   static const int dims[] = {8, 16, 32, 48, 64, 96, 120};

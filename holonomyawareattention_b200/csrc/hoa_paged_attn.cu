@@ -34,7 +34,7 @@ template <int R, bool V4>
 __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   constexpr int RT = 8 * R;
   extern __shared__ float sm[];
-  pa_let_next_start();
+  pa_begin(p.leads);
   const int d = p.d, ld = ps_ld(d), d4 = (d + 3) / 4;
   float* Qs = sm;                                      // [RT][ld]
   float* Ks = Qs + RT * ld;                            // [64][ld]
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __gri
   for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
-  pa_end_after_previous();
+  wait_previous();
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (!my[i].ok) continue;
@@ -198,21 +198,21 @@ __global__ void __launch_bounds__(kPsThreads) paged_attn_simt_kernel(const __gri
 }
 
 template <int R, bool V4>
-static int launch_simt(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+static int launch_simt(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
   const int ld = ((a.d + 3) / 4 | 1) * 4;
   const size_t smem = ((8 * R + 2 * kPsKeys) * (size_t)ld + 8 * R * 68) * sizeof(float);
   static std::atomic<unsigned long long> done{0};
   const size_t most = ((8 * R + 2 * kPsKeys) * (size_t)132 + 8 * R * 68) * sizeof(float);   // at d = 128
   if (!allow_smem(paged_attn_simt_kernel<R, V4>, most, done)) return HOA_ERR_LAUNCH;
-  return pa_launch(paged_attn_simt_kernel<R, V4>, items, kPsThreads, smem, s, early, a, first);
+  return launch_early(paged_attn_simt_kernel<R, V4>, items, 1, kPsThreads, smem, s, a, first);
 }
 
-static int paged_attn_simt(const PaArgs& a, int tile_rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
+static int paged_attn_simt(const PaArgs& a, int tile_rows, unsigned first, unsigned items, cudaStream_t s) {
   const bool v4 = a.dtype == HOA_F32 && a.d % 4 == 0 &&
                   ((reinterpret_cast<uintptr_t>(a.kp) | reinterpret_cast<uintptr_t>(a.vp) | (uintptr_t)(a.ps * 4) |
                     (uintptr_t)(a.hs * 4) | (uintptr_t)(a.ts * 4)) & 15) == 0;
-  if (tile_rows == 32) return v4 ? launch_simt<4, true>(a, first, items, early, s) : launch_simt<4, false>(a, first, items, early, s);
-  return v4 ? launch_simt<2, true>(a, first, items, early, s) : launch_simt<2, false>(a, first, items, early, s);
+  if (tile_rows == 32) return v4 ? launch_simt<4, true>(a, first, items, s) : launch_simt<4, false>(a, first, items, s);
+  return v4 ? launch_simt<2, true>(a, first, items, s) : launch_simt<2, false>(a, first, items, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -227,7 +227,7 @@ template <int CH, int NR>
 __global__ void __launch_bounds__(kPvThreads) paged_attn_vec_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   __shared__ float s_o[4][NR][32 * CH];
   __shared__ float2 s_ml[4][NR];
-  pa_let_next_start();
+  pa_begin(p.leads);
   const PaItem it = pa_item(p, first + blockIdx.x, NR, 16);
   const int warp = threadIdx.x >> 5, lid = threadIdx.x & 31, gl = lid & 7, g = lid >> 3, d = p.d;
   const float* q = static_cast<const float*>(p.q);
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kPvThreads) paged_attn_vec_kernel(const __grid
     }
     if (lid == 0) s_ml[warp][r] = make_float2(mx, l[r]);
   }
-  pa_end_after_previous();
+  wait_previous();
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
@@ -341,18 +341,18 @@ __global__ void __launch_bounds__(kPvThreads) paged_attn_vec_kernel(const __grid
 }
 
 template <int CH>
-static int launch_vec(const PaArgs& a, int rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
-  if (rows == 1) return pa_launch(paged_attn_vec_kernel<CH, 1>, items, kPvThreads, 0, s, early, a, first);
-  if (rows == 2) return pa_launch(paged_attn_vec_kernel<CH, 2>, items, kPvThreads, 0, s, early, a, first);
-  return pa_launch(paged_attn_vec_kernel<CH, 4>, items, kPvThreads, 0, s, early, a, first);
+static int launch_vec(const PaArgs& a, int rows, unsigned first, unsigned items, cudaStream_t s) {
+  if (rows == 1) return launch_early(paged_attn_vec_kernel<CH, 1>, items, 1, kPvThreads, 0, s, a, first);
+  if (rows == 2) return launch_early(paged_attn_vec_kernel<CH, 2>, items, 1, kPvThreads, 0, s, a, first);
+  return launch_early(paged_attn_vec_kernel<CH, 4>, items, 1, kPvThreads, 0, s, a, first);
 }
 
-static int paged_attn_vec(const PaArgs& a, int rows, unsigned first, unsigned items, bool early, cudaStream_t s) {
+static int paged_attn_vec(const PaArgs& a, int rows, unsigned first, unsigned items, cudaStream_t s) {
   switch ((a.d + 31) / 32) {
-    case 1: return launch_vec<1>(a, rows, first, items, early, s);
-    case 2: return launch_vec<2>(a, rows, first, items, early, s);
-    case 3: return launch_vec<3>(a, rows, first, items, early, s);
-    default: return launch_vec<4>(a, rows, first, items, early, s);
+    case 1: return launch_vec<1>(a, rows, first, items, s);
+    case 2: return launch_vec<2>(a, rows, first, items, s);
+    case 3: return launch_vec<3>(a, rows, first, items, s);
+    default: return launch_vec<4>(a, rows, first, items, s);
   }
 }
 
@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
   const int d = p.d, slots = p.ns1 + p.ns2, warp = threadIdx.x >> 5, lid = threadIdx.x & 31;
   const int w = warp % kWpr;
   const long long g = (long long)blockIdx.x * (8 / kWpr) + warp / kWpr;
+  if (p.leads) wait_previous();                        // (a call without items: nothing before it has waited for P)
   const bool ok = g < p.rows;                          // (uniform in the warps that share a row)
   float4 P[4][4];                                      // pass, chunk of 4 columns
   const int pr = threadIdx.x >> 3, pq = threadIdx.x & 7;
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
         }
       }
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!p.leads) wait_previous();
   float m = -INFINITY;
   if (ok)
     for (int s = lid; s < slots; s += 32) {
@@ -490,20 +491,20 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
 }
 
 template <int V, int kWpr, bool kPaths>
-static int launch_join(const PaArgs& a, bool early, cudaStream_t s) {
+static int launch_join(const PaArgs& a, cudaStream_t s) {
   const long long blocks = (a.rows + 8 / kWpr - 1) / (8 / kWpr);
   if (blocks > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;
-  return pa_launch(paged_attn_join_kernel<V, kWpr, kPaths>, (unsigned)blocks, kPjThreads, 0, s, early, a);
+  return launch_early(paged_attn_join_kernel<V, kWpr, kPaths>, (unsigned)blocks, 1, kPjThreads, 0, s, a);
 }
 
-static int join(const PaArgs& a, bool early, cudaStream_t s) {
+static int join(const PaArgs& a, cudaStream_t s) {
   // 16-byte accesses: four columns a lane of o, the parts and P
   const bool v4 = a.d % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.paths) |
                                     reinterpret_cast<uintptr_t>(a.part_o)) & 15) == 0;
-  if (a.paths) return v4 ? launch_join<4, 8, true>(a, early, s) : launch_join<1, 8, true>(a, early, s);
+  if (a.paths) return v4 ? launch_join<4, 8, true>(a, s) : launch_join<1, 8, true>(a, s);
   // eight warps a row where one a row would leave SMs without work and there are parts to share
-  if (a.rows < 148 * 16 && a.ns1 + a.ns2 > 4) return v4 ? launch_join<4, 8, false>(a, early, s) : launch_join<1, 8, false>(a, early, s);
-  return v4 ? launch_join<4, 1, false>(a, early, s) : launch_join<1, 1, false>(a, early, s);
+  if (a.rows < 148 * 16 && a.ns1 + a.ns2 > 4) return v4 ? launch_join<4, 8, false>(a, s) : launch_join<1, 8, false>(a, s);
+  return v4 ? launch_join<4, 1, false>(a, s) : launch_join<1, 1, false>(a, s);
 }
 
 }  // namespace hoa
@@ -530,13 +531,12 @@ extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, i
   return most;
 }
 
-// `early`: may start while the launch before it (the other part's items) still runs
-static int run_items(int kind, const PaArgs& a, long long first, long long items, bool early, cudaStream_t s) {
+static int run_items(int kind, const PaArgs& a, long long first, long long items, cudaStream_t s) {
   if (items == 0) return HOA_OK;
-  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, early, s);
-  if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, early, s);
-  if (kind < kPaSimt) return paged_attn_vec(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, early, s);
-  return paged_attn_simt(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, early, s);
+  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, s);
+  if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, s);
+  if (kind < kPaSimt) return paged_attn_vec(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, s);
+  return paged_attn_simt(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, s);
 }
 
 extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -579,16 +579,19 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
   a.page_shift = sh - 1;
   a.ns1 = pl.ns1; a.ns2 = pl.ns2; a.tiles1 = pl.tiles1; a.tiles2 = pl.tiles2;
   a.status = status;
+  a.leads = 1;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)(pl.ns1 + pl.ns2) * a.rows * d);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int st;
   if (pl.kind1 == pl.kind2) {                      // one launch for both parts
-    st = run_items(pl.kind1, a, 0, items1 + items2, false, s);
+    st = run_items(pl.kind1, a, 0, items1 + items2, s);
   } else {
-    st = run_items(pl.kind1, a, 0, items1, false, s);
-    if (st == HOA_OK) st = run_items(pl.kind2, a, items1, items2, items1 > 0, s);
+    st = run_items(pl.kind1, a, 0, items1, s);
+    a.leads = items1 == 0;
+    if (st == HOA_OK) st = run_items(pl.kind2, a, items1, items2, s);
   }
   if (st != HOA_OK) return st;
-  return join(a, items1 + items2 > 0, s);
+  a.leads = items1 + items2 == 0;
+  return join(a, s);
 }

@@ -23,6 +23,7 @@ struct PaArgs {
   int dtype, B, Tq, H, Hk, G, d, page, n_pages;
   unsigned page_mul; int page_shift;               // j / page = umulhi(j, page_mul) >> page_shift for 0 <= j < 2^31 (page > 1)
   int tiles1, ns1, tiles2, ns2;
+  int leads;                                       // this launch is the first of the call
   int* status;
 };
 
@@ -192,31 +193,17 @@ HOA_DEVICE long long pa_key(const PaArgs& p, const PaItem& it, int j) {
   return id * p.ps + it.kvh * p.hs + (long long)(j - pg * p.page) * p.ts;
 }
 
-// The launches of a call overlap (programmatic dependent launch): the items of part 2 may run beside those of
-// part 1, and the join comes up while the last items run.  Every kernel lets the next one start at once, and waits
-// for the one before it at its own end at the latest, so that a kernel has completed only after all before it have:
-// the join's wait then covers both.  The first launch of a call is an ordinary one.
-HOA_DEVICE void pa_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-HOA_DEVICE void pa_end_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <class K, class... A>
-static int pa_launch(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t s, bool early, const A&... args) {
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(grid);
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &at;
-  c.numAttrs = early ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, args...);
-  return e == cudaSuccess ? launch_status() : (cudaGetLastError(), (int)HOA_ERR_LAUNCH);
+// The launches of a call overlap (launch_early).  The first one waits for the work before the call and then lets the
+// next start; the items of part 2 may so run beside those of part 1, and the join comes up while the last items run.
+// Each later launch waits for the one before it at its own end at the latest, so that a kernel has completed only
+// after all before it have: the join's wait covers both.  `leads`: the first launch of a call.
+HOA_DEVICE void pa_begin(bool leads) {
+  if (leads) wait_previous();
+  let_next_start();
 }
 
 // items first .. first + items - 1
-int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s);
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s);
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
+int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
 
 }  // namespace hoa

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kPmWarps * 32, PmCfg<D8>::kMinBlocks)
 paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
   using C = PmCfg<D8>;
   extern __shared__ __align__(16) uint8_t smem[];
-  pa_let_next_start();
+  pa_begin(p.leads);
   PaItem it = pa_item(p, first + blockIdx.x, 16, kPmKeys);
   const int tid = threadIdx.x, w = tid >> 5, lid = tid & 31, r0 = lid >> 2, q2 = (lid & 3) * 2;
   const uint32_t ring = sm100::smem_u32(smem) + w * C::kWarp;
@@ -260,7 +260,7 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
     for (int h = 0; h < 2; ++h) l[h] += __shfl_xor_sync(0xffffffffu, l[h], k);
 
   // ---- join the warps
-  pa_end_after_previous();
+  wait_previous();
   cp_wait<0>();
   __syncthreads();
   float* jn = reinterpret_cast<float*>(smem);
@@ -310,39 +310,39 @@ paged_attn_mma_kernel(const __grid_constant__ PaArgs p, unsigned first) {
 }
 
 template <int D8, bool kHalf>
-static int launch_mma_h(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+static int launch_mma_h(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
   using C = PmCfg<D8>;
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(paged_attn_mma_kernel<D8, kHalf>, C::kSmem, done)) return HOA_ERR_LAUNCH;
-  return pa_launch(paged_attn_mma_kernel<D8, kHalf>, items, kPmWarps * 32, C::kSmem, s, early, a, first);
+  return launch_early(paged_attn_mma_kernel<D8, kHalf>, items, 1, kPmWarps * 32, C::kSmem, s, a, first);
 }
 
 template <int D8>
-static int launch_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+static int launch_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
   // the rows of an item: of the whole batch where the launch has items of part 1
   const bool part1 = first < (unsigned)a.tiles1 * a.Hk * a.ns1;
   const long long rows = (part1 ? a.B : 1) * (long long)a.Tq * a.G;
-  return rows <= 8 ? launch_mma_h<D8, true>(a, first, items, early, s) : launch_mma_h<D8, false>(a, first, items, early, s);
+  return rows <= 8 ? launch_mma_h<D8, true>(a, first, items, s) : launch_mma_h<D8, false>(a, first, items, s);
 }
 
-int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
   switch (a.d / 8) {
-    case 1: return launch_mma<1>(a, first, items, early, s);
-    case 2: return launch_mma<2>(a, first, items, early, s);
-    case 3: return launch_mma<3>(a, first, items, early, s);
-    case 4: return launch_mma<4>(a, first, items, early, s);
-    case 5: return launch_mma<5>(a, first, items, early, s);
-    case 6: return launch_mma<6>(a, first, items, early, s);
-    case 7: return launch_mma<7>(a, first, items, early, s);
-    case 8: return launch_mma<8>(a, first, items, early, s);
-    case 9: return launch_mma<9>(a, first, items, early, s);
-    case 10: return launch_mma<10>(a, first, items, early, s);
-    case 11: return launch_mma<11>(a, first, items, early, s);
-    case 12: return launch_mma<12>(a, first, items, early, s);
-    case 13: return launch_mma<13>(a, first, items, early, s);
-    case 14: return launch_mma<14>(a, first, items, early, s);
-    case 15: return launch_mma<15>(a, first, items, early, s);
-    case 16: return launch_mma<16>(a, first, items, early, s);
+    case 1: return launch_mma<1>(a, first, items, s);
+    case 2: return launch_mma<2>(a, first, items, s);
+    case 3: return launch_mma<3>(a, first, items, s);
+    case 4: return launch_mma<4>(a, first, items, s);
+    case 5: return launch_mma<5>(a, first, items, s);
+    case 6: return launch_mma<6>(a, first, items, s);
+    case 7: return launch_mma<7>(a, first, items, s);
+    case 8: return launch_mma<8>(a, first, items, s);
+    case 9: return launch_mma<9>(a, first, items, s);
+    case 10: return launch_mma<10>(a, first, items, s);
+    case 11: return launch_mma<11>(a, first, items, s);
+    case 12: return launch_mma<12>(a, first, items, s);
+    case 13: return launch_mma<13>(a, first, items, s);
+    case 14: return launch_mma<14>(a, first, items, s);
+    case 15: return launch_mma<15>(a, first, items, s);
+    case 16: return launch_mma<16>(a, first, items, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
 }

@@ -85,10 +85,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
   volatile int* s_abort = reinterpret_cast<volatile int*>(bars + 25);
   int* s_seen = reinterpret_cast<int*>(bars + 26);   // [2] the last key that a row of the tile sees, + 1
 
-  pa_let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int KT = pt.kt;
-  const PaItem it = pa_item(p, first + blockIdx.x, 256, KT);
   if (tid == 0) {
     mbar_init(q_full, 8);
     for (int i = 0; i < 2; ++i) {
@@ -111,6 +109,8 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  pa_begin(p.leads);
+  const PaItem it = pa_item(p, first + blockIdx.x, 256, KT);
   __syncthreads();
   PaRow my{};
   int seen = 0;
@@ -367,7 +367,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     }
   }
 
-  pa_end_after_previous();
+  wait_previous();
   bad = __syncthreads_or(bad || *s_abort != 0);
   if (bad && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
@@ -407,14 +407,14 @@ static bool page_map(CUtensorMap* m, const void* base, const PaArgs& a, int box)
 
 template <int DP16>
 static int launch_ptc(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, unsigned first,
-                      unsigned items, bool early, cudaStream_t s) {
+                      unsigned items, cudaStream_t s) {
   using L = PtLayout<DP16>;
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(paged_attn_tc_kernel<DP16>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
-  return pa_launch(paged_attn_tc_kernel<DP16>, items, kPtThreads, L::kAlloc, s, early, mk, mv, a, t, first);
+  return launch_early(paged_attn_tc_kernel<DP16>, items, 1, kPtThreads, L::kAlloc, s, mk, mv, a, t, first);
 }
 
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, bool early, cudaStream_t s) {
+int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
   PtArgs t;
   t.kt = pa_tile_keys(a.page);
   t.box = a.page < t.kt ? a.page : t.kt;
@@ -423,14 +423,14 @@ int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, bool early, c
   CUtensorMap mk, mv;
   if (t.kt == 0 || !page_map(&mk, a.kp, a, t.box) || !page_map(&mv, a.vp, a, t.box)) return HOA_ERR_INVALID_ARG;
   switch ((a.d + 15) / 16) {
-    case 1: return launch_ptc<16>(mk, mv, a, t, first, items, early, s);
-    case 2: return launch_ptc<32>(mk, mv, a, t, first, items, early, s);
-    case 3: return launch_ptc<48>(mk, mv, a, t, first, items, early, s);
-    case 4: return launch_ptc<64>(mk, mv, a, t, first, items, early, s);
-    case 5: return launch_ptc<80>(mk, mv, a, t, first, items, early, s);
-    case 6: return launch_ptc<96>(mk, mv, a, t, first, items, early, s);
-    case 7: return launch_ptc<112>(mk, mv, a, t, first, items, early, s);
-    case 8: return launch_ptc<128>(mk, mv, a, t, first, items, early, s);
+    case 1: return launch_ptc<16>(mk, mv, a, t, first, items, s);
+    case 2: return launch_ptc<32>(mk, mv, a, t, first, items, s);
+    case 3: return launch_ptc<48>(mk, mv, a, t, first, items, s);
+    case 4: return launch_ptc<64>(mk, mv, a, t, first, items, s);
+    case 5: return launch_ptc<80>(mk, mv, a, t, first, items, s);
+    case 6: return launch_ptc<96>(mk, mv, a, t, first, items, s);
+    case 7: return launch_ptc<112>(mk, mv, a, t, first, items, s);
+    case 8: return launch_ptc<128>(mk, mv, a, t, first, items, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
 }

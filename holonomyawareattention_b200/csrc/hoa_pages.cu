@@ -177,13 +177,15 @@ struct PgTakeArgs {
 };
 
 template <bool kFork>
-__global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
+__global__ void __launch_bounds__(kPgThreads)
 pages_take_kernel(PgTakeArgs p, const __grid_constant__ PgCopyArgs cp) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ int s_warp[kPgWarps];
   __shared__ int s_free, s_need, s_bad;
   __shared__ unsigned s_seen[kFork ? kPgMaxRows / 32 : 1];
   const int rank = (int)cl.block_rank(), tid = threadIdx.x, gt = rank * kPgThreads + tid;
+  wait_previous();
+  let_next_start();                        // (the payload's launch, which waits for this one to complete)
   const PgState& st = p.st;
   const int page = st.page, W = st.W, S = st.S;
   pg_copy(st.table, st.table_out, (long long)S * W, gt);
@@ -300,9 +302,10 @@ pages_take_kernel(PgTakeArgs p, const __grid_constant__ PgCopyArgs cp) {
 // ---------------------------------------------------------------------------
 struct PgFreeArgs { PgState st; const int* rows; int n; int* status; };
 
-__global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads) pages_free_kernel(PgFreeArgs p) {
+__global__ void __launch_bounds__(kPgThreads) pages_free_kernel(PgFreeArgs p) {
   cg::cluster_group cl = cg::this_cluster();
   const int tid = threadIdx.x, gt = (int)cl.block_rank() * kPgThreads + tid, lid = tid & 31;
+  wait_previous();
   const PgState& st = p.st;
   const int W = st.W;
   pg_copy(st.table, st.table_out, (long long)st.S * W, gt);
@@ -346,12 +349,14 @@ struct PgCompactArgs {
   int* status;
 };
 
-__global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
+__global__ void __launch_bounds__(kPgThreads)
 pages_compact_kernel(PgCompactArgs p, const __grid_constant__ PgCopyArgs cp) {
   cg::cluster_group cl = cg::this_cluster();
   __shared__ int s_warp[kPgWarps];
   __shared__ int s_live, s_hole, s_move;
   const int rank = (int)cl.block_rank(), tid = threadIdx.x, gt = rank * kPgThreads + tid;
+  wait_previous();
+  let_next_start();                        // (the payload's launch, which waits for this one to complete)
   constexpr int NT = kPgCluster * kPgThreads;
   const PgState& st = p.st;
   const int* refs = st.refs;
@@ -403,6 +408,7 @@ pages_compact_kernel(PgCompactArgs p, const __grid_constant__ PgCopyArgs cp) {
 // The copy as a launch of its own, bound by HBM.
 template <class V>
 __global__ void __launch_bounds__(kCpThreads) pages_copy_kernel(const __grid_constant__ PgCopyArgs p) {
+  wait_previous();
   const int n = p.count != nullptr ? min(*p.count, p.n) : p.n;
   const long long units = (long long)n * p.pools * p.chunks;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) pg_copy_unit<V, kCpThreads>(p, u, threadIdx.x);
@@ -413,8 +419,7 @@ static int launch_copy(PgCopyArgs a, long long most, cudaStream_t s) {
   a.chunks = (int)((most / (long long)sizeof(V) + kCpThreads * kCpVecs - 1) / (kCpThreads * kCpVecs));
   if (a.chunks < 1) a.chunks = 1;
   const long long units = (long long)a.n * a.pools * a.chunks;
-  pages_copy_kernel<V><<<(unsigned)(units < 148 * 8 ? units : 148 * 8), kCpThreads, 0, s>>>(a);
-  return launch_status();
+  return launch_early(pages_copy_kernel<V>, (unsigned)(units < 148 * 8 ? units : 148 * 8), 1, kCpThreads, 0, s, a);
 }
 
 struct PgPools { void* const* base; const long long* stride; const long long* bytes; int n; };
@@ -480,6 +485,7 @@ struct PgWriteArgs {
 };
 
 __global__ void __launch_bounds__(256) pages_write_kernel(PgWriteArgs p) {
+  wait_previous();
   const long long rows = (long long)p.B * p.T * p.H;
   const int lid = threadIdx.x & 31;
   for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
@@ -528,8 +534,8 @@ extern "C" int hoa_pages_reserve(const int* table, const int* lens, const int* r
   int* ws = static_cast<int*>(workspace);
   PgTakeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page},
                counts, nullptr, S, ws, ws + S, nullptr, nullptr, status};
-  pages_take_kernel<false><<<kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, PgCopyArgs{});
-  return launch_status();
+  return launch_early(pages_take_kernel<false>, kPgCluster, kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream), a,
+                      PgCopyArgs{});
 }
 
 extern "C" int hoa_pages_fork(const int* table, const int* lens, const int* refs, const int* src, const int* dst, int n,
@@ -548,8 +554,7 @@ extern "C" int hoa_pages_fork(const int* table, const int* lens, const int* refs
                src, dst, n, ws, ws + 3 * (size_t)n, from, to, status};
   const PgPools q{pools, strides, bytes, n_pools};
   const PgCopyArgs cp = inline_copy(q, from, to, n, n_pages, status);
-  pages_take_kernel<true><<<kPgCluster, kPgThreads, 0, s>>>(a, cp);
-  const int st = launch_status();
+  const int st = launch_early(pages_take_kernel<true>, kPgCluster, kPgCluster, kPgThreads, 0, s, a, cp);
   if (st != HOA_OK || cp.n > 0) return st;
   return copy_pools(q, from, to, nullptr, n, n_pages, status, s);
 }
@@ -561,8 +566,7 @@ extern "C" int hoa_pages_free(const int* table, const int* lens, const int* refs
     return HOA_ERR_INVALID_ARG;
   if (S > kPgMaxRows) return HOA_ERR_UNSUPPORTED;
   PgFreeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page}, rows, n, status};
-  pages_free_kernel<<<kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status();
+  return launch_early(pages_free_kernel, kPgCluster, kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream), a);
 }
 
 extern "C" int hoa_pages_compact(const int* table, const int* refs, int* table_out, int* refs_out, int* live, int S, int W,
@@ -580,8 +584,7 @@ extern "C" int hoa_pages_compact(const int* table, const int* refs, int* table_o
   // at most half of the pages move: a mover needs a hole below it
   const PgPools q{pools, strides, bytes, n_pools};
   const PgCopyArgs cp = inline_copy(q, from, to, n_pages / 2, n_pages, status);
-  pages_compact_kernel<<<kPgCluster, kPgThreads, 0, s>>>(a, cp);
-  const int st = launch_status();
+  const int st = launch_early(pages_compact_kernel, kPgCluster, kPgCluster, kPgThreads, 0, s, a, cp);
   if (st != HOA_OK || cp.n > 0) return st;
   return copy_pools(q, from, to, moves, n_pages / 2, n_pages, status, s);
 }
@@ -606,6 +609,6 @@ extern "C" int hoa_pages_write(const void* k, const void* v, int src_dtype, cons
                 k_pages, v_pages, page_strides[0], page_strides[1], page_strides[2], table, table_stride, lens,
                 B, T, H, d, page, W, n_pages, src_dtype, dtype, status};
   const long long blocks = ((long long)B * T * H + 7) / 8;
-  pages_write_kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status();
+  return launch_early(pages_write_kernel, (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 1, 256, 0,
+                      reinterpret_cast<cudaStream_t>(stream), a);
 }

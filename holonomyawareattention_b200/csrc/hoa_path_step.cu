@@ -340,6 +340,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  wait_previous();
   fetch(blockIdx.x);
 
   // the token's vectors and its page, read one row ahead too
@@ -656,8 +657,7 @@ static int launch_step_v(const StepArgs& s, int num_sms, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(path_step_kernel<DP, V>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
   const int units = s.B * s.H;
-  path_step_kernel<DP, V><<<(unsigned)(units < 2 * num_sms ? units : 2 * num_sms), kStThreads, L::kAlloc, stream>>>(s);
-  return launch_status();
+  return launch_early(path_step_kernel<DP, V>, (unsigned)(units < 2 * num_sms ? units : 2 * num_sms), 1, kStThreads, L::kAlloc, stream, s);
 }
 
 template <int DP>
