@@ -367,6 +367,44 @@ static int paged_attn_vec(const PaArgs& a, int rows, unsigned first, unsigned it
 // head - are under way when the parts arrive.
 constexpr int kPjThreads = 256;
 
+// One row's P (d x d): 8 lanes a row of it (thread: row pr + 32 x, columns 4 (pq + 8 y) .. + 3).
+template <int V>
+HOA_DEVICE void load_path(const float* __restrict__ Pg, int d, int pr, int pq, float4 (&P)[4][4]) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int r = pr + 32 * x, c = 4 * (pq + 8 * y);
+      P[x][y] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < d) {
+        if (V == 4) {
+          if (c < d) P[x][y] = *reinterpret_cast<const float4*>(Pg + r * d + c);
+        } else {
+          const float* at = Pg + r * d + c;
+          if (c < d) P[x][y].x = at[0];
+          if (c + 1 < d) P[x][y].y = at[1];
+          if (c + 2 < d) P[x][y].z = at[2];
+          if (c + 3 < d) P[x][y].w = at[3];
+        }
+      }
+    }
+}
+
+// out row g = P q
+HOA_DEVICE void apply_path(const PaArgs& p, long long g, int pr, int pq, const float4 (&P)[4][4], const float4 (&q)[4]) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    float y = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      y = fmaf(P[x][k].x, q[k].x, fmaf(P[x][k].y, q[k].y, fmaf(P[x][k].z, q[k].z, fmaf(P[x][k].w, q[k].w, y))));
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
+    const int r = pr + 32 * x;
+    if (pq == 0 && r < p.d) store_elem(p.out, g * p.d + r, p.out_dtype, y);
+  }
+}
+
 template <int V, int kWpr, bool kPaths>
 __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __grid_constant__ PaArgs p) {
   static_assert(!kPaths || kWpr == 8, "P takes the whole CTA");
@@ -379,28 +417,9 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
   const bool ok = g < p.rows;                          // (uniform in the warps that share a row)
   float4 P[4][4];                                      // pass, chunk of 4 columns
   const int pr = threadIdx.x >> 3, pq = threadIdx.x & 7;
-  if constexpr (kPaths) {
-    const float* Pg = p.paths + g * d * d;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int r = pr + 32 * x, c = 4 * (pq + 8 * y);
-        P[x][y] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < d) {
-          if (V == 4) {
-            if (c < d) P[x][y] = *reinterpret_cast<const float4*>(Pg + r * d + c);
-          } else {
-            const float* at = Pg + r * d + c;
-            if (c < d) P[x][y].x = at[0];
-            if (c + 1 < d) P[x][y].y = at[1];
-            if (c + 2 < d) P[x][y].z = at[2];
-            if (c + 3 < d) P[x][y].w = at[3];
-          }
-        }
-      }
-  }
+  if constexpr (kPaths) load_path<V>(p.paths + g * d * d, d, pr, pq, P);
   if (!p.leads) wait_previous();
+  if (p.more) let_next_start();
   float m = -INFINITY;
   if (ok)
     for (int s = lid; s < slots; s += 32) {
@@ -462,17 +481,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
     float4 q[4];
 #pragma unroll
     for (int y = 0; y < 4; ++y) q[y] = *reinterpret_cast<const float4*>(so + 4 * (pq + 8 * y));
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      float y = 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        y = fmaf(P[x][k].x, q[k].x, fmaf(P[x][k].y, q[k].y, fmaf(P[x][k].z, q[k].z, fmaf(P[x][k].w, q[k].w, y))));
-#pragma unroll
-      for (int k = 1; k < 8; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
-      const int r = pr + 32 * x;
-      if (pq == 0 && r < d) store_elem(p.out, g * d + r, p.out_dtype, y);
-    }
+    apply_path(p, g, pr, pq, P, q);
   } else if (w == 0) {
     if (V == 4 && 4 * lid < d) {
       if (p.out_dtype == HOA_BF16) {
@@ -490,6 +499,33 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
   }
 }
 
+// out = P o for many rows, o fp32 from the join: a stream of P alone, every load of a CTA's row at once and nothing to
+// wait for but o.  Measured at 128 rows x 24 heads of 120 (177 MB of P): fused with the join 48 us, apart 6 + 33.
+template <int V>
+__global__ void __launch_bounds__(kPjThreads) paged_attn_transport_kernel(const __grid_constant__ PaArgs p) {
+  const int d = p.d, pr = threadIdx.x >> 3, pq = threadIdx.x & 7;
+  const long long g = blockIdx.x;
+  float4 P[4][4];
+  load_path<V>(p.paths + g * d * d, d, pr, pq, P);     // (the launches before let this one start after they had waited for P)
+  wait_previous();
+  float4 q[4];
+  const float* o = p.o + g * d;
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    const int c = 4 * (pq + 8 * y);
+    q[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (V == 4) {
+      if (c < d) q[y] = *reinterpret_cast<const float4*>(o + c);
+    } else {
+      if (c < d) q[y].x = o[c];
+      if (c + 1 < d) q[y].y = o[c + 1];
+      if (c + 2 < d) q[y].z = o[c + 2];
+      if (c + 3 < d) q[y].w = o[c + 3];
+    }
+  }
+  apply_path(p, g, pr, pq, P, q);
+}
+
 template <int V, int kWpr, bool kPaths>
 static int launch_join(const PaArgs& a, cudaStream_t s) {
   const long long blocks = (a.rows + 8 / kWpr - 1) / (8 / kWpr);
@@ -501,7 +537,18 @@ static int join(const PaArgs& a, cudaStream_t s) {
   // 16-byte accesses: four columns a lane of o, the parts and P
   const bool v4 = a.d % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.paths) |
                                     reinterpret_cast<uintptr_t>(a.part_o)) & 15) == 0;
-  if (a.paths) return v4 ? launch_join<4, 8, true>(a, s) : launch_join<1, 8, true>(a, s);
+  if (a.paths) {
+    if (a.rows < 8 * 148) return v4 ? launch_join<4, 8, true>(a, s) : launch_join<1, 8, true>(a, s);
+    PaArgs j = a;                                      // the join writes o, fp32
+    j.paths = nullptr;
+    j.out = a.o;
+    j.out_dtype = HOA_F32;
+    j.more = 1;
+    const int st = v4 ? launch_join<4, 1, false>(j, s) : launch_join<1, 1, false>(j, s);
+    if (st != HOA_OK) return st;
+    if (a.rows > 0x7fffffffll) return HOA_ERR_UNSUPPORTED;
+    return launch_early(v4 ? paged_attn_transport_kernel<4> : paged_attn_transport_kernel<1>, (unsigned)a.rows, 1, kPjThreads, 0, s, a);
+  }
   // eight warps a row where one a row would leave SMs without work and there are parts to share
   if (a.rows < 148 * 16 && a.ns1 + a.ns2 > 4) return v4 ? launch_join<4, 8, false>(a, s) : launch_join<1, 8, false>(a, s);
   return v4 ? launch_join<4, 1, false>(a, s) : launch_join<1, 1, false>(a, s);
@@ -517,7 +564,8 @@ static bool pa_shape_ok(int B, int Tq, int H, int Hk, int d, int page, int n_sha
 }
 
 static size_t pa_bytes(const PaPlan& pl, int B, int Tq, int H, int d) {
-  return ((size_t)pl.ns1 + pl.ns2) * B * Tq * H * (8 + 4 * (size_t)d) + 256;
+  // the parts (O, then m and l), and one token's o before its transport
+  return ((size_t)pl.ns1 + pl.ns2) * B * Tq * H * (8 + 4 * (size_t)d) + (Tq == 1 ? 4 * (size_t)B * H * d : 0) + 256;
 }
 
 extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W,
@@ -581,7 +629,10 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
   a.status = status;
   a.leads = 1;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)(pl.ns1 + pl.ns2) * a.rows * d);
+  const size_t parts = (size_t)(pl.ns1 + pl.ns2) * a.rows * d;
+  a.o = a.part_o + parts;
+  // (m, l) pairs are read 8 bytes at a time: the floats before them rounded up to 16 bytes
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + ((parts + (Tq == 1 ? (size_t)a.rows * d : 0) + 3) & ~(size_t)3));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int st;
   if (pl.kind1 == pl.kind2) {                      // one launch for both parts

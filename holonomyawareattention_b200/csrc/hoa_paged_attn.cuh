@@ -18,12 +18,13 @@ struct PaArgs {
   const float* paths;                              // (B, H, d, d) or nullptr
   void* out; int out_dtype; float* lse;            // (B, Tq, H, d), (B, Tq, H)
   float* part_o; float2* part_ml;                  // (slots, rows, d) unnormalised; (slots, rows) (m, l), l = 0: no key
+  float* o;                                        // (rows, d) fp32: o before its transport (Tq = 1)
   long long rows;                                  // B * Tq * H
   float scale_log2;
   int dtype, B, Tq, H, Hk, G, d, page, n_pages;
   unsigned page_mul; int page_shift;               // j / page = umulhi(j, page_mul) >> page_shift for 0 <= j < 2^31 (page > 1)
   int tiles1, ns1, tiles2, ns2;
-  int leads;                                       // this launch is the first of the call
+  int leads, more;                                 // this launch is the first of the call; the join: the transport follows
   int* status;
 };
 

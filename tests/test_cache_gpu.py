@@ -296,6 +296,8 @@ ATTN = [
     ([4096 + 9, 4096 + 300], 64, 5, 64, 1, 1, 96, 1),                # splits along the keys
     ([2100] * 3, 16, 9, 128, 2, 2, 104, 3),
     ([520, 531] * 70, 8, 1, 64, 1, 1, 40, 2),                        # more than one tile of rows
+    ([5], 0, 1, 16, 1, 1, 33, 1),                                    # odd counts of floats before the (m, l) pairs
+    ([7], 0, 1, 16, 1, 1, 35, 3),
 ]
 
 
@@ -333,6 +335,28 @@ def test_paged_attn_paths_strides_streams(d, page, dtype):
         torch.cuda.current_stream().synchronize()
     assert out.dtype == F32
     check_attn((out, lse), (ro, rl), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,H,d", [(400, 3, 24), (150, 8, 50), (1190, 1, 120)])
+def test_paged_attn_paths_many_rows(B, H, d, dtype):
+    """More rows than the join takes P for itself: the transport in a launch of its own."""
+    page, n_shared = 16, 1
+    r = np.random.RandomState(B)
+    lens = [int(x) for x in r.randint(0, 60, size=B)]
+    kp, vp, table, shared, rows = make_cache(B, lens, n_shared, 3, page, H, d, dtype)
+    q = torch.randn(B, 1, H, d, device=DEV).to(dtype)
+    P = torch.randn(B, H, d, d, device=DEV)
+    out, lse = ops.paged_attn_fwd(q, kp, vp, table, i32(lens), 0.2, shared=shared, paths=P)
+    plain, lse2 = ops.paged_attn_fwd(q, kp, vp, table, i32(lens), 0.2, shared=shared, out_dtype=F32)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert torch.equal(lse, lse2)
+    want = torch.einsum("bhij,bthj->bthi", P.double(), plain.double())
+    assert rel(out, want) <= TOL[dtype]
+    some = [0, 1, B // 2, B - 1]
+    ro, _ = attn_ref(q[some], [rows[b] for b in some], [lens[b] for b in some], 0.2)
+    assert rel(plain[some], ro) <= TOL[dtype]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
@@ -448,3 +472,79 @@ def test_path_step_bad_page_is_reported():
             ops.check_status()
         assert e.value.status == _lib.HOA_ERR_PAGES
         assert bool((kp[0] == 0).all())
+
+
+# ---------------------------------------------------------------------------
+# the two host sides of a call
+# ---------------------------------------------------------------------------
+def test_both_host_sides_give_the_same(monkeypatch):
+    """The ordinary calls' C++ side against the Python functions behind it, bit for bit; a call that the
+    C++ side does not take (here: another pool stride, an integer scale) reaches them by itself."""
+    class Declines:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    d, H, page = 48, 2, 16
+    bk = Books(6, 4, 40, page)
+    bk.reserve([50, 20, 0, 7, 0, 0])
+    state = bk.tensors()
+    pools = [torch.randn(40, H, page, d, device=DEV) for _ in range(2)]
+    q = torch.randn(6, 1, H, d, device=DEV)
+    P = torch.linalg.qr(torch.randn(6, H, d, d, device=DEV))[0].contiguous()
+    a, qkv = torch.randn(6, H * d * (d - 1) // 2, device=DEV), torch.randn(6, 3 * H * d, device=DEV)
+
+    def all_calls():
+        kp, vp = (p.clone() for p in pools)
+        out = list(ops.pages_reserve(*state, i32([3, 0, 0, 20, 0, 1]), page))
+        out += ops.pages_fork([kp, vp], *state, i32([0, 1]), i32([2, 4]), page)
+        out += ops.pages_free(*state, i32([0]), page)
+        out += ops.pages_compact([kp, vp], state[0], state[2])
+        out += ops.paged_attn_fwd(q, kp, vp, state[0], state[1], 0.25, paths=P)
+        out += ops.path_step(a, P, qkv, H, 0.05, kp, vp, state[0], state[1])
+        torch.cuda.synchronize()
+        ops.check_status()
+        return out + [kp, vp]
+
+    fast = all_calls()
+    monkeypatch.setattr(ops, "_HOST", Declines())
+    slow = all_calls()
+    monkeypatch.undo()
+    assert len(fast) == len(slow) and all(torch.equal(x, y) for x, y in zip(fast, slow))
+    wide = torch.randn(40, 2, H, page, d, device=DEV)
+    assert ops.paged_attn_fwd(q, wide[:, 0], wide[:, 1], state[0], state[1], 1)[0].shape == q.shape
+    with pytest.raises(ValueError, match="must be"):
+        ops.paged_attn_fwd(q, pools[0], pools[1], state[0].long(), state[1], 0.25)
+    with pytest.raises(ValueError, match="contiguous int32"):
+        ops.pages_free(state[0], state[1][::2], state[2], i32([0]), page)
+    with pytest.raises(NotImplementedError, match="CUDA"):
+        ops.paged_attn_fwd(q, pools[0], pools[1], state[0].cpu(), state[1], 0.25)
+
+
+def test_calls_under_graph_capture():
+    """A decode step (reserve apart) captured once and replayed on new inputs."""
+    d, H, page, B = 96, 4, 64, 3
+    table = i32([[0, 1], [2, 3], [4, 5]])
+    lens = i32([70, 100, 1])
+    kp, vp = (torch.randn(6, H, page, d, device=DEV).to(BF) for _ in range(2))
+    P = torch.linalg.qr(torch.randn(B, H, d, d, device=DEV))[0].contiguous()
+    a, qkv = 0.3 * torch.randn(B, H * d * (d - 1) // 2, device=DEV), torch.randn(B, 3 * H * d, device=DEV).to(BF)
+
+    def step():
+        P2, qh = ops.path_step(a, P, qkv, H, 0.05, kp, vp, table, lens)
+        return ops.paged_attn_fwd(qh.view(B, 1, H, d), kp, vp, table, lens, 0.1, paths=P2)
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = step()
+    for seed in (1, 2):
+        torch.manual_seed(seed)
+        a.normal_(0, 0.3)
+        qkv.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    ops.check_status()
