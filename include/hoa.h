@@ -31,6 +31,9 @@
  *     per device;
  *   - hoa_set_wait_bound sets the bound of the device-side waits of every
  *     kernel launched after it (a diagnostic; the default is seconds).
+ * The generation entry points ask the driver once per device for their kernels'
+ * shared memory, and their kernels may come up while the one before them in the
+ * stream drains; each waits for all work before it before it touches memory.
  * Kernels whose bounded waits can give up report HOA_ERR_TIMEOUT through a
  * device status word (hoa_core_forward: the first 4 bytes of the workspace;
  * the stage entry points: their `status` argument).  The status of a launch is
@@ -411,7 +414,9 @@ int hoa_pages_write(const void* k, const void* v, int src_dtype, const long long
  *   lse (B, Tq, H) = the log of the softmax's sum, -inf there.
  * paths (nullable, Tq = 1): (B, H, d, d) fp32, then out = P o, the inverse
  * transport (core/attention_fast_chunked.py:171).  q and the pools share `dtype`;
- * d <= 128.  Slots that no query sees may hold anything, NaN included.
+ * d <= 128.  Slots that no query sees may hold anything, NaN included.  The
+ * workspace is 16-byte aligned; calls that may overlap on the GPU use different
+ * ones.
  */
 size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms);
 int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
@@ -431,6 +436,9 @@ int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_
  * rows `qkv_stride` elements apart.  lens[b] counts the token itself: at lens 1
  * there is no edge and P_out = I; at lens 0 P_out = P, q^ = 0 and nothing is
  * written.  P_out may be P.  qh and the pools share `dtype`; 2 <= d <= 120.
+ * The products run on the tensor cores in fixed-point ranges: entries of P are
+ * those of a rotation (at most 1; up to 255 stay exact to 2^-22), and
+ * |edge_scale * (a + a_bias)| < 4094.  `status` may also receive HOA_ERR_TIMEOUT.
  */
 int hoa_path_step(const float* a, int a_dtype, const float* a_bias, float edge_scale, const float* P, float* P_out,
                   const void* qkv, int qkv_dtype, long long qkv_stride, void* qh, void* k_pages, void* v_pages,
