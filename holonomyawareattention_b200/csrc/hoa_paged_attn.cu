@@ -585,7 +585,7 @@ extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, i
 
 static int run_items(int kind, const PaArgs& a, long long first, long long items, cudaStream_t s) {
   if (items == 0) return HOA_OK;
-  if (kind == kPaTc) return paged_attn_tc(a, (unsigned)first, (unsigned)items, s);
+  if (pa_is_tc(kind)) return paged_attn_tc(a, kind == kPaTc128, (unsigned)first, (unsigned)items, s);
   if (kind == kPaMma) return paged_attn_mma(a, (unsigned)first, (unsigned)items, s);
   if (kind < kPaSimt) return paged_attn_vec(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, s);
   return paged_attn_simt(a, pa_tile_rows(kind), (unsigned)first, (unsigned)items, s);

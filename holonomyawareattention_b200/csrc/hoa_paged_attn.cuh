@@ -64,10 +64,11 @@ inline int pa_tile_keys(int page) {
 //   vec:  fp32 with 16-byte rows, up to 4 rows a head (1, 2 or 4 a tile).
 //   simt: fp32, head dims or strides that the copies do not take; 16 rows a tile, 32 where there are more.
 //   mma:  bf16, 16 rows a tile, any page size.
-//   tc:   bf16, 256 rows a tile, pages that tile (pa_tile_keys).
-enum PaKind { kPaVec1, kPaVec2, kPaVec4, kPaSimt, kPaSimt32, kPaMma, kPaTc };
+//   tc:   bf16, pages that tile (pa_tile_keys); 256 rows a tile, or 128 where a head has no more.
+enum PaKind { kPaVec1, kPaVec2, kPaVec4, kPaSimt, kPaSimt32, kPaMma, kPaTc128, kPaTc };
+inline bool pa_is_tc(int kind) { return kind >= kPaTc128; }
 inline int pa_tile_rows(int kind) {
-  const int rows[] = {1, 2, 4, 16, 32, 16, 256};
+  const int rows[] = {1, 2, 4, 16, 32, 16, 128, 256};
   return rows[kind];
 }
 
@@ -87,10 +88,12 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   tc = tc && kt > 0;
   auto kind_of = [&](long long rows) -> int {
     if (vec && rows <= 4) return rows == 1 ? kPaVec1 : rows == 2 ? kPaVec2 : kPaVec4;
-    return tc && rows >= kPaTcRows ? kPaTc : tensor ? kPaMma : rows > 16 ? kPaSimt32 : kPaSimt;
+    return tc && rows >= kPaTcRows ? (rows <= 128 ? kPaTc128 : kPaTc) : tensor ? kPaMma : rows > 16 ? kPaSimt32 : kPaSimt;
   };
   pl.kind1 = kind_of(rows1);
   pl.kind2 = kind_of(rows2);
+  if (pa_is_tc(pl.kind1) && pa_is_tc(pl.kind2) && keys1 > 0 && keys2 > 0 && pl.kind1 != pl.kind2)
+    pl.kind1 = pl.kind2 = kPaTc;                   // one launch for both parts
   const long long r1 = pa_tile_rows(pl.kind1), r2 = pa_tile_rows(pl.kind2);
   const long long t1 = keys1 > 0 ? (rows1 + r1 - 1) / r1 : 0, t2 = keys2 > 0 ? (rows2 + r2 - 1) / r2 : 0;
   const long long u1 = t1 * Hk, u2 = t2 * Hk * B;
@@ -107,7 +110,7 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   auto splits = [&](int kind, long long units, long long keys, long long cost) -> int {
     if (units == 0) return 0;
     long long ns, most;
-    if (kind == kPaTc) {                           // one CTA an SM: split only what leaves SMs without one
+    if (pa_is_tc(kind)) {                         // one CTA an SM: split only what leaves SMs without one
       ns = num_sms / units;
       most = (keys + kt - 1) / kt;
     } else {
@@ -205,6 +208,6 @@ HOA_DEVICE void pa_begin(bool leads) {
 
 // items first .. first + items - 1
 int paged_attn_mma(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s);
+int paged_attn_tc(const PaArgs& a, bool dup, unsigned first, unsigned items, cudaStream_t s);
 
 }  // namespace hoa

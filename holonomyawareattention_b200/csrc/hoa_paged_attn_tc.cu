@@ -11,6 +11,11 @@
 //   * Q rows are gathered (rows of different sequences, grouped heads, any
 //     strides), so the softmax threads place their own row in the swizzled tile.
 //   * every row has its own last key, and a row may see none.
+//   * items of at most 128 rows (kDup) give both warpgroups the same rows and every
+//     other key tile each: one alone takes 3.7K cycles for 128 keys, slower than HBM
+//     brings them.  Their two O lie in the same lanes, where the first joins them.
+//     Measured (d = 96, 16 heads, 32768 shared keys): 64 rows 95 -> 81 us, 24 rows
+//     83 -> 70; 128 rows x 8 heads of 64 over 16384 keys 42 -> 37.
 //   * the result is the item's unnormalised (m, l, O).
 // What bounds it: 128 keys of a pair of tiles take 3.9K cycles, of which the issuing
 // lane is busy 2.6K (scores 600 a tile, P V 730: about 95 cycles a product of 64, while
@@ -69,7 +74,7 @@ struct PtArgs {
   long long max_wait;
 };
 
-template <int DP16>
+template <int DP16, bool kDup>
 __global__ void __launch_bounds__(kPtThreads, 1)
 paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                      const __grid_constant__ PaArgs p, const PtArgs pt, unsigned first) {
@@ -116,12 +121,12 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     tmem_relinquish();
   }
   pa_begin(p.leads);
-  const PaItem it = pa_item(p, first + blockIdx.x, 256, KT);
+  const PaItem it = pa_item(p, first + blockIdx.x, kDup ? 128 : 256, KT);
   __syncthreads();
   PaRow my{};
   int seen = 0;
   if (warp < 8) {
-    my = pa_row(p, it, it.row0 + tid);               // warps 0-3: tile 0, warps 4-7: tile 1
+    my = pa_row(p, it, it.row0 + (kDup ? tid & 127 : tid));     // warps 0-3: tile 0, warps 4-7: tile 1
     seen = my.ok ? max(0, min(my.seen - it.key_base, it.k1)) : 0;
     const int top = __reduce_max_sync(0xffffffffu, seen);
     if (lid == 0) atomicMax(&s_seen[warp >> 2], top);
@@ -136,7 +141,13 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     n_t[i] = s_seen[i] > it.k0 ? (s_seen[i] - it.k0 + KT - 1) / KT : 0;
     kmax = max(kmax, s_seen[i]);
   }
-  const int nkt = max(n_t[0], n_t[1]);
+  const int nkt = max(n_t[0], n_t[1]);               // key tiles of the item
+  if (kDup) {
+    n_t[0] = (nkt + 1) / 2;
+    n_t[1] = nkt / 2;
+  }
+  // the key tile that warpgroup i takes as its j-th
+  auto tile = [](int i, int j) { return kDup ? 2 * j + i : j; };
   bool bad = false;
 
   if (warp == 9) {
@@ -186,7 +197,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       const uint32_t idS = make_idesc(kFmtBF16, 128, KT);
       constexpr uint32_t idO = make_idesc(kFmtBF16, 128, DP16, true);
       constexpr int KSTEPS = DP16 / 16;
-      const uint64_t dQ[2] = {desc_sw128(smem_u32(sm + L::offQ)), desc_sw128(smem_u32(sm + L::offQ + L::kQ))};
+      const uint64_t dQ[2] = {desc_sw128(smem_u32(sm + L::offQ)), desc_sw128(smem_u32(sm + L::offQ + (kDup ? 0 : L::kQ)))};
       const uint32_t colS[2] = {tmem + L::colS0, tmem + L::colS1};
       const uint32_t colO[2] = {tmem + L::colO0, tmem + L::colO1};
       bool ok = mbar_wait_abortable(q_full, 0, s_abort, pt.max_wait);
@@ -195,11 +206,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       // exponentials (with S0 S1 PV0 PV1 both waited for all four).
       int have = 0, v_have = 0;                      // K and V tiles known to have landed
       auto scores = [&](int i, int j) {
-        const int s = j % L::NS;
-        if (j >= have) {
-          ok = mbar_wait_abortable(&k_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+        const int t = tile(i, j), s = t % L::NS;
+        if (t >= have) {
+          ok = mbar_wait_abortable(&k_full[s], (t / L::NS) & 1, s_abort, pt.max_wait);
           if (!ok) return;
-          have = j + 1;
+          have = t + 1;
         }
         tc_fence_after();
         const uint64_t dK = desc_sw128(smem_u32(sm + L::offStage + s * L::kStage));
@@ -209,31 +220,31 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
           mma_bf16(colS[i], dQ[i] + off, dK + off, idS, kk > 0 ? 1u : 0u);
         }
         tc_commit(&s_full[i]);
-        if (i == 1 || j >= n_t[1]) tc_commit(&k_empty[s]);     // the tile's last scores
+        if (kDup || i == 1 || j >= n_t[1]) tc_commit(&k_empty[s]);      // the tile's last scores
       };
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (ok && n_t[i] > 0) scores(i, 0);
-      for (int j = 0; j < nkt && ok; ++j) {
-        const int s = j % L::NS;
-        const uint64_t dV = desc_sw128_mn(smem_u32(sm + L::offStage + s * L::kStage) + L::kQ, L::kBlk);
+      for (int j = 0; j < max(n_t[0], n_t[1]) && ok; ++j) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (j >= n_t[i] || !ok) continue;
+          const int t = tile(i, j), s = t % L::NS;
+          const uint64_t dV = desc_sw128_mn(smem_u32(sm + L::offStage + s * L::kStage) + L::kQ, L::kBlk);
           ok = mbar_wait_abortable(&p_full[i], j & 1, s_abort, pt.max_wait);
           if (!ok) break;
-          if (v_have <= j) {
-            ok = mbar_wait_abortable(&v_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+          if (t >= v_have) {
+            ok = mbar_wait_abortable(&v_full[s], (t / L::NS) & 1, s_abort, pt.max_wait);
             if (!ok) break;
-            v_have = j + 1;
+            v_have = t + 1;
           }
           tc_fence_after();
           for (int kk = 0; kk < KT / 16; ++kk)         // 16 keys: 16 rows of 128 bytes of every V slab
             mma_bf16_ts(colO[i], colS[i] + kk * 8, dV + (uint64_t)(kk * 2048 >> 4), idO, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit(&pv_done[i]);
+          if (kDup || i == 1 || j >= n_t[1]) tc_commit(&v_empty[s]);    // the tile's last weights
           if (j + 1 < n_t[i]) scores(i, j + 1);
         }
-        tc_commit(&v_empty[s]);
       }
       if (!ok) bad = true;
       tc_commit(fin);
@@ -250,6 +261,7 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
 #pragma unroll
       for (int ch = 0; ch < L::NKB * 8; ++ch) {
         uint4 v = make_uint4(0, 0, 0, 0);
+        if (kDup && i == 1) break;                    // (the rows are in place already)
         if (my.ok && ch * 8 < p.d) {
           if (pt.qvec) {
             v = *reinterpret_cast<const uint4*>(q + ch * 8);
@@ -275,11 +287,11 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     for (int j = 0; j < ni; ++j) {
       bad |= !mbar_wait_abortable(&s_full[i], j & 1, s_abort, pt.max_wait);
       tc_fence_after();
-      const int k0 = it.k0 + j * KT;
-      if (j == nkt - 1 && kmax - k0 < KT) {
+      const int t = tile(i, j), k0 = it.k0 + t * KT;
+      if (t == nkt - 1 && kmax - k0 < KT) {
         // V rows past the last key that is seen: zero (each warpgroup that runs this tile)
-        const int s = j % L::NS;
-        bad |= !mbar_wait_abortable(&v_full[s], (j / L::NS) & 1, s_abort, pt.max_wait);
+        const int s = t % L::NS;
+        bad |= !mbar_wait_abortable(&v_full[s], (t / L::NS) & 1, s_abort, pt.max_wait);
         uint8_t* v = sm + L::offStage + s * L::kStage + L::kQ;
         if (r >= kmax - k0 && r < KT)
 #pragma unroll
@@ -354,20 +366,49 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
     if (ni > 0) bad |= !mbar_wait_abortable(&pv_done[i], (ni - 1) & 1, s_abort, pt.max_wait);
     tc_fence_after();
     const long long part = (long long)it.slot * p.rows + my.grow;
-    if (my.ok) p.part_ml[part] = make_float2(m_ref, bad ? 0.f : l_run);
-    if (live) {
-      float* orow = p.part_o + part * p.d;
+    float f0 = 1.f, f1 = 0.f;                        // factors of this warpgroup's O, of the second one's
+    if (kDup) {
+      // the second warpgroup's (m, l) through shared memory (the Q slabs of the absent tile), its O from TMEM
+      float2* s_ml = reinterpret_cast<float2*>(sm + L::offQ + L::kQ);
+      if (i == 1) s_ml[r] = make_float2(m_ref, bad ? 0.f : l_run);
+      tc_fence_before();
+      named_sync(1, 256);
+      tc_fence_after();
+      if (i == 0) {
+        const float2 o2 = s_ml[r];
+        if (o2.y > 0.f) {
+          const float m = fmaxf(m_ref, o2.x);
+          f0 = l_run > 0.f ? pa_ex2(m_ref - m) : 0.f;
+          f1 = pa_ex2(o2.x - m);
+          l_run = l_run * f0 + o2.y * f1;
+          m_ref = m;
+        }
+      }
+    }
+    if (!kDup || i == 0) {
+      const bool first_ran = ni > 0, second_ran = kDup && n_t[1] > 0;
+      if (my.ok) p.part_ml[part] = make_float2(m_ref, bad ? 0.f : l_run);
+      if (live) {
+        float* orow = p.part_o + part * p.d;
 #pragma unroll
-      for (int c16 = 0; c16 < DP16 / 16; ++c16) {
-        float ov[16];
-        tmem_ld16(cO + 16 * c16, ov);
-        tmem_wait_ld();
-        tmem_touch(ov);
-        if (my.ok && !bad && l_run > 0.f) {
+        for (int c16 = 0; c16 < DP16 / 16; ++c16) {
+          float ov[16], ow[kDup ? 16 : 1];
+          if (first_ran) tmem_ld16(cO + 16 * c16, ov);
+          if constexpr (kDup) {
+            if (second_ran) tmem_ld16(tmem + L::colO1 + lane + 16 * c16, ow);
+          }
+          tmem_wait_ld();
+          tmem_touch(ov);
+          tmem_touch(ow);
+          if (my.ok && !bad && l_run > 0.f) {
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)            // (d is a multiple of 8)
-            if (16 * c16 + e < p.d)
-              *reinterpret_cast<float4*>(orow + 16 * c16 + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+            for (int e = 0; e < 16; ++e)
+              if (second_ran) ov[e] = (f0 > 0.f ? ov[e] * f0 : 0.f) + (f1 > 0.f ? ow[kDup ? e : 0] * f1 : 0.f);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)          // (d is a multiple of 8)
+              if (16 * c16 + e < p.d)
+                *reinterpret_cast<float4*>(orow + 16 * c16 + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          }
         }
       }
     }
@@ -411,16 +452,22 @@ static bool page_map(CUtensorMap* m, const void* base, const PaArgs& a, int box)
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP16>
-static int launch_ptc(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, unsigned first,
+template <int DP16, bool kDup>
+static int launch_ptc_d(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, unsigned first,
                       unsigned items, cudaStream_t s) {
   using L = PtLayout<DP16>;
   static std::atomic<unsigned long long> done{0};
-  if (!allow_smem(paged_attn_tc_kernel<DP16>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
-  return launch_early(paged_attn_tc_kernel<DP16>, items, 1, kPtThreads, L::kAlloc, s, mk, mv, a, t, first);
+  if (!allow_smem(paged_attn_tc_kernel<DP16, kDup>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
+  return launch_early(paged_attn_tc_kernel<DP16, kDup>, items, 1, kPtThreads, L::kAlloc, s, mk, mv, a, t, first);
 }
 
-int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t s) {
+template <int DP16>
+static int launch_ptc(const CUtensorMap& mk, const CUtensorMap& mv, const PaArgs& a, const PtArgs& t, bool dup, unsigned first,
+                      unsigned items, cudaStream_t s) {
+  return dup ? launch_ptc_d<DP16, true>(mk, mv, a, t, first, items, s) : launch_ptc_d<DP16, false>(mk, mv, a, t, first, items, s);
+}
+
+int paged_attn_tc(const PaArgs& a, bool dup, unsigned first, unsigned items, cudaStream_t s) {
   PtArgs t;
   t.kt = pa_tile_keys(a.page);
   t.box = a.page < t.kt ? a.page : t.kt;
@@ -429,14 +476,14 @@ int paged_attn_tc(const PaArgs& a, unsigned first, unsigned items, cudaStream_t 
   CUtensorMap mk, mv;
   if (t.kt == 0 || !page_map(&mk, a.kp, a, t.box) || !page_map(&mv, a.vp, a, t.box)) return HOA_ERR_INVALID_ARG;
   switch ((a.d + 15) / 16) {
-    case 1: return launch_ptc<16>(mk, mv, a, t, first, items, s);
-    case 2: return launch_ptc<32>(mk, mv, a, t, first, items, s);
-    case 3: return launch_ptc<48>(mk, mv, a, t, first, items, s);
-    case 4: return launch_ptc<64>(mk, mv, a, t, first, items, s);
-    case 5: return launch_ptc<80>(mk, mv, a, t, first, items, s);
-    case 6: return launch_ptc<96>(mk, mv, a, t, first, items, s);
-    case 7: return launch_ptc<112>(mk, mv, a, t, first, items, s);
-    case 8: return launch_ptc<128>(mk, mv, a, t, first, items, s);
+    case 1: return launch_ptc<16>(mk, mv, a, t, dup, first, items, s);
+    case 2: return launch_ptc<32>(mk, mv, a, t, dup, first, items, s);
+    case 3: return launch_ptc<48>(mk, mv, a, t, dup, first, items, s);
+    case 4: return launch_ptc<64>(mk, mv, a, t, dup, first, items, s);
+    case 5: return launch_ptc<80>(mk, mv, a, t, dup, first, items, s);
+    case 6: return launch_ptc<96>(mk, mv, a, t, dup, first, items, s);
+    case 7: return launch_ptc<112>(mk, mv, a, t, dup, first, items, s);
+    case 8: return launch_ptc<128>(mk, mv, a, t, dup, first, items, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
 }
