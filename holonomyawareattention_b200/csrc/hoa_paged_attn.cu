@@ -577,7 +577,7 @@ extern "C" size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, i
   if (!pa_shape_ok(B, Tq, H, Hk, d, page, n_shared, W, num_sms)) return 0;
   size_t most = 0;                                 // enough for whichever kernels take the call
   for (int k = 0; k < 4; ++k) {
-    const size_t n = pa_bytes(pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, k == 1, k > 1, k > 2), B, Tq, H, d);
+    const size_t n = pa_bytes(pa_plan(B, Tq, H, Hk, d, page, n_shared, W, num_sms, k == 1, k > 1, k > 2), B, Tq, H, d);
     most = n > most ? n : most;
   }
   return most;
@@ -611,7 +611,7 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
                          (uintptr_t)(page_strides[0] * e) | (uintptr_t)(page_strides[1] * e) | (uintptr_t)(page_strides[2] * e);
   const bool rows16 = (bits & 15) == 0;              // every token's row is 16-byte aligned
   const bool tensor = dtype == HOA_BF16 && d % 8 == 0 && rows16;
-  const PaPlan pl = pa_plan(B, Tq, H, Hk, page, n_shared, W, num_sms, dtype == HOA_F32 && d % 4 == 0 && rows16, tensor,
+  const PaPlan pl = pa_plan(B, Tq, H, Hk, d, page, n_shared, W, num_sms, dtype == HOA_F32 && d % 4 == 0 && rows16, tensor,
                             tensor && softmax_scale > 0.f);
   if (workspace_bytes < pa_bytes(pl, B, Tq, H, d)) return HOA_ERR_WORKSPACE;
   const long long items1 = (long long)pl.tiles1 * Hk * pl.ns1, items2 = (long long)B * Hk * pl.tiles2 * pl.ns2;

@@ -79,7 +79,7 @@ struct PaPlan { int kind1, tiles1, ns1, kind2, tiles2, ns2; };
 
 // `vec`: fp32 with d % 4 == 0 and 16-byte strides, `tensor`: bf16 with d % 8 == 0 and 16-byte strides, `tc`: tcgen05
 // takes the call (tensor, scale > 0).
-inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int W, int num_sms, bool vec, bool tensor,
+inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms, bool vec, bool tensor,
                       bool tc) {
   PaPlan pl{};
   const long long G = H / Hk, keys1 = (long long)n_shared * page, keys2 = (long long)W * page;
@@ -101,8 +101,11 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
   // their part (of the room that the rows have: shorter rows split what they have as finely).  Measured at 65536
   // shared tokens and 8 rows: one wave 96 us, two 103, three 107.  A simt item spends about four times as long on a key
   // as the others, which only read it.  At least 64 keys: there an item's time is its latency.
-  auto range_of = [&](long long cost) -> long long {
-    const long long r = (cost + 4ll * num_sms - 1) / (4ll * num_sms);
+  // Simt items get 3 CTAs an SM, what their shared memory holds, or 4 with 16 rows and a head dim of up to 88.  Measured
+  // for 3 and for 4 at 8 rows of 32 queries: 88 us and 110; 64 such rows: 71 and 79; bf16, d = 20: 86 and 69.
+  auto range_of = [&](int kind, long long cost) -> long long {
+    const long long slots = (kind == kPaSimt32 || (kind == kPaSimt && d > 88) ? 3ll : 4ll) * num_sms;
+    const long long r = (cost + slots - 1) / slots;
     return r < 64 ? 64 : r;
   };
   auto weight = [](int kind) -> long long { return kind == kPaSimt || kind == kPaSimt32 ? 4 : 1; };
@@ -114,7 +117,7 @@ inline PaPlan pa_plan(int B, int Tq, int H, int Hk, int page, int n_shared, int 
       ns = num_sms / units;
       most = (keys + kt - 1) / kt;
     } else {
-      ns = (keys * weight(kind) + range_of(cost) - 1) / range_of(cost);
+      ns = (keys * weight(kind) + range_of(kind, cost) - 1) / range_of(kind, cost);
       most = (keys + 63) / 64;
     }
     ns = ns > most ? most : ns;
