@@ -424,11 +424,12 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
   if constexpr (kPaths) load_path<V>(p.paths + g * d * d, d, pr, pq, P);
   if (!p.leads) wait_previous();
   if (p.more) let_next_start();
+  // a part without a key has l = 0; one that saw a score of NaN or +inf has l = NaN, which makes the row NaN
   float m = -INFINITY;
   if (ok)
     for (int s = lid; s < slots; s += 32) {
       const float2 ml = p.part_ml[s * p.rows + g];
-      if (ml.y > 0.f) m = fmaxf(m, ml.x);
+      if (ml.y != 0.f) m = fmaxf(m, ml.y > 0.f ? ml.x : INFINITY);
     }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
 #pragma unroll 4
     for (int s = w; s < slots; s += kWpr) {
       const float2 ml = p.part_ml[s * p.rows + g];
-      const float f = ml.y > 0.f ? exp2f(ml.x - m) : 0.f;
+      const float f = ml.y != 0.f ? exp2f(ml.x - m) : 0.f;
       l = fmaf(f, ml.y, l);
       const float* at = p.part_o + (s * p.rows + g) * d;
       if (V == 4) {
@@ -467,10 +468,10 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
     for (int e = 0; e < 4; ++e) o[e] = t[e];
   }
   if (!ok) return;
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
-  if (w == 0 && lid == 0) p.lse[g] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
+  if (w == 0 && lid == 0) p.lse[g] = l != 0.f ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
   if constexpr (kPaths) {
     float* so = reinterpret_cast<float*>(s_o);         // o in column order, zero past d
     __syncthreads();

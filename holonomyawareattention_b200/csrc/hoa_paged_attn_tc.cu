@@ -376,9 +376,9 @@ paged_attn_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_consta
       tc_fence_after();
       if (i == 0) {
         const float2 o2 = s_ml[r];
-        if (o2.y > 0.f) {
+        if (o2.y != 0.f) {                           // (NaN stays NaN)
           const float m = fmaxf(m_ref, o2.x);
-          f0 = l_run > 0.f ? pa_ex2(m_ref - m) : 0.f;
+          f0 = l_run != 0.f ? pa_ex2(m_ref - m) : 0.f;
           f1 = pa_ex2(o2.x - m);
           l_run = l_run * f0 + o2.y * f1;
           m_ref = m;

@@ -374,6 +374,45 @@ def test_paged_attn_peaked(B, Tq, dtype):
     assert bool(((got[1].double().cpu() - rl).abs() <= 1e-5 * rl.abs().clamp(min=1)).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("lens,n_shared,Tq,H,Hk,d", [
+    ([300, 257, 0], 2, 1, 2, 2, 96),              # one row a head of its own, three of the shared part
+    ([300, 257], 0, 1, 8, 2, 50),                 # a head dim that no copy takes
+    ([300, 280], 2, 3, 4, 2, 96),
+    ([300, 280], 2, 40, 4, 2, 64),                # 80 rows a head
+    ([400, 380, 390], 3, 130, 2, 2, 96),          # more than one tile of rows
+])
+def test_paged_attn_nan_and_inf_in_what_is_seen(lens, n_shared, Tq, H, Hk, d, dtype):
+    """A query of NaN, a key of +inf: NaN in the rows that see them, nothing in the others."""
+    page, W = 64, 6
+    kp, vp, table, shared, rows = make_cache(d, lens, n_shared, W, page, Hk, d, dtype)
+    q = torch.randn(len(lens), Tq, H, d, device=DEV).to(dtype)
+    args = (vp, table, i32(lens), 0.1)
+    clean, lse0 = ops.paged_attn_fwd(q, kp, *args, shared=shared)
+    bad = q.clone()
+    bad[0, Tq - 1, 1, 3] = float("nan")
+    out, lse = ops.paged_attn_fwd(bad, kp, *args, shared=shared)
+    torch.cuda.synchronize()
+    hit = torch.zeros(len(lens), Tq, H, dtype=torch.bool, device=DEV)
+    hit[0, Tq - 1, 1] = True
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], lse0[~hit])
+    # the last key of sequence 0, seen by its last query alone; 0 * inf in no other score
+    k2 = kp.clone()
+    k2[table[0, (lens[0] - 1) // page - n_shared].item(), 0, (lens[0] - 1) % page] = float("inf")
+    q2 = q.clone()
+    q2[0, Tq - 1] = 1.0                           # a score of +inf
+    out, lse = ops.paged_attn_fwd(q2, k2, *args, shared=shared)
+    torch.cuda.synchronize()
+    ops.check_status()
+    hit[:] = False
+    hit[0, Tq - 1, :H // Hk] = True
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    rest = ~hit
+    rest[0, Tq - 1] = False
+    assert torch.equal(out[rest], clean[rest]) and torch.equal(lse[rest], lse0[rest])
+
+
 def test_paged_attn_bad_page_is_reported():
     lens = [100, 90]
     kp, vp, table, shared, rows = make_cache(1, lens, 0, 7, 16, 2, 48, BF)
