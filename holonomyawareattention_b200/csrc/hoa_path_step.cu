@@ -188,7 +188,7 @@ HOA_DEVICE void st_product(uint8_t* sm, uint32_t tmem, bool accumulate, uint64_t
   const uint32_t t[2] = {tmem + L::colHi, tmem + L::colLo};
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    const int a = pass == 2, b = pass == 1;                    // hi hi, hi lo, lo hi
+    const int a = pass == 1, b = pass == 0;                    // hi lo, lo hi, hi hi
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       const uint64_t rk = r[b] + (uint64_t)(k * 2048 >> 4);

@@ -413,6 +413,59 @@ def test_paged_attn_nan_and_inf_in_what_is_seen(lens, n_shared, Tq, H, Hk, d, dt
     assert torch.equal(out[rest], clean[rest]) and torch.equal(lse[rest], lse0[rest])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,Tq,H,Hk,d,page", [
+    (1, 1, 2, 2, 96, 64), (3, 1, 2, 2, 48, 16), (3, 1, 4, 2, 50, 32), (9, 2, 2, 1, 64, 24),
+    (40, 1, 2, 2, 96, 64), (3, 50, 2, 2, 120, 32), (2, 150, 2, 2, 64, 128), (5, 30, 1, 1, 33, 13),
+])
+def test_paged_attn_rows_that_end_in_the_shared_pages(B, Tq, H, Hk, d, page, dtype):
+    """No row fills the shared pages: what lies after the longest one is NaN, and is in no result."""
+    n_shared = 6 if page >= 64 else 12
+    room = n_shared * page
+    lens = [room // 2 - 5 + (7 * b) % (room // 3) for b in range(B)]
+    kp, vp, table, shared, rows = make_cache(page, lens, n_shared, 1, page, Hk, d, dtype)
+    for x in range(max(lens), room):
+        for pool in (kp, vp):
+            pool[shared[x // page].item(), :, x % page] = float("nan")
+    q = torch.randn(B, Tq, H, d, device=DEV).to(dtype)
+    got = ops.paged_attn_fwd(q, kp, vp, table, i32(lens), 1 / math.sqrt(d), shared=shared)
+    check_attn(got, attn_ref(q, rows, lens, 1 / math.sqrt(d)), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_offsets_past_32_bits(dtype):
+    """Pages at the far end of a pool of more than 2^31 elements: the same bits as from a small one."""
+    page, H, d, W, B = 64, 8, 96, 4, 3
+    n_pages = 2 ** 31 // (H * page * d) + 64
+    lens = [page * 3 + 9, page * 2, 70]
+    kp, vp, table, shared, rows = make_cache(5, lens, 2, W, page, H, d, dtype)
+    small = kp.shape[0]
+    kp, vp = kp.nan_to_num(0.0), vp.nan_to_num(0.0)
+    far = n_pages - small
+    K, V = (torch.empty(n_pages, H, page, d, device=DEV, dtype=dtype) for _ in range(2))
+    K[far:], V[far:] = kp, vp
+    T = torch.where(table >= 0, table + far, table)
+    for Tq in (1, 5, 60):
+        q = torch.randn(B, Tq, H, d, device=DEV).to(dtype)
+        want = ops.paged_attn_fwd(q, kp, vp, table, i32(lens), 0.1, shared=shared)
+        got = ops.paged_attn_fwd(q, K, V, T, i32(lens), 0.1, shared=shared + far)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    k, v = (torch.randn(B, 3, H, d, device=DEV).to(dtype) for _ in range(2))
+    a, qkv = torch.randn(B, H * d * (d - 1) // 2, device=DEV), torch.randn(B, 3 * H * d, device=DEV).to(dtype)
+    P = torch.eye(d, device=DEV).repeat(B, H, 1, 1)
+    own = i32([page * 2 + 1, page, 70])
+    step = []
+    for x, y, t, at in ((kp, vp, table, 0), (K, V, T, far)):
+        full = torch.cat([(shared + at).repeat(B, 1), t], 1)
+        ops.pages_write(k, v, x, y, full, own)
+        step.append(ops.path_step(a, P, qkv, H, 0.1, x, y, full, own + 2 * (own < 70).int()))
+        ops.pages_copy([x, y], i32([at + 1]), i32([at + small - 1]))
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert torch.equal(step[0][0], step[1][0]) and torch.equal(step[0][1], step[1][1])
+    assert torch.equal(K[far:], kp) and torch.equal(V[far:], vp)
+
+
 def test_paged_attn_bad_page_is_reported():
     lens = [100, 90]
     kp, vp, table, shared, rows = make_cache(1, lens, 0, 7, 16, 2, 48, BF)
