@@ -39,15 +39,15 @@ HOA_DEVICE void st_fail(int* status) {
 // One CTA of 256 threads per row (b, h), its products on tcgen05 with fp32
 // accuracy: every factor x is split into x s = hi + lo, two f16 of 11 bits each (s a
 // power of two that puts the factor's bound near 2^10), and a product is the three
-// tensor-core products hi hi + hi lo + lo hi with fp32 accumulation; lo lo, 2^-22 of
-// it, is left out.  f16 runs at twice the rate of tf32 and has its 11 bits; its
+// tensor-core products hi lo + lo hi + hi hi with fp32 accumulation (the small ones
+// first: sums are cut off after each 16 columns); lo lo, 2^-22 of it, is left out.  f16 runs at twice the rate of tf32 and has its 11 bits; its
 // short exponent is no loss, because the bounds are known: theta <= 0.6 after
 // scaling, |P| <= 1.  (A itself is split at 16 A: entries up to 4094 fit, and what
 // f16 drops of small ones, 2^-29, is below fp32's rounding of P'.)
 //
 //   P1  A2 = A A                                  scale 2^-s from ||A2||_1 >= ||A||_2^2
 //   P2  A4 = A2 T,        T = x1 A + x2 A2
-//   P3  E = E0 + L R,     L = x3 A2 + A4, R = x5 A + x6 A2 + x7 A4, E0 = A + y2 A2 + L
+//   P3  E = E0 + L R,     L = x3 A2 + A4, R = x5 A + x6 A2 + x7 A4, E0 = A + y2 A2 + L  (s > 0: A added after L R)
 //   (s times  E <- 2 E + E E)
 //   P4  P' = P + E P
 // G = I + E: the identity stays out of every product, so that the accumulator's
@@ -62,7 +62,7 @@ HOA_DEVICE void st_fail(int* status) {
 // shared memory at d = 120, so two CTAs run on an SM and one's products overlap the
 // other's element work.
 //
-// Measured at 128 rows x 24 heads of 120 (446 MB, 42.7 GFLOP of fp32-accurate work): 249 us, 1.8 TB/s and 171 TFLOP/s,
+// Measured at 128 rows x 24 heads of 120 (446 MB, 42.7 GFLOP of fp32-accurate work): 255 us, 1.75 TB/s and 167 TFLOP/s,
 // against 2.9 ms on the CUDA cores; 256 heads of 96: 21 us, one head's latency (22.8K cycles from its generators to its
 // outputs).  The tensor pipe is busy 27%, the schedulers issue 50%: the rest is each CTA's chain of products (1.5K cycles
 // each) and the element work between them (split, join, store: 2 to 5K).  More threads a row (384, 512) spill and are
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       peek(u + gridDim.x, next);
       continue;
     }
-    asm volatile("" : "+r"(pr));                               // (as rr below)
+    asm volatile("" : "+r"(pr));                               // (as the row's index math below)
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();                                           // the staged generators are in; the last row's sums were read
 #pragma unroll
@@ -398,67 +398,71 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       }
       // Row r of A, 16 columns at a time: entry (r, c) is +gen{r, c} right of the diagonal, -gen{c, r} left of
       // it.  A chunk that the diagonal misses in all 32 rows of the warp has one rule for all of them.
-      const int w0 = row & ~31, rr = min(row, d - 1);          // (rows past the matrix read its last row and get 0)
-      const float sr = row < d ? p.edge_scale * kSA : 0.f;
-      const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1;   // packed: {r, c}, r < c, lies at base_r + c
-      if (w0 < DP) {
-#pragma unroll 1
-        for (int c = un.group; c < L::NC; c += kStGroups) {
-          const int c0 = 16 * c;
-          float v[16];
-          float sg = sr;
-          if (p.banked) {                                      // gen_banked_slot, 32 x 32 block by block
-            const int nb = d >> 5, ba = w0 >> 5, bb = c0 >> 5, v0 = c0 & 31, lo = min(ba, bb), hi = max(ba, bb);
-            const float* blk = gen + (lo * nb - lo * (lo + 1) / 2 + hi - lo - 1) * 1024;
-            if (ba < bb) {
+      // (0 in the pad)  y = 16 columns from c0 on, in units of 1 / kSA
+      auto row_of_A = [&](int c0, F2 (&y)[8]) {
+        int at = row;
+        asm volatile("" : "+r"(at));                           // (its index math stays here: no registers across the products)
+        const int w0 = at & ~31, rr = min(at, d - 1);          // (rows past the matrix read its last row and get 0)
+        const float sr = at < d ? p.edge_scale * kSA : 0.f;
+        const int base_r = rr * (2 * d - rr - 1) / 2 - rr - 1; // packed: {r, c}, r < c, lies at base_r + c
+        float v[16];
+        float sg = sr;
+        if (p.banked) {                                      // gen_banked_slot, 32 x 32 block by block
+          const int nb = d >> 5, ba = w0 >> 5, bb = c0 >> 5, v0 = c0 & 31, lo = min(ba, bb), hi = max(ba, bb);
+          const float* blk = gen + (lo * nb - lo * (lo + 1) / 2 + hi - lo - 1) * 1024;
+          if (ba < bb) {
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] = blk[lid * 32 + ((v0 + e) ^ (4 * (lid & 7)))];
-            } else if (ba > bb) {
-              sg = -sr;
+            for (int e = 0; e < 16; ++e) v[e] = blk[lid * 32 + ((v0 + e) ^ (4 * (lid & 7)))];
+          } else if (ba > bb) {
+            sg = -sr;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) v[e] = blk[(v0 + e) * 32 + (lid ^ (4 * ((v0 + e) & 7)))];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int cc = c0 + e;
-                const float g = gen[cc != rr ? gen_banked_slot(rr, cc, d) : 0];
-                v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
-              }
-            }
-          } else if (c0 > w0 + 31) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = gen[base_r + c0 + e];
+            for (int e = 0; e < 16; ++e) v[e] = blk[(v0 + e) * 32 + (lid ^ (4 * ((v0 + e) & 7)))];
           } else {
-            int base_c = c0 * (2 * d - c0 - 1) / 2 - c0 - 1;
-            if (c0 + 15 < w0) {
-              sg = -sr;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                v[e] = gen[base_c + rr];
-                base_c += d - c0 - e - 2;
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const int cc = c0 + e;
-                const float g = gen[max(0, min(cc > rr ? base_r + cc : base_c + rr, p.stride - 1))];
-                v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
-                base_c += d - cc - 2;
-              }
+            for (int e = 0; e < 16; ++e) {
+              const int cc = c0 + e;
+              const float g = gen[cc != rr ? gen_banked_slot(rr, cc, d) : 0];
+              v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
             }
           }
-          if (c0 + 16 > d)                                     // pad columns
+        } else if (c0 > w0 + 31) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = c0 + e < d ? v[e] : 0.f;
+          for (int e = 0; e < 16; ++e) v[e] = gen[base_r + c0 + e];
+        } else {
+          int base_c = c0 * (2 * d - c0 - 1) / 2 - c0 - 1;
+          if (c0 + 15 < w0) {
+            sg = -sr;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              v[e] = gen[base_c + rr];
+              base_c += d - c0 - e - 2;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int cc = c0 + e;
+              const float g = gen[max(0, min(cc > rr ? base_r + cc : base_c + rr, p.stride - 1))];
+              v[e] = cc > rr ? g : (cc < rr ? -g : 0.f);
+              base_c += d - cc - 2;
+            }
+          }
+        }
+        if (c0 + 16 > d)                                       // pad columns
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = c0 + e < d ? v[e] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), f2(sg));
+      };
+      if ((row & ~31) < DP) {
+#pragma unroll 1
+        for (int c = un.group; c < L::NC; c += kStGroups) {
           F2 y[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), f2(sg));
+          row_of_A(16 * c, y);
           un.put_right(c, y);
         }
       }
       // ---- P1: A2, and the scaling: ||A2||_1 (A2 is symmetric: row sums) bounds ||A||_2^2
       issue(Yes{}, false);
-      fetch(u + gridDim.x);                                    // (the staged row has been read)
       wait();
       float rs = 0.f;
       chunks(load_acc, [&](int, Acc& x) {
@@ -500,13 +504,18 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       issue(No{}, false);
       wait();
       // ---- P3: E = E0 + L R, in units of 1 / (kSL kSR)
-      {
+      auto p3 = [&](auto squares) {
         // with t = T kST, a = A2 kSA2, q = A4 kSA2 kST and A = (T - x2 A2) / x1:
         //   l = L kSL,  r = R kSR,  e = E0 kSL kSR
         const F2 la = f2(kStX3 * kSL / kSA2), lq = f2(kSL / (kSA2 * kST));
         const F2 rt = f2(kStX5 / kStX1 * kSR / kST), ra = f2((kStX6 - kStX5 * kStX2 / kStX1) * kSR / kSA2),
                  rq = f2(kStX7 * kSR / (kSA2 * kST));
-        const F2 et = f2(kSL * kSR / (kStX1 * kST)), ea = f2((kStY2 - kStX2 / kStX1) * kSL * kSR / kSA2), el = f2(kSR);
+        // The tensor core cuts its sums off (it does not round), 3 DP / 16 times over what stands in D before the product,
+        // and each squaring doubles that: where there are squarings, A, most of E0, stays out of it and is added behind
+        // the product.  Measured error of P', d = 72 and five squarings: 1.8e-6 with A in E0, 6.5e-7 without (fp32 all
+        // through: 5.0e-7), for 14 us of 297 at 128 rows x 24 heads of 120.
+        const F2 et = f2(squares ? 0.f : kSL * kSR / (kStX1 * kST)),
+                 ea = f2((squares ? kStY2 : kStY2 - kStX2 / kStX1) * kSL * kSR / kSA2), el = f2(kSR);
         chunks(load_left, [&](int c, AccLeft& x) {
           F2 t[8], a2[8];
           un.get_right(c, t);
@@ -515,7 +524,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
           for (int e = 0; e < 8; ++e) {
             const F2 q = f2(x.v[2 * e], x.v[2 * e + 1]);
             const F2 l = f2_fma(q, lq, f2_mul(a2[e], la));
-            const float2 e0 = f2_get(f2_fma(l, el, f2_fma(a2[e], ea, f2_mul(t[e], et))));
+            const float2 e0 = f2_get(f2_fma(l, el, squares ? f2_mul(a2[e], ea) : f2_fma(a2[e], ea, f2_mul(t[e], et))));
             t[e] = f2_fma(q, rq, f2_fma(a2[e], ra, f2_mul(t[e], rt)));
             a2[e] = l;
             x.v[2 * e] = e0.x;
@@ -525,12 +534,32 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
           un.put_right(c, t);
           tmem_st16(un.tmem + L::colD + 16 * c, x.v);
         });
-      }
+      };
+      if (nsq > 0) p3(Yes{}); else p3(No{});
       issue(No{}, true);
+      // ---- E, squared nsq times: (I + E)^2 = I + (2 E + E E)
       load_P(P);
       wait();
-      // ---- E, squared nsq times: (I + E)^2 = I + (2 E + E E)
-      if (nsq == 0) put_P();
+      if (nsq == 0) {
+        put_P();
+      } else {
+#pragma unroll 1
+        for (int c = (row & ~31) < DP ? un.group : L::NC; c < L::NC; c += kStGroups) {
+          F2 y[8];
+          row_of_A(16 * c, y);
+          Acc x = load_acc(c);
+          tmem_wait_ld();
+          x.touch();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float2 v = f2_get(f2_fma(y[e], f2(kSL * kSR * sa), f2(x.v[2 * e], x.v[2 * e + 1])));
+            x.v[2 * e] = v.x;
+            x.v[2 * e + 1] = v.y;
+          }
+          tmem_st16(un.tmem + L::colD + 16 * c, x.v);
+        }
+        tmem_wait_st();
+      }
       chunks(load_acc, [&](int c, Acc& x) {
         F2 e1[8];
 #pragma unroll
@@ -558,6 +587,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
       }
       // ---- P4: E P
       issue(No{}, false);
+      fetch(u + gridDim.x);                                    // (the staged row has been read)
       load_P(P);                                               // again, for P + E P (from L2)
       wait();
       chunks(load_acc, [&](int c, Acc& x) {

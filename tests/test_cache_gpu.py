@@ -536,6 +536,28 @@ def test_path_step(d, es, dtype):
         assert torch.equal(Q2, Q)
 
 
+@pytest.mark.parametrize("d", [32, 63, 80, 120])
+@pytest.mark.parametrize("es", [0.02, 0.1, 0.5, 1.5])
+def test_path_step_as_exact_as_fp32(d, es):
+    """Within twice the error of fp32's own matrix exponential and product, from no squaring to six (2e-7: products of
+    factors and sums with 2^-23 each, where fp32 is nearly exact)."""
+    torch.manual_seed(d)
+    B, H = 6, 2
+    a = 0.3 * torch.randn(B, H * d * (d - 1) // 2, device=DEV)
+    P = torch.linalg.qr(torch.randn(B, H, d, d, device=DEV, dtype=torch.float64))[0].float().contiguous()
+    kp, vp = (torch.zeros(B, H, 4, d, device=DEV) for _ in range(2))
+    got, _ = ops.path_step(a, P, torch.randn(B, 3 * H * d, device=DEV), H, es, kp, vp, i32([[b] for b in range(B)]), i32([2] * B))
+    torch.cuda.synchronize()
+    ops.check_status()
+    i, j = torch.triu_indices(d, d, 1)
+    A = torch.zeros(B, H, d, d, device=DEV)
+    A[:, :, i, j] = es * a.view(B, H, -1)
+    A = A - A.transpose(2, 3)
+    want = torch.linalg.matrix_exp(A.double().cpu()) @ P.double().cpu()
+    fp32 = torch.linalg.matrix_exp(A.cpu()) @ P.cpu()
+    assert rel(got, want) <= 2 * rel(fp32, want) + 2e-7, (rel(got, want), rel(fp32, want))
+
+
 def test_path_step_keeps_rotations():
     """A thousand steps: P stays orthogonal to fp32 accuracy (the errors of the steps add like a
     random walk at worst linearly: 1000 x 1e-7)."""
