@@ -27,7 +27,7 @@ namespace hoa {
 // are padded to an odd number of 16-byte chunks, so that the 16 keys of a warp's read fall on different
 // banks.  Few rows (R = 2) are bound by the loads, 8 d bytes a key; many (R = 4) by the FMAs, 4 d a key
 // and row: 32 rows halve the shared-memory reads an FMA needs.  Measured in fp32: 16 rows of 16 heads of 96 over 4096
-// shared tokens and their own 91 us; 32 queries of 8 rows over 2048 tokens 113 us, 13 TFLOP/s.
+// shared tokens and their own 85 us; 32 queries of 8 rows over 2048 tokens 88 us, 17 TFLOP/s.
 constexpr int kPsKeys = 64, kPsThreads = 128;
 
 HOA_DEVICE int ps_ld(int d) { return ((d + 3) / 4 | 1) * 4; }    // floats of a padded row
