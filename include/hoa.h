@@ -414,9 +414,9 @@ int hoa_pages_write(const void* k, const void* v, int src_dtype, const long long
  *   lse (B, Tq, H) = the log of the softmax's sum, -inf there.
  * paths (nullable, Tq = 1): (B, H, d, d) fp32, then out = P o, the inverse
  * transport (core/attention_fast_chunked.py:171).  q and the pools share `dtype`;
- * d <= 128.  Slots that no query sees may hold anything, NaN included; a NaN or
- * an infinite score that a query sees makes its out and lse NaN.  The workspace is 16-byte aligned; calls that may overlap on the GPU use different
- * ones.
+ * d <= 128.  Slots that no query sees may hold anything, NaN included; a NaN or a
+ * score of +inf that a query sees makes its out and lse NaN.  The workspace is
+ * 16-byte aligned; calls that may overlap on the GPU use different ones.
  */
 size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms);
 int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_pages, const void* v_pages,
