@@ -36,7 +36,7 @@ struct Device { int sms = 0; int* status = nullptr; };
 constexpr int kMaxDevices = 64;
 Device g_dev[kMaxDevices];
 
-constexpr size_t kScratchMost = 32u << 20;          // as ops._SCRATCH_MOST
+constexpr size_t kScratchMost = 32u << 20;          // larger ones are allocated for their call alone
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
@@ -58,8 +58,8 @@ bool code(const at::Tensor& t, int* c) {
   return true;
 }
 
-// Scratch of a call: one buffer a device and stream (calls on a stream run in order), except large ones and under
-// graph capture.  The buffers are never destroyed: at the interpreter's exit the CUDA context may be gone first.
+// Scratch of a call: one buffer a device and stream, except large ones and under graph capture.  A call enqueues all its
+// launches under the interpreter's lock, so no other call's come between them on the stream.  The buffers are never destroyed: at the interpreter's exit the CUDA context may be gone first.
 struct Scratch { void* p; at::Tensor keep; };
 Scratch scratch(const at::Tensor& like, int idx, cudaStream_t s, size_t n) {
   static auto& held = *new std::map<std::pair<int, cudaStream_t>, at::Tensor>;

@@ -720,25 +720,13 @@ def _run(idx: int, name: str, *args) -> None:
         _lib.check(name, st)
 
 
-# Scratch of these calls, one buffer a device and stream: calls on a stream run in order, so they can share
-# it.  Large ones, and calls under graph capture (whose memory belongs to the graph), allocate their own.
-_SCRATCH = {}
-_SCRATCH_MOST = 32 << 20
-
-
+# Scratch of one call.  The library is called without the interpreter's lock, so the launches of two threads' calls may
+# alternate on a stream: each call hands its parts over in memory of its own, which the allocator gives out again in
+# stream order once the call has returned.  (The C++ side holds the lock over a call and keeps one buffer a stream.)
 def _scratch(idx: int, n: int):
     """(address of n bytes of scratch on device idx's current stream, what keeps them alive)."""
-    if n <= _SCRATCH_MOST and not torch._C._cuda_isCurrentStreamCapturing():
-        key = idx, torch._C._cuda_getCurrentRawStream(idx)
-        v = _SCRATCH.get(key)
-        if v is None or v[2] < n:
-            # the old buffer may still be in use on its stream: the allocator hands it out again in stream order
-            with torch.inference_mode(False):
-                t = torch.empty(max(n, 1 << 20), dtype=torch.uint8, device=torch.device("cuda", idx))
-            v = _SCRATCH[key] = (t.data_ptr(), t, t.numel())
-        return v
     t = torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", idx))
-    return t.data_ptr(), t, n
+    return t.data_ptr(), t
 
 
 def _longs(*values):

@@ -1,0 +1,127 @@
+"""Generation when something goes wrong around a call: threads, errors in the middle of a step, lists and
+modes that are out of the ordinary.  What a call reports, and what it leaves behind.
+"""
+import threading
+
+import pytest
+import torch
+
+from holonomyawareattention_b200 import PathCache, PathOrderedGeometricMHA, _lib, decode, ops, prefill  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    """No status of one test is left for the next."""
+    yield
+    torch.cuda.synchronize()
+    try:
+        ops.check_status()
+    except _lib.HoaError:
+        pass
+
+
+def pages(n, H=2, page=16, d=48, dtype=BF, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return [torch.randn(n, H, page, d, device=DEV, generator=g).to(dtype) for _ in range(2)]
+
+
+def module(D=64, H=2, dtype=F32):
+    torch.manual_seed(D)
+    return PathOrderedGeometricMHA(D, n_heads=H, edge_scale=0.05).to(DEV, dtype).eval()
+
+
+def state_of(cache):
+    live = [r for r in range(cache.rows) if cache.tokens[r]]
+    return ([t.clone() for t in (cache.table, cache.lens, cache.refs, cache.P[live], cache.last[live])],
+            (list(cache.tokens), [list(h) for h in cache._held], dict(cache._count), cache.n_shared))
+
+
+def same_state(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a[0], b[0])) and a[1] == b[1]
+
+
+# ---------------------------------------------------------------------------
+# host threads
+# ---------------------------------------------------------------------------
+def attn_args(seed, B=6, H=2, d=48, W=24, page=16):
+    kp, vp = pages(B * W, H, page, d, seed=seed)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = torch.randn(B, 1, H, d, device=DEV, generator=g).to(BF)
+    table = i32([[b * W + j for j in range(W)] for b in range(B)])
+    return q, kp, vp, table, i32([W * page - 3 * b for b in range(B)]), 0.2
+
+
+def test_calls_in_progress_share_no_scratch(monkeypatch):
+    """A call that begins while another one on the same stream has not returned (two threads: the library is
+    called without the interpreter's lock) hands its parts over in memory of its own."""
+    a, b = attn_args(1), attn_args(2)
+    ops.paged_attn_fwd(*a, out_dtype=F32)         # (what is looked up once is known)
+    real, seen = ops._fn, []
+
+    def fn(name):
+        f = real(name)
+
+        def call(*args):
+            if name == "hoa_paged_attn_fwd":
+                seen.append(args[-4])             # the workspace
+                if len(seen) == 1:
+                    ops.paged_attn_fwd(*b, out_dtype=F32)
+            return f(*args)
+        return call
+
+    monkeypatch.setattr(ops, "_fn", fn)
+    ops.paged_attn_fwd(*a, out_dtype=F32)
+    torch.cuda.synchronize()
+    assert len(seen) == 2 and seen[0] != seen[1]
+
+
+def test_two_threads_on_one_stream():
+    """Attention, fork and prefill from two threads on the default stream: each result as in one thread alone."""
+    attn = module(192, 4, BF)
+    prompts = [torch.randn(2, 90, 192, device=DEV, generator=torch.Generator(device=DEV).manual_seed(i)).to(BF) for i in range(2)]
+    args = [attn_args(i) for i in range(2)]
+
+    def work(i, n):
+        out = []
+        with torch.no_grad():
+            for k in range(n):
+                out += ops.paged_attn_fwd(*args[i], out_dtype=F32)
+                if k % 10 == 0:
+                    cache = PathCache(attn, rows=4, max_tokens=128, page=16)
+                    y = prefill(attn, prompts[i], cache, [0, 1])
+                    # pools as a tuple: the Python side of the call
+                    st = ops.pages_fork((cache.k_pages, cache.v_pages), cache.table, cache.lens, cache.refs, i32([0, 1]), i32([2, 3]), 16)
+                    new = st[0][2:, 5].long()
+                    out += [y, *st, cache.k_pages[new], cache.v_pages[new]]
+        torch.cuda.current_stream().synchronize()
+        return out
+
+    want = [work(i, 10) for i in range(2)]
+    got = [None, None]
+
+    def run(i):
+        got[i] = work(i, 200)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    per = len(want[0])
+    for i in range(2):
+        assert len(got[i]) == 20 * per
+        # slots that no token was written to are whatever the pool's memory held: compare the written ones
+        for k, x in enumerate(got[i]):
+            w = want[i][k % per]
+            if x.dim() == 4 and x.shape[0] == 2 and x.dtype == BF and x.shape[2] == 16:
+                x, w = x[:, :, :90 % 16], w[:, :, :90 % 16]
+            assert torch.equal(x, w), (i, k)
+    ops.check_status()
