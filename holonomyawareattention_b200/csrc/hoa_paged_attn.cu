@@ -605,8 +605,9 @@ extern "C" int hoa_paged_attn_fwd(const void* q, const long long* q_strides, con
     return HOA_ERR_INVALID_ARG;
   if ((dtype != HOA_F32 && dtype != HOA_BF16) || (out_dtype != HOA_F32 && out_dtype != HOA_BF16) || d > 128)
     return HOA_ERR_UNSUPPORTED;
-  // key positions and item numbers are ints
+  // key positions, row numbers (a tile past the last one included) and item numbers are ints
   if ((long long)(n_shared + (long long)W) * page > 0x7fff0000ll) return HOA_ERR_UNSUPPORTED;
+  if ((long long)B * Tq > 0x7fff0000ll / H) return HOA_ERR_UNSUPPORTED;
   const int e = dtype == HOA_BF16 ? 2 : 4;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(k_pages) | reinterpret_cast<uintptr_t>(v_pages) |
                          (uintptr_t)(page_strides[0] * e) | (uintptr_t)(page_strides[1] * e) | (uintptr_t)(page_strides[2] * e);

@@ -1,0 +1,30 @@
+"""Generation operators at the ends of their integer ranges: refused on the host before anything runs, or
+shown on the index arithmetic alone (no GPU needed).
+"""
+import ctypes
+
+import pytest
+import torch
+
+from holonomyawareattention_b200 import _lib, ops
+
+UNS = _lib.HOA_ERR_UNSUPPORTED
+BIG = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from holonomyawareattention_b200 import _build
+    _build.build()
+    return _lib.load()
+
+
+p, q, none = ctypes.c_void_p(16), ctypes.c_void_p(32), None
+s3 = (ctypes.c_longlong * 3)(8, 8, 8)
+
+
+@pytest.mark.parametrize("B,Tq,H", [(2 ** 31 - 1, 2, 1), (2 ** 20, 2 ** 11, 1), (1, 2 ** 30, 2), (2 ** 16, 2 ** 12, 8)])
+def test_attention_rows_beyond_int(lib, B, Tq, H):
+    """The kernels number the rows of a head, (b, t, g), with an int: 2^31 of them would come out negative."""
+    assert lib.hoa_paged_attn_fwd(p, s3, p, p, s3, 0, p, 4, p, 1, 1, p, none, p, 0, p, 1.0, B, Tq, H, 1, 8, 16, 4, 148, p, 1 << 62,
+                                  none, none) == UNS
