@@ -716,7 +716,7 @@ extern "C" int hoa_path_step(const float* a, int a_dtype, const float* a_bias, f
     return HOA_ERR_INVALID_ARG;
   const int stride = gen_row_stride(a_dtype, d);
   if (d > 120 || stride == 0 || gen_elem_dtype(a_dtype) != HOA_F32 || (qkv_dtype != HOA_F32 && qkv_dtype != HOA_BF16) ||
-      (dtype != HOA_F32 && dtype != HOA_BF16) || (long long)B * H > 0x7fffffffll)
+      (dtype != HOA_F32 && dtype != HOA_BF16) || (long long)B * H > 0x7fff0000ll)   // (a CTA steps past the last unit by the grid)
     return HOA_ERR_UNSUPPORTED;
   StepArgs s{a, gen_is_banked(a_dtype) ? 1 : 0, stride, a_bias, edge_scale, P, P_out, qkv, qkv_dtype, qkv_stride, qh,
              k_pages, v_pages, dtype, page_strides[0], page_strides[1], page_strides[2], table, table_stride, lens,

@@ -436,7 +436,8 @@ int hoa_paged_attn_fwd(const void* q, const long long* q_strides, const void* k_
  * to this one (a_dtype HOA_F32, with or without HOA_GEN_BANKED); qkv (B, H, 3d)
  * rows `qkv_stride` elements apart.  lens[b] counts the token itself: at lens 1
  * there is no edge and P_out = I; at lens 0 P_out = P, q^ = 0 and nothing is
- * written.  P_out may be P.  qh and the pools share `dtype`; 2 <= d <= 120.
+ * written.  P_out may be P.  qh and the pools share `dtype`; 2 <= d <= 120,
+ * B * H at most 2^31 - 65536.
  * The products run on the tensor cores in fixed-point ranges: entries of P are
  * those of a rotation (at most 1; up to 255 stay exact to 2^-22), and
  * |edge_scale * (a + a_bias)| < 4094.  `status` may also receive HOA_ERR_TIMEOUT.

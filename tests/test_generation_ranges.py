@@ -28,3 +28,9 @@ def test_attention_rows_beyond_int(lib, B, Tq, H):
     """The kernels number the rows of a head, (b, t, g), with an int: 2^31 of them would come out negative."""
     assert lib.hoa_paged_attn_fwd(p, s3, p, p, s3, 0, p, 4, p, 1, 1, p, none, p, 0, p, 1.0, B, Tq, H, 1, 8, 16, 4, 148, p, 1 << 62,
                                   none, none) == UNS
+
+
+@pytest.mark.parametrize("B,H", [(BIG, 1), (BIG - 200, 1), (2 ** 25 - 1, 64), (2 ** 30, 2)])
+def test_path_step_units_beyond_int(lib, B, H):
+    """A CTA steps from one (row, head) to the next by the size of the grid, also past the last one: with an int."""
+    assert lib.hoa_path_step(p, 0, none, 1.0, p, p, p, 0, 6, p, p, p, 0, s3, p, 1, 1, p, B, H, 2, 4, 4, none, none) == UNS
