@@ -510,6 +510,9 @@ __global__ void __launch_bounds__(256) pages_write_kernel(PgWriteArgs p) {
   }
 }
 
+// The loops over pages and requests count past the last one, by up to a cluster's threads, with an int.
+constexpr int kPgMost = 0x7fff0000;
+
 static bool pg_state_ok(const int* table, const int* lens, const int* refs, const int* t2, const int* l2,
                         const int* r2, int S, int W, int n_pages, int page) {
   return table && lens && refs && t2 && l2 && r2 && table != t2 && lens != l2 && refs != r2 && S >= 1 && W >= 1 &&
@@ -532,7 +535,7 @@ extern "C" int hoa_pages_reserve(const int* table, const int* lens, const int* r
                                  size_t workspace_bytes, int* status, void* stream) {
   if (!pg_state_ok(table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page) || !counts || !workspace)
     return HOA_ERR_INVALID_ARG;
-  if (S > kPgMaxRows) return HOA_ERR_UNSUPPORTED;
+  if (S > kPgMaxRows || n_pages > kPgMost) return HOA_ERR_UNSUPPORTED;
   if (workspace_bytes < hoa_pages_workspace_bytes(S, n_pages)) return HOA_ERR_WORKSPACE;
   int* ws = static_cast<int*>(workspace);
   PgTakeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page},
@@ -548,7 +551,7 @@ extern "C" int hoa_pages_fork(const int* table, const int* lens, const int* refs
   if (!pg_state_ok(table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page) || n < 0 || n_pools < 0 ||
       (n > 0 && (!src || !dst)) || (n_pools > 0 && (!pools || !strides || !bytes)) || !workspace)
     return HOA_ERR_INVALID_ARG;
-  if (S > kPgMaxRows || n > S) return HOA_ERR_UNSUPPORTED;
+  if (S > kPgMaxRows || n > S || n_pages > kPgMost) return HOA_ERR_UNSUPPORTED;
   if (workspace_bytes < hoa_pages_workspace_bytes(n, n_pages)) return HOA_ERR_WORKSPACE;
   int* ws = static_cast<int*>(workspace);
   int *from = ws + n, *to = ws + 2 * (size_t)n;
@@ -567,7 +570,7 @@ extern "C" int hoa_pages_free(const int* table, const int* lens, const int* refs
                               void* stream) {
   if (!pg_state_ok(table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page) || n < 0 || (n > 0 && !rows))
     return HOA_ERR_INVALID_ARG;
-  if (S > kPgMaxRows) return HOA_ERR_UNSUPPORTED;
+  if (S > kPgMaxRows || n > kPgMost || n_pages > kPgMost) return HOA_ERR_UNSUPPORTED;
   PgFreeArgs a{{table, lens, refs, table_out, lens_out, refs_out, S, W, n_pages, page}, rows, n, status};
   return launch_early(pages_free_kernel, kPgCluster, kPgCluster, kPgThreads, 0, reinterpret_cast<cudaStream_t>(stream), a);
 }
@@ -578,7 +581,7 @@ extern "C" int hoa_pages_compact(const int* table, const int* refs, int* table_o
   if (!pg_state_ok(table, table, refs, table_out, table_out, refs_out, S, W, n_pages, 1) || !live || n_pools < 0 ||
       (n_pools > 0 && (!pools || !strides || !bytes)) || !workspace)
     return HOA_ERR_INVALID_ARG;
-  if (S > kPgMaxRows) return HOA_ERR_UNSUPPORTED;
+  if (S > kPgMaxRows || n_pages > kPgMost) return HOA_ERR_UNSUPPORTED;
   if (workspace_bytes < hoa_pages_workspace_bytes(0, n_pages)) return HOA_ERR_WORKSPACE;
   int* ws = static_cast<int*>(workspace);
   int *from = ws, *to = ws + n_pages, *remap = ws + 2 * (size_t)n_pages, *moves = ws + 3 * (size_t)n_pages;

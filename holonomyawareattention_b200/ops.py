@@ -761,6 +761,8 @@ def _books(table, lens, refs, page):
     _ints(refs, "refs", (n_pages,), idx)
     if page < 1:
         raise ValueError("page must be at least 1")
+    if S * W >= 2 ** 31 or n_pages >= 2 ** 31 or page >= 2 ** 31:      # (the library takes them as int)
+        raise ValueError("S * W, n_pages and page must be below 2^31")
     return idx, S, W, n_pages
 
 

@@ -34,3 +34,28 @@ def test_attention_rows_beyond_int(lib, B, Tq, H):
 def test_path_step_units_beyond_int(lib, B, H):
     """A CTA steps from one (row, head) to the next by the size of the grid, also past the last one: with an int."""
     assert lib.hoa_path_step(p, 0, none, 1.0, p, p, p, 0, 6, p, p, p, 0, s3, p, 1, 1, p, B, H, 2, 4, 4, none, none) == UNS
+
+
+@pytest.mark.parametrize("n_pages", [BIG, BIG - 100])
+def test_pages_beyond_int(lib, n_pages):
+    """The loops over pages and requests step past the last one with an int."""
+    big = 1 << 62
+    assert lib.hoa_pages_reserve(p, p, p, p, q, q, q, 1, 1, n_pages, 1, p, big, none, none) == UNS
+    assert lib.hoa_pages_fork(p, p, p, p, p, 1, q, q, q, 1, 1, n_pages, 1, none, none, none, 0, p, big, none, none) == UNS
+    assert lib.hoa_pages_free(p, p, p, p, 1, q, q, q, 1, 1, n_pages, 1, none, none) == UNS
+    assert lib.hoa_pages_free(p, p, p, p, n_pages, q, q, q, 1, 1, 4, 1, none, none) == UNS
+    assert lib.hoa_pages_compact(p, p, q, q, q, 1, 1, n_pages, none, none, none, 0, p, big, none, none) == UNS
+
+
+def test_sizes_beyond_int_are_refused_in_python(monkeypatch):
+    """Sizes that the C entry points take as int do not wrap on the way there."""
+    monkeypatch.setattr(ops, "_index", lambda t: 0)
+    monkeypatch.setattr(ops, "_ints", lambda *a: None)
+    huge = torch.empty(1, dtype=torch.int32).expand(2 ** 32 + 5)
+    small = torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops._books(small, None, huge, 4)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops._books(torch.empty(1, 1, dtype=torch.int32).expand(2 ** 16, 2 ** 16 + 1), None, small[0], 4)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ops._books(small, None, small[0], 2 ** 32 + 1)
