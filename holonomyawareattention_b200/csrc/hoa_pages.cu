@@ -221,7 +221,8 @@ pages_take_kernel(PgTakeArgs p, const __grid_constant__ PgCopyArgs cp) {
           }
         } else {
           const int len = st.lens[i], c = p.a[i];
-          bad = len < 0 || c < 0 || (long long)len + c > (long long)W * page;
+          // (lengths are ints: a row may have room for more tokens than one counts)
+          bad = len < 0 || c < 0 || (long long)len + c > min((long long)W * page, 0x7fffffffll);
           if (!bad) need = pg_used(len + c, page) - pg_used(len, page);
         }
       }

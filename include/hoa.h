@@ -371,7 +371,7 @@ int hoa_edge_gemm_fp8_acc(const void* lo, const void* w, float* out, float alpha
  *            follows, so that the pool's tail can be given up.
  * reserve and fork are all or nothing: with too few free pages or an invalid
  * request (a row outside the table, a dst that is not empty or listed twice, a
- * row longer than W pages) the new state equals the old one, no payload moves,
+ * row longer than W pages or 2^31 - 1 tokens) the new state equals the old one, no payload moves,
  * and `status` is set.  S <= 65536, S * W < 2^31, and n and n_pages
  * at most 2^31 - 65536.
  * pools / strides / bytes: n_pools base pointers, bytes between pages and bytes

@@ -125,3 +125,24 @@ def test_two_threads_on_one_stream():
                 x, w = x[:, :, :90 % 16], w[:, :, :90 % 16]
             assert torch.equal(x, w), (i, k)
     ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+# arguments
+# ---------------------------------------------------------------------------
+def test_reserve_of_more_tokens_than_an_int_counts():
+    """Pages so large that W of them hold 2^31 tokens and more: a row that would pass an int is refused, one that comes
+    just up to it is not."""
+    page, W = 2 ** 30, 4
+    state = i32([[0, 1, -1, -1], [-1] * 4]), i32([2 ** 31 - 10, 0]), i32([1, 1, 0, 0, 0, 0])
+    for counts in ([10, 5], [2 ** 31 - 1, 2 ** 31 - 1]):
+        out = ops.pages_reserve(*state, i32(counts), page)
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.HoaError) as e:
+            ops.check_status()
+        assert e.value.status == _lib.HOA_ERR_PAGES
+        assert all(torch.equal(a, b) for a, b in zip(out, state))
+    t, n, r = ops.pages_reserve(*state, i32([9, 2 ** 30 + 1]), page)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert t.tolist() == [[0, 1, -1, -1], [2, 3, -1, -1]] and n.tolist() == [2 ** 31 - 1, 2 ** 30 + 1] and r.tolist() == [1, 1, 1, 1, 0, 0]
