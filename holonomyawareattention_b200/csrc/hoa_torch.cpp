@@ -111,7 +111,8 @@ bool pools(PyObject* list, const Books& b, Pools* q) {
     const at::Tensor* t = tensor(PyList_GET_ITEM(list, i));
     if (!t || !t->is_cuda() || t->get_device() != b.idx || t->dim() < 2 || t->size(0) != b.n_pages || !t->is_contiguous()) return false;
     q->base[i] = t->data_ptr();
-    q->stride[i] = q->bytes[i] = (long long)t->stride(0) * t->element_size();
+    q->bytes[i] = (long long)t->numel() / b.n_pages * t->element_size();   // (a pool of one page may have any stride)
+    q->stride[i] = (long long)t->stride(0) * t->element_size();
   }
   return true;
 }

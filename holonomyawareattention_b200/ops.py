@@ -777,7 +777,7 @@ def _pool_args(pools, n_pages, idx):
         e = t.element_size()
         st = t.stride(0) * e
         if t.is_contiguous():
-            size.append(st)
+            size.append(t.numel() // max(1, n_pages) * e)      # (not st: a pool of one page may have any stride)
         else:
             p = t[0]
             if not p.is_contiguous() or t.stride(0) < p.numel():

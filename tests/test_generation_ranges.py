@@ -59,3 +59,12 @@ def test_sizes_beyond_int_are_refused_in_python(monkeypatch):
         ops._books(torch.empty(1, 1, dtype=torch.int32).expand(2 ** 16, 2 ** 16 + 1), None, small[0], 4)
     with pytest.raises(ValueError, match="2\\^31"):
         ops._books(small, None, small[0], 2 ** 32 + 1)
+
+
+def test_a_pool_of_one_page_is_as_large_as_its_page():
+    """A pool cut down to one page keeps the stride of the pool it was cut from, and counts as contiguous."""
+    wide = torch.zeros(6, 4, 5)
+    one = wide[::3][:1]
+    assert one.is_contiguous() and one.stride(0) == 60
+    keep, base, stride, size, n = ops._pool_args([one], 1, one.get_device())
+    assert n == 1 and list(keep) == [one.data_ptr(), 240, 80]
