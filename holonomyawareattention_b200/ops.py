@@ -54,7 +54,8 @@ def _contig(t: torch.Tensor, name: str) -> torch.Tensor:
 # only once the stream has run, so every op here queues a 4-byte copy of it to
 # pinned host memory behind its kernels: poll_status() raises for the copies
 # that have landed (the module calls it at every forward), check_status() waits
-# for all of them first (call it after synchronising, e.g. at the end of a run).
+# for the device first (call it at the end of a run).  The generation kernels set
+# a word in mapped host memory instead, which both functions read too.
 # ---------------------------------------------------------------------------
 class _StatusWatch:
     RING = 256
@@ -112,6 +113,9 @@ class _StatusWatch:
             self._poll_locked()
 
     def check(self) -> None:
+        # the whole device: the mapped word has no event behind it, and its kernels run on any stream
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.synchronize(self.dev)
         with self.lock:
             for _, ev, _ in self.pending:
                 ev.synchronize()
@@ -133,13 +137,14 @@ def _watch(dev: torch.device) -> _StatusWatch:
 
 def poll_status(device=None) -> None:
     """Raise HoaError for any finished launch on ``device`` whose device-side wait
-    gave up (HOA_ERR_TIMEOUT).  Does not wait for launches still running."""
+    gave up (HOA_ERR_TIMEOUT), or that found a page or row outside its cache
+    (HOA_ERR_PAGES).  Does not wait for launches still running."""
     _watch(device if device is not None else "cuda").poll()
 
 
 def check_status(device=None) -> None:
-    """Wait for every launch queued so far on ``device`` and raise HoaError if any
-    of them reported HOA_ERR_TIMEOUT."""
+    """Wait for every launch queued so far on ``device``, on all its streams, and raise
+    HoaError if any of them reported HOA_ERR_TIMEOUT or HOA_ERR_PAGES."""
     _watch(device if device is not None else "cuda").check()
 
 

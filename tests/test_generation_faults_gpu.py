@@ -146,3 +146,23 @@ def test_reserve_of_more_tokens_than_an_int_counts():
     torch.cuda.synchronize()
     ops.check_status()
     assert t.tolist() == [[0, 1, -1, -1], [2, 3, -1, -1]] and n.tolist() == [2 ** 31 - 1, 2 ** 30 + 1] and r.tolist() == [1, 1, 1, 1, 0, 0]
+
+
+# ---------------------------------------------------------------------------
+# what check_status waits for
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("side", [False, True])
+def test_check_status_waits_for_the_cache_kernels(side):
+    """A page outside the pool, in a call that is still queued behind other work (on any stream)."""
+    q, kp, vp, table, lens, scale = attn_args(3)
+    bad = table.clone()
+    bad[1, 2] = kp.shape[0]
+    ops.paged_attn_fwd(q, kp, vp, table, lens, scale)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream() if side else torch.cuda.current_stream()):
+        torch.cuda._sleep(200_000_000)
+        ops.paged_attn_fwd(q, kp, vp, bad, lens, scale)
+    with pytest.raises(_lib.HoaError) as e:
+        ops.check_status()
+    assert e.value.status == _lib.HOA_ERR_PAGES
+    ops.check_status()
