@@ -57,6 +57,21 @@ def _contig(t: torch.Tensor, name: str) -> torch.Tensor:
 # for the device first (call it at the end of a run).  The generation kernels set
 # a word in mapped host memory instead, which both functions read too.
 # ---------------------------------------------------------------------------
+# device -> (word, the same as an array): a word in mapped host memory that the generation kernels
+# set themselves (no copy to queue behind a call of a few microseconds), 0 until something went
+# wrong.  Kept for good: its address is handed out once a device and may be in flight at any time.
+_MAPPED = {}
+
+
+def _mapped_word(dev: torch.device):
+    v = _MAPPED.get(dev)
+    if v is None:
+        with torch.inference_mode(False):
+            t = torch.zeros(1, dtype=torch.int32).pin_memory()
+        v = _MAPPED.setdefault(dev, (t, t.numpy()))
+    return v[1]
+
+
 class _StatusWatch:
     RING = 256
 
@@ -68,11 +83,7 @@ class _StatusWatch:
             # the word the stage entry points share: set by a kernel, cleared here
             self.sticky = torch.zeros(1, dtype=torch.int32, device=dev)
             self.host = torch.zeros(self.RING, dtype=torch.int32).pin_memory()
-            # a word in mapped host memory that the cache kernels set themselves (no copy to
-            # queue behind a call of a few microseconds): 0 until something went wrong
-            self.mapped = torch.zeros(1, dtype=torch.int32).pin_memory()
-        self.mapped_np = self.mapped.numpy()
-        self.mapped_ptr = self.mapped.data_ptr()
+        self.mapped = _mapped_word(dev)
         self.pending = collections.deque()        # (slot, event, what)
         self.next = 0
         self.lock = threading.Lock()
@@ -93,9 +104,9 @@ class _StatusWatch:
             self.pending.append((slot, ev, what))
 
     def _poll_locked(self) -> None:
-        st = int(self.mapped_np[0])
+        st = int(self.mapped[0])
         if st != 0:
-            self.mapped_np[0] = 0
+            self.mapped[0] = 0
             _lib.check("a cache operation", st)
         while self.pending and self.pending[0][1].query():
             slot, _, what = self.pending.popleft()
@@ -692,7 +703,7 @@ def _device(idx: int):
     v = _DEVICES.get(idx)
     if v is None:
         v = _DEVICES[idx] = (torch.cuda.get_device_properties(idx).multi_processor_count,
-                             _watch(torch.device("cuda", idx)).mapped_ptr)
+                             _mapped_word(torch.device("cuda", idx)).ctypes.data)
         _host().device(idx, *v)
     return v
 

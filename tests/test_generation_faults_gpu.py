@@ -166,3 +166,18 @@ def test_check_status_waits_for_the_cache_kernels(side):
         ops.check_status()
     assert e.value.status == _lib.HOA_ERR_PAGES
     ops.check_status()
+
+
+def test_status_outlives_its_watch():
+    """The word that the kernels set stays the one that is read when the watch of a device is made anew."""
+    q, kp, vp, table, lens, scale = attn_args(3)
+    ops.paged_attn_fwd(q, kp, vp, table, lens, scale)
+    torch.cuda.synchronize()
+    ops._WATCH.clear()
+    bad = table.clone()
+    bad[0, 0] = -1
+    ops.paged_attn_fwd(q, kp, vp, bad, lens, scale)
+    torch.cuda.synchronize()
+    with pytest.raises(_lib.HoaError) as e:
+        ops.check_status()
+    assert e.value.status == _lib.HOA_ERR_PAGES
