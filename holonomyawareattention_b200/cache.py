@@ -18,11 +18,19 @@ launched.
 """
 from __future__ import annotations
 
+import contextlib
 from typing import List, Optional, Sequence
 
 import torch
 
 from . import _lib, ops
+
+
+@contextlib.contextmanager
+def _plain():
+    """Tensors made here may be updated in place in any mode (those of inference mode only within it)."""
+    with torch.inference_mode(False), torch.no_grad():
+        yield
 
 
 class PathCache:
@@ -45,13 +53,14 @@ class PathCache:
         self.max_tokens = max_tokens
         self.n_pages = rows * self.W if n_pages is None else n_pages
         dev, H, d = w.device, attn.h, attn.d
-        self.k_pages = torch.empty(self.n_pages, H, page, d, dtype=w.dtype, device=dev)
-        self.v_pages = torch.empty_like(self.k_pages)
-        self.table = torch.full((rows, self.W), -1, dtype=torch.int32, device=dev)
-        self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
-        self.refs = torch.zeros(self.n_pages, dtype=torch.int32, device=dev)
-        self.P = torch.eye(d, device=dev).expand(rows, H, d, d).contiguous()
-        self.last = torch.zeros(rows, H * d, dtype=w.dtype, device=dev)
+        with _plain():
+            self.k_pages = torch.empty(self.n_pages, H, page, d, dtype=w.dtype, device=dev)
+            self.v_pages = torch.empty_like(self.k_pages)
+            self.table = torch.full((rows, self.W), -1, dtype=torch.int32, device=dev)
+            self.lens = torch.zeros(rows, dtype=torch.int32, device=dev)
+            self.refs = torch.zeros(self.n_pages, dtype=torch.int32, device=dev)
+            self.P = torch.eye(d, device=dev).expand(rows, H, d, d).contiguous()
+            self.last = torch.zeros(rows, H * d, dtype=w.dtype, device=dev)
         self.tokens: List[int] = [0] * rows
         # which rows hold a page in common, by serial numbers of their own (not the page ids, which
         # only the device knows): enough to tell what is free and what is shared
@@ -238,5 +247,6 @@ def decode(attn, x: torch.Tensor, cache: PathCache) -> torch.Tensor:
                           cache.lens, a_bias=bias, gen_layout=layout, P_out=cache.P)
     o, _ = ops.paged_attn_fwd(qh.view(S, 1, H, d), cache.k_pages, cache.v_pages, cache.table[:, cache.n_shared:], cache.lens,
                               attn.scale, shared=cache.shared, paths=cache.P)
-    cache.last = x.clone() if all(live) else torch.where(cache.lens.view(-1, 1) > 0, x, cache.last)
+    with _plain():
+        cache.last = x.clone() if all(live) else torch.where(cache.lens.view(-1, 1) > 0, x, cache.last)
     return attn.out(o.view(S, H * d))

@@ -181,3 +181,28 @@ def test_status_outlives_its_watch():
     with pytest.raises(_lib.HoaError) as e:
         ops.check_status()
     assert e.value.status == _lib.HOA_ERR_PAGES
+
+
+def test_cache_across_inference_mode():
+    """Made and fed in inference mode, then outside it, and the other way round."""
+    attn = module(96, 2)
+    x = torch.randn(2, 10, 96, device=DEV)
+    outs = []
+    for modes in ((torch.inference_mode, torch.no_grad), (torch.no_grad, torch.inference_mode), (torch.no_grad, torch.no_grad)):
+        got = []
+        with modes[0]():
+            cache = PathCache(attn, rows=3, max_tokens=60, page=16)
+            got.append(prefill(attn, x, cache, [0, 1]))
+            got.append(decode(attn, torch.ones(3, 96, device=DEV), cache))
+        with modes[1]():
+            got.append(prefill(attn, x + 1, cache, [0, 1]))
+            cache.fork([0], [2])
+            got.append(decode(attn, torch.ones(3, 96, device=DEV), cache))
+            cache.share(0, 0)
+        with modes[0]():
+            got.append(prefill(attn, x - 1, cache, [2, 1]))
+            got.append(decode(attn, torch.ones(3, 96, device=DEV), cache))
+        outs.append(got)
+    for got in outs[:2]:
+        assert all(torch.equal(a, b) for a, b in zip(got, outs[2]))
+    ops.check_status()
