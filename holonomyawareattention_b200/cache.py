@@ -119,9 +119,10 @@ class PathCache:
             return
         self._need(sum(1 for r in src if self.tokens[r] % self.page))
         a, b = self._ints(src), self._ints(dst)
+        # (first what writes to the empty rows only, then the state: an error in between leaves it as it was)
+        ops.pages_copy([self.P, self.last], a, b)            # a row of these is a page too
         self.table, self.lens, self.refs = ops.pages_fork([self.k_pages, self.v_pages], self.table, self.lens, self.refs, a, b,
                                                           self.page)
-        ops.pages_copy([self.P, self.last], a, b)            # a row of these is a page too
         for s, t in zip(src, dst):
             full = self.tokens[s] // self.page
             self._held[t] = self._held[s][:full] + self._take(1 if self.tokens[s] % self.page else 0)
@@ -248,5 +249,6 @@ def decode(attn, x: torch.Tensor, cache: PathCache) -> torch.Tensor:
     o, _ = ops.paged_attn_fwd(qh.view(S, 1, H, d), cache.k_pages, cache.v_pages, cache.table[:, cache.n_shared:], cache.lens,
                               attn.scale, shared=cache.shared, paths=cache.P)
     with _plain():
-        cache.last = x.clone() if all(live) else torch.where(cache.lens.view(-1, 1) > 0, x, cache.last)
+        cache.last = x.clone(memory_format=torch.contiguous_format) if all(live) else \
+            torch.where(cache.lens.view(-1, 1) > 0, x, cache.last).contiguous()
     return attn.out(o.view(S, H * d))

@@ -206,3 +206,62 @@ def test_cache_across_inference_mode():
     for got in outs[:2]:
         assert all(torch.equal(a, b) for a, b in zip(got, outs[2]))
     ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+# an error in the middle of an operation
+# ---------------------------------------------------------------------------
+class Boom(Exception):
+    pass
+
+
+def failing(real, after=0):
+    """``real``, but the call after ``after`` good ones raises."""
+    left = [after]
+
+    def call(*a, **k):
+        if left[0] == 0:
+            raise Boom
+        left[0] -= 1
+        return real(*a, **k)
+    return call
+
+
+def test_fork_after_transposed_hidden_states():
+    """decode with hidden states of other strides (a transposed view), then a fork, with and without idle rows."""
+    attn = module(96, 2)
+    x = torch.randn(96, 3, device=DEV)
+    with torch.no_grad():
+        caches = [PathCache(attn, rows=3, max_tokens=60, page=16) for _ in range(2)]
+        for cache, y in zip(caches, (x.t(), x.t().contiguous())):
+            prefill(attn, torch.ones(1, 20, 96, device=DEV), cache, [0])
+            decode(attn, y, cache)
+            cache.fork([0], [2])
+            decode(attn, y, cache)
+            cache.fork([2], [1])
+            decode(attn, y, cache)                                # every row has tokens
+            cache.free([0])
+            cache.fork([1], [0])
+        assert same_state(state_of(caches[0]), state_of(caches[1]))
+        for cache in caches:                                      # (k^ and v^: GEMMs of other layouts round otherwise)
+            assert torch.equal(cache.P[0], cache.P[1]) and torch.equal(cache.last[0], cache.last[1])
+        ops.check_status()
+
+
+@pytest.mark.parametrize("where", ["pages_fork", "pages_copy", "_ints"])
+def test_fork_that_fails_changes_nothing(monkeypatch, where):
+    attn = module(96, 2)
+    with torch.no_grad():
+        cache = PathCache(attn, rows=3, max_tokens=60, page=16)
+        prefill(attn, torch.randn(1, 20, 96, device=DEV), cache, [0])
+        before = state_of(cache)
+        with monkeypatch.context() as m:
+            owner = cache if where == "_ints" else ops
+            m.setattr(owner, where, failing(getattr(owner, where), after=1 if where == "_ints" else 0))
+            with pytest.raises(Boom):
+                cache.fork([0, 0], [1, 2])
+        assert same_state(state_of(cache), before)
+        cache.fork([0, 0], [1, 2])
+        assert cache.tokens == [20] * 3 and cache.lens.tolist() == [20] * 3
+        assert torch.equal(cache.P[1], cache.P[0]) and torch.equal(cache.last[2], cache.last[0])
+        ops.check_status()
