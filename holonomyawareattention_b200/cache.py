@@ -91,6 +91,23 @@ class PathCache:
     def _ints(self, values) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32, device=self.table.device)
 
+    @contextlib.contextmanager
+    def _undo_on_error(self):
+        """The rows are as long as before, should the body raise after it has reserved tokens.  (The device's state is replaced,
+        not changed, so the old one still holds; P and last are the body's to change once nothing can fail any more.)"""
+        state = self.table, self.lens, self.refs, self.tokens
+        held, serial = [len(h) for h in self._held], self._serial
+        try:
+            yield
+        except BaseException:
+            self.table, self.lens, self.refs, self.tokens = state
+            for h, n in zip(self._held, held):
+                del h[n:]
+            for i in range(serial, self._serial):
+                self._count.pop(i, None)
+            self._serial = serial
+            raise
+
     def reserve(self, counts: Sequence[int]) -> None:
         """Row s grows by counts[s] tokens.  Without enough free pages: HoaError with HOA_ERR_PAGES,
         nothing changed (fork: likewise)."""
@@ -183,7 +200,8 @@ def _check(attn, x, cache) -> None:
 def prefill(attn, x: torch.Tensor, cache: PathCache, rows: Sequence[int]) -> torch.Tensor:
     """x (len(rows), T, D): the next T hidden states of the rows, all of them empty or none; their outputs
     (len(rows), T, D).  The link, carry and transport kernels of the forward, k^ and v^ written to the
-    pages, attention over the cache (the shared pages read once)."""
+    pages, attention over the cache (the shared pages read once).  An error leaves the cache as it was
+    (decode: likewise)."""
     rows = cache._rows(rows, "rows")
     if x.dim() != 3 or x.shape[0] != len(rows) or x.shape[1] < 1 or not rows:
         raise ValueError("x must be (len(rows), T, D)")
@@ -198,15 +216,22 @@ def prefill(attn, x: torch.Tensor, cache: PathCache, rows: Sequence[int]) -> tor
     grow = [0] * cache.rows
     for r in rows:
         grow[r] = T
-    cache.reserve(grow)
-    y = torch.empty_like(x)
-    step = max(1, attn.PIECE_TOKENS // T)
-    for i in range(0, len(rows), step):
-        y[i:i + step] = _prefill_rows(attn, x[i:i + step], cache, rows[i:i + step], go_on)
+    with cache._undo_on_error():
+        cache.reserve(grow)
+        y = torch.empty_like(x)
+        P = []
+        step = max(1, attn.PIECE_TOKENS // T)
+        for i in range(0, len(rows), step):
+            y[i:i + step], p = _prefill_rows(attn, x[i:i + step], cache, rows[i:i + step], go_on)
+            P.append(p)
+        idx, P, newest = torch.tensor(rows, device=x.device), torch.cat(P), x[:, -1].contiguous()
+        cache.P.index_copy_(0, idx, P)
+        cache.last.index_copy_(0, idx, newest)
     return y
 
 
 def _prefill_rows(attn, x, cache, rows, go_on):
+    """(outputs, the rows' P after the last token); the cache's pages are written, its P and last are not."""
     B, T, D = x.shape
     H, d = attn.h, attn.d
     idx = torch.tensor(rows, device=x.device)
@@ -228,9 +253,8 @@ def _prefill_rows(attn, x, cache, rows, go_on):
     full = torch.zeros(B, H, L, d, dtype=torch.float32, device=x.device)
     full[:, :, lead:] = o.permute(0, 2, 1, 3)
     out = ops.out_transport(full.view(B * H, L, d), R, C, chunk, B, H, x.dtype)[:, lead:]
-    cache.P[idx] = ops.compose_paths(R[:, -1:].contiguous(), C[:, -1:].contiguous(), 1).view(B, H, d, d)
-    cache.last[idx] = x[:, -1]
-    return attn.out(out)
+    P = ops.compose_paths(R[:, -1:].contiguous(), C[:, -1:].contiguous(), 1).view(B, H, d, d)
+    return attn.out(out), P
 
 
 def decode(attn, x: torch.Tensor, cache: PathCache) -> torch.Tensor:
@@ -241,14 +265,18 @@ def decode(attn, x: torch.Tensor, cache: PathCache) -> torch.Tensor:
     _check(attn, x, cache)
     H, d, S = attn.h, attn.d, cache.rows
     live = [1 if t else 0 for t in cache.tokens]
-    cache.reserve(live)
-    a, bias, layout = attn._edge_generators_nobias(cache.last.unsqueeze(1), x.unsqueeze(1), cache.max_tokens)
-    qkv = attn.qkv(x)
-    _, qh = ops.path_step(a.view(S, -1), cache.P, qkv, H, attn.edge_scale, cache.k_pages, cache.v_pages, cache.table,
-                          cache.lens, a_bias=bias, gen_layout=layout, P_out=cache.P)
-    o, _ = ops.paged_attn_fwd(qh.view(S, 1, H, d), cache.k_pages, cache.v_pages, cache.table[:, cache.n_shared:], cache.lens,
-                              attn.scale, shared=cache.shared, paths=cache.P)
-    with _plain():
-        cache.last = x.clone(memory_format=torch.contiguous_format) if all(live) else \
-            torch.where(cache.lens.view(-1, 1) > 0, x, cache.last).contiguous()
-    return attn.out(o.view(S, H * d))
+    with cache._undo_on_error():
+        cache.reserve(live)
+        a, bias, layout = attn._edge_generators_nobias(cache.last.unsqueeze(1), x.unsqueeze(1), cache.max_tokens)
+        qkv = attn.qkv(x)
+        with _plain():
+            P = torch.empty_like(cache.P)
+            last = x.clone(memory_format=torch.contiguous_format) if all(live) else \
+                torch.where(cache.lens.view(-1, 1) > 0, x, cache.last).contiguous()
+        _, qh = ops.path_step(a.view(S, -1), cache.P, qkv, H, attn.edge_scale, cache.k_pages, cache.v_pages, cache.table,
+                              cache.lens, a_bias=bias, gen_layout=layout, P_out=P)
+        o, _ = ops.paged_attn_fwd(qh.view(S, 1, H, d), cache.k_pages, cache.v_pages, cache.table[:, cache.n_shared:], cache.lens,
+                                  attn.scale, shared=cache.shared, paths=P)
+        y = attn.out(o.view(S, H * d))
+    cache.P, cache.last = P, last
+    return y

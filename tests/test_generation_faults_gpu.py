@@ -265,3 +265,53 @@ def test_fork_that_fails_changes_nothing(monkeypatch, where):
         assert cache.tokens == [20] * 3 and cache.lens.tolist() == [20] * 3
         assert torch.equal(cache.P[1], cache.P[0]) and torch.equal(cache.last[2], cache.last[0])
         ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("where,after", [("paged_attn_fwd", 0), ("compose_paths", 0), ("paged_attn_fwd", 1), ("compose_paths", 1)])
+def test_prefill_that_fails_changes_nothing(monkeypatch, where, after, dtype):
+    """In the first or the second piece of rows, for new rows and for rows that go on: the cache is as it was,
+    and the same prompt then gives what a cache that never failed gives."""
+    attn = module(96, 2, dtype)
+    monkeypatch.setattr(attn, "PIECE_TOKENS", 50)                 # a row a piece
+    x = [torch.randn(3, 40, 96, device=DEV).to(dtype) for _ in range(2)]
+    with torch.no_grad():
+        good, cache = (PathCache(attn, rows=4, max_tokens=100, page=16) for _ in range(2))
+        for c in (good, cache):
+            prefill(attn, x[0][:1, :7], c, [3])
+        for step in range(2):
+            before = state_of(cache)
+            with monkeypatch.context() as m:
+                m.setattr(ops, where, failing(getattr(ops, where), after))
+                with pytest.raises(Boom):
+                    prefill(attn, x[step], cache, [2, 0, 1])
+            assert same_state(state_of(cache), before)
+            want, got = (prefill(attn, x[step], c, [2, 0, 1]) for c in (good, cache))
+            assert torch.equal(want, got) and same_state(state_of(good), state_of(cache))
+        ops.check_status()
+
+
+@pytest.mark.parametrize("where", ["path_step", "paged_attn_fwd", "out", "qkv"])
+@pytest.mark.parametrize("idle", [False, True])
+def test_decode_that_fails_changes_nothing(monkeypatch, where, idle):
+    attn = module(96, 2)
+    rows = 3
+    x = torch.randn(2, rows, 96, device=DEV)
+    with torch.no_grad():
+        good, cache = (PathCache(attn, rows=rows + idle, max_tokens=100, page=16) for _ in range(2))
+        xs = torch.cat([x, torch.zeros(2, idle, 96, device=DEV)], 1)
+        for c in (good, cache):
+            prefill(attn, torch.randn(rows, 16, 96, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)), c, range(rows))
+        for step in range(2):
+            before = state_of(cache)
+            with monkeypatch.context() as m:
+                if where in ("out", "qkv"):
+                    m.setattr(getattr(attn, where), "forward", failing(None))
+                else:
+                    m.setattr(ops, where, failing(getattr(ops, where)))
+                with pytest.raises(Boom):
+                    decode(attn, xs[step], cache)
+            assert same_state(state_of(cache), before)
+            want, got = (decode(attn, xs[step], c) for c in (good, cache))
+            assert torch.equal(want, got) and same_state(state_of(good), state_of(cache))
+        ops.check_status()
