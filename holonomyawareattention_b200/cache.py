@@ -167,9 +167,10 @@ class PathCache:
 
     def compact(self) -> torch.Tensor:
         """The live pages move to the front of the pools; their number (1,) int32, on the device."""
-        self.table, self.refs, live = ops.pages_compact([self.k_pages, self.v_pages], self.table, self.refs)
-        if self.n_shared:
-            self.shared = self.table[self._shared_row, :self.n_shared].clone()
+        # (pages move into free ones only: until the new table is taken, the old one still holds)
+        table, refs, live = ops.pages_compact([self.k_pages, self.v_pages], self.table, self.refs)
+        shared = table[self._shared_row, :self.n_shared].clone() if self.n_shared else self.shared
+        self.table, self.refs, self.shared = table, refs, shared
         return live
 
     def share(self, row: int, tokens: Optional[int] = None) -> int:

@@ -315,3 +315,25 @@ def test_decode_that_fails_changes_nothing(monkeypatch, where, idle):
             want, got = (decode(attn, xs[step], c) for c in (good, cache))
             assert torch.equal(want, got) and same_state(state_of(good), state_of(cache))
         ops.check_status()
+
+
+def test_compact_that_fails_changes_nothing(monkeypatch):
+    """The copy of the shared pages' ids fails after the pages were moved: the old state still holds."""
+    attn = module(96, 2)
+    with torch.no_grad():
+        cache = PathCache(attn, rows=4, max_tokens=60, page=16)
+        prefill(attn, torch.randn(2, 40, 96, device=DEV), cache, [0, 3])
+        cache.free([0])                           # row 3's pages lie behind row 0's
+        cache.fork([3], [1])
+        cache.share(3)
+        before, shared = state_of(cache), cache.shared.clone()
+        with monkeypatch.context() as m:
+            m.setattr(torch.Tensor, "clone", failing(None), raising=False)
+            with pytest.raises(Boom):
+                cache.compact()
+        assert same_state(state_of(cache), before) and torch.equal(cache.shared, shared)
+        live = cache.compact()
+        assert int(live) == len(cache._count) and torch.equal(cache.shared, cache.table[3, :2])
+        y = decode(attn, torch.ones(4, 96, device=DEV), cache)
+        assert torch.isfinite(y).all() and torch.equal(y[3], y[1])
+        ops.check_status()
