@@ -178,6 +178,8 @@ class PathCache:
         rows from now on: the number of tokens shared, a multiple of the page.  Every row that has
         tokens must begin with the same pages, i.e. be a fork.  share(row, 0) ends it."""
         (row,) = self._rows([row], "row")
+        if tokens is not None and tokens < 0:
+            raise ValueError(f"tokens must be at least 0, got {tokens}")
         n = (self.tokens[row] if tokens is None else min(tokens, self.tokens[row])) // self.page
         if n:
             if any(self._held[r][:n] != self._held[row][:n] for r in range(self.rows) if self.tokens[r]):

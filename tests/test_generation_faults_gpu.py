@@ -337,3 +337,17 @@ def test_compact_that_fails_changes_nothing(monkeypatch):
         y = decode(attn, torch.ones(4, 96, device=DEV), cache)
         assert torch.isfinite(y).all() and torch.equal(y[3], y[1])
         ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+def test_share_refuses_a_negative_length():
+    attn = module()
+    with torch.no_grad():
+        cache = PathCache(attn, rows=2, max_tokens=80, page=16)
+        prefill(attn, torch.randn(1, 50, 64, device=DEV), cache, [0])
+        cache.fork([0], [1])
+        for tokens in (-1, -16, -40):
+            with pytest.raises(ValueError, match="tokens"):
+                cache.share(0, tokens)
+            assert cache.n_shared == 0 and cache.shared is None
+        assert cache.share(0, 47) == 32 and cache.share(0, 0) == 0
