@@ -110,12 +110,15 @@ class PathCache:
 
     def reserve(self, counts: Sequence[int]) -> None:
         """Row s grows by counts[s] tokens.  Without enough free pages: HoaError with HOA_ERR_PAGES,
-        nothing changed (fork: likewise)."""
+        nothing changed (fork: likewise).  While pages are shared every row begins with them: an empty
+        row cannot grow, it can become a fork."""
         counts = [int(c) for c in counts]
         if len(counts) != self.rows or any(c < 0 for c in counts):
             raise ValueError(f"counts must be {self.rows} numbers of tokens")
         if any(t + c > self.max_tokens for t, c in zip(self.tokens, counts)):
             raise ValueError(f"a row would pass max_tokens = {self.max_tokens}")
+        if self.n_shared and any(c and not t for t, c in zip(self.tokens, counts)):
+            raise ValueError("a new row does not begin with the shared pages: end the sharing first (share(row, 0))")
         new = [-(-(t + c) // self.page) - len(h) for t, c, h in zip(self.tokens, counts, self._held)]
         self._need(sum(new))
         self.table, self.lens, self.refs = ops.pages_reserve(self.table, self.lens, self.refs, self._ints(counts), self.page)

@@ -351,3 +351,21 @@ def test_share_refuses_a_negative_length():
                 cache.share(0, tokens)
             assert cache.n_shared == 0 and cache.shared is None
         assert cache.share(0, 47) == 32 and cache.share(0, 0) == 0
+
+
+def test_reserve_refuses_an_empty_row_while_pages_are_shared():
+    """Attention reads the shared pages as every row's first ones: a row that begins with others cannot start."""
+    attn = module()
+    with torch.no_grad():
+        cache = PathCache(attn, rows=3, max_tokens=80, page=16)
+        prefill(attn, torch.randn(1, 40, 64, device=DEV), cache, [0])
+        cache.share(0)
+        before = state_of(cache)
+        with pytest.raises(ValueError, match="shared pages"):
+            cache.reserve([1, 0, 5])
+        assert same_state(state_of(cache), before)
+        cache.reserve([1, 0, 0])
+        cache.share(0, 0)
+        cache.reserve([0, 0, 5])
+        assert cache.tokens == [41, 0, 5] and cache.lens.tolist() == [41, 0, 5]
+        ops.check_status()
