@@ -331,8 +331,14 @@ __global__ void __launch_bounds__(kPgThreads) pages_free_kernel(PgFreeArgs p) {
     for (int j = lid; j < W; j += 32) {
       if (j < used) {
         const int id = src[j];
-        // (a page that its row does not own, by a table that was made wrongly, is not taken below zero)
-        if (id < 0 || id >= st.n_pages || atomicSub(&st.refs_out[id], 1) <= 0) pg_fail(p.status);
+        if (id < 0 || id >= st.n_pages) {
+          pg_fail(p.status);
+        } else if (atomicSub(&st.refs_out[id], 1) <= 0) {
+          // a page that its row does not own, by a table that was made wrongly: it stays as it was, at 0 (each of those that
+          // come too late adds what it took, so the sum does not depend on their order)
+          atomicAdd(&st.refs_out[id], 1);
+          pg_fail(p.status);
+        }
       }
       dst[j] = -1;
     }

@@ -369,3 +369,19 @@ def test_reserve_refuses_an_empty_row_while_pages_are_shared():
         cache.reserve([0, 0, 5])
         assert cache.tokens == [41, 0, 5] and cache.lens.tolist() == [41, 0, 5]
         ops.check_status()
+
+
+def test_free_of_a_page_that_nobody_counts():
+    """A table that holds pages with refs 0 (or fewer references than rows): reported, refs stay at 0, and the pages can be
+    taken again."""
+    table, lens, refs = i32([[0, 1, -1], [1, 2, -1], [1, -1, -1]]), i32([8, 7, 3]), i32([1, 1, 0, 0])
+    t, n, r = ops.pages_free(table, lens, refs, i32([0, 1, 2]), 4)
+    with pytest.raises(_lib.HoaError) as e:
+        torch.cuda.synchronize()
+        ops.check_status()
+    assert e.value.status == _lib.HOA_ERR_PAGES
+    assert r.tolist() == [0, 0, 0, 0] and n.tolist() == [0, 0, 0] and bool((t == -1).all())
+    t, n, r = ops.pages_reserve(t, n, r, i32([8, 8, 0]), 4)
+    assert t.tolist() == [[0, 1, -1], [2, 3, -1], [-1, -1, -1]] and r.tolist() == [1, 1, 1, 1]
+    torch.cuda.synchronize()
+    ops.check_status()
