@@ -394,8 +394,8 @@ HOA_DEVICE void load_path(const float* __restrict__ Pg, int d, int pr, int pq, f
     }
 }
 
-// out row g = P q
-HOA_DEVICE void apply_path(const PaArgs& p, long long g, int pr, int pq, const float4 (&P)[4][4], const float4 (&q)[4]) {
+// out row g = P q, or 0 where no key was `seen` (an idle row's P may hold anything)
+HOA_DEVICE void apply_path(const PaArgs& p, long long g, int pr, int pq, const float4 (&P)[4][4], const float4 (&q)[4], bool seen) {
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     float y = 0.f;
@@ -405,7 +405,7 @@ HOA_DEVICE void apply_path(const PaArgs& p, long long g, int pr, int pq, const f
 #pragma unroll
     for (int k = 1; k < 8; k <<= 1) y += __shfl_xor_sync(0xffffffffu, y, k);
     const int r = pr + 32 * x;
-    if (pq == 0 && r < p.d) store_elem(p.out, g * p.d + r, p.out_dtype, y);
+    if (pq == 0 && r < p.d) store_elem(p.out, g * p.d + r, p.out_dtype, seen ? y : 0.f);
   }
 }
 
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_join_kernel(const __gri
     float4 q[4];
 #pragma unroll
     for (int y = 0; y < 4; ++y) q[y] = *reinterpret_cast<const float4*>(so + 4 * (pq + 8 * y));
-    apply_path(p, g, pr, pq, P, q);
+    apply_path(p, g, pr, pq, P, q, l != 0.f);
   } else if (w == 0) {
     if (V == 4 && 4 * lid < d) {
       if (p.out_dtype == HOA_BF16) {
@@ -513,6 +513,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_transport_kernel(const 
   float4 P[4][4];
   load_path<V>(p.paths + g * d * d, d, pr, pq, P);     // (the launches before let this one start after they had waited for P)
   wait_previous();
+  const bool seen = p.lse[g] != -INFINITY;             // (by the join; NaN counts as seen)
   float4 q[4];
   const float* o = p.o + g * d;
 #pragma unroll
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(kPjThreads) paged_attn_transport_kernel(const 
       if (c + 3 < d) q[y].w = o[c + 3];
     }
   }
-  apply_path(p, g, pr, pq, P, q);
+  apply_path(p, g, pr, pq, P, q, seen);
 }
 
 template <int V, int kWpr, bool kPaths>

@@ -414,7 +414,8 @@ int hoa_pages_write(const void* k, const void* v, int src_dtype, const long long
  *   out (B, Tq, H, d) = softmax(q k^T * scale) v, 0 where a query sees no key;
  *   lse (B, Tq, H) = the log of the softmax's sum, -inf there.
  * paths (nullable, Tq = 1): (B, H, d, d) fp32, then out = P o, the inverse
- * transport (core/attention_fast_chunked.py:171).  q and the pools share `dtype`;
+ * transport (core/attention_fast_chunked.py:171); a row that sees no key gives 0
+ * whatever its P holds.  q and the pools share `dtype`;
  * d <= 128; B * Tq * H and (n_shared + W) * page at most 2^31 - 65536.
  * Slots that no query sees may hold anything, NaN included; a NaN or a
  * score of +inf that a query sees makes its out and lse NaN.  The workspace is

@@ -385,3 +385,43 @@ def test_free_of_a_page_that_nobody_counts():
     assert t.tolist() == [[0, 1, -1], [2, 3, -1], [-1, -1, -1]] and r.tolist() == [1, 1, 1, 1]
     torch.cuda.synchronize()
     ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+# rows that are idle
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,H,d", [(5, 2, 96), (4, 3, 50), (700, 2, 48), (400, 3, 25)])
+def test_an_idle_row_gives_zeros_whatever_its_path_holds(B, H, d, dtype):
+    """out is 0 where a query sees no key: NaN and infinities in that row's P do not reach it (few rows: the join applies
+    P; many: a launch of its own)."""
+    page, W = 16, 2
+    kp, vp = pages(B * W, H, page, d, dtype)
+    q = torch.randn(B, 1, H, d, device=DEV).to(dtype)
+    lens = [0 if b % 4 == 1 else 1 + (5 * b) % (W * page) for b in range(B)]
+    idle = torch.tensor([n == 0 for n in lens], device=DEV)
+    P = torch.randn(B, H, d, d, device=DEV)
+    args = (q, kp, vp, i32([[b * W, b * W + 1] for b in range(B)]), i32(lens), 0.2)
+    want = ops.paged_attn_fwd(*args, paths=P)
+    bad = P.clone()
+    bad[idle] = float("nan")
+    bad[1, 0, 0, 0] = float("inf")
+    out, lse = ops.paged_attn_fwd(*args, paths=bad)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert bool((out[idle] == 0).all()) and bool(torch.isneginf(lse[idle]).all())
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_a_row_freed_after_nan_decodes_to_zero():
+    attn = module(96, 2)
+    with torch.no_grad():
+        cache = PathCache(attn, rows=2, max_tokens=40, page=16)
+        x = torch.randn(2, 5, 96, device=DEV)
+        x[1] = float("nan")
+        prefill(attn, x, cache, [0, 1])
+        cache.free([1])
+        y = decode(attn, torch.ones(2, 96, device=DEV), cache)
+        torch.cuda.synchronize()
+        assert torch.isfinite(y[0]).all() and bool((y[1] == 0).all())
+        ops.check_status()
