@@ -29,6 +29,7 @@ struct StepArgs {
   const int* table; long long tstride; const int* lens;
   int B, H, d, page, W, n_pages;
   int* status;
+  long long max_wait;                                      // bound of a wait for a product, SM cycles (wait_bound_cycles())
 };
 
 HOA_DEVICE void st_fail(int* status) {
@@ -211,12 +212,14 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
   float* sum = reinterpret_cast<float*>(sm + L::offSum);
   uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* delta = reinterpret_cast<float*>(sm);
   float* part = reinterpret_cast<float*>(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int d = p.d, dd = d * d;
   if (tid == 0) {
     mbar_init(done, 1);
+    *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -322,14 +325,24 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
-    if (tid == 0) {
+    if (tid == 0 && !bad) {
       tc_fence_after();
       st_product<DP, decltype(smem_left)::value>(sm, tmem, accumulate, done);
     }
   };
+  // A thread that has given up waits for no more products, and thread 0 issues none: the row's chain runs out on what is
+  // there, without touching memory outside the CTA, and the CTA leaves before it stores the row.  (The clock is read
+  // around the wait as well: a try may be suspended for longer than a short bound.)
   auto wait = [&]() {
-    bad |= !mbar_wait(done, phase);
-    phase ^= 1;
+    if (!bad) {
+      const unsigned c0 = (unsigned)clock();
+      bad = !mbar_wait_abortable(done, phase, s_abort, p.max_wait);
+      if (!bad && (unsigned)clock() - c0 > (unsigned)p.max_wait) {
+        bad = true;
+        *s_abort = 1;
+      }
+      if (!bad) phase ^= 1;
+    }
     tc_fence_after();
   };
   using Yes = std::true_type;
@@ -683,6 +696,7 @@ __global__ void __launch_bounds__(kStThreads, 2) path_step_kernel(const __grid_c
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (tid == 0 && bad) mbar_wait(done, phase);                 // the product that it gave up on may still read shared memory
   if (__syncthreads_or(bad) && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, L::kCols);
@@ -720,7 +734,7 @@ extern "C" int hoa_path_step(const float* a, int a_dtype, const float* a_bias, f
     return HOA_ERR_UNSUPPORTED;
   StepArgs s{a, gen_is_banked(a_dtype) ? 1 : 0, stride, a_bias, edge_scale, P, P_out, qkv, qkv_dtype, qkv_stride, qh,
              k_pages, v_pages, dtype, page_strides[0], page_strides[1], page_strides[2], table, table_stride, lens,
-             B, H, d, page, W, n_pages, status};
+             B, H, d, page, W, n_pages, status, wait_bound_cycles()};
   static const int num_sms = []() {                        // of the device that calls first: every GPU here is the same
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)

@@ -425,3 +425,65 @@ def test_a_row_freed_after_nan_decodes_to_zero():
         torch.cuda.synchronize()
         assert torch.isfinite(y[0]).all() and bool((y[1] == 0).all())
         ops.check_status()
+
+
+# ---------------------------------------------------------------------------
+# waits that give up
+# ---------------------------------------------------------------------------
+def test_path_step_surfaces_a_timed_out_wait():
+    """With a short wait bound the step gives up on its products, leaves, and reports it; with the default bound the same
+    call then gives the first result.  Seven products a head: the time of a call that gives up is bounded too."""
+    B, H, d = 40, 4, 120
+    g = torch.Generator(device=DEV).manual_seed(0)
+    a = torch.randn(B, H * d * (d - 1) // 2, device=DEV, generator=g)
+    P = torch.linalg.qr(torch.randn(B, H, d, d, device=DEV, generator=g))[0].contiguous()
+    qkv = torch.randn(B, 3 * H * d, device=DEV, generator=g)
+    table, lens = i32([[b] for b in range(B)]), i32([3] * B)
+
+    def step():
+        kp = torch.zeros(B, H, 4, d, device=DEV)
+        return ops.path_step(a, P, qkv, H, 0.5, kp, kp.clone(), table, lens)
+
+    want = step()
+    torch.cuda.synchronize()
+    ops.check_status()
+    ops.set_wait_bound(1)
+    try:
+        step()
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.HoaError) as e:
+            ops.check_status()
+        assert e.value.status == _lib.HOA_ERR_TIMEOUT
+    finally:
+        ops.set_wait_bound(0)
+    for _ in range(3):
+        got = step()
+        torch.cuda.synchronize()
+        ops.check_status()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("Tq", [30, 200])
+def test_paged_attention_surfaces_a_timed_out_wait(Tq):
+    """The tcgen05 kernel, one and two tiles of rows."""
+    H, d, page, W = 2, 96, 64, 40
+    kp, vp = pages(2 * W, H, page, d)
+    q = torch.randn(2, Tq, H, d, device=DEV).to(BF)
+    table, lens = i32([[b * W + j for j in range(W)] for b in range(2)]), i32([W * page, W * page - 9])
+    args = (q, kp, vp, table, lens, 0.1)
+    want = ops.paged_attn_fwd(*args)
+    torch.cuda.synchronize()
+    ops.check_status()
+    ops.set_wait_bound(1)
+    try:
+        ops.paged_attn_fwd(*args)
+        torch.cuda.synchronize()
+        with pytest.raises(_lib.HoaError) as e:
+            ops.check_status()
+        assert e.value.status == _lib.HOA_ERR_TIMEOUT
+    finally:
+        ops.set_wait_bound(0)
+    got = ops.paged_attn_fwd(*args)
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
