@@ -10,7 +10,8 @@ hoa_debug_bounds) for a range outside its buffer, skipping that access.
 The library exposes only the C ABI declared in include/hoa.h (no torch types),
 so it can be bound from ctypes, cgo, JNI or C/C++ alike.  Beside it, the host
 compiler makes _hoa_torch.so (csrc/hoa_torch.cpp): the ordinary case of the
-generation operators' Python side, in C++ against torch's headers.
+generation operators' Python side, in C++ against torch's headers.  The library
+does not need it: without it the Python functions take every call.
 """
 from __future__ import annotations
 
@@ -19,6 +20,7 @@ import os
 import shutil
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -28,6 +30,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhoa.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 LIB_TORCH = os.path.join(PKG, "_hoa_torch.so")
+TORCH_STAMP = os.path.join(BUILD_DIR, "torch_stamp")
 LIB_DEBUG = os.path.join(PKG, "libhoa_debug.so")
 BUILD_DIR_DEBUG = os.path.join(PKG, "_build", "debug_bounds")
 
@@ -65,10 +68,18 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), debug_boun
     build_dir = BUILD_DIR_DEBUG if debug_bounds else BUILD_DIR
     if debug_bounds:
         extra_flags = (*extra_flags, "-DHOA_DEBUG_BOUNDS")
+    if force or not up_to_date(lib):
+        _compile(lib, build_dir, extra_flags, verbose)
     if not debug_bounds:
-        build_torch(force)
-    if not force and up_to_date(lib):
-        return lib
+        # the library is whole without its torch side, which only makes calls from Python shorter
+        try:
+            build_torch(force)
+        except Exception as e:
+            warnings.warn(f"{lib} is built, _hoa_torch.so is not: the Python functions take its calls ({e})", RuntimeWarning)
+    return lib
+
+
+def _compile(lib: str, build_dir: str, extra_flags, verbose: bool) -> None:
     nvcc = nvcc_path()
     os.makedirs(build_dir, exist_ok=True)
     objs = []
@@ -95,14 +106,29 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), debug_boun
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, lib)
-    return lib
+
+
+def _torch_stamp() -> str:
+    import torch
+    return f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
+def torch_up_to_date() -> bool:
+    """Whether _hoa_torch.so is there, newer than its sources, and made against this torch and Python."""
+    src = (os.path.join(CSRC, "hoa_torch.cpp"), os.path.join(INCLUDE, "hoa.h"))
+    if not os.path.exists(LIB_TORCH) or any(os.path.getmtime(p) > os.path.getmtime(LIB_TORCH) for p in src):
+        return False
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read() == _torch_stamp()
+    except OSError:
+        return False
 
 
 def build_torch(force: bool = False) -> str:
     """_hoa_torch.so, against the torch that is importable here."""
     src = os.path.join(CSRC, "hoa_torch.cpp")
-    if not force and os.path.exists(LIB_TORCH) and \
-            all(os.path.getmtime(p) <= os.path.getmtime(LIB_TORCH) for p in (src, os.path.join(INCLUDE, "hoa.h"))):
+    if not force and torch_up_to_date():
         return LIB_TORCH
     import sysconfig
 
@@ -120,6 +146,9 @@ def build_torch(force: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"the host compiler failed on {src}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_TORCH)
+    os.makedirs(os.path.dirname(TORCH_STAMP), exist_ok=True)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(_torch_stamp())
     return LIB_TORCH
 
 

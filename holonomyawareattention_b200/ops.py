@@ -11,6 +11,7 @@ import collections
 import ctypes
 import math
 import threading
+import warnings
 from typing import Optional, Tuple
 
 import torch
@@ -679,14 +680,22 @@ _HOST_FNS = ("hoa_pages_workspace_bytes", "hoa_pages_reserve", "hoa_pages_fork",
              "hoa_paged_attn_workspace_bytes", "hoa_paged_attn_fwd", "hoa_path_step")
 
 
+class _Declines:
+    """Stands in for a C++ side that cannot be loaded: no call is ordinary."""
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
 def _host():
     global _HOST
     if _HOST is None:
         try:
             from . import _hoa_torch as m
         except ImportError as e:
-            raise RuntimeError(f"_hoa_torch.so cannot be loaded ({e}): build it with "
-                               "`python -m holonomyawareattention_b200._build`") from None
+            warnings.warn(f"_hoa_torch.so cannot be loaded ({e}): the generation operators' host side runs in Python, about 10 us "
+                          "a call slower.  Build it with `python -m holonomyawareattention_b200._build`", RuntimeWarning)
+            _HOST = _Declines()
+            return _HOST
         m.bind(*(ctypes.cast(_fn(n), ctypes.c_void_p).value for n in _HOST_FNS))
         _HOST = m
     return _HOST
