@@ -27,10 +27,14 @@ from . import _lib, ops
 
 
 @contextlib.contextmanager
-def _plain():
-    """Tensors made here may be updated in place in any mode (those of inference mode only within it)."""
+def _outside_inference_mode():
     with torch.inference_mode(False), torch.no_grad():
         yield
+
+
+def _plain():
+    """Tensors made under this may be updated in place in any mode (those of inference mode only within it)."""
+    return _outside_inference_mode() if torch.is_inference_mode_enabled() else contextlib.nullcontext()
 
 
 class PathCache:
@@ -224,23 +228,23 @@ def prefill(attn, x: torch.Tensor, cache: PathCache, rows: Sequence[int]) -> tor
         grow[r] = T
     with cache._undo_on_error():
         cache.reserve(grow)
-        y = torch.empty_like(x)
-        P = []
+        y, P = torch.empty_like(x), []
+        idx = torch.tensor(rows, device=x.device)
         step = max(1, attn.PIECE_TOKENS // T)
         for i in range(0, len(rows), step):
-            y[i:i + step], p = _prefill_rows(attn, x[i:i + step], cache, rows[i:i + step], go_on)
+            y[i:i + step], p = _prefill_rows(attn, x[i:i + step], cache, idx[i:i + step], go_on)
             P.append(p)
-        idx, P, newest = torch.tensor(rows, device=x.device), torch.cat(P), x[:, -1].contiguous()
+        P = P[0] if len(P) == 1 else torch.cat(P)
         cache.P.index_copy_(0, idx, P)
-        cache.last.index_copy_(0, idx, newest)
+        cache.last.index_copy_(0, idx, x[:, -1])
     return y
 
 
-def _prefill_rows(attn, x, cache, rows, go_on):
-    """(outputs, the rows' P after the last token); the cache's pages are written, its P and last are not."""
+def _prefill_rows(attn, x, cache, idx, go_on):
+    """Rows ``idx`` (on the device): (outputs, their P after the last token).  The cache's pages are written, its P and last
+    are not."""
     B, T, D = x.shape
     H, d = attn.h, attn.d
-    idx = torch.tensor(rows, device=x.device)
     # rows that go on: the chain starts at the newest cached token (its P is the carry), whose edge
     # leads to the first new one; `lead` positions are recomputed and left out below
     lead = 1 if go_on else 0
