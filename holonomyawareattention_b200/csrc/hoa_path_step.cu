@@ -59,13 +59,13 @@ HOA_DEVICE void st_fail(int* status) {
 // from shared memory, where the same slabs are also the K-major operand.  No matrix
 // is kept in registers between products: a thread owns a row and every other 16
 // columns, and reads A and A2 back from their own halves (A from T) - 2^-22 of them,
-// as the products.  TMEM: D, left hi and lo, 2 DP of the 512 columns, and 64 KB of
-// shared memory at d = 120, so two CTAs run on an SM and one's products overlap the
-// other's element work.
+// as the products.  TMEM: D, left hi and lo, 2 DP of the 512 columns, and 98 KB of
+// shared memory at d = 120 (64 of them the right factor, 28 the next row's generators),
+// so two CTAs run on an SM and one's products overlap the other's element work.
 //
-// Measured at 128 rows x 24 heads of 120 (446 MB, 42.7 GFLOP of fp32-accurate work): 255 us, 1.75 TB/s and 167 TFLOP/s,
-// against 2.9 ms on the CUDA cores; 256 heads of 96: 21 us, one head's latency (22.8K cycles from its generators to its
-// outputs).  The tensor pipe is busy 27%, the schedulers issue 50%: the rest is each CTA's chain of products (1.5K cycles
+// Measured at 128 rows x 24 heads of 120 (446 MB, 42.7 GFLOP of fp32-accurate work): 266 us, 1.68 TB/s and 160 TFLOP/s,
+// against 2.9 ms on the CUDA cores; 256 heads of 96: 20 us, one head's latency (22.8K cycles from its generators to its
+// outputs).  The tensor pipe is busy 25%, the schedulers issue 48%: the rest is each CTA's chain of products (1.5K cycles
 // each) and the element work between them (split, join, store: 2 to 5K).  More threads a row (384, 512) spill and are
 // slower (283, 292 us), so are 8 columns a chunk (262) and a rolled loop over the products (292: a product takes the
 // issuing lane about 95 cycles either way, but rolled they no longer follow one another closely).

@@ -418,7 +418,9 @@ int hoa_pages_write(const void* k, const void* v, int src_dtype, const long long
  * whatever its P holds.  q and the pools share `dtype`;
  * d <= 128; B * Tq * H and (n_shared + W) * page at most 2^31 - 65536.
  * Slots that no query sees may hold anything, NaN included; a NaN or a
- * score of +inf that a query sees makes its out and lse NaN.  The workspace is
+ * score of +inf that a query sees makes its out and lse NaN.  (A NaN or infinity in
+ * v also reaches, as 0 times it, queries that do not see it but share a tile of keys
+ * and rows with one that does.)  The workspace is
  * 16-byte aligned; calls that may overlap on the GPU use different ones.
  */
 size_t hoa_paged_attn_workspace_bytes(int B, int Tq, int H, int Hk, int d, int page, int n_shared, int W, int num_sms);
