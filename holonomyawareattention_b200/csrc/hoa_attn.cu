@@ -12,6 +12,10 @@
 
 namespace hoa {
 
+// hoa_attn_tc.cu: v row-major (v_rows) or transposed; lse may be null
+int attn_tc(const void* qh, const void* kh, const void* vh, bool v_rows, float* o, float* lse, int* status,
+            float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, void* stream);
+
 constexpr int kBQ = 64, kBK = 64, kAttnThreads = 256;
 constexpr int kLDT = kBQ + 4;   // row stride of the transposed tiles (keeps float4 alignment)
 
@@ -26,6 +30,7 @@ struct AttnArgs {
   const void* qh; const void* kh; const void* vh; int hat_dtype;
   float* o; float scale;
   int Tq, Tk, q_offset, d;   // query rows are global positions q_offset .. q_offset + Tq - 1
+  float* lse;                // (BH, Tq) log-sum-exp of the scaled scores, or null
 };
 
 template <int N>
@@ -169,6 +174,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_fwd_simt_kernel(AttnArgs p)
     if (t >= Tq || !HOA_IN(((long long)chain * Tq + t) * d, d, BH * Tq * d)) continue;
     const float inv = 1.f / fmaxf(lrow[i], 1e-20f);
     float* orow = p.o + ((long long)chain * Tq + t) * d;
+    if (p.lse != nullptr && tx == 0) p.lse[(long long)chain * Tq + t] = mrow[i] + logf(lrow[i]);
 #pragma unroll
     for (int j = 0; j < CPT; ++j) {
       const int e = tx * CPT + j;
@@ -192,14 +198,14 @@ int launch_attn(const AttnArgs& a, int BH, cudaStream_t s) {
 
 using namespace hoa;
 
-extern "C" int hoa_attn_fwd(const void* qh, const void* kh, const void* vh, int hat_dtype,
-                            float* o, float softmax_scale, int BH, int Tq, int Tk, int q_offset,
-                            int d, void* stream) {
+namespace hoa {
+int attn_simt(const void* qh, const void* kh, const void* vh, int hat_dtype, float* o, float* lse, float softmax_scale,
+              int BH, int Tq, int Tk, int q_offset, int d, void* stream) {
   if (!qh || !kh || !vh || !o || BH < 1 || Tq < 1 || Tk < 1 || d < 1) return HOA_ERR_INVALID_ARG;
   if (q_offset < 0 || q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
   if (hat_dtype != HOA_F32 && hat_dtype != HOA_BF16) return HOA_ERR_UNSUPPORTED;
   if (BH > 65535) return HOA_ERR_UNSUPPORTED;
-  AttnArgs a{qh, kh, vh, hat_dtype, o, softmax_scale, Tq, Tk, q_offset, d};
+  AttnArgs a{qh, kh, vh, hat_dtype, o, softmax_scale, Tq, Tk, q_offset, d, lse};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int da = ((d + 15) / 16) * 16;
   switch (da) {
@@ -213,4 +219,21 @@ extern "C" int hoa_attn_fwd(const void* qh, const void* kh, const void* vh, int 
     case 128: return launch_attn<128>(a, BH, s);
     default: return HOA_ERR_UNSUPPORTED;
   }
+}
+}  // namespace hoa
+
+extern "C" int hoa_attn_fwd(const void* qh, const void* kh, const void* vh, int hat_dtype,
+                            float* o, float softmax_scale, int BH, int Tq, int Tk, int q_offset,
+                            int d, void* stream) {
+  return attn_simt(qh, kh, vh, hat_dtype, o, nullptr, softmax_scale, BH, Tq, Tk, q_offset, d, stream);
+}
+
+extern "C" int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, float* o, float* lse,
+                                float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, int* status, void* stream) {
+  if (!lse) return HOA_ERR_INVALID_ARG;
+  // the tensor-core form takes rows of whole 16-byte pieces (TMA), from 16-byte boundaries
+  const bool aligned = ((reinterpret_cast<uintptr_t>(qh) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vh)) & 15) == 0;
+  if (dtype == HOA_BF16 && d % 8 == 0 && d <= 128 && aligned)
+    return attn_tc(qh, kh, vh, true, o, lse, status, softmax_scale, BH, Tq, Tk, q_offset, d, stream);
+  return attn_simt(qh, kh, vh, dtype, o, lse, softmax_scale, BH, Tq, Tk, q_offset, d, stream);
 }

@@ -35,13 +35,15 @@ using namespace sm100;
 constexpr int kFaThreads = 320;
 constexpr int kFaRescaleLog2 = 8;
 
-template <int DP16>
+// kVRows: V comes row-major (keys, d), as the training forward has it, and is the MN-major right operand of P V; else
+// transposed (d, keys), the K-major one.
+template <int DP16, bool kVRows>
 struct FaLayout {
   static constexpr int NKB = (DP16 + 63) / 64;        // 64-column boxes of a Q or K tile
   static constexpr int kBlk = 128 * 128;              // bytes: 128 rows x 128 B
   static constexpr int kQ = NKB * kBlk;               // one Q (or K) tile
   static constexpr int kVblk = DP16 * 128;            // one 64-key box of V^T
-  static constexpr int kStage = kQ + 2 * kVblk;       // K tile + V^T tile (128 keys)
+  static constexpr int kStage = kQ + (kVRows ? kQ : 2 * kVblk);   // K tile + V (or V^T) tile (128 keys)
   static constexpr int NS = 2;
   static constexpr int offQ = 0;                      // Q tiles 0 and 1
   static constexpr int offStage = 2 * kQ;
@@ -60,6 +62,7 @@ struct AttnTcArgs {
   int Tq, Tk, q_offset, d;   // query rows are global positions q_offset .. q_offset + Tq - 1
   float scale_log2;
   long long max_wait;        // bound of the abortable waits, SM cycles (wait_bound_cycles())
+  float* lse;                // (BH, Tq) log-sum-exp of the scaled scores, or null
 };
 
 HOA_DEVICE uint32_t pack_bf16x2(float lo, float hi) {
@@ -70,11 +73,11 @@ HOA_DEVICE uint32_t pack_bf16x2(float lo, float hi) {
 // key tiles (of 128) that the query rows starting at global position gq0 see
 HOA_DEVICE int fa_key_tiles(int gq0, int Tk) { return min((gq0 + 127) / 128, (Tk - 1) / 128) + 1; }
 
-template <int DP16>
+template <int DP16, bool kVRows>
 __global__ void __launch_bounds__(kFaThreads, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                const __grid_constant__ CUtensorMap tv, AttnTcArgs p) {
-  using L = FaLayout<DP16>;
+  using L = FaLayout<DP16, kVRows>;
   extern __shared__ uint8_t smem_raw[];
   // 1024-aligned base by pointer arithmetic on the shared array, so that the
   // compiler keeps every derived pointer in the shared address space
@@ -128,7 +131,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
           for (int kb = 0; kb < L::NKB; ++kb)
             tma_load_3d(sm + L::offQ + i * L::kQ + kb * L::kBlk, &tq, q_full, kb * 64,
                         (2 * pair + i) * 128, chain);
-      const uint32_t v_bytes = 2u * 64u * (uint32_t)p.d * 2u;
+      const uint32_t v_bytes = kVRows ? kq : 2u * 64u * (uint32_t)p.d * 2u;
       int issued[2] = {0, 0};
       for (int j = 0; j < nkt; ++j) {
         const int s = j & 1;
@@ -136,8 +139,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
         uint8_t* st = sm + L::offStage + s * L::kStage;
         mbar_arrive_expect_tx(&kv_full[s], kq + v_bytes);
         for (int kb = 0; kb < L::NKB; ++kb) tma_load_3d(st + kb * L::kBlk, &tk, &kv_full[s], kb * 64, j * 128, chain);
-        tma_load_3d(st + L::kQ, &tv, &kv_full[s], j * 128, 0, chain);
-        tma_load_3d(st + L::kQ + L::kVblk, &tv, &kv_full[s], j * 128 + 64, 0, chain);
+        if (kVRows) {
+          for (int kb = 0; kb < L::NKB; ++kb) tma_load_3d(st + L::kQ + kb * L::kBlk, &tv, &kv_full[s], kb * 64, j * 128, chain);
+        } else {
+          tma_load_3d(st + L::kQ, &tv, &kv_full[s], j * 128, 0, chain);
+          tma_load_3d(st + L::kQ + L::kVblk, &tv, &kv_full[s], j * 128 + 64, 0, chain);
+        }
         issued[s] = j + 1;
       }
       // copies in flight land before the CTA exits (the last fill of each stage)
@@ -150,7 +157,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
     // ------------------------------------------------------------------ MMA
     if (lid == 0) {
       constexpr uint32_t idS = make_idesc(kFmtBF16, 128, 128);
-      constexpr uint32_t idO = make_idesc(kFmtBF16, 128, DP16);
+      constexpr uint32_t idO = make_idesc(kFmtBF16, 128, DP16, kVRows);
       constexpr int KSTEPS = DP16 / 16;
       const uint64_t dQ[2] = {desc_sw128(smem_u32(sm + L::offQ)), desc_sw128(smem_u32(sm + L::offQ + L::kQ))};
       const uint32_t colS[2] = {tmem + L::colS0, tmem + L::colS1};
@@ -162,7 +169,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
         if (!ok) break;
         tc_fence_after();
         const uint32_t st = smem_u32(sm + L::offStage + s * L::kStage);
-        const uint64_t dK = desc_sw128(st), dV = desc_sw128(st + L::kQ);
+        const uint64_t dK = desc_sw128(st), dV = kVRows ? desc_sw128_mn(st + L::kQ, L::kBlk) : desc_sw128(st + L::kQ);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (j >= n_t[i]) continue;
@@ -181,7 +188,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t boff = (uint64_t)(((kk >> 2) * L::kVblk + (kk & 3) * 32) >> 4);
+            const uint64_t boff = (uint64_t)((kVRows ? kk * 2048 : (kk >> 2) * L::kVblk + (kk & 3) * 32) >> 4);
             mma_bf16_ts(colO[i], colS[i] + kk * 8, dV + boff, idO, (j > 0 || kk > 0) ? 1u : 0u);
           }
           tc_commit(&pv_done[i]);
@@ -279,6 +286,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
       // (debug build) the output row inside o, else not written
       const bool o_ok = lrow < p.Tq &&
                         HOA_IN(((long long)chain * p.Tq + lrow) * p.d, p.d, (long long)gridDim.y * p.Tq * p.d);
+      if (p.lse != nullptr && o_ok && !bad)
+        p.lse[(long long)chain * p.Tq + lrow] = (m_ref + log2f(l_run)) * 0.6931471805599453f;
 #pragma unroll
       for (int c16 = 0; c16 < DP16 / 16; ++c16) {
         float ov[16];
@@ -295,7 +304,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
   }
 
   bad = __syncthreads_or(bad || *s_abort != 0);
-  if (bad && tid == 0 && p.status != nullptr) atomicExch(p.status, HOA_ERR_TIMEOUT);
+  if (bad && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;   // (may be mapped host memory)
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
@@ -334,16 +343,50 @@ static bool make_map(CUtensorMap* m, const void* base, uint64_t x, uint64_t y, u
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP16>
+template <int DP16, bool kVRows>
 static int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                      const AttnTcArgs& a, int BH, cudaStream_t s) {
-  using L = FaLayout<DP16>;
-  if (cudaFuncSetAttribute(attn_tc_kernel<DP16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  using L = FaLayout<DP16, kVRows>;
+  if (cudaFuncSetAttribute(attn_tc_kernel<DP16, kVRows>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            L::kAlloc) != cudaSuccess)
     return HOA_ERR_LAUNCH;
   dim3 grid((unsigned)ceil_div(ceil_div(a.Tq, 128), 2), (unsigned)BH);
-  attn_tc_kernel<DP16><<<grid, kFaThreads, L::kAlloc, s>>>(mq, mk, mv, a);
+  attn_tc_kernel<DP16, kVRows><<<grid, kFaThreads, L::kAlloc, s>>>(mq, mk, mv, a);
   return launch_status();
+}
+
+template <bool kVRows>
+static int dispatch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnTcArgs& a, int BH,
+                       cudaStream_t s) {
+  switch ((a.d + 15) / 16) {
+    case 1: return launch_tc<16, kVRows>(mq, mk, mv, a, BH, s);
+    case 2: return launch_tc<32, kVRows>(mq, mk, mv, a, BH, s);
+    case 3: return launch_tc<48, kVRows>(mq, mk, mv, a, BH, s);
+    case 4: return launch_tc<64, kVRows>(mq, mk, mv, a, BH, s);
+    case 5: return launch_tc<80, kVRows>(mq, mk, mv, a, BH, s);
+    case 6: return launch_tc<96, kVRows>(mq, mk, mv, a, BH, s);
+    case 7: return launch_tc<112, kVRows>(mq, mk, mv, a, BH, s);
+    case 8: return launch_tc<128, kVRows>(mq, mk, mv, a, BH, s);
+    default: return HOA_ERR_UNSUPPORTED;
+  }
+}
+
+// vh: (BH, Tk, d) for v_rows, else (BH, d, hoa_vt_stride(Tk)); lse may be null.
+int attn_tc(const void* qh, const void* kh, const void* vh, bool v_rows, float* o, float* lse, int* status,
+            float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, void* stream) {
+  if (!qh || !kh || !vh || !o || BH < 1 || Tq < 1 || Tk < 1 || d < 1) return HOA_ERR_INVALID_ARG;
+  if (q_offset < 0 || q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (BH > 65535 || d > 128 || d % 8 != 0) return HOA_ERR_UNSUPPORTED;
+  const uint64_t tp = (uint64_t)hoa_vt_stride(Tk);
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, qh, d, Tq, BH, (uint64_t)d * 2, (uint64_t)Tq * d * 2, 128) ||
+      !make_map(&mk, kh, d, Tk, BH, (uint64_t)d * 2, (uint64_t)Tk * d * 2, 128) ||
+      !(v_rows ? make_map(&mv, vh, d, Tk, BH, (uint64_t)d * 2, (uint64_t)Tk * d * 2, 128)
+               : make_map(&mv, vh, Tk, d, BH, tp * 2, tp * d * 2, (uint32_t)d)))
+    return HOA_ERR_INVALID_ARG;
+  AttnTcArgs a{o, status, Tq, Tk, q_offset, d, softmax_scale * 1.4426950408889634f, wait_bound_cycles(), lse};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return v_rows ? dispatch_tc<true>(mq, mk, mv, a, BH, s) : dispatch_tc<false>(mq, mk, mv, a, BH, s);
 }
 
 }  // namespace hoa
@@ -357,28 +400,5 @@ extern "C" int hoa_vt_stride(int T) { return ((T + 7) / 8) * 8; }
 extern "C" int hoa_attn_tc_fwd(const void* qh, const void* kh, const void* vhT, float* o,
                                int* status, float softmax_scale, int BH, int Tq, int Tk,
                                int q_offset, int d, void* stream) {
-  if (!qh || !kh || !vhT || !o || BH < 1 || Tq < 1 || Tk < 1 || d < 1) return HOA_ERR_INVALID_ARG;
-  if (q_offset < 0 || q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
-  if (BH > 65535 || d > 128 || d % 8 != 0) return HOA_ERR_UNSUPPORTED;
-  const int dp16 = ((d + 15) / 16) * 16;
-  const uint64_t tp = (uint64_t)hoa_vt_stride(Tk);
-  CUtensorMap mq, mk, mv;
-  if (!make_map(&mq, qh, d, Tq, BH, (uint64_t)d * 2, (uint64_t)Tq * d * 2, 128) ||
-      !make_map(&mk, kh, d, Tk, BH, (uint64_t)d * 2, (uint64_t)Tk * d * 2, 128) ||
-      !make_map(&mv, vhT, Tk, d, BH, tp * 2, tp * d * 2, (uint32_t)d))
-    return HOA_ERR_INVALID_ARG;
-  AttnTcArgs a{o, status, Tq, Tk, q_offset, d, softmax_scale * 1.4426950408889634f,
-               wait_bound_cycles()};
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  switch (dp16) {
-    case 16: return launch_tc<16>(mq, mk, mv, a, BH, s);
-    case 32: return launch_tc<32>(mq, mk, mv, a, BH, s);
-    case 48: return launch_tc<48>(mq, mk, mv, a, BH, s);
-    case 64: return launch_tc<64>(mq, mk, mv, a, BH, s);
-    case 80: return launch_tc<80>(mq, mk, mv, a, BH, s);
-    case 96: return launch_tc<96>(mq, mk, mv, a, BH, s);
-    case 112: return launch_tc<112>(mq, mk, mv, a, BH, s);
-    case 128: return launch_tc<128>(mq, mk, mv, a, BH, s);
-    default: return HOA_ERR_UNSUPPORTED;
-  }
+  return attn_tc(qh, kh, vhT, false, o, nullptr, status, softmax_scale, BH, Tq, Tk, q_offset, d, stream);
 }

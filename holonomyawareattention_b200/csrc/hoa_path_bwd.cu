@@ -1,0 +1,874 @@
+// Gradients through the path (the reference differentiates core/attention_fast_chunked.py:86-110
+// and :171 with autograd): of the generators, and of q, k, v.
+//
+//   P_{t+1} = G_t P_t, G_t = expm(A_t), A_t = skew(edge_scale a_t)
+//   q^ = P^T q, k^ = P^T k, v^ = P^T v, out = P o
+//
+// The gradient of P_s from its own uses has rank 4; with do^ = P^T dout,
+//   P_s^T dP_s = q^ dq^T + k^ dk^T + v^ dv^T + do^ o^T      (vectors of position s).
+// Every P is orthogonal, so seen from the first position the gradients of all later uses of
+// G_t simply add up:  Z_t = sum_{s > t} skew(P_s^T dP_s), skew(X) = X - X^T, and
+//   W_t = P_t Z_t P_t^T,   M_t = phi(ad_A) W_t,  phi(z) = (e^z - 1) / z,  ad_A X = A X - X A,
+//   da_t[i, j] = edge_scale M_t[i, j] (i < j);   dq = P dq^, dk = P dk^, dv = P dv^
+// (the derivative of expm at A is G times the integral of e^{-sA} . e^{sA} over s in [0, 1]).
+// The closing edge t = T - 1 is on no path: its gradient is 0.
+//
+// P_t = R_t C_k as the forward left them.  The sums run in the chunk's frame, Y = C Z C^T,
+// so that W = R Y R^T takes R alone.  Four kernels, over runs of at most 32 positions:
+//   sums    S_run = sum over the run of skew(X^T Y)               (one CTA a run)
+//   suffix  S_run <- sum of all later runs                        (fp64, one thread an entry)
+//   scan    Y_t for every position of a run, from its last one back (one CTA a run)
+//   main    W, M, da, dq, dk, dv of every position                (tcgen05, below)
+#include "hoa_split_f16.cuh"
+
+namespace hoa {
+using namespace sm100;
+
+constexpr int kPbRun = 32;
+
+struct PathBwdArgs {
+  const float* a; int banked, stride; const float* a_bias; float edge_scale;
+  const float* R; const float* C; int chunk, K, rpc, NR;       // runs of a chunk, of a chain
+  const void* x[3]; const float* o;                            // q^, k^, v^ (BH, T, d) in dtype, o in fp32
+  const void* y[4];                                            // dq^, dk^, dv^, do^
+  int dtype;
+  float* da; void* dqkv; int out_dtype;
+  int B, H, T, d;
+  float* S;                                                    // (BH, NR, d, d)
+  float* Y; float* F;                                          // of a group of runs: (runs, kPbRun, d, d), (runs, kPbRun, 3, d)
+  float4* V;                                                   // two old iterates a CTA (main, large norms)
+  long long run0; int runs;                                    // the group
+  int* status;
+  long long max_wait;
+};
+
+// chain, positions [t0, t1) and chunk of run r
+struct PbRun { int chain, t0, t1, k; };
+HOA_DEVICE PbRun pb_run(const PathBwdArgs& p, long long r) {
+  PbRun x;
+  x.chain = (int)(r / p.NR);
+  const int i = (int)(r - (long long)x.chain * p.NR);
+  x.k = i / p.rpc;
+  x.t0 = x.k * p.chunk + (i - x.k * p.rpc) * kPbRun;
+  x.t1 = min(min(x.t0 + kPbRun, (x.k + 1) * p.chunk), p.T);
+  return x;
+}
+
+constexpr int kPsThreads = 256;
+
+// The 8 vectors of `n` positions from t on -> rows 8 i + w of X (row stride ld, DP columns, zero past d):
+// w = 0..3 q^, k^, v^, do^ and w = 4..7 dq^, dk^, dv^, o.  Rows past the n-th position are zero.
+template <int DP>
+HOA_DEVICE void pb_vectors(const PathBwdArgs& p, int chain, int t, int n, float* X, int ld) {
+  for (int i = threadIdx.x; i < 64 * DP; i += kPsThreads) {
+    const int row = i / DP, e = i % DP, w = row & 7;
+    float v = 0.f;
+    if ((row >> 3) < n && e < p.d) {
+      const long long at = ((long long)chain * p.T + t + (row >> 3)) * p.d + e;
+      v = w == 7 ? p.o[at] : load_elem(w < 3 ? p.x[w] : w == 3 ? p.y[3] : p.y[w - 4], at, p.dtype);
+    }
+    X[row * ld + e] = v;
+  }
+}
+
+// Y += skew of position i's vectors (rows 8 i .. of X): thread (ty, tx) owns rows ty + 16 a, columns tx + 16 b
+template <int DP>
+HOA_DEVICE void pb_add(const float* X, int ld, int i, int ty, int tx, float (&Y)[DP / 16][DP / 16]) {
+  constexpr int N = DP / 16;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float* x = X + (8 * i + w) * ld;
+    const float* y = x + 4 * ld;
+    float xr[N], yr[N], xc[N], yc[N];
+#pragma unroll
+    for (int a = 0; a < N; ++a) {
+      xr[a] = x[ty + 16 * a];
+      yr[a] = y[ty + 16 * a];
+      xc[a] = x[tx + 16 * a];
+      yc[a] = y[tx + 16 * a];
+    }
+#pragma unroll
+    for (int a = 0; a < N; ++a)
+#pragma unroll
+      for (int b = 0; b < N; ++b) Y[a][b] = fmaf(xr[a], yc[b], fmaf(-yr[a], xc[b], Y[a][b]));
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kPsThreads) path_bwd_sums_kernel(const __grid_constant__ PathBwdArgs p) {
+  constexpr int N = DP / 16;
+  __shared__ __align__(16) float X[64 * DP];
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  const PbRun r = pb_run(p, blockIdx.x);
+  float Y[N][N];
+#pragma unroll
+  for (int a = 0; a < N; ++a)
+#pragma unroll
+    for (int b = 0; b < N; ++b) Y[a][b] = 0.f;
+  for (int t = r.t0; t < r.t1; t += 8) {
+    const int n = min(8, r.t1 - t);
+    __syncthreads();
+    pb_vectors<DP>(p, r.chain, t, n, X, DP);
+    __syncthreads();
+    for (int i = 0; i < n; ++i) pb_add<DP>(X, DP, i, ty, tx, Y);
+  }
+  float* S = p.S + (long long)blockIdx.x * p.d * p.d;
+#pragma unroll
+  for (int a = 0; a < N; ++a)
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+      if (ty + 16 * a < p.d && tx + 16 * b < p.d) S[(ty + 16 * a) * p.d + tx + 16 * b] = Y[a][b];
+}
+
+// S_r <- sum of S_{r'} over the chain's later runs r' > r
+__global__ void __launch_bounds__(256) path_bwd_suffix_kernel(const __grid_constant__ PathBwdArgs p, long long entries) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= entries) return;
+  const long long dd = (long long)p.d * p.d;
+  const long long chain = i / dd;
+  float* s = p.S + chain * p.NR * dd + (i - chain * dd);
+  double acc = 0.0;
+  int r = p.NR - 1;
+  for (; r >= 3; r -= 4) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = s[(r - k) * dd];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s[(r - k) * dd] = (float)acc;
+      acc += v[k];
+    }
+  }
+  for (; r >= 0; --r) {
+    const float v = s[r * dd];
+    s[r * dd] = (float)acc;
+    acc += v;
+  }
+}
+
+template <int DP> struct PbScan {
+  static constexpr int kLd = DP + 4;
+  static constexpr size_t kSmem = (size_t)(2 * DP + 64) * kLd * sizeof(float);
+};
+
+// acc[a][b] (+)= X[ty + 16 a] . Y[tx + 16 b] over DP columns
+template <int DP, int NA, int NB>
+HOA_DEVICE void pb_nt(const float* X, const float* Y, int ty, int tx, float (&acc)[NA][NB]) {
+  constexpr int kLd = PbScan<DP>::kLd;
+#pragma unroll
+  for (int a = 0; a < NA; ++a)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[a][b] = 0.f;
+#pragma unroll 1
+  for (int e = 0; e < DP; e += 4) {
+    float4 x[NA];
+#pragma unroll
+    for (int a = 0; a < NA; ++a) x[a] = *reinterpret_cast<const float4*>(X + (ty + 16 * a) * kLd + e);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float4 y = *reinterpret_cast<const float4*>(Y + (tx + 16 * b) * kLd + e);
+#pragma unroll
+      for (int a = 0; a < NA; ++a) {
+        acc[a][b] = fmaf(x[a].x, y.x, acc[a][b]);
+        acc[a][b] = fmaf(x[a].y, y.y, acc[a][b]);
+        acc[a][b] = fmaf(x[a].z, y.z, acc[a][b]);
+        acc[a][b] = fmaf(x[a].w, y.w, acc[a][b]);
+      }
+    }
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_constant__ PathBwdArgs p) {
+  constexpr int N = DP / 16, kLd = PbScan<DP>::kLd;
+  extern __shared__ __align__(16) float smem[];
+  float* C = smem;
+  float* Z = C + DP * kLd;
+  float* X = Z + DP * kLd;
+  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, d = p.d;
+  const long long run = p.run0 + blockIdx.x;
+  const PbRun r = pb_run(p, run);
+  if (r.t0 >= r.t1) return;
+  const float* Cg = p.C + ((long long)r.chain * p.K + r.k) * d * d;
+  const float* Zg = p.S + run * d * d;
+  for (int i = tid; i < DP * DP; i += kPsThreads) {
+    const int a = i / DP, b = i % DP;
+    const bool in = a < d && b < d;
+    C[a * kLd + b] = in ? Cg[a * d + b] : 0.f;
+    Z[b * kLd + a] = in ? Zg[a * d + b] : 0.f;             // transposed: Z^T = -Z
+  }
+  __syncthreads();
+  float Y[N][N];
+  pb_nt<DP, N, N>(C, Z, ty, tx, Y);                        // C Z
+  __syncthreads();
+#pragma unroll
+  for (int a = 0; a < N; ++a)
+#pragma unroll
+    for (int b = 0; b < N; ++b) Z[(ty + 16 * a) * kLd + tx + 16 * b] = Y[a][b];
+  __syncthreads();
+  pb_nt<DP, N, N>(Z, C, ty, tx, Y);                        // (C Z) C^T
+  for (int tb = r.t0 + (r.t1 - r.t0 - 1) / 8 * 8; tb >= r.t0; tb -= 8) {
+    const int n = min(8, r.t1 - tb);
+    __syncthreads();
+    pb_vectors<DP>(p, r.chain, tb, n, X, kLd);
+    __syncthreads();
+    float f[4][N];
+    pb_nt<DP, 4, N>(X, C, ty, tx, f);                      // the vectors in the chunk's frame
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < N; ++b) X[(ty + 16 * a) * kLd + tx + 16 * b] = f[a][b];
+    __syncthreads();
+    float* F = p.F + ((long long)blockIdx.x * kPbRun + (tb - r.t0)) * 3 * d;
+    for (int i = tid; i < n * 3 * d; i += kPsThreads) {
+      const int e = i % d, w = i / d % 3, j = i / (3 * d);
+      F[i] = X[(8 * j + 4 + w) * kLd + e];
+    }
+    for (int i = n - 1; i >= 0; --i) {
+      float* Yg = p.Y + ((long long)blockIdx.x * kPbRun + (tb + i - r.t0)) * d * d;
+#pragma unroll
+      for (int a = 0; a < N; ++a)
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+          if (ty + 16 * a < d && tx + 16 * b < d) Yg[(ty + 16 * a) * d + tx + 16 * b] = Y[a][b];
+      pb_add<DP>(X, kLd, i, ty, tx, Y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// main: one CTA of 128 G threads a position at a time.  Products on tcgen05 with fp32
+// accuracy: each factor is two f16 parts (hoa_split_f16.cuh), a product three tensor-core
+// products.  With |R| <= 1, entries of Y scaled to [2^9, 2^10) and those of W to [2^5, 2^6)
+// (a power of two, per position), no part leaves f16's range: a conjugation or a commutator
+// keeps the Frobenius norm or grows it by less than 2.7 (below), so an entry stays below
+// 2^6 128 2.7 < 65504, and what f16 drops of small ones is 2^-31 of the largest.
+//
+//   U = R Y          both from shared memory (R's slabs are the K-major left operand)
+//   W = U R^T        U in TMEM; the same slabs, as the K-major right operand, are R^T
+//   V_0 = W;  V_k = alpha_k [A, V_{k-1}] (+ V_{k-2}),  M = sum_k gamma_k V_k
+// A is the left operand in TMEM for all k.  A and V are skew, so [A, V] = A V - (A V)^T: one
+// product, transposed through shared memory.  M stays in registers (a thread owns a row and
+// every G-th 16 columns).
+//
+// The sum: with x >= 2 ||A||_2 (from ||A||_inf and ||A||_F / sqrt 2),
+//   x <= 4   Taylor: alpha_k = 1 / (k + 1), gamma = 1, ended once what is left is below 2^-24 of
+//            W: entries of [A, V] are at most 2 ||A||_inf times those of V.
+//   x > 4    Chebyshev (Taylor's terms would grow before they fall): alpha = 2 / x (1 / x first),
+//            V_{k-2} added, gamma_k = (2 - [k = 0]) / x * integral of J_k over [0, x]
+//            = (2 - [k = 0]) / x * 2 sum_m J_{k + 2m + 1}(x), the Bessel functions by Miller's
+//            backward recurrence in fp64; about x + 15 products.  x <= kPbMaxX, else NaN.
+// ---------------------------------------------------------------------------
+constexpr float kPbR = 256.f, kPbA = 16.f;
+constexpr int kPbCoef = 640;
+constexpr float kPbMaxX = 480.f;
+
+template <int DP> struct PbLayout {
+  static constexpr int G = DP >= 112 ? 4 : 2, kThreads = 128 * G;
+  static constexpr int NKB = (DP + 63) / 64, NC = DP / 16, NCG = (NC + G - 1) / G;
+  static constexpr int kSlab = DP * 128, kMat = NKB * kSlab, kTwo = 2 * kMat;
+  static constexpr int kDim = DP < 120 ? DP : 120;
+  static constexpr int kLdT = DP + 4;
+  static constexpr int kT = kDim * kLdT * 4;                       // A V, to be read transposed
+  static constexpr int kR = ((kTwo > kT ? kTwo : kT) + 1023) / 1024 * 1024;
+  static constexpr int offV = kR;
+  // (R as the left factor is read as 128 rows a slab: past its own end into what follows)
+  static constexpr int kMats = kR + kTwo > kTwo + 128 * 128 ? kR + kTwo : kTwo + 128 * 128;
+  static constexpr int offVec = kMats;                             // dq^, dk^, dv^ in the chunk's frame
+  static constexpr int offPart = offVec + 3 * DP * 4;
+  static constexpr int offRed = offPart + 3 * kThreads * 4;
+  static constexpr int offCoef = offRed + kThreads * 4;
+  static constexpr int offBar = offCoef + kPbCoef * 4;
+  static constexpr int kAlloc = offBar + 64 + 1024;
+  static constexpr int kMinBlocks = kAlloc <= 113 * 1024 ? 2 : 1;
+  static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
+  static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
+  static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2 + kThreads - 1) / kThreads;
+  static constexpr int kScratch = 2 * NCG * 4 * kThreads;          // float4s of a CTA's old iterates
+};
+
+// power of two that puts x into [2^e, 2^(e+1)), as an exponent; 0 where x is 0 or not finite
+HOA_DEVICE int pb_exponent(float x, int e) {
+  if (!(x > 0.f) || !(x <= 3.0e38f)) return 0;
+  return max(-100, min(100, e - ilogbf(x)));
+}
+
+template <int DP>
+__global__ void __launch_bounds__(PbLayout<DP>::kThreads, PbLayout<DP>::kMinBlocks)
+path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
+  using L = PbLayout<DP>;
+  constexpr int G = L::G, NT = L::kThreads, NCG = L::NCG;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* gen = reinterpret_cast<float*>(sm);                        // R's place, once R is done with
+  float* T = reinterpret_cast<float*>(sm);
+  float* vec = reinterpret_cast<float*>(sm + L::offVec);
+  float* part = reinterpret_cast<float*>(sm + L::offPart);
+  float* red = reinterpret_cast<float*>(sm + L::offRed);
+  float* coef = reinterpret_cast<float*>(sm + L::offCoef);
+  uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* s_terms = s_abort + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
+  const int d = p.d;
+  if (tid == 0) {
+    mbar_init(done, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, L::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
+  const int row = (warp & 3) * 32 + lid, group = warp >> 2;
+  const bool works = (warp & 3) * 32 < DP;                          // (the warp has rows of the matrix)
+  uint32_t phase = 0;
+  bool bad = false;
+
+  // ---- matrices from global memory, DP / 4 threads a row, 4 columns each
+  constexpr int n4 = DP / 4, RG = NT / n4, kRows = (DP + RG - 1) / RG;
+  const int pr = tid / n4, pc = (tid % n4) * 4;
+  float4 pv[kRows];
+  auto load_mat = [&](const float* m) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = pr + k * RG;
+      pv[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (pr >= RG || r >= d || pc >= d) continue;
+      const float* at = m + r * d + pc;
+      if (vec4) {
+        pv[k] = *reinterpret_cast<const float4*>(at);
+      } else {
+        pv[k].x = at[0];
+        if (pc + 1 < d) pv[k].y = at[1];
+        if (pc + 2 < d) pv[k].z = at[2];
+        if (pc + 3 < d) pv[k].w = at[3];
+      }
+    }
+  };
+  auto put_mat = [&](uint8_t* mat, float scale) {
+    uint8_t* slab = mat + (pc >> 6) * L::kSlab + (pc & 7) * 2;
+    const uint32_t ch = (pc & 63) >> 3;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int r = pr + k * RG;
+      if (pr >= RG || r >= DP) continue;
+      uint2 hi, lo;
+      st_split2(f2_mul(f2(pv[k].x, pv[k].y), f2(scale)), hi.x, lo.x);
+      st_split2(f2_mul(f2(pv[k].z, pv[k].w), f2(scale)), hi.y, lo.y);
+      uint8_t* at = slab + sw128_offset(r, ch);
+      *reinterpret_cast<uint2*>(at) = hi;
+      *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+    }
+  };
+  // ---- a thread's own 16 columns (chunk c) of its row
+  auto put_right = [&](int c, const F2 (&v)[8]) {
+    if (row >= DP) return;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint4 h, l;
+      st_split2(v[4 * q], h.x, l.x);
+      st_split2(v[4 * q + 1], h.y, l.y);
+      st_split2(v[4 * q + 2], h.z, l.z);
+      st_split2(v[4 * q + 3], h.w, l.w);
+      const int ch = 2 * c + q;
+      uint8_t* at = sm + L::offV + (ch >> 3) * L::kSlab + sw128_offset(row, ch & 7);
+      *reinterpret_cast<uint4*>(at) = h;
+      *reinterpret_cast<uint4*>(at + L::kMat) = l;
+    }
+  };
+  auto put_left = [&](int c, const F2 (&v)[8]) {
+    float h[8], l[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t hi, lo;
+      st_split2(v[e], hi, lo);
+      h[e] = __uint_as_float(hi);
+      l[e] = __uint_as_float(lo);
+    }
+    tmem_st8(lanes + L::colHi + 8 * c, h);
+    tmem_st8(lanes + L::colLo + 8 * c, l);
+  };
+  auto load_D = [&](int c, float (&v)[16]) {
+    tmem_ld16(lanes + L::colD + 16 * c, v);
+    tmem_wait_ld();
+    tmem_touch(v);
+  };
+
+  // this row's columns 16 c .. of a d x d matrix, times f; 0 outside
+  auto mask_row = [&](int c, float f, float (&v)[16]) {
+    int n = row < d ? d - 16 * c : 0;
+    asm volatile("" : "+r"(n));
+    if (n >= 16) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] *= f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = e < n ? v[e] * f : 0.f;
+    }
+  };
+
+  // ---- products.  Left R from shared memory or the left factor in TMEM; right: the slabs at V by rows, or R^T
+  const uint32_t base = smem_u32(sm);
+  const uint64_t rK[2] = {desc_sw128(base), desc_sw128(base + L::kMat)};
+  const uint64_t vN[2] = {desc_sw128_mn(base + L::offV, L::kSlab), desc_sw128_mn(base + L::offV + L::kMat, L::kSlab)};
+  constexpr uint32_t idN = make_idesc(0, 128, DP, true), idK = make_idesc(0, 128, DP, false);
+  auto mma = [&](bool left_R, bool right_R) {
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int a = pass == 1, b = pass == 0;                       // hi lo, lo hi, hi hi
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint64_t kk = (uint64_t)(((k >> 2) * L::kSlab + (k & 3) * 32) >> 4);
+        const uint32_t acc = pass > 0 || k > 0 ? 1u : 0u;
+        const uint64_t rd = right_R ? rK[b] + kk : vN[b] + (uint64_t)(k * 2048 >> 4);
+        if (left_R) mma_bf16(tmem + L::colD, rK[a] + kk, rd, idN, acc);
+        else mma_bf16_ts(tmem + L::colD, tmem + (a ? L::colLo : L::colHi) + 8 * k, rd, right_R ? idK : idN, acc);
+      }
+    }
+    tc_commit(done);
+  };
+  // what every thread wrote (shared memory, TMEM) -> the tensor core
+  auto publish = [&]() {
+    tmem_wait_st();
+    fence_proxy_async_smem();
+    tc_fence_before();
+  };
+  auto issue = [&](bool left_R, bool right_R) {
+    if (tid == 0 && !bad) {
+      tc_fence_after();
+      mma(left_R, right_R);
+    }
+  };
+  auto wait = [&]() {
+    if (!bad) {
+      const unsigned c0 = (unsigned)clock();
+      bad = !mbar_wait_abortable(done, phase, s_abort, p.max_wait);
+      if (!bad && (unsigned)clock() - c0 > (unsigned)p.max_wait) {
+        bad = true;
+        *s_abort = 1;
+      }
+      if (!bad) phase ^= 1;
+    }
+    tc_fence_after();
+  };
+  // the largest over the CTA of v >= 0 (NaN and infinity show as infinity); one barrier inside
+  auto top_of = [&](float v, float* at) {
+    v = v <= 3.0e38f ? v : INFINITY;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (lid == 0) at[warp] = v;
+    __syncthreads();
+    float t = at[0];
+#pragma unroll
+    for (int w = 1; w < NT / 32; ++w) t = fmaxf(t, at[w]);
+    return t;
+  };
+
+  float4* scratch = p.V + (long long)blockIdx.x * L::kScratch + tid;
+  const long long units = (long long)p.runs * kPbRun;
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const long long lr = u / kPbRun;
+    const PbRun r = pb_run(p, p.run0 + lr);
+    const int t = r.t0 + (int)(u - lr * kPbRun);
+    if (t >= r.t1) continue;                                        // (block-uniform)
+    const int b = r.chain / p.H, h = r.chain - b * p.H;
+    const long long pos = ((long long)b * p.T + t) * p.H + h;
+    // ---- R and Y as factors
+    load_mat(p.R + ((long long)r.chain * p.T + t) * d * d);
+    put_mat(sm, kPbR);
+    load_mat(p.Y + u * d * d);
+    for (int i = tid; i < 3 * DP; i += NT) vec[i] = i % DP < d ? p.F[u * 3 * d + i / DP * d + i % DP] : 0.f;
+    float top = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      // (fmaxf drops a NaN: the sum carries it)
+      const float s = fabsf(pv[k].x) + fabsf(pv[k].y) + fabsf(pv[k].z) + fabsf(pv[k].w);
+      top = s <= 3.0e38f ? fmaxf(top, fmaxf(fmaxf(fabsf(pv[k].x), fabsf(pv[k].y)), fmaxf(fabsf(pv[k].z), fabsf(pv[k].w)))) : INFINITY;
+    }
+    top = top_of(top, red);
+    bool lost = !(top <= 3.0e38f);                                  // nothing finite can come of this position
+    const int e_y = pb_exponent(top, 9);
+    put_mat(sm + L::offV, ldexpf(1.f, e_y));
+    publish();
+    __syncthreads();
+    issue(true, false);                                             // U = R Y, in units of 2^-e_y / kPbR
+    // ---- meanwhile: the generators on their way, and dq, dk, dv = R (.)
+    float g[L::kGen];
+    const float* ag = p.a + pos * p.stride;
+#pragma unroll
+    for (int k = 0; k < L::kGen; ++k) {
+      const int i = tid + k * NT;
+      g[k] = i < p.stride ? ag[i] : 0.f;
+      if (p.a_bias != nullptr && i < p.stride) g[k] += p.a_bias[(long long)h * p.stride + i];
+    }
+    {
+      float y[3] = {0.f, 0.f, 0.f};
+      if (works)
+        for (int c = group; c < L::NC; c += G) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int ch = 2 * c + q;
+            const uint8_t* at = sm + (ch >> 3) * L::kSlab + sw128_offset(row < DP ? row : 0, ch & 7);
+            const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + L::kMat);
+            const float2 m[4] = {f2_get(st_join2(hi.x, lo.x)), f2_get(st_join2(hi.y, lo.y)), f2_get(st_join2(hi.z, lo.z)),
+                                 f2_get(st_join2(hi.w, lo.w))};
+#pragma unroll
+            for (int w = 0; w < 3; ++w)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 x = *reinterpret_cast<const float2*>(vec + w * DP + 8 * ch + 2 * e);
+                y[w] = fmaf(m[e].x, x.x, fmaf(m[e].y, x.y, y[w]));
+              }
+          }
+        }
+#pragma unroll
+      for (int w = 0; w < 3; ++w) part[w * NT + group * 128 + row] = y[w];
+    }
+    wait();
+    if (works) {
+#pragma unroll 1
+      for (int c = group; c < L::NC; c += G) {
+        float v[16];
+        F2 x[8];
+        load_D(c, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), f2(1.f / (16.f * kPbR)));
+        put_left(c, x);
+      }
+    }
+    publish();
+    __syncthreads();
+    issue(false, true);                                             // W = U R^T, in units of 16 2^-e_y / kPbR
+    for (int i = tid; i < 3 * d; i += NT) {
+      const int w = i / d, e = i - w * d;
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) s += part[w * NT + k * 128 + e];
+      store_elem(p.dqkv, pos * 3 * d + i, p.out_dtype, s * (1.f / kPbR));
+    }
+    wait();
+    top = 0.f;
+    if (works) {
+#pragma unroll 1
+      for (int c = group; c < L::NC; c += G) {
+        float v[16];
+        load_D(c, v);
+        if (row < d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < L::kGen; ++k)
+      if (tid + k * NT < p.stride) gen[tid + k * NT] = g[k];
+    top = top_of(top, red);
+    lost |= !(top <= 3.0e38f);
+    const int e_w = pb_exponent(top, 5);
+    const float f_w = ldexpf(1.f, e_w);
+    const float wmax = top * f_w;
+    // ---- V_0 = W as the right factor, A as the left one; the norms of A
+    float M[NCG][16], rs = 0.f, sq = 0.f;
+#pragma unroll
+    for (int ci = 0; ci < NCG; ++ci) {
+      const int c = group + ci * G;
+      if (!works || c >= L::NC) continue;
+      F2 x[8];
+      load_D(c, M[ci]);
+      mask_row(c, f_w, M[ci]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = f2(M[ci][2 * e], M[ci][2 * e + 1]);
+      put_right(c, x);
+      int at = row;
+      asm volatile("" : "+r"(at));                                  // (its index math stays here: no registers across the products)
+      gen_row16(gen, p.banked != 0, p.stride, d, at, lid, 16 * c, p.edge_scale * kPbA, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 v = f2_get(x[e]);
+        rs += fabsf(v.x) + fabsf(v.y);
+        sq = fmaf(v.x, v.x, fmaf(v.y, v.y, sq));
+      }
+      put_left(c, x);
+    }
+    part[NT + group * 128 + row] = rs;                              // (not red: a slow warp may still read top_of's values there)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+    if (lid == 0) part[warp] = sq;
+    publish();
+    __syncthreads();
+    issue(false, false);                                            // A V_0
+    float inf = 0.f, fro = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < G; ++k) s += part[NT + k * 128 + lid + 32 * q];
+      inf = s <= 3.0e38f ? fmaxf(inf, lid + 32 * q < d ? s : 0.f) : INFINITY;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) inf = fmaxf(inf, __shfl_xor_sync(0xffffffffu, inf, o));
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) fro += part[w];
+    inf *= 1.00001f / kPbA;                                         // (bounds: rounded up)
+    fro = sqrtf(0.5f * fro) * (1.00001f / kPbA);
+    const float x2 = 2.f * fminf(inf, fro);
+    lost |= !(x2 <= kPbMaxX);
+    const bool cheb = !lost && x2 > 4.f;
+    if (cheb && tid == 32) {
+      // J_n by the recurrence J_{n-1} = 2 n / x J_n - J_{n+1} downwards from J_{N+1} = 0 and any small J_N; the first
+      // pass finds what to divide by (J_0 + 2 (J_2 + J_4 + ...) = 1), the second one leaves the coefficients
+      const double x = (double)x2, i2x = 2.0 / x;
+      const int N = min(kPbCoef - 2, (int)(x + 40.0 + 8.0 * cbrt(x)));
+      double start = 1e-100;
+      int terms = 1;
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        double j1 = 0.0, j0 = start, even = 0.0, odd = 0.0;          // sums of J_n, J_{n+2}, ... so far, by the parity of n
+#pragma unroll 1
+        for (int n = N; n >= 1; --n) {
+          double& tail = n & 1 ? odd : even;
+          tail += j0;
+          if (pass == 1) {
+            const float v = (float)(tail * (n == 1 ? 2.0 : 4.0) / x);
+            coef[n - 1] = v;
+            if (terms == 1 && fabsf(v) > 2e-9f) terms = max(1, n - 1);
+          }
+          const double j = n * i2x * j0 - j1;
+          j1 = j0;
+          j0 = j;
+        }
+        start /= j0 + 2.0 * even;
+      }
+      *s_terms = terms;
+    }
+    // ---- the series
+    const float a_t = 1.f / kPbA;
+    for (int k = 1;; ++k) {
+      wait();
+#pragma unroll
+      for (int ci = 0; ci < NCG; ++ci) {
+        const int c = group + ci * G;
+        if (!works || c >= L::NC) continue;
+        float v[16];
+        load_D(c, v);
+        if (row < d)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(T + row * L::kLdT + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      }
+      __syncthreads();
+      const int terms = cheb ? *s_terms : 64;
+      const float alpha = cheb ? (k == 1 ? a_t : 2.f * a_t) / x2 : a_t / (float)(k + 1);
+      const float gamma = cheb ? coef[k] : 1.f;
+      float vtop = 0.f;
+#pragma unroll
+      for (int ci = 0; ci < NCG; ++ci) {
+        const int c = group + ci * G;
+        if (!works || c >= L::NC) continue;
+        float v[16];
+        load_D(c, v);
+        int at = 16 * c * L::kLdT + row;
+        asm volatile("" : "+r"(at));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] -= T[at + e * L::kLdT];   // (rows past d: whatever lies there, masked below)
+        mask_row(c, alpha, v);
+        if (cheb) {
+          float4* at = scratch + (long long)(((k & 1) * NCG + ci) * 4) * NT;
+          if (k == 1) {
+            float4* old = scratch + (long long)(ci * 4) * NT;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) old[q * NT] = make_float4(M[ci][4 * q], M[ci][4 * q + 1], M[ci][4 * q + 2], M[ci][4 * q + 3]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) M[ci][e] *= coef[0];
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float4 o = at[q * NT];
+              v[4 * q] += o.x;
+              v[4 * q + 1] += o.y;
+              v[4 * q + 2] += o.z;
+              v[4 * q + 3] += o.w;
+            }
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) at[q * NT] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+        F2 x[8];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          M[ci][e] = fmaf(gamma, v[e], M[ci][e]);
+          vtop = fmaxf(vtop, fabsf(v[e]));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = f2(v[2 * e], v[2 * e + 1]);
+        put_right(c, x);
+      }
+      // Taylor: entries of the terms still to come sum to at most vtop rho / (1 - rho)
+      const float rho = 2.f * inf / (float)(k + 2);
+      bool more = cheb || (rho < 1.f ? vtop * rho > 5.96e-8f * wmax * (1.f - rho) : true);
+      more = more && k < terms && !lost;
+      publish();
+      if (!__syncthreads_or(more)) break;
+      issue(false, false);
+    }
+    // ---- da: the upper triangle in the generators' layout, through shared memory
+    float* out = T;
+    if (p.banked)
+      for (int i = tid; i < p.stride; i += NT) out[i] = 0.f;
+    if (p.banked) __syncthreads();
+    {
+      const float nan = __int_as_float(0x7fffffff);
+      const bool last = t == p.T - 1;
+      const float f1 = ldexpf(1.f, -e_y), f2w = ldexpf(p.edge_scale, -e_w - 4);
+      const int base_r = row * (2 * d - row - 1) / 2 - row - 1;
+#pragma unroll
+      for (int ci = 0; ci < NCG; ++ci) {
+        const int c = group + ci * G;
+        if (!works || c >= L::NC || row >= d) continue;
+        int at = row, c0 = 16 * c;
+        asm volatile("" : "+r"(at), "+r"(c0));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int cc = c0 + e;
+          if (cc <= at || cc >= d) continue;
+          const float v = last ? 0.f : lost ? nan : M[ci][e] * f2w * f1;
+          out[p.banked ? gen_banked_slot(at, cc, d) : base_r + cc] = v;
+        }
+      }
+    }
+    if (__syncthreads_or(bad)) break;
+    float* dg = p.da + pos * p.stride;
+    for (int i = tid; i < p.stride; i += NT) dg[i] = out[i];
+    __syncthreads();                                                // the next position writes R there
+  }
+  if (tid == 0 && bad) mbar_wait(done, phase);                      // the product that it gave up on may still read shared memory
+  if (__syncthreads_or(bad) && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, L::kCols);
+}
+
+
+// ---------------------------------------------------------------------------
+struct PbPlan {
+  int rpc, K, NR;
+  long long group;                                     // runs of one pass of scan and main
+  size_t off_Y, off_F, off_V, bytes;
+};
+
+static int pb_sms() {
+  static const int n = []() {                          // of the device that calls first: every GPU here is the same
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+    return v;
+  }();
+  return n;
+}
+
+// CTAs of the main kernel and float4s of their old iterates, by the padded head dim
+template <int DP> static size_t pb_scratch(int sms) { return (size_t)sms * PbLayout<DP>::kMinBlocks * PbLayout<DP>::kScratch * sizeof(float4); }
+static size_t pb_scratch_of(int d, int sms) {
+  switch ((d + 15) / 16) {
+    case 1: return pb_scratch<16>(sms);
+    case 2: return pb_scratch<32>(sms);
+    case 3: return pb_scratch<48>(sms);
+    case 4: return pb_scratch<64>(sms);
+    case 5: return pb_scratch<80>(sms);
+    case 6: return pb_scratch<96>(sms);
+    case 7: return pb_scratch<112>(sms);
+    default: return pb_scratch<128>(sms);
+  }
+}
+
+// The matrices Y of a pass take 1 GiB at most (4 d^2 bytes a position): longer inputs go through in several passes.
+static bool pb_plan(int B, int H, int T, int d, int chunk, int sms, PbPlan& x) {
+  if (B < 1 || H < 1 || T < 1 || d < 2 || d > 120 || chunk < 1 || sms < 1) return false;
+  x.K = (int)(((long long)T + chunk - 1) / chunk);
+  x.rpc = ((chunk < T ? chunk : T) + kPbRun - 1) / kPbRun;
+  const long long NR = (long long)x.K * x.rpc, runs = NR * B * H;
+  if ((long long)B * H > 0x7fffffff || NR > 0x7fffffff || runs > 0x7fffffff || (long long)T + chunk > 0x7fffff00) return false;
+  x.NR = (int)NR;
+  const size_t dd = (size_t)d * d * sizeof(float);
+  x.group = (long long)((1ull << 30) / (dd * kPbRun));
+  if (x.group < 1) x.group = 1;
+  if (x.group > runs) x.group = runs;
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  x.off_Y = up((size_t)runs * dd);
+  x.off_F = x.off_Y + up((size_t)x.group * kPbRun * dd);
+  x.off_V = x.off_F + up((size_t)x.group * kPbRun * 3 * d * sizeof(float));
+  x.bytes = x.off_V + pb_scratch_of(d, sms);
+  return true;
+}
+
+template <int DP>
+static int launch_path_bwd(PathBwdArgs a, const PbPlan& x, int sms, cudaStream_t s) {
+  using L = PbLayout<DP>;
+  static std::atomic<unsigned long long> done_scan{0}, done_main{0};
+  if (!allow_smem(path_bwd_scan_kernel<DP>, PbScan<DP>::kSmem, done_scan) || !allow_smem(path_bwd_kernel<DP>, L::kAlloc, done_main))
+    return HOA_ERR_LAUNCH;
+  const long long runs = (long long)a.B * a.H * x.NR, entries = (long long)a.B * a.H * a.d * a.d;
+  if ((entries + 255) / 256 > 0x7fffffff) return HOA_ERR_UNSUPPORTED;
+  const bool vec4 = a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.R) & 15) == 0;
+  path_bwd_sums_kernel<DP><<<(unsigned)runs, kPsThreads, 0, s>>>(a);
+  if (int st = launch_status()) return st;
+  path_bwd_suffix_kernel<<<(unsigned)((entries + 255) / 256), 256, 0, s>>>(a, entries);
+  if (int st = launch_status()) return st;
+  for (long long r = 0; r < runs; r += x.group) {
+    a.run0 = r;
+    a.runs = (int)(runs - r < x.group ? runs - r : x.group);
+    path_bwd_scan_kernel<DP><<<(unsigned)a.runs, kPsThreads, PbScan<DP>::kSmem, s>>>(a);
+    if (int st = launch_status()) return st;
+    const long long units = (long long)a.runs * kPbRun, most = (long long)sms * L::kMinBlocks;
+    path_bwd_kernel<DP><<<(unsigned)(units < most ? units : most), L::kThreads, L::kAlloc, s>>>(a, vec4);
+    if (int st = launch_status()) return st;
+  }
+  return HOA_OK;
+}
+
+}  // namespace hoa
+
+using namespace hoa;
+
+extern "C" size_t hoa_path_bwd_workspace_bytes(int B, int H, int T, int d, int chunk) {
+  PbPlan x;
+  return pb_plan(B, H, T, d, chunk, pb_sms(), x) ? x.bytes : 0;
+}
+
+extern "C" int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias, float edge_scale, const float* R, const float* C,
+                            int chunk, const void* qh, const void* kh, const void* vh, const float* o, const void* dqh,
+                            const void* dkh, const void* dvh, const void* doh, int hat_dtype, float* da, void* dqkv, int out_dtype,
+                            int B, int H, int T, int d, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  if (!a_all || !R || !C || !qh || !kh || !vh || !o || !dqh || !dkh || !dvh || !doh || !da || !dqkv || !workspace)
+    return HOA_ERR_INVALID_ARG;
+  if (B < 1 || H < 1 || T < 1 || d < 2 || chunk < 1) return HOA_ERR_INVALID_ARG;
+  const int stride = gen_row_stride(a_dtype, d);
+  if (d > 120 || stride == 0 || gen_elem_dtype(a_dtype) != HOA_F32 || (hat_dtype != HOA_F32 && hat_dtype != HOA_BF16) ||
+      (out_dtype != HOA_F32 && out_dtype != HOA_BF16))
+    return HOA_ERR_UNSUPPORTED;
+  const int sms = pb_sms();
+  PbPlan x;
+  if (!pb_plan(B, H, T, d, chunk, sms, x)) return HOA_ERR_UNSUPPORTED;
+  if (workspace_bytes < x.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return HOA_ERR_WORKSPACE;
+  unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  PathBwdArgs p{a_all, gen_is_banked(a_dtype) ? 1 : 0, stride, a_bias, edge_scale, R, C, chunk, x.K, x.rpc, x.NR,
+                {qh, kh, vh}, o, {dqh, dkh, dvh, doh}, hat_dtype, da, dqkv, out_dtype, B, H, T, d,
+                reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + x.off_Y), reinterpret_cast<float*>(ws + x.off_F),
+                reinterpret_cast<float4*>(ws + x.off_V), 0, 0, status, wait_bound_cycles()};
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  switch ((d + 15) / 16) {
+    case 1: return launch_path_bwd<16>(p, x, sms, s);
+    case 2: return launch_path_bwd<32>(p, x, sms, s);
+    case 3: return launch_path_bwd<48>(p, x, sms, s);
+    case 4: return launch_path_bwd<64>(p, x, sms, s);
+    case 5: return launch_path_bwd<80>(p, x, sms, s);
+    case 6: return launch_path_bwd<96>(p, x, sms, s);
+    case 7: return launch_path_bwd<112>(p, x, sms, s);
+    default: return launch_path_bwd<128>(p, x, sms, s);
+  }
+}

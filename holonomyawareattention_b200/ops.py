@@ -1054,3 +1054,157 @@ def path_step(a, P, qkv, n_heads: int, edge_scale: float, k_pages, v_pages, tabl
          P.data_ptr(), P_out.data_ptr(), qkv.data_ptr(), _dtype_code(qkv.dtype), qkv.stride(0), qh.data_ptr(),
          k_pages.data_ptr(), v_pages.data_ptr(), code, ps, table.data_ptr(), tw, W, lens.data_ptr(), B, H, d, page, n_pages)
     return P_out, qh
+
+
+# ---------------------------------------------------------------------------
+# training: the backward passes of attention and of the path, the AdamW step
+# ---------------------------------------------------------------------------
+def _like(t, name, shape, dtype, idx) -> None:
+    if t.get_device() != idx:
+        _index(t)
+        raise ValueError(f"{name} must be on cuda:{idx}, got {t.device}")
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+
+
+def _attn_shapes(qh, kh, vh, q_offset):
+    """(device index, dtype code, BH, Tq, Tk, d) of causal attention's inputs, checked."""
+    idx = _index(qh)
+    code = _dtype_code(qh.dtype)
+    if qh.dim() != 3 or kh.dim() != 3 or qh.numel() == 0 or kh.numel() == 0:
+        raise ValueError("q^ must be (BH, Tq, d) and k^, v^ (BH, Tk, d), none empty")
+    BH, Tq, d = qh.shape
+    Tk = kh.shape[1]
+    _like(qh, "q^", (BH, Tq, d), qh.dtype, idx)
+    _like(kh, "k^", (BH, Tk, d), qh.dtype, idx)
+    _like(vh, "v^", (BH, Tk, d), qh.dtype, idx)
+    if q_offset < 0 or q_offset + Tq > Tk:
+        raise ValueError(f"the queries q_offset .. q_offset + Tq = {q_offset} .. {q_offset + Tq} must lie in the {Tk} keys")
+    if d > 128:
+        raise NotImplementedError(f"head dim {d} (at most 128)")
+    if BH > 65535 or Tk >= 2 ** 31 - 256:
+        raise NotImplementedError(f"at most 65535 chains and 2^31 - 257 keys, got {BH} and {Tk}")
+    return idx, code, BH, Tq, Tk, d
+
+
+def attn_fwd_lse(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, softmax_scale: float, q_offset: int = 0):
+    """attn_fwd for training: (o (BH,Tq,d) fp32, lse (BH,Tq) fp32), lse the log-sum-exp of each row's scaled
+    scores; bf16 (v^ row-major here) runs on the tensor cores where d % 8 == 0.  hoa_attn_fwd_lse."""
+    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset)
+    o = qh.new_empty((BH, Tq, d), dtype=torch.float32)
+    lse = qh.new_empty((BH, Tq), dtype=torch.float32)
+    _run(idx, "hoa_attn_fwd_lse", qh.data_ptr(), kh.data_ptr(), vh.data_ptr(), code, o.data_ptr(), lse.data_ptr(), softmax_scale,
+         BH, Tq, Tk, q_offset, d)
+    return o, lse
+
+
+def attn_bwd(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, do: torch.Tensor,
+             softmax_scale: float, q_offset: int = 0):
+    """Gradients (dq^, dk^, dv^) of causal attention for the gradient ``do`` (BH,Tq,d) of its output.
+
+    q^ (BH,Tq,d), k^ and v^ (BH,Tk,d), do and the results share a type (fp32 or bf16); o and lse are what
+    attn_fwd_lse gave.  The probabilities are recomputed from lse; sums are fp32 and of a fixed order.
+    hoa_attn_bwd."""
+    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset)
+    _like(o, "o", (BH, Tq, d), torch.float32, idx)
+    _like(lse, "lse", (BH, Tq), torch.float32, idx)
+    _like(do, "do", (BH, Tq, d), qh.dtype, idx)
+    dq, dk, dv = torch.empty_like(qh), torch.empty_like(kh), torch.empty_like(vh)
+    nb = _bytes_of("hoa_attn_bwd_workspace_bytes", BH, Tq)
+    ws = _scratch(idx, nb)
+    _run(idx, "hoa_attn_bwd", qh.data_ptr(), kh.data_ptr(), vh.data_ptr(), o.data_ptr(), lse.data_ptr(), do.data_ptr(), code,
+         dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), softmax_scale, BH, Tq, Tk, q_offset, d, ws[0], nb)
+    return dq, dk, dv
+
+
+def path_bwd(a_all: torch.Tensor, R: torch.Tensor, C: torch.Tensor, chunk: int, n_heads: int, edge_scale: float, hats, dhats,
+             a_bias: Optional[torch.Tensor] = None, gen_layout: str = "packed", out_dtype: Optional[torch.dtype] = None):
+    """Gradients through the path products: (da (B,T,H*m) fp32 of the raw generators, dqkv (B,T,3D)).
+
+    a_all, a_bias, edge_scale, gen_layout as link_local's (da has a_all's layout), R and C what link_local and
+    carry_scan gave for ``chunk``.  hats: (q^, k^, v^, o), each (BH,T,d), o in fp32; dhats: (dq^, dk^, dv^, do^), the
+    gradients of the first three and P^T dout (apply_paths with transpose).  q^, k^, v^ and dhats share a type, which
+    dqkv has too unless ``out_dtype`` says otherwise.  The gradient of the closing edge (t = T - 1) is 0, as the causal
+    forward does not use it.  hoa_path_bwd."""
+    idx = _index(a_all)
+    if a_all.dim() != 3 or R.dim() != 4 or len(hats) != 4 or len(dhats) != 4:
+        raise ValueError("a_all must be (B,T,H*stride), R (BH,T,d,d), hats and dhats four tensors each")
+    if a_all.dtype is not torch.float32:
+        raise NotImplementedError("the path's backward pass takes fp32 generators")
+    B, T, H, d = a_all.shape[0], a_all.shape[1], n_heads, R.shape[3]
+    if B < 1 or T < 1 or H < 1 or chunk < 1:
+        raise ValueError("B, T, n_heads and chunk must be at least 1")
+    if d < 2 or d > 120:
+        raise NotImplementedError(f"head dim {d} (2 to 120)")
+    a_code, width = _gen_code(a_all, gen_layout), _gen_width(H, d, gen_layout)
+    dt = hats[0].dtype
+    code = _dtype_code(dt)
+    out_dtype = out_dtype or dt
+    _like(a_all, "a_all", (B, T, width), torch.float32, idx)
+    _check_bias(a_bias, width)
+    if a_bias is not None and a_bias.get_device() != idx:
+        raise ValueError(f"a_bias must be on cuda:{idx}, got {a_bias.device}")
+    _like(R, "R", (B * H, T, d, d), torch.float32, idx)
+    _like(C, "C", (B * H, (T + chunk - 1) // chunk, d, d), torch.float32, idx)
+    for i, name in enumerate(("q^", "k^", "v^", "o")):
+        _like(hats[i], name, (B * H, T, d), dt if i < 3 else torch.float32, idx)
+    for i, name in enumerate(("dq^", "dk^", "dv^", "do^")):
+        _like(dhats[i], name, (B * H, T, d), dt, idx)
+    chunk = min(chunk, T)
+    with torch.cuda.device(idx):
+        nb = _bytes_of("hoa_path_bwd_workspace_bytes", B, H, T, d, chunk)
+    if nb == 0:
+        raise NotImplementedError(f"B H T = {B} {H} {T} with chunk {chunk} is too large")
+    ws = _scratch(idx, nb)
+    da = torch.empty_like(a_all)
+    dqkv = a_all.new_empty((B, T, 3 * H * d), dtype=out_dtype)
+    _run(idx, "hoa_path_bwd", a_all.data_ptr(), a_code, a_bias.data_ptr() if a_bias is not None else None, edge_scale, R.data_ptr(),
+         C.data_ptr(), chunk, *(t.data_ptr() for t in hats), *(t.data_ptr() for t in dhats), code, da.data_ptr(), dqkv.data_ptr(),
+         _dtype_code(out_dtype), B, H, T, d, ws[0], nb)
+    return da, dqkv
+
+
+ADAMW_BLOCK = 256               # elements of a block of 8-bit moments
+
+
+def _pointers(ts):
+    return (ctypes.c_void_p * len(ts))(*(None if t is None else t.data_ptr() for t in ts))
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.01, masters=None, scales=None) -> None:
+    """One AdamW step over all tensors of the lists, in place, in one launch (256 tensors each).
+
+    params fp32 or bf16, grads fp32 or bf16; ``masters``: fp32 copies that the step is made on (the parameter is then the
+    copy, rounded), or None.  exp_avg and exp_avg_sq: fp32 moments; or, with ``scales``, 8-bit ones: float8_e4m3fn tensors
+    of m and of sqrt(v), in blocks of ADAMW_BLOCK elements with scales[i] (2, blocks) fp32 (value = e4m3 * scale).
+    ``step``: int32 (1,) on the device, the number of this step, from 1 (read on the device: a captured step may be replayed).
+    hoa_adamw_step."""
+    n = len(params)
+    lists = [("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)]
+    lists += [(k, v) for k, v in (("masters", masters), ("scales", scales)) if v is not None]
+    for name, v in lists:
+        if len(v) != n:
+            raise ValueError(f"{name} must have {n} tensors as params, got {len(v)}")
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+        raise ValueError("betas must lie in [0, 1) and eps be at least 0")
+    if n == 0:
+        return
+    idx = _index(params[0])
+    _ints(step, "step", (1,), idx)
+    p_code, g_code = _dtype_code(params[0].dtype), _dtype_code(grads[0].dtype)
+    moment = torch.float32 if scales is None else torch.float8_e4m3fn
+    for i, p in enumerate(params):
+        _like(p, f"params[{i}]", p.shape, params[0].dtype, idx)
+        _like(grads[i], f"grads[{i}]", p.shape, grads[0].dtype, idx)
+        _like(exp_avg[i], f"exp_avg[{i}]", p.shape, moment, idx)
+        _like(exp_avg_sq[i], f"exp_avg_sq[{i}]", p.shape, moment, idx)
+        if masters is not None:
+            _like(masters[i], f"masters[{i}]", p.shape, torch.float32, idx)
+        if scales is not None:
+            _like(scales[i], f"scales[{i}]", (2, -(-p.numel() // ADAMW_BLOCK)), torch.float32, idx)
+    with torch.cuda.device(idx):
+        _lib.call("hoa_adamw_step", _pointers(params), p_code, _pointers(masters) if masters is not None else None, _pointers(grads),
+                  g_code, _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None,
+                  32 if scales is None else 8, _longs(*(p.numel() for p in params)), n, step.data_ptr(), lr, betas[0], betas[1], eps,
+                  weight_decay, torch._C._cuda_getCurrentRawStream(idx))

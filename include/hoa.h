@@ -452,6 +452,62 @@ int hoa_path_step(const float* a, int a_dtype, const float* a_bias, float edge_s
                   const int* lens, int B, int H, int d, int page, int n_pages, int* status, void* stream);
 
 /*
+ * Training: the backward passes of kernels (1)-(4) and the optimizer's step.  (The reference
+ * differentiates core/attention_fast_chunked.py:63-177 with autograd; kernel/attention_kernel.py:166-187
+ * recomputes the forward.)
+ *
+ * hoa_attn_fwd_lse - hoa_attn_fwd that also leaves lse (B*H, Tq) fp32, the log-sum-exp of a row's scaled
+ * scores, which the backward pass recomputes the probabilities from; v^ row-major.  bf16 with d % 8 == 0
+ * runs on tcgen05, the rest in fp32 on the CUDA cores; d <= 128.
+ */
+int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, float* o, float* lse,
+                     float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, int* status, void* stream);
+
+/*
+ * hoa_attn_bwd - gradients of causal attention (hoa_attn_fwd_lse) for the gradient `dout` (B*H, Tq, d) of o:
+ *   p_ij = exp(scale q^_i.k^_j - lse_i) (j <= q_offset + i),  ds_ij = p_ij (dout_i.v^_j - dout_i.o_i)
+ *   dq_i = scale sum_j ds_ij k^_j,  dk_j = scale sum_i ds_ij q^_i,  dv_j = sum_i p_ij dout_i
+ * q^, k^, v^, dout and the three outputs are `dtype`, o and lse fp32; every output is written in full
+ * (keys that no query sees: 0).  Sums have a fixed order: two calls give the same bits.  A NaN or
+ * infinity in a position's k^ or v^ may also reach, as 0 times it, queries that do not see it.  d <= 128,
+ * B*H <= 65535.  `status` may receive HOA_ERR_TIMEOUT.
+ */
+size_t hoa_attn_bwd_workspace_bytes(int BH, int Tq);
+int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, const float* o, const float* lse, const void* dout,
+                 int dtype, void* dq, void* dk, void* dv, float softmax_scale, int BH, int Tq, int Tk, int q_offset,
+                 int d, void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * hoa_path_bwd - gradients through the path P_t = R_t C_{t/chunk} (hoa_link_local, hoa_carry_scan) for those
+ * of the attention's inputs (dq^, dk^, dv^: hoa_attn_bwd) and of its output o, doh = P^T dout
+ * (hoa_apply_paths): da (B, T, H*stride) fp32 of the raw generators (in a_all's layout, unused slots 0; the
+ * closing edge t = T - 1 gets 0) and dqkv (B, T, H, 3d) in out_dtype, [P dq^ | P dk^ | P dv^] a head.
+ *   Z_t = sum_{s>t} skew(q^ dq^T + k^ dk^T + v^ dv^T + doh o^T)_s,  W = P_t Z_t P_t^T,
+ *   da_t = edge_scale (phi(ad_A) W)_{i<j},  A = skew(edge_scale (a + a_bias)_t),  phi(z) = (e^z - 1)/z
+ * q^, k^, v^, dq^, dk^, dv^, doh (B*H, T, d) are hat_dtype, o and everything between fp32.  P is taken as
+ * orthogonal.  A position whose bound 2 min(||A||_inf, ||A||_F / sqrt 2) passes 480, or whose sums are not
+ * finite, gets NaN.  2 <= d <= 120.  The workspace is 256-byte aligned.
+ */
+size_t hoa_path_bwd_workspace_bytes(int B, int H, int T, int d, int chunk);
+int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias, float edge_scale, const float* R, const float* C,
+                 int chunk, const void* qh, const void* kh, const void* vh, const float* o, const void* dqh,
+                 const void* dkh, const void* dvh, const void* doh, int hat_dtype, float* da, void* dqkv, int out_dtype,
+                 int B, int H, int T, int d, void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * hoa_adamw_step - one AdamW step over `count` tensors (host arrays of device pointers and of element
+ * counts), in place, in one launch a 256 tensors:
+ *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  x = x (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ * params p_dtype, grads g_dtype (each HOA_F32 or HOA_BF16).  masters (nullable, entries too): fp32 copies that the
+ * step is made on; the parameter is then the copy, rounded.  state_bits 32: m and v fp32.  8: m and sqrt(v)
+ * as e4m3 bytes, blocks of 256 elements, scales[i] (2, blocks) fp32: value = byte * scale, for m and for
+ * sqrt(v).  step: device int32, the number t of this step, from 1.
+ */
+int hoa_adamw_step(void* const* params, int p_dtype, float* const* masters, const void* const* grads, int g_dtype,
+                   void* const* m, void* const* v, float* const* scales, int state_bits, const long long* sizes, int count,
+                   const int* step, double lr, double beta1, double beta2, double eps, double weight_decay, void* stream);
+
+/*
  * hoa_selftest_wait — no counterpart in the reference.  Diagnostic for the
  * bounded device-side waits every kernel of this library uses (mbarrier waits
  * on TMA and tensor-core completion): one CTA of two warps waits on two
