@@ -228,6 +228,9 @@ extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, cons
   if (rows > 32ll * 0x7fffffff) return HOA_ERR_UNSUPPORTED;
   attn_bwd_delta_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
   if (int st = launch_status()) return st;
+  uintptr_t at = 0;                                                  // TMA and the outputs' 16-byte stores
+  for (const void* x : {qh, kh, vh, dout, (const void*)dq, (const void*)dk, (const void*)dv}) at |= reinterpret_cast<uintptr_t>(x);
+  if (dtype == HOA_BF16 && d % 8 == 0 && (at & 15) == 0) return attn_bwd_tc(a, BH, s);
   switch ((d + 15) / 16) {
     case 1: return launch_both<16>(a, BH, s);
     case 2: return launch_both<32>(a, BH, s);

@@ -17,4 +17,7 @@ struct AttnBwdArgs {
   long long max_wait;                               // bound of a wait, SM cycles (wait_bound_cycles())
 };
 
+// the tcgen05 form (hoa_attn_bwd_tc.cu): bf16, d % 8 == 0, every tensor from a 16-byte boundary; delta is there
+int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s);
+
 }  // namespace hoa

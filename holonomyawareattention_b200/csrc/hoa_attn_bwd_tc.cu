@@ -1,0 +1,328 @@
+// Gradients of causal attention, bf16 form on tcgen05 / TMEM (formulas: hoa_attn_bwd.cu).
+//
+// One kernel in two roles.  A CTA owns 128 rows of one side - keys (outputs dk, dv) or
+// queries (output dq) - and streams 64-row tiles of the other side:
+//
+//              own X0, X1   stream Y0, Y1   S = X0 Y0^T   G = X1 Y1^T    accumulators in TMEM
+//   keys       K, V         Q, dO           S^T           dP^T           dV += P^T dO,  dK += dS^T Q
+//   queries    Q, dO        K, V            S             dP                            dQ += dS K
+//
+// so a row of the CTA's matrices is a TMEM lane and a thread throughout, P and dS go back over S
+// and G as packed bf16 (the left operand of the second products, from TMEM), and the streamed
+// tile serves as the K-major right operand of the first products and, by rows, as the MN-major
+// one of the second.
+//
+// Warps (320 threads): 0-3 and 4-7 are two softmax warpgroups that take the streamed tiles in
+// turn (one's exponentials run beside the products of the other's tile), 8 issues the
+// products, 9 the TMA loads.  TMEM: S and G of two tiles (4 x 64 columns), the accumulators
+// (2 x 128).
+#include "hoa_attn_bwd.cuh"
+#include "hoa_f32x2.cuh"
+#include "hoa_tma.cuh"
+
+namespace hoa {
+using namespace sm100;
+
+constexpr int kBwThreads = 320, kBwOwn = 128, kBwStr = 64;
+
+template <int DP>
+struct BwLayout {
+  static constexpr int NKB = (DP + 63) / 64;
+  static constexpr int kOwnBlk = kBwOwn * 128, kStrBlk = kBwStr * 128;     // 64 columns of a tile
+  static constexpr int kOwn = NKB * kOwnBlk, kStr = NKB * kStrBlk;
+  static constexpr int kStage = 2 * kStr, NS = 4;
+  static constexpr int offStage = 2 * kOwn;
+  static constexpr int offCol = offStage + NS * kStage;                    // -lse log2 e and -D of the streamed queries
+  static constexpr int offBar = offCol + 2 * 2 * 128 * 4;
+  static constexpr int kAlloc = offBar + 256 + 1024;
+  static_assert(kAlloc <= 232448, "shared memory budget");
+  static constexpr uint32_t colA0 = 256, colA1 = 384;
+};
+
+HOA_DEVICE float bw_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+HOA_DEVICE float bw_pack(F2 x) {
+  const float2 v = f2_get(x);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
+}
+
+template <int DP, bool kKeys>
+__global__ void __launch_bounds__(kBwThreads, 1)
+attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant__ CUtensorMap x1,
+                   const __grid_constant__ CUtensorMap y0, const __grid_constant__ CUtensorMap y1,
+                   const __grid_constant__ AttnBwdArgs p) {
+  using L = BwLayout<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* cols = reinterpret_cast<float*>(sm + L::offCol);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::offBar);
+  uint64_t* own_full = bars;
+  uint64_t* full = bars + 1;         // [NS]
+  uint64_t* empty = full + L::NS;    // [NS]
+  uint64_t* s_full = empty + L::NS;  // [2]
+  uint64_t* p_full = s_full + 2;     // [2]
+  uint64_t* fin = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(fin + 2);
+  const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
+  const int chain = blockIdx.y, d = p.d;
+  // the longest walks first: early keys, late queries
+  const int own0 = (kKeys ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x)) * kBwOwn;
+  int first = 0, n;
+  if (kKeys) {
+    first = max(0, own0 - p.q_offset) / kBwStr;
+    n = max(0, (p.Tq + kBwStr - 1) / kBwStr - first);
+  } else {
+    n = (p.q_offset + min(own0 + kBwOwn, p.Tq) - 1) / kBwStr + 1;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2 + 2 * L::NS + 4; ++i) mbar_init(&bars[i], &bars[i] == p_full || &bars[i] == p_full + 1 ? 4 : 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool bad = false;
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ TMA
+    if (lid == 0 && n > 0) {
+      mbar_arrive_expect_tx(own_full, 2u * L::kOwn);
+      for (int kb = 0; kb < L::NKB; ++kb) {
+        tma_load_3d(sm + kb * L::kOwnBlk, &x0, own_full, kb * 64, own0, chain);
+        tma_load_3d(sm + L::kOwn + kb * L::kOwnBlk, &x1, own_full, kb * 64, own0, chain);
+      }
+      int issued = 0;
+      for (int j = 0; j < n; ++j) {
+        const int s = j % L::NS;
+        if (j >= L::NS && !mbar_wait_abortable(&empty[s], (j / L::NS - 1) & 1, s_abort, p.max_wait)) { bad = true; break; }
+        uint8_t* st = sm + L::offStage + s * L::kStage;
+        mbar_arrive_expect_tx(&full[s], (uint32_t)L::kStage);
+        for (int kb = 0; kb < L::NKB; ++kb) {
+          tma_load_3d(st + kb * L::kStrBlk, &y0, &full[s], kb * 64, (first + j) * kBwStr, chain);
+          tma_load_3d(st + L::kStr + kb * L::kStrBlk, &y1, &full[s], kb * 64, (first + j) * kBwStr, chain);
+        }
+        issued = j + 1;
+      }
+      // copies in flight land before the CTA exits (the last fill of each stage)
+      for (int j = max(0, issued - L::NS); j < issued; ++j) bad |= !mbar_wait(&full[j % L::NS], (j / L::NS) & 1);
+      bad |= !mbar_wait(own_full, 0);
+    }
+    __syncwarp();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ MMA
+    if (lid == 0 && n > 0) {
+      constexpr uint32_t idS = make_idesc(kFmtBF16, 128, kBwStr), idA = make_idesc(kFmtBF16, 128, DP, true);
+      const uint64_t dX0 = desc_sw128(smem_u32(sm)), dX1 = desc_sw128(smem_u32(sm + L::kOwn));
+      bool ok = mbar_wait_abortable(own_full, 0, s_abort, p.max_wait);
+      auto front = [&](int j) {
+        const int s = j % L::NS;
+        ok = ok && mbar_wait_abortable(&full[s], (j / L::NS) & 1, s_abort, p.max_wait);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t st = smem_u32(sm + L::offStage + s * L::kStage);
+        const uint64_t dY0 = desc_sw128(st), dY1 = desc_sw128(st + L::kStr);
+        const uint32_t cS = tmem + (j & 1) * 128;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
+          const uint64_t oy = (uint64_t)(((kk >> 2) * L::kStrBlk + (kk & 3) * 32) >> 4);
+          mma_bf16(cS, dX0 + ox, dY0 + oy, idS, kk > 0 ? 1u : 0u);
+        }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
+          const uint64_t oy = (uint64_t)(((kk >> 2) * L::kStrBlk + (kk & 3) * 32) >> 4);
+          mma_bf16(cS + 64, dX1 + ox, dY1 + oy, idS, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[j & 1]);
+      };
+      front(0);
+      for (int j = 0; j < n && ok; ++j) {
+        if (j + 1 < n) front(j + 1);
+        ok = ok && mbar_wait_abortable(&p_full[j & 1], (j >> 1) & 1, s_abort, p.max_wait);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t st = smem_u32(sm + L::offStage + (j % L::NS) * L::kStage);
+        const uint64_t mY0 = desc_sw128_mn(st, L::kStrBlk), mY1 = desc_sw128_mn(st + L::kStr, L::kStrBlk);
+        const uint32_t cS = tmem + (j & 1) * 128;
+        if (kKeys) {
+#pragma unroll
+          for (int kk = 0; kk < kBwStr / 16; ++kk)
+            mma_bf16_ts(tmem + L::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u);
+        }
+#pragma unroll
+        for (int kk = 0; kk < kBwStr / 16; ++kk)
+          mma_bf16_ts(tmem + L::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u);
+        tc_commit(&empty[j % L::NS]);
+      }
+      if (!ok) bad = true;
+      tc_commit(fin);
+      bad |= !mbar_wait(fin, 0);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- softmax
+    const int g = warp >> 2;                                      // takes the tiles g, g + 2, ...
+    const int r = tid & 127;                                      // row of the own tile = TMEM lane
+    const uint32_t lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t cS = tmem + lane + g * 128;
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float c = p.scale * kLog2e;
+    const long long qrow = (long long)chain * p.Tq;
+    // rows that are not there: exp2 of -infinity
+    auto stat = [&](const float* x, int q, float past, float f) { return q < p.Tq ? x[qrow + q] * f : past; };
+    float my_l = 0.f, my_D = 0.f, next = 0.f;
+    if (kKeys) {
+      const int q = (first + g) * kBwStr + (r & 63);
+      if (g < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
+    } else {
+      my_l = stat(p.lse, own0 + r, -INFINITY, -kLog2e);
+      my_D = stat(p.delta, own0 + r, 0.f, -1.f);
+    }
+    for (int j = g; j < n; j += 2) {
+      const int t0 = (first + j) * kBwStr;
+      float* col = cols + (g * 2 + ((j >> 1) & 1)) * 128;
+      if (kKeys) {
+        col[r] = next;
+        named_sync(1 + g, 128);
+        const int q = t0 + 2 * kBwStr + (r & 63);
+        if (j + 2 < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
+      }
+      bad |= !mbar_wait_abortable(&s_full[g], (j >> 1) & 1, s_abort, p.max_wait);
+      tc_fence_after();
+      // columns of this row that count: keys, its own key up to the query; queries, keys up to its own
+      int lo = 0, hi = kBwStr;
+      if (kKeys) lo = own0 + r - p.q_offset - t0; else hi = p.q_offset + own0 + r - t0 + 1;
+      const bool masked = kKeys ? own0 + kBwOwn - 1 > p.q_offset + t0 : t0 + kBwStr - 1 > p.q_offset + own0;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float s[32], gr[32];
+        tmem_ld32(cS + 32 * half, s);
+        tmem_ld32(cS + 64 + 32 * half, gr);
+        tmem_wait_ld();
+        tmem_touch(s);
+        tmem_touch(gr);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (kKeys ? 32 * half + e < lo : 32 * half + e >= hi) s[e] = -INFINITY;
+        }
+        float pk[16], dk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          F2 l[2], D[2];
+          if (kKeys) {
+            const float4 lv = *reinterpret_cast<const float4*>(col + 32 * half + e);
+            const float4 dv = *reinterpret_cast<const float4*>(col + 64 + 32 * half + e);
+            l[0] = f2(lv.x, lv.y);
+            l[1] = f2(lv.z, lv.w);
+            D[0] = f2(dv.x, dv.y);
+            D[1] = f2(dv.z, dv.w);
+          } else {
+            l[0] = l[1] = f2(my_l);
+            D[0] = D[1] = f2(my_D);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int i = e + 2 * k;
+            const float2 z = f2_get(f2_fma(f2(s[i], s[i + 1]), f2(c), l[k]));
+            const F2 pr = f2(bw_exp2(z.x), bw_exp2(z.y));
+            if (kKeys) pk[i / 2] = bw_pack(pr);
+            dk[i / 2] = bw_pack(f2_mul(pr, f2_add(f2(gr[i], gr[i + 1]), D[k])));
+          }
+        }
+        // (16 columns over the first half of S, which is in registers; the second half lies behind them)
+        if (kKeys) tmem_st16(cS + 16 * half, pk);
+        tmem_st16(cS + 64 + 16 * half, dk);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lid == 0) mbar_arrive(&p_full[g]);
+    }
+    // ---- epilogue: rows of the own tile that exist; two warpgroups: dv and dk, or the halves of dq
+    if (n > 0) bad |= !mbar_wait_abortable(fin, 0, s_abort, p.max_wait);
+    tc_fence_after();
+    const int rows = kKeys ? p.Tk : p.Tq;
+    const uint32_t acc = tmem + lane + (kKeys && g == 0 ? L::colA0 : L::colA1);
+    const float f = kKeys && g == 0 ? 1.f : p.scale;
+    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(!kKeys ? p.dq : g == 0 ? p.dv : p.dk) +
+                         ((long long)chain * rows + own0 + r) * d;
+#pragma unroll
+    for (int c16 = 0; c16 < DP / 16; ++c16) {
+      if (!kKeys && (c16 & 1) != g) continue;
+      float v[16];
+      if (n > 0) {
+        tmem_ld16(acc + 16 * c16, v);
+        tmem_wait_ld();
+        tmem_touch(v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = 0.f;
+      }
+      if (own0 + r >= rows || bad) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (16 * c16 + 8 * h >= d) continue;
+        uint4 w;
+        uint32_t* u = &w.x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(bw_pack(f2(v[8 * h + 2 * e] * f, v[8 * h + 2 * e + 1] * f)));
+        *reinterpret_cast<uint4*>(out + 16 * c16 + 8 * h) = w;
+      }
+    }
+  }
+
+  bad = __syncthreads_or(bad || *s_abort != 0);
+  if (bad && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <int DP, bool kKeys>
+static int launch_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+  using L = BwLayout<DP>;
+  CUtensorMap m[4];
+  const void* x[4] = {kKeys ? a.k : a.q, kKeys ? a.v : a.dout, kKeys ? a.q : a.k, kKeys ? a.dout : a.v};
+  for (int i = 0; i < 4; ++i) {
+    const int rows = (i < 2) == kKeys ? a.Tk : a.Tq;
+    if (!make_map(&m[i], x[i], a.d, rows, BH, (uint64_t)a.d * 2, (uint64_t)rows * a.d * 2, i < 2 ? kBwOwn : kBwStr)) return HOA_ERR_INVALID_ARG;
+  }
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(attn_bwd_tc_kernel<DP, kKeys>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
+  const dim3 grid((unsigned)ceil_div(kKeys ? a.Tk : a.Tq, kBwOwn), (unsigned)BH);
+  attn_bwd_tc_kernel<DP, kKeys><<<grid, kBwThreads, L::kAlloc, s>>>(m[0], m[1], m[2], m[3], a);
+  return launch_status();
+}
+
+template <int DP>
+static int launch_bwd_both(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+  const int st = launch_bwd_tc<DP, true>(a, BH, s);
+  return st == HOA_OK ? launch_bwd_tc<DP, false>(a, BH, s) : st;
+}
+
+int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+  switch ((a.d + 15) / 16) {
+    case 1: return launch_bwd_both<16>(a, BH, s);
+    case 2: return launch_bwd_both<32>(a, BH, s);
+    case 3: return launch_bwd_both<48>(a, BH, s);
+    case 4: return launch_bwd_both<64>(a, BH, s);
+    case 5: return launch_bwd_both<80>(a, BH, s);
+    case 6: return launch_bwd_both<96>(a, BH, s);
+    case 7: return launch_bwd_both<112>(a, BH, s);
+    default: return launch_bwd_both<128>(a, BH, s);
+  }
+}
+
+}  // namespace hoa

@@ -9,9 +9,7 @@
 // consumed by the inverse transport (kernel 4).
 // Queries may be a shard of the sequence: local row i is global position
 // q_offset + i and attends to keys 0 .. q_offset + i of the (gathered) key set.
-#include <cudaTypedefs.h>
-
-#include "hoa_sm100.cuh"
+#include "hoa_tma.cuh"
 
 namespace hoa {
 using namespace sm100;
@@ -312,37 +310,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ C
 // ---------------------------------------------------------------------------
 // host side: tensor maps and launch
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    return reinterpret_cast<EncodeTiledFn>(f);
-  }();
-  return fn;
-}
-
-// 3-D bf16 map over (x fastest, y, z) with a {64, box_y, 1} box, 128B swizzle, zero OOB fill.
-static bool make_map(CUtensorMap* m, const void* base, uint64_t x, uint64_t y, uint64_t z,
-                     uint64_t stride_y_bytes, uint64_t stride_z_bytes, uint32_t box_y) {
-  EncodeTiledFn enc = encode_fn();
-  if (enc == nullptr) return false;
-  cuuint64_t dims[3] = {x, y, z};
-  cuuint64_t strides[2] = {stride_y_bytes, stride_z_bytes};
-  cuuint32_t box[3] = {64, box_y, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int DP16, bool kVRows>
 static int launch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                      const AttnTcArgs& a, int BH, cudaStream_t s) {
