@@ -238,23 +238,25 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_
 }
 
 // ---------------------------------------------------------------------------
-// main: one CTA of 128 G threads a position at a time.  Products on tcgen05 with fp32
+// main: a CTA takes PP positions at a time, 128 / PP rows of its tiles each (head dims up to 32: 4,
+// up to 64: 2, else 1), so that short rows fill the 128 lanes too.  Products on tcgen05 with fp32
 // accuracy: each factor is two f16 parts (hoa_split_f16.cuh), a product three tensor-core
-// products.  With |R| <= 1, entries of Y scaled to [2^9, 2^10) and those of W to [2^5, 2^6)
-// (a power of two, per position), no part leaves f16's range: a conjugation or a commutator
-// keeps the Frobenius norm or grows it by less than 2.7 (below), so an entry stays below
-// 2^6 128 2.7 < 65504, and what f16 drops of small ones is 2^-31 of the largest.
+// products.  With |R| <= 1 and the entries of Y scaled below 2^10 (a power of two, per position),
+// entries of W = R Y R^T, at most ||Y||_F <= 128 2^10, are taken 2^-4 times: no part leaves f16's range, as a
+// commutator's Frobenius norm grows by less than 2.7 (below), so an entry stays below 2^13 2.7 < 65504;
+// what f16 drops of small ones, 2^-25, is far below 2^-22 of the usual ones.
 //
 //   U = R Y          both from shared memory (R's slabs are the K-major left operand)
 //   W = U R^T        U in TMEM; the same slabs, as the K-major right operand, are R^T
 //   V_0 = W;  V_k = alpha_k [A, V_{k-1}] (+ V_{k-2}),  M = sum_k gamma_k V_k
 // A is the left operand in TMEM for all k.  A and V are skew, so [A, V] = A V - (A V)^T: one
 // product, transposed through shared memory.  M stays in registers (a thread owns a row and
-// every G-th 16 columns).
+// every G-th 16 columns).  The right factors of the PP positions lie side by side: the product of one's
+// left rows with another's right columns is computed and not used.
 //
 // The sum: with x >= 2 ||A||_2 (from ||A||_inf and ||A||_F / sqrt 2),
-//   x <= 4   Taylor: alpha_k = 1 / (k + 1), gamma = 1, ended once what is left is below 2^-24 of
-//            W: entries of [A, V] are at most 2 ||A||_inf times those of V.
+//   x <= 4   Taylor: alpha_k = 1 / (k + 1), gamma = 1, ended once what is left, ||V_k||_F r / (1 - r) with r = x / (k + 2),
+//            is below 2^-22 of ||W||_F, what the products are good for.
 //   x > 4    Chebyshev (Taylor's terms would grow before they fall): alpha = 2 / x (1 / x first),
 //            V_{k-2} added, gamma_k = (2 - [k = 0]) / x * integral of J_k over [0, x]
 //            = (2 - [k = 0]) / x * 2 sum_m J_{k + 2m + 1}(x), the Bessel functions by Miller's
@@ -265,52 +267,86 @@ constexpr int kPbCoef = 640;
 constexpr float kPbMaxX = 480.f;
 
 template <int DP> struct PbLayout {
-  static constexpr int G = DP >= 112 ? 4 : 2, kThreads = 128 * G;
-  static constexpr int NKB = (DP + 63) / 64, NC = DP / 16, NCG = (NC + G - 1) / G;
-  static constexpr int kSlab = DP * 128, kMat = NKB * kSlab, kTwo = 2 * kMat;
+  static constexpr int RS = DP <= 32 ? 32 : DP <= 64 ? 64 : 128, PP = 128 / RS;    // rows of a position, positions
+  static constexpr int G = DP <= 16 ? 1 : DP <= 32 ? 2 : DP <= 48 ? 3 : DP <= 96 ? 2 : 4;
+  static constexpr int NT = 128 * G;
+  static constexpr int NC = DP / 16, NCG = (NC + G - 1) / G;
+  static constexpr int ND = PP > 1 ? 128 : DP;                     // columns of a product
   static constexpr int kDim = DP < 120 ? DP : 120;
+  // R: rows of 64 columns a slab, all positions' rows stacked; hi, then lo
+  static constexpr int kRowsR = PP > 1 ? 128 : DP;
+  static constexpr int kSlabR = kRowsR * 128, kMatR = (DP + 63) / 64 * kSlabR, kTwoR = 2 * kMatR;
+  // Y, V: DP rows of 64 columns a slab, the positions side by side
+  static constexpr int kSlabV = DP * 128, kMatV = (ND + 63) / 64 * kSlabV, kTwoV = 2 * kMatV;
   static constexpr int kLdT = DP + 4;
-  static constexpr int kT = kDim * kLdT * 4;                       // A V, to be read transposed
-  static constexpr int kR = ((kTwo > kT ? kTwo : kT) + 1023) / 1024 * 1024;
+  static constexpr int kT = (PP > 1 ? 128 : kDim) * kLdT * 4;      // A V, to be read transposed
+  static constexpr int kR = ((kTwoR > kT ? kTwoR : kT) + 1023) / 1024 * 1024;
   static constexpr int offV = kR;
   // (R as the left factor is read as 128 rows a slab: past its own end into what follows)
-  static constexpr int kMats = kR + kTwo > kTwo + 128 * 128 ? kR + kTwo : kTwo + 128 * 128;
+  static constexpr int kMats = kR + kTwoV > kTwoR + 128 * 128 ? kR + kTwoV : kTwoR + 128 * 128;
   static constexpr int offVec = kMats;                             // dq^, dk^, dv^ in the chunk's frame
-  static constexpr int offPart = offVec + 3 * DP * 4;
-  static constexpr int offRed = offPart + 3 * kThreads * 4;
-  static constexpr int offCoef = offRed + kThreads * 4;
-  static constexpr int offBar = offCoef + kPbCoef * 4;
+  static constexpr int offPart = offVec + PP * 3 * DP * 4;
+  static constexpr int offRed = offPart + 3 * NT * 4;
+  static constexpr int offPos = offRed + 2 * 16 * 4;               // of each position: top, norm bound, terms
+  static constexpr int offCoef = offPos + 4 * 4 * 4;
+  static constexpr int offBar = offCoef + PP * kPbCoef * 4;
   static constexpr int kAlloc = offBar + 64 + 1024;
   static constexpr int kMinBlocks = kAlloc <= 113 * 1024 ? 2 : 1;
-  static constexpr uint32_t kCols = DP <= 16 ? 32 : DP <= 32 ? 64 : DP <= 64 ? 128 : 256;
-  static constexpr uint32_t colD = 0, colHi = DP, colLo = DP + DP / 2;
-  static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2 + kThreads - 1) / kThreads;
-  static constexpr int kScratch = 2 * NCG * 4 * kThreads;          // float4s of a CTA's old iterates
+  static constexpr uint32_t kCols = ND + DP <= 256 ? 256 : 512;
+  static constexpr uint32_t colD = 0, colHi = ND, colLo = ND + DP / 2;
+  static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2 + NT - 1) / NT;
+  static constexpr int kScratch = 2 * NCG * 4 * NT;                // float4s of a CTA's old iterates
+  static_assert(kPbRun % PP == 0, "a pass stays in its run");
 };
 
-// power of two that puts x into [2^e, 2^(e+1)), as an exponent; 0 where x is 0 or not finite
-HOA_DEVICE int pb_exponent(float x, int e) {
-  if (!(x > 0.f) || !(x <= 3.0e38f)) return 0;
-  return max(-100, min(100, e - ilogbf(x)));
+// gamma_k (k >= 0) for x, and how many terms they need
+HOA_DEVICE int pb_chebyshev(double x, float* coef) {
+  // J_n by the recurrence J_{n-1} = 2 n / x J_n - J_{n+1} downwards from J_{N+1} = 0 and any small J_N; the first
+  // pass finds what to divide by (J_0 + 2 (J_2 + J_4 + ...) = 1), the second one leaves the coefficients
+  const double i2x = 2.0 / x;
+  const int N = min(kPbCoef - 2, (int)(x + 40.0 + 8.0 * cbrt(x)));
+  double start = 1e-100;
+  int terms = 1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    double j1 = 0.0, j0 = start, even = 0.0, odd = 0.0;              // sums of J_n, J_{n+2}, ... so far, by the parity of n
+#pragma unroll 1
+    for (int n = N; n >= 1; --n) {
+      double& tail = n & 1 ? odd : even;
+      tail += j0;
+      if (pass == 1) {
+        const float v = (float)(tail * (n == 1 ? 2.0 : 4.0) / x);
+        coef[n - 1] = v;
+        if (terms == 1 && fabsf(v) > 2e-9f) terms = max(1, n - 1);
+      }
+      const double j = n * i2x * j0 - j1;
+      j1 = j0;
+      j0 = j;
+    }
+    start /= j0 + 2.0 * even;
+  }
+  return terms;
 }
 
 template <int DP>
-__global__ void __launch_bounds__(PbLayout<DP>::kThreads, PbLayout<DP>::kMinBlocks)
+__global__ void __launch_bounds__(PbLayout<DP>::NT, PbLayout<DP>::kMinBlocks)
 path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
   using L = PbLayout<DP>;
-  constexpr int G = L::G, NT = L::kThreads, NCG = L::NCG;
+  constexpr int G = L::G, NT = L::NT, NCG = L::NCG, PP = L::PP, RS = L::RS, NW = NT / 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* gen = reinterpret_cast<float*>(sm);                        // R's place, once R is done with
   float* T = reinterpret_cast<float*>(sm);
   float* vec = reinterpret_cast<float*>(sm + L::offVec);
   float* part = reinterpret_cast<float*>(sm + L::offPart);
-  float* red = reinterpret_cast<float*>(sm + L::offRed);
+  float* red = reinterpret_cast<float*>(sm + L::offRed);           // [2][16]
+  unsigned* s_top = reinterpret_cast<unsigned*>(sm + L::offPos);   // [4] the largest |Y|, as bits
+  float* s_x = reinterpret_cast<float*>(sm + L::offPos) + 4;       // [4] x
+  int* s_terms = reinterpret_cast<int*>(sm + L::offPos) + 8;       // [4] Chebyshev: products
   float* coef = reinterpret_cast<float*>(sm + L::offCoef);
   uint64_t* done = reinterpret_cast<uint64_t*>(sm + L::offBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* s_terms = s_abort + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int d = p.d;
   if (tid == 0) {
@@ -318,6 +354,7 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
     *s_abort = 0;
     fence_mbar_init();
   }
+  if (tid < 4) s_top[tid] = 0;
   if (warp == 0) {
     tmem_alloc(tmem_slot, L::kCols);
     tmem_relinquish();
@@ -327,22 +364,26 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);
-  const int row = (warp & 3) * 32 + lid, group = warp >> 2;
-  const bool works = (warp & 3) * 32 < DP;                          // (the warp has rows of the matrix)
+  const int lrow = (warp & 3) * 32 + lid, group = warp >> 2;        // TMEM lane
+  const int mine = (warp & 3) * 32 / RS, row0 = (warp & 3) * 32 - mine * RS, row = row0 + lid;   // position, row of its matrix
+  const bool works = row0 < DP;                                     // (the warp has rows of a matrix)
+  const uint32_t laneD = lanes + L::colD + (PP > 1 ? mine * RS : 0);
   uint32_t phase = 0;
   bool bad = false;
 
-  // ---- matrices from global memory, DP / 4 threads a row, 4 columns each
-  constexpr int n4 = DP / 4, RG = NT / n4, kRows = (DP + RG - 1) / RG;
+  // ---- the positions' matrices from global memory, DP / 4 threads a row, 4 columns each
+  constexpr int n4 = DP / 4, RG = NT / n4, kRows = (PP * DP + RG - 1) / RG;
   const int pr = tid / n4, pc = (tid % n4) * 4;
   float4 pv[kRows];
-  auto load_mat = [&](const float* m) {
+  auto load_mat = [&](const float* m, int live) {                   // of `live` positions, d x d each
+    int r0 = pr;
+    asm volatile("" : "+r"(r0));
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int r = pr + k * RG;
+      const int q = r0 + k * RG, w = PP > 1 ? q / DP : 0, r = q - w * DP;
       pv[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (pr >= RG || r >= d || pc >= d) continue;
-      const float* at = m + r * d + pc;
+      if (r0 >= RG || w >= live || r >= d || pc >= d) continue;
+      const float* at = m + (w * d + r) * d + pc;
       if (vec4) {
         pv[k] = *reinterpret_cast<const float4*>(at);
       } else {
@@ -353,19 +394,32 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
       }
     }
   };
-  auto put_mat = [&](uint8_t* mat, float scale) {
-    uint8_t* slab = mat + (pc >> 6) * L::kSlab + (pc & 7) * 2;
-    const uint32_t ch = (pc & 63) >> 3;
+  auto put_half = [&](uint8_t* at, int mat, float4 v, float scale) {
+    uint2 hi, lo;
+    st_split2(f2_mul(f2(v.x, v.y), f2(scale)), hi.x, lo.x);
+    st_split2(f2_mul(f2(v.z, v.w), f2(scale)), hi.y, lo.y);
+    *reinterpret_cast<uint2*>(at) = hi;
+    *reinterpret_cast<uint2*>(at + mat) = lo;
+  };
+  auto put_R = [&]() {
+    int r0 = pr;
+    asm volatile("" : "+r"(r0));
+    uint8_t* slab = sm + (pc >> 6) * L::kSlabR + (pc & 7) * 2;
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      const int r = pr + k * RG;
-      if (pr >= RG || r >= DP) continue;
-      uint2 hi, lo;
-      st_split2(f2_mul(f2(pv[k].x, pv[k].y), f2(scale)), hi.x, lo.x);
-      st_split2(f2_mul(f2(pv[k].z, pv[k].w), f2(scale)), hi.y, lo.y);
-      uint8_t* at = slab + sw128_offset(r, ch);
-      *reinterpret_cast<uint2*>(at) = hi;
-      *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+      const int q = r0 + k * RG, w = PP > 1 ? q / DP : 0, r = q - w * DP + w * RS;
+      if (r0 >= RG || q >= PP * DP) continue;
+      put_half(slab + sw128_offset(r, (pc & 63) >> 3), L::kMatR, pv[k], kPbR);
+    }
+  };
+  auto put_Y = [&](const float* scales) {                           // a scale a position
+    int r0 = pr;
+    asm volatile("" : "+r"(r0));
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const int q = r0 + k * RG, w = PP > 1 ? q / DP : 0, r = q - w * DP, c = pc + w * RS;
+      if (r0 >= RG || q >= PP * DP) continue;
+      put_half(sm + L::offV + (c >> 6) * L::kSlabV + (c & 7) * 2 + sw128_offset(r, (c & 63) >> 3), L::kMatV, pv[k], scales[w]);
     }
   };
   // ---- a thread's own 16 columns (chunk c) of its row
@@ -378,10 +432,10 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
       st_split2(v[4 * q + 1], h.y, l.y);
       st_split2(v[4 * q + 2], h.z, l.z);
       st_split2(v[4 * q + 3], h.w, l.w);
-      const int ch = 2 * c + q;
-      uint8_t* at = sm + L::offV + (ch >> 3) * L::kSlab + sw128_offset(row, ch & 7);
+      const int ch = 2 * c + q + (PP > 1 ? mine * RS / 8 : 0);
+      uint8_t* at = sm + L::offV + (ch >> 3) * L::kSlabV + sw128_offset(row, ch & 7);
       *reinterpret_cast<uint4*>(at) = h;
-      *reinterpret_cast<uint4*>(at + L::kMat) = l;
+      *reinterpret_cast<uint4*>(at + L::kMatV) = l;
     }
   };
   auto put_left = [&](int c, const F2 (&v)[8]) {
@@ -397,36 +451,37 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
     tmem_st8(lanes + L::colLo + 8 * c, l);
   };
   auto load_D = [&](int c, float (&v)[16]) {
-    tmem_ld16(lanes + L::colD + 16 * c, v);
+    tmem_ld16(laneD + 16 * c, v);
     tmem_wait_ld();
     tmem_touch(v);
   };
-
   // this row's columns 16 c .. of a d x d matrix, times f; 0 outside
-  auto mask_row = [&](int c, float f, float (&v)[16]) {
+  auto mask_row = [&](int c, float f, const float (&v)[16], F2 (&x)[8]) {
     int n = row < d ? d - 16 * c : 0;
     asm volatile("" : "+r"(n));
     if (n >= 16) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] *= f;
+      for (int e = 0; e < 8; ++e) x[e] = f2_mul(f2(v[2 * e], v[2 * e + 1]), f2(f));
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = e < n ? v[e] * f : 0.f;
+      for (int e = 0; e < 8; ++e) x[e] = f2(2 * e < n ? v[2 * e] * f : 0.f, 2 * e + 1 < n ? v[2 * e + 1] * f : 0.f);
     }
   };
 
   // ---- products.  Left R from shared memory or the left factor in TMEM; right: the slabs at V by rows, or R^T
   const uint32_t base = smem_u32(sm);
-  const uint64_t rK[2] = {desc_sw128(base), desc_sw128(base + L::kMat)};
-  const uint64_t vN[2] = {desc_sw128_mn(base + L::offV, L::kSlab), desc_sw128_mn(base + L::offV + L::kMat, L::kSlab)};
-  constexpr uint32_t idN = make_idesc(0, 128, DP, true), idK = make_idesc(0, 128, DP, false);
-  auto mma = [&](bool left_R, bool right_R) {
+  const uint64_t rK[2] = {desc_sw128(base), desc_sw128(base + L::kMatR)};
+  const uint64_t vN[2] = {desc_sw128_mn(base + L::offV, L::kSlabV), desc_sw128_mn(base + L::offV + L::kMatV, L::kSlabV)};
+  constexpr uint32_t idN = make_idesc(0, 128, L::ND, true), idK = make_idesc(0, 128, L::ND, false);
+  auto issue = [&](bool left_R, bool right_R) {
+    if (tid != 0 || bad) return;
+    tc_fence_after();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int a = pass == 1, b = pass == 0;                       // hi lo, lo hi, hi hi
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        const uint64_t kk = (uint64_t)(((k >> 2) * L::kSlab + (k & 3) * 32) >> 4);
+        const uint64_t kk = (uint64_t)(((k >> 2) * L::kSlabR + (k & 3) * 32) >> 4);
         const uint32_t acc = pass > 0 || k > 0 ? 1u : 0u;
         const uint64_t rd = right_R ? rK[b] + kk : vN[b] + (uint64_t)(k * 2048 >> 4);
         if (left_R) mma_bf16(tmem + L::colD, rK[a] + kk, rd, idN, acc);
@@ -435,17 +490,11 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
     }
     tc_commit(done);
   };
-  // what every thread wrote (shared memory, TMEM) -> the tensor core
+  // what every thread wrote (shared memory, TMEM) -> the tensor core, after a barrier
   auto publish = [&]() {
     tmem_wait_st();
     fence_proxy_async_smem();
     tc_fence_before();
-  };
-  auto issue = [&](bool left_R, bool right_R) {
-    if (tid == 0 && !bad) {
-      tc_fence_after();
-      mma(left_R, right_R);
-    }
   };
   auto wait = [&]() {
     if (!bad) {
@@ -459,78 +508,115 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
     }
     tc_fence_after();
   };
-  // the largest over the CTA of v >= 0 (NaN and infinity show as infinity); one barrier inside
-  auto top_of = [&](float v, float* at) {
-    v = v <= 3.0e38f ? v : INFINITY;
+  // the sum of the NW per-warp values in `at` that belong to position w
+  auto sum_of = [&](const float* at, int w) {
+    float s = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (lid == 0) at[warp] = v;
-    __syncthreads();
-    float t = at[0];
+    for (int i = 0; i < NW; ++i)
+      if ((i & 3) * 32 / RS == w) s += at[i];
+    return s;
+  };
+  auto warp_sum = [&](float v) {
 #pragma unroll
-    for (int w = 1; w < NT / 32; ++w) t = fmaxf(t, at[w]);
-    return t;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   };
 
   float4* scratch = p.V + (long long)blockIdx.x * L::kScratch + tid;
-  const long long units = (long long)p.runs * kPbRun;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
-    const long long lr = u / kPbRun;
+  const long long passes = (long long)p.runs * (kPbRun / PP);
+  for (long long u = blockIdx.x; u < passes; u += gridDim.x) {
+    const long long lr = u / (kPbRun / PP);
     const PbRun r = pb_run(p, p.run0 + lr);
-    const int t = r.t0 + (int)(u - lr * kPbRun);
+    const int t = r.t0 + (int)(u - lr * (kPbRun / PP)) * PP;
     if (t >= r.t1) continue;                                        // (block-uniform)
+    const int live = min(PP, r.t1 - t);
     const int b = r.chain / p.H, h = r.chain - b * p.H;
-    const long long pos = ((long long)b * p.T + t) * p.H + h;
+    const long long pos = ((long long)b * p.T + t) * p.H + h;       // position w: pos + w H
     // ---- R and Y as factors
-    load_mat(p.R + ((long long)r.chain * p.T + t) * d * d);
-    put_mat(sm, kPbR);
-    load_mat(p.Y + u * d * d);
-    for (int i = tid; i < 3 * DP; i += NT) vec[i] = i % DP < d ? p.F[u * 3 * d + i / DP * d + i % DP] : 0.f;
-    float top = 0.f;
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      // (fmaxf drops a NaN: the sum carries it)
-      const float s = fabsf(pv[k].x) + fabsf(pv[k].y) + fabsf(pv[k].z) + fabsf(pv[k].w);
-      top = s <= 3.0e38f ? fmaxf(top, fmaxf(fmaxf(fabsf(pv[k].x), fabsf(pv[k].y)), fmaxf(fabsf(pv[k].z), fabsf(pv[k].w)))) : INFINITY;
+    load_mat(p.R + ((long long)r.chain * p.T + t) * d * d, live);
+    put_R();
+    load_mat(p.Y + u * PP * d * d, live);
+    for (int i = tid; i < PP * 3 * DP; i += NT) {
+      const int w = i / (3 * DP), e = i % DP;
+      vec[i] = w < live && e < d ? p.F[((u * PP + w) * 3 + i / DP % 3) * d + e] : 0.f;
     }
-    top = top_of(top, red);
-    bool lost = !(top <= 3.0e38f);                                  // nothing finite can come of this position
-    const int e_y = pb_exponent(top, 9);
-    put_mat(sm + L::offV, ldexpf(1.f, e_y));
+    {
+      unsigned top[PP];
+#pragma unroll
+      for (int w = 0; w < PP; ++w) top[w] = 0;
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int w = PP > 1 ? (pr + k * RG) / DP : 0;
+        // (as bits: a NaN is above infinity)
+        const unsigned v = max(max(__float_as_uint(fabsf(pv[k].x)), __float_as_uint(fabsf(pv[k].y))),
+                               max(__float_as_uint(fabsf(pv[k].z)), __float_as_uint(fabsf(pv[k].w))));
+#pragma unroll
+        for (int i = 0; i < PP; ++i) top[i] = i == w ? max(top[i], v) : top[i];
+      }
+#pragma unroll
+      for (int w = 0; w < PP; ++w) {
+        const unsigned v = __reduce_max_sync(0xffffffffu, top[w]);
+        if (lid == 0) atomicMax(&s_top[w], v);
+      }
+    }
+    __syncthreads();
+    bool lost = false;                                              // nothing finite can come of this thread's position
+    int e_y = 0;
+    {
+      float scales[PP];
+#pragma unroll
+      for (int w = 0; w < PP; ++w) {
+        const float top = __uint_as_float(s_top[w]);
+        const bool fin = top <= 3.0e38f;
+        const int e = fin && top > 0.f ? max(-100, min(100, 9 - ilogbf(top))) : 0;
+        scales[w] = ldexpf(1.f, e);
+        if (w == mine) {
+          e_y = e;
+          lost = !fin;
+        }
+      }
+      put_Y(scales);
+    }
     publish();
     __syncthreads();
     issue(true, false);                                             // U = R Y, in units of 2^-e_y / kPbR
     // ---- meanwhile: the generators on their way, and dq, dk, dv = R (.)
-    float g[L::kGen];
-    const float* ag = p.a + pos * p.stride;
+    float g[PP][L::kGen];
 #pragma unroll
-    for (int k = 0; k < L::kGen; ++k) {
-      const int i = tid + k * NT;
-      g[k] = i < p.stride ? ag[i] : 0.f;
-      if (p.a_bias != nullptr && i < p.stride) g[k] += p.a_bias[(long long)h * p.stride + i];
+    for (int w = 0; w < PP; ++w) {
+      const float* ag = p.a + (pos + (long long)w * p.H) * p.stride;
+#pragma unroll
+      for (int k = 0; k < L::kGen; ++k) {
+        const int i = tid + k * NT;
+        g[w][k] = i < p.stride && w < live ? ag[i] : 0.f;
+        if (p.a_bias != nullptr && i < p.stride) g[w][k] += p.a_bias[(long long)h * p.stride + i];
+      }
     }
     {
       float y[3] = {0.f, 0.f, 0.f};
-      if (works)
+      if (works) {
+        const float* my = vec + mine * 3 * DP;
+#pragma unroll 1
         for (int c = group; c < L::NC; c += G) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int ch = 2 * c + q;
-            const uint8_t* at = sm + (ch >> 3) * L::kSlab + sw128_offset(row < DP ? row : 0, ch & 7);
-            const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + L::kMat);
+            const uint8_t* at = sm + (ch >> 3) * L::kSlabR + sw128_offset(min(row, DP - 1) + mine * RS, ch & 7);
+            const uint4 hi = *reinterpret_cast<const uint4*>(at), lo = *reinterpret_cast<const uint4*>(at + L::kMatR);
             const float2 m[4] = {f2_get(st_join2(hi.x, lo.x)), f2_get(st_join2(hi.y, lo.y)), f2_get(st_join2(hi.z, lo.z)),
                                  f2_get(st_join2(hi.w, lo.w))};
 #pragma unroll
             for (int w = 0; w < 3; ++w)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 x = *reinterpret_cast<const float2*>(vec + w * DP + 8 * ch + 2 * e);
-                y[w] = fmaf(m[e].x, x.x, fmaf(m[e].y, x.y, y[w]));
+              for (int e = 0; e < 4; e += 2) {
+                const float4 x = *reinterpret_cast<const float4*>(my + w * DP + 8 * ch + 2 * e);
+                y[w] = fmaf(m[e].x, x.x, fmaf(m[e].y, x.y, fmaf(m[e + 1].x, x.z, fmaf(m[e + 1].y, x.w, y[w]))));
               }
           }
         }
+      }
 #pragma unroll
-      for (int w = 0; w < 3; ++w) part[w * NT + group * 128 + row] = y[w];
+      for (int w = 0; w < 3; ++w) part[w * NT + group * 128 + lrow] = y[w];
     }
     wait();
     if (works) {
@@ -547,109 +633,82 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
     publish();
     __syncthreads();
     issue(false, true);                                             // W = U R^T, in units of 16 2^-e_y / kPbR
-    for (int i = tid; i < 3 * d; i += NT) {
-      const int w = i / d, e = i - w * d;
+    if (tid < 4) s_top[tid] = 0;                                    // (read before the last barrier)
+    for (int i = tid; i < live * 3 * d; i += NT) {
+      const int q = i / d, e = i - q * d, pw = q / 3, w = q - 3 * pw;
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < G; ++k) s += part[w * NT + k * 128 + e];
-      store_elem(p.dqkv, pos * 3 * d + i, p.out_dtype, s * (1.f / kPbR));
+      for (int k = 0; k < G; ++k) s += part[w * NT + k * 128 + pw * RS + e];
+      store_elem(p.dqkv, (pos + (long long)pw * p.H) * 3 * d + w * d + e, p.out_dtype, s * (1.f / kPbR));
     }
     wait();
-    top = 0.f;
-    if (works) {
-#pragma unroll 1
-      for (int c = group; c < L::NC; c += G) {
+#pragma unroll
+    for (int w = 0; w < PP; ++w)
+#pragma unroll
+      for (int k = 0; k < L::kGen; ++k)
+        if (tid + k * NT < p.stride) gen[w * p.stride + tid + k * NT] = g[w][k];
+    __syncthreads();
+    // ---- V_0 = W as the right factor (units: 2^(4 - e_y)), A as the left one; the norms of W and of A
+    F2 M[NCG][8];
+    float rs = 0.f;
+    {
+      F2 sq = f2(0.f), sw = f2(0.f);
+#pragma unroll
+      for (int ci = 0; ci < NCG; ++ci) {
+        const int c = group + ci * G;
+        if (!works || c >= L::NC) continue;
         float v[16];
+        F2 x[8];
         load_D(c, v);
-        if (row < d)
+        mask_row(c, 1.f / kPbR, v, M[ci]);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(v[e]));
+        for (int e = 0; e < 8; ++e) sw = f2_fma(M[ci][e], M[ci][e], sw);
+        put_right(c, M[ci]);
+        int at = row;
+        asm volatile("" : "+r"(at));                                // (its index math stays here: no registers across the products)
+        gen_row16(gen + mine * p.stride, p.banked != 0, p.stride, d, at, lid, 16 * c, p.edge_scale * kPbA, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 a = f2_get(x[e]);
+          rs += fabsf(a.x) + fabsf(a.y);
+          sq = f2_fma(x[e], x[e], sq);
+        }
+        put_left(c, x);
+      }
+      part[group * 128 + lrow] = rs;
+      const float2 a = f2_get(sq), w = f2_get(sw);
+      const float ta = warp_sum(a.x + a.y), tw = warp_sum(w.x + w.y);
+      if (lid == 0) {
+        part[NT + warp] = ta;
+        red[warp] = tw;
       }
     }
-#pragma unroll
-    for (int k = 0; k < L::kGen; ++k)
-      if (tid + k * NT < p.stride) gen[tid + k * NT] = g[k];
-    top = top_of(top, red);
-    lost |= !(top <= 3.0e38f);
-    const int e_w = pb_exponent(top, 5);
-    const float f_w = ldexpf(1.f, e_w);
-    const float wmax = top * f_w;
-    // ---- V_0 = W as the right factor, A as the left one; the norms of A
-    float M[NCG][16], rs = 0.f, sq = 0.f;
-#pragma unroll
-    for (int ci = 0; ci < NCG; ++ci) {
-      const int c = group + ci * G;
-      if (!works || c >= L::NC) continue;
-      F2 x[8];
-      load_D(c, M[ci]);
-      mask_row(c, f_w, M[ci]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = f2(M[ci][2 * e], M[ci][2 * e + 1]);
-      put_right(c, x);
-      int at = row;
-      asm volatile("" : "+r"(at));                                  // (its index math stays here: no registers across the products)
-      gen_row16(gen, p.banked != 0, p.stride, d, at, lid, 16 * c, p.edge_scale * kPbA, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 v = f2_get(x[e]);
-        rs += fabsf(v.x) + fabsf(v.y);
-        sq = fmaf(v.x, v.x, fmaf(v.y, v.y, sq));
-      }
-      put_left(c, x);
-    }
-    part[NT + group * 128 + row] = rs;                              // (not red: a slow warp may still read top_of's values there)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    if (lid == 0) part[warp] = sq;
     publish();
     __syncthreads();
     issue(false, false);                                            // A V_0
-    float inf = 0.f, fro = 0.f;
+    {
+      float inf = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float s = 0.f;
+      for (int q = 0; q < RS / 32; ++q) {
+        float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < G; ++k) s += part[NT + k * 128 + lid + 32 * q];
-      inf = s <= 3.0e38f ? fmaxf(inf, lid + 32 * q < d ? s : 0.f) : INFINITY;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) inf = fmaxf(inf, __shfl_xor_sync(0xffffffffu, inf, o));
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) fro += part[w];
-    inf *= 1.00001f / kPbA;                                         // (bounds: rounded up)
-    fro = sqrtf(0.5f * fro) * (1.00001f / kPbA);
-    const float x2 = 2.f * fminf(inf, fro);
-    lost |= !(x2 <= kPbMaxX);
-    const bool cheb = !lost && x2 > 4.f;
-    if (cheb && tid == 32) {
-      // J_n by the recurrence J_{n-1} = 2 n / x J_n - J_{n+1} downwards from J_{N+1} = 0 and any small J_N; the first
-      // pass finds what to divide by (J_0 + 2 (J_2 + J_4 + ...) = 1), the second one leaves the coefficients
-      const double x = (double)x2, i2x = 2.0 / x;
-      const int N = min(kPbCoef - 2, (int)(x + 40.0 + 8.0 * cbrt(x)));
-      double start = 1e-100;
-      int terms = 1;
-#pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
-        double j1 = 0.0, j0 = start, even = 0.0, odd = 0.0;          // sums of J_n, J_{n+2}, ... so far, by the parity of n
-#pragma unroll 1
-        for (int n = N; n >= 1; --n) {
-          double& tail = n & 1 ? odd : even;
-          tail += j0;
-          if (pass == 1) {
-            const float v = (float)(tail * (n == 1 ? 2.0 : 4.0) / x);
-            coef[n - 1] = v;
-            if (terms == 1 && fabsf(v) > 2e-9f) terms = max(1, n - 1);
-          }
-          const double j = n * i2x * j0 - j1;
-          j1 = j0;
-          j0 = j;
-        }
-        start /= j0 + 2.0 * even;
+        for (int k = 0; k < G; ++k) s += part[k * 128 + mine * RS + lid + 32 * q];
+        if (lid + 32 * q < DP) inf = s <= 3.0e38f ? fmaxf(inf, s) : INFINITY;
       }
-      *s_terms = terms;
+      inf = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(inf)));
+      // (a bound: rounded up)
+      const float x = 2.00002f / kPbA * fminf(inf, sqrtf(0.5f * sum_of(part + NT, mine)));
+      lost |= !(x <= kPbMaxX);
+      // one warp of each position leaves what all need to know; Taylor for what is lost, ended at once
+      if (row0 == 0 && group == G - 1 && lid == 0) {
+        s_x[mine] = lost ? 0.f : x;
+        s_terms[mine] = !lost && x > 4.f ? pb_chebyshev((double)x, coef + mine * kPbCoef) : 0;
+      }
     }
     // ---- the series
-    const float a_t = 1.f / kPbA;
+    float wq[PP];
+#pragma unroll
+    for (int w = 0; w < PP; ++w) wq[w] = sum_of(red, w);
     for (int k = 1;; ++k) {
       wait();
 #pragma unroll
@@ -661,99 +720,119 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
         if (row < d)
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4*>(T + row * L::kLdT + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            *reinterpret_cast<float4*>(T + lrow * L::kLdT + 16 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       }
       __syncthreads();
-      const int terms = cheb ? *s_terms : 64;
-      const float alpha = cheb ? (k == 1 ? a_t : 2.f * a_t) / x2 : a_t / (float)(k + 1);
-      const float gamma = cheb ? coef[k] : 1.f;
-      float vtop = 0.f;
+      const int terms = s_terms[mine];
+      const bool cheb = terms > 0;
+      const float alpha = cheb ? (k == 1 ? 1.f / kPbA : 2.f / kPbA) / s_x[mine] : 1.f / (kPbA * (float)(k + 1));
+      const float gamma = cheb ? (k <= terms ? coef[mine * kPbCoef + k] : 0.f) : 1.f;
+      F2 vv = f2(0.f);
 #pragma unroll
       for (int ci = 0; ci < NCG; ++ci) {
         const int c = group + ci * G;
         if (!works || c >= L::NC) continue;
         float v[16];
+        F2 x[8];
         load_D(c, v);
-        int at = 16 * c * L::kLdT + row;
+        int at = (16 * c + mine * RS) * L::kLdT + row;
         asm volatile("" : "+r"(at));
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] -= T[at + e * L::kLdT];   // (rows past d: whatever lies there, masked below)
-        mask_row(c, alpha, v);
+        mask_row(c, alpha, v, x);
         if (cheb) {
-          float4* at = scratch + (long long)(((k & 1) * NCG + ci) * 4) * NT;
+          float4* at4 = scratch + (long long)(((k & 1) * NCG + ci) * 4) * NT;
           if (k == 1) {
             float4* old = scratch + (long long)(ci * 4) * NT;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) old[q * NT] = make_float4(M[ci][4 * q], M[ci][4 * q + 1], M[ci][4 * q + 2], M[ci][4 * q + 3]);
+            for (int q = 0; q < 4; ++q) {
+              const float2 lo = f2_get(M[ci][2 * q]), hi = f2_get(M[ci][2 * q + 1]);
+              old[q * NT] = make_float4(lo.x, lo.y, hi.x, hi.y);
+            }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) M[ci][e] *= coef[0];
+            for (int e = 0; e < 8; ++e) M[ci][e] = f2_mul(M[ci][e], f2(coef[mine * kPbCoef]));
           } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const float4 o = at[q * NT];
-              v[4 * q] += o.x;
-              v[4 * q + 1] += o.y;
-              v[4 * q + 2] += o.z;
-              v[4 * q + 3] += o.w;
+              const float4 o = at4[q * NT];
+              x[2 * q] = f2_add(x[2 * q], f2(o.x, o.y));
+              x[2 * q + 1] = f2_add(x[2 * q + 1], f2(o.z, o.w));
             }
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) at[q * NT] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        }
-        F2 x[8];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          M[ci][e] = fmaf(gamma, v[e], M[ci][e]);
-          vtop = fmaxf(vtop, fabsf(v[e]));
+          for (int q = 0; q < 4; ++q) {
+            const float2 lo = f2_get(x[2 * q]), hi = f2_get(x[2 * q + 1]);
+            at4[q * NT] = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f2(v[2 * e], v[2 * e + 1]);
+        for (int e = 0; e < 8; ++e) {
+          M[ci][e] = f2_fma(x[e], f2(gamma), M[ci][e]);
+          vv = f2_fma(x[e], x[e], vv);
+        }
         put_right(c, x);
       }
-      // Taylor: entries of the terms still to come sum to at most vtop rho / (1 - rho)
-      const float rho = 2.f * inf / (float)(k + 2);
-      bool more = cheb || (rho < 1.f ? vtop * rho > 5.96e-8f * wmax * (1.f - rho) : true);
-      more = more && k < terms && !lost;
+      {
+        const float2 v = f2_get(vv);
+        const float tv = warp_sum(v.x + v.y);
+        if (lid == 0) red[(k & 1) * 16 + warp] = tv;
+      }
       publish();
-      if (!__syncthreads_or(more)) break;
+      __syncthreads();
+      bool more = false;
+#pragma unroll
+      for (int w = 0; w < PP; ++w) {
+        const int n = s_terms[w];
+        const float rr = s_x[w] / (float)(k + 2);
+        const float left = rr / (1.f - rr);
+        more |= n > 0 ? k < n : k < 64 && (rr >= 1.f || sum_of(red + (k & 1) * 16, w) * left * left > 5.7e-14f * wq[w]);
+      }
+      if (!more) break;
       issue(false, false);
     }
     // ---- da: the upper triangle in the generators' layout, through shared memory
-    float* out = T;
-    if (p.banked)
-      for (int i = tid; i < p.stride; i += NT) out[i] = 0.f;
-    if (p.banked) __syncthreads();
+    float* out = T + mine * p.stride;
+    if (p.banked) {
+      for (int i = tid; i < PP * p.stride; i += NT) T[i] = 0.f;
+      __syncthreads();
+    }
     {
-      const float nan = __int_as_float(0x7fffffff);
-      const bool last = t == p.T - 1;
-      const float f1 = ldexpf(1.f, -e_y), f2w = ldexpf(p.edge_scale, -e_w - 4);
-      const int base_r = row * (2 * d - row - 1) / 2 - row - 1;
+      const bool last = t + mine == p.T - 1;
+      const float f1 = lost ? __int_as_float(0x7fffffff) : ldexpf(1.f, -e_y), f2w = 16.f * p.edge_scale;
+      int base_r = row * (2 * d - row - 1) / 2 - row - 1;
+      asm volatile("" : "+r"(base_r));
 #pragma unroll
       for (int ci = 0; ci < NCG; ++ci) {
         const int c = group + ci * G;
-        if (!works || c >= L::NC || row >= d) continue;
-        int at = row, c0 = 16 * c;
-        asm volatile("" : "+r"(at), "+r"(c0));
+        if (!works || c >= L::NC || row >= d || 16 * c + 15 <= row0) continue;
+        int n = d - 16 * c, k0 = row - 16 * c, at = row;             // columns k0 < e < n of the chunk
+        asm volatile("" : "+r"(n), "+r"(k0), "+r"(at));
+        float* o = out + base_r + 16 * c;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int cc = c0 + e;
-          if (cc <= at || cc >= d) continue;
-          const float v = last ? 0.f : lost ? nan : M[ci][e] * f2w * f1;
-          out[p.banked ? gen_banked_slot(at, cc, d) : base_r + cc] = v;
+          const float2 m = f2_get(M[ci][e / 2]);
+          const float v = last ? 0.f : (e & 1 ? m.y : m.x) * f2w * f1;
+          if (e > k0 && e < n) {
+            if (p.banked) out[gen_banked_slot(at, 16 * c + e, d)] = v;
+            else o[e] = v;
+          }
         }
       }
     }
     if (__syncthreads_or(bad)) break;
-    float* dg = p.da + pos * p.stride;
-    for (int i = tid; i < p.stride; i += NT) dg[i] = out[i];
-    __syncthreads();                                                // the next position writes R there
+#pragma unroll
+    for (int w = 0; w < PP; ++w) {
+      if (w >= live) break;
+      float* dg = p.da + (pos + (long long)w * p.H) * p.stride;
+      for (int i = tid; i < p.stride; i += NT) dg[i] = T[w * p.stride + i];
+    }
+    __syncthreads();                                                // the next pass writes R there
   }
   if (tid == 0 && bad) mbar_wait(done, phase);                      // the product that it gave up on may still read shared memory
   if (__syncthreads_or(bad) && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
   if (warp == 0) tmem_dealloc(tmem, L::kCols);
 }
-
 
 // ---------------------------------------------------------------------------
 struct PbPlan {
@@ -824,8 +903,8 @@ static int launch_path_bwd(PathBwdArgs a, const PbPlan& x, int sms, cudaStream_t
     a.runs = (int)(runs - r < x.group ? runs - r : x.group);
     path_bwd_scan_kernel<DP><<<(unsigned)a.runs, kPsThreads, PbScan<DP>::kSmem, s>>>(a);
     if (int st = launch_status()) return st;
-    const long long units = (long long)a.runs * kPbRun, most = (long long)sms * L::kMinBlocks;
-    path_bwd_kernel<DP><<<(unsigned)(units < most ? units : most), L::kThreads, L::kAlloc, s>>>(a, vec4);
+    const long long passes = (long long)a.runs * (kPbRun / L::PP), most = (long long)sms * L::kMinBlocks;
+    path_bwd_kernel<DP><<<(unsigned)(passes < most ? passes : most), L::NT, L::kAlloc, s>>>(a, vec4);
     if (int st = launch_status()) return st;
   }
   return HOA_OK;
