@@ -121,7 +121,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
     __syncwarp();
   } else if (warp == 8) {
     // ------------------------------------------------------------------ MMA
-    if (lid == 0 && n > 0) {
+    if (n > 0 && elect_one()) {
       constexpr uint32_t idS = make_idesc(kFmtBF16, 128, kBwStr), idA = make_idesc(kFmtBF16, 128, DP, true);
       const uint64_t dX0 = desc_sw128(smem_u32(sm)), dX1 = desc_sw128(smem_u32(sm + L::kOwn));
       bool ok = mbar_wait_abortable(own_full, 0, s_abort, p.max_wait);

@@ -133,6 +133,18 @@ HOA_DEVICE void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// One lane of a converged warp, the same one each time.  (The products of a branch on it take their descriptors from uniform
+// registers; behind a branch on the lane number each one moves them there first.)
+HOA_DEVICE bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ---- tcgen05 -----------------------------------------------------------------
 HOA_DEVICE void tmem_alloc(uint32_t* slot, uint32_t ncols) {   // one full warp
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
