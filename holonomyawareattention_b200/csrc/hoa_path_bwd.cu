@@ -287,7 +287,7 @@ template <int DP> struct PbLayout {
   static constexpr int offVec = kMats;                             // dq^, dk^, dv^ in the chunk's frame
   static constexpr int offPart = offVec + PP * 3 * DP * 4;
   static constexpr int offRed = offPart + 3 * NT * 4;
-  static constexpr int offPos = offRed + 2 * 16 * 4;               // of each position: top, norm bound, terms
+  static constexpr int offPos = offRed + 2 * 32 * 4;               // of each position: top, norm bound, terms
   static constexpr int offCoef = offPos + 4 * 4 * 4;
   static constexpr int offBar = offCoef + PP * kPbCoef * 4;
   static constexpr int kAlloc = offBar + 64 + 1024;
@@ -296,7 +296,7 @@ template <int DP> struct PbLayout {
   static constexpr uint32_t colD = 0, colHi = ND, colLo = ND + DP / 2;
   static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2 + NT - 1) / NT;
   static constexpr int kScratch = 2 * NCG * 4 * NT;                // float4s of a CTA's old iterates
-  static_assert(kPbRun % PP == 0, "a pass stays in its run");
+  static_assert(NT <= 1024 && kPbRun % PP == 0, "a pass stays in its run");
 };
 
 // gamma_k (k >= 0) for x, and how many terms they need
@@ -339,7 +339,7 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
   float* T = reinterpret_cast<float*>(sm);
   float* vec = reinterpret_cast<float*>(sm + L::offVec);
   float* part = reinterpret_cast<float*>(sm + L::offPart);
-  float* red = reinterpret_cast<float*>(sm + L::offRed);           // [2][16]
+  float* red = reinterpret_cast<float*>(sm + L::offRed);           // [2][32]
   unsigned* s_top = reinterpret_cast<unsigned*>(sm + L::offPos);   // [4] the largest |Y|, as bits
   float* s_x = reinterpret_cast<float*>(sm + L::offPos) + 4;       // [4] x
   int* s_terms = reinterpret_cast<int*>(sm + L::offPos) + 8;       // [4] Chebyshev: products
@@ -474,7 +474,7 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
   const uint64_t vN[2] = {desc_sw128_mn(base + L::offV, L::kSlabV), desc_sw128_mn(base + L::offV + L::kMatV, L::kSlabV)};
   constexpr uint32_t idN = make_idesc(0, 128, L::ND, true), idK = make_idesc(0, 128, L::ND, false);
   auto issue = [&](bool left_R, bool right_R) {
-    if (tid != 0 || bad) return;
+    if (warp != 0 || !elect_one() || bad) return;
     tc_fence_after();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
@@ -658,12 +658,15 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
         const int c = group + ci * G;
         if (!works || c >= L::NC) continue;
         float v[16];
-        F2 x[8];
         load_D(c, v);
         mask_row(c, 1.f / kPbR, v, M[ci]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sw = f2_fma(M[ci][e], M[ci][e], sw);
         put_right(c, M[ci]);
+      }
+#pragma unroll 1
+      for (int c = works ? group : L::NC; c < L::NC; c += G) {
+        F2 x[8];
         int at = row;
         asm volatile("" : "+r"(at));                                // (its index math stays here: no registers across the products)
         gen_row16(gen + mine * p.stride, p.banked != 0, p.stride, d, at, lid, 16 * c, p.edge_scale * kPbA, x);
@@ -710,11 +713,18 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
 #pragma unroll
     for (int w = 0; w < PP; ++w) wq[w] = sum_of(red, w);
     for (int k = 1;; ++k) {
-      wait();
+      // (while the product runs) the norm above which another term is needed, of each position; Chebyshev: a number of terms
+      float need[PP];
+      if (k > 1) {
 #pragma unroll
-      for (int ci = 0; ci < NCG; ++ci) {
-        const int c = group + ci * G;
-        if (!works || c >= L::NC) continue;
+        for (int w = 0; w < PP; ++w) {
+          const float rr = s_x[w] / (float)(k + 2), left = rr / (1.f - rr);
+          need[w] = s_terms[w] > 0 ? (k < s_terms[w] ? -1.f : INFINITY) : k >= 64 ? INFINITY : rr >= 1.f ? -1.f : 5.7e-14f * wq[w] / (left * left);
+        }
+      }
+      wait();
+#pragma unroll 1
+      for (int c = works ? group : L::NC; c < L::NC; c += G) {
         float v[16];
         load_D(c, v);
         if (row < d)
@@ -774,57 +784,71 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
       }
       {
         const float2 v = f2_get(vv);
-        const float tv = warp_sum(v.x + v.y);
-        if (lid == 0) red[(k & 1) * 16 + warp] = tv;
+        const float sum = warp_sum(v.x + v.y);
+        if (lid == 0) red[(k & 1) * 32 + warp] = sum;
       }
       publish();
       __syncthreads();
-      bool more = false;
+      bool more = k == 1;                                           // (the first check comes with the second term)
+      if (k > 1)
 #pragma unroll
-      for (int w = 0; w < PP; ++w) {
-        const int n = s_terms[w];
-        const float rr = s_x[w] / (float)(k + 2);
-        const float left = rr / (1.f - rr);
-        more |= n > 0 ? k < n : k < 64 && (rr >= 1.f || sum_of(red + (k & 1) * 16, w) * left * left > 5.7e-14f * wq[w]);
-      }
+        for (int w = 0; w < PP; ++w) more |= sum_of(red + (k & 1) * 32, w) > need[w];
       if (!more) break;
       issue(false, false);
     }
-    // ---- da: the upper triangle in the generators' layout, through shared memory
-    float* out = T + mine * p.stride;
-    if (p.banked) {
-      for (int i = tid; i < PP * p.stride; i += NT) T[i] = 0.f;
-      __syncthreads();
-    }
+    // ---- da: M by rows through shared memory, its upper triangle in the generators' layout to global memory
     {
-      const bool last = t + mine == p.T - 1;
-      const float f1 = lost ? __int_as_float(0x7fffffff) : ldexpf(1.f, -e_y), f2w = 16.f * p.edge_scale;
-      int base_r = row * (2 * d - row - 1) / 2 - row - 1;
-      asm volatile("" : "+r"(base_r));
+      const float f = lost ? __int_as_float(0x7fffffff) : ldexpf(1.f, -e_y), es = 16.f * p.edge_scale;
 #pragma unroll
       for (int ci = 0; ci < NCG; ++ci) {
         const int c = group + ci * G;
-        if (!works || c >= L::NC || row >= d || 16 * c + 15 <= row0) continue;
-        int n = d - 16 * c, k0 = row - 16 * c, at = row;             // columns k0 < e < n of the chunk
-        asm volatile("" : "+r"(n), "+r"(k0), "+r"(at));
-        float* o = out + base_r + 16 * c;
+        if (!works || c >= L::NC || row >= d) continue;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float2 m = f2_get(M[ci][e / 2]);
-          const float v = last ? 0.f : (e & 1 ? m.y : m.x) * f2w * f1;
-          if (e > k0 && e < n) {
-            if (p.banked) out[gen_banked_slot(at, 16 * c + e, d)] = v;
-            else o[e] = v;
-          }
+        for (int q = 0; q < 4; ++q) {
+          const float2 lo = f2_get(f2_mul(M[ci][2 * q], f2(es))), hi = f2_get(f2_mul(M[ci][2 * q + 1], f2(es)));
+          *reinterpret_cast<float4*>(T + lrow * L::kLdT + 16 * c + 4 * q) = make_float4(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
         }
       }
     }
     if (__syncthreads_or(bad)) break;
-#pragma unroll
-    for (int w = 0; w < PP; ++w) {
-      if (w >= live) break;
+#pragma unroll 1
+    for (int w = 0; w < live; ++w) {
       float* dg = p.da + (pos + (long long)w * p.H) * p.stride;
-      for (int i = tid; i < p.stride; i += NT) dg[i] = T[w * p.stride + i];
+      const float* Tw = T + w * RS * L::kLdT;
+      if (t + w == p.T - 1) {                                       // the closing edge
+        for (int i = tid; i < p.stride; i += NT) dg[i] = 0.f;
+      } else if (p.banked) {
+        // gen_banked_slot's lines of 32 slots: those of a pair of blocks, then 16 a diagonal block
+        const int nb = d >> 5, off = nb * (nb - 1) / 2 * 32;
+#pragma unroll 1
+        for (int line = warp; line < off + 16 * nb; line += NW) {
+          float v;
+          if (line < off) {
+            int pair = line >> 5, a = 0;
+            while (pair >= nb - 1 - a) pair -= nb - 1 - a++;
+            const int u0 = line & 31;
+            v = Tw[(32 * a + u0) * L::kLdT + 32 * (a + 1 + pair) + (lid ^ (4 * (u0 & 7)))];
+          } else {
+            // slot (k, s): offsets u + v = s mod 32 with w = u - ceil(s / 2) = k + 1 - s mod 2; the one with u = v is unused
+            const int o = (line - off) >> 4, k = (line - off) & 15, e = lid & 1;
+            const int u0 = (k + 1 - e + ((lid + 1) >> 1)) & 31, v0 = (lid - u0) & 31;
+            v = u0 == v0 ? 0.f : Tw[(32 * o + min(u0, v0)) * L::kLdT + 32 * o + max(u0, v0)];
+          }
+          dg[line * 32 + lid] = v;
+        }
+      } else {
+        constexpr int NJ = (DP + 31) / 32;
+#pragma unroll 2
+        for (int i = warp; i < d - 1; i += NW) {
+          float* o = dg + i * (2 * d - i - 1) / 2 - i - 1;
+          float m[NJ];
+#pragma unroll
+          for (int k = 0; k < NJ; ++k) m[k] = Tw[i * L::kLdT + min(lid + 32 * k, DP - 1)];
+#pragma unroll
+          for (int k = 0; k < NJ; ++k)
+            if (lid + 32 * k > i && lid + 32 * k < d) o[lid + 32 * k] = m[k];
+        }
+      }
     }
     __syncthreads();                                                // the next pass writes R there
   }
