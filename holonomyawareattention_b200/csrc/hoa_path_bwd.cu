@@ -38,6 +38,7 @@ struct PathBwdArgs {
   float* Y; float* F;                                          // of a group of runs: (runs, kPbRun, d, d), (runs, kPbRun, 3, d)
   float4* V;                                                   // two old iterates a CTA (main, large norms)
   long long run0; int runs;                                    // the group
+  int vec4;                                                    // rows of R, Y and the vectors from 16-byte (bf16: 8-byte) boundaries
   int* status;
   long long max_wait;
 };
@@ -60,64 +61,101 @@ constexpr int kPsThreads = 256;
 // w = 0..3 q^, k^, v^, do^ and w = 4..7 dq^, dk^, dv^, o.  Rows past the n-th position are zero.
 template <int DP>
 HOA_DEVICE void pb_vectors(const PathBwdArgs& p, int chain, int t, int n, float* X, int ld) {
-  for (int i = threadIdx.x; i < 64 * DP; i += kPsThreads) {
-    const int row = i / DP, e = i % DP, w = row & 7;
-    float v = 0.f;
-    if ((row >> 3) < n && e < p.d) {
-      const long long at = ((long long)chain * p.T + t + (row >> 3)) * p.d + e;
-      v = w == 7 ? p.o[at] : load_elem(w < 3 ? p.x[w] : w == 3 ? p.y[3] : p.y[w - 4], at, p.dtype);
+  static_assert(kPsThreads == 256, "a warp a vector");
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31, d = p.d;
+  const void* src = w == 7 ? (const void*)p.o : w < 3 ? p.x[w] : w == 3 ? p.y[3] : p.y[w - 4];
+  const bool f32 = w == 7 || p.dtype == HOA_F32;
+  const long long at = ((long long)chain * p.T + t) * d;
+  float* out = X + w * ld;
+  if (p.vec4) {
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i >= n || 4 * l >= d) continue;
+      if (f32) {
+        v[i] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(src) + at + i * d + 4 * l);
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(src) + at + i * d + 4 * l);
+        v[i] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                           __uint_as_float(u.y & 0xffff0000u));
+      }
     }
-    X[row * ld + e] = v;
+    if (4 * l < DP)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(out + 8 * i * ld + 4 * l) = v[i];
+  } else {
+#pragma unroll
+    for (int e = l; e < DP; e += 32)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        out[8 * i * ld + e] = i < n && e < d ? load_elem(src, at + i * d + e, f32 ? HOA_F32 : HOA_BF16) : 0.f;
   }
 }
 
-// Y += skew of position i's vectors (rows 8 i .. of X): thread (ty, tx) owns rows ty + 16 a, columns tx + 16 b
+// A d x d matrix over the CTA's 8 warps: warp w has rows w DP / 8 + i, lane l columns l + 32 b, rows in pairs.
+template <int DP> struct PbTile {
+  static constexpr int NR = DP / 8, NB = (DP + 31) / 32;
+  F2 v[NR / 2][NB];
+};
+
+// Y += skew of position i's vectors (rows 8 i .. of X)
 template <int DP>
-HOA_DEVICE void pb_add(const float* X, int ld, int i, int ty, int tx, float (&Y)[DP / 16][DP / 16]) {
-  constexpr int N = DP / 16;
+HOA_DEVICE void pb_add(const float* X, int ld, int i, PbTile<DP>& Y) {
+  using T = PbTile<DP>;
+  const int r0 = (threadIdx.x >> 5) * T::NR, l = threadIdx.x & 31;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     const float* x = X + (8 * i + w) * ld;
     const float* y = x + 4 * ld;
-    float xr[N], yr[N], xc[N], yc[N];
+    F2 xc[T::NB], yc[T::NB];
 #pragma unroll
-    for (int a = 0; a < N; ++a) {
-      xr[a] = x[ty + 16 * a];
-      yr[a] = y[ty + 16 * a];
-      xc[a] = x[tx + 16 * a];
-      yc[a] = y[tx + 16 * a];
+    for (int b = 0; b < T::NB; ++b) {
+      const int c = min(l + 32 * b, DP - 1);
+      xc[b] = f2(-x[c]);
+      yc[b] = f2(y[c]);
     }
 #pragma unroll
-    for (int a = 0; a < N; ++a)
+    for (int a = 0; a < T::NR / 2; ++a) {
+      const float2 xr = *reinterpret_cast<const float2*>(x + r0 + 2 * a), yr = *reinterpret_cast<const float2*>(y + r0 + 2 * a);
 #pragma unroll
-      for (int b = 0; b < N; ++b) Y[a][b] = fmaf(xr[a], yc[b], fmaf(-yr[a], xc[b], Y[a][b]));
+      for (int b = 0; b < T::NB; ++b) Y.v[a][b] = f2_fma(f2(xr.x, xr.y), yc[b], f2_fma(f2(yr.x, yr.y), xc[b], Y.v[a][b]));
+    }
   }
 }
 
 template <int DP>
+HOA_DEVICE void pb_store(const PbTile<DP>& Y, float* out, int d) {
+  using T = PbTile<DP>;
+  const int r0 = (threadIdx.x >> 5) * T::NR, l = threadIdx.x & 31;
+#pragma unroll
+  for (int a = 0; a < T::NR / 2; ++a)
+#pragma unroll
+    for (int b = 0; b < T::NB; ++b) {
+      const float2 v = f2_get(Y.v[a][b]);
+      const int r = r0 + 2 * a, c = l + 32 * b;
+      if (c < d && r < d) out[r * d + c] = v.x;
+      if (c < d && r + 1 < d) out[(r + 1) * d + c] = v.y;
+    }
+}
+
+template <int DP>
 __global__ void __launch_bounds__(kPsThreads) path_bwd_sums_kernel(const __grid_constant__ PathBwdArgs p) {
-  constexpr int N = DP / 16;
   __shared__ __align__(16) float X[64 * DP];
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
   const PbRun r = pb_run(p, blockIdx.x);
-  float Y[N][N];
+  PbTile<DP> Y;
 #pragma unroll
-  for (int a = 0; a < N; ++a)
+  for (int a = 0; a < PbTile<DP>::NR / 2; ++a)
 #pragma unroll
-    for (int b = 0; b < N; ++b) Y[a][b] = 0.f;
+    for (int b = 0; b < PbTile<DP>::NB; ++b) Y.v[a][b] = f2(0.f);
   for (int t = r.t0; t < r.t1; t += 8) {
     const int n = min(8, r.t1 - t);
     __syncthreads();
     pb_vectors<DP>(p, r.chain, t, n, X, DP);
     __syncthreads();
-    for (int i = 0; i < n; ++i) pb_add<DP>(X, DP, i, ty, tx, Y);
+    for (int i = 0; i < n; ++i) pb_add<DP>(X, DP, i, Y);
   }
-  float* S = p.S + (long long)blockIdx.x * p.d * p.d;
-#pragma unroll
-  for (int a = 0; a < N; ++a)
-#pragma unroll
-    for (int b = 0; b < N; ++b)
-      if (ty + 16 * a < p.d && tx + 16 * b < p.d) S[(ty + 16 * a) * p.d + tx + 16 * b] = Y[a][b];
+  pb_store<DP>(Y, p.S + (long long)blockIdx.x * p.d * p.d, p.d);
 }
 
 // S_r <- sum of S_{r'} over the chain's later runs r' > r
@@ -129,12 +167,12 @@ __global__ void __launch_bounds__(256) path_bwd_suffix_kernel(const __grid_const
   float* s = p.S + chain * p.NR * dd + (i - chain * dd);
   double acc = 0.0;
   int r = p.NR - 1;
-  for (; r >= 3; r -= 4) {
-    float v[4];
+  for (; r >= 15; r -= 16) {
+    float v[16];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = s[(r - k) * dd];
+    for (int k = 0; k < 16; ++k) v[k] = s[(r - k) * dd];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 16; ++k) {
       s[(r - k) * dd] = (float)acc;
       acc += v[k];
     }
@@ -151,14 +189,16 @@ template <int DP> struct PbScan {
   static constexpr size_t kSmem = (size_t)(2 * DP + 64) * kLd * sizeof(float);
 };
 
-// acc[a][b] (+)= X[ty + 16 a] . Y[tx + 16 b] over DP columns
-template <int DP, int NA, int NB>
-HOA_DEVICE void pb_nt(const float* X, const float* Y, int ty, int tx, float (&acc)[NA][NB]) {
-  constexpr int kLd = PbScan<DP>::kLd;
+// out[ty + 16 a][tx + 16 b] = X[ty + 16 a] . Y[tx + 16 b] over DP columns, rows of kLd floats, once all have read X and Y
+template <int DP, int NA>
+HOA_DEVICE void pb_nt(const float* X, const float* Y, float* out) {
+  constexpr int kLd = PbScan<DP>::kLd, NB = DP / 16;
+  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
+  F2 acc[NA][NB];
 #pragma unroll
   for (int a = 0; a < NA; ++a)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[a][b] = 0.f;
+    for (int b = 0; b < NB; ++b) acc[a][b] = f2(0.f);
 #pragma unroll 1
   for (int e = 0; e < DP; e += 4) {
     float4 x[NA];
@@ -168,24 +208,29 @@ HOA_DEVICE void pb_nt(const float* X, const float* Y, int ty, int tx, float (&ac
     for (int b = 0; b < NB; ++b) {
       const float4 y = *reinterpret_cast<const float4*>(Y + (tx + 16 * b) * kLd + e);
 #pragma unroll
-      for (int a = 0; a < NA; ++a) {
-        acc[a][b] = fmaf(x[a].x, y.x, acc[a][b]);
-        acc[a][b] = fmaf(x[a].y, y.y, acc[a][b]);
-        acc[a][b] = fmaf(x[a].z, y.z, acc[a][b]);
-        acc[a][b] = fmaf(x[a].w, y.w, acc[a][b]);
-      }
+      for (int a = 0; a < NA; ++a)                                 // (even and odd columns in the two halves)
+        acc[a][b] = f2_fma(f2(x[a].x, x[a].y), f2(y.x, y.y), f2_fma(f2(x[a].z, x[a].w), f2(y.z, y.w), acc[a][b]));
     }
   }
+  __syncthreads();
+#pragma unroll
+  for (int a = 0; a < NA; ++a)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float2 v = f2_get(acc[a][b]);
+      out[(ty + 16 * a) * kLd + tx + 16 * b] = v.x + v.y;
+    }
+  __syncthreads();
 }
 
 template <int DP>
 __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_constant__ PathBwdArgs p) {
-  constexpr int N = DP / 16, kLd = PbScan<DP>::kLd;
+  constexpr int kLd = PbScan<DP>::kLd;
   extern __shared__ __align__(16) float smem[];
   float* C = smem;
   float* Z = C + DP * kLd;
   float* X = Z + DP * kLd;
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, d = p.d;
+  const int tid = threadIdx.x, d = p.d;
   const long long run = p.run0 + blockIdx.x;
   const PbRun r = pb_run(p, run);
   if (r.t0 >= r.t1) return;
@@ -195,44 +240,37 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_
     const int a = i / DP, b = i % DP;
     const bool in = a < d && b < d;
     C[a * kLd + b] = in ? Cg[a * d + b] : 0.f;
-    Z[b * kLd + a] = in ? Zg[a * d + b] : 0.f;             // transposed: Z^T = -Z
+    Z[a * kLd + b] = in ? -Zg[a * d + b] : 0.f;            // Z^T = -Z
   }
   __syncthreads();
-  float Y[N][N];
-  pb_nt<DP, N, N>(C, Z, ty, tx, Y);                        // C Z
-  __syncthreads();
+  pb_nt<DP, DP / 16>(C, Z, Z);                             // C Z
+  pb_nt<DP, DP / 16>(Z, C, Z);                             // (C Z) C^T
+  PbTile<DP> Y;
+  {
+    using T = PbTile<DP>;
+    const int r0 = (tid >> 5) * T::NR, l = tid & 31;
 #pragma unroll
-  for (int a = 0; a < N; ++a)
+    for (int a = 0; a < T::NR / 2; ++a)
 #pragma unroll
-    for (int b = 0; b < N; ++b) Z[(ty + 16 * a) * kLd + tx + 16 * b] = Y[a][b];
-  __syncthreads();
-  pb_nt<DP, N, N>(Z, C, ty, tx, Y);                        // (C Z) C^T
+      for (int b = 0; b < T::NB; ++b) {
+        const int c = min(l + 32 * b, DP - 1);
+        Y.v[a][b] = f2(Z[(r0 + 2 * a) * kLd + c], Z[(r0 + 2 * a + 1) * kLd + c]);
+      }
+  }
   for (int tb = r.t0 + (r.t1 - r.t0 - 1) / 8 * 8; tb >= r.t0; tb -= 8) {
     const int n = min(8, r.t1 - tb);
     __syncthreads();
     pb_vectors<DP>(p, r.chain, tb, n, X, kLd);
     __syncthreads();
-    float f[4][N];
-    pb_nt<DP, 4, N>(X, C, ty, tx, f);                      // the vectors in the chunk's frame
-    __syncthreads();
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int b = 0; b < N; ++b) X[(ty + 16 * a) * kLd + tx + 16 * b] = f[a][b];
-    __syncthreads();
+    pb_nt<DP, 4>(X, C, X);                                 // the vectors in the chunk's frame
     float* F = p.F + ((long long)blockIdx.x * kPbRun + (tb - r.t0)) * 3 * d;
     for (int i = tid; i < n * 3 * d; i += kPsThreads) {
       const int e = i % d, w = i / d % 3, j = i / (3 * d);
       F[i] = X[(8 * j + 4 + w) * kLd + e];
     }
     for (int i = n - 1; i >= 0; --i) {
-      float* Yg = p.Y + ((long long)blockIdx.x * kPbRun + (tb + i - r.t0)) * d * d;
-#pragma unroll
-      for (int a = 0; a < N; ++a)
-#pragma unroll
-        for (int b = 0; b < N; ++b)
-          if (ty + 16 * a < d && tx + 16 * b < d) Yg[(ty + 16 * a) * d + tx + 16 * b] = Y[a][b];
-      pb_add<DP>(X, kLd, i, ty, tx, Y);
+      pb_store<DP>(Y, p.Y + ((long long)blockIdx.x * kPbRun + (tb + i - r.t0)) * d * d, d);
+      pb_add<DP>(X, kLd, i, Y);
     }
   }
 }
@@ -330,7 +368,7 @@ HOA_DEVICE int pb_chebyshev(double x, float* coef) {
 
 template <int DP>
 __global__ void __launch_bounds__(PbLayout<DP>::NT, PbLayout<DP>::kMinBlocks)
-path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
+path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
   using L = PbLayout<DP>;
   constexpr int G = L::G, NT = L::NT, NCG = L::NCG, PP = L::PP, RS = L::RS, NW = NT / 32;
   extern __shared__ uint8_t smem_raw[];
@@ -384,7 +422,7 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p, bool vec4) {
       pv[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r0 >= RG || w >= live || r >= d || pc >= d) continue;
       const float* at = m + (w * d + r) * d + pc;
-      if (vec4) {
+      if (p.vec4) {
         pv[k] = *reinterpret_cast<const float4*>(at);
       } else {
         pv[k].x = at[0];
@@ -917,7 +955,6 @@ static int launch_path_bwd(PathBwdArgs a, const PbPlan& x, int sms, cudaStream_t
     return HOA_ERR_LAUNCH;
   const long long runs = (long long)a.B * a.H * x.NR, entries = (long long)a.B * a.H * a.d * a.d;
   if ((entries + 255) / 256 > 0x7fffffff) return HOA_ERR_UNSUPPORTED;
-  const bool vec4 = a.d % 4 == 0 && (reinterpret_cast<uintptr_t>(a.R) & 15) == 0;
   path_bwd_sums_kernel<DP><<<(unsigned)runs, kPsThreads, 0, s>>>(a);
   if (int st = launch_status()) return st;
   path_bwd_suffix_kernel<<<(unsigned)((entries + 255) / 256), 256, 0, s>>>(a, entries);
@@ -928,7 +965,7 @@ static int launch_path_bwd(PathBwdArgs a, const PbPlan& x, int sms, cudaStream_t
     path_bwd_scan_kernel<DP><<<(unsigned)a.runs, kPsThreads, PbScan<DP>::kSmem, s>>>(a);
     if (int st = launch_status()) return st;
     const long long passes = (long long)a.runs * (kPbRun / L::PP), most = (long long)sms * L::kMinBlocks;
-    path_bwd_kernel<DP><<<(unsigned)(passes < most ? passes : most), L::NT, L::kAlloc, s>>>(a, vec4);
+    path_bwd_kernel<DP><<<(unsigned)(passes < most ? passes : most), L::NT, L::kAlloc, s>>>(a);
     if (int st = launch_status()) return st;
   }
   return HOA_OK;
@@ -959,10 +996,13 @@ extern "C" int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias
   if (!pb_plan(B, H, T, d, chunk, sms, x)) return HOA_ERR_UNSUPPORTED;
   if (workspace_bytes < x.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return HOA_ERR_WORKSPACE;
   unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
+  uintptr_t at = reinterpret_cast<uintptr_t>(R);
+  for (const void* v : {qh, kh, vh, (const void*)o, dqh, dkh, dvh, doh}) at |= reinterpret_cast<uintptr_t>(v);
+  const int vec4 = d % 4 == 0 && (at & 15) == 0;
   PathBwdArgs p{a_all, gen_is_banked(a_dtype) ? 1 : 0, stride, a_bias, edge_scale, R, C, chunk, x.K, x.rpc, x.NR,
                 {qh, kh, vh}, o, {dqh, dkh, dvh, doh}, hat_dtype, da, dqkv, out_dtype, B, H, T, d,
                 reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + x.off_Y), reinterpret_cast<float*>(ws + x.off_F),
-                reinterpret_cast<float4*>(ws + x.off_V), 0, 0, status, wait_bound_cycles()};
+                reinterpret_cast<float4*>(ws + x.off_V), 0, 0, vec4, status, wait_bound_cycles()};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch ((d + 15) / 16) {
     case 1: return launch_path_bwd<16>(p, x, sms, s);
