@@ -17,9 +17,11 @@ core/attention_fast_chunked.py:175-177 does.  Dropout must be inactive and the
 input on CUDA; anything else raises NotImplementedError: there is no CPU or
 PyTorch fallback.
 
-Forward only.  The projections (qkv, edge_mlp, out) run as PyTorch GEMMs;
-everything between them — link rotations, prefix composition, transport,
-causal attention and the inverse transport — runs in libhoa.
+The projections (qkv, edge_mlp, out) run as PyTorch GEMMs; everything between
+them — link rotations, prefix composition, transport, causal attention and the
+inverse transport — runs in libhoa.  Under autograd the causal forward with
+attn_mask tril(L) is differentiable (training.py): gradients of x and of every
+parameter, the backward passes in libhoa too.
 """
 from __future__ import annotations
 
@@ -30,7 +32,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import ops, training
 
 
 def _is_exact_tril(mask: Optional[torch.Tensor], L: int) -> bool:
@@ -111,13 +113,16 @@ class PathOrderedGeometricMHA(nn.Module):
             why = "dropout must be 0 or the module in eval mode"
         elif x.dim() != 3 or x.shape[-1] != self.h * self.d:
             why = f"x must be (B, L, {self.h * self.d})"
-        elif torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
-            why = "forward-only kernels: call under torch.no_grad() / torch.inference_mode()"
+        elif self._needs_grad(x) and (return_geometry or self.mode != "causal"):
+            why = "gradients need mode 'causal' and no geometry: call under torch.no_grad() / torch.inference_mode()"
         elif attn_mask is not None and (tuple(attn_mask.shape) != (x.shape[1], x.shape[1])
                                         or attn_mask.dtype != torch.bool):
             why = "attn_mask must be None or an (L, L) bool tensor (True = allowed)"
         if why is not None:
             raise NotImplementedError(f"PathOrderedGeometricMHA (B200): {why}")
+
+    def _needs_grad(self, x: torch.Tensor) -> bool:
+        return torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
 
     def _mask_is_tril(self, mask, L: int) -> bool:
         if mask is None:
@@ -198,13 +203,23 @@ class PathOrderedGeometricMHA(nn.Module):
             return F.linear(self.edge_mlp[1](lin0(pair)), w2, b2), None, layout
         if x.dtype != torch.bfloat16:
             raise NotImplementedError(f"dtype {x.dtype} is not supported (float32 or bfloat16)")
-        mode = self._generator_mode(seq_len if seq_len is not None else
-                                    (L if x_next is None else None))
         p2 = pair.reshape(B * L, 2 * D)
         w1t, b1 = self._w1t()
         h = ops.edge_gemm(p2, w1t, b1)            # fp32 out, the bias added in the epilogue
-        if mode == "split8" and not self._fp8_shape_ok(B * L, h.shape[1]):
-            mode = "split"                        # shapes the fp8 GEMM does not take
+        mode = self._precision_for(seq_len if seq_len is not None else (L if x_next is None else None), B * L, h.shape[1])
+        hidden = [h]
+        del h                                     # (the callee frees it once it has been split)
+        return self._generators_of_hidden(hidden.pop(), mode).view(B, L, -1), None, layout
+
+    def _precision_for(self, seq_len: Optional[int], rows: int, hidden: int) -> str:
+        """The form of the bf16 edge MLP's second layer for this many rows of a sequence of seq_len positions."""
+        mode = self._generator_mode(seq_len)
+        if mode == "split8" and not self._fp8_shape_ok(rows, hidden):
+            return "split"                        # shapes the fp8 GEMM does not take
+        return mode
+
+    def _generators_of_hidden(self, h: torch.Tensor, mode: str) -> torch.Tensor:
+        """GELU and the bf16 edge MLP's second layer: h (rows, 4D) fp32 -> (rows, H*width) fp32, in the form ``mode``."""
         if mode == "split8":
             # W2 g_hi in bf16 (the bias in the epilogue), then += W2 g_lo with both operands in
             # e4m3 (hoa_edge_gelu_split8, hoa_edge_gemm_fp8_acc)
@@ -215,7 +230,7 @@ class PathOrderedGeometricMHA(nn.Module):
             del hi
             w8, alpha = self._w2_fp8()
             ops.edge_gemm_fp8_acc(lo, w8, a, alpha)
-            return a.view(B, L, -1), None, layout
+            return a
         split = mode != "bf16"
         # GEMM operand [g_hi | g_lo] ("bf16": g_hi), g = GELU(h), in one pass (hoa_edge_gelu_split),
         # against [W2^T ; W2^T] (W2^T): W2 g_hi + W2 g_lo in fp32, the bias added in the GEMM's
@@ -223,8 +238,7 @@ class PathOrderedGeometricMHA(nn.Module):
         lhs = ops.edge_gelu_split(h, split)
         del h
         wt, bias = self._stacked_w2t(split)
-        a = ops.edge_gemm(lhs, wt, bias)
-        return a.view(B, L, -1), None, layout
+        return ops.edge_gemm(lhs, wt, bias)
 
     # sequences longer than this use the split generators under "auto"
     AUTO_SPLIT_ABOVE = 8192
@@ -323,6 +337,13 @@ class PathOrderedGeometricMHA(nn.Module):
         # any other mask, the inert ablation) takes the general fp32 path
         general = not (self.mode == "causal" and self._mask_is_tril(attn_mask, L))
         mask = attn_mask.to(x.device) if (general and attn_mask is not None) else None
+        if self._needs_grad(x):
+            if general:
+                raise NotImplementedError("PathOrderedGeometricMHA (B200): gradients need attn_mask = tril(L)")
+            if torch.cuda.is_current_stream_capturing():
+                raise NotImplementedError("PathOrderedGeometricMHA (B200): a forward that needs gradients cannot be captured")
+            pieces = [training.forward_rows(self, x[b0:b0 + rows]) for b0 in range(0, B, rows)]
+            return (pieces[0] if len(pieces) == 1 else torch.cat(pieces)), None
         if return_geometry:
             # {"C": P (B,H,L,d,d), "H": Hol (B,H,d,d)} in x's dtype, as
             # core/attention_fast_chunked.py:175-177 returns them

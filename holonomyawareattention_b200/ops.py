@@ -1208,3 +1208,5 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
                   g_code, _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None,
                   32 if scales is None else 8, _longs(*(p.numel() for p in params)), n, step.data_ptr(), lr, betas[0], betas[1], eps,
                   weight_decay, torch._C._cuda_getCurrentRawStream(idx))
+    # written behind autograd's back: what was saved of them, or laid out from them, is out of date
+    torch.autograd.graph.increment_version([t for t in (*params, *(masters or ())) if not t.is_inference()])

@@ -1,0 +1,237 @@
+"""Training of PathOrderedGeometricMHA: the module's forward under autograd, AdamW, one training step.
+
+The reference trains its module with autograd (core/attention_fast_chunked.py:98-177 is differentiable; its kernel
+drop-in recomputes the forward in the backward pass, kernel/attention_kernel.py:166-187).  Here the core region
+between the projections is one autograd node: link rotations, carries, transports and attention forward, and
+attn_bwd and path_bwd backward.  The projections are differentiated as the linears they are.
+
+    attn = PathOrderedGeometricMHA(d_model, n_heads=H, edge_scale=0.05).cuda()
+    opt = AdamW(attn.parameters(), lr=3e-4, state_bits=8)
+    loss = train_step(attn, x, opt, lambda y: ((y - target) ** 2).mean())      # causal, tril mask
+
+or, with any loss around it, `y, _ = attn(x, attn_mask=tril)`, `loss.backward()`, `opt.step()`.
+"""
+from __future__ import annotations
+
+from typing import Callable, Optional
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+class PathCore(torch.autograd.Function):
+    """heads (B,T,D) = core region of (a_all (B,T,H*stride) fp32, qkv (B,T,3D)); a_bias: one generator row or None."""
+
+    @staticmethod
+    def forward(ctx, a_all, qkv, a_bias, n_heads, edge_scale, scale, chunk, layout):
+        B, T, threeD = qkv.shape
+        a_all, qkv = a_all.contiguous(), qkv.contiguous()
+        R, U, M = ops.link_local(a_all, qkv, n_heads, edge_scale, chunk, a_bias, layout)
+        C, _ = ops.carry_scan(M)
+        del M
+        qh, kh, vh = ops.carry_apply(U, C, chunk, qkv.dtype)
+        del U
+        o, lse = ops.attn_fwd_lse(qh, kh, vh, scale)
+        ctx.save_for_backward(a_all, a_bias, R, C, qh, kh, vh, o, lse)
+        ctx.args = n_heads, edge_scale, scale, chunk, layout
+        return ops.out_transport(o, R, C, chunk, B, n_heads, qkv.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dheads):
+        a_all, a_bias, R, C, qh, kh, vh, o, lse = ctx.saved_tensors
+        H, edge_scale, scale, chunk, layout = ctx.args
+        BH, T, d = qh.shape
+        dout = dheads.reshape(BH // H, T, H, d).permute(0, 2, 1, 3).float().contiguous().view(BH, T, d)
+        doh = ops.apply_paths(dout, R, C, chunk, transpose=True).to(qh.dtype)          # P^T dout
+        dqh, dkh, dvh = ops.attn_bwd(qh, kh, vh, o, lse, doh, scale)
+        da, dqkv = ops.path_bwd(a_all, R, C, chunk, H, edge_scale, (qh, kh, vh, o), (dqh, dkh, dvh, doh), a_bias, layout)
+        db = da.sum((0, 1)) if a_bias is not None and ctx.needs_input_grad[2] else None
+        return da, dqkv, db, None, None, None, None, None
+
+
+class EdgeLayer0(torch.autograd.Function):
+    """The edge MLP's first layer in bf16, fp32 out (hoa_edge_gemm).  w1t, b1f: its weight transposed and its fp32 bias,
+    as the module keeps them."""
+
+    @staticmethod
+    def forward(ctx, pair, weight, bias, w1t, b1f):
+        ctx.save_for_backward(pair, weight)
+        return ops.edge_gemm(pair, w1t, b1f)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        pair, weight = ctx.saved_tensors
+        db = dh.sum(0).to(weight.dtype)
+        dh = dh.to(torch.bfloat16)
+        return dh @ weight if ctx.needs_input_grad[0] else None, dh.t() @ pair, db, None, None
+
+
+class EdgeLayer2(torch.autograd.Function):
+    """GELU and the edge MLP's second layer: generators (rows, width) fp32 of the hidden layer h (rows, F) fp32.
+    ``forward_`` computes them (the module's form for its generator_precision), ``wt`` (F, width) and ``index`` (the
+    place of every weight row among the generators, None: in order) say how the weight is laid out."""
+
+    @staticmethod
+    def forward(ctx, h, weight, bias, forward_, wt, index):
+        ctx.save_for_backward(h, wt, index)
+        return forward_(h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, da):
+        h, wt, index = ctx.saved_tensors
+        db = da.sum(0)
+        da = da.to(torch.bfloat16)
+        g = F.gelu(h).to(torch.bfloat16)
+        dw = da.t() @ g                                        # (width, F)
+        dg = da @ wt.t()
+        if index is not None:
+            dw, db = dw[index], db[index]
+        return torch.ops.aten.gelu_backward(dg.float(), h), dw, db.to(torch.bfloat16), None, None, None
+
+
+_INDEX = {}
+
+
+def _banked_index(d: int, h: int, device) -> torch.Tensor:
+    i = _INDEX.get((d, h, device))
+    if i is None:
+        with torch.inference_mode(False):
+            i = _INDEX[d, h, device] = ops.gen_banked_index(d, h, device)
+    return i
+
+
+def edge_generators(attn, x: torch.Tensor):
+    """(a_all (B, L, H*stride) fp32, layout) of the module's edge MLP, differentiable (attn._edge_generators_nobias)."""
+    B, L, D = x.shape
+    partner = torch.roll(x, shifts=-1, dims=1)
+    if attn.link_mode == "additive":
+        return attn.gqproj(x).float() + attn.gkproj(partner).float(), "packed"
+    pair = torch.cat([x, partner], dim=-1)
+    if x.dtype == torch.float32:
+        return attn.edge_mlp(pair), "packed"
+    layout = attn._gen_layout()
+    lin0, lin2 = attn.edge_mlp[0], attn.edge_mlp[2]
+    w1t, b1f = attn._w1t()
+    h = EdgeLayer0.apply(pair.reshape(B * L, 2 * D), lin0.weight, lin0.bias, w1t, b1f)
+    mode = attn._precision_for(L, B * L, h.shape[1])
+    wt, _ = attn._stacked_w2t(False)
+    index = _banked_index(attn.d, attn.h, x.device) if layout == "banked" else None
+    a = EdgeLayer2.apply(h, lin2.weight, lin2.bias, lambda t: attn._generators_of_hidden(t, mode), wt, index)
+    return a.view(B, L, -1), layout
+
+
+def forward_rows(attn, x: torch.Tensor) -> torch.Tensor:
+    """The module's causal forward (tril mask) of some batch rows, differentiable."""
+    B, L, _ = x.shape
+    qkv = attn.qkv(x)
+    a, layout = edge_generators(attn, x)
+    chunk = attn.chunk or ops.plan_chunk(B, attn.h, L, attn.d, x.device)
+    heads = PathCore.apply(a, qkv, None, attn.h, attn.edge_scale, attn.scale, chunk, layout)
+    return attn.out(heads)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with one launch for all tensors of a type (ops.adamw_step).
+
+    ``state_bits`` 32: fp32 moments; 8: 8-bit ones in blocks of 256 elements (2 bytes an element for both instead of 8).
+    bf16 parameters are stepped on fp32 master copies, kept in the state, unless ``masters`` is False.  The steps are
+    counted on the host: under graph capture step() raises (ops.adamw_step takes a count on the device)."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32, masters: bool = True):
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("lr, eps and weight_decay must be at least 0 and betas in [0, 1)")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters))
+
+    def _init(self, p, group):
+        s = self.state[p]
+        if s:
+            return s
+        s["step"] = 0
+        moment = torch.float32 if group["state_bits"] == 32 else torch.float8_e4m3fn
+        for k in ("exp_avg", "exp_avg_sq"):
+            s[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(moment)
+        if group["state_bits"] == 8:
+            s["scales"] = torch.zeros(2, -(-p.numel() // ops.ADAMW_BLOCK), device=p.device)
+        if p.dtype == torch.bfloat16 and group["masters"]:
+            s["master"] = p.detach().float().contiguous()
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise NotImplementedError("AdamW.step counts its steps on the host and cannot be captured: capture ops.adamw_step")
+        for group in self.param_groups:
+            calls = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if not p.is_cuda or p.grad.is_sparse or p.dtype not in (torch.float32, torch.bfloat16):
+                    raise NotImplementedError("AdamW takes dense fp32 or bf16 CUDA parameters")
+                if not p.is_contiguous():
+                    raise ValueError("parameters must be contiguous")
+                s = self._init(p, group)
+                g = p.grad.contiguous()
+                calls.setdefault((p.device, p.dtype, g.dtype, s["step"], "master" in s), []).append((p, g, s))
+            for (dev, _, _, n, masters), items in calls.items():
+                ps, gs, ss = zip(*items)
+                ops.adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
+                               torch.full((1,), n + 1, dtype=torch.int32, device=dev), lr=group["lr"], betas=group["betas"],
+                               eps=group["eps"], weight_decay=group["weight_decay"], masters=[s["master"] for s in ss] if masters else None,
+                               scales=[s["scales"] for s in ss] if group["state_bits"] == 8 else None)
+                for s in ss:
+                    s["step"] = n + 1
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        """As torch.optim.Optimizer's; the state keeps its types (the base class would make it the parameters')."""
+        super().load_state_dict(state_dict)
+        old = [i for g in state_dict["param_groups"] for i in g["params"]]
+        new = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(old, new):
+            for k, v in state_dict["state"].get(i, {}).items():
+                self.state[p][k] = v.detach().to(p.device, copy=True) if torch.is_tensor(v) else v
+
+
+_TRIL = {}
+
+
+def _tril(L: int, device) -> torch.Tensor:
+    m = _TRIL.get(device)
+    if m is None or m.shape[0] != L:
+        with torch.inference_mode(False):
+            m = _TRIL[device] = torch.ones(L, L, dtype=torch.bool, device=device).tril()
+    return m
+
+
+def train_step(attn, x: torch.Tensor, optimizer, loss: Callable[[torch.Tensor], torch.Tensor], attn_mask: Optional[torch.Tensor] = None,
+               max_grad_norm: Optional[float] = None) -> torch.Tensor:
+    """One step: y = attn(x) under the causal mask (``attn_mask``, default tril), loss(y), gradients (their norm held to
+    ``max_grad_norm``, if given), the optimizer's step.  Gradients start and end at None.  Returns the loss, detached, on the
+    device; nothing waits for the GPU."""
+    L = x.shape[1]
+    if attn_mask is None:
+        attn_mask = _tril(L, x.device)
+    optimizer.zero_grad(set_to_none=True)
+    with torch.enable_grad():
+        y, _ = attn(x, attn_mask=attn_mask)
+        value = loss(y)
+        value.backward()
+    if max_grad_norm is not None:
+        torch.nn.utils.clip_grad_norm_([p for g in optimizer.param_groups for p in g["params"] if p.grad is not None], max_grad_norm)
+    optimizer.step()
+    optimizer.zero_grad(set_to_none=True)
+    return value.detach()
