@@ -11,8 +11,9 @@
 // element with a small gradient is never divided by eps alone.  The step itself uses the
 // new moments before they are rounded to 8 bits.
 //
-// Every operation is rounded by itself (no fused multiply-add): the new moments, and so
-// the 8-bit values, are those of the same formula written in separate fp32 operations.
+// The moments' operations are rounded one by one (no fused multiply-add): the new moments, and so
+// the 8-bit values, are those of the same formula written in separate fp32 operations.  The
+// update, which nothing is kept of but its sum with x, takes fast division.
 #include <cuda_fp8.h>
 
 #include "hoa_common.cuh"
@@ -39,22 +40,27 @@ struct AwArgs {
 };
 static_assert(sizeof(AwArgs) <= 32000, "kernel parameters");
 
-HOA_DEVICE unsigned char aw_e4m3(float x) { return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
-HOA_DEVICE float aw_value(unsigned char c) {
-  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
-  return __half2float(__half(h));
+// two e4m3 bytes <-> values
+HOA_DEVICE float2 aw_values(unsigned pair) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
+  return __half22float2(__half2(h));
 }
+HOA_DEVICE unsigned aw_e4m3(float x, float y) { return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3); }
 
 // a / b rounded to nearest, b the same for many a: with y = 1 / b rounded to nearest and q = a y, q + (a - q b) y is the
 // correctly rounded quotient (Markstein, IBM J. Res. Dev. 34, 1990, theorem 8), as long as nothing leaves the normal range.
+// (Here |a| <= 448 b and 1e-12 < b < 1e12; what underflows is far below half the smallest e4m3 value and rounds to 0 anyway.)
 HOA_DEVICE float aw_div(float a, float b, float y) {
-  const float m = fabsf(a);
-  if (!(m == 0.f || (m > 1e-25f && m < 1e25f))) return __fdiv_rn(a, b);
   const float q = __fmul_rn(a, y);
   return fmaf(fmaf(-q, b, a), y, q);
 }
-// whether aw_div may be used with b
 HOA_DEVICE bool aw_div_by(float b) { return b > 1e-12f && b < 1e12f; }
+
+HOA_DEVICE float aw_sqrt(float x) {                     // to an ulp or two: for the update, not for what is kept
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // N consecutive elements from i on, in 16-byte pieces (kVec: the address is a multiple of what a piece takes), those past
 // n as 0
@@ -111,83 +117,80 @@ HOA_DEVICE void aw_store(void* x, int dtype, long long i, long long n, const flo
   }
 }
 
-// N bytes from i on
-template <bool kVec, int N>
-HOA_DEVICE void aw_load8(const void* x, long long i, long long n, unsigned char (&v)[N]) {
-  static_assert(N == 8, "one 8-byte piece");
+// 8 bytes from i on, as words
+template <bool kVec>
+HOA_DEVICE uint2 aw_load8(const void* x, long long i, long long n) {
   const unsigned char* b = reinterpret_cast<const unsigned char*>(x) + i;
-  if (kVec && i + N <= n) {
-    const uint2 t = *reinterpret_cast<const uint2*>(b);
+  if (kVec && i + 8 <= n) return *reinterpret_cast<const uint2*>(b);
+  unsigned u[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = (unsigned char)(t.x >> (8 * e));
-      v[4 + e] = (unsigned char)(t.y >> (8 * e));
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = i + e < n ? b[e] : 0;
-  }
+  for (int e = 0; e < 8; ++e)
+    if (i + e < n) u[e / 4] |= (unsigned)b[e] << (8 * (e & 3));
+  return make_uint2(u[0], u[1]);
 }
-template <bool kVec, int N>
-HOA_DEVICE void aw_store8(void* x, long long i, long long n, const unsigned char (&v)[N]) {
+template <bool kVec>
+HOA_DEVICE void aw_store8(void* x, long long i, long long n, uint2 v) {
   unsigned char* b = reinterpret_cast<unsigned char*>(x) + i;
-  if (kVec && i + N <= n) {
-    uint2 t = make_uint2(0, 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      t.x |= (uint32_t)v[e] << (8 * e);
-      t.y |= (uint32_t)v[4 + e] << (8 * e);
-    }
-    *reinterpret_cast<uint2*>(b) = t;
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (i + e < n) b[e] = v[e];
+  if (kVec && i + 8 <= n) {
+    *reinterpret_cast<uint2*>(b) = v;
+    return;
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (i + e < n) b[e] = (unsigned char)((e < 4 ? v.x : v.y) >> (8 * (e & 3)));
+}
+// e4m3 bytes of x[0..8), each times what f says
+template <class Fn>
+HOA_DEVICE uint2 aw_pack8(const float (&x)[8], Fn f) {
+  unsigned u[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    u[h] = aw_e4m3(f(x[4 * h]), f(x[4 * h + 1])) | aw_e4m3(f(x[4 * h + 2]), f(x[4 * h + 3])) << 16;
+  return make_uint2(u[0], u[1]);
 }
 
 // A warp has one block of 256 elements, a lane 8 consecutive ones of it.
 template <int kBits, bool kVec>
-HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float c2, float y2) {
+HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float y2) {
   const int lid = threadIdx.x & 31;
   const long long i = blk * kAwBlock + 8 * lid, n = t.n;
   const long long blocks = (n + kAwBlock - 1) / kAwBlock;
   float g[8], x[8], m[8], v[8];
-  unsigned char mb[8], vb[8];
+  uint2 mb = make_uint2(0, 0), vb = mb;
   float ms = 0.f, vs = 0.f;
   // all loads first
   aw_load<kVec>(t.g, a.g_dtype, i, n, g);
   if (t.master) aw_load<kVec>(t.master, HOA_F32, i, n, x);
   else aw_load<kVec>(t.p, a.p_dtype, i, n, x);
   if (kBits == 8) {
-    aw_load8<kVec>(t.m, i, n, mb);
-    aw_load8<kVec>(t.v, i, n, vb);
+    mb = aw_load8<kVec>(t.m, i, n);
+    vb = aw_load8<kVec>(t.v, i, n);
     ms = t.scales[blk];
     vs = t.scales[blocks + blk];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m[e] = __fmul_rn(aw_value(mb[e]), ms);
-      const float r = __fmul_rn(aw_value(vb[e]), vs);
-      v[e] = __fmul_rn(r, r);
+    for (int e = 0; e < 8; e += 2) {
+      const float2 mv = aw_values((e < 4 ? mb.x : mb.y) >> (8 * (e & 3)) & 0xffffu);
+      const float2 rv = aw_values((e < 4 ? vb.x : vb.y) >> (8 * (e & 3)) & 0xffffu);
+      m[e] = __fmul_rn(mv.x, ms);
+      m[e + 1] = __fmul_rn(mv.y, ms);
+      const float r0 = __fmul_rn(rv.x, vs), r1 = __fmul_rn(rv.y, vs);
+      v[e] = __fmul_rn(r0, r0);
+      v[e + 1] = __fmul_rn(r1, r1);
     }
   } else {
     aw_load<kVec>(t.m, HOA_F32, i, n, m);
     aw_load<kVec>(t.v, HOA_F32, i, n, v);
   }
-  float r[8], mtop = 0.f, rtop = 0.f;
-  bool nan_m = false, nan_r = false;
+  float r[8];
+  const bool tail = kBits == 8 && i + 8 > n;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     m[e] = __fadd_rn(__fmul_rn(m[e], a.b1), __fmul_rn(g[e], a.nb1));
     v[e] = __fadd_rn(__fmul_rn(v[e], a.b2), __fmul_rn(__fmul_rn(g[e], g[e]), a.nb2));
-    if (kBits == 8 && i + e >= n) m[e] = v[e] = 0.f;              // (a scale of NaN reaches the elements past the end too)
-    r[e] = __fsqrt_rn(v[e]);
-    const float den = __fadd_rn(aw_div(r[e], c2, y2), a.eps);
-    x[e] = __fsub_rn(__fmul_rn(x[e], a.keep), __fmul_rn(__fdiv_rn(m[e], den), lr));
-    mtop = fmaxf(mtop, fabsf(m[e]));
-    rtop = fmaxf(rtop, r[e]);
-    nan_m |= m[e] != m[e];
-    nan_r |= r[e] != r[e];
+    if (tail && i + e >= n) m[e] = v[e] = 0.f;                    // (a scale of NaN reaches the elements past the end too)
+    r[e] = kBits == 8 ? __fsqrt_rn(v[e]) : aw_sqrt(v[e]);
+    const float den = fmaf(r[e], y2, a.eps);
+    x[e] = fmaf(x[e], a.keep, -lr * __fdividef(m[e], den));
   }
   if (t.master) aw_store<kVec>(t.master, HOA_F32, i, n, x);
   aw_store<kVec>(t.p, a.p_dtype, i, n, x);
@@ -196,23 +199,27 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
     aw_store<kVec>(t.v, HOA_F32, i, n, v);
     return;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mtop = fmaxf(mtop, __shfl_xor_sync(0xffffffffu, mtop, o));
-    rtop = fmaxf(rtop, __shfl_xor_sync(0xffffffffu, rtop, o));
-  }
-  // (a NaN among the moments is the block's scale, as a maximum that propagates it would be)
-  const float nan = __int_as_float(0x7fffffff);
-  ms = __any_sync(0xffffffffu, nan_m) ? nan : __fmul_rn(mtop, 1.f / 448.f);
-  vs = __any_sync(0xffffffffu, nan_r) ? nan : __fmul_rn(rtop, 1.f / 448.f);
-  const float ym = aw_div_by(ms) ? __frcp_rn(ms) : 0.f, yr = aw_div_by(vs) ? __frcp_rn(vs) : 0.f;   // (uniform in the warp)
+  // the largest of the block, as bits (a NaN is above all else, and is the scale then)
+  unsigned mt = 0, rt = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float qm = ym > 0.f ? aw_div(m[e], ms, ym) : ms > 0.f ? __fdiv_rn(m[e], ms) : 0.f;
-    float qr = yr > 0.f ? aw_div(r[e], vs, yr) : vs > 0.f ? __fdiv_rn(r[e], vs) : 0.f;
-    if (r[e] > 0.f) qr = fmaxf(qr, 0.001953125f);
-    mb[e] = aw_e4m3(qm);
-    vb[e] = aw_e4m3(qr);
+    mt = max(mt, __float_as_uint(fabsf(m[e])));
+    rt = max(rt, __float_as_uint(fabsf(r[e])));
+  }
+  ms = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, mt)), 1.f / 448.f);
+  vs = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, rt)), 1.f / 448.f);
+  if (aw_div_by(ms)) {                                            // (uniform in the warp)
+    const float y = __frcp_rn(ms);
+    mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, y); });
+  } else {
+    mb = aw_pack8(m, [&](float q) { return ms > 0.f ? __fdiv_rn(q, ms) : 0.f; });
+  }
+  constexpr float kLeast = 0.001953125f;                          // 2^-9
+  if (aw_div_by(vs)) {
+    const float y = __frcp_rn(vs);
+    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, y), kLeast) : q; });
+  } else {
+    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(vs > 0.f ? __fdiv_rn(q, vs) : 0.f, kLeast) : 0.f; });
   }
   aw_store8<kVec>(t.m, i, n, mb);
   aw_store8<kVec>(t.v, i, n, vb);
@@ -231,7 +238,7 @@ __global__ void __launch_bounds__(kAwThreads) adamw_kernel(const __grid_constant
     s_c2 = (float)sqrt(1.0 - pow(a.b2d, t));
   }
   __syncthreads();
-  const float lr = s_lr, c2 = s_c2, y2 = __frcp_rn(c2);
+  const float lr = s_lr, y2 = __frcp_rn(s_c2);
   int lo = 0;
   for (unsigned c = blockIdx.x; c < a.ctas; c += gridDim.x) {
     int hi = a.count - 1;                              // the tensor of this part: the last one that starts at or before it
@@ -242,8 +249,8 @@ __global__ void __launch_bounds__(kAwThreads) adamw_kernel(const __grid_constant
     const AwTensor& t = a.t[lo];
     const long long blk = (long long)(c - a.first[lo]) * (kAwSpan / kAwBlock) + (threadIdx.x >> 5);
     if (blk * kAwBlock >= t.n) continue;
-    if (t.vec) aw_block<kBits, true>(a, t, blk, lr, c2, y2);
-    else aw_block<kBits, false>(a, t, blk, lr, c2, y2);
+    if (t.vec) aw_block<kBits, true>(a, t, blk, lr, y2);
+    else aw_block<kBits, false>(a, t, blk, lr, y2);
   }
 }
 

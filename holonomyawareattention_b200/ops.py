@@ -8,6 +8,7 @@ tensor or an unsupported shape raises.
 from __future__ import annotations
 
 import collections
+import contextlib
 import ctypes
 import math
 import threading
@@ -734,6 +735,11 @@ def _bytes_of(fn: str, *sizes) -> int:
     return n
 
 
+def _current(idx: int):
+    """Device ``idx`` is current inside."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == idx else torch.cuda.device(idx)
+
+
 def _run(idx: int, name: str, *args) -> None:
     """Call ``name`` with device ``idx`` current, its status word and its current stream as the last arguments."""
     if torch.cuda.current_device() == idx:
@@ -1151,7 +1157,7 @@ def path_bwd(a_all: torch.Tensor, R: torch.Tensor, C: torch.Tensor, chunk: int, 
     for i, name in enumerate(("dq^", "dk^", "dv^", "do^")):
         _like(dhats[i], name, (B * H, T, d), dt, idx)
     chunk = min(chunk, T)
-    with torch.cuda.device(idx):
+    with _current(idx):
         nb = _bytes_of("hoa_path_bwd_workspace_bytes", B, H, T, d, chunk)
     if nb == 0:
         raise NotImplementedError(f"B H T = {B} {H} {T} with chunk {chunk} is too large")
@@ -1192,21 +1198,30 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
         return
     idx = _index(params[0])
     _ints(step, "step", (1,), idx)
-    p_code, g_code = _dtype_code(params[0].dtype), _dtype_code(grads[0].dtype)
+    p_dt, g_dt = params[0].dtype, grads[0].dtype
+    p_code, g_code = _dtype_code(p_dt), _dtype_code(g_dt)
     moment = torch.float32 if scales is None else torch.float8_e4m3fn
-    for i, p in enumerate(params):
-        _like(p, f"params[{i}]", p.shape, params[0].dtype, idx)
-        _like(grads[i], f"grads[{i}]", p.shape, grads[0].dtype, idx)
-        _like(exp_avg[i], f"exp_avg[{i}]", p.shape, moment, idx)
-        _like(exp_avg_sq[i], f"exp_avg_sq[{i}]", p.shape, moment, idx)
-        if masters is not None:
+    # (one pass, the names only where something is wrong: a step of a few tensors takes as long as these checks)
+    rows = zip(params, grads, exp_avg, exp_avg_sq)
+    if not all(p.get_device() == g.get_device() == m.get_device() == v.get_device() == idx and p.dtype is p_dt and g.dtype is g_dt
+               and m.dtype is moment and v.dtype is moment and p.shape == g.shape == m.shape == v.shape and p.is_contiguous()
+               and g.is_contiguous() and m.is_contiguous() and v.is_contiguous() for p, g, m, v in rows):
+        for i, p in enumerate(params):
+            _like(p, f"params[{i}]", p.shape, p_dt, idx)
+            _like(grads[i], f"grads[{i}]", p.shape, g_dt, idx)
+            _like(exp_avg[i], f"exp_avg[{i}]", p.shape, moment, idx)
+            _like(exp_avg_sq[i], f"exp_avg_sq[{i}]", p.shape, moment, idx)
+    sizes = [p.numel() for p in params]
+    if masters is not None:
+        for i, p in enumerate(params):
             _like(masters[i], f"masters[{i}]", p.shape, torch.float32, idx)
-        if scales is not None:
-            _like(scales[i], f"scales[{i}]", (2, -(-p.numel() // ADAMW_BLOCK)), torch.float32, idx)
-    with torch.cuda.device(idx):
-        _lib.call("hoa_adamw_step", _pointers(params), p_code, _pointers(masters) if masters is not None else None, _pointers(grads),
-                  g_code, _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None,
-                  32 if scales is None else 8, _longs(*(p.numel() for p in params)), n, step.data_ptr(), lr, betas[0], betas[1], eps,
-                  weight_decay, torch._C._cuda_getCurrentRawStream(idx))
+    if scales is not None:
+        for i, n_i in enumerate(sizes):
+            _like(scales[i], f"scales[{i}]", (2, -(-n_i // ADAMW_BLOCK)), torch.float32, idx)
+    with _current(idx):
+        _lib.check("hoa_adamw_step", _fn("hoa_adamw_step")(
+            _pointers(params), p_code, _pointers(masters) if masters is not None else None, _pointers(grads), g_code,
+            _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None, 32 if scales is None else 8,
+            _longs(*sizes), n, step.data_ptr(), lr, betas[0], betas[1], eps, weight_decay, torch._C._cuda_getCurrentRawStream(idx)))
     # written behind autograd's back: what was saved of them, or laid out from them, is out of date
     torch.autograd.graph.increment_version([t for t in (*params, *(masters or ())) if not t.is_inference()])
