@@ -16,12 +16,15 @@
 // update, which nothing is kept of but its sum with x, takes fast division.
 #include <cuda_fp8.h>
 
+#include <cmath>
+
 #include "hoa_common.cuh"
 
 namespace hoa {
 
 constexpr int kAwThreads = 256, kAwBlock = 256, kAwPer = 8;       // a CTA: 8 elements a thread
 constexpr int kAwSpan = kAwThreads * kAwPer;                      // elements of a CTA, a multiple of kAwBlock
+constexpr int kAwCtas = 4;                                        // CTAs of an SM: 3 leave loads too little room, 5 and 6 spill
 constexpr int kAwMost = 256;                                      // tensors of one launch
 
 struct AwTensor {
@@ -36,7 +39,8 @@ struct AwArgs {
   int count, p_dtype, g_dtype;
   const int* step;
   float b1, nb1, b2, nb2, eps, keep;
-  double lr, b1d, b2d;
+  float lr;
+  double ln1, ln2;                // of the betas
 };
 static_assert(sizeof(AwArgs) <= 32000, "kernel parameters");
 
@@ -230,15 +234,10 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
 }
 
 template <int kBits>
-__global__ void __launch_bounds__(kAwThreads) adamw_kernel(const __grid_constant__ AwArgs a) {
-  __shared__ float s_lr, s_c2;
-  if (threadIdx.x == 0) {
-    const double t = (double)*a.step;
-    s_lr = (float)(a.lr / (1.0 - pow(a.b1d, t)));
-    s_c2 = (float)sqrt(1.0 - pow(a.b2d, t));
-  }
-  __syncthreads();
-  const float lr = s_lr, y2 = __frcp_rn(s_c2);
+__global__ void __launch_bounds__(kAwThreads, kAwCtas) adamw_kernel(const __grid_constant__ AwArgs a) {
+  // 1 - b^t = -(e^{t ln b} - 1)
+  const double t = (double)*a.step;
+  const float lr = a.lr / -expm1f((float)(t * a.ln1)), y2 = rsqrtf(-expm1f((float)(t * a.ln2)));
   int lo = 0;
   for (unsigned c = blockIdx.x; c < a.ctas; c += gridDim.x) {
     int hi = a.count - 1;                              // the tensor of this part: the last one that starts at or before it
@@ -246,11 +245,11 @@ __global__ void __launch_bounds__(kAwThreads) adamw_kernel(const __grid_constant
       const int mid = (lo + hi + 1) / 2;
       if (a.first[mid] <= c) lo = mid; else hi = mid - 1;
     }
-    const AwTensor& t = a.t[lo];
+    const AwTensor& x = a.t[lo];
     const long long blk = (long long)(c - a.first[lo]) * (kAwSpan / kAwBlock) + (threadIdx.x >> 5);
-    if (blk * kAwBlock >= t.n) continue;
-    if (t.vec) aw_block<kBits, true>(a, t, blk, lr, y2);
-    else aw_block<kBits, false>(a, t, blk, lr, y2);
+    if (blk * kAwBlock >= x.n) continue;
+    if (x.vec) aw_block<kBits, true>(a, x, blk, lr, y2);
+    else aw_block<kBits, false>(a, x, blk, lr, y2);
   }
 }
 
@@ -277,7 +276,7 @@ extern "C" int hoa_adamw_step(void* const* params, int p_dtype, float* const* ma
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       n = 148;
-    return (unsigned)n * 4;
+    return (unsigned)n * kAwCtas;
   }();
   for (int i = 0; i < count;) {
     AwArgs a{};
@@ -304,7 +303,8 @@ extern "C" int hoa_adamw_step(void* const* params, int p_dtype, float* const* ma
     a.b2 = (float)beta2; a.nb2 = (float)(1.0 - beta2);
     a.eps = (float)eps;
     a.keep = (float)(1.0 - lr * weight_decay);
-    a.lr = lr; a.b1d = beta1; a.b2d = beta2;
+    a.lr = (float)lr;
+    a.ln1 = log(beta1); a.ln2 = log(beta2);
     const unsigned grid = ctas < most ? ctas : most;
     if (state_bits == 8) adamw_kernel<8><<<grid, kAwThreads, 0, s>>>(a);
     else adamw_kernel<32><<<grid, kAwThreads, 0, s>>>(a);
