@@ -97,10 +97,10 @@ __global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p
   float* lse = dS + C::kP;
   float* D = lse + kAbT;
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
-  const int chain = blockIdx.y, d = p.d;
+  const int chain = blockIdx.x, d = p.d;                             // (all chains' longest walks first)
   const int nq = (p.Tq + kAbT - 1) / kAbT, nk = (p.Tk + kAbT - 1) / kAbT;
   const long long qbase = (long long)chain * p.Tq * d, kbase = (long long)chain * p.Tk * d;
-  const int own = kKeys ? blockIdx.x : nq - 1 - blockIdx.x;        // the longest walks first
+  const int own = kKeys ? blockIdx.y : nq - 1 - blockIdx.y;
   int first = 0, last = nq;
   if (kKeys) {
     first = max(0, (own * kAbT - p.q_offset) / kAbT);              // the first query tile that sees one of the keys
@@ -177,13 +177,38 @@ __global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p
   }
 }
 
-// D_i = do_i . o_i, 8 lanes a row.
+// D_i = do_i . o_i, 8 lanes a row; kVec: 8 elements a load (d % 8 == 0, 16-byte boundaries).
+template <bool kVec>
 __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(AttnBwdArgs p, long long rows) {
   const long long r = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int l = threadIdx.x & 7;
   float t = 0.f;
-  if (r < rows)
-    for (int e = l; e < p.d; e += 8) t = fmaf(load_elem(p.dout, r * p.d + e, p.dtype), p.o[r * p.d + e], t);
+  if (r < rows) {
+    if (kVec) {
+      for (int e = 8 * l; e < p.d; e += 64) {
+        float x[8];
+        if (p.dtype == HOA_BF16) {
+          const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.dout) + r * p.d + e);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            x[2 * k] = __uint_as_float(w[k] << 16);
+            x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+          }
+        } else {
+          const float4* f = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.dout) + r * p.d + e);
+          const float4 a = f[0], b = f[1];
+          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        }
+        const float4* f = reinterpret_cast<const float4*>(p.o + r * p.d + e);
+        const float4 a = f[0], b = f[1];
+        t = fmaf(x[0], a.x, fmaf(x[1], a.y, fmaf(x[2], a.z, fmaf(x[3], a.w, t))));
+        t = fmaf(x[4], b.x, fmaf(x[5], b.y, fmaf(x[6], b.z, fmaf(x[7], b.w, t))));
+      }
+    } else {
+      for (int e = l; e < p.d; e += 8) t = fmaf(load_elem(p.dout, r * p.d + e, p.dtype), p.o[r * p.d + e], t);
+    }
+  }
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   if (r < rows && l == 0) p.delta[r] = t;
@@ -193,7 +218,9 @@ template <int DA, bool kKeys>
 static int launch_simt(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(attn_bwd_simt_kernel<DA, kKeys>, AbCfg<DA>::kSmem, done)) return HOA_ERR_LAUNCH;
-  const dim3 grid((unsigned)ceil_div(kKeys ? a.Tk : a.Tq, kAbT), (unsigned)BH);
+  const int tiles = ceil_div(kKeys ? a.Tk : a.Tq, kAbT);
+  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)BH, (unsigned)tiles);
   attn_bwd_simt_kernel<DA, kKeys><<<grid, kAbThreads, AbCfg<DA>::kSmem, s>>>(a);
   return launch_status();
 }
@@ -226,7 +253,9 @@ extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, cons
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const long long rows = (long long)BH * Tq;
   if (rows > 32ll * 0x7fffffff) return HOA_ERR_UNSUPPORTED;
-  attn_bwd_delta_kernel<<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
+  const uintptr_t od = reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(dout);
+  if (d % 8 == 0 && (od & 15) == 0) attn_bwd_delta_kernel<true><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
+  else attn_bwd_delta_kernel<false><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
   if (int st = launch_status()) return st;
   uintptr_t at = 0;                                                  // TMA and the outputs' 16-byte stores
   for (const void* x : {qh, kh, vh, dout, (const void*)dq, (const void*)dk, (const void*)dv}) at |= reinterpret_cast<uintptr_t>(x);

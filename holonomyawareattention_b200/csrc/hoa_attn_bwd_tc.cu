@@ -12,10 +12,12 @@
 // tile serves as the K-major right operand of the first products and, by rows, as the MN-major
 // one of the second.
 //
-// Warps (320 threads): 0-3 and 4-7 are two softmax warpgroups that take the streamed tiles in
-// turn (one's exponentials run beside the products of the other's tile), 8 issues the
-// products, 9 the TMA loads.  TMEM: S and G of two tiles (4 x 64 columns), the accumulators
-// (2 x 128).
+// Warps: W softmax warpgroups that take the streamed tiles in turn, one warp that issues the
+// products, one for the TMA loads.  One's exponentials run beside the products of another's tile:
+// head dims above 64 have W = 2 in a CTA (TMEM: S and G of two tiles, 4 x 64 columns, and the
+// accumulators, 2 x 128: an SM's 512); up to 64 a CTA has W = 1 in 256 columns and 80 KB, and two
+// run on an SM, so that one's start and end overlap the other's work too (256 x 512 x 48:
+// 114 us with W = 2).  CTAs with the longest walks, of all chains, start first.
 #include "hoa_attn_bwd.cuh"
 #include "hoa_f32x2.cuh"
 #include "hoa_tma.cuh"
@@ -23,20 +25,21 @@
 namespace hoa {
 using namespace sm100;
 
-constexpr int kBwThreads = 320, kBwOwn = 128, kBwStr = 64;
+constexpr int kBwOwn = 128, kBwStr = 64;
 
 template <int DP>
 struct BwLayout {
+  static constexpr int W = DP <= 64 ? 1 : 2, kThreads = 128 * W + 64;
   static constexpr int NKB = (DP + 63) / 64;
   static constexpr int kOwnBlk = kBwOwn * 128, kStrBlk = kBwStr * 128;     // 64 columns of a tile
   static constexpr int kOwn = NKB * kOwnBlk, kStr = NKB * kStrBlk;
-  static constexpr int kStage = 2 * kStr, NS = 4;
+  static constexpr int kStage = 2 * kStr, NS = W == 1 ? 3 : 4;
   static constexpr int offStage = 2 * kOwn;
   static constexpr int offCol = offStage + NS * kStage;                    // -lse log2 e and -D of the streamed queries
-  static constexpr int offBar = offCol + 2 * 2 * 128 * 4;
+  static constexpr int offBar = offCol + W * 2 * 128 * 4;
   static constexpr int kAlloc = offBar + 256 + 1024;
   static_assert(kAlloc <= 232448, "shared memory budget");
-  static constexpr uint32_t colA0 = 256, colA1 = 384;
+  static constexpr uint32_t kAcc = W == 1 ? 64 : 128, colA0 = 128 * W, colA1 = colA0 + kAcc, kCols = 256 * W;
 };
 
 HOA_DEVICE float bw_exp2(float x) {
@@ -51,11 +54,12 @@ HOA_DEVICE float bw_pack(F2 x) {
 }
 
 template <int DP, bool kKeys>
-__global__ void __launch_bounds__(kBwThreads, 1)
+__global__ void __launch_bounds__(BwLayout<DP>::kThreads, BwLayout<DP>::W == 1 ? 2 : 1)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant__ CUtensorMap x1,
                    const __grid_constant__ CUtensorMap y0, const __grid_constant__ CUtensorMap y1,
                    const __grid_constant__ AttnBwdArgs p) {
   using L = BwLayout<DP>;
+  constexpr int W = L::W;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* cols = reinterpret_cast<float*>(sm + L::offCol);
@@ -63,15 +67,15 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
   uint64_t* own_full = bars;
   uint64_t* full = bars + 1;         // [NS]
   uint64_t* empty = full + L::NS;    // [NS]
-  uint64_t* s_full = empty + L::NS;  // [2]
-  uint64_t* p_full = s_full + 2;     // [2]
-  uint64_t* fin = p_full + 2;
+  uint64_t* s_full = empty + L::NS;  // [W]
+  uint64_t* p_full = s_full + W;     // [W]
+  uint64_t* fin = p_full + W;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(fin + 2);
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
-  const int chain = blockIdx.y, d = p.d;
+  const int chain = blockIdx.x, d = p.d;
   // the longest walks first: early keys, late queries
-  const int own0 = (kKeys ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x)) * kBwOwn;
+  const int own0 = (kKeys ? (int)blockIdx.y : (int)(gridDim.y - 1 - blockIdx.y)) * kBwOwn;
   int first = 0, n;
   if (kKeys) {
     first = max(0, own0 - p.q_offset) / kBwStr;
@@ -80,12 +84,12 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
     n = (p.q_offset + min(own0 + kBwOwn, p.Tq) - 1) / kBwStr + 1;
   }
   if (tid == 0) {
-    for (int i = 0; i < 2 + 2 * L::NS + 4; ++i) mbar_init(&bars[i], &bars[i] == p_full || &bars[i] == p_full + 1 ? 4 : 1);
+    for (uint64_t* b = bars; b <= fin; ++b) mbar_init(b, b >= p_full && b < fin ? 4 : 1);
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 0) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, L::kCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -94,7 +98,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
   const uint32_t tmem = *tmem_slot;
   bool bad = false;
 
-  if (warp == 9) {
+  if (warp == 4 * W + 1) {
     // ------------------------------------------------------------------ TMA
     if (lid == 0 && n > 0) {
       mbar_arrive_expect_tx(own_full, 2u * L::kOwn);
@@ -119,7 +123,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
       bad |= !mbar_wait(own_full, 0);
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == 4 * W) {
     // ------------------------------------------------------------------ MMA
     if (n > 0 && elect_one()) {
       constexpr uint32_t idS = make_idesc(kFmtBF16, 128, kBwStr), idA = make_idesc(kFmtBF16, 128, DP, true);
@@ -132,7 +136,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
         tc_fence_after();
         const uint32_t st = smem_u32(sm + L::offStage + s * L::kStage);
         const uint64_t dY0 = desc_sw128(st), dY1 = desc_sw128(st + L::kStr);
-        const uint32_t cS = tmem + (j & 1) * 128;
+        const uint32_t cS = tmem + (j % W) * 128;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
@@ -145,17 +149,17 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
           const uint64_t oy = (uint64_t)(((kk >> 2) * L::kStrBlk + (kk & 3) * 32) >> 4);
           mma_bf16(cS + 64, dX1 + ox, dY1 + oy, idS, kk > 0 ? 1u : 0u);
         }
-        tc_commit(&s_full[j & 1]);
+        tc_commit(&s_full[j % W]);
       };
       front(0);
       for (int j = 0; j < n && ok; ++j) {
-        if (j + 1 < n) front(j + 1);
-        ok = ok && mbar_wait_abortable(&p_full[j & 1], (j >> 1) & 1, s_abort, p.max_wait);
+        if (W > 1 && j + 1 < n) front(j + 1);
+        ok = ok && mbar_wait_abortable(&p_full[j % W], (j / W) & 1, s_abort, p.max_wait);
         if (!ok) break;
         tc_fence_after();
         const uint32_t st = smem_u32(sm + L::offStage + (j % L::NS) * L::kStage);
         const uint64_t mY0 = desc_sw128_mn(st, L::kStrBlk), mY1 = desc_sw128_mn(st + L::kStr, L::kStrBlk);
-        const uint32_t cS = tmem + (j & 1) * 128;
+        const uint32_t cS = tmem + (j % W) * 128;
         if (kKeys) {
 #pragma unroll
           for (int kk = 0; kk < kBwStr / 16; ++kk)
@@ -165,6 +169,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
         for (int kk = 0; kk < kBwStr / 16; ++kk)
           mma_bf16_ts(tmem + L::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u);
         tc_commit(&empty[j % L::NS]);
+        if (W == 1 && j + 1 < n) front(j + 1);                     // (over P and dS, behind the products that read them)
       }
       if (!ok) bad = true;
       tc_commit(fin);
@@ -173,7 +178,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
     __syncwarp();
   } else {
     // -------------------------------------------------------------- softmax
-    const int g = warp >> 2;                                      // takes the tiles g, g + 2, ...
+    const int g = warp >> 2;                                      // takes the tiles g, g + W, ...
     const int r = tid & 127;                                      // row of the own tile = TMEM lane
     const uint32_t lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t cS = tmem + lane + g * 128;
@@ -190,16 +195,16 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
       my_l = stat(p.lse, own0 + r, -INFINITY, -kLog2e);
       my_D = stat(p.delta, own0 + r, 0.f, -1.f);
     }
-    for (int j = g; j < n; j += 2) {
+    for (int j = g; j < n; j += W) {
       const int t0 = (first + j) * kBwStr;
-      float* col = cols + (g * 2 + ((j >> 1) & 1)) * 128;
+      float* col = cols + (g * 2 + ((j / W) & 1)) * 128;
       if (kKeys) {
         col[r] = next;
         named_sync(1 + g, 128);
-        const int q = t0 + 2 * kBwStr + (r & 63);
-        if (j + 2 < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
+        const int q = t0 + W * kBwStr + (r & 63);
+        if (j + W < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
       }
-      bad |= !mbar_wait_abortable(&s_full[g], (j >> 1) & 1, s_abort, p.max_wait);
+      bad |= !mbar_wait_abortable(&s_full[g], (j / W) & 1, s_abort, p.max_wait);
       tc_fence_after();
       // columns of this row that count: keys, its own key up to the query; queries, keys up to its own
       int lo = 0, hi = kBwStr;
@@ -251,20 +256,20 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
       __syncwarp();
       if (lid == 0) mbar_arrive(&p_full[g]);
     }
-    // ---- epilogue: rows of the own tile that exist; two warpgroups: dv and dk, or the halves of dq
+    // ---- epilogue: rows of the own tile that exist; 16 columns of dv, dk (or dq) a warpgroup in turn
     if (n > 0) bad |= !mbar_wait_abortable(fin, 0, s_abort, p.max_wait);
     tc_fence_after();
     const int rows = kKeys ? p.Tk : p.Tq;
-    const uint32_t acc = tmem + lane + (kKeys && g == 0 ? L::colA0 : L::colA1);
-    const float f = kKeys && g == 0 ? 1.f : p.scale;
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(!kKeys ? p.dq : g == 0 ? p.dv : p.dk) +
-                         ((long long)chain * rows + own0 + r) * d;
+    const long long row_at = ((long long)chain * rows + own0 + r) * d;
+    constexpr int kC = DP / 16;
 #pragma unroll
-    for (int c16 = 0; c16 < DP / 16; ++c16) {
-      if (!kKeys && (c16 & 1) != g) continue;
+    for (int i = 0; i < (kKeys ? 2 : 1) * kC; ++i) {
+      if (i % W != g) continue;
+      const bool is_dv = kKeys && i < kC;
+      const int c16 = i % kC;
       float v[16];
       if (n > 0) {
-        tmem_ld16(acc + 16 * c16, v);
+        tmem_ld16(tmem + lane + (is_dv ? L::colA0 : L::colA1) + 16 * c16, v);
         tmem_wait_ld();
         tmem_touch(v);
       } else {
@@ -272,6 +277,8 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
         for (int e = 0; e < 16; ++e) v[e] = 0.f;
       }
       if (own0 + r >= rows || bad) continue;
+      const float f = is_dv ? 1.f : p.scale;
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(!kKeys ? p.dq : is_dv ? p.dv : p.dk) + row_at + 16 * c16;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (16 * c16 + 8 * h >= d) continue;
@@ -279,7 +286,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
         uint32_t* u = &w.x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) u[e] = __float_as_uint(bw_pack(f2(v[8 * h + 2 * e] * f, v[8 * h + 2 * e + 1] * f)));
-        *reinterpret_cast<uint4*>(out + 16 * c16 + 8 * h) = w;
+        *reinterpret_cast<uint4*>(out + 8 * h) = w;
       }
     }
   }
@@ -287,7 +294,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
   bad = __syncthreads_or(bad || *s_abort != 0);
   if (bad && tid == 0 && p.status != nullptr) *reinterpret_cast<volatile int*>(p.status) = HOA_ERR_TIMEOUT;
   tc_fence_after();
-  if (warp == 0) tmem_dealloc(tmem, 512);
+  if (warp == 0) tmem_dealloc(tmem, L::kCols);
 }
 
 template <int DP, bool kKeys>
@@ -301,8 +308,9 @@ static int launch_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   }
   static std::atomic<unsigned long long> done{0};
   if (!allow_smem(attn_bwd_tc_kernel<DP, kKeys>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
-  const dim3 grid((unsigned)ceil_div(kKeys ? a.Tk : a.Tq, kBwOwn), (unsigned)BH);
-  attn_bwd_tc_kernel<DP, kKeys><<<grid, kBwThreads, L::kAlloc, s>>>(m[0], m[1], m[2], m[3], a);
+  const int tiles = ceil_div(kKeys ? a.Tk : a.Tq, kBwOwn);
+  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
+  attn_bwd_tc_kernel<DP, kKeys><<<dim3((unsigned)BH, (unsigned)tiles), L::kThreads, L::kAlloc, s>>>(m[0], m[1], m[2], m[3], a);
   return launch_status();
 }
 
