@@ -27,14 +27,36 @@ template <int DA> struct AbCfg {
   static constexpr size_t kSmem = (4 * kTile + 2 * kP + 2 * kAbT) * sizeof(float);
 };
 
-// 64 rows from `row0` of x (rows, d) -> tile, zero outside
-template <int DA>
-HOA_DEVICE void ab_load(float* tile, const void* x, int dtype, long long base, int row0, int rows, int d) {
-  for (int i = threadIdx.x; i < kAbT * DA; i += kAbThreads) {
-    const int r = i / DA, e = i % DA;
-    tile[r * AbCfg<DA>::kLd + e] = row0 + r < rows && e < d ? load_elem(x, base + (long long)(row0 + r) * d + e, dtype) : 0.f;
+// 64 rows from `row0` of x (rows, d) -> registers, zero outside (kVec: fp32, d % 4 == 0, 16-byte boundaries) -> tile
+template <int DA> struct AbRegs {
+  static constexpr int N4 = DA / 4, K = kAbT * N4 / kAbThreads;      // float4s of a thread
+  float4 v[K];
+  template <bool kVec>
+  HOA_DEVICE void load(const void* x, int dtype, long long base, int row0, int rows, int d) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = threadIdx.x + k * kAbThreads, r = row0 + i / N4, e = i % N4 * 4;
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= rows || e >= d) continue;
+      const long long at = base + (long long)r * d + e;
+      if (kVec) {
+        v[k] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+      } else {
+        v[k].x = load_elem(x, at, dtype);
+        if (e + 1 < d) v[k].y = load_elem(x, at + 1, dtype);
+        if (e + 2 < d) v[k].z = load_elem(x, at + 2, dtype);
+        if (e + 3 < d) v[k].w = load_elem(x, at + 3, dtype);
+      }
+    }
   }
-}
+  HOA_DEVICE void store(float* tile) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = threadIdx.x + k * kAbThreads;
+      *reinterpret_cast<float4*>(tile + i / N4 * AbCfg<DA>::kLd + i % N4 * 4) = v[k];
+    }
+  }
+};
 
 // acc[a][b] = X[ty + 16 a] . Y[tx + 16 b]
 template <int DA>
@@ -64,29 +86,38 @@ HOA_DEVICE void ab_nt(const float* X, const float* Y, int ty, int tx, float (&ac
   }
 }
 
-// acc[a][c] += sum_k P[k][4 ty + a] Y[k][tx + 16 c]
+// acc[a][c] += sum over k0 <= k < k1 of P[k][8 ty + a] Y[k][tx + 16 c]
 template <int DA>
-HOA_DEVICE void ab_tn(const float* P, const float* Y, int ty, int tx, float (&acc)[4][AbCfg<DA>::CPT]) {
+HOA_DEVICE void ab_tn(const float* P, const float* Y, int k0, int k1, int ty, int tx, float (&acc)[8][AbCfg<DA>::CPT]) {
   constexpr int kLd = AbCfg<DA>::kLd, CPT = AbCfg<DA>::CPT;
 #pragma unroll 4
-  for (int k = 0; k < kAbT; ++k) {
-    const float4 p = *reinterpret_cast<const float4*>(P + k * kAbLdP + 4 * ty);
+  for (int k = k0; k < k1; ++k) {
+    const float4 p0 = *reinterpret_cast<const float4*>(P + k * kAbLdP + 8 * ty);
+    const float4 p1 = *reinterpret_cast<const float4*>(P + k * kAbLdP + 8 * ty + 4);
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
       const float y = Y[k * kLd + tx + 16 * c];
-      acc[0][c] = fmaf(p.x, y, acc[0][c]);
-      acc[1][c] = fmaf(p.y, y, acc[1][c]);
-      acc[2][c] = fmaf(p.z, y, acc[2][c]);
-      acc[3][c] = fmaf(p.w, y, acc[3][c]);
+      acc[0][c] = fmaf(p0.x, y, acc[0][c]);
+      acc[1][c] = fmaf(p0.y, y, acc[1][c]);
+      acc[2][c] = fmaf(p0.z, y, acc[2][c]);
+      acc[3][c] = fmaf(p0.w, y, acc[3][c]);
+      acc[4][c] = fmaf(p1.x, y, acc[4][c]);
+      acc[5][c] = fmaf(p1.y, y, acc[5][c]);
+      acc[6][c] = fmaf(p1.z, y, acc[6][c]);
+      acc[7][c] = fmaf(p1.w, y, acc[7][c]);
     }
   }
 }
 
-// kKeys: the CTA's own tile holds keys (outputs dk, dv), else queries (output dq).
-template <int DA, bool kKeys>
-__global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p) {
+// kKeys: the CTA's own tile holds keys (outputs dk, dv), else queries (output dq).  The second products take half of the
+// threads each, 8 rows a thread (4 rows a thread would ask more of shared memory than of the FMA pipes): dv and dk, or the
+// two halves of the keys for dq.  The next tile of the other side is loaded while one is worked on (head dims up to 64;
+// above, the registers do not hold it).
+template <int DA, bool kKeys, bool kVec>
+__global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_kernel(AttnBwdArgs p) {
   using C = AbCfg<DA>;
   constexpr int CPT = C::CPT;
+  constexpr bool kAhead = DA <= 64;
   extern __shared__ __align__(16) float smem[];
   float* Q = smem;
   float* dO = Q + C::kTile;
@@ -97,6 +128,7 @@ __global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p
   float* lse = dS + C::kP;
   float* D = lse + kAbT;
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int half = tid / 128, ty8 = tid % 128 / 16;
   const int chain = blockIdx.x, d = p.d;                             // (all chains' longest walks first)
   const int nq = (p.Tq + kAbT - 1) / kAbT, nk = (p.Tk + kAbT - 1) / kAbT;
   const long long qbase = (long long)chain * p.Tq * d, kbase = (long long)chain * p.Tk * d;
@@ -107,30 +139,42 @@ __global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p
   } else {
     last = min((p.q_offset + own * kAbT + kAbT - 1) / kAbT, nk - 1) + 1;
   }
+  AbRegs<DA> r0, r1;
+  float stat = 0.f;                                                // threads 0-63: lse, 64-127: D, of the streamed queries
   auto load_keys = [&](int t) {
-    ab_load<DA>(K, p.k, p.dtype, kbase, t * kAbT, p.Tk, d);
-    ab_load<DA>(V, p.v, p.dtype, kbase, t * kAbT, p.Tk, d);
+    r0.template load<kVec>(p.k, p.dtype, kbase, t * kAbT, p.Tk, d);
+    r1.template load<kVec>(p.v, p.dtype, kbase, t * kAbT, p.Tk, d);
   };
   auto load_queries = [&](int t) {
-    ab_load<DA>(Q, p.q, p.dtype, qbase, t * kAbT, p.Tq, d);
-    ab_load<DA>(dO, p.dout, p.dtype, qbase, t * kAbT, p.Tq, d);
-    if (tid < kAbT) {
-      const bool in = t * kAbT + tid < p.Tq;
-      lse[tid] = in ? p.lse[(long long)chain * p.Tq + t * kAbT + tid] : 0.f;
-      D[tid] = in ? p.delta[(long long)chain * p.Tq + t * kAbT + tid] : 0.f;
-    }
+    r0.template load<kVec>(p.q, p.dtype, qbase, t * kAbT, p.Tq, d);
+    r1.template load<kVec>(p.dout, p.dtype, qbase, t * kAbT, p.Tq, d);
+    const int q = t * kAbT + (tid & 63);
+    if (tid < 128) stat = q < p.Tq ? (tid < 64 ? p.lse : p.delta)[(long long)chain * p.Tq + q] : 0.f;
   };
-  if (kKeys) load_keys(own); else load_queries(own);
+  auto store_queries = [&]() {
+    r0.store(Q);
+    r1.store(dO);
+    if (tid < 128) lse[tid] = stat;                                // (D lies behind lse)
+  };
+  auto store_keys = [&]() {
+    r0.store(K);
+    r1.store(V);
+  };
+  if (kKeys) { load_keys(own); store_keys(); } else { load_queries(own); store_queries(); }
+  auto load = [&](int t) { if (kKeys) load_queries(t); else load_keys(t); };
 
-  float acc0[4][CPT], acc1[4][CPT];
+  float acc[8][CPT];
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
+  for (int a = 0; a < 8; ++a)
 #pragma unroll
-    for (int c = 0; c < CPT; ++c) acc0[a][c] = acc1[a][c] = 0.f;
+    for (int c = 0; c < CPT; ++c) acc[a][c] = 0.f;
 
+  if (first < last) load(first);
   for (int t = first; t < last; ++t) {
-    if (kKeys) load_queries(t); else load_keys(t);
+    if (!kAhead && t > first) load(t);
+    if (kKeys) store_queries(); else store_keys();
     __syncthreads();
+    if (kAhead && t + 1 < last) load(t + 1);
     const int q0 = (kKeys ? t : own) * kAbT, k0 = (kKeys ? own : t) * kAbT;
     float s[4][4], g[4][4];
     ab_nt<DA>(Q, K, ty, tx, s);
@@ -151,28 +195,39 @@ __global__ void __launch_bounds__(kAbThreads) attn_bwd_simt_kernel(AttnBwdArgs p
         }
       }
     __syncthreads();
-    if (kKeys) {
-      ab_tn<DA>(P, dO, ty, tx, acc0);
-      ab_tn<DA>(dS, Q, ty, tx, acc1);
-    } else {
-      ab_tn<DA>(dS, K, ty, tx, acc1);
-    }
+    if (kKeys) ab_tn<DA>(half ? dS : P, half ? Q : dO, 0, kAbT, ty8, tx, acc);
+    else ab_tn<DA>(dS, K, half * (kAbT / 2), (half + 1) * (kAbT / 2), ty8, tx, acc);
     __syncthreads();
   }
 
+  if (!kKeys) {                                                    // the second half's sums, through shared memory
+    static_assert(C::kLd <= 2 * kAbLdP, "P and dS together hold 64 rows");
+    float* X = P;
+    if (half) {
+#pragma unroll
+      for (int a = 0; a < 8; ++a)
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) X[(8 * ty8 + a) * C::kLd + tx + 16 * c] = acc[a][c];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int a = 0; a < 8; ++a)
+#pragma unroll
+      for (int c = 0; c < CPT; ++c) acc[a][c] += X[(8 * ty8 + a) * C::kLd + tx + 16 * c];
+  }
   const int rows = kKeys ? p.Tk : p.Tq;
   const long long base = kKeys ? kbase : qbase;
+  const bool is_dv = kKeys && half == 0;
+  void* out = kKeys ? (is_dv ? p.dv : p.dk) : p.dq;
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    const int r = own * kAbT + 4 * ty + a;
+  for (int a = 0; a < 8; ++a) {
+    const int r = own * kAbT + 8 * ty8 + a;
     if (r >= rows) continue;
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
       const int e = tx + 16 * c;
-      if (e >= d) continue;
-      const long long at = base + (long long)r * d + e;
-      if (kKeys) store_elem(p.dv, at, p.dtype, acc0[a][c]);
-      store_elem(kKeys ? p.dk : p.dq, at, p.dtype, acc1[a][c] * p.scale);
+      if (e < d) store_elem(out, base + (long long)r * d + e, p.dtype, acc[a][c] * (is_dv ? 1.f : p.scale));
     }
   }
 }
@@ -214,21 +269,27 @@ __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(AttnBwdArgs p, long
   if (r < rows && l == 0) p.delta[r] = t;
 }
 
-template <int DA, bool kKeys>
+template <int DA, bool kKeys, bool kVec>
 static int launch_simt(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  if (!allow_smem(attn_bwd_simt_kernel<DA, kKeys>, AbCfg<DA>::kSmem, done)) return HOA_ERR_LAUNCH;
+  if (!allow_smem(attn_bwd_simt_kernel<DA, kKeys, kVec>, AbCfg<DA>::kSmem, done)) return HOA_ERR_LAUNCH;
   const int tiles = ceil_div(kKeys ? a.Tk : a.Tq, kAbT);
   if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)BH, (unsigned)tiles);
-  attn_bwd_simt_kernel<DA, kKeys><<<grid, kAbThreads, AbCfg<DA>::kSmem, s>>>(a);
+  attn_bwd_simt_kernel<DA, kKeys, kVec><<<dim3((unsigned)BH, (unsigned)tiles), kAbThreads, AbCfg<DA>::kSmem, s>>>(a);
   return launch_status();
+}
+
+template <int DA, bool kVec>
+static int launch_sides(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+  const int st = launch_simt<DA, true, kVec>(a, BH, s);
+  return st == HOA_OK ? launch_simt<DA, false, kVec>(a, BH, s) : st;
 }
 
 template <int DA>
 static int launch_both(const AttnBwdArgs& a, int BH, cudaStream_t s) {
-  const int st = launch_simt<DA, true>(a, BH, s);
-  return st == HOA_OK ? launch_simt<DA, false>(a, BH, s) : st;
+  uintptr_t at = 0;
+  for (const void* x : {a.q, a.k, a.v, a.dout}) at |= reinterpret_cast<uintptr_t>(x);
+  return a.dtype == HOA_F32 && a.d % 4 == 0 && (at & 15) == 0 ? launch_sides<DA, true>(a, BH, s) : launch_sides<DA, false>(a, BH, s);
 }
 
 }  // namespace hoa
