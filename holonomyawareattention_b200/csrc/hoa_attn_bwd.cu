@@ -114,7 +114,7 @@ HOA_DEVICE void ab_tn(const float* P, const float* Y, int k0, int k1, int ty, in
 // two halves of the keys for dq.  The next tile of the other side is loaded while one is worked on (head dims up to 64;
 // above, the registers do not hold it).
 template <int DA, bool kKeys, bool kVec>
-__global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_kernel(AttnBwdArgs p) {
+HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
   using C = AbCfg<DA>;
   constexpr int CPT = C::CPT;
   constexpr bool kAhead = DA <= 64;
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_ke
   const int nq = (p.Tq + kAbT - 1) / kAbT, nk = (p.Tk + kAbT - 1) / kAbT;
   const long long qbase = (long long)chain * p.Tq * d, kbase = (long long)chain * p.Tk * d;
   const int own = kKeys ? blockIdx.y : nq - 1 - blockIdx.y;
+  if (own < 0 || own >= (kKeys ? nk : nq)) return;
   int first = 0, last = nq;
   if (kKeys) {
     first = max(0, (own * kAbT - p.q_offset) / kAbT);              // the first query tile that sees one of the keys
@@ -232,6 +233,14 @@ __global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_ke
   }
 }
 
+// Both sides in one launch (blockIdx.z): neither waits for the other, and few tiles leave SMs to both.
+template <int DA, bool kVec>
+__global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_kernel(const __grid_constant__ AttnBwdArgs p) {
+  wait_previous();                                                 // D
+  if (blockIdx.z == 0) attn_bwd_simt<DA, true, kVec>(p);
+  else attn_bwd_simt<DA, false, kVec>(p);
+}
+
 // D_i = do_i . o_i, 8 lanes a row; kVec: 8 elements a load (d % 8 == 0, 16-byte boundaries).
 template <bool kVec>
 __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(AttnBwdArgs p, long long rows) {
@@ -269,20 +278,13 @@ __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(AttnBwdArgs p, long
   if (r < rows && l == 0) p.delta[r] = t;
 }
 
-template <int DA, bool kKeys, bool kVec>
-static int launch_simt(const AttnBwdArgs& a, int BH, cudaStream_t s) {
-  static std::atomic<unsigned long long> done{0};
-  if (!allow_smem(attn_bwd_simt_kernel<DA, kKeys, kVec>, AbCfg<DA>::kSmem, done)) return HOA_ERR_LAUNCH;
-  const int tiles = ceil_div(kKeys ? a.Tk : a.Tq, kAbT);
-  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
-  attn_bwd_simt_kernel<DA, kKeys, kVec><<<dim3((unsigned)BH, (unsigned)tiles), kAbThreads, AbCfg<DA>::kSmem, s>>>(a);
-  return launch_status();
-}
-
 template <int DA, bool kVec>
 static int launch_sides(const AttnBwdArgs& a, int BH, cudaStream_t s) {
-  const int st = launch_simt<DA, true, kVec>(a, BH, s);
-  return st == HOA_OK ? launch_simt<DA, false, kVec>(a, BH, s) : st;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(attn_bwd_simt_kernel<DA, kVec>, AbCfg<DA>::kSmem, done)) return HOA_ERR_LAUNCH;
+  const int tiles = ceil_div(a.Tk, kAbT);                          // (Tq <= Tk)
+  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
+  return launch_early(attn_bwd_simt_kernel<DA, kVec>, dim3((unsigned)BH, (unsigned)tiles, 2), 1, kAbThreads, AbCfg<DA>::kSmem, s, a);
 }
 
 template <int DA>

@@ -53,11 +53,10 @@ HOA_DEVICE float bw_pack(F2 x) {
   return __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
 }
 
+struct BwMaps { CUtensorMap x0, x1, y0, y1; };
+
 template <int DP, bool kKeys>
-__global__ void __launch_bounds__(BwLayout<DP>::kThreads, BwLayout<DP>::W == 1 ? 2 : 1)
-attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant__ CUtensorMap x1,
-                   const __grid_constant__ CUtensorMap y0, const __grid_constant__ CUtensorMap y1,
-                   const __grid_constant__ AttnBwdArgs p) {
+HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
   using L = BwLayout<DP>;
   constexpr int W = L::W;
   extern __shared__ uint8_t smem_raw[];
@@ -75,7 +74,8 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lid = tid & 31;
   const int chain = blockIdx.x, d = p.d;
   // the longest walks first: early keys, late queries
-  const int own0 = (kKeys ? (int)blockIdx.y : (int)(gridDim.y - 1 - blockIdx.y)) * kBwOwn;
+  const int own0 = (kKeys ? (int)blockIdx.y : (int)((p.Tq + kBwOwn - 1) / kBwOwn - 1 - blockIdx.y)) * kBwOwn;
+  if (own0 < 0) return;                                             // (a launch has tiles for the longer side)
   int first = 0, n;
   if (kKeys) {
     first = max(0, own0 - p.q_offset) / kBwStr;
@@ -103,8 +103,8 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
     if (lid == 0 && n > 0) {
       mbar_arrive_expect_tx(own_full, 2u * L::kOwn);
       for (int kb = 0; kb < L::NKB; ++kb) {
-        tma_load_3d(sm + kb * L::kOwnBlk, &x0, own_full, kb * 64, own0, chain);
-        tma_load_3d(sm + L::kOwn + kb * L::kOwnBlk, &x1, own_full, kb * 64, own0, chain);
+        tma_load_3d(sm + kb * L::kOwnBlk, &maps.x0, own_full, kb * 64, own0, chain);
+        tma_load_3d(sm + L::kOwn + kb * L::kOwnBlk, &maps.x1, own_full, kb * 64, own0, chain);
       }
       int issued = 0;
       for (int j = 0; j < n; ++j) {
@@ -113,8 +113,8 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
         uint8_t* st = sm + L::offStage + s * L::kStage;
         mbar_arrive_expect_tx(&full[s], (uint32_t)L::kStage);
         for (int kb = 0; kb < L::NKB; ++kb) {
-          tma_load_3d(st + kb * L::kStrBlk, &y0, &full[s], kb * 64, (first + j) * kBwStr, chain);
-          tma_load_3d(st + L::kStr + kb * L::kStrBlk, &y1, &full[s], kb * 64, (first + j) * kBwStr, chain);
+          tma_load_3d(st + kb * L::kStrBlk, &maps.y0, &full[s], kb * 64, (first + j) * kBwStr, chain);
+          tma_load_3d(st + L::kStr + kb * L::kStrBlk, &maps.y1, &full[s], kb * 64, (first + j) * kBwStr, chain);
         }
         issued = j + 1;
       }
@@ -297,39 +297,43 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap x0, const __grid_constant
   if (warp == 0) tmem_dealloc(tmem, L::kCols);
 }
 
-template <int DP, bool kKeys>
-static int launch_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
-  using L = BwLayout<DP>;
-  CUtensorMap m[4];
-  const void* x[4] = {kKeys ? a.k : a.q, kKeys ? a.v : a.dout, kKeys ? a.q : a.k, kKeys ? a.dout : a.v};
-  for (int i = 0; i < 4; ++i) {
-    const int rows = (i < 2) == kKeys ? a.Tk : a.Tq;
-    if (!make_map(&m[i], x[i], a.d, rows, BH, (uint64_t)a.d * 2, (uint64_t)rows * a.d * 2, i < 2 ? kBwOwn : kBwStr)) return HOA_ERR_INVALID_ARG;
-  }
-  static std::atomic<unsigned long long> done{0};
-  if (!allow_smem(attn_bwd_tc_kernel<DP, kKeys>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
-  const int tiles = ceil_div(kKeys ? a.Tk : a.Tq, kBwOwn);
-  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
-  attn_bwd_tc_kernel<DP, kKeys><<<dim3((unsigned)BH, (unsigned)tiles), L::kThreads, L::kAlloc, s>>>(m[0], m[1], m[2], m[3], a);
-  return launch_status();
+// Both roles in one launch (blockIdx.z): neither waits for the other.
+template <int DP>
+__global__ void __launch_bounds__(BwLayout<DP>::kThreads, BwLayout<DP>::W == 1 ? 2 : 1)
+attn_bwd_tc_kernel(const __grid_constant__ BwMaps keys, const __grid_constant__ BwMaps queries, const __grid_constant__ AttnBwdArgs p) {
+  wait_previous();                                                  // D
+  if (blockIdx.z == 0) attn_bwd_tc_role<DP, true>(keys, p);
+  else attn_bwd_tc_role<DP, false>(queries, p);
 }
 
 template <int DP>
-static int launch_bwd_both(const AttnBwdArgs& a, int BH, cudaStream_t s) {
-  const int st = launch_bwd_tc<DP, true>(a, BH, s);
-  return st == HOA_OK ? launch_bwd_tc<DP, false>(a, BH, s) : st;
+static int launch_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+  using L = BwLayout<DP>;
+  BwMaps m[2];                                                      // of keys and of queries that own the tile
+  auto map = [&](CUtensorMap* to, const void* x, int rows, int box) {
+    return make_map(to, x, a.d, rows, BH, (uint64_t)a.d * 2, (uint64_t)rows * a.d * 2, box);
+  };
+  if (!map(&m[0].x0, a.k, a.Tk, kBwOwn) || !map(&m[0].x1, a.v, a.Tk, kBwOwn) || !map(&m[0].y0, a.q, a.Tq, kBwStr) ||
+      !map(&m[0].y1, a.dout, a.Tq, kBwStr) || !map(&m[1].x0, a.q, a.Tq, kBwOwn) || !map(&m[1].x1, a.dout, a.Tq, kBwOwn) ||
+      !map(&m[1].y0, a.k, a.Tk, kBwStr) || !map(&m[1].y1, a.v, a.Tk, kBwStr))
+    return HOA_ERR_INVALID_ARG;
+  static std::atomic<unsigned long long> done{0};
+  if (!allow_smem(attn_bwd_tc_kernel<DP>, L::kAlloc, done)) return HOA_ERR_LAUNCH;
+  const int tiles = ceil_div(a.Tk, kBwOwn);                         // (Tq <= Tk)
+  if (tiles > 65535) return HOA_ERR_UNSUPPORTED;
+  return launch_early(attn_bwd_tc_kernel<DP>, dim3((unsigned)BH, (unsigned)tiles, 2), 1, L::kThreads, L::kAlloc, s, m[0], m[1], a);
 }
 
 int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   switch ((a.d + 15) / 16) {
-    case 1: return launch_bwd_both<16>(a, BH, s);
-    case 2: return launch_bwd_both<32>(a, BH, s);
-    case 3: return launch_bwd_both<48>(a, BH, s);
-    case 4: return launch_bwd_both<64>(a, BH, s);
-    case 5: return launch_bwd_both<80>(a, BH, s);
-    case 6: return launch_bwd_both<96>(a, BH, s);
-    case 7: return launch_bwd_both<112>(a, BH, s);
-    default: return launch_bwd_both<128>(a, BH, s);
+    case 1: return launch_bwd_tc<16>(a, BH, s);
+    case 2: return launch_bwd_tc<32>(a, BH, s);
+    case 3: return launch_bwd_tc<48>(a, BH, s);
+    case 4: return launch_bwd_tc<64>(a, BH, s);
+    case 5: return launch_bwd_tc<80>(a, BH, s);
+    case 6: return launch_bwd_tc<96>(a, BH, s);
+    case 7: return launch_bwd_tc<112>(a, BH, s);
+    default: return launch_bwd_tc<128>(a, BH, s);
   }
 }
 

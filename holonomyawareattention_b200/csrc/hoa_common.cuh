@@ -99,10 +99,10 @@ HOA_DEVICE void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memor
 HOA_DEVICE void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <class K, class... A>
-inline int launch_early(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t smem, cudaStream_t s,
+inline int launch_early(K kernel, dim3 grid, unsigned cluster, unsigned threads, size_t smem, cudaStream_t s,
                         const A&... args) {
   cudaLaunchConfig_t c{};
-  c.gridDim = dim3(grid);
+  c.gridDim = grid;
   c.blockDim = dim3(threads);
   c.dynamicSmemBytes = smem;
   c.stream = s;
