@@ -125,54 +125,50 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
     __syncwarp();
   } else if (warp == 4 * W) {
     // ------------------------------------------------------------------ MMA
-    if (n > 0 && elect_one()) {
+    if (n > 0) {
+      // the whole warp runs this alike; one lane issues
+      const uint32_t lead = elect_one() ? 1u : 0u, tm = warp_uniform(tmem), base = warp_uniform(smem_u32(sm));
       constexpr uint32_t idS = make_idesc(kFmtBF16, 128, kBwStr), idA = make_idesc(kFmtBF16, 128, DP, true);
-      const uint64_t dX0 = desc_sw128(smem_u32(sm)), dX1 = desc_sw128(smem_u32(sm + L::kOwn));
+      const uint64_t dX0 = desc_sw128(base), dX1 = desc_sw128(base + L::kOwn);
       bool ok = mbar_wait_abortable(own_full, 0, s_abort, p.max_wait);
       auto front = [&](int j) {
         const int s = j % L::NS;
-        ok = ok && mbar_wait_abortable(&full[s], (j / L::NS) & 1, s_abort, p.max_wait);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_abortable(&full[s], (j / L::NS) & 1, s_abort, p.max_wait));
         if (!ok) return;
         tc_fence_after();
-        const uint32_t st = smem_u32(sm + L::offStage + s * L::kStage);
+        const uint32_t st = base + L::offStage + s * L::kStage;
         const uint64_t dY0 = desc_sw128(st), dY1 = desc_sw128(st + L::kStr);
-        const uint32_t cS = tmem + (j % W) * 128;
+        const uint32_t cS = tm + (j % W) * 128;
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
+        for (int kk = 0; kk < DP / 16; ++kk) {                        // (in turn: one's sums do not wait for the other's)
           const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
           const uint64_t oy = (uint64_t)(((kk >> 2) * L::kStrBlk + (kk & 3) * 32) >> 4);
-          mma_bf16(cS, dX0 + ox, dY0 + oy, idS, kk > 0 ? 1u : 0u);
+          mma_bf16_warp(cS, dX0 + ox, dY0 + oy, idS, kk > 0 ? 1u : 0u, lead);
+          mma_bf16_warp(cS + 64, dX1 + ox, dY1 + oy, idS, kk > 0 ? 1u : 0u, lead);
         }
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
-          const uint64_t oy = (uint64_t)(((kk >> 2) * L::kStrBlk + (kk & 3) * 32) >> 4);
-          mma_bf16(cS + 64, dX1 + ox, dY1 + oy, idS, kk > 0 ? 1u : 0u);
-        }
-        tc_commit(&s_full[j % W]);
+        tc_commit_warp(&s_full[j % W], lead);
       };
+      ok = __all_sync(0xffffffffu, ok);
       front(0);
       for (int j = 0; j < n && ok; ++j) {
         if (W > 1 && j + 1 < n) front(j + 1);
-        ok = ok && mbar_wait_abortable(&p_full[j % W], (j / W) & 1, s_abort, p.max_wait);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_abortable(&p_full[j % W], (j / W) & 1, s_abort, p.max_wait));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t st = smem_u32(sm + L::offStage + (j % L::NS) * L::kStage);
+        const uint32_t st = base + L::offStage + (j % L::NS) * L::kStage;
         const uint64_t mY0 = desc_sw128_mn(st, L::kStrBlk), mY1 = desc_sw128_mn(st + L::kStr, L::kStrBlk);
-        const uint32_t cS = tmem + (j % W) * 128;
-        if (kKeys) {
+        const uint32_t cS = tm + (j % W) * 128;
 #pragma unroll
-          for (int kk = 0; kk < kBwStr / 16; ++kk)
-            mma_bf16_ts(tmem + L::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < kBwStr / 16; ++kk) {
+          if (kKeys)
+            mma_bf16_ts_warp(tm + L::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
+          mma_bf16_ts_warp(tm + L::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
         }
-#pragma unroll
-        for (int kk = 0; kk < kBwStr / 16; ++kk)
-          mma_bf16_ts(tmem + L::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u);
-        tc_commit(&empty[j % L::NS]);
+        tc_commit_warp(&empty[j % L::NS], lead);
         if (W == 1 && j + 1 < n) front(j + 1);                     // (over P and dS, behind the products that read them)
       }
       if (!ok) bad = true;
-      tc_commit(fin);
+      tc_commit_warp(fin, lead);
       bad |= !mbar_wait(fin, 0);
     }
     __syncwarp();
