@@ -115,6 +115,8 @@ class PathOrderedGeometricMHA(nn.Module):
             why = f"x must be (B, L, {self.h * self.d})"
         elif self._needs_grad(x) and (return_geometry or self.mode != "causal"):
             why = "gradients need mode 'causal' and no geometry: call under torch.no_grad() / torch.inference_mode()"
+        elif self._needs_grad(x) and torch.cuda.is_current_stream_capturing():
+            why = "a forward that needs gradients cannot be captured into a graph"
         elif attn_mask is not None and (tuple(attn_mask.shape) != (x.shape[1], x.shape[1])
                                         or attn_mask.dtype != torch.bool):
             why = "attn_mask must be None or an (L, L) bool tensor (True = allowed)"
@@ -340,8 +342,6 @@ class PathOrderedGeometricMHA(nn.Module):
         if self._needs_grad(x):
             if general:
                 raise NotImplementedError("PathOrderedGeometricMHA (B200): gradients need attn_mask = tril(L)")
-            if torch.cuda.is_current_stream_capturing():
-                raise NotImplementedError("PathOrderedGeometricMHA (B200): a forward that needs gradients cannot be captured")
             pieces = [training.forward_rows(self, x[b0:b0 + rows]) for b0 in range(0, B, rows)]
             return (pieces[0] if len(pieces) == 1 else torch.cat(pieces)), None
         if return_geometry:
