@@ -14,10 +14,17 @@
 //
 // Warps: W softmax warpgroups that take the streamed tiles in turn, one warp that issues the
 // products, one for the TMA loads.  One's exponentials run beside the products of another's tile:
-// head dims above 64 have W = 2 in a CTA (TMEM: S and G of two tiles, 4 x 64 columns, and the
-// accumulators, 2 x 128: an SM's 512); up to 64 a CTA has W = 1 in 256 columns and 80 KB, and two
-// run on an SM, so that one's start and end overlap the other's work too (256 x 512 x 48:
-// 114 us with W = 2).  CTAs with the longest walks, of all chains, start first.
+// head dims above 64 have W = 2 in a CTA (TMEM: S and G of two tiles, 4 x 64 columns, and 2 x 128 of
+// accumulators: an SM's 512); up to 64 a CTA has W = 1 in 256 columns and 80 KB, and two run on an
+// SM, so that one's start and end overlap the other's work too (256 x 512 x 48: 114 us with W = 2,
+// 80 so).  CTAs with the longest walks, of all chains, start first.
+//
+// Measured: 16 x 4096 x 96 188 us (0.69 PFLOP/s of the five products), 96 x 2048 x 120 415 us (0.58).
+// A tile takes about 1475 cycles for keys and 1345 for queries, of which the tensor core is busy 910
+// and 730: the rest is the softmax's chain (TMEM loads, exponentials, stores and hand-overs, 2000
+// cycles a tile over two warpgroups); and a CTA's start and end, about 8000 cycles, which with W = 2
+// nothing overlaps.  Own tiles in TMEM (their products 30 cycles instead of 46), a third S and G, P and
+// dS in columns of their own, the second half's TMEM loads ahead: no gain.
 #include "hoa_attn_bwd.cuh"
 #include "hoa_f32x2.cuh"
 #include "hoa_tma.cuh"
@@ -39,7 +46,13 @@ struct BwLayout {
   static constexpr int offBar = offCol + W * 2 * 128 * 4;
   static constexpr int kAlloc = offBar + 256 + 1024;
   static_assert(kAlloc <= 232448, "shared memory budget");
-  static constexpr uint32_t kAcc = W == 1 ? 64 : 128, colA0 = 128 * W, colA1 = colA0 + kAcc, kCols = 256 * W;
+  static constexpr uint32_t kCols = 256 * W;
+  // TMEM of a role: S and G of NB tiles, then the accumulators (keys: A0 and A1)
+  template <bool kKeys> struct Role {
+    static constexpr int NB = W;      // (a third one for queries, whose columns allow it: 187 us for 188, and 434 for 415)
+    static constexpr uint32_t colA0 = 128 * NB, colA1 = colA0 + (kKeys ? DP : 0);
+    static_assert(colA1 + DP <= kCols, "TMEM columns");
+  };
 };
 
 HOA_DEVICE float bw_exp2(float x) {
@@ -58,7 +71,8 @@ struct BwMaps { CUtensorMap x0, x1, y0, y1; };
 template <int DP, bool kKeys>
 HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
   using L = BwLayout<DP>;
-  constexpr int W = L::W;
+  using Role = typename L::template Role<kKeys>;
+  constexpr int W = L::W, NB = Role::NB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float* cols = reinterpret_cast<float*>(sm + L::offCol);
@@ -66,8 +80,8 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
   uint64_t* own_full = bars;
   uint64_t* full = bars + 1;         // [NS]
   uint64_t* empty = full + L::NS;    // [NS]
-  uint64_t* s_full = empty + L::NS;  // [W]
-  uint64_t* p_full = s_full + W;     // [W]
+  uint64_t* s_full = empty + L::NS;  // [NB] S and G are there
+  uint64_t* p_full = s_full + NB;    // [W] P and dS are there
   uint64_t* fin = p_full + W;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(fin + 2);
@@ -138,7 +152,7 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
         tc_fence_after();
         const uint32_t st = base + L::offStage + s * L::kStage;
         const uint64_t dY0 = desc_sw128(st), dY1 = desc_sw128(st + L::kStr);
-        const uint32_t cS = tm + (j % W) * 128;
+        const uint32_t cS = tm + (j % NB) * 128;
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {                        // (in turn: one's sums do not wait for the other's)
           const uint64_t ox = (uint64_t)(((kk >> 2) * L::kOwnBlk + (kk & 3) * 32) >> 4);
@@ -146,23 +160,25 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
           mma_bf16_warp(cS, dX0 + ox, dY0 + oy, idS, kk > 0 ? 1u : 0u, lead);
           mma_bf16_warp(cS + 64, dX1 + ox, dY1 + oy, idS, kk > 0 ? 1u : 0u, lead);
         }
-        tc_commit_warp(&s_full[j % W], lead);
+        tc_commit_warp(&s_full[j % NB], lead);
       };
       ok = __all_sync(0xffffffffu, ok);
-      front(0);
+      // (S and G of tile j + NB - 1 go where those of tile j - 1 were: behind the products that read P and dS there)
+      constexpr int kAhead = NB - 1;
+      for (int j = 0; j < min(kAhead, n); ++j) front(j);
       for (int j = 0; j < n && ok; ++j) {
-        if (W > 1 && j + 1 < n) front(j + 1);
+        if (j + kAhead < n && (kAhead > 0 || j == 0)) front(j + kAhead);
         ok = __all_sync(0xffffffffu, ok && mbar_wait_abortable(&p_full[j % W], (j / W) & 1, s_abort, p.max_wait));
         if (!ok) break;
         tc_fence_after();
         const uint32_t st = base + L::offStage + (j % L::NS) * L::kStage;
         const uint64_t mY0 = desc_sw128_mn(st, L::kStrBlk), mY1 = desc_sw128_mn(st + L::kStr, L::kStrBlk);
-        const uint32_t cS = tm + (j % W) * 128;
+        const uint32_t cS = tm + (j % NB) * 128;
 #pragma unroll
         for (int kk = 0; kk < kBwStr / 16; ++kk) {
           if (kKeys)
-            mma_bf16_ts_warp(tm + L::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
-          mma_bf16_ts_warp(tm + L::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
+            mma_bf16_ts_warp(tm + Role::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
+          mma_bf16_ts_warp(tm + Role::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
         }
         tc_commit_warp(&empty[j % L::NS], lead);
         if (W == 1 && j + 1 < n) front(j + 1);                     // (over P and dS, behind the products that read them)
@@ -177,31 +193,32 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
     const int g = warp >> 2;                                      // takes the tiles g, g + W, ...
     const int r = tid & 127;                                      // row of the own tile = TMEM lane
     const uint32_t lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t cS = tmem + lane + g * 128;
     constexpr float kLog2e = 1.4426950408889634f;
     const float c = p.scale * kLog2e;
     const long long qrow = (long long)chain * p.Tq;
+    // (the scaling by -log2 e and -1 waits until the value is used: the load is on its way a tile long)
     // rows that are not there: exp2 of -infinity
-    auto stat = [&](const float* x, int q, float past, float f) { return q < p.Tq ? x[qrow + q] * f : past; };
+    auto stat = [&](const float* x, int q, float past) { return q < p.Tq ? x[qrow + q] : past; };
     float my_l = 0.f, my_D = 0.f, next = 0.f;
     if (kKeys) {
       const int q = (first + g) * kBwStr + (r & 63);
-      if (g < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
+      if (g < n) next = r < 64 ? stat(p.lse, q, INFINITY) : stat(p.delta, q, 0.f);
     } else {
-      my_l = stat(p.lse, own0 + r, -INFINITY, -kLog2e);
-      my_D = stat(p.delta, own0 + r, 0.f, -1.f);
+      my_l = -kLog2e * stat(p.lse, own0 + r, INFINITY);
+      my_D = -stat(p.delta, own0 + r, 0.f);
     }
     for (int j = g; j < n; j += W) {
       const int t0 = (first + j) * kBwStr;
       float* col = cols + (g * 2 + ((j / W) & 1)) * 128;
       if (kKeys) {
-        col[r] = next;
+        col[r] = next * (r < 64 ? -kLog2e : -1.f);
         named_sync(1 + g, 128);
         const int q = t0 + W * kBwStr + (r & 63);
-        if (j + W < n) next = r < 64 ? stat(p.lse, q, -INFINITY, -kLog2e) : stat(p.delta, q, 0.f, -1.f);
+        if (j + W < n) next = r < 64 ? stat(p.lse, q, INFINITY) : stat(p.delta, q, 0.f);
       }
-      bad |= !mbar_wait_abortable(&s_full[g], (j / W) & 1, s_abort, p.max_wait);
+      bad |= !mbar_wait_abortable(&s_full[j % NB], (j / NB) & 1, s_abort, p.max_wait);
       tc_fence_after();
+      const uint32_t cS = tmem + lane + (j % NB) * 128;
       // columns of this row that count: keys, its own key up to the query; queries, keys up to its own
       int lo = 0, hi = kBwStr;
       if (kKeys) lo = own0 + r - p.q_offset - t0; else hi = p.q_offset + own0 + r - t0 + 1;
@@ -265,7 +282,7 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
       const int c16 = i % kC;
       float v[16];
       if (n > 0) {
-        tmem_ld16(tmem + lane + (is_dv ? L::colA0 : L::colA1) + 16 * c16, v);
+        tmem_ld16(tmem + lane + (is_dv ? Role::colA0 : Role::colA1) + 16 * c16, v);
         tmem_wait_ld();
         tmem_touch(v);
       } else {
