@@ -511,16 +511,18 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
   const uint64_t rK[2] = {desc_sw128(base), desc_sw128(base + L::kMatR)};
   const uint64_t vN[2] = {desc_sw128_mn(base + L::offV, L::kSlabV), desc_sw128_mn(base + L::offV + L::kMatV, L::kSlabV)};
   constexpr uint32_t idN = make_idesc(0, 128, L::ND, true), idK = make_idesc(0, 128, L::ND, false);
-  auto issue = [&](bool left_R, bool right_R) {
+  // hi_only: one of the three products alone, 2^-11 of the result off
+  auto issue = [&](bool left_R, bool right_R, bool hi_only = false) {
     if (warp != 0 || !elect_one() || bad) return;
     tc_fence_after();
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int a = pass == 1, b = pass == 0;                       // hi lo, lo hi, hi hi
+      if (pass < 2 && hi_only) continue;
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
         const uint64_t kk = (uint64_t)(((k >> 2) * L::kSlabR + (k & 3) * 32) >> 4);
-        const uint32_t acc = pass > 0 || k > 0 ? 1u : 0u;
+        const uint32_t acc = k > 0 || (pass == 1 || (pass == 2 && !hi_only)) ? 1u : 0u;
         const uint64_t rd = right_R ? rK[b] + kk : vN[b] + (uint64_t)(k * 2048 >> 4);
         if (left_R) mma_bf16(tmem + L::colD, rK[a] + kk, rd, idN, acc);
         else mma_bf16_ts(tmem + L::colD, tmem + (a ? L::colLo : L::colHi) + 8 * k, rd, right_R ? idK : idN, acc);
@@ -752,12 +754,16 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
     for (int w = 0; w < PP; ++w) wq[w] = sum_of(red, w);
     for (int k = 1;; ++k) {
       // (while the product runs) the norm above which another term is needed, of each position; Chebyshev: a number of terms
-      float need[PP];
+      // and the one below which the next product may do with its high parts: V_{k+1}, at most x / (k + 2) of V_k, is then
+      // below 2^-12.5 of W, and 2^-11 sqrt 2 of it below 2^-23
+      float need[PP], fine[PP];
       if (k > 1) {
 #pragma unroll
         for (int w = 0; w < PP; ++w) {
           const float rr = s_x[w] / (float)(k + 2), left = rr / (1.f - rr);
-          need[w] = s_terms[w] > 0 ? (k < s_terms[w] ? -1.f : INFINITY) : k >= 64 ? INFINITY : rr >= 1.f ? -1.f : 5.7e-14f * wq[w] / (left * left);
+          const bool cheb = s_terms[w] > 0;
+          need[w] = cheb ? (k < s_terms[w] ? -1.f : INFINITY) : k >= 64 ? INFINITY : rr >= 1.f ? -1.f : 5.7e-14f * wq[w] / (left * left);
+          fine[w] = cheb ? -1.f : 2.98e-8f * wq[w] / (rr * rr);
         }
       }
       wait();
@@ -820,19 +826,23 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
         }
         put_right(c, x);
       }
-      {
+      if (k > 1) {
         const float2 v = f2_get(vv);
         const float sum = warp_sum(v.x + v.y);
         if (lid == 0) red[(k & 1) * 32 + warp] = sum;
       }
       publish();
       __syncthreads();
-      bool more = k == 1;                                           // (the first check comes with the second term)
+      bool more = k == 1, hi_only = k > 1;                          // (the first check comes with the second term)
       if (k > 1)
 #pragma unroll
-        for (int w = 0; w < PP; ++w) more |= sum_of(red + (k & 1) * 32, w) > need[w];
+        for (int w = 0; w < PP; ++w) {
+          const float sum = sum_of(red + (k & 1) * 32, w);
+          more |= sum > need[w];
+          hi_only &= sum <= fine[w];
+        }
       if (!more) break;
-      issue(false, false);
+      issue(false, false, hi_only);
     }
     // ---- da: M by rows through shared memory, its upper triangle in the generators' layout to global memory
     {
