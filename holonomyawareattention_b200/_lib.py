@@ -83,7 +83,7 @@ SIGNATURES = {
                               c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_ll, c_int, c_void_p] + [c_int] * 5
                       + [c_void_p] * 2),
     "hoa_attn_fwd_lse": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_float] + [c_int] * 5 + [c_void_p] * 2),
-    "hoa_attn_bwd_workspace_bytes": (c_size_t, [c_int] * 2),
+    "hoa_attn_bwd_workspace_bytes": (c_size_t, [c_int] * 6),
     "hoa_attn_bwd": (c_int, [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_float] + [c_int] * 5
                      + [c_void_p, c_size_t, c_void_p, c_void_p]),
     "hoa_path_bwd_workspace_bytes": (c_size_t, [c_int] * 5),

@@ -10,8 +10,7 @@
 // the other side, so every sum has one owner and a fixed order, and no atomics; S and dP
 // are computed twice (7 products instead of 5).
 //
-// This file: the dispatch, D, and the form with every product in fp32 on the CUDA cores
-// (fp32 inputs, and bf16 ones whose head dim the tensor-core form does not take).
+// This file: the dispatch, D, and the form for fp32, every product in fp32 on the CUDA cores.
 #include "hoa_attn_bwd.cuh"
 
 namespace hoa {
@@ -27,12 +26,13 @@ template <int DA> struct AbCfg {
   static constexpr size_t kSmem = (4 * kTile + 2 * kP + 2 * kAbT) * sizeof(float);
 };
 
-// 64 rows from `row0` of x (rows, d) -> registers, zero outside (kVec: fp32, d % 4 == 0, 16-byte boundaries) -> tile
+// 64 rows from `row0` of x (rows, d) -> registers, zero outside (kVec: d % 4 == 0, 16-byte boundaries) -> tile
 template <int DA> struct AbRegs {
   static constexpr int N4 = DA / 4, K = kAbT * N4 / kAbThreads;      // float4s of a thread
   float4 v[K];
   template <bool kVec>
-  HOA_DEVICE void load(const void* x, int dtype, long long base, int row0, int rows, int d) {
+  HOA_DEVICE void load(const void* px, long long base, int row0, int rows, int d) {
+    const float* x = reinterpret_cast<const float*>(px);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int i = threadIdx.x + k * kAbThreads, r = row0 + i / N4, e = i % N4 * 4;
@@ -40,12 +40,12 @@ template <int DA> struct AbRegs {
       if (r >= rows || e >= d) continue;
       const long long at = base + (long long)r * d + e;
       if (kVec) {
-        v[k] = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(x) + at);
+        v[k] = *reinterpret_cast<const float4*>(x + at);
       } else {
-        v[k].x = load_elem(x, at, dtype);
-        if (e + 1 < d) v[k].y = load_elem(x, at + 1, dtype);
-        if (e + 2 < d) v[k].z = load_elem(x, at + 2, dtype);
-        if (e + 3 < d) v[k].w = load_elem(x, at + 3, dtype);
+        v[k].x = x[at];
+        if (e + 1 < d) v[k].y = x[at + 1];
+        if (e + 2 < d) v[k].z = x[at + 2];
+        if (e + 3 < d) v[k].w = x[at + 3];
       }
     }
   }
@@ -143,12 +143,12 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
   AbRegs<DA> r0, r1;
   float stat = 0.f;                                                // threads 0-63: lse, 64-127: D, of the streamed queries
   auto load_keys = [&](int t) {
-    r0.template load<kVec>(p.k, p.dtype, kbase, t * kAbT, p.Tk, d);
-    r1.template load<kVec>(p.v, p.dtype, kbase, t * kAbT, p.Tk, d);
+    r0.template load<kVec>(p.k, kbase, t * kAbT, p.Tk, d);
+    r1.template load<kVec>(p.v, kbase, t * kAbT, p.Tk, d);
   };
   auto load_queries = [&](int t) {
-    r0.template load<kVec>(p.q, p.dtype, qbase, t * kAbT, p.Tq, d);
-    r1.template load<kVec>(p.dout, p.dtype, qbase, t * kAbT, p.Tq, d);
+    r0.template load<kVec>(p.q, qbase, t * kAbT, p.Tq, d);
+    r1.template load<kVec>(p.dout, qbase, t * kAbT, p.Tq, d);
     const int q = t * kAbT + (tid & 63);
     if (tid < 128) stat = q < p.Tq ? (tid < 64 ? p.lse : p.delta)[(long long)chain * p.Tq + q] : 0.f;
   };
@@ -220,7 +220,7 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
   const int rows = kKeys ? p.Tk : p.Tq;
   const long long base = kKeys ? kbase : qbase;
   const bool is_dv = kKeys && half == 0;
-  void* out = kKeys ? (is_dv ? p.dv : p.dk) : p.dq;
+  float* out = reinterpret_cast<float*>(kKeys ? (is_dv ? p.dv : p.dk) : p.dq);
 #pragma unroll
   for (int a = 0; a < 8; ++a) {
     const int r = own * kAbT + 8 * ty8 + a;
@@ -228,7 +228,7 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
       const int e = tx + 16 * c;
-      if (e < d) store_elem(out, base + (long long)r * d + e, p.dtype, acc[a][c] * (is_dv ? 1.f : p.scale));
+      if (e < d) out[base + (long long)r * d + e] = acc[a][c] * (is_dv ? 1.f : p.scale);
     }
   }
 }
@@ -291,15 +291,23 @@ template <int DA>
 static int launch_both(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   uintptr_t at = 0;
   for (const void* x : {a.q, a.k, a.v, a.dout}) at |= reinterpret_cast<uintptr_t>(x);
-  return a.dtype == HOA_F32 && a.d % 4 == 0 && (at & 15) == 0 ? launch_sides<DA, true>(a, BH, s) : launch_sides<DA, false>(a, BH, s);
+  return a.d % 4 == 0 && (at & 15) == 0 ? launch_sides<DA, true>(a, BH, s) : launch_sides<DA, false>(a, BH, s);
 }
 
 }  // namespace hoa
 
 using namespace hoa;
 
-extern "C" size_t hoa_attn_bwd_workspace_bytes(int BH, int Tq) {
-  return BH < 1 || Tq < 1 ? 0 : (size_t)BH * Tq * sizeof(float);
+// D, and for bf16 rows that the tensor-core form takes through copies (`direct` 0) those
+static size_t ab_bytes(int BH, int Tq, int Tk, int d, int dtype, bool direct, size_t* copies_at) {
+  const size_t D = ((size_t)BH * Tq * sizeof(float) + 255) / 256 * 256;
+  *copies_at = D;
+  return D + (dtype == HOA_BF16 && !(direct && d % 8 == 0) ? attn_bwd_tc_bytes(BH, Tq, Tk, d) : 0);
+}
+
+extern "C" size_t hoa_attn_bwd_workspace_bytes(int BH, int Tq, int Tk, int d, int dtype, int aligned) {
+  size_t at;
+  return BH < 1 || Tq < 1 || Tk < 1 || d < 1 ? 0 : ab_bytes(BH, Tq, Tk, d, dtype, aligned != 0, &at);
 }
 
 extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, const float* o, const float* lse, const void* dout,
@@ -310,7 +318,11 @@ extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, cons
   if (q_offset < 0 || (long long)q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
   if ((dtype != HOA_F32 && dtype != HOA_BF16) || d > 128 || BH > 65535) return HOA_ERR_UNSUPPORTED;
   if (Tk > 0x7fffff00) return HOA_ERR_UNSUPPORTED;                   // (tile starts are counted with ints)
-  if (workspace_bytes < hoa_attn_bwd_workspace_bytes(BH, Tq)) return HOA_ERR_WORKSPACE;
+  uintptr_t at = 0;                                                  // TMA and the outputs' 16-byte stores
+  for (const void* x : {qh, kh, vh, dout, (const void*)dq, (const void*)dk, (const void*)dv}) at |= reinterpret_cast<uintptr_t>(x);
+  size_t copies_at;
+  const size_t need = ab_bytes(BH, Tq, Tk, d, dtype, (at & 15) == 0, &copies_at);
+  if (workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0) return HOA_ERR_WORKSPACE;
   AttnBwdArgs a{qh, kh, vh, o, lse, dout, reinterpret_cast<float*>(workspace), dq, dk, dv, dtype, softmax_scale, Tq, Tk, q_offset, d,
                 status, wait_bound_cycles()};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -320,9 +332,8 @@ extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, cons
   if (d % 8 == 0 && (od & 15) == 0) attn_bwd_delta_kernel<true><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
   else attn_bwd_delta_kernel<false><<<(unsigned)((rows + 31) / 32), 256, 0, s>>>(a, rows);
   if (int st = launch_status()) return st;
-  uintptr_t at = 0;                                                  // TMA and the outputs' 16-byte stores
-  for (const void* x : {qh, kh, vh, dout, (const void*)dq, (const void*)dk, (const void*)dv}) at |= reinterpret_cast<uintptr_t>(x);
-  if (dtype == HOA_BF16 && d % 8 == 0 && (at & 15) == 0) return attn_bwd_tc(a, BH, s);
+  if (dtype == HOA_BF16)
+    return attn_bwd_tc(a, BH, need > copies_at ? reinterpret_cast<unsigned char*>(workspace) + copies_at : nullptr, s);
   switch ((d + 15) / 16) {
     case 1: return launch_both<16>(a, BH, s);
     case 2: return launch_both<32>(a, BH, s);

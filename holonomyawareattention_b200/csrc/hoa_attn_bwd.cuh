@@ -1,4 +1,4 @@
-// Arguments of the attention's backward pass, shared by its two forms.
+// Arguments of the attention's backward pass, shared by its two forms (bf16, fp32).
 #pragma once
 
 #include "hoa_common.cuh"
@@ -17,7 +17,9 @@ struct AttnBwdArgs {
   long long max_wait;                               // bound of a wait, SM cycles (wait_bound_cycles())
 };
 
-// the tcgen05 form (hoa_attn_bwd_tc.cu): bf16, d % 8 == 0, every tensor from a 16-byte boundary; delta is there
-int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s);
+// The tcgen05 form (hoa_attn_bwd_tc.cu) for bf16; delta is there.  copies: attn_bwd_tc_bytes of scratch where d % 8 != 0
+// or a tensor does not start at a 16-byte boundary, else null.
+size_t attn_bwd_tc_bytes(int BH, int Tq, int Tk, int d);
+int attn_bwd_tc(const AttnBwdArgs& a, int BH, void* copies, cudaStream_t s);
 
 }  // namespace hoa

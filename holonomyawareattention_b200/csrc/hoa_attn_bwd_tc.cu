@@ -50,6 +50,10 @@ struct BwLayout {
   // TMEM of a role: S and G of NB tiles, then the accumulators (keys: A0 and A1)
   template <bool kKeys> struct Role {
     static constexpr int NB = W;      // (a third one for queries, whose columns allow it: 187 us for 188, and 434 for 415)
+    // dS is rounded to bf16 as an operand, 2^-8 of a term at most.  With few columns the terms of dq cancel (the ds of a row
+    // sum to 0, and its keys' shares along so few directions are alike), and the rounding would be 1.55 of dq's own: there dS
+    // is taken in two bf16 parts.
+    static constexpr bool kSplit = !kKeys && DP <= 32;
     static constexpr uint32_t colA0 = 128 * NB, colA1 = colA0 + (kKeys ? DP : 0);
     static_assert(colA1 + DP <= kCols, "TMEM columns");
   };
@@ -179,6 +183,7 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
           if (kKeys)
             mma_bf16_ts_warp(tm + Role::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
           mma_bf16_ts_warp(tm + Role::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
+          if (Role::kSplit) mma_bf16_ts_warp(tm + Role::colA1, cS + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, 1u, lead);
         }
         tc_commit_warp(&empty[j % L::NS], lead);
         if (W == 1 && j + 1 < n) front(j + 1);                     // (over P and dS, behind the products that read them)
@@ -257,11 +262,16 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
             const float2 z = f2_get(f2_fma(f2(s[i], s[i + 1]), f2(c), l[k]));
             const F2 pr = f2(bw_exp2(z.x), bw_exp2(z.y));
             if (kKeys) pk[i / 2] = bw_pack(pr);
-            dk[i / 2] = bw_pack(f2_mul(pr, f2_add(f2(gr[i], gr[i + 1]), D[k])));
+            const F2 ds = f2_mul(pr, f2_add(f2(gr[i], gr[i + 1]), D[k]));
+            dk[i / 2] = bw_pack(ds);
+            if (Role::kSplit) {                                     // what the rounding left, over S's first half (P's place for keys)
+              const uint32_t u = __float_as_uint(dk[i / 2]);
+              pk[i / 2] = bw_pack(f2_fma(f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), f2(-1.f), ds));
+            }
           }
         }
         // (16 columns over the first half of S, which is in registers; the second half lies behind them)
-        if (kKeys) tmem_st16(cS + 16 * half, pk);
+        if (kKeys || Role::kSplit) tmem_st16(cS + 16 * half, pk);
         tmem_st16(cS + 64 + 16 * half, dk);
       }
       tmem_wait_st();
@@ -337,7 +347,7 @@ static int launch_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   return launch_early(attn_bwd_tc_kernel<DP>, dim3((unsigned)BH, (unsigned)tiles, 2), 1, L::kThreads, L::kAlloc, s, m[0], m[1], a);
 }
 
-int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
+static int attn_bwd_tc_of(const AttnBwdArgs& a, int BH, cudaStream_t s) {
   switch ((a.d + 15) / 16) {
     case 1: return launch_bwd_tc<16>(a, BH, s);
     case 2: return launch_bwd_tc<32>(a, BH, s);
@@ -348,6 +358,68 @@ int attn_bwd_tc(const AttnBwdArgs& a, int BH, cudaStream_t s) {
     case 7: return launch_bwd_tc<112>(a, BH, s);
     default: return launch_bwd_tc<128>(a, BH, s);
   }
+}
+
+// Rows of d elements <-> rows of d8 = d rounded up to 8, zeros behind; a thread 8 elements, blockIdx.y the tensor.
+struct BwCopy { const void* src[4]; void* dst[4]; long long rows[4]; int d, d8; };
+
+template <bool kPad>
+__global__ void __launch_bounds__(256) attn_bwd_copy_kernel(const __grid_constant__ BwCopy p) {
+  const int per = p.d8 / 8, t = blockIdx.y;
+  const long long n = p.rows[t] * per;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const long long row = i / per;
+    const int e = (int)(i - row * per) * 8;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    unsigned short* u = reinterpret_cast<unsigned short*>(&w);
+    if (kPad) {
+      const unsigned short* src = reinterpret_cast<const unsigned short*>(p.src[t]) + row * p.d + e;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e + k < p.d) u[k] = src[k];
+      reinterpret_cast<uint4*>(p.dst[t])[i] = w;
+    } else {
+      w = reinterpret_cast<const uint4*>(p.src[t])[i];
+      unsigned short* dst = reinterpret_cast<unsigned short*>(p.dst[t]) + row * p.d + e;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (e + k < p.d) dst[k] = u[k];
+    }
+  }
+}
+
+static size_t bw_up(size_t v) { return (v + 255) / 256 * 256; }
+
+size_t attn_bwd_tc_bytes(int BH, int Tq, int Tk, int d) {
+  const size_t row = (size_t)(d + 7) / 8 * 16;
+  return 3 * bw_up((size_t)BH * Tq * row) + 4 * bw_up((size_t)BH * Tk * row);
+}
+
+int attn_bwd_tc(const AttnBwdArgs& a, int BH, void* copies, cudaStream_t s) {
+  if (copies == nullptr) return attn_bwd_tc_of(a, BH, s);
+  // rows that TMA does not take (d % 8 != 0, or tensors off 16-byte boundaries) go through copies of rounded-up rows: the zeros
+  // behind change no product.  2 x 1500 x 50: 230 us on the CUDA cores.
+  const int d8 = (a.d + 7) / 8 * 8;
+  const long long q = (long long)BH * a.Tq, k = (long long)BH * a.Tk;
+  unsigned char* at = reinterpret_cast<unsigned char*>(copies);
+  auto take = [&](long long rows) {
+    void* x = at;
+    at += bw_up((size_t)rows * d8 * 2);
+    return x;
+  };
+  AttnBwdArgs b = a;
+  BwCopy in{{a.q, a.dout, a.k, a.v}, {take(q), take(q), take(k), take(k)}, {q, q, k, k}, a.d, d8};
+  BwCopy out{{take(q), take(k), take(k)}, {a.dq, a.dk, a.dv}, {q, k, k}, a.d, d8};
+  b.q = in.dst[0]; b.dout = in.dst[1]; b.k = in.dst[2]; b.v = in.dst[3];
+  b.dq = const_cast<void*>(out.src[0]); b.dk = const_cast<void*>(out.src[1]); b.dv = const_cast<void*>(out.src[2]);
+  b.d = d8;
+  const long long ctas = (k * (d8 / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(ctas < 4096 ? ctas : 4096);
+  attn_bwd_copy_kernel<true><<<dim3(grid, 4), 256, 0, s>>>(in);
+  if (int st = launch_status()) return st;
+  if (int st = attn_bwd_tc_of(b, BH, s)) return st;
+  attn_bwd_copy_kernel<false><<<dim3(grid, 3), 256, 0, s>>>(out);
+  return launch_status();
 }
 
 }  // namespace hoa

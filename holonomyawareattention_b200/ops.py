@@ -1116,7 +1116,8 @@ def attn_bwd(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, o: torch.Tens
     _like(lse, "lse", (BH, Tq), torch.float32, idx)
     _like(do, "do", (BH, Tq, d), qh.dtype, idx)
     dq, dk, dv = torch.empty_like(qh), torch.empty_like(kh), torch.empty_like(vh)
-    nb = _bytes_of("hoa_attn_bwd_workspace_bytes", BH, Tq)
+    at = qh.data_ptr() | kh.data_ptr() | vh.data_ptr() | do.data_ptr() | dq.data_ptr() | dk.data_ptr() | dv.data_ptr()
+    nb = _bytes_of("hoa_attn_bwd_workspace_bytes", BH, Tq, Tk, d, code, int(at % 16 == 0))
     ws = _scratch(idx, nb)
     _run(idx, "hoa_attn_bwd", qh.data_ptr(), kh.data_ptr(), vh.data_ptr(), o.data_ptr(), lse.data_ptr(), do.data_ptr(), code,
          dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), softmax_scale, BH, Tq, Tk, q_offset, d, ws[0], nb)

@@ -470,9 +470,11 @@ int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, 
  * q^, k^, v^, dout and the three outputs are `dtype`, o and lse fp32; every output is written in full
  * (keys that no query sees: 0).  Sums have a fixed order: two calls give the same bits.  A NaN or
  * infinity in a position's k^ or v^ may also reach, as 0 times it, queries that do not see it.  d <= 128,
- * B*H <= 65535.  `status` may receive HOA_ERR_TIMEOUT.
+ * B*H <= 65535.  The workspace is 256-byte aligned; `aligned`: q^, k^, v^, dout and the outputs all start at
+ * 16-byte boundaries (bf16 otherwise, and with d % 8 != 0, goes through copies).  `status` may receive
+ * HOA_ERR_TIMEOUT.
  */
-size_t hoa_attn_bwd_workspace_bytes(int BH, int Tq);
+size_t hoa_attn_bwd_workspace_bytes(int BH, int Tq, int Tk, int d, int dtype, int aligned);
 int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, const float* o, const float* lse, const void* dout,
                  int dtype, void* dq, void* dk, void* dv, float softmax_scale, int BH, int Tq, int Tk, int q_offset,
                  int d, void* workspace, size_t workspace_bytes, int* status, void* stream);

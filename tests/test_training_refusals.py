@@ -38,7 +38,11 @@ def test_attn_bwd_abi():
     assert attn_bwd(Tk=2 ** 31 - 1) == UNSUPPORTED
     assert attn_bwd(ws=8) == WORKSPACE
     lib = _lib.load()
-    assert lib.hoa_attn_bwd_workspace_bytes(3, 5) == 60 and lib.hoa_attn_bwd_workspace_bytes(0, 5) == 0
+    f = lib.hoa_attn_bwd_workspace_bytes
+    assert f(3, 5, 9, 16, _lib.HOA_F32, 0) == f(3, 5, 9, 16, _lib.HOA_BF16, 1) == 256 and f(0, 5, 9, 16, _lib.HOA_F32, 1) == 0
+    # copies of 3 + 4 tensors, rows of 24 for 20, each from a 256-byte boundary
+    assert f(3, 5, 9, 20, _lib.HOA_BF16, 1) == 256 + 3 * 768 + 4 * 1536 and f(3, 5, 9, 16, _lib.HOA_BF16, 0) > 256
+    assert attn_bwd(d=20, ws=1024) == WORKSPACE
     assert lib.hoa_attn_fwd_lse(P, P, P, _lib.HOA_F32, P, None, 0.1, 1, 1, 1, 0, 8, None, None) == INVALID
     assert lib.hoa_attn_fwd_lse(P, P, P, 9, P, P, 0.1, 1, 1, 1, 0, 8, None, None) == UNSUPPORTED
 
