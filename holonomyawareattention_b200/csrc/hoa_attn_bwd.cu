@@ -127,8 +127,10 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
   float* dS = P + C::kP;
   float* lse = dS + C::kP;
   float* D = lse + kAbT;
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
-  const int half = tid / 128, ty8 = tid % 128 / 16;
+  // a warp has 4 x 8 of the 16 x 16 threads of the first products: its 16-byte loads meet 4 and 8 different rows (2 and 16
+  // with rows of 16 threads)
+  const int tid = threadIdx.x, ty = tid / 64 * 4 + tid % 32 / 8, tx = tid % 64 / 32 * 8 + tid % 8;
+  const int half = tid / 128, ty8 = tid % 128 / 16, tx16 = tid % 16;
   const int chain = blockIdx.x, d = p.d;                             // (all chains' longest walks first)
   const int nq = (p.Tq + kAbT - 1) / kAbT, nk = (p.Tk + kAbT - 1) / kAbT;
   const long long qbase = (long long)chain * p.Tq * d, kbase = (long long)chain * p.Tk * d;
@@ -196,8 +198,8 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
         }
       }
     __syncthreads();
-    if (kKeys) ab_tn<DA>(half ? dS : P, half ? Q : dO, 0, kAbT, ty8, tx, acc);
-    else ab_tn<DA>(dS, K, half * (kAbT / 2), (half + 1) * (kAbT / 2), ty8, tx, acc);
+    if (kKeys) ab_tn<DA>(half ? dS : P, half ? Q : dO, 0, kAbT, ty8, tx16, acc);
+    else ab_tn<DA>(dS, K, half * (kAbT / 2), (half + 1) * (kAbT / 2), ty8, tx16, acc);
     __syncthreads();
   }
 
@@ -208,14 +210,14 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
 #pragma unroll
       for (int a = 0; a < 8; ++a)
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) X[(8 * ty8 + a) * C::kLd + tx + 16 * c] = acc[a][c];
+        for (int c = 0; c < CPT; ++c) X[(8 * ty8 + a) * C::kLd + tx16 + 16 * c] = acc[a][c];
     }
     __syncthreads();
     if (half) return;
 #pragma unroll
     for (int a = 0; a < 8; ++a)
 #pragma unroll
-      for (int c = 0; c < CPT; ++c) acc[a][c] += X[(8 * ty8 + a) * C::kLd + tx + 16 * c];
+      for (int c = 0; c < CPT; ++c) acc[a][c] += X[(8 * ty8 + a) * C::kLd + tx16 + 16 * c];
   }
   const int rows = kKeys ? p.Tk : p.Tq;
   const long long base = kKeys ? kbase : qbase;
@@ -227,7 +229,7 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
     if (r >= rows) continue;
 #pragma unroll
     for (int c = 0; c < CPT; ++c) {
-      const int e = tx + 16 * c;
+      const int e = tx16 + 16 * c;
       if (e < d) out[base + (long long)r * d + e] = acc[a][c] * (is_dv ? 1.f : p.scale);
     }
   }

@@ -398,7 +398,7 @@ size_t attn_bwd_tc_bytes(int BH, int Tq, int Tk, int d) {
 int attn_bwd_tc(const AttnBwdArgs& a, int BH, void* copies, cudaStream_t s) {
   if (copies == nullptr) return attn_bwd_tc_of(a, BH, s);
   // rows that TMA does not take (d % 8 != 0, or tensors off 16-byte boundaries) go through copies of rounded-up rows: the zeros
-  // behind change no product.  2 x 1500 x 50: 230 us on the CUDA cores.
+  // behind change no product.  2 x 1500 x 50: 39 us, 8 of them the copies.
   const int d8 = (a.d + 7) / 8 * 8;
   const long long q = (long long)BH * a.Tq, k = (long long)BH * a.Tk;
   unsigned char* at = reinterpret_cast<unsigned char*>(copies);

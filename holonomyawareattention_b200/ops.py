@@ -1213,6 +1213,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
             _like(exp_avg[i], f"exp_avg[{i}]", p.shape, moment, idx)
             _like(exp_avg_sq[i], f"exp_avg_sq[{i}]", p.shape, moment, idx)
     sizes = [p.numel() for p in params]
+    if len({p.data_ptr() for p, k in zip(params, sizes) if k}) != sum(1 for k in sizes if k):
+        raise ValueError("params must be different tensors: the step of one is not a place for another's")
     if masters is not None:
         for i, p in enumerate(params):
             _like(masters[i], f"masters[{i}]", p.shape, torch.float32, idx)

@@ -188,7 +188,7 @@ class AdamW(torch.optim.Optimizer):
             for (dev, _, _, n, masters), items in calls.items():
                 ps, gs, ss = zip(*items)
                 ops.adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
-                               torch.full((1,), n + 1, dtype=torch.int32, device=dev), lr=group["lr"], betas=group["betas"],
+                               torch.full((1,), n + 1, dtype=torch.int32, device=dev), lr=float(group["lr"]), betas=group["betas"],
                                eps=group["eps"], weight_decay=group["weight_decay"], masters=[s["master"] for s in ss] if masters else None,
                                scales=[s["scales"] for s in ss] if group["state_bits"] == 8 else None)
                 for s in ss:

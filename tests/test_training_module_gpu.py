@@ -147,6 +147,28 @@ def test_other_stream_and_accumulation():
     assert torch.equal(m.qkv.weight.grad, once)
 
 
+def test_checkpointed_layers():
+    """Two layers, each recomputed in the backward pass (torch.utils.checkpoint): the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    layers = [module(64, 4, torch.bfloat16, 0.1, seed=i) for i in (10, 11)]
+    x = torch.randn(2, 40, 64, device=DEV).to(torch.bfloat16).requires_grad_()
+
+    def run(wrap):
+        y = x
+        for m in layers:
+            y = y + wrap(lambda t, m=m: m(t, attn_mask=tril(40))[0], y)
+        y.float().square().sum().backward()
+        grads = [x.grad] + [p.grad for m in layers for p in m.parameters() if p.grad is not None]
+        x.grad = None
+        for m in layers:
+            m.zero_grad()
+        return grads
+
+    plain = run(lambda f, y: f(y))
+    again = run(lambda f, y: checkpoint(f, y, use_reentrant=False))
+    assert len(plain) == len(again) == 13 and all(torch.equal(a, b) for a, b in zip(plain, again))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_train_step_is_torch_adamw(dtype):
     m = module(64, 4, dtype, 0.1, seed=6)

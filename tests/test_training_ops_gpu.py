@@ -440,6 +440,8 @@ def test_adamw_refusals():
     with pytest.raises(ValueError, match="scales"):
         q = [torch.zeros(8, device=DEV).to(torch.float8_e4m3fn)]
         ops.adamw_step(x, x, q, q, step, lr=0.1, scales=[torch.zeros(2, 2, device=DEV)])
+    with pytest.raises(ValueError, match="different"):
+        ops.adamw_step(x * 2, x * 2, x * 2, x * 2, step, lr=0.1)
     with pytest.raises(ValueError, match="betas"):
         ops.adamw_step(x, x, x, x, step, lr=0.1, betas=(1.0, 0.9))
     with pytest.raises(NotImplementedError, match="dtype"):
