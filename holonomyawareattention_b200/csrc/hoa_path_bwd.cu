@@ -14,7 +14,8 @@
 // The closing edge t = T - 1 is on no path: its gradient is 0.
 //
 // P_t = R_t C_k as the forward left them.  The sums run in the chunk's frame, Y = C Z C^T,
-// so that W = R Y R^T takes R alone.  Four kernels, over runs of at most 32 positions:
+// so that W = R Y R^T takes R alone.  Four kernels, over runs of 32 positions (of 8 in
+// short sequences, which have few: 8 chains of 128, d = 48, take 71 us so and 84 in runs of 32):
 //   sums    S_run = sum over the run of skew(X^T Y)               (one CTA a run)
 //   suffix  S_run <- sum of all later runs                        (fp64, one thread an entry)
 //   scan    Y_t for every position of a run, from its last one back (one CTA a run)
@@ -24,7 +25,7 @@
 namespace hoa {
 using namespace sm100;
 
-constexpr int kPbRun = 32;
+constexpr int kPbRun = 32, kPbRunMin = 8, kPbShort = 256;      // positions of a run, of one in sequences up to kPbShort
 
 struct PathBwdArgs {
   const float* a; int banked, stride; const float* a_bias; float edge_scale;
@@ -35,9 +36,9 @@ struct PathBwdArgs {
   float* da; void* dqkv; int out_dtype;
   int B, H, T, d;
   float* S;                                                    // (BH, NR, d, d)
-  float* Y; float* F;                                          // of a group of runs: (runs, kPbRun, d, d), (runs, kPbRun, 3, d)
+  float* Y; float* F;                                          // of a group of runs: (runs, run, d, d), (runs, run, 3, d)
   float4* V;                                                   // two old iterates a CTA (main, large norms)
-  long long run0; int runs;                                    // the group
+  long long run0; int runs, run, run_log;                      // the group, positions of a run
   int vec4;                                                    // rows of R, Y and the vectors from 16-byte (bf16: 8-byte) boundaries
   int* status;
   long long max_wait;
@@ -50,8 +51,8 @@ HOA_DEVICE PbRun pb_run(const PathBwdArgs& p, long long r) {
   x.chain = (int)(r / p.NR);
   const int i = (int)(r - (long long)x.chain * p.NR);
   x.k = i / p.rpc;
-  x.t0 = x.k * p.chunk + (i - x.k * p.rpc) * kPbRun;
-  x.t1 = min(min(x.t0 + kPbRun, (x.k + 1) * p.chunk), p.T);
+  x.t0 = x.k * p.chunk + (i - x.k * p.rpc) * p.run;
+  x.t1 = min(min(x.t0 + p.run, (x.k + 1) * p.chunk), p.T);
   return x;
 }
 
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_sums_kernel(const __grid_
 
 // S_r <- sum of S_{r'} over the chain's later runs r' > r
 __global__ void __launch_bounds__(256) path_bwd_suffix_kernel(const __grid_constant__ PathBwdArgs p, long long entries) {
+  wait_previous();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= entries) return;
   const long long dd = (long long)p.d * p.d;
@@ -233,6 +235,7 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_
   const int tid = threadIdx.x, d = p.d;
   const long long run = p.run0 + blockIdx.x;
   const PbRun r = pb_run(p, run);
+  wait_previous();
   if (r.t0 >= r.t1) return;
   const float* Cg = p.C + ((long long)r.chain * p.K + r.k) * d * d;
   const float* Zg = p.S + run * d * d;
@@ -263,13 +266,13 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_
     pb_vectors<DP>(p, r.chain, tb, n, X, kLd);
     __syncthreads();
     pb_nt<DP, 4>(X, C, X);                                 // the vectors in the chunk's frame
-    float* F = p.F + ((long long)blockIdx.x * kPbRun + (tb - r.t0)) * 3 * d;
+    float* F = p.F + ((long long)blockIdx.x * p.run + (tb - r.t0)) * 3 * d;
     for (int i = tid; i < n * 3 * d; i += kPsThreads) {
       const int e = i % d, w = i / d % 3, j = i / (3 * d);
       F[i] = X[(8 * j + 4 + w) * kLd + e];
     }
     for (int i = n - 1; i >= 0; --i) {
-      pb_store<DP>(Y, p.Y + ((long long)blockIdx.x * kPbRun + (tb + i - r.t0)) * d * d, d);
+      pb_store<DP>(Y, p.Y + ((long long)blockIdx.x * p.run + (tb + i - r.t0)) * d * d, d);
       pb_add<DP>(X, kLd, i, Y);
     }
   }
@@ -299,6 +302,14 @@ __global__ void __launch_bounds__(kPsThreads) path_bwd_scan_kernel(const __grid_
 //            V_{k-2} added, gamma_k = (2 - [k = 0]) / x * integral of J_k over [0, x]
 //            = (2 - [k = 0]) / x * 2 sum_m J_{k + 2m + 1}(x), the Bessel functions by Miller's
 //            backward recurrence in fp64; about x + 15 products.  x <= kPbMaxX, else NaN.
+//
+// What bounds it: the chain of a position's dependent products and the element work between them
+// (d = 96: 61.6K cycles with one CTA on the SM, 66K each with two; the schedulers issue 35-40%, the tensor pipe
+// is busy 21%).  Two CTAs are what registers (128 a thread: M, a matrix being loaded and a chunk being
+// split), 256 TMEM columns and 106 KB allow.  Measured, all four kernels: 65536 positions of 96 8.5 ms,
+// 131072 of 48 6.2, 24000 of 120 6.15 (plain: 169, 49, 93).  Not kept: the next pass's matrices loaded ahead
+// or the next chunk's TMEM loads (spills; 10.6 to 13 ms at d = 96), 3 or 4 warpgroups at 96 (10.3),
+// products issued by a whole warp with uniform descriptors (its registers spill the rest: 13.8).
 // ---------------------------------------------------------------------------
 constexpr float kPbR = 256.f, kPbA = 16.f;
 constexpr int kPbCoef = 640;
@@ -334,7 +345,7 @@ template <int DP> struct PbLayout {
   static constexpr uint32_t colD = 0, colHi = ND, colLo = ND + DP / 2;
   static constexpr int kGen = (kDim * (kDim - 1) / 2 + kDim / 2 + NT - 1) / NT;
   static constexpr int kScratch = 2 * NCG * 4 * NT;                // float4s of a CTA's old iterates
-  static_assert(NT <= 1024 && kPbRun % PP == 0, "a pass stays in its run");
+  static_assert(NT <= 1024 && kPbRunMin % PP == 0, "a pass stays in its run");
 };
 
 // gamma_k (k >= 0) for x, and how many terms they need
@@ -562,12 +573,14 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
     return v;
   };
 
+  wait_previous();
   float4* scratch = p.V + (long long)blockIdx.x * L::kScratch + tid;
-  const long long passes = (long long)p.runs * (kPbRun / PP);
+  constexpr int kLogPP = PP == 4 ? 2 : PP == 2 ? 1 : 0;
+  const long long passes = ((long long)p.runs << p.run_log) / PP;
   for (long long u = blockIdx.x; u < passes; u += gridDim.x) {
-    const long long lr = u / (kPbRun / PP);
+    const long long lr = u >> (p.run_log - kLogPP);
     const PbRun r = pb_run(p, p.run0 + lr);
-    const int t = r.t0 + (int)(u - lr * (kPbRun / PP)) * PP;
+    const int t = r.t0 + (int)(u - (lr << (p.run_log - kLogPP))) * PP;
     if (t >= r.t1) continue;                                        // (block-uniform)
     const int live = min(PP, r.t1 - t);
     const int b = r.chain / p.H, h = r.chain - b * p.H;
@@ -908,7 +921,7 @@ path_bwd_kernel(const __grid_constant__ PathBwdArgs p) {
 
 // ---------------------------------------------------------------------------
 struct PbPlan {
-  int rpc, K, NR;
+  int rpc, K, NR, run_log;
   long long group;                                     // runs of one pass of scan and main
   size_t off_Y, off_F, off_V, bytes;
 };
@@ -941,18 +954,21 @@ static size_t pb_scratch_of(int d, int sms) {
 static bool pb_plan(int B, int H, int T, int d, int chunk, int sms, PbPlan& x) {
   if (B < 1 || H < 1 || T < 1 || d < 2 || d > 120 || chunk < 1 || sms < 1) return false;
   x.K = (int)(((long long)T + chunk - 1) / chunk);
-  x.rpc = ((chunk < T ? chunk : T) + kPbRun - 1) / kPbRun;
+  // (by the length alone: a sequence's gradients are the same bits in a batch of any size)
+  const int run = T <= kPbShort ? kPbRunMin : kPbRun;
+  x.run_log = T <= kPbShort ? 3 : 5;
+  x.rpc = ((chunk < T ? chunk : T) + run - 1) / run;
   const long long NR = (long long)x.K * x.rpc, runs = NR * B * H;
   if ((long long)B * H > 0x7fffffff || NR > 0x7fffffff || runs > 0x7fffffff || (long long)T + chunk > 0x7fffff00) return false;
   x.NR = (int)NR;
   const size_t dd = (size_t)d * d * sizeof(float);
-  x.group = (long long)((1ull << 30) / (dd * kPbRun));
+  x.group = (long long)((1ull << 30) / (dd * run));
   if (x.group < 1) x.group = 1;
   if (x.group > runs) x.group = runs;
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   x.off_Y = up((size_t)runs * dd);
-  x.off_F = x.off_Y + up((size_t)x.group * kPbRun * dd);
-  x.off_V = x.off_F + up((size_t)x.group * kPbRun * 3 * d * sizeof(float));
+  x.off_F = x.off_Y + up((size_t)x.group * run * dd);
+  x.off_V = x.off_F + up((size_t)x.group * run * 3 * d * sizeof(float));
   x.bytes = x.off_V + pb_scratch_of(d, sms);
   return true;
 }
@@ -967,16 +983,13 @@ static int launch_path_bwd(PathBwdArgs a, const PbPlan& x, int sms, cudaStream_t
   if ((entries + 255) / 256 > 0x7fffffff) return HOA_ERR_UNSUPPORTED;
   path_bwd_sums_kernel<DP><<<(unsigned)runs, kPsThreads, 0, s>>>(a);
   if (int st = launch_status()) return st;
-  path_bwd_suffix_kernel<<<(unsigned)((entries + 255) / 256), 256, 0, s>>>(a, entries);
-  if (int st = launch_status()) return st;
+  if (int st = launch_early(path_bwd_suffix_kernel, (unsigned)((entries + 255) / 256), 1, 256, 0, s, a, entries)) return st;
   for (long long r = 0; r < runs; r += x.group) {
     a.run0 = r;
     a.runs = (int)(runs - r < x.group ? runs - r : x.group);
-    path_bwd_scan_kernel<DP><<<(unsigned)a.runs, kPsThreads, PbScan<DP>::kSmem, s>>>(a);
-    if (int st = launch_status()) return st;
-    const long long passes = (long long)a.runs * (kPbRun / L::PP), most = (long long)sms * L::kMinBlocks;
-    path_bwd_kernel<DP><<<(unsigned)(passes < most ? passes : most), L::NT, L::kAlloc, s>>>(a);
-    if (int st = launch_status()) return st;
+    if (int st = launch_early(path_bwd_scan_kernel<DP>, (unsigned)a.runs, 1, kPsThreads, PbScan<DP>::kSmem, s, a)) return st;
+    const long long passes = ((long long)a.runs << x.run_log) / L::PP, most = (long long)sms * L::kMinBlocks;
+    if (int st = launch_early(path_bwd_kernel<DP>, (unsigned)(passes < most ? passes : most), 1, L::NT, L::kAlloc, s, a)) return st;
   }
   return HOA_OK;
 }
@@ -1012,7 +1025,7 @@ extern "C" int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias
   PathBwdArgs p{a_all, gen_is_banked(a_dtype) ? 1 : 0, stride, a_bias, edge_scale, R, C, chunk, x.K, x.rpc, x.NR,
                 {qh, kh, vh}, o, {dqh, dkh, dvh, doh}, hat_dtype, da, dqkv, out_dtype, B, H, T, d,
                 reinterpret_cast<float*>(ws), reinterpret_cast<float*>(ws + x.off_Y), reinterpret_cast<float*>(ws + x.off_F),
-                reinterpret_cast<float4*>(ws + x.off_V), 0, 0, vec4, status, wait_bound_cycles()};
+                reinterpret_cast<float4*>(ws + x.off_V), 0, 0, 1 << x.run_log, x.run_log, vec4, status, wait_bound_cycles()};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   switch ((d + 15) / 16) {
     case 1: return launch_path_bwd<16>(p, x, sms, s);
