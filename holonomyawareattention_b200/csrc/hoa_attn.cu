@@ -230,7 +230,7 @@ extern "C" int hoa_attn_fwd(const void* qh, const void* kh, const void* vh, int 
 
 extern "C" int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, float* o, float* lse,
                                 float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, int* status, void* stream) {
-  if (!lse) return HOA_ERR_INVALID_ARG;
+  if (!lse || !(softmax_scale > 0.f && softmax_scale < INFINITY)) return HOA_ERR_INVALID_ARG;   // (masked scores: scale * -infinity)
   // the tensor-core form takes rows of whole 16-byte pieces (TMA), from 16-byte boundaries
   const bool aligned = ((reinterpret_cast<uintptr_t>(qh) | reinterpret_cast<uintptr_t>(kh) | reinterpret_cast<uintptr_t>(vh)) & 15) == 0;
   if (dtype == HOA_BF16 && d % 8 == 0 && d <= 128 && aligned)

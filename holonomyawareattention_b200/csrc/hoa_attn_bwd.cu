@@ -318,6 +318,7 @@ extern "C" int hoa_attn_bwd(const void* qh, const void* kh, const void* vh, cons
   if (!qh || !kh || !vh || !o || !lse || !dout || !dq || !dk || !dv || !workspace || BH < 1 || Tq < 1 || Tk < 1 || d < 1)
     return HOA_ERR_INVALID_ARG;
   if (q_offset < 0 || (long long)q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (!(softmax_scale > 0.f && softmax_scale < INFINITY)) return HOA_ERR_INVALID_ARG;   // (masked scores are scale * -infinity)
   if ((dtype != HOA_F32 && dtype != HOA_BF16) || d > 128 || BH > 65535) return HOA_ERR_UNSUPPORTED;
   if (Tk > 0x7fffff00) return HOA_ERR_UNSUPPORTED;                   // (tile starts are counted with ints)
   uintptr_t at = 0;                                                  // TMA and the outputs' 16-byte stores

@@ -1073,7 +1073,7 @@ def _like(t, name, shape, dtype, idx) -> None:
         raise ValueError(f"{name} must be a contiguous {tuple(shape)} {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
 
 
-def _attn_shapes(qh, kh, vh, q_offset):
+def _attn_shapes(qh, kh, vh, q_offset, softmax_scale):
     """(device index, dtype code, BH, Tq, Tk, d) of causal attention's inputs, checked."""
     idx = _index(qh)
     code = _dtype_code(qh.dtype)
@@ -1086,6 +1086,8 @@ def _attn_shapes(qh, kh, vh, q_offset):
     _like(vh, "v^", (BH, Tk, d), qh.dtype, idx)
     if q_offset < 0 or q_offset + Tq > Tk:
         raise ValueError(f"the queries q_offset .. q_offset + Tq = {q_offset} .. {q_offset + Tq} must lie in the {Tk} keys")
+    if not 0.0 < softmax_scale < math.inf:
+        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     if d > 128:
         raise NotImplementedError(f"head dim {d} (at most 128)")
     if BH > 65535 or Tk >= 2 ** 31 - 256:
@@ -1096,7 +1098,7 @@ def _attn_shapes(qh, kh, vh, q_offset):
 def attn_fwd_lse(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, softmax_scale: float, q_offset: int = 0):
     """attn_fwd for training: (o (BH,Tq,d) fp32, lse (BH,Tq) fp32), lse the log-sum-exp of each row's scaled
     scores; bf16 (v^ row-major here) runs on the tensor cores where d % 8 == 0.  hoa_attn_fwd_lse."""
-    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset)
+    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset, softmax_scale)
     o = qh.new_empty((BH, Tq, d), dtype=torch.float32)
     lse = qh.new_empty((BH, Tq), dtype=torch.float32)
     _run(idx, "hoa_attn_fwd_lse", qh.data_ptr(), kh.data_ptr(), vh.data_ptr(), code, o.data_ptr(), lse.data_ptr(), softmax_scale,
@@ -1111,7 +1113,7 @@ def attn_bwd(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, o: torch.Tens
     q^ (BH,Tq,d), k^ and v^ (BH,Tk,d), do and the results share a type (fp32 or bf16); o and lse are what
     attn_fwd_lse gave.  The probabilities are recomputed from lse; sums are fp32 and of a fixed order.
     hoa_attn_bwd."""
-    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset)
+    idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset, softmax_scale)
     _like(o, "o", (BH, Tq, d), torch.float32, idx)
     _like(lse, "lse", (BH, Tq), torch.float32, idx)
     _like(do, "do", (BH, Tq, d), qh.dtype, idx)

@@ -458,7 +458,8 @@ int hoa_path_step(const float* a, int a_dtype, const float* a_bias, float edge_s
  *
  * hoa_attn_fwd_lse - hoa_attn_fwd that also leaves lse (B*H, Tq) fp32, the log-sum-exp of a row's scaled
  * scores, which the backward pass recomputes the probabilities from; v^ row-major.  bf16 with d % 8 == 0
- * runs on tcgen05, the rest in fp32 on the CUDA cores; d <= 128.
+ * runs on tcgen05, the rest in fp32 on the CUDA cores; d <= 128.  softmax_scale is positive and finite, here
+ * and in hoa_attn_bwd.
  */
 int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, float* o, float* lse,
                      float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, int* status, void* stream);

@@ -47,6 +47,15 @@ def test_attn_bwd_abi():
     assert lib.hoa_attn_fwd_lse(P, P, P, 9, P, P, 0.1, 1, 1, 1, 0, 8, None, None) == UNSUPPORTED
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.25, float("inf"), float("-inf"), float("nan")])
+def test_softmax_scale(scale):
+    """A masked score is -infinity times the scale: only a positive, finite one leaves it masked."""
+    lib = _lib.load()
+    for dtype in (_lib.HOA_F32, _lib.HOA_BF16):
+        assert lib.hoa_attn_fwd_lse(P, P, P, dtype, P, P, scale, 1, 1, 1, 0, 8, None, None) == INVALID
+        assert lib.hoa_attn_bwd(P, P, P, P, P, P, dtype, P, P, P, scale, 1, 1, 1, 0, 8, P, 1 << 20, None, None) == INVALID
+
+
 def path_bwd(a_dtype=_lib.HOA_F32, chunk=4, hat=_lib.HOA_F32, out=_lib.HOA_F32, B=1, H=2, T=8, d=8, ws=1 << 40, a=P, wsp=P):
     return _lib.load().hoa_path_bwd(a, a_dtype, None, 0.1, P, P, chunk, P, P, P, P, P, P, P, P, hat, P, P, out, B, H, T, d, wsp, ws, None, None)
 
