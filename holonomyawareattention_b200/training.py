@@ -210,10 +210,12 @@ _TRIL = {}
 
 
 def _tril(L: int, device) -> torch.Tensor:
-    m = _TRIL.get(device)
+    """The causal mask, kept for the next step on the same stream (another stream would have to wait for it)."""
+    key = device, torch.cuda.current_stream(device).cuda_stream if device.type == "cuda" else 0
+    m = _TRIL.get(key)
     if m is None or m.shape[0] != L:
         with torch.inference_mode(False):
-            m = _TRIL[device] = torch.ones(L, L, dtype=torch.bool, device=device).tril()
+            m = _TRIL[key] = torch.ones(L, L, dtype=torch.bool, device=device).tril()
     return m
 
 
@@ -221,7 +223,9 @@ def train_step(attn, x: torch.Tensor, optimizer, loss: Callable[[torch.Tensor], 
                max_grad_norm: Optional[float] = None) -> torch.Tensor:
     """One step: y = attn(x) under the causal mask (``attn_mask``, default tril), loss(y), gradients (their norm held to
     ``max_grad_norm``, if given), the optimizer's step.  Gradients start and end at None.  Returns the loss, detached, on the
-    device; nothing waits for the GPU."""
+    device; nothing waits for the GPU.  Not under graph capture."""
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise NotImplementedError("train_step cannot be captured into a graph")
     L = x.shape[1]
     if attn_mask is None:
         attn_mask = _tril(L, x.device)

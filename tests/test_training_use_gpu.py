@@ -5,7 +5,7 @@ import threading
 import pytest
 import torch
 
-from holonomyawareattention_b200 import AdamW, PathOrderedGeometricMHA, _lib, ops
+from holonomyawareattention_b200 import AdamW, PathOrderedGeometricMHA, _lib, ops, train_step, training
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -122,6 +122,31 @@ def test_adamw_captured():
     with pytest.raises(NotImplementedError, match="captured"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             opt.step()
+
+
+def test_train_step_refuses_capture():
+    """... before it touches anything: the gradients stay, and no mask made during the capture is kept for later steps."""
+    m = PathOrderedGeometricMHA(64, n_heads=4).to(DEV)
+    opt, x = AdamW(m.parameters()), torch.randn(1, 23, 64, device=DEV)
+    m.qkv.weight.grad = g = torch.randn_like(m.qkv.weight)
+    held = dict(training._TRIL)
+    torch.cuda.synchronize()
+    with pytest.raises(NotImplementedError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            train_step(m, x, opt, lambda y: y.square().mean())
+    assert m.qkv.weight.grad is g and training._TRIL == held
+    a = train_step(m, x, opt, lambda y: y.square().mean())
+    assert bool(torch.isfinite(a))
+
+
+def test_masks_are_of_a_stream():
+    m = torch.ones(9, 9, dtype=torch.bool, device=DEV).tril()
+    one = training._tril(9, m.device)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        two = training._tril(9, m.device)
+        assert two is training._tril(9, m.device) and two is not one
+    torch.cuda.synchronize()
+    assert one is training._tril(9, m.device) and torch.equal(one, m) and torch.equal(two, m)
 
 
 def test_forward_with_gradients_refuses_capture():
