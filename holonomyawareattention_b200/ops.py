@@ -109,7 +109,7 @@ class _StatusWatch:
         st = int(self.mapped[0])
         if st != 0:
             self.mapped[0] = 0
-            _lib.check("a cache operation", st)
+            _lib.check("a cache or training operation", st)
         while self.pending and self.pending[0][1].query():
             slot, _, what = self.pending.popleft()
             st = int(self.host[slot])

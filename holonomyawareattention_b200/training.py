@@ -114,7 +114,7 @@ def edge_generators(attn, x: torch.Tensor):
         return attn.gqproj(x).float() + attn.gkproj(partner).float(), "packed"
     pair = torch.cat([x, partner], dim=-1)
     if x.dtype == torch.float32:
-        return attn.edge_mlp(pair), "packed"
+        return attn.edge_mlp(pair).float(), "packed"             # (under autocast the linears' results are bf16)
     layout = attn._gen_layout()
     lin0, lin2 = attn.edge_mlp[0], attn.edge_mlp[2]
     w1t, b1f = attn._w1t()

@@ -8,7 +8,7 @@ heads and y; their gradients back to qkv; the generators', the hidden layer's tw
 import pytest
 import torch
 
-from holonomyawareattention_b200 import AdamW, PathOrderedGeometricMHA, ops, train_step
+from holonomyawareattention_b200 import AdamW, PathOrderedGeometricMHA, ops, train_step, training
 from oracle import torch_ref
 
 pytestmark = pytest.mark.gpu
@@ -145,6 +145,27 @@ def test_other_stream_and_accumulation():
         m(x, attn_mask=tril(40))[0].sum().backward()
     s.synchronize()
     assert torch.equal(m.qkv.weight.grad, once)
+
+
+def test_autocast():
+    """fp32 weights, bf16 linears: what the core region is given then gives the same bits without autocast."""
+    m = module(96, 3, torch.float32, seed=9)
+    x, w = torch.randn(2, 50, 96, device=DEV), torch.randn(2, 50, 96, device=DEV)
+    with torch.autocast("cuda", torch.bfloat16):
+        y, _ = m(x, attn_mask=tril(50))
+    (y * w).sum().backward()
+    got = {k: p.grad for k, p in m.named_parameters()}
+    m.zero_grad()
+    with torch.autocast("cuda", torch.bfloat16):
+        qkv, a = m.qkv(x), m.edge_mlp(torch.cat([x, torch.roll(x, -1, 1)], -1))
+    assert qkv.dtype is a.dtype is torch.bfloat16
+    heads = training.PathCore.apply(a.float(), qkv, None, m.h, m.edge_scale, m.scale, ops.plan_chunk(2, m.h, 50, m.d, x.device), "packed")
+    with torch.autocast("cuda", torch.bfloat16):
+        z = m.out(heads)
+    (z * w).sum().backward()
+    assert y.dtype is torch.bfloat16 and torch.equal(y, z)
+    for k, p in m.named_parameters():
+        assert (got[k] is None and p.grad is None) or (torch.equal(got[k], p.grad) and bool(p.grad.any())), k
 
 
 def test_checkpointed_layers():
