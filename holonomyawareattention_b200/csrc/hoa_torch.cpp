@@ -1,7 +1,7 @@
-// The ordinary case of the generation operators' host side (ops.py: pages_reserve, pages_fork,
-// pages_free, pages_compact, paged_attn_fwd, path_step), for calls whose time on the GPU is a few
-// microseconds: the same checks, allocations and library call as the Python functions, without their
-// 10 us of interpreter.  Anything that is not ordinary - a wrong type, shape, device or stride, another
+// The ordinary case of the generation and training operators' host side (ops.py: pages_reserve, pages_fork,
+// pages_free, pages_compact, paged_attn_fwd, path_step; attn_fwd_lse, attn_bwd, path_bwd, adamw_step), for
+// calls whose time on the GPU is a few microseconds: the same checks, allocations and library call as the Python
+// functions, without their 10 to 30 us of interpreter.  Anything that is not ordinary - a wrong type, shape, device or stride, another
 // current device - returns None before anything is allocated or launched, and the Python function takes
 // the call: its errors are the ones a user sees.  A status that the library returns comes back as an int.
 //
@@ -14,8 +14,11 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
 #include <map>
 #include <utility>
+#include <vector>
 
 #include "../../include/hoa.h"
 
@@ -30,7 +33,14 @@ struct Fns {
   decltype(&hoa_paged_attn_workspace_bytes) attn_ws;
   decltype(&hoa_paged_attn_fwd) attn;
   decltype(&hoa_path_step) step;
+  decltype(&hoa_attn_fwd_lse) fwd_lse;
+  decltype(&hoa_attn_bwd_workspace_bytes) attn_bwd_ws;
+  decltype(&hoa_attn_bwd) attn_bwd;
+  decltype(&hoa_path_bwd_workspace_bytes) path_bwd_ws;
+  decltype(&hoa_path_bwd) path_bwd;
+  decltype(&hoa_adamw_step) adamw;
 } g_fn{};
+constexpr int kFns = sizeof(Fns) / sizeof(void*);
 
 struct Device { int sms = 0; int* status = nullptr; };
 constexpr int kMaxDevices = 64;
@@ -128,9 +138,9 @@ PyObject* status(int st) { return PyLong_FromLong(st); }
 
 // ---------------------------------------------------------------------------
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 8) { PyErr_SetString(PyExc_TypeError, "bind takes 8 addresses"); return nullptr; }
+  if (n != kFns) { PyErr_Format(PyExc_TypeError, "bind takes %d addresses", kFns); return nullptr; }
   void** f = reinterpret_cast<void**>(&g_fn);
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < kFns; ++i) {
     f[i] = PyLong_AsVoidPtr(a[i]);
     if (PyErr_Occurred()) return nullptr;
   }
@@ -283,6 +293,153 @@ PyObject* path_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return st ? status(st) : wrap2(out, qh);
 }
 
+// ---------------------------------------------------------------------------
+// training
+bool like(const at::Tensor* t, int idx, at::ScalarType dt, at::IntArrayRef shape) {
+  return t && t->scalar_type() == dt && t->is_cuda() && t->get_device() == idx && t->sizes() == shape && t->is_contiguous();
+}
+
+struct Attn { int idx, code, BH, Tq, Tk, d, off; float scale; cudaStream_t s; };
+bool attn(const at::Tensor* q, const at::Tensor* k, const at::Tensor* v, PyObject* scale, PyObject* off, Attn* c) {
+  if (!q || !k || q->dim() != 3 || k->dim() != 3 || q->numel() == 0 || k->numel() == 0 || !code(*q, &c->code) || !PyFloat_Check(scale) ||
+      !PyLong_Check(off))
+    return false;
+  c->idx = dev_index(*q);
+  const long long o = PyLong_AsLongLong(off);
+  if (PyErr_Occurred()) { PyErr_Clear(); return false; }
+  const int64_t BH = q->size(0), Tq = q->size(1), d = q->size(2), Tk = k->size(1);
+  if (c->idx < 0 || !like(q, c->idx, q->scalar_type(), {BH, Tq, d}) || !like(k, c->idx, q->scalar_type(), {BH, Tk, d}) ||
+      !like(v, c->idx, q->scalar_type(), {BH, Tk, d}) || Tk > 0x7fffff00 || BH > 65535 || d > 128 || o < 0 || o > Tk - Tq)
+    return false;
+  c->BH = (int)BH; c->Tq = (int)Tq; c->Tk = (int)Tk; c->d = (int)d; c->off = (int)o;
+  c->scale = (float)PyFloat_AS_DOUBLE(scale);
+  c->s = c10::cuda::getCurrentCUDAStream(c->idx).stream();
+  return c->scale > 0.f && std::isfinite(c->scale);
+}
+
+// q^, k^, v^, softmax_scale, q_offset
+PyObject* attn_fwd_lse(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Attn c;
+  if (n != 5) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]);
+  if (!attn(q, k, v, a[3], a[4], &c)) Py_RETURN_NONE;
+  const auto f32 = q->options().dtype(at::kFloat);
+  at::Tensor o = at::empty({c.BH, c.Tq, c.d}, f32), lse = at::empty({c.BH, c.Tq}, f32);
+  const int st = g_fn.fwd_lse(q->data_ptr(), k->data_ptr(), v->data_ptr(), c.code, o.data_ptr<float>(), lse.data_ptr<float>(), c.scale,
+                              c.BH, c.Tq, c.Tk, c.off, c.d, g_dev[c.idx].status, c.s);
+  return st ? status(st) : wrap2(o, lse);
+}
+
+// q^, k^, v^, o, lse, do, softmax_scale, q_offset
+PyObject* attn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  Attn c;
+  if (n != 8) Py_RETURN_NONE;
+  const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *o = tensor(a[3]), *lse = tensor(a[4]), *dy = tensor(a[5]);
+  if (!attn(q, k, v, a[6], a[7], &c) || !like(o, c.idx, at::kFloat, q->sizes()) || !like(lse, c.idx, at::kFloat, {c.BH, c.Tq}) ||
+      !like(dy, c.idx, q->scalar_type(), q->sizes()))
+    Py_RETURN_NONE;
+  at::Tensor dq = at::empty(q->sizes(), q->options()), dk = at::empty(k->sizes(), q->options()), dv = at::empty(k->sizes(), q->options());
+  uintptr_t at = 0;
+  for (const at::Tensor* t : {q, k, v, dy, (const at::Tensor*)&dq, (const at::Tensor*)&dk, (const at::Tensor*)&dv})
+    at |= reinterpret_cast<uintptr_t>(t->data_ptr());
+  const size_t nb = g_fn.attn_bwd_ws(c.BH, c.Tq, c.Tk, c.d, c.code, (at & 15) == 0);
+  const Scratch ws = scratch(*q, c.idx, c.s, nb);
+  const int st = g_fn.attn_bwd(q->data_ptr(), k->data_ptr(), v->data_ptr(), o->data_ptr<float>(), lse->data_ptr<float>(), dy->data_ptr(),
+                               c.code, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), c.scale, c.BH, c.Tq, c.Tk, c.off, c.d, ws.p, nb,
+                               g_dev[c.idx].status, c.s);
+  return st ? status(st) : wrap3(dq, dk, dv);
+}
+
+// a_all (packed, no bias), R, C, chunk, n_heads, edge_scale, hats, dhats (dqkv in q^'s type)
+PyObject* path_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  long long chunk, heads;
+  if (n != 8 || !PyFloat_Check(a[5]) || !integer(a[3], &chunk) || !integer(a[4], &heads) || !PyTuple_Check(a[6]) || !PyTuple_Check(a[7]) ||
+      PyTuple_GET_SIZE(a[6]) != 4 || PyTuple_GET_SIZE(a[7]) != 4)
+    Py_RETURN_NONE;
+  const at::Tensor *g = tensor(a[0]), *R = tensor(a[1]), *C = tensor(a[2]), *x[4], *y[4];
+  for (int i = 0; i < 4; ++i) {
+    x[i] = tensor(PyTuple_GET_ITEM(a[6], i));
+    y[i] = tensor(PyTuple_GET_ITEM(a[7], i));
+  }
+  int hat;
+  if (!g || !R || g->dim() != 3 || R->dim() != 4 || !x[0] || !code(*x[0], &hat)) Py_RETURN_NONE;
+  const int idx = dev_index(*g);
+  const int64_t B = g->size(0), T = g->size(1), H = heads, d = R->size(3);
+  if (idx < 0 || B < 1 || T < 1 || d < 2 || d > 120 || B > 0x7fffffff / H || T > 0x7fffffff) Py_RETURN_NONE;
+  chunk = std::min<long long>(chunk, T);
+  const auto dt = x[0]->scalar_type();
+  if (!like(g, idx, at::kFloat, {B, T, H * (d * (d - 1) / 2)}) || !like(R, idx, at::kFloat, {B * H, T, d, d}) ||
+      !like(C, idx, at::kFloat, {B * H, (T + chunk - 1) / chunk, d, d}))
+    Py_RETURN_NONE;
+  for (int i = 0; i < 4; ++i)
+    if (!like(x[i], idx, i < 3 ? dt : at::kFloat, {B * H, T, d}) || !like(y[i], idx, dt, {B * H, T, d})) Py_RETURN_NONE;
+  const size_t nb = g_fn.path_bwd_ws((int)B, (int)H, (int)T, (int)d, (int)chunk);
+  if (nb == 0) Py_RETURN_NONE;
+  const cudaStream_t s = c10::cuda::getCurrentCUDAStream(idx).stream();
+  at::Tensor da = at::empty(g->sizes(), g->options()), dqkv = at::empty({B, T, 3 * H * d}, x[0]->options());
+  const Scratch ws = scratch(*g, idx, s, nb);
+  const int st = g_fn.path_bwd(g->data_ptr<float>(), HOA_F32, nullptr, (float)PyFloat_AS_DOUBLE(a[5]), R->data_ptr<float>(),
+                               C->data_ptr<float>(), (int)chunk, x[0]->data_ptr(), x[1]->data_ptr(), x[2]->data_ptr(),
+                               x[3]->data_ptr<float>(), y[0]->data_ptr(), y[1]->data_ptr(), y[2]->data_ptr(), y[3]->data_ptr(), hat,
+                               da.data_ptr<float>(), dqkv.data_ptr(), hat, (int)B, (int)H, (int)T, (int)d, ws.p, nb, g_dev[idx].status, s);
+  return st ? status(st) : wrap2(da, dqkv);
+}
+
+bool sequence(PyObject* o, Py_ssize_t n) { return (PyList_Check(o) || PyTuple_Check(o)) && PySequence_Fast_GET_SIZE(o) == n; }
+
+// params, grads, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, weight_decay, masters or None, scales or None
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 12 || !(PyList_Check(a[0]) || PyTuple_Check(a[0]))) Py_RETURN_NONE;
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(a[0]);
+  const bool has_master = a[10] != Py_None, bits8 = a[11] != Py_None;
+  if (count < 1 || count > 0x7fffffff || !sequence(a[1], count) || !sequence(a[2], count) || !sequence(a[3], count) ||
+      (has_master && !sequence(a[10], count)) || (bits8 && !sequence(a[11], count)))
+    Py_RETURN_NONE;
+  double num[5];
+  for (int i = 0; i < 5; ++i) {
+    if (!PyFloat_Check(a[5 + i])) Py_RETURN_NONE;
+    num[i] = PyFloat_AS_DOUBLE(a[5 + i]);
+  }
+  if (!(num[1] >= 0.0 && num[1] < 1.0 && num[2] >= 0.0 && num[2] < 1.0 && num[3] >= 0.0)) Py_RETURN_NONE;
+  auto item = [&](int list, Py_ssize_t i) { return tensor(PySequence_Fast_GET_ITEM(a[list], i)); };
+  const at::Tensor *p0 = item(0, 0), *g0 = item(1, 0), *step = tensor(a[4]);
+  int p_code, g_code;
+  if (!p0 || !g0 || !code(*p0, &p_code) || !code(*g0, &g_code)) Py_RETURN_NONE;
+  const int idx = dev_index(*p0);
+  if (idx < 0 || !ints(step, idx, {1})) Py_RETURN_NONE;
+  const auto moment = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
+  std::vector<void*> ptr[6];                                      // params, grads, m, v, masters, scales
+  for (auto& v : ptr) v.resize(count);
+  std::vector<long long> sizes(count);
+  std::vector<void*> places;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const at::Tensor* p = item(0, i);
+    if (!p) Py_RETURN_NONE;
+    const at::Tensor *t[6] = {p, item(1, i), item(2, i), item(3, i), has_master ? item(10, i) : nullptr, bits8 ? item(11, i) : nullptr};
+    sizes[i] = p->numel();
+    if (!like(p, idx, p0->scalar_type(), p->sizes()) || !like(t[1], idx, g0->scalar_type(), p->sizes()) ||
+        !like(t[2], idx, moment, p->sizes()) || !like(t[3], idx, moment, p->sizes()) ||
+        (has_master && !like(t[4], idx, at::kFloat, p->sizes())) || (bits8 && !like(t[5], idx, at::kFloat, {2, (sizes[i] + 255) / 256})))
+      Py_RETURN_NONE;
+    for (int k = 0; k < 6; ++k) ptr[k][i] = t[k] ? t[k]->data_ptr() : nullptr;
+    if (sizes[i] > 0) places.push_back(ptr[0][i]);
+  }
+  std::sort(places.begin(), places.end());
+  if (std::adjacent_find(places.begin(), places.end()) != places.end()) Py_RETURN_NONE;
+  const int st = g_fn.adamw(ptr[0].data(), p_code, has_master ? (float* const*)ptr[4].data() : nullptr, (const void* const*)ptr[1].data(),
+                            g_code, ptr[2].data(), ptr[3].data(), bits8 ? (float* const*)ptr[5].data() : nullptr, bits8 ? 8 : 32,
+                            sizes.data(), (int)count, step->data_ptr<int>(), num[0], num[1], num[2], num[3], num[4],
+                            c10::cuda::getCurrentCUDAStream(idx).stream());
+  if (st == 0)                                                    // (what was saved of them, or laid out from them, is out of date)
+    for (Py_ssize_t i = 0; i < count; ++i)
+      for (int list : {0, 10}) {
+        if (list == 10 && !has_master) continue;
+        const at::Tensor* t = item(list, i);
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+      }
+  return status(st);
+}
+
 // No C++ exception leaves a function: an allocation that fails (out of memory) or any other error of the tensor
 // library becomes None, and the Python function meets it again with its own message.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
@@ -297,7 +454,8 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 #define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&guarded<f>)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(device), METHOD(pages_reserve), METHOD(pages_fork), METHOD(pages_free),
-                         METHOD(pages_compact), METHOD(paged_attn_fwd), METHOD(path_step), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(pages_compact), METHOD(paged_attn_fwd), METHOD(path_step), METHOD(attn_fwd_lse), METHOD(attn_bwd), METHOD(path_bwd),
+                         METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hoa_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -678,7 +678,8 @@ def _fn(name: str):
 # the call is not ordinary (another device, an option, a mistake) and that the code below takes it.
 _HOST = None
 _HOST_FNS = ("hoa_pages_workspace_bytes", "hoa_pages_reserve", "hoa_pages_fork", "hoa_pages_free", "hoa_pages_compact",
-             "hoa_paged_attn_workspace_bytes", "hoa_paged_attn_fwd", "hoa_path_step")
+             "hoa_paged_attn_workspace_bytes", "hoa_paged_attn_fwd", "hoa_path_step", "hoa_attn_fwd_lse", "hoa_attn_bwd_workspace_bytes",
+             "hoa_attn_bwd", "hoa_path_bwd_workspace_bytes", "hoa_path_bwd", "hoa_adamw_step")
 
 
 class _Declines:
@@ -693,8 +694,8 @@ def _host():
         try:
             from . import _hoa_torch as m
         except ImportError as e:
-            warnings.warn(f"_hoa_torch.so cannot be loaded ({e}): the generation operators' host side runs in Python, about 10 us "
-                          "a call slower.  Build it with `python -m holonomyawareattention_b200._build`", RuntimeWarning)
+            warnings.warn(f"_hoa_torch.so cannot be loaded ({e}): the generation and training operators' host side runs in Python, 10 "
+                          "to 30 us a call slower.  Build it with `python -m holonomyawareattention_b200._build`", RuntimeWarning)
             _HOST = _Declines()
             return _HOST
         m.bind(*(ctypes.cast(_fn(n), ctypes.c_void_p).value for n in _HOST_FNS))
@@ -1098,6 +1099,9 @@ def _attn_shapes(qh, kh, vh, q_offset, softmax_scale):
 def attn_fwd_lse(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, softmax_scale: float, q_offset: int = 0):
     """attn_fwd for training: (o (BH,Tq,d) fp32, lse (BH,Tq) fp32), lse the log-sum-exp of each row's scaled
     scores; bf16 (v^ row-major here) runs on the tensor cores where d % 8 == 0.  hoa_attn_fwd_lse."""
+    r = (_HOST or _host()).attn_fwd_lse(qh, kh, vh, softmax_scale, q_offset)
+    if r is not None:
+        return _done("hoa_attn_fwd_lse", r)
     idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset, softmax_scale)
     o = qh.new_empty((BH, Tq, d), dtype=torch.float32)
     lse = qh.new_empty((BH, Tq), dtype=torch.float32)
@@ -1113,6 +1117,9 @@ def attn_bwd(qh: torch.Tensor, kh: torch.Tensor, vh: torch.Tensor, o: torch.Tens
     q^ (BH,Tq,d), k^ and v^ (BH,Tk,d), do and the results share a type (fp32 or bf16); o and lse are what
     attn_fwd_lse gave.  The probabilities are recomputed from lse; sums are fp32 and of a fixed order.
     hoa_attn_bwd."""
+    r = (_HOST or _host()).attn_bwd(qh, kh, vh, o, lse, do, softmax_scale, q_offset)
+    if r is not None:
+        return _done("hoa_attn_bwd", r)
     idx, code, BH, Tq, Tk, d = _attn_shapes(qh, kh, vh, q_offset, softmax_scale)
     _like(o, "o", (BH, Tq, d), torch.float32, idx)
     _like(lse, "lse", (BH, Tq), torch.float32, idx)
@@ -1135,6 +1142,10 @@ def path_bwd(a_all: torch.Tensor, R: torch.Tensor, C: torch.Tensor, chunk: int, 
     gradients of the first three and P^T dout (apply_paths with transpose).  q^, k^, v^ and dhats share a type, which
     dqkv has too unless ``out_dtype`` says otherwise.  The gradient of the closing edge (t = T - 1) is 0, as the causal
     forward does not use it.  hoa_path_bwd."""
+    if a_bias is None and out_dtype is None and gen_layout == "packed":
+        r = (_HOST or _host()).path_bwd(a_all, R, C, chunk, n_heads, edge_scale, hats, dhats)
+        if r is not None:
+            return _done("hoa_path_bwd", r)
     idx = _index(a_all)
     if a_all.dim() != 3 or R.dim() != 4 or len(hats) != 4 or len(dhats) != 4:
         raise ValueError("a_all must be (B,T,H*stride), R (BH,T,d,d), hats and dhats four tensors each")
@@ -1189,6 +1200,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
     of m and of sqrt(v), in blocks of ADAMW_BLOCK elements with scales[i] (2, blocks) fp32 (value = e4m3 * scale).
     ``step``: int32 (1,) on the device, the number of this step, from 1 (read on the device: a captured step may be replayed).
     hoa_adamw_step."""
+    r = (_HOST or _host()).adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas[0], betas[1], eps, weight_decay, masters, scales)
+    if r is not None:
+        _done("hoa_adamw_step", r)
+        return
     n = len(params)
     lists = [("grads", grads), ("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)]
     lists += [(k, v) for k, v in (("masters", masters), ("scales", scales)) if v is not None]
@@ -1224,6 +1239,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
         for i, n_i in enumerate(sizes):
             _like(scales[i], f"scales[{i}]", (2, -(-n_i // ADAMW_BLOCK)), torch.float32, idx)
     with _current(idx):
+        if idx not in _DEVICES and not torch.cuda.is_current_stream_capturing():
+            _device(idx)                       # (from now on the C++ side takes such calls)
         _lib.check("hoa_adamw_step", _fn("hoa_adamw_step")(
             _pointers(params), p_code, _pointers(masters) if masters is not None else None, _pointers(grads), g_code,
             _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None, 32 if scales is None else 8,

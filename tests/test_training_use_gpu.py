@@ -248,3 +248,77 @@ def test_adamw_past_32_bits():
     for part in (slice(0, 5), slice(n - 800, n)):
         assert bool((p[part].float() == 0.75).all()) and bool((m[part].float() == 448).all()) and bool((v[part].float() == 448).all())
     assert bool((scales[0] == scales[0, 0]).all()) and abs(float(scales[0, 0]) - 0.05 / 448) < 1e-9
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_host_sides_agree(dt, monkeypatch):
+    """The C++ host side takes the ordinary calls and gives the Python functions' bits."""
+    torch.manual_seed(3)
+    B, H, T, d, chunk = 2, 3, 37, 20, 9
+    a = 0.3 * torch.randn(B, T, H * (d * (d - 1) // 2), device=DEV)
+    qkv = torch.randn(B, T, 3 * H * d, device=DEV).to(dt)
+
+    def calls():
+        R, U, M = ops.link_local(a, qkv, H, 0.5, chunk)
+        C, _ = ops.carry_scan(M)
+        q, k, v = ops.carry_apply(U, C, chunk, dt)
+        o, lse = ops.attn_fwd_lse(q[:, 5:].contiguous(), k, v, 0.2, 5)
+        do = torch.ones_like(o).to(dt)
+        back = ops.attn_bwd(q[:, 5:].contiguous(), k, v, o, lse, do, 0.2, 5)
+        oo, _ = ops.attn_fwd_lse(q, k, v, 0.2)
+        da, dqkv = ops.path_bwd(a, R, C, chunk, H, 0.5, (q, k, v, oo), (v, q, k, q))
+        out = [o, lse, *back, da, dqkv]
+        for bits in (32, 8):
+            m = torch.float32 if bits == 32 else torch.float8_e4m3fn
+            p = [qkv.clone(), qkv[0, :3, :5].clone()]
+            st = [[torch.zeros(x.shape, device=DEV).to(m) for x in p] for _ in range(2)]
+            sc = [torch.zeros(2, -(-x.numel() // 256), device=DEV) for x in p] if bits == 8 else None
+            ms = [x.float() for x in p] if dt is torch.bfloat16 else None
+            before = [x._version for x in p]
+            for i in range(2):
+                ops.adamw_step(p, [torch.cos(x) for x in p], *st, torch.full((1,), i + 1, dtype=torch.int32, device=DEV), 1e-2,
+                               weight_decay=0.1, masters=ms, scales=sc)
+            assert [x._version for x in p] == [v + 2 for v in before]
+            out += p + [x.float() for s in st for x in s] + (ms or [])
+        return out
+
+    first = calls()                                       # (introduces the device)
+    taken = []
+    host = ops._host()
+
+    class Watch:
+        def __getattr__(self, name):
+            def call(*args):
+                r = getattr(host, name)(*args)
+                taken.append((name, r is not None))
+                return r
+            return call
+
+    monkeypatch.setattr(ops, "_HOST", Watch())
+    fast = calls()
+    assert {n for n, _ in taken} == {"attn_fwd_lse", "attn_bwd", "path_bwd", "adamw_step"} and all(t for _, t in taken)
+    monkeypatch.setattr(ops, "_HOST", ops._Declines())
+    slow = calls()
+    ops.check_status()
+    assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(first, fast, slow))
+
+
+def test_host_side_declines_what_python_refuses():
+    x = torch.randn(2, 6, 16, device=DEV)
+    o, lse = ops.attn_fwd_lse(x, x, x, 0.2)
+    host = ops._host()
+    assert host.attn_fwd_lse(x, x, x, 0.2, 0) is not None
+    for bad in ((x, x, x, 0.0, 0), (x, x, x, -0.2, 0), (x, x, x, 0.2, 1), (x, x, x, 0.2, -1), (x, x, x[:1], 0.2, 0), (x.half(), x, x, 0.2, 0),
+                (x, x, x.bfloat16(), 0.2, 0), (x.cpu(), x, x, 0.2, 0), (x[:, ::2], x, x, 0.2, 0), (x[:, :0], x, x, 0.2, 0), (x, x, None, 0.2, 0)):
+        assert host.attn_fwd_lse(*bad) is None
+        assert host.attn_bwd(*bad[:3], o, lse, x, *bad[3:]) is None
+    assert host.attn_bwd(x, x, x, o, lse[:, :3], x, 0.2, 0) is None and host.attn_bwd(x, x, x, o.bfloat16(), lse, x, 0.2, 0) is None
+    p, g = torch.zeros(8, device=DEV), torch.ones(8, device=DEV)
+    m, v, n = torch.zeros(8, device=DEV), torch.zeros(8, device=DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    num = (1e-2, 0.9, 0.99, 1e-8, 0.0)
+    for bad in (([p, p], [g, g], [m, m], [v, v], n, *num, None, None), ([p], [g, g], [m], [v], n, *num, None, None),
+                ([p], [g[:4]], [m], [v], n, *num, None, None), ([p], [g], [m], [v], n.long(), *num, None, None),
+                ([p], [g], [m], [v], n, 1e-2, 1.0, 0.99, 1e-8, 0.0, None, None), ([p], [g], [m], [v], n, *num, [m.bfloat16()], None),
+                ([p], [g], [m], [v], n, *num, None, [torch.zeros(2, 1, device=DEV)]), ([p], [None], [m], [v], n, *num, None, None)):
+        assert host.adamw_step(*bad) is None
+    assert not p.any() and not m.any()
