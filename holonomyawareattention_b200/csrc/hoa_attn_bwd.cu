@@ -151,6 +151,8 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
   auto load_queries = [&](int t) {
     r0.template load<kVec>(p.q, qbase, t * kAbT, p.Tq, d);
     r1.template load<kVec>(p.dout, qbase, t * kAbT, p.Tq, d);
+  };
+  auto load_stats = [&](int t) {
     const int q = t * kAbT + (tid & 63);
     if (tid < 128) stat = q < p.Tq ? (tid < 64 ? p.lse : p.delta)[(long long)chain * p.Tq + q] : 0.f;
   };
@@ -163,8 +165,29 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
     r0.store(K);
     r1.store(V);
   };
-  if (kKeys) { load_keys(own); store_keys(); } else { load_queries(own); store_queries(); }
-  auto load = [&](int t) { if (kKeys) load_queries(t); else load_keys(t); };
+  // The kernel before, which leaves D, starts when all before it has completed, so q, k, v, do and lse are there: they are
+  // loaded while it runs (8 chains of 128, d = 48: 21.3 -> 20.5 us).
+  if (kKeys) {
+    load_keys(own);
+    store_keys();
+    if (first < last) load_queries(first);
+    wait_previous();                                               // D
+    if (first < last) load_stats(first);
+  } else {
+    load_queries(own);
+    wait_previous();
+    load_stats(own);
+    store_queries();
+    if (first < last) load_keys(first);
+  }
+  auto load = [&](int t) {
+    if (kKeys) {
+      load_queries(t);
+      load_stats(t);
+    } else {
+      load_keys(t);
+    }
+  };
 
   float acc[8][CPT];
 #pragma unroll
@@ -172,7 +195,6 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
 #pragma unroll
     for (int c = 0; c < CPT; ++c) acc[a][c] = 0.f;
 
-  if (first < last) load(first);
   for (int t = first; t < last; ++t) {
     if (!kAhead && t > first) load(t);
     if (kKeys) store_queries(); else store_keys();
@@ -238,7 +260,6 @@ HOA_DEVICE void attn_bwd_simt(const AttnBwdArgs& p) {
 // Both sides in one launch (blockIdx.z): neither waits for the other, and few tiles leave SMs to both.
 template <int DA, bool kVec>
 __global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_kernel(const __grid_constant__ AttnBwdArgs p) {
-  wait_previous();                                                 // D
   if (blockIdx.z == 0) attn_bwd_simt<DA, true, kVec>(p);
   else attn_bwd_simt<DA, false, kVec>(p);
 }
@@ -246,6 +267,7 @@ __global__ void __launch_bounds__(kAbThreads, DA <= 64 ? 2 : 1) attn_bwd_simt_ke
 // D_i = do_i . o_i, 8 lanes a row; kVec: 8 elements a load (d % 8 == 0, 16-byte boundaries).
 template <bool kVec>
 __global__ void __launch_bounds__(256) attn_bwd_delta_kernel(AttnBwdArgs p, long long rows) {
+  let_next_start();
   const long long r = (long long)blockIdx.x * 32 + threadIdx.x / 8;
   const int l = threadIdx.x & 7;
   float t = 0.f;

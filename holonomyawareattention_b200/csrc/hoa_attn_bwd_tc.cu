@@ -115,6 +115,7 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool bad = false;
+  wait_previous();                                                  // D, copied rows
 
   if (warp == 4 * W + 1) {
     // ------------------------------------------------------------------ TMA
@@ -324,7 +325,6 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
 template <int DP>
 __global__ void __launch_bounds__(BwLayout<DP>::kThreads, BwLayout<DP>::W == 1 ? 2 : 1)
 attn_bwd_tc_kernel(const __grid_constant__ BwMaps keys, const __grid_constant__ BwMaps queries, const __grid_constant__ AttnBwdArgs p) {
-  wait_previous();                                                  // D
   if (blockIdx.z == 0) attn_bwd_tc_role<DP, true>(keys, p);
   else attn_bwd_tc_role<DP, false>(queries, p);
 }

@@ -92,7 +92,8 @@ inline bool allow_smem(K kernel, size_t bytes, std::atomic<unsigned long long>& 
 
 // Programmatic dependent launch.  A kernel launched with launch_early may come up while the one before it in the
 // stream drains: its CTAs are placed and set themselves up, and wait_previous() returns once all work before it has
-// completed and is visible.  Every such kernel waits before it touches global memory, so nothing but its start moves;
+// completed and is visible.  Every such kernel waits before it touches global memory (but for inputs that were there
+// before the kernel ahead of it began), so nothing but its start moves;
 // back to back, small kernels otherwise leave about two microseconds between them.  let_next_start() (after the wait)
 // lets the next launch of the same call come up at once.
 HOA_DEVICE void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -299,6 +299,8 @@ bool like(const at::Tensor* t, int idx, at::ScalarType dt, at::IntArrayRef shape
   return t && t->scalar_type() == dt && t->is_cuda() && t->get_device() == idx && t->sizes() == shape && t->is_contiguous();
 }
 
+bool sequence(PyObject* o, Py_ssize_t n) { return (PyList_Check(o) || PyTuple_Check(o)) && PySequence_Fast_GET_SIZE(o) == n; }
+
 struct Attn { int idx, code, BH, Tq, Tk, d, off; float scale; cudaStream_t s; };
 bool attn(const at::Tensor* q, const at::Tensor* k, const at::Tensor* v, PyObject* scale, PyObject* off, Attn* c) {
   if (!q || !k || q->dim() != 3 || k->dim() != 3 || q->numel() == 0 || k->numel() == 0 || !code(*q, &c->code) || !PyFloat_Check(scale) ||
@@ -353,13 +355,12 @@ PyObject* attn_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // a_all (packed, no bias), R, C, chunk, n_heads, edge_scale, hats, dhats (dqkv in q^'s type)
 PyObject* path_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   long long chunk, heads;
-  if (n != 8 || !PyFloat_Check(a[5]) || !integer(a[3], &chunk) || !integer(a[4], &heads) || !PyTuple_Check(a[6]) || !PyTuple_Check(a[7]) ||
-      PyTuple_GET_SIZE(a[6]) != 4 || PyTuple_GET_SIZE(a[7]) != 4)
+  if (n != 8 || !PyFloat_Check(a[5]) || !integer(a[3], &chunk) || !integer(a[4], &heads) || !sequence(a[6], 4) || !sequence(a[7], 4))
     Py_RETURN_NONE;
   const at::Tensor *g = tensor(a[0]), *R = tensor(a[1]), *C = tensor(a[2]), *x[4], *y[4];
   for (int i = 0; i < 4; ++i) {
-    x[i] = tensor(PyTuple_GET_ITEM(a[6], i));
-    y[i] = tensor(PyTuple_GET_ITEM(a[7], i));
+    x[i] = tensor(PySequence_Fast_GET_ITEM(a[6], i));
+    y[i] = tensor(PySequence_Fast_GET_ITEM(a[7], i));
   }
   int hat;
   if (!g || !R || g->dim() != 3 || R->dim() != 4 || !x[0] || !code(*x[0], &hat)) Py_RETURN_NONE;
@@ -384,8 +385,6 @@ PyObject* path_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                da.data_ptr<float>(), dqkv.data_ptr(), hat, (int)B, (int)H, (int)T, (int)d, ws.p, nb, g_dev[idx].status, s);
   return st ? status(st) : wrap2(da, dqkv);
 }
-
-bool sequence(PyObject* o, Py_ssize_t n) { return (PyList_Check(o) || PyTuple_Check(o)) && PySequence_Fast_GET_SIZE(o) == n; }
 
 // params, grads, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, weight_decay, masters or None, scales or None
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
