@@ -14,6 +14,10 @@
 // The moments' operations are rounded one by one (no fused multiply-add): the new moments, and so
 // the 8-bit values, are those of the same formula written in separate fp32 operations.  The
 // update, which nothing is kept of but its sum with x, takes fast division.
+//
+// HBM bounds it: every byte is read and written once, a thread's loads come before all else.  Measured: 477 M elements,
+// bf16 with masters and 8-bit moments (16 bytes an element), 1.57 to 1.66 ms, 4.6 to 4.9 TB/s (conversions, roots and the
+// block's maxima beside the loads); 3.9 M fp32 in six tensors (28 bytes an element) 20 us, 5.4 TB/s.
 #include <cuda_fp8.h>
 
 #include <cmath>
