@@ -26,7 +26,8 @@ parameter, the backward passes in libhoa too.
 from __future__ import annotations
 
 import math
-from typing import Dict, Optional, Tuple
+import weakref
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -41,6 +42,34 @@ def _is_exact_tril(mask: Optional[torch.Tensor], L: int) -> bool:
         return False
     tril = torch.ones(L, L, dtype=torch.bool, device=mask.device).tril()
     return bool(torch.equal(mask.bool(), tril))
+
+
+class Kept:
+    """Values that follow from tensors, each kept while its tensors are what they were: in the same memory - the storage
+    itself, held weakly, as an address comes back to another tensor once the first is freed - and without an in-place write
+    that torch has counted since.  Copies and pickles of the owner start empty."""
+
+    MOST = 64
+
+    def __init__(self):
+        self._entries = {}
+
+    def __reduce__(self):
+        return Kept, ()
+
+    def of(self, slot, tensors, make):
+        """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
+        if any(t.is_inference() for t in tensors):               # (torch counts no writes of those)
+            return make()
+        key = tuple((t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors)
+        e = self._entries.get(slot)
+        if e is not None and e[0] == key and all(r() is t.untyped_storage() for r, t in zip(e[1], tensors)):
+            return e[2]
+        value = make()
+        if len(self._entries) >= self.MOST:
+            self._entries.clear()
+        self._entries[slot] = key, tuple(weakref.ref(t.untyped_storage()) for t in tensors), value
+        return value
 
 
 class PathOrderedGeometricMHA(nn.Module):
@@ -98,7 +127,7 @@ class PathOrderedGeometricMHA(nn.Module):
         self.link_mode = "interaction"
         self.generator_precision = "auto"
         self.chunk: Optional[int] = None          # None: hoa_plan_chunk decides
-        self._tril_ok: Dict[Tuple, bool] = {}
+        self._tril_ok = Kept()
 
     # ------------------------------------------------------------------
     def _check_supported(self, x: torch.Tensor, attn_mask, return_geometry: bool) -> None:
@@ -129,14 +158,7 @@ class PathOrderedGeometricMHA(nn.Module):
     def _mask_is_tril(self, mask, L: int) -> bool:
         if mask is None:
             return False
-        key = (mask.data_ptr(), tuple(mask.shape), mask.dtype, mask._version, str(mask.device))
-        ok = self._tril_ok.get(key)
-        if ok is None:
-            ok = _is_exact_tril(mask, L)
-            if len(self._tril_ok) > 64:
-                self._tril_ok.clear()
-            self._tril_ok[key] = ok
-        return ok
+        return self._tril_ok.of(("tril", L, mask.data_ptr()), (mask,), lambda: _is_exact_tril(mask, L))
 
     def edge_generators(self, x: torch.Tensor) -> torch.Tensor:
         """a_all (B, L, H*m) in fp32, unscaled: edge_mlp([x_t, x_{t+1 mod L}]), in the
