@@ -25,6 +25,7 @@ parameter, the backward passes in libhoa too.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 import weakref
 from typing import Optional
@@ -42,6 +43,14 @@ def _is_exact_tril(mask: Optional[torch.Tensor], L: int) -> bool:
         return False
     tril = torch.ones(L, L, dtype=torch.bool, device=mask.device).tril()
     return bool(torch.equal(mask.bool(), tril))
+
+
+@contextlib.contextmanager
+def _laying_out():
+    """Copies of weights are made without gradients but outside inference mode, whatever mode the call that needs them has:
+    a later one may save them for its backward pass."""
+    with torch.inference_mode(False), torch.no_grad():
+        yield
 
 
 class Kept:
@@ -298,11 +307,12 @@ class PathOrderedGeometricMHA(nn.Module):
         w = self.edge_mlp[2].weight
         key = (w.data_ptr(), w._version, w.dtype, str(w.device))
         if getattr(self, "_w2fp8_key", None) != key:
-            wr, _ = self._w2_rows(w.detach(), self.edge_mlp[2].bias.detach())
-            wf = wr.float()
-            amax = float(wf.abs().max())
-            s = 2.0 ** math.floor(math.log2(448.0 / amax)) if amax > 0 else 1.0
-            self._w2fp8 = ((wf * s).to(torch.float8_e4m3fn).contiguous(), 1.0 / (s * ops.SPLIT8_LO_SCALE))
+            with _laying_out():
+                wr, _ = self._w2_rows(w.detach(), self.edge_mlp[2].bias.detach())
+                wf = wr.float()
+                amax = float(wf.abs().max())
+                s = 2.0 ** math.floor(math.log2(448.0 / amax)) if amax > 0 else 1.0
+                self._w2fp8 = ((wf * s).to(torch.float8_e4m3fn).contiguous(), 1.0 / (s * ops.SPLIT8_LO_SCALE))
             self._w2fp8_key = key
         return self._w2fp8
 
@@ -313,10 +323,11 @@ class PathOrderedGeometricMHA(nn.Module):
         w, b = lin2.weight, lin2.bias
         key = (w.data_ptr(), w._version, b.data_ptr(), b._version, w.dtype, str(w.device), split)
         if getattr(self, "_w2cat_key", None) != key:
-            wr, br = self._w2_rows(w.detach(), b.detach())
-            wt = wr.t().to(torch.bfloat16)
-            self._w2cat = (torch.cat([wt, wt], dim=0) if split else wt).contiguous()
-            self._b2f = br.float().contiguous()
+            with _laying_out():
+                wr, br = self._w2_rows(w.detach(), b.detach())
+                wt = wr.t().to(torch.bfloat16)
+                self._w2cat = (torch.cat([wt, wt], dim=0) if split else wt).contiguous()
+                self._b2f = br.float().contiguous()
             self._w2cat_key = key
         return self._w2cat, self._b2f
 
@@ -327,7 +338,8 @@ class PathOrderedGeometricMHA(nn.Module):
         w, b = lin0.weight, lin0.bias
         key = (w.data_ptr(), w._version, b.data_ptr(), b._version, w.dtype, str(w.device))
         if getattr(self, "_w1t_key", None) != key:
-            self._w1t_cache = (w.detach().t().to(torch.bfloat16).contiguous(), b.detach().float().contiguous())
+            with _laying_out():
+                self._w1t_cache = (w.detach().t().to(torch.bfloat16).contiguous(), b.detach().float().contiguous())
             self._w1t_key = key
         return self._w1t_cache
 
@@ -337,8 +349,9 @@ class PathOrderedGeometricMHA(nn.Module):
         w, b = lin2.weight, lin2.bias
         key = (w.data_ptr(), w._version, b.data_ptr(), b._version, str(w.device))
         if getattr(self, "_w2f_key", None) != key:
-            wr, br = self._w2_rows(w.detach().float(), b.detach().float())
-            self._w2f = (wr.contiguous(), br.contiguous())
+            with _laying_out():
+                wr, br = self._w2_rows(w.detach().float(), b.detach().float())
+                self._w2f = (wr.contiguous(), br.contiguous())
             self._w2f_key = key
         return self._w2f
 
