@@ -56,25 +56,34 @@ def _laying_out():
 class Kept:
     """Values that follow from tensors, each kept while its tensors are what they were: in the same memory - the storage
     itself, held weakly, as an address comes back to another tensor once the first is freed - and without an in-place write
-    that torch has counted since.  Copies and pickles of the owner start empty."""
+    that torch has counted since.  What is made while a CUDA graph is captured is not kept (it is there when the graph runs),
+    and what a graph was given stays for as long as its owner.  Copies and pickles of the owner start empty."""
 
     MOST = 64
 
     def __init__(self):
-        self._entries = {}
+        self._entries, self._in_graphs = {}, []
 
     def __reduce__(self):
         return Kept, ()
 
+    def clear(self):
+        self._entries.clear()
+
     def of(self, slot, tensors, make):
         """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
+        capturing = tensors[0].is_cuda and torch.cuda.is_current_stream_capturing()
         if any(t.is_inference() for t in tensors):               # (torch counts no writes of those)
             return make()
         key = tuple((t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors)
         e = self._entries.get(slot)
         if e is not None and e[0] == key and all(r() is t.untyped_storage() for r, t in zip(e[1], tensors)):
+            if capturing and not any(v is e[2] for v in self._in_graphs):
+                self._in_graphs.append(e[2])
             return e[2]
         value = make()
+        if capturing:
+            return value
         if len(self._entries) >= self.MOST:
             self._entries.clear()
         self._entries[slot] = key, tuple(weakref.ref(t.untyped_storage()) for t in tensors), value
@@ -137,6 +146,7 @@ class PathOrderedGeometricMHA(nn.Module):
         self.generator_precision = "auto"
         self.chunk: Optional[int] = None          # None: hoa_plan_chunk decides
         self._tril_ok = Kept()
+        self._copies = Kept()
 
     # ------------------------------------------------------------------
     def _check_supported(self, x: torch.Tensor, attn_mask, return_geometry: bool) -> None:
@@ -251,17 +261,18 @@ class PathOrderedGeometricMHA(nn.Module):
             return "split"                        # shapes the fp8 GEMM does not take
         return mode
 
-    def _generators_of_hidden(self, h: torch.Tensor, mode: str) -> torch.Tensor:
-        """GELU and the bf16 edge MLP's second layer: h (rows, 4D) fp32 -> (rows, H*width) fp32, in the form ``mode``."""
+    def _generators_of_hidden(self, h: torch.Tensor, mode: str, layer=()) -> torch.Tensor:
+        """GELU and the bf16 edge MLP's second layer: h (rows, 4D) fp32 -> (rows, H*width) fp32, in the form ``mode``.
+        ``layer``: (weight, bias, where their copies are kept), default the module's own."""
         if mode == "split8":
             # W2 g_hi in bf16 (the bias in the epilogue), then += W2 g_lo with both operands in
             # e4m3 (hoa_edge_gelu_split8, hoa_edge_gemm_fp8_acc)
             hi, lo = ops.edge_gelu_split8(h)
             del h
-            wt, bias = self._stacked_w2t(False)
+            wt, bias = self._stacked_w2t(False, *layer)
             a = ops.edge_gemm(hi, wt, bias)
             del hi
-            w8, alpha = self._w2_fp8()
+            w8, alpha = self._w2_fp8(*layer)
             ops.edge_gemm_fp8_acc(lo, w8, a, alpha)
             return a
         split = mode != "bf16"
@@ -270,7 +281,7 @@ class PathOrderedGeometricMHA(nn.Module):
         # epilogue (hoa_edge_gemm, cuBLASLt)
         lhs = ops.edge_gelu_split(h, split)
         del h
-        wt, bias = self._stacked_w2t(split)
+        wt, bias = self._stacked_w2t(split, *layer)
         return ops.edge_gemm(lhs, wt, bias)
 
     # sequences longer than this use the split generators under "auto"
@@ -301,59 +312,72 @@ class PathOrderedGeometricMHA(nn.Module):
         sequence of L positions (None: a shard of a longer sequence)."""
         return self._generator_mode(L) != "bf16"
 
-    def _w2_fp8(self):
+    # The copies of the edge MLP's weights that the kernels read, in layouts of their own.  Forwards without gradients keep
+    # them from one to the next; one that trains the weights makes its own (training.forward) and ends what was kept, so that
+    # writes that torch does not count (an optimizer's through .data, a parametrization's) are seen too.
+    def weights_changed(self) -> None:
+        """Forget the laid-out copies of the weights.  Needed only after a write that torch does not count (through ``.data``
+        or a raw pointer) with no training forward, train(), eval() or move of the module since."""
+        self._copies.clear()
+
+    def train(self, mode: bool = True):
+        self.weights_changed()
+        return super().train(mode)
+
+    def _apply(self, fn, *args, **kwargs):
+        self.weights_changed()
+        return super()._apply(fn, *args, **kwargs)
+
+    def _w2_fp8(self, w=None, b=None, kept: Optional[Kept] = None):
         """(W2 in e4m3 (rows in the generator layout) times a power-of-two scale s, and
-        alpha = 1 / (s * ops.SPLIT8_LO_SCALE)), cached until edge_mlp.2 changes."""
-        w = self.edge_mlp[2].weight
-        key = (w.data_ptr(), w._version, w.dtype, str(w.device))
-        if getattr(self, "_w2fp8_key", None) != key:
+        alpha = 1 / (s * ops.SPLIT8_LO_SCALE))."""
+        if w is None:
+            w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+
+        def make():
             with _laying_out():
-                wr, _ = self._w2_rows(w.detach(), self.edge_mlp[2].bias.detach())
+                wr, _ = self._w2_rows(w.detach(), b.detach())
                 wf = wr.float()
                 amax = float(wf.abs().max())
                 s = 2.0 ** math.floor(math.log2(448.0 / amax)) if amax > 0 else 1.0
-                self._w2fp8 = ((wf * s).to(torch.float8_e4m3fn).contiguous(), 1.0 / (s * ops.SPLIT8_LO_SCALE))
-            self._w2fp8_key = key
-        return self._w2fp8
+                return (wf * s).to(torch.float8_e4m3fn).contiguous(), 1.0 / (s * ops.SPLIT8_LO_SCALE)
 
-    def _stacked_w2t(self, split: bool = True):
-        """([W2^T ; W2^T] (8D x m*H; W2^T alone for split=False) in bf16, the output bias in
-        fp32), cached until edge_mlp.2 changes."""
-        lin2 = self.edge_mlp[2]
-        w, b = lin2.weight, lin2.bias
-        key = (w.data_ptr(), w._version, b.data_ptr(), b._version, w.dtype, str(w.device), split)
-        if getattr(self, "_w2cat_key", None) != key:
+        return (self._copies if kept is None else kept).of("w2fp8", (w, b), make)
+
+    def _stacked_w2t(self, split: bool = True, w=None, b=None, kept: Optional[Kept] = None):
+        """([W2^T ; W2^T] (8D x m*H; W2^T alone for split=False) in bf16, the output bias in fp32)."""
+        if w is None:
+            w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+
+        def make():
             with _laying_out():
                 wr, br = self._w2_rows(w.detach(), b.detach())
                 wt = wr.t().to(torch.bfloat16)
-                self._w2cat = (torch.cat([wt, wt], dim=0) if split else wt).contiguous()
-                self._b2f = br.float().contiguous()
-            self._w2cat_key = key
-        return self._w2cat, self._b2f
+                return (torch.cat([wt, wt], dim=0) if split else wt).contiguous(), br.float().contiguous()
 
-    def _w1t(self):
-        """(W1^T (2D x 4D) in bf16, b1 in fp32) of the edge MLP's first layer, cached until
-        edge_mlp.0 changes."""
-        lin0 = self.edge_mlp[0]
-        w, b = lin0.weight, lin0.bias
-        key = (w.data_ptr(), w._version, b.data_ptr(), b._version, w.dtype, str(w.device))
-        if getattr(self, "_w1t_key", None) != key:
+        return (self._copies if kept is None else kept).of(("w2t", split), (w, b), make)
+
+    def _w1t(self, w=None, b=None, kept: Optional[Kept] = None):
+        """(W1^T (2D x 4D) in bf16, b1 in fp32) of the edge MLP's first layer."""
+        if w is None:
+            w, b = self.edge_mlp[0].weight, self.edge_mlp[0].bias
+
+        def make():
             with _laying_out():
-                self._w1t_cache = (w.detach().t().to(torch.bfloat16).contiguous(), b.detach().float().contiguous())
-            self._w1t_key = key
-        return self._w1t_cache
+                return w.detach().t().to(torch.bfloat16).contiguous(), b.detach().float().contiguous()
+
+        return (self._copies if kept is None else kept).of("w1t", (w, b), make)
 
     def _w2f32(self):
-        """(W2, b2) in fp32 with rows in the banked layout, cached until edge_mlp.2 changes."""
-        lin2 = self.edge_mlp[2]
-        w, b = lin2.weight, lin2.bias
-        key = (w.data_ptr(), w._version, b.data_ptr(), b._version, str(w.device))
-        if getattr(self, "_w2f_key", None) != key:
+        """(W2, b2) in fp32 with rows in the banked layout."""
+        w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+
+        def make():
             with _laying_out():
                 wr, br = self._w2_rows(w.detach().float(), b.detach().float())
-                self._w2f = (wr.contiguous(), br.contiguous())
-            self._w2f_key = key
-        return self._w2f
+                return wr.contiguous(), br.contiguous()
+
+        return self._copies.of("w2f32", (w, b), make)
 
     # Batch rows are independent: the forward runs over pieces of about this many
     # tokens (whole rows).  The edge-MLP GEMM and the link kernel then alternate in
@@ -377,8 +401,7 @@ class PathOrderedGeometricMHA(nn.Module):
         if self._needs_grad(x):
             if general:
                 raise NotImplementedError("PathOrderedGeometricMHA (B200): gradients need attn_mask = tril(L)")
-            pieces = [training.forward_rows(self, x[b0:b0 + rows]) for b0 in range(0, B, rows)]
-            return (pieces[0] if len(pieces) == 1 else torch.cat(pieces)), None
+            return training.forward(self, x, rows), None
         if return_geometry:
             # {"C": P (B,H,L,d,d), "H": Hol (B,H,d,d)} in x's dtype, as
             # core/attention_fast_chunked.py:175-177 returns them

@@ -106,34 +106,54 @@ def _banked_index(d: int, h: int, device) -> torch.Tensor:
     return i
 
 
-def edge_generators(attn, x: torch.Tensor):
+class EdgeWeights:
+    """The bf16 edge MLP's weights in one forward, as autograd sees them, and the copies that its kernels read.  Those of a
+    layer that is trained are made from these very tensors and end with the forward's graph: its weights change at every
+    step, by whatever means.  Those of a frozen layer are kept with the module."""
+
+    def __init__(self, attn):
+        from .attention import Kept
+        own = Kept()
+        lin0, lin2 = attn.edge_mlp[0], attn.edge_mlp[2]
+        self.first, self.second = (
+            (w, b, own if w.requires_grad or b.requires_grad else attn._copies) for w, b in ((lin0.weight, lin0.bias), (lin2.weight, lin2.bias)))
+
+
+def edge_generators(attn, x: torch.Tensor, weights: Optional[EdgeWeights]):
     """(a_all (B, L, H*stride) fp32, layout) of the module's edge MLP, differentiable (attn._edge_generators_nobias)."""
     B, L, D = x.shape
     partner = torch.roll(x, shifts=-1, dims=1)
     if attn.link_mode == "additive":
         return attn.gqproj(x).float() + attn.gkproj(partner).float(), "packed"
     pair = torch.cat([x, partner], dim=-1)
-    if x.dtype == torch.float32:
+    if weights is None:
         return attn.edge_mlp(pair).float(), "packed"             # (under autocast the linears' results are bf16)
     layout = attn._gen_layout()
-    lin0, lin2 = attn.edge_mlp[0], attn.edge_mlp[2]
-    w1t, b1f = attn._w1t()
-    h = EdgeLayer0.apply(pair.reshape(B * L, 2 * D), lin0.weight, lin0.bias, w1t, b1f)
+    h = EdgeLayer0.apply(pair.reshape(B * L, 2 * D), *weights.first[:2], *attn._w1t(*weights.first))
     mode = attn._precision_for(L, B * L, h.shape[1])
-    wt, _ = attn._stacked_w2t(False)
+    wt, _ = attn._stacked_w2t(False, *weights.second)
     index = _banked_index(attn.d, attn.h, x.device) if layout == "banked" else None
-    a = EdgeLayer2.apply(h, lin2.weight, lin2.bias, lambda t: attn._generators_of_hidden(t, mode), wt, index)
+    a = EdgeLayer2.apply(h, *weights.second[:2], lambda t: attn._generators_of_hidden(t, mode, weights.second), wt, index)
     return a.view(B, L, -1), layout
 
 
-def forward_rows(attn, x: torch.Tensor) -> torch.Tensor:
+def forward_rows(attn, x: torch.Tensor, weights: Optional[EdgeWeights]) -> torch.Tensor:
     """The module's causal forward (tril mask) of some batch rows, differentiable."""
     B, L, _ = x.shape
     qkv = attn.qkv(x)
-    a, layout = edge_generators(attn, x)
+    a, layout = edge_generators(attn, x, weights)
     chunk = attn.chunk or ops.plan_chunk(B, attn.h, L, attn.d, x.device)
     heads = PathCore.apply(a, qkv, None, attn.h, attn.edge_scale, attn.scale, chunk, layout)
     return attn.out(heads)
+
+
+def forward(attn, x: torch.Tensor, rows: int) -> torch.Tensor:
+    """The module's causal forward (tril mask), differentiable, ``rows`` batch rows at a time."""
+    if any(p.requires_grad for p in attn.edge_mlp.parameters()):
+        attn.weights_changed()                                   # (for the forwards without gradients that follow)
+    weights = EdgeWeights(attn) if attn.link_mode != "additive" and x.dtype != torch.float32 else None
+    pieces = [forward_rows(attn, x[b0:b0 + rows], weights) for b0 in range(0, x.shape[0], rows)]
+    return pieces[0] if len(pieces) == 1 else torch.cat(pieces)
 
 
 class AdamW(torch.optim.Optimizer):

@@ -44,3 +44,123 @@ def test_evaluated_in_inference_mode_between_steps(D, H, mode):
         seen.append(grads_of(m, x))
     ops.check_status()
     assert seen[0].keys() == seen[1].keys() and all(torch.equal(seen[0][k], seen[1][k]) for k in seen[0])
+
+
+def same(m, x):
+    """m's forward and gradients are those of a fresh module with its weights."""
+    fresh = PathOrderedGeometricMHA(m.h * m.d, n_heads=m.h, edge_scale=m.edge_scale).to(DEV, x.dtype)
+    fresh.generator_precision = m.generator_precision
+    fresh.load_state_dict(m.state_dict())
+    with torch.no_grad():
+        if not torch.equal(m(x, attn_mask=tril(x.shape[1]))[0], fresh(x, attn_mask=tril(x.shape[1]))[0]):
+            return False
+    a, b = grads_of(m, x), grads_of(fresh, x)
+    return a.keys() == b.keys() and all(torch.equal(a[k], b[k]) for k in a)
+
+
+@pytest.mark.parametrize("mode", ["bf16", "split", "split8"])
+@pytest.mark.parametrize("D,H,dtype", [(192, 4, torch.bfloat16), (128, 4, torch.bfloat16), (128, 4, torch.float32)])
+def test_weights_written_past_torch(D, H, dtype, mode):
+    """An optimizer that writes through .data, as many do: no version changes, and each training forward has the new weights,
+    and the evaluation after it."""
+    m = module(D, H, dtype, seed=2)
+    m.generator_precision = mode
+    x = torch.randn(2, 32, D, device=DEV).to(dtype)
+    assert same(m, x)
+    for step in range(3):
+        g = grads_of(m, x)
+        before = [p._version for p in m.parameters()]
+        for k, p in m.named_parameters():
+            if k in g:
+                p.data.add_(g[k], alpha=-0.02 / float(g[k].float().norm()))
+        assert before == [p._version for p in m.parameters()]
+        y = m(x, attn_mask=tril(32))[0]                           # (trains: what was kept ends)
+        assert y.requires_grad and same(m, x)
+
+
+def test_written_past_torch_without_training():
+    m = module(128, 4, seed=3)
+    x = torch.randn(1, 32, 128, device=DEV).to(torch.bfloat16)
+    with torch.no_grad():
+        old = m(x, attn_mask=tril(32))[0]
+        for forget in (m.weights_changed, m.eval, m.train, lambda: m.to("cpu").to(DEV)):
+            m.edge_mlp[2].weight.data.mul_(1.5)
+            forget()
+            new = m(x, attn_mask=tril(32))[0]
+            assert not torch.equal(new, old)
+            old = new
+        m.edge_mlp[2].weight.mul_(0.5)                            # (counted)
+        assert not torch.equal(m(x, attn_mask=tril(32))[0], old)
+
+
+@pytest.mark.parametrize("D,H", [(192, 4), (128, 4)])
+def test_parametrized_weights(D, H):
+    """weight_norm makes a new weight at every access, each at an address that an earlier one may have had."""
+    from torch.nn.utils.parametrizations import weight_norm
+    m = module(D, H, seed=4)
+    weight_norm(m.edge_mlp[2])
+    weight_norm(m.edge_mlp[0])
+    x = torch.randn(1, 32, D, device=DEV).to(torch.bfloat16)
+    opt = torch.optim.SGD(m.parameters(), lr=1e-3)
+    for _ in range(4):
+        y = m(x, attn_mask=tril(32))[0]
+        with torch.no_grad():
+            plain = module(D, H, seed=5)
+            plain.load_state_dict({**{k: v for k, v in m.state_dict().items() if "edge" not in k},
+                                   **{f"edge_mlp.{i}.{n}": getattr(m.edge_mlp[i], n).detach() for i in (0, 2) for n in ("weight", "bias")}})
+            want = plain(x, attn_mask=tril(32))[0]
+            assert torch.equal(m(x, attn_mask=tril(32))[0], want)
+        p = grads_of(plain, x)
+        opt.zero_grad()
+        y.float().square().sum().backward()
+        assert torch.equal(y, plain(x, attn_mask=tril(32))[0])
+        assert torch.equal(m.edge_mlp[2].bias.grad, p["edge_mlp.2.bias"]) and torch.equal(m.qkv.weight.grad, p["qkv.weight"])
+        assert m.edge_mlp[2].parametrizations.weight.original1.grad.any()
+        opt.step()
+
+
+def test_frozen_layers_keep_their_copies():
+    """Training around a frozen edge MLP lays its weights out once."""
+    m = module(128, 4, seed=6)
+    m.edge_mlp.requires_grad_(False)
+    x = torch.randn(4, 32, 128, device=DEV).to(torch.bfloat16)
+    m.PIECE_TOKENS = 32
+    laid, real = [], m._w2_rows
+    m._w2_rows = lambda *a: laid.append(1) or real(*a)
+    for _ in range(3):
+        m(x, attn_mask=tril(32))[0].float().sum().backward()
+    assert len(laid) == 1
+    m.edge_mlp.requires_grad_(True)
+    m(x, attn_mask=tril(32))[0].float().sum().backward()
+    assert len(laid) == 2                                         # (once a forward, not once a piece)
+
+
+@pytest.mark.parametrize("D,H", [(192, 4), (128, 4)])
+def test_captured_forward(D, H):
+    """A captured forward goes on with the copies of its capture while eager ones follow the weights; one that is captured
+    before the copies were made leaves none that are not there yet (packed: the banked copies' index comes from the host)."""
+    m = module(D, H, seed=7)
+    x, mask = torch.randn(1, 32, D, device=DEV).to(torch.bfloat16), tril(32)
+    with torch.no_grad():
+        old = m(x, attn_mask=mask)[0]
+        ops.check_status()                                        # (a launch whose status is still to be read cannot be polled in a capture)
+        g, cold = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = m(x, attn_mask=mask)[0]
+        if D == 192:
+            m.weights_changed()
+            with torch.cuda.graph(cold):
+                z = m(x, attn_mask=mask)[0]
+        assert torch.equal(m(x, attn_mask=mask)[0], old)
+        m.edge_mlp[2].weight.mul_(0.5)
+        new = m(x, attn_mask=mask)[0]
+        junk = [torch.full((2 << 20,), 7.0, device=DEV) for _ in range(8)]      # (would take the memory of copies that were let go)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, old) and not torch.equal(new, old)
+        if D == 192:
+            cold.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(z, new)
+        assert torch.equal(m(x, attn_mask=mask)[0], new)
+        del junk
