@@ -73,7 +73,7 @@ class Kept:
     def of(self, slot, tensors, make):
         """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
         capturing = tensors[0].is_cuda and torch.cuda.is_current_stream_capturing()
-        if any(t.is_inference() for t in tensors):               # (torch counts no writes of those)
+        if any(t.is_inference() or ops.written_by_graphs(t) for t in tensors):   # (torch counts no writes of those)
             return make()
         key = tuple((t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors)
         e = self._entries.get(slot)

@@ -406,6 +406,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!p0 || !g0 || !code(*p0, &p_code) || !code(*g0, &g_code)) Py_RETURN_NONE;
   const int idx = dev_index(*p0);
   if (idx < 0 || !ints(step, idx, {1})) Py_RETURN_NONE;
+  const cudaStream_t s = c10::cuda::getCurrentCUDAStream(idx).stream();
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;      // (a captured step is noted on the parameters: Python's side)
+  if (cudaStreamIsCapturing(s, &cap) != cudaSuccess || cap != cudaStreamCaptureStatusNone) Py_RETURN_NONE;
   const auto moment = bits8 ? at::kFloat8_e4m3fn : at::kFloat;
   std::vector<void*> ptr[6];                                      // params, grads, m, v, masters, scales
   for (auto& v : ptr) v.resize(count);
@@ -427,8 +430,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (std::adjacent_find(places.begin(), places.end()) != places.end()) Py_RETURN_NONE;
   const int st = g_fn.adamw(ptr[0].data(), p_code, has_master ? (float* const*)ptr[4].data() : nullptr, (const void* const*)ptr[1].data(),
                             g_code, ptr[2].data(), ptr[3].data(), bits8 ? (float* const*)ptr[5].data() : nullptr, bits8 ? 8 : 32,
-                            sizes.data(), (int)count, step->data_ptr<int>(), num[0], num[1], num[2], num[3], num[4],
-                            c10::cuda::getCurrentCUDAStream(idx).stream());
+                            sizes.data(), (int)count, step->data_ptr<int>(), num[0], num[1], num[2], num[3], num[4], s);
   if (st == 0)                                                    // (what was saved of them, or laid out from them, is out of date)
     for (Py_ssize_t i = 0; i < count; ++i)
       for (int list : {0, 10}) {

@@ -1187,6 +1187,11 @@ def path_bwd(a_all: torch.Tensor, R: torch.Tensor, C: torch.Tensor, chunk: int, 
 ADAMW_BLOCK = 256               # elements of a block of 8-bit moments
 
 
+def written_by_graphs(t: torch.Tensor) -> bool:
+    """Whether a captured adamw_step writes ``t``: its replays change it and no version says so."""
+    return getattr(t.untyped_storage(), "_hoa_written_by_graphs", False)
+
+
 def _pointers(ts):
     return (ctypes.c_void_p * len(ts))(*(None if t is None else t.data_ptr() for t in ts))
 
@@ -1198,7 +1203,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
     params fp32 or bf16, grads fp32 or bf16; ``masters``: fp32 copies that the step is made on (the parameter is then the
     copy, rounded), or None.  exp_avg and exp_avg_sq: fp32 moments; or, with ``scales``, 8-bit ones: float8_e4m3fn tensors
     of m and of sqrt(v), in blocks of ADAMW_BLOCK elements with scales[i] (2, blocks) fp32 (value = e4m3 * scale).
-    ``step``: int32 (1,) on the device, the number of this step, from 1 (read on the device: a captured step may be replayed).
+    ``step``: int32 (1,) on the device, the number of this step, from 1 (read on the device: a captured step may be replayed;
+    torch counts no writes of the replays, so nothing is kept from then on that was laid out from these params).
     hoa_adamw_step."""
     r = (_HOST or _host()).adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas[0], betas[1], eps, weight_decay, masters, scales)
     if r is not None:
@@ -1245,5 +1251,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
             _pointers(params), p_code, _pointers(masters) if masters is not None else None, _pointers(grads), g_code,
             _pointers(exp_avg), _pointers(exp_avg_sq), _pointers(scales) if scales is not None else None, 32 if scales is None else 8,
             _longs(*sizes), n, step.data_ptr(), lr, betas[0], betas[1], eps, weight_decay, torch._C._cuda_getCurrentRawStream(idx)))
+        if torch.cuda.is_current_stream_capturing():
+            for p in params:
+                p.untyped_storage()._hoa_written_by_graphs = True
     # written behind autograd's back: what was saved of them, or laid out from them, is out of date
     torch.autograd.graph.increment_version([t for t in (*params, *(masters or ())) if not t.is_inference()])
