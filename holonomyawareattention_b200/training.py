@@ -53,9 +53,14 @@ class PathCore(torch.autograd.Function):
         return da, dqkv, db, None, None, None, None, None
 
 
+def _weight_grad(dy: torch.Tensor, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """dy^T x of bf16 factors, in the weight's type (fp32 weights: the product's fp32 sums as they are)."""
+    return torch.mm(dy.t(), x) if dtype is torch.bfloat16 else torch.mm(dy.t(), x, out_dtype=torch.float32)
+
+
 class EdgeLayer0(torch.autograd.Function):
-    """The edge MLP's first layer in bf16, fp32 out (hoa_edge_gemm).  w1t, b1f: its weight transposed and its fp32 bias,
-    as the module keeps them."""
+    """The edge MLP's first layer in bf16, fp32 out (hoa_edge_gemm); its weights may be fp32 (autocast).  w1t, b1f: its
+    weight transposed in bf16 and its fp32 bias."""
 
     @staticmethod
     def forward(ctx, pair, weight, bias, w1t, b1f):
@@ -68,7 +73,8 @@ class EdgeLayer0(torch.autograd.Function):
         pair, weight = ctx.saved_tensors
         db = dh.sum(0).to(weight.dtype)
         dh = dh.to(torch.bfloat16)
-        return dh @ weight if ctx.needs_input_grad[0] else None, dh.t() @ pair, db, None, None
+        dx = dh @ weight.to(torch.bfloat16) if ctx.needs_input_grad[0] else None
+        return dx, _weight_grad(dh, pair, weight.dtype), db, None, None
 
 
 class EdgeLayer2(torch.autograd.Function):
@@ -79,6 +85,7 @@ class EdgeLayer2(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, weight, bias, forward_, wt, index):
         ctx.save_for_backward(h, wt, index)
+        ctx.dtype = weight.dtype
         return forward_(h)
 
     @staticmethod
@@ -88,11 +95,11 @@ class EdgeLayer2(torch.autograd.Function):
         db = da.sum(0)
         da = da.to(torch.bfloat16)
         g = F.gelu(h).to(torch.bfloat16)
-        dw = da.t() @ g                                        # (width, F)
+        dw = _weight_grad(da, g, ctx.dtype)                    # (width, F)
         dg = da @ wt.t()
         if index is not None:
             dw, db = dw[index], db[index]
-        return torch.ops.aten.gelu_backward(dg.float(), h), dw, db.to(torch.bfloat16), None, None, None
+        return torch.ops.aten.gelu_backward(dg.float(), h), dw, db.to(ctx.dtype), None, None, None
 
 
 _INDEX = {}
