@@ -8,8 +8,9 @@
 // puts its largest magnitude at 448, the largest e4m3 value; m and the root r are held as
 // e4m3 (r, not v: its range in a block is the square root of v's, and e4m3 has 2^17.8 of
 // it).  A root that is not zero is held as at least e4m3's smallest value, so that an
-// element with a small gradient is never divided by eps alone.  The step itself uses the
-// new moments before they are rounded to 8 bits.
+// element with a small gradient is never divided by eps alone.  A moment that is not finite is
+// held as e4m3's NaN and takes no part in its block's scale: as in fp32 it loses its own element
+// and no other.  The step itself uses the new moments before they are rounded to 8 bits.
 //
 // The moments' operations are rounded one by one (no fused multiply-add): the new moments, and so
 // the 8-bit values, are those of the same formula written in separate fp32 operations.  The
@@ -207,27 +208,41 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
     aw_store<kVec>(t.v, HOA_F32, i, n, v);
     return;
   }
-  // the largest of the block, as bits (a NaN is above all else, and is the scale then)
+  // the largest of the block, as bits (infinity and NaN are above all else)
   unsigned mt = 0, rt = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     mt = max(mt, __float_as_uint(fabsf(m[e])));
     rt = max(rt, __float_as_uint(fabsf(r[e])));
   }
-  ms = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, mt)), 1.f / 448.f);
-  vs = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, rt)), 1.f / 448.f);
+  mt = __reduce_max_sync(0xffffffffu, mt);
+  rt = __reduce_max_sync(0xffffffffu, rt);
+  constexpr unsigned kInf = 0x7f800000u;
+  if (max(mt, rt) >= kInf) {                                      // what is not finite: NaN, and no part of the scale
+    mt = rt = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned mu = __float_as_uint(fabsf(m[e])), ru = __float_as_uint(fabsf(r[e]));
+      if (mu < kInf) mt = max(mt, mu); else m[e] = __uint_as_float(0x7fffffffu);
+      if (ru < kInf) rt = max(rt, ru); else r[e] = __uint_as_float(0x7fffffffu);
+    }
+    mt = __reduce_max_sync(0xffffffffu, mt);
+    rt = __reduce_max_sync(0xffffffffu, rt);
+  }
+  ms = __fmul_rn(__uint_as_float(mt), 1.f / 448.f);
+  vs = __fmul_rn(__uint_as_float(rt), 1.f / 448.f);
   if (aw_div_by(ms)) {                                            // (uniform in the warp)
     const float y = __frcp_rn(ms);
     mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, y); });
   } else {
-    mb = aw_pack8(m, [&](float q) { return ms > 0.f ? __fdiv_rn(q, ms) : 0.f; });
+    mb = aw_pack8(m, [&](float q) { return ms > 0.f ? __fdiv_rn(q, ms) : q == q ? 0.f : q; });
   }
   constexpr float kLeast = 0.001953125f;                          // 2^-9
   if (aw_div_by(vs)) {
     const float y = __frcp_rn(vs);
     vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, y), kLeast) : q; });
   } else {
-    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(vs > 0.f ? __fdiv_rn(q, vs) : 0.f, kLeast) : 0.f; });
+    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(vs > 0.f ? __fdiv_rn(q, vs) : 0.f, kLeast) : q; });
   }
   aw_store8<kVec>(t.m, i, n, mb);
   aw_store8<kVec>(t.v, i, n, vb);
