@@ -12,6 +12,11 @@
 // held as e4m3's NaN and takes no part in its block's scale: as in fp32 it loses its own element
 // and no other.  The step itself uses the new moments before they are rounded to 8 bits.
 //
+// Rounding.  To the nearest, but for m below 2^-5, where all steps are the smallest one (2^-9), if the
+// gradient adds less than half of it (of the scale before): towards 0.  To the nearest, 4 of these steps
+// times 0.9 are 4 again, so a weight whose gradient has ended would be moved for good (by 0.13 lr a
+// step, betas 0.9 and 0.95: its root stays too, at 20 steps).
+//
 // The moments' operations are rounded one by one (no fused multiply-add): the new moments, and so
 // the 8-bit values, are those of the same formula written in separate fp32 operations.  The
 // update, which nothing is kept of but its sum with x, takes fast division.
@@ -31,6 +36,8 @@ constexpr int kAwThreads = 256, kAwBlock = 256, kAwPer = 8;       // a CTA: 8 el
 constexpr int kAwSpan = kAwThreads * kAwPer;                      // elements of a CTA, a multiple of kAwBlock
 constexpr int kAwCtas = 4;                                        // CTAs of an SM: 3 leave loads too little room, 5 and 6 spill
 constexpr int kAwMost = 256;                                      // tensors of one launch
+constexpr float kAwLeast = 0.001953125f;                          // 2^-9, the smallest e4m3 value: the least a root is held as
+constexpr float kAwHalf = 0.5f * kAwLeast;
 
 struct AwTensor {
   void* p; float* master; const void* g; void* m; void* v; float* scales;
@@ -64,6 +71,21 @@ HOA_DEVICE float aw_div(float a, float b, float y) {
   return fmaf(fmaf(-q, b, a), y, q);
 }
 HOA_DEVICE bool aw_div_by(float b) { return b > 1e-12f && b < 1e12f; }
+
+// the largest of a warp's values, none below 0
+HOA_DEVICE float aw_warp_max(float x) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x))); }
+// a block's scale, of its finite values alone
+HOA_DEVICE float aw_scale(const float (&x)[8], float scale) {
+  if (scale < INFINITY) return scale;
+  float t = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t = fabsf(x[e]) < INFINITY ? fmaxf(t, fabsf(x[e])) : t;
+  return __fmul_rn(aw_warp_max(t), 1.f / 448.f);
+}
+// x in units of a scale of any size (0 where that is 0; infinity and NaN: NaN)
+HOA_DEVICE float aw_quotient(float x, float scale) {
+  return !(fabsf(x) < INFINITY) ? __uint_as_float(0x7fffffffu) : scale > 0.f ? __fdiv_rn(x, scale) : 0.f;
+}
 
 HOA_DEVICE float aw_sqrt(float x) {                     // to an ulp or two: for the update, not for what is kept
   float y;
@@ -158,15 +180,50 @@ HOA_DEVICE uint2 aw_pack8(const float (&x)[8], Fn f) {
   return make_uint2(u[0], u[1]);
 }
 
+// The moments of a block that is not as most are, from shared memory (m, then r, kAwThreads apart), out of line and at the
+// block's end: its registers are not the others'.  old: m's scale before.
+template <bool kVec>
+__device__ __noinline__ void aw_rare(const AwTensor& t, long long blk, int g_dtype, float nb1, float old, float ms, float vs, const float* at) {
+  const int lid = threadIdx.x & 31;
+  const long long i = blk * kAwBlock + 8 * lid, blocks = (t.n + kAwBlock - 1) / kAwBlock;
+  float x[8], g[8];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = at[(from + e) * kAwThreads];
+  };
+  load(0);
+  ms = aw_scale(x, ms);
+  aw_load<kVec>(t.g, g_dtype, i, t.n, g);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = aw_quotient(x[e], ms);
+    if (__fmul_rn(fabsf(g[e]), nb1) < kAwHalf * old && fabsf(x[e]) < 0.03125f) x[e] = truncf(x[e] * 512.f) * (1.f / 512.f);
+  }
+  aw_store8<kVec>(t.m, i, t.n, aw_pack8(x, [](float q) { return q; }));
+  load(8);
+  vs = aw_scale(x, vs);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float q = aw_quotient(x[e], vs);
+    x[e] = x[e] > 0.f && q < kAwLeast ? kAwLeast : q;
+  }
+  aw_store8<kVec>(t.v, i, t.n, aw_pack8(x, [](float q) { return q; }));
+  if (lid == 0) {
+    t.scales[blk] = ms;
+    t.scales[blocks + blk] = vs;
+  }
+}
+
 // A warp has one block of 256 elements, a lane 8 consecutive ones of it.
 template <int kBits, bool kVec>
-HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float y2) {
+HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float y2, float* rare) {
   const int lid = threadIdx.x & 31;
   const long long i = blk * kAwBlock + 8 * lid, n = t.n;
   const long long blocks = (n + kAwBlock - 1) / kAwBlock;
   float g[8], x[8], m[8], v[8];
   uint2 mb = make_uint2(0, 0), vb = mb;
   float ms = 0.f, vs = 0.f;
+  bool ended = false;
   // all loads first
   aw_load<kVec>(t.g, a.g_dtype, i, n, g);
   if (t.master) aw_load<kVec>(t.master, HOA_F32, i, n, x);
@@ -176,6 +233,10 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
     vb = aw_load8<kVec>(t.v, i, n);
     ms = t.scales[blk];
     vs = t.scales[blocks + blk];
+    float least = INFINITY;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) least = fminf(least, fminf(fabsf(g[e]), fabsf(g[e + 1])));
+    ended = __fmul_rn(least, a.nb1) < kAwHalf * ms;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       const float2 mv = aw_values((e < 4 ? mb.x : mb.y) >> (8 * (e & 3)) & 0xffffu);
@@ -208,42 +269,29 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
     aw_store<kVec>(t.v, HOA_F32, i, n, v);
     return;
   }
-  // the largest of the block, as bits (infinity and NaN are above all else)
-  unsigned mt = 0, rt = 0;
+  // the largest of the block (a NaN is passed over)
+  float mt = 0.f, rt = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    mt = max(mt, __float_as_uint(fabsf(m[e])));
-    rt = max(rt, __float_as_uint(fabsf(r[e])));
+  for (int e = 0; e < 8; e += 2) {
+    mt = fmaxf(mt, fmaxf(fabsf(m[e]), fabsf(m[e + 1])));
+    rt = fmaxf(rt, fmaxf(r[e], r[e + 1]));
   }
-  mt = __reduce_max_sync(0xffffffffu, mt);
-  rt = __reduce_max_sync(0xffffffffu, rt);
-  constexpr unsigned kInf = 0x7f800000u;
-  if (max(mt, rt) >= kInf) {                                      // what is not finite: NaN, and no part of the scale
-    mt = rt = 0;
+  const float old = ms;
+  ms = __fmul_rn(aw_warp_max(mt), 1.f / 448.f);
+  vs = __fmul_rn(aw_warp_max(rt), 1.f / 448.f);
+  if (__any_sync(0xffffffffu, ended) || !aw_div_by(ms) || !aw_div_by(vs)) {                // (uniform in the warp)
+    float* at = rare + threadIdx.x;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const unsigned mu = __float_as_uint(fabsf(m[e])), ru = __float_as_uint(fabsf(r[e]));
-      if (mu < kInf) mt = max(mt, mu); else m[e] = __uint_as_float(0x7fffffffu);
-      if (ru < kInf) rt = max(rt, ru); else r[e] = __uint_as_float(0x7fffffffu);
+      at[e * kAwThreads] = m[e];
+      at[(8 + e) * kAwThreads] = r[e];
     }
-    mt = __reduce_max_sync(0xffffffffu, mt);
-    rt = __reduce_max_sync(0xffffffffu, rt);
+    aw_rare<kVec>(t, blk, a.g_dtype, a.nb1, old, ms, vs, at);
+    return;
   }
-  ms = __fmul_rn(__uint_as_float(mt), 1.f / 448.f);
-  vs = __fmul_rn(__uint_as_float(rt), 1.f / 448.f);
-  if (aw_div_by(ms)) {                                            // (uniform in the warp)
-    const float y = __frcp_rn(ms);
-    mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, y); });
-  } else {
-    mb = aw_pack8(m, [&](float q) { return ms > 0.f ? __fdiv_rn(q, ms) : q == q ? 0.f : q; });
-  }
-  constexpr float kLeast = 0.001953125f;                          // 2^-9
-  if (aw_div_by(vs)) {
-    const float y = __frcp_rn(vs);
-    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, y), kLeast) : q; });
-  } else {
-    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(vs > 0.f ? __fdiv_rn(q, vs) : 0.f, kLeast) : q; });
-  }
+  const float ym = __frcp_rn(ms), yr = __frcp_rn(vs);
+  mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, ym); });
+  vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, yr), kAwLeast) : q; });
   aw_store8<kVec>(t.m, i, n, mb);
   aw_store8<kVec>(t.v, i, n, vb);
   if (lid == 0) {
@@ -254,6 +302,7 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
 
 template <int kBits>
 __global__ void __launch_bounds__(kAwThreads, kAwCtas) adamw_kernel(const __grid_constant__ AwArgs a) {
+  __shared__ float rare[kBits == 8 ? 16 * kAwThreads : 1];
   // 1 - b^t = -(e^{t ln b} - 1)
   const double t = (double)*a.step;
   const float lr = a.lr / -expm1f((float)(t * a.ln1)), y2 = rsqrtf(-expm1f((float)(t * a.ln2)));
@@ -267,8 +316,8 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas) adamw_kernel(const __grid
     const AwTensor& x = a.t[lo];
     const long long blk = (long long)(c - a.first[lo]) * (kAwSpan / kAwBlock) + (threadIdx.x >> 5);
     if (blk * kAwBlock >= x.n) continue;
-    if (x.vec) aw_block<kBits, true>(a, x, blk, lr, y2);
-    else aw_block<kBits, false>(a, x, blk, lr, y2);
+    if (x.vec) aw_block<kBits, true>(a, x, blk, lr, y2, rare);
+    else aw_block<kBits, false>(a, x, blk, lr, y2, rare);
   }
 }
 
