@@ -17,13 +17,17 @@
 // times 0.9 are 4 again, so a weight whose gradient has ended would be moved for good (by 0.13 lr a
 // step, betas 0.9 and 0.95: its root stays too, at 20 steps).
 //
-// The moments' operations are rounded one by one (no fused multiply-add): the new moments, and so
-// the 8-bit values, are those of the same formula written in separate fp32 operations.  The
-// update, which nothing is kept of but its sum with x, takes fast division.
+// With beta1 above 15/16 or beta2 above 0.95, up or down by chance, so that the mean is exact.  To the nearest, a moment
+// that a step changes by less than half of its last place (3 to 6% of it) stays where it is: m falls by 1 - beta1 of itself at
+// most, a root by (1 - beta2) / 2.  Held over true roots (their median) 60, 100 and 200 steps after gradients have fallen
+// tenfold: beta2 0.95 to the nearest 1.6, 1.7 and 1.1, 0.97 to the nearest 2.4, 3.9 and 5.7, 0.999 to the nearest for good 6;
+// by chance all 0.95 to 1.03, 1% to 99% of them within a factor of 1.4 at 0.97 and 2 at 0.999.  The chance is a hash of the
+// element's number and the step's: the same state and gradients give the same bits.
 //
 // HBM bounds it: every byte is read and written once, a thread's loads come before all else.  Measured: 477 M elements,
-// bf16 with masters and 8-bit moments (16 bytes an element), 1.57 to 1.66 ms, 4.6 to 4.9 TB/s (conversions, roots and the
-// block's maxima beside the loads); 3.9 M fp32 in six tensors (28 bytes an element) 20 us, 5.4 TB/s.
+// bf16 with masters and 8-bit moments (16 bytes an element), to the nearest 1.60 to 1.68 ms, 4.5 to 4.8 TB/s (conversions,
+// roots and the block's maxima beside the loads), by chance 2.0 ms (the hash and the second rounding: 30 operations an
+// element), with half of the gradients ended 1.96; 3.9 M fp32 in six tensors (28 bytes an element) 20 to 23 us, 4.8 to 5.4 TB/s.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -180,10 +184,29 @@ HOA_DEVICE uint2 aw_pack8(const float (&x)[8], Fn f) {
   return make_uint2(u[0], u[1]);
 }
 
+// 32 bits that are as good as random, of an element's number and a step's (multiplications by odd numbers and shifts; any
+// would do that spread one bit's change over all)
+HOA_DEVICE uint32_t aw_noise(long long i, uint32_t step) {
+  uint32_t x = (uint32_t)i * 0x9e3779b1u ^ (uint32_t)((unsigned long long)i >> 32) * 0xb5297a4du;
+  x += step * 0x68e31da5u;
+  x = (x ^ (x >> 16)) * 0x7a3f5c2bu;
+  x = (x ^ (x >> 15)) * 0xc4d1e6b7u;
+  return x ^ (x >> 16);
+}
+// q -> one of the two e4m3 values around it, by 16 random bits: those added below the last place (2^-9 up to 2^-6), the rest
+// cut off.  (The half behind them keeps a value of e4m3 that is a few ulps off where it is.)
+HOA_DEVICE float aw_chance(float q, uint32_t u) {
+  const float a = fabsf(q);
+  const float big = __uint_as_float((__float_as_uint(a) + (u << 4 | 8u)) & 0xfff00000u);
+  const float small = floorf(fmaf(a, 512.f, fmaf((float)u, 1.f / 65536.f, 0.5f / 65536.f))) * (1.f / 512.f);
+  return copysignf(a >= 0.015625f ? big : small, q);
+}
+
 // The moments of a block that is not as most are, from shared memory (m, then r, kAwThreads apart), out of line and at the
 // block's end: its registers are not the others'.  old: m's scale before.
-template <bool kVec>
-__device__ __noinline__ void aw_rare(const AwTensor& t, long long blk, int g_dtype, float nb1, float old, float ms, float vs, const float* at) {
+template <bool kVec, bool kChance>
+__device__ __noinline__ void aw_rare(const AwTensor& t, long long blk, int g_dtype, float nb1, float old, float ms, float vs, uint32_t step,
+                                     const float* at) {
   const int lid = threadIdx.x & 31;
   const long long i = blk * kAwBlock + 8 * lid, blocks = (t.n + kAwBlock - 1) / kAwBlock;
   float x[8], g[8];
@@ -193,18 +216,20 @@ __device__ __noinline__ void aw_rare(const AwTensor& t, long long blk, int g_dty
   };
   load(0);
   ms = aw_scale(x, ms);
-  aw_load<kVec>(t.g, g_dtype, i, t.n, g);
+  if (!kChance) aw_load<kVec>(t.g, g_dtype, i, t.n, g);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     x[e] = aw_quotient(x[e], ms);
-    if (__fmul_rn(fabsf(g[e]), nb1) < kAwHalf * old && fabsf(x[e]) < 0.03125f) x[e] = truncf(x[e] * 512.f) * (1.f / 512.f);
+    if (kChance) x[e] = aw_chance(x[e], aw_noise(i + e, step) >> 16);
+    else if (__fmul_rn(fabsf(g[e]), nb1) < kAwHalf * old && fabsf(x[e]) < 0.03125f) x[e] = truncf(x[e] * 512.f) * (1.f / 512.f);
   }
   aw_store8<kVec>(t.m, i, t.n, aw_pack8(x, [](float q) { return q; }));
   load(8);
   vs = aw_scale(x, vs);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float q = aw_quotient(x[e], vs);
+    float q = aw_quotient(x[e], vs);
+    if (kChance) q = aw_chance(q, aw_noise(i + e, step) & 0xffffu);
     x[e] = x[e] > 0.f && q < kAwLeast ? kAwLeast : q;
   }
   aw_store8<kVec>(t.v, i, t.n, aw_pack8(x, [](float q) { return q; }));
@@ -215,8 +240,8 @@ __device__ __noinline__ void aw_rare(const AwTensor& t, long long blk, int g_dty
 }
 
 // A warp has one block of 256 elements, a lane 8 consecutive ones of it.
-template <int kBits, bool kVec>
-HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float y2, float* rare) {
+template <int kBits, bool kVec, bool kChance>
+HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, float lr, float y2, uint32_t step, float* rare) {
   const int lid = threadIdx.x & 31;
   const long long i = blk * kAwBlock + 8 * lid, n = t.n;
   const long long blocks = (n + kAwBlock - 1) / kAwBlock;
@@ -235,7 +260,7 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
     vs = t.scales[blocks + blk];
     float least = INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) least = fminf(least, fminf(fabsf(g[e]), fabsf(g[e + 1])));
+    for (int e = 0; e < 8 && !kChance; e += 2) least = fminf(least, fminf(fabsf(g[e]), fabsf(g[e + 1])));
     ended = __fmul_rn(least, a.nb1) < kAwHalf * ms;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
@@ -286,12 +311,23 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
       at[e * kAwThreads] = m[e];
       at[(8 + e) * kAwThreads] = r[e];
     }
-    aw_rare<kVec>(t, blk, a.g_dtype, a.nb1, old, ms, vs, at);
+    aw_rare<kVec, kChance>(t, blk, a.g_dtype, a.nb1, old, ms, vs, step, at);
     return;
   }
   const float ym = __frcp_rn(ms), yr = __frcp_rn(vs);
-  mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, ym); });
-  vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, yr), kAwLeast) : q; });
+  if (kChance) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t u = aw_noise(i + e, step);
+      m[e] = aw_chance(aw_div(m[e], ms, ym), u >> 16);
+      r[e] = r[e] > 0.f ? fmaxf(aw_chance(aw_div(r[e], vs, yr), u & 0xffffu), kAwLeast) : r[e];
+    }
+    mb = aw_pack8(m, [](float q) { return q; });
+    vb = aw_pack8(r, [](float q) { return q; });
+  } else {
+    mb = aw_pack8(m, [&](float q) { return aw_div(q, ms, ym); });
+    vb = aw_pack8(r, [&](float q) { return q > 0.f ? fmaxf(aw_div(q, vs, yr), kAwLeast) : q; });
+  }
   aw_store8<kVec>(t.m, i, n, mb);
   aw_store8<kVec>(t.v, i, n, vb);
   if (lid == 0) {
@@ -300,11 +336,12 @@ HOA_DEVICE void aw_block(const AwArgs& a, const AwTensor& t, long long blk, floa
   }
 }
 
-template <int kBits>
+template <int kBits, bool kChance>
 __global__ void __launch_bounds__(kAwThreads, kAwCtas) adamw_kernel(const __grid_constant__ AwArgs a) {
   __shared__ float rare[kBits == 8 ? 16 * kAwThreads : 1];
   // 1 - b^t = -(e^{t ln b} - 1)
-  const double t = (double)*a.step;
+  const int step = *a.step;
+  const double t = (double)step;
   const float lr = a.lr / -expm1f((float)(t * a.ln1)), y2 = rsqrtf(-expm1f((float)(t * a.ln2)));
   int lo = 0;
   for (unsigned c = blockIdx.x; c < a.ctas; c += gridDim.x) {
@@ -316,8 +353,8 @@ __global__ void __launch_bounds__(kAwThreads, kAwCtas) adamw_kernel(const __grid
     const AwTensor& x = a.t[lo];
     const long long blk = (long long)(c - a.first[lo]) * (kAwSpan / kAwBlock) + (threadIdx.x >> 5);
     if (blk * kAwBlock >= x.n) continue;
-    if (x.vec) aw_block<kBits, true>(a, x, blk, lr, y2, rare);
-    else aw_block<kBits, false>(a, x, blk, lr, y2, rare);
+    if (x.vec) aw_block<kBits, true, kChance>(a, x, blk, lr, y2, (uint32_t)step, rare);
+    else aw_block<kBits, false, kChance>(a, x, blk, lr, y2, (uint32_t)step, rare);
   }
 }
 
@@ -374,8 +411,9 @@ extern "C" int hoa_adamw_step(void* const* params, int p_dtype, float* const* ma
     a.lr = (float)lr;
     a.ln1 = log(beta1); a.ln2 = log(beta2);
     const unsigned grid = ctas < most ? ctas : most;
-    if (state_bits == 8) adamw_kernel<8><<<grid, kAwThreads, 0, s>>>(a);
-    else adamw_kernel<32><<<grid, kAwThreads, 0, s>>>(a);
+    if (state_bits == 32) adamw_kernel<32, false><<<grid, kAwThreads, 0, s>>>(a);
+    else if (beta1 > 0.9375 || beta2 > 0.95) adamw_kernel<8, true><<<grid, kAwThreads, 0, s>>>(a);
+    else adamw_kernel<8, false><<<grid, kAwThreads, 0, s>>>(a);
     if (int st = launch_status()) return st;
   }
   return HOA_OK;

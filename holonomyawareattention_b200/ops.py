@@ -1202,7 +1202,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
 
     params fp32 or bf16, grads fp32 or bf16; ``masters``: fp32 copies that the step is made on (the parameter is then the
     copy, rounded), or None.  exp_avg and exp_avg_sq: fp32 moments; or, with ``scales``, 8-bit ones: float8_e4m3fn tensors
-    of m and of sqrt(v), in blocks of ADAMW_BLOCK elements with scales[i] (2, blocks) fp32 (value = e4m3 * scale).
+    of m and of sqrt(v), in blocks of ADAMW_BLOCK elements with scales[i] (2, blocks) fp32 (value = e4m3 * scale), rounded to the
+    nearest for betas up to 15/16 and 0.95, above by a chance that follows from the element's place and ``step`` (to the nearest
+    they would stop moving).
     ``step``: int32 (1,) on the device, the number of this step, from 1 (read on the device: a captured step may be replayed;
     torch counts no writes of the replays, so nothing is kept from then on that was laid out from these params).
     hoa_adamw_step."""

@@ -166,7 +166,8 @@ def forward(attn, x: torch.Tensor, rows: int) -> torch.Tensor:
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with one launch for all tensors of a type (ops.adamw_step).
 
-    ``state_bits`` 32: fp32 moments; 8: 8-bit ones in blocks of 256 elements (2 bytes an element for both instead of 8).
+    ``state_bits`` 32: fp32 moments; 8: 8-bit ones in blocks of 256 elements (2 bytes an element for both instead of 8): a held
+    root is within a factor of about 2 of the fp32 one at betas[1] 0.999, 1.4 up to 0.97.
     bf16 parameters are stepped on fp32 master copies, kept in the state, unless ``masters`` is False.  The steps are
     counted on the host: under graph capture step() raises (ops.adamw_step takes a count on the device)."""
 

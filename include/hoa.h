@@ -504,7 +504,10 @@ int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias, float edg
  * params p_dtype, grads g_dtype (each HOA_F32 or HOA_BF16).  masters (nullable, entries too): fp32 copies that the
  * step is made on; the parameter is then the copy, rounded.  state_bits 32: m and v fp32.  8: m and sqrt(v)
  * as e4m3 bytes, blocks of 256 elements, scales[i] (2, blocks) fp32: value = byte * scale, for m and for
- * sqrt(v).  step: device int32, the number t of this step, from 1.
+ * sqrt(v).  step: device int32, the number t of this step, from 1.  The bytes are rounded to the nearest for beta1 up to
+ * 15/16 and beta2 up to 0.95 (m towards 0 below 2^-5 of its scale where the gradient adds less than half of the smallest
+ * step), else up or down by a hash of the element's number and t, so that the mean is exact.  A moment that is not finite
+ * is held as NaN and is no part of its block's scale.
  */
 int hoa_adamw_step(void* const* params, int p_dtype, float* const* masters, const void* const* grads, int g_dtype,
                    void* const* m, void* const* v, float* const* scales, int state_bits, const long long* sizes, int count,
