@@ -138,7 +138,7 @@ def edge_generators(attn, x: torch.Tensor, weights: Optional[EdgeWeights]):
     layout = attn._gen_layout()
     h = EdgeLayer0.apply(pair.reshape(B * L, 2 * D), *weights.first[:2], *attn._w1t(*weights.first))
     mode = attn._precision_for(L, B * L, h.shape[1])
-    wt, _ = attn._stacked_w2t(False, *weights.second)
+    wt = attn._stacked_w2t(mode == "split", *weights.second)[0][:h.shape[1]]        # (split: the first of its two, for both passes)
     index = _banked_index(attn.d, attn.h, x.device) if layout == "banked" else None
     a = EdgeLayer2.apply(h, *weights.second[:2], lambda t: attn._generators_of_hidden(t, mode, weights.second), wt, index)
     return a.view(B, L, -1), layout

@@ -199,3 +199,21 @@ def test_replayed_adamw_steps(D, H, dtype):
             g.replay()
             f.replay()
             assert torch.equal(m(x, attn_mask=mask)[0], y) and not torch.equal(y, old)
+
+
+@pytest.mark.parametrize("D,H", [(192, 4), (128, 4)])
+@pytest.mark.parametrize("mode,copies", [("bf16", 1), ("split", 1), ("split8", 2)])
+def test_one_copy_a_form(D, H, mode, copies):
+    """A training forward lays the second layer's weight out once for each type that its products take, however many pieces
+    the batch has, and the backward pass reads the forward's copy."""
+    m = module(D, H, seed=10)
+    m.generator_precision = mode
+    m.PIECE_TOKENS = 32
+    x = torch.randn(3, 32, D, device=DEV).to(torch.bfloat16)
+    laid, real = [], m._w2_rows
+    m._w2_rows = lambda *a: laid.append(1) or real(*a)
+    for _ in range(2):
+        y = m(x, attn_mask=tril(32))[0]
+        y.float().square().sum().backward()
+        assert len(laid) == copies
+        laid.clear()
