@@ -203,7 +203,7 @@ class PathOrderedGeometricMHA(nn.Module):
         generator layout (zero rows at the banked layout's unused slots)."""
         if self._gen_layout() == "packed":
             return w, b
-        idx = ops.gen_banked_index(self.d, self.h, w.device)
+        idx = ops.banked_index_on(self.d, self.h, w.device)
         width = self.h * ops.gen_stride(self.d, "banked")
         wb = w.new_zeros(width, w.shape[1])
         wb[idx] = w

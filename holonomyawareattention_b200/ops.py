@@ -180,6 +180,7 @@ def plan_chunk(B: int, H: int, T: int, d: int, device=None) -> int:
 # unused slots, so that the link kernel reads rows without bank conflicts)
 # ---------------------------------------------------------------------------
 _BANKED_MAPS = {}
+_BANKED_INDICES = {}
 
 
 def gen_stride(d: int, layout: str = "packed") -> int:
@@ -205,6 +206,15 @@ def gen_banked_index(d: int, n_heads: int, device=None) -> torch.Tensor:
     slots = gen_banked_map(d)
     idx = (torch.arange(n_heads).unsqueeze(1) * S + slots.unsqueeze(0)).reshape(-1)
     return idx if device is None else idx.to(device)
+
+
+def banked_index_on(d: int, n_heads: int, device) -> torch.Tensor:
+    """gen_banked_index on a device, kept: not to be written."""
+    i = _BANKED_INDICES.get((d, n_heads, device))
+    if i is None:
+        with torch.inference_mode(False):
+            i = _BANKED_INDICES[d, n_heads, device] = gen_banked_index(d, n_heads, device)
+    return i
 
 
 def gen_to_banked(a: torch.Tensor, n_heads: int, d: int) -> torch.Tensor:

@@ -102,17 +102,6 @@ class EdgeLayer2(torch.autograd.Function):
         return torch.ops.aten.gelu_backward(dg.float(), h), dw, db.to(ctx.dtype), None, None, None
 
 
-_INDEX = {}
-
-
-def _banked_index(d: int, h: int, device) -> torch.Tensor:
-    i = _INDEX.get((d, h, device))
-    if i is None:
-        with torch.inference_mode(False):
-            i = _INDEX[d, h, device] = ops.gen_banked_index(d, h, device)
-    return i
-
-
 class EdgeWeights:
     """The bf16 edge MLP's weights in one forward, as autograd sees them, and the copies that its kernels read.  Those of a
     layer that is trained are made from these very tensors and end with the forward's graph: its weights change at every
@@ -139,7 +128,7 @@ def edge_generators(attn, x: torch.Tensor, weights: Optional[EdgeWeights]):
     h = EdgeLayer0.apply(pair.reshape(B * L, 2 * D), *weights.first[:2], *attn._w1t(*weights.first))
     mode = attn._precision_for(L, B * L, h.shape[1])
     wt = attn._stacked_w2t(mode == "split", *weights.second)[0][:h.shape[1]]        # (split: the first of its two, for both passes)
-    index = _banked_index(attn.d, attn.h, x.device) if layout == "banked" else None
+    index = ops.banked_index_on(attn.d, attn.h, x.device) if layout == "banked" else None
     a = EdgeLayer2.apply(h, *weights.second[:2], lambda t: attn._generators_of_hidden(t, mode, weights.second), wt, index)
     return a.view(B, L, -1), layout
 
@@ -250,8 +239,10 @@ def _tril(L: int, device) -> torch.Tensor:
 def train_step(attn, x: torch.Tensor, optimizer, loss: Callable[[torch.Tensor], torch.Tensor], attn_mask: Optional[torch.Tensor] = None,
                max_grad_norm: Optional[float] = None) -> torch.Tensor:
     """One step: y = attn(x) under the causal mask (``attn_mask``, default tril), loss(y), gradients (their norm held to
-    ``max_grad_norm``, if given), the optimizer's step.  Gradients start and end at None.  Returns the loss, detached, on the
-    device; nothing waits for the GPU.  Not under graph capture."""
+    ``max_grad_norm``, if given), the optimizer's step.  The optimizer's gradients start and end at None.  Returns the loss,
+    detached, on the device.  Nothing waits for the GPU, but where an ``attn_mask`` is given that was not seen before (what it
+    holds decides the path) and in the form "split8" of the generators ("auto" beyond 8192 positions: the largest weight
+    gives the fp8 product's scale on the host, once a forward while the weights are trained).  Not under graph capture."""
     if x.is_cuda and torch.cuda.is_current_stream_capturing():
         raise NotImplementedError("train_step cannot be captured into a graph")
     L = x.shape[1]

@@ -217,3 +217,19 @@ def test_one_copy_a_form(D, H, mode, copies):
         y.float().square().sum().backward()
         assert len(laid) == copies
         laid.clear()
+
+
+@pytest.mark.parametrize("dtype,mode", [(torch.float32, "auto"), (torch.bfloat16, "auto"), (torch.bfloat16, "split")])
+def test_train_step_waits_for_nothing(dtype, mode):
+    m = module(128, 4, dtype, seed=11)
+    m.generator_precision = mode
+    x = torch.randn(2, 32, 128, device=DEV).to(dtype)
+    opt = AdamW(m.parameters(), lr=1e-3, state_bits=8)
+    for i in range(3):
+        if i:
+            torch.cuda.set_sync_debug_mode("error")
+        try:
+            train_step(m, x, opt, lambda y: y.float().square().sum(), max_grad_norm=1.0)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    ops.check_status()
