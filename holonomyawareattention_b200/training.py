@@ -48,9 +48,14 @@ class PathCore(torch.autograd.Function):
         dout = dheads.reshape(BH // H, T, H, d).permute(0, 2, 1, 3).float().contiguous().view(BH, T, d)
         doh = ops.apply_paths(dout, R, C, chunk, transpose=True).to(qh.dtype)          # P^T dout
         dqh, dkh, dvh = ops.attn_bwd(qh, kh, vh, o, lse, doh, scale)
+        want_a, _, want_bias = ctx.needs_input_grad[:3]
+        if not (want_a or want_bias):                                  # (frozen generators: the vectors' gradients alone)
+            dqkv = torch.empty(BH // H, T, H, 3, d, dtype=dheads.dtype, device=dheads.device)
+            for i, t in enumerate((dqh, dkh, dvh)):
+                dqkv[:, :, :, i] = ops.apply_paths(t.float(), R, C, chunk).view(BH // H, H, T, d).transpose(1, 2)
+            return None, dqkv.view(BH // H, T, 3 * H * d), None, None, None, None, None, None
         da, dqkv = ops.path_bwd(a_all, R, C, chunk, H, edge_scale, (qh, kh, vh, o), (dqh, dkh, dvh, doh), a_bias, layout)
-        db = da.sum((0, 1)) if a_bias is not None and ctx.needs_input_grad[2] else None
-        return da, dqkv, db, None, None, None, None, None
+        return da, dqkv, da.sum((0, 1)) if want_bias else None, None, None, None, None, None
 
 
 def _weight_grad(dy: torch.Tensor, x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -71,10 +76,11 @@ class EdgeLayer0(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh):
         pair, weight = ctx.saved_tensors
-        db = dh.sum(0).to(weight.dtype)
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        db = dh.sum(0).to(weight.dtype) if want_b else None
         dh = dh.to(torch.bfloat16)
-        dx = dh @ weight.to(torch.bfloat16) if ctx.needs_input_grad[0] else None
-        return dx, _weight_grad(dh, pair, weight.dtype), db, None, None
+        dx = dh @ weight.to(torch.bfloat16) if want_x else None
+        return dx, _weight_grad(dh, pair, weight.dtype) if want_w else None, db, None, None
 
 
 class EdgeLayer2(torch.autograd.Function):
@@ -92,14 +98,18 @@ class EdgeLayer2(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, da):
         h, wt, index = ctx.saved_tensors
-        db = da.sum(0)
+        want_h, want_w, want_b = ctx.needs_input_grad[:3]
+        dh = dw = db = None
+        if want_b:
+            db = da.sum(0).to(ctx.dtype)
+            db = db if index is None else db[index]
         da = da.to(torch.bfloat16)
-        g = F.gelu(h).to(torch.bfloat16)
-        dw = _weight_grad(da, g, ctx.dtype)                    # (width, F)
-        dg = da @ wt.t()
-        if index is not None:
-            dw, db = dw[index], db[index]
-        return torch.ops.aten.gelu_backward(dg.float(), h), dw, db.to(ctx.dtype), None, None, None
+        if want_w:
+            dw = _weight_grad(da, F.gelu(h).to(torch.bfloat16), ctx.dtype)     # (width, F)
+            dw = dw if index is None else dw[index]
+        if want_h:
+            dh = torch.ops.aten.gelu_backward((da @ wt.t()).float(), h)
+        return dh, dw, db, None, None, None
 
 
 class EdgeWeights:
