@@ -167,8 +167,10 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 32: fp32 moments; 8: 8-bit ones in blocks of 256 elements (2 bytes an element for both instead of 8): a held
     root is within a factor of about 2 of the fp32 one at betas[1] 0.999, 1.4 up to 0.97.
-    bf16 parameters are stepped on fp32 master copies, kept in the state, unless ``masters`` is False.  The steps are
-    counted on the host: under graph capture step() raises (ops.adamw_step takes a count on the device)."""
+    bf16 parameters are stepped on fp32 master copies, kept in the state, unless ``masters`` is False; an element of a
+    parameter that something else wrote since the last step (load_state_dict, a clamp; not through ``.data``, which torch
+    does not count) is taken as it is.  The steps are counted on the host: under graph capture step() raises
+    (ops.adamw_step takes a count on the device)."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, masters: bool = True):
@@ -176,11 +178,19 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr, eps and weight_decay must be at least 0 and betas in [0, 1)")
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
+        self._left = {}                                          # parameter -> (address, version) that the last step left
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters))
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._left = {}
 
     def _init(self, p, group):
         s = self.state[p]
         if s:
+            if "master" in s and self._left.get(p) != (p.data_ptr(), p._version):
+                m = s["master"]                                  # (its low bits stay where the parameter is still its rounding)
+                m.copy_(torch.where(m.to(p.dtype) == p, m, p))
             return s
         s["step"] = 0
         moment = torch.float32 if group["state_bits"] == 32 else torch.float8_e4m3fn
@@ -218,8 +228,10 @@ class AdamW(torch.optim.Optimizer):
                                torch.full((1,), n + 1, dtype=torch.int32, device=dev), lr=float(group["lr"]), betas=group["betas"],
                                eps=group["eps"], weight_decay=group["weight_decay"], masters=[s["master"] for s in ss] if masters else None,
                                scales=[s["scales"] for s in ss] if group["state_bits"] == 8 else None)
-                for s in ss:
+                for p, s in zip(ps, ss):
                     s["step"] = n + 1
+                    if masters:
+                        self._left[p] = p.data_ptr(), p._version
         return loss
 
     @torch.no_grad()
