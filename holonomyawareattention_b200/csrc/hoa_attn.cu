@@ -202,7 +202,8 @@ namespace hoa {
 int attn_simt(const void* qh, const void* kh, const void* vh, int hat_dtype, float* o, float* lse, float softmax_scale,
               int BH, int Tq, int Tk, int q_offset, int d, void* stream) {
   if (!qh || !kh || !vh || !o || BH < 1 || Tq < 1 || Tk < 1 || d < 1) return HOA_ERR_INVALID_ARG;
-  if (q_offset < 0 || q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (q_offset < 0 || (long long)q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (Tk > 0x7fffff00) return HOA_ERR_UNSUPPORTED;                   // (tile starts are counted with ints)
   if (hat_dtype != HOA_F32 && hat_dtype != HOA_BF16) return HOA_ERR_UNSUPPORTED;
   if (BH > 65535) return HOA_ERR_UNSUPPORTED;
   AttnArgs a{qh, kh, vh, hat_dtype, o, softmax_scale, Tq, Tk, q_offset, d, lse};

@@ -342,7 +342,8 @@ static int dispatch_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUten
 int attn_tc(const void* qh, const void* kh, const void* vh, bool v_rows, float* o, float* lse, int* status,
             float softmax_scale, int BH, int Tq, int Tk, int q_offset, int d, void* stream) {
   if (!qh || !kh || !vh || !o || BH < 1 || Tq < 1 || Tk < 1 || d < 1) return HOA_ERR_INVALID_ARG;
-  if (q_offset < 0 || q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (q_offset < 0 || (long long)q_offset + Tq > Tk) return HOA_ERR_INVALID_ARG;
+  if (Tk > 0x7fffff00) return HOA_ERR_UNSUPPORTED;                   // (tile starts are counted with ints)
   if (BH > 65535 || d > 128 || d % 8 != 0) return HOA_ERR_UNSUPPORTED;
   const uint64_t tp = (uint64_t)hoa_vt_stride(Tk);
   CUtensorMap mq, mk, mv;
