@@ -413,7 +413,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   std::vector<void*> ptr[6];                                      // params, grads, m, v, masters, scales
   for (auto& v : ptr) v.resize(count);
   std::vector<long long> sizes(count);
-  std::vector<void*> places;
+  struct Span { uintptr_t from, to; int writes; };
+  std::vector<Span> spans;                                        // what a step writes shares no memory with anything else (ops._apart)
+  spans.reserve(6 * count);
   for (Py_ssize_t i = 0; i < count; ++i) {
     const at::Tensor* p = item(0, i);
     if (!p) Py_RETURN_NONE;
@@ -423,11 +425,19 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !like(t[2], idx, moment, p->sizes()) || !like(t[3], idx, moment, p->sizes()) ||
         (has_master && !like(t[4], idx, at::kFloat, p->sizes())) || (bits8 && !like(t[5], idx, at::kFloat, {2, (sizes[i] + 255) / 256})))
       Py_RETURN_NONE;
-    for (int k = 0; k < 6; ++k) ptr[k][i] = t[k] ? t[k]->data_ptr() : nullptr;
-    if (sizes[i] > 0) places.push_back(ptr[0][i]);
+    for (int k = 0; k < 6; ++k) {
+      ptr[k][i] = t[k] ? t[k]->data_ptr() : nullptr;
+      if (sizes[i] == 0 || !t[k] || (k == 4 && p_code == HOA_F32 && ptr[4][i] == ptr[0][i])) continue;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(ptr[k][i]);
+      spans.push_back({at, at + (uintptr_t)t[k]->nbytes(), k != 1});
+    }
   }
-  std::sort(places.begin(), places.end());
-  if (std::adjacent_find(places.begin(), places.end()) != places.end()) Py_RETURN_NONE;
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+  uintptr_t end[2] = {0, 0};                                      // of the grads and of the written ones so far
+  for (const Span& x : spans) {
+    if (x.from < end[1] || (x.writes && x.from < end[0])) Py_RETURN_NONE;
+    end[x.writes] = std::max(end[x.writes], x.to);
+  }
   const int st = g_fn.adamw(ptr[0].data(), p_code, has_master ? (float* const*)ptr[4].data() : nullptr, (const void* const*)ptr[1].data(),
                             g_code, ptr[2].data(), ptr[3].data(), bits8 ? (float* const*)ptr[5].data() : nullptr, bits8 ? 8 : 32,
                             sizes.data(), (int)count, step->data_ptr<int>(), num[0], num[1], num[2], num[3], num[4], s);

@@ -1206,6 +1206,22 @@ def _pointers(ts):
     return (ctypes.c_void_p * len(ts))(*(None if t is None else t.data_ptr() for t in ts))
 
 
+def _apart(params, grads, exp_avg, exp_avg_sq, masters, scales) -> None:
+    """What a step writes shares no memory with anything else that it writes or reads (an fp32 parameter may be its own master)."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+    own = [None if p.dtype is not torch.float32 else p.data_ptr() for p in params]
+    written = [span(t) for ts in (params, exp_avg, exp_avg_sq, scales or ()) for t in ts if t.numel()]
+    written += [span(t) for t, at in zip(masters or (), own) if t.numel() and t.data_ptr() != at]
+    both = sorted([(*x, 1) for x in written] + [(*span(t), 0) for t in grads if t.numel()])
+    end = [0, 0]                                                  # of the grads and of the written ones so far
+    for a, b, writes in both:
+        if a < end[1] or (writes and a < end[0]):
+            raise ValueError("params, masters, moments and scales must share no memory with one another or with the grads")
+        end[writes] = max(end[writes], b)
+
+
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 0.01, masters=None, scales=None) -> None:
     """One AdamW step over all tensors of the lists, in place, in one launch (256 tensors each).
@@ -1256,6 +1272,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
     if scales is not None:
         for i, n_i in enumerate(sizes):
             _like(scales[i], f"scales[{i}]", (2, -(-n_i // ADAMW_BLOCK)), torch.float32, idx)
+    _apart(params, grads, exp_avg, exp_avg_sq, masters, scales)
     with _current(idx):
         if idx not in _DEVICES and not torch.cuda.is_current_stream_capturing():
             _device(idx)                       # (from now on the C++ side takes such calls)

@@ -502,7 +502,8 @@ int hoa_path_bwd(const float* a_all, int a_dtype, const float* a_bias, float edg
  * counts), in place, in one launch a 256 tensors:
  *   m = b1 m + (1-b1) g,  v = b2 v + (1-b2) g^2,  x = x (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
  * params p_dtype, grads g_dtype (each HOA_F32 or HOA_BF16).  masters (nullable, entries too): fp32 copies that the
- * step is made on; the parameter is then the copy, rounded.  state_bits 32: m and v fp32.  8: m and sqrt(v)
+ * step is made on; the parameter is then the copy, rounded.  What is written shares no memory with anything else that a
+ * call is given (an fp32 parameter may be its own master).  state_bits 32: m and v fp32.  8: m and sqrt(v)
  * as e4m3 bytes, blocks of 256 elements, scales[i] (2, blocks) fp32: value = byte * scale, for m and for
  * sqrt(v).  step: device int32, the number t of this step, from 1.  The bytes are rounded to the nearest for beta1 up to
  * 15/16 and beta2 up to 0.95 (m towards 0 below 2^-5 of its scale where the gradient adds less than half of the smallest
