@@ -174,12 +174,16 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, masters: bool = True):
-        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0 or not all(0.0 <= b < 1.0 for b in betas):
-            raise ValueError("lr, eps and weight_decay must be at least 0 and betas in [0, 1)")
-        if state_bits not in (8, 32):
-            raise ValueError("state_bits must be 8 or 32")
         self._left = {}                                          # parameter -> (address, version) that the last step left
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters))
+
+    def add_param_group(self, param_group):
+        g = {**self.defaults, **param_group}
+        if not (g["lr"] >= 0.0 and g["eps"] >= 0.0 and g["weight_decay"] >= 0.0 and all(0.0 <= b < 1.0 for b in g["betas"])):
+            raise ValueError("lr, eps and weight_decay must be at least 0 and betas in [0, 1)")
+        if g["state_bits"] not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        super().add_param_group(param_group)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -197,28 +201,30 @@ class AdamW(torch.optim.Optimizer):
         for k in ("exp_avg", "exp_avg_sq"):
             s[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device).to(moment)
         if group["state_bits"] == 8:
-            s["scales"] = torch.zeros(2, -(-p.numel() // ops.ADAMW_BLOCK), device=p.device)
+            s["scales"] = torch.zeros(2, -(-p.numel() // ops.ADAMW_BLOCK), dtype=torch.float32, device=p.device)
         if p.dtype == torch.bfloat16 and group["masters"]:
             s["master"] = p.detach().float().contiguous()
         return s
 
     @torch.no_grad()
     def step(self, closure=None):
+        """One step; what is refused is refused before any parameter changes."""
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise NotImplementedError("AdamW.step counts its steps on the host and cannot be captured: capture ops.adamw_step")
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise NotImplementedError("AdamW.step counts its steps on the host and cannot be captured: capture ops.adamw_step")
+        for p in (p for group in self.param_groups for p in group["params"] if p.grad is not None):
+            if not p.is_cuda or p.grad.is_sparse or not {p.dtype, p.grad.dtype} <= {torch.float32, torch.bfloat16}:
+                raise NotImplementedError("AdamW takes dense fp32 or bf16 CUDA parameters and gradients")
+            if not p.is_contiguous():
+                raise ValueError("parameters must be contiguous")
         for group in self.param_groups:
             calls = {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                if not p.is_cuda or p.grad.is_sparse or p.dtype not in (torch.float32, torch.bfloat16):
-                    raise NotImplementedError("AdamW takes dense fp32 or bf16 CUDA parameters")
-                if not p.is_contiguous():
-                    raise ValueError("parameters must be contiguous")
                 s = self._init(p, group)
                 g = p.grad.contiguous()
                 calls.setdefault((p.device, p.dtype, g.dtype, s["step"], "master" in s), []).append((p, g, s))
