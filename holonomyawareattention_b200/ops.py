@@ -570,14 +570,20 @@ def edge_gelu_split8(h: torch.Tensor):
     return hi, lo
 
 
-_GEMM_WS = {}
+_GEMM_WS = {}                   # (device, stream) -> workspace of the products that are queued there, one behind the other
 _GEMM_WS_BYTES = 32 << 20
 
 
 def _gemm_ws(dev):
-    ws = _GEMM_WS.get(dev)
+    """The GEMMs' workspace on ``dev``'s current stream.  A product may leave partial sums in it, so products that may run at
+    once - on two streams, in a graph beside eager ones - have two; a captured one's is its graph's."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
+    key = dev, _stream(dev)
+    ws = _GEMM_WS.get(key)
     if ws is None:
-        ws = _GEMM_WS[dev] = torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
+        with torch.inference_mode(False):
+            ws = _GEMM_WS[key] = torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
     return ws
 
 
@@ -594,8 +600,8 @@ def edge_gemm_fp8_acc(lo: torch.Tensor, w: torch.Tensor, out: torch.Tensor, alph
     if w.shape[1] != K or out.shape != (M, N):
         raise ValueError(f"shapes: lo {tuple(lo.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
     dev = lo.device
-    _lib.call("hoa_edge_gemm_fp8_acc", _ptr(lo), _ptr(w), _ptr(out), float(alpha), M, N, K, _ptr(_gemm_ws(dev)),
-              _GEMM_WS_BYTES, _stream(dev))
+    ws = _gemm_ws(dev)
+    _lib.call("hoa_edge_gemm_fp8_acc", _ptr(lo), _ptr(w), _ptr(out), float(alpha), M, N, K, _ptr(ws), _GEMM_WS_BYTES, _stream(dev))
     return out
 
 
@@ -616,9 +622,7 @@ def edge_gemm(hidden: torch.Tensor, wt: torch.Tensor, bias: Optional[torch.Tenso
             raise ValueError("bias must be float32 with N elements")
         bias = bias.contiguous()
     dev = hidden.device
-    ws = _GEMM_WS.get(dev)
-    if ws is None:
-        ws = _GEMM_WS[dev] = torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
+    ws = _gemm_ws(dev)
     out = torch.empty(M, N, dtype=torch.float32, device=dev)
     try:
         _lib.call("hoa_edge_gemm", _ptr(hidden), _ptr(wt), _ptr(bias), _ptr(out), M, N, K, _ptr(ws),
