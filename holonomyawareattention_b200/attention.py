@@ -72,22 +72,32 @@ class Kept:
 
     def of(self, slot, tensors, make):
         """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
-        capturing = tensors[0].is_cuda and torch.cuda.is_current_stream_capturing()
-        if any(t.is_inference() or ops.written_by_graphs(t) for t in tensors):   # (torch counts no writes of those)
-            return make()
-        key = tuple((t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors)
         e = self._entries.get(slot)
-        if e is not None and e[0] == key and all(r() is t.untyped_storage() for r, t in zip(e[1], tensors)):
-            if capturing and not any(v is e[2] for v in self._in_graphs):
-                self._in_graphs.append(e[2])
-            return e[2]
+        if e is not None and self._holds(e, tensors):
+            if e[2] and torch.cuda.is_current_stream_capturing() and not any(v is e[1] for v in self._in_graphs):
+                self._in_graphs.append(e[1])
+            return e[1]
         value = make()
-        if capturing:
+        cuda = tensors[0].is_cuda
+        if any(t.is_inference() or ops.written_by_graphs(t) for t in tensors):   # (torch counts no writes of those)
+            return value
+        if cuda and torch.cuda.is_current_stream_capturing():
             return value
         if len(self._entries) >= self.MOST:
             self._entries.clear()
-        self._entries[slot] = key, tuple(weakref.ref(t.untyped_storage()) for t in tensors), value
+        self._entries[slot] = (tuple((weakref.ref(t.untyped_storage()), t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors),
+                               value, cuda, ops.graph_writes())
         return value
+
+    @staticmethod
+    def _holds(e, tensors) -> bool:
+        if e[3] != ops.graph_writes() and any(ops.written_by_graphs(t) for t in tensors):
+            return False
+        for t, (storage, at, version, dtype, shape, stride) in zip(tensors, e[0]):
+            if (storage() is not t.untyped_storage() or t.is_inference() or t._version != version or t.data_ptr() != at
+                    or t.dtype is not dtype or t.shape != shape or t.stride() != stride):
+                return False
+        return True
 
 
 class PathOrderedGeometricMHA(nn.Module):
@@ -332,7 +342,8 @@ class PathOrderedGeometricMHA(nn.Module):
         """(W2 in e4m3 (rows in the generator layout) times a power-of-two scale s, and
         alpha = 1 / (s * ops.SPLIT8_LO_SCALE))."""
         if w is None:
-            w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+            lin2 = self.edge_mlp[2]
+            w, b = lin2.weight, lin2.bias
 
         def make():
             with _laying_out():
@@ -347,7 +358,8 @@ class PathOrderedGeometricMHA(nn.Module):
     def _stacked_w2t(self, split: bool = True, w=None, b=None, kept: Optional[Kept] = None):
         """([W2^T ; W2^T] (8D x m*H; W2^T alone for split=False) in bf16, the output bias in fp32)."""
         if w is None:
-            w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+            lin2 = self.edge_mlp[2]
+            w, b = lin2.weight, lin2.bias
 
         def make():
             with _laying_out():
@@ -360,7 +372,8 @@ class PathOrderedGeometricMHA(nn.Module):
     def _w1t(self, w=None, b=None, kept: Optional[Kept] = None):
         """(W1^T (2D x 4D) in bf16, b1 in fp32) of the edge MLP's first layer."""
         if w is None:
-            w, b = self.edge_mlp[0].weight, self.edge_mlp[0].bias
+            lin0 = self.edge_mlp[0]
+            w, b = lin0.weight, lin0.bias
 
         def make():
             with _laying_out():
@@ -370,7 +383,8 @@ class PathOrderedGeometricMHA(nn.Module):
 
     def _w2f32(self):
         """(W2, b2) in fp32 with rows in the banked layout."""
-        w, b = self.edge_mlp[2].weight, self.edge_mlp[2].bias
+        lin2 = self.edge_mlp[2]
+        w, b = lin2.weight, lin2.bias
 
         def make():
             with _laying_out():

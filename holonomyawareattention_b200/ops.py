@@ -574,12 +574,12 @@ _GEMM_WS = {}                   # (device, stream) -> workspace of the products 
 _GEMM_WS_BYTES = 32 << 20
 
 
-def _gemm_ws(dev):
+def _gemm_ws(dev, stream=None):
     """The GEMMs' workspace on ``dev``'s current stream.  A product may leave partial sums in it, so products that may run at
     once - on two streams, in a graph beside eager ones - have two; a captured one's is its graph's."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
-    key = dev, _stream(dev)
+    key = dev, _stream(dev) if stream is None else stream
     ws = _GEMM_WS.get(key)
     if ws is None:
         with torch.inference_mode(False):
@@ -600,8 +600,9 @@ def edge_gemm_fp8_acc(lo: torch.Tensor, w: torch.Tensor, out: torch.Tensor, alph
     if w.shape[1] != K or out.shape != (M, N):
         raise ValueError(f"shapes: lo {tuple(lo.shape)}, w {tuple(w.shape)}, out {tuple(out.shape)}")
     dev = lo.device
-    ws = _gemm_ws(dev)
-    _lib.call("hoa_edge_gemm_fp8_acc", _ptr(lo), _ptr(w), _ptr(out), float(alpha), M, N, K, _ptr(ws), _GEMM_WS_BYTES, _stream(dev))
+    stream = _stream(dev)
+    ws = _gemm_ws(dev, stream)
+    _lib.call("hoa_edge_gemm_fp8_acc", _ptr(lo), _ptr(w), _ptr(out), float(alpha), M, N, K, _ptr(ws), _GEMM_WS_BYTES, stream)
     return out
 
 
@@ -622,11 +623,12 @@ def edge_gemm(hidden: torch.Tensor, wt: torch.Tensor, bias: Optional[torch.Tenso
             raise ValueError("bias must be float32 with N elements")
         bias = bias.contiguous()
     dev = hidden.device
-    ws = _gemm_ws(dev)
+    stream = _stream(dev)
+    ws = _gemm_ws(dev, stream)
     out = torch.empty(M, N, dtype=torch.float32, device=dev)
     try:
         _lib.call("hoa_edge_gemm", _ptr(hidden), _ptr(wt), _ptr(bias), _ptr(out), M, N, K, _ptr(ws),
-                  _GEMM_WS_BYTES, _stream(dev))
+                  _GEMM_WS_BYTES, stream)
     except _lib.HoaError as e:
         if e.status != _lib.HOA_ERR_UNSUPPORTED:
             raise
@@ -1201,6 +1203,14 @@ def path_bwd(a_all: torch.Tensor, R: torch.Tensor, C: torch.Tensor, chunk: int, 
 ADAMW_BLOCK = 256               # elements of a block of 8-bit moments
 
 
+_GRAPH_WRITES = [0]
+
+
+def graph_writes() -> int:
+    """How many steps have been captured so far."""
+    return _GRAPH_WRITES[0]
+
+
 def written_by_graphs(t: torch.Tensor) -> bool:
     """Whether a captured adamw_step writes ``t``: its replays change it and no version says so."""
     return getattr(t.untyped_storage(), "_hoa_written_by_graphs", False)
@@ -1287,5 +1297,6 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step: torch.Tensor, lr: float
         if torch.cuda.is_current_stream_capturing():
             for p in params:
                 p.untyped_storage()._hoa_written_by_graphs = True
+            _GRAPH_WRITES[0] += 1
     # written behind autograd's back: what was saved of them, or laid out from them, is out of date
     torch.autograd.graph.increment_version([t for t in (*params, *(masters or ())) if not t.is_inference()])

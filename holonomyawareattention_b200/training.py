@@ -162,6 +162,9 @@ def forward(attn, x: torch.Tensor, rows: int) -> torch.Tensor:
     return pieces[0] if len(pieces) == 1 else torch.cat(pieces)
 
 
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) with one launch for all tensors of a type (ops.adamw_step).
 
@@ -215,19 +218,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for p in (p for group in self.param_groups for p in group["params"] if p.grad is not None):
-            if not p.is_cuda or p.grad.is_sparse or not {p.dtype, p.grad.dtype} <= {torch.float32, torch.bfloat16}:
+        found = [[(p, p.grad) for p in group["params"] if p.grad is not None] for group in self.param_groups]
+        for p, g in (x for xs in found for x in xs):
+            if not p.is_cuda or g.is_sparse or p.dtype not in _FLOATS or g.dtype not in _FLOATS:
                 raise NotImplementedError("AdamW takes dense fp32 or bf16 CUDA parameters and gradients")
             if not p.is_contiguous():
                 raise ValueError("parameters must be contiguous")
-        for group in self.param_groups:
+        for group, xs in zip(self.param_groups, found):
             calls = {}
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
+            for p, g in xs:
                 s = self._init(p, group)
-                g = p.grad.contiguous()
-                calls.setdefault((p.device, p.dtype, g.dtype, s["step"], "master" in s), []).append((p, g, s))
+                calls.setdefault((p.device, p.dtype, g.dtype, s["step"], "master" in s), []).append((p, g.contiguous(), s))
             for (dev, _, _, n, masters), items in calls.items():
                 ps, gs, ss = zip(*items)
                 ops.adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
