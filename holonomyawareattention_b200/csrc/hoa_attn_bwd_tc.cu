@@ -8,7 +8,7 @@
 //   queries    Q, dO        K, V            S             dP                            dQ += dS K
 //
 // so a row of the CTA's matrices is a TMEM lane and a thread throughout, P and dS go back over S
-// and G as packed bf16 (the left operand of the second products, from TMEM), and the streamed
+// and G in two bf16 parts each (the left operands of the second products, from TMEM), and the streamed
 // tile serves as the K-major right operand of the first products and, by rows, as the MN-major
 // one of the second.
 //
@@ -16,14 +16,17 @@
 // products, one for the TMA loads.  One's exponentials run beside the products of another's tile:
 // head dims above 64 have W = 2 in a CTA (TMEM: S and G of two tiles, 4 x 64 columns, and 2 x 128 of
 // accumulators: an SM's 512); up to 64 a CTA has W = 1 in 256 columns and 80 KB, and two run on an
-// SM, so that one's start and end overlap the other's work too (256 x 512 x 48: 114 us with W = 2,
-// 80 so).  CTAs with the longest walks, of all chains, start first.
+// SM, so that one's start and end overlap the other's work too (256 x 512 x 48, P and dS of one part: 114 us
+// with W = 2, 80 so).  CTAs with the longest walks, of all chains, start first.
 //
-// Measured: 16 x 4096 x 96 188 us (0.69 PFLOP/s of the five products), 96 x 2048 x 120 415 us (0.58).
-// A tile takes about 1475 cycles for keys and 1345 for queries, of which the tensor core is busy 910
-// and 730: the rest is the softmax's chain (TMEM loads, exponentials, stores and hand-overs, 2000
-// cycles a tile over two warpgroups); and a CTA's start and end, about 8000 cycles, which with W = 2
-// nothing overlaps.  Own tiles in TMEM (their products 30 cycles instead of 46), a third S and G, P and
+// P and dS are hi + lo to 2^-16, so that a result is off by its own rounding (2^-8) and no more.  Of one part
+// each they would add as much again: errors of 1.41 of the results' rounding, up to 1.8 in short sequences,
+// 1.55 for dq at head dims up to 32, whose terms cancel; and 76, 212 and 491 us for the times below.
+//
+// Measured: 256 x 512 x 48 85 us, 16 x 4096 x 96 252 us (0.51 PFLOP/s of the formula's five products), 96 x 2048 x 120
+// 574 us (0.42).  The tensor core is busy 52% (d = 96) and 35% (d = 48), issue 34% and 43%: the rest is the softmax's
+// chain (TMEM loads, exponentials, the parts, stores and hand-overs) and a CTA's start and end, which with W = 2 nothing
+// overlaps.  With P and dS of one part: own tiles in TMEM (their products 30 cycles instead of 46), a third S and G, P and
 // dS in columns of their own, the second half's TMEM loads ahead: no gain.
 #include "hoa_attn_bwd.cuh"
 #include "hoa_f32x2.cuh"
@@ -49,11 +52,7 @@ struct BwLayout {
   static constexpr uint32_t kCols = 256 * W;
   // TMEM of a role: S and G of NB tiles, then the accumulators (keys: A0 and A1)
   template <bool kKeys> struct Role {
-    static constexpr int NB = W;      // (a third one for queries, whose columns allow it: 187 us for 188, and 434 for 415)
-    // dS is rounded to bf16 as an operand, 2^-8 of a term at most.  With few columns the terms of dq cancel (the ds of a row
-    // sum to 0, and its keys' shares along so few directions are alike), and the rounding would be 1.55 of dq's own: there dS
-    // is taken in two bf16 parts.
-    static constexpr bool kSplit = !kKeys && DP <= 32;
+    static constexpr int NB = W;      // (a third one for queries, whose columns allow it: no gain)
     static constexpr uint32_t colA0 = 128 * NB, colA1 = colA0 + (kKeys ? DP : 0);
     static_assert(colA1 + DP <= kCols, "TMEM columns");
   };
@@ -69,6 +68,16 @@ HOA_DEVICE float bw_pack(F2 x) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
   return __uint_as_float(*reinterpret_cast<const uint32_t*>(&h));
 }
+
+// x = hi + lo to 2^-16, two bf16 each
+HOA_DEVICE void bw_split(F2 x, float& hi, float& lo) {
+  hi = bw_pack(x);
+  const uint32_t u = __float_as_uint(hi);
+  lo = bw_pack(f2_fma(f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), f2(-1.f), x));
+}
+// columns (8 of them a 16 keys or queries) of the high and low parts of matrix rows in the place of their 64 fp32 values:
+// [hi lo] of the first 32, [hi lo] of the second, so that either half goes over what was loaded of it
+HOA_DEVICE constexpr uint32_t bw_part(int kk, bool lo) { return (kk >> 1) * 32 + (lo ? 16 : 0) + (kk & 1) * 8; }
 
 struct BwMaps { CUtensorMap x0, x1, y0, y1; };
 
@@ -180,11 +189,11 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
         const uint64_t mY0 = desc_sw128_mn(st, L::kStrBlk), mY1 = desc_sw128_mn(st + L::kStr, L::kStrBlk);
         const uint32_t cS = tm + (j % NB) * 128;
 #pragma unroll
-        for (int kk = 0; kk < kBwStr / 16; ++kk) {
-          if (kKeys)
-            mma_bf16_ts_warp(tm + Role::colA0, cS + kk * 8, mY1 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
-          mma_bf16_ts_warp(tm + Role::colA1, cS + 64 + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, j > 0 || kk > 0 ? 1u : 0u, lead);
-          if (Role::kSplit) mma_bf16_ts_warp(tm + Role::colA1, cS + kk * 8, mY0 + (uint64_t)(kk * 2048 >> 4), idA, 1u, lead);
+        for (int i = 0; i < kBwStr / 8; ++i) {
+          const int kk = i >> 1;
+          const uint32_t at = bw_part(kk, (i & 1) == 0), acc = j > 0 || i > 0 ? 1u : 0u;      // (the small parts first)
+          if (kKeys) mma_bf16_ts_warp(tm + Role::colA0, cS + at, mY1 + (uint64_t)(kk * 2048 >> 4), idA, acc, lead);
+          mma_bf16_ts_warp(tm + Role::colA1, cS + 64 + at, mY0 + (uint64_t)(kk * 2048 >> 4), idA, acc, lead);
         }
         tc_commit_warp(&empty[j % L::NS], lead);
         if (W == 1 && j + 1 < n) front(j + 1);                     // (over P and dS, behind the products that read them)
@@ -242,7 +251,7 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
           for (int e = 0; e < 32; ++e)
             if (kKeys ? 32 * half + e < lo : 32 * half + e >= hi) s[e] = -INFINITY;
         }
-        float pk[16], dk[16];
+        float ph[16], pl[16], dh[16], dl[16];                      // P's and dS's high and low parts
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           F2 l[2], D[2];
@@ -262,18 +271,16 @@ HOA_DEVICE void attn_bwd_tc_role(const BwMaps& maps, const AttnBwdArgs& p) {
             const int i = e + 2 * k;
             const float2 z = f2_get(f2_fma(f2(s[i], s[i + 1]), f2(c), l[k]));
             const F2 pr = f2(bw_exp2(z.x), bw_exp2(z.y));
-            if (kKeys) pk[i / 2] = bw_pack(pr);
-            const F2 ds = f2_mul(pr, f2_add(f2(gr[i], gr[i + 1]), D[k]));
-            dk[i / 2] = bw_pack(ds);
-            if (Role::kSplit) {                                     // what the rounding left, over S's first half (P's place for keys)
-              const uint32_t u = __float_as_uint(dk[i / 2]);
-              pk[i / 2] = bw_pack(f2_fma(f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)), f2(-1.f), ds));
-            }
+            if (kKeys) bw_split(pr, ph[i / 2], pl[i / 2]);
+            bw_split(f2_mul(pr, f2_add(f2(gr[i], gr[i + 1]), D[k])), dh[i / 2], dl[i / 2]);
           }
         }
-        // (16 columns over the first half of S, which is in registers; the second half lies behind them)
-        if (kKeys || Role::kSplit) tmem_st16(cS + 16 * half, pk);
-        tmem_st16(cS + 64 + 16 * half, dk);
+        if (kKeys) {
+          tmem_st16(cS + 32 * half, ph);
+          tmem_st16(cS + 32 * half + 16, pl);
+        }
+        tmem_st16(cS + 64 + 32 * half, dh);
+        tmem_st16(cS + 64 + 32 * half + 16, dl);
       }
       tmem_wait_st();
       tc_fence_before();

@@ -469,8 +469,10 @@ int hoa_attn_fwd_lse(const void* qh, const void* kh, const void* vh, int dtype, 
  *   p_ij = exp(scale q^_i.k^_j - lse_i) (j <= q_offset + i),  ds_ij = p_ij (dout_i.v^_j - dout_i.o_i)
  *   dq_i = scale sum_j ds_ij k^_j,  dk_j = scale sum_i ds_ij q^_i,  dv_j = sum_i p_ij dout_i
  * q^, k^, v^, dout and the three outputs are `dtype`, o and lse fp32; every output is written in full
- * (keys that no query sees: 0).  Sums have a fixed order: two calls give the same bits.  A NaN or
- * infinity in a position's k^ or v^ may also reach, as 0 times it, queries that do not see it.  d <= 128,
+ * (keys that no query sees: 0) and shares no memory with what is read.  Sums have a fixed order: two calls
+ * give the same bits.  p and ds are fp32, in bf16 calls hi + lo to 2^-16 as operands; sums are fp32.  A NaN or
+ * infinity in a position's k^ or v^ may also reach, as 0 times it, queries that do not see it, and one in a
+ * query's q^, dout, o or lse keys that it does not see (in its tile of 64).  d <= 128,
  * B*H <= 65535.  The workspace is 256-byte aligned; `aligned`: q^, k^, v^, dout and the outputs all start at
  * 16-byte boundaries (bf16 otherwise, and with d % 8 != 0, goes through copies).  `status` may receive
  * HOA_ERR_TIMEOUT.
