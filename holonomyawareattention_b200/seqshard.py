@@ -199,11 +199,14 @@ def sequence_sharded_forward(mod, x_shard: torch.Tensor, group=None,
     computed with the sequence split across the ranks of ``group``.
 
     ``x_shard`` is this rank's local tensor in ``layout`` (see shard_sequence);
-    the result has the same layout.  The local segments run through the link,
-    carry and transport kernels as extra batch rows; attention runs once per
-    local segment, at that segment's query offset."""
+    the result has the same layout.  Forward only: a call that would need
+    gradients raises.  The local segments run through the link, carry and
+    transport kernels as extra batch rows; attention runs once per local
+    segment, at that segment's query offset."""
     if mod.mode != "causal" or mod.link_mode != "interaction":
         raise NotImplementedError("sequence sharding serves mode='causal', link_mode='interaction'")
+    if torch.is_grad_enabled() and (x_shard.requires_grad or any(p.requires_grad for p in mod.parameters())):
+        raise NotImplementedError("forward-only kernels: call under torch.no_grad() / torch.inference_mode()")
     if not x_shard.is_cuda:
         raise NotImplementedError("the B200 kernels need CUDA tensors (there is no CPU path)")
     world, rank = _world(group)
