@@ -158,6 +158,10 @@ class PathOrderedGeometricMHA(nn.Module):
         self._tril_ok = Kept()
         self._copies = Kept()
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._tril_ok, self._copies = Kept(), Kept()              # (pickles of earlier versions hold others in their places)
+
     # ------------------------------------------------------------------
     def _check_supported(self, x: torch.Tensor, attn_mask, return_geometry: bool) -> None:
         why = None

@@ -74,6 +74,16 @@ def test_module_copies():
         assert not twin._mask_is_tril(~a, L) and twin._mask_is_tril(a, L)
 
 
+def test_pickles_of_earlier_versions():
+    """A module that was pickled with a dictionary of masks and without copies of weights."""
+    m = PathOrderedGeometricMHA(32, n_heads=4)
+    m._tril_ok = {}
+    del m._copies
+    twin = pickle.loads(pickle.dumps(m))
+    assert twin._mask_is_tril(tril(), L) and not twin._mask_is_tril(~tril(), L)
+    twin.eval().train()
+
+
 @pytest.mark.gpu
 def test_freed_masks_on_the_gpu():
     """A freed causal mask's memory with another mask in it: the forward is that mask's, with gradients it is refused."""
