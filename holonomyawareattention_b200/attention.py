@@ -67,8 +67,10 @@ class Kept:
     def __reduce__(self):
         return Kept, ()
 
-    def clear(self):
-        self._entries.clear()
+    def clear(self, kind=None):
+        """Forget all values, or those whose slots start with ``kind``."""
+        for slot in [s for s in self._entries if kind is None or s[0] == kind]:
+            self._entries.pop(slot, None)
 
     def of(self, slot, tensors, make):
         """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
@@ -357,7 +359,7 @@ class PathOrderedGeometricMHA(nn.Module):
                 s = 2.0 ** math.floor(math.log2(448.0 / amax)) if amax > 0 else 1.0
                 return (wf * s).to(torch.float8_e4m3fn).contiguous(), 1.0 / (s * ops.SPLIT8_LO_SCALE)
 
-        return (self._copies if kept is None else kept).of("w2fp8", (w, b), make)
+        return (self._copies if kept is None else kept).of((2, "fp8"), (w, b), make)
 
     def _stacked_w2t(self, split: bool = True, w=None, b=None, kept: Optional[Kept] = None):
         """([W2^T ; W2^T] (8D x m*H; W2^T alone for split=False) in bf16, the output bias in fp32)."""
@@ -371,7 +373,7 @@ class PathOrderedGeometricMHA(nn.Module):
                 wt = wr.t().to(torch.bfloat16)
                 return (torch.cat([wt, wt], dim=0) if split else wt).contiguous(), br.float().contiguous()
 
-        return (self._copies if kept is None else kept).of(("w2t", split), (w, b), make)
+        return (self._copies if kept is None else kept).of((2, "transposed", split), (w, b), make)
 
     def _w1t(self, w=None, b=None, kept: Optional[Kept] = None):
         """(W1^T (2D x 4D) in bf16, b1 in fp32) of the edge MLP's first layer."""
@@ -383,7 +385,7 @@ class PathOrderedGeometricMHA(nn.Module):
             with _laying_out():
                 return w.detach().t().to(torch.bfloat16).contiguous(), b.detach().float().contiguous()
 
-        return (self._copies if kept is None else kept).of("w1t", (w, b), make)
+        return (self._copies if kept is None else kept).of((0, "transposed"), (w, b), make)
 
     def _w2f32(self):
         """(W2, b2) in fp32 with rows in the banked layout."""
@@ -395,7 +397,7 @@ class PathOrderedGeometricMHA(nn.Module):
                 wr, br = self._w2_rows(w.detach().float(), b.detach().float())
                 return wr.contiguous(), br.contiguous()
 
-        return self._copies.of("w2f32", (w, b), make)
+        return self._copies.of((2, "fp32"), (w, b), make)
 
     # Batch rows are independent: the forward runs over pieces of about this many
     # tokens (whole rows).  The edge-MLP GEMM and the link kernel then alternate in

@@ -155,8 +155,9 @@ def forward_rows(attn, x: torch.Tensor, weights: Optional[EdgeWeights]) -> torch
 
 def forward(attn, x: torch.Tensor, rows: int) -> torch.Tensor:
     """The module's causal forward (tril mask), differentiable, ``rows`` batch rows at a time."""
-    if any(p.requires_grad for p in attn.edge_mlp.parameters()):
-        attn.weights_changed()                                   # (for the forwards without gradients that follow)
+    for layer in (0, 2):
+        if any(p.requires_grad for p in attn.edge_mlp[layer].parameters()):
+            attn._copies.clear(layer)                            # (for the forwards without gradients that follow)
     weights = EdgeWeights(attn) if attn.link_mode != "additive" and x.dtype != torch.float32 else None
     pieces = [forward_rows(attn, x[b0:b0 + rows], weights) for b0 in range(0, x.shape[0], rows)]
     return pieces[0] if len(pieces) == 1 else torch.cat(pieces)

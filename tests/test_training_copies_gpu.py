@@ -233,3 +233,21 @@ def test_train_step_waits_for_nothing(dtype, mode):
         finally:
             torch.cuda.set_sync_debug_mode("default")
     ops.check_status()
+
+
+def test_one_frozen_layer_keeps_its_copies():
+    """... and so does training the first layer before a frozen second one; the first one's end with each step."""
+    m = module(128, 4, seed=12)
+    m.edge_mlp[2].requires_grad_(False)
+    x = torch.randn(2, 32, 128, device=DEV).to(torch.bfloat16)
+    laid, real = [], m._w2_rows
+    m._w2_rows = lambda *a: laid.append(1) or real(*a)
+    for _ in range(3):
+        m(x, attn_mask=tril(32))[0].float().sum().backward()
+        m.edge_mlp[0].weight.data.mul_(1.01)
+        with torch.no_grad():
+            m(x, attn_mask=tril(32))
+    assert len(laid) == 1
+    m(x, attn_mask=tril(32))[0].float().sum().backward()
+    m.edge_mlp.requires_grad_(True)
+    assert same(m, x)
