@@ -56,50 +56,72 @@ def _laying_out():
 class Kept:
     """Values that follow from tensors, each kept while its tensors are what they were: in the same memory - the storage
     itself, held weakly, as an address comes back to another tensor once the first is freed - and without an in-place write
-    that torch has counted since.  What is made while a CUDA graph is captured is not kept (it is there when the graph runs),
-    and what a graph was given stays for as long as its owner.  Copies and pickles of the owner start empty."""
+    that torch has counted since.  A stream that did not make the value waits for the one that did.  What is made while a
+    CUDA graph is captured is not kept (it is there when the graph runs), and what a graph was given stays for as long as its
+    owner.  Copies and pickles of the owner start empty."""
 
     MOST = 64
 
-    def __init__(self):
-        self._entries, self._in_graphs = {}, []
+    def __init__(self, streams: bool = True):
+        """streams=False: of use on one stream alone."""
+        self._entries, self._in_graphs, self._streams = {}, [], streams
 
     def __reduce__(self):
-        return Kept, ()
+        return Kept, (self._streams,)
 
     def clear(self, kind=None):
         """Forget all values, or those whose slots start with ``kind``."""
-        for slot in [s for s in self._entries if kind is None or s[0] == kind]:
-            self._entries.pop(slot, None)
+        for slot in list(self._entries):                         # (a copy of the keys: another thread may add some)
+            if kind is None or slot[0] == kind:
+                self._entries.pop(slot, None)
 
     def of(self, slot, tensors, make):
         """The value of ``slot``, from make() unless the one kept there still follows from ``tensors``."""
         e = self._entries.get(slot)
+        if e is not None and e[3] == ops.graph_writes():
+            # (the same tensor objects, as a module's weights are: where they lie and what was written)
+            for t, (one, storage, at, version, _) in zip(tensors, e[0]):
+                if one() is not t or storage() is not t.untyped_storage() or t._version != version or t.data_ptr() != at:
+                    break
+            else:
+                return e[1] if e[2] is None else self._for_this_stream(e)
         if e is not None and self._holds(e, tensors):
-            if e[2] and torch.cuda.is_current_stream_capturing() and not any(v is e[1] for v in self._in_graphs):
-                self._in_graphs.append(e[1])
-            return e[1]
+            return e[1] if e[2] is None else self._for_this_stream(e)
         value = make()
-        cuda = tensors[0].is_cuda
         if any(t.is_inference() or ops.written_by_graphs(t) for t in tensors):   # (torch counts no writes of those)
             return value
-        if cuda and torch.cuda.is_current_stream_capturing():
-            return value
+        made = None
+        if isinstance(value, tuple):                             # (of tensors on the device, still to be written there)
+            if torch.cuda.is_current_stream_capturing():
+                return value
+            if self._streams:
+                stream = torch.cuda.current_stream(tensors[0].device)
+                made = stream.device_index, stream.cuda_stream, stream.record_event()
         if len(self._entries) >= self.MOST:
             self._entries.clear()
-        self._entries[slot] = (tuple((weakref.ref(t.untyped_storage()), t.data_ptr(), t._version, t.dtype, t.shape, t.stride()) for t in tensors),
-                               value, cuda, ops.graph_writes())
+        self._entries[slot] = (tuple((weakref.ref(t), weakref.ref(t.untyped_storage()), t.data_ptr(), t._version, (t.dtype, t.shape, t.stride()))
+                                     for t in tensors), value, made, ops.graph_writes())
         return value
 
     @staticmethod
     def _holds(e, tensors) -> bool:
-        if e[3] != ops.graph_writes() and any(ops.written_by_graphs(t) for t in tensors):
-            return False
-        for t, (storage, at, version, dtype, shape, stride) in zip(tensors, e[0]):
-            if (storage() is not t.untyped_storage() or t.is_inference() or t._version != version or t.data_ptr() != at
-                    or t.dtype is not dtype or t.shape != shape or t.stride() != stride):
-                return False
-        return True
+        return all(storage() is t.untyped_storage() and not t.is_inference() and t._version == version and t.data_ptr() == at
+                   and (t.dtype, t.shape, t.stride()) == form and (e[3] == ops.graph_writes() or not ops.written_by_graphs(t))
+                   for t, (_, storage, at, version, form) in zip(tensors, e[0]))
+
+    def _for_this_stream(self, e):
+        """The copies of entry ``e``, to be read on the current stream."""
+        _, value, (device, stream, event), _ = e
+        if torch.cuda.is_current_stream_capturing():             # (a capture begins when all before it is done)
+            if not any(v is value for v in self._in_graphs):
+                self._in_graphs.append(value)
+        elif torch._C._cuda_getCurrentRawStream(device) != stream:
+            now = torch.cuda.current_stream(device)
+            now.wait_event(event)
+            for t in value:
+                if torch.is_tensor(t):
+                    t.record_stream(now)
+        return value
 
 
 class PathOrderedGeometricMHA(nn.Module):

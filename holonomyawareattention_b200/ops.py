@@ -579,7 +579,7 @@ def _gemm_ws(dev, stream=None):
     once - on two streams, in a graph beside eager ones - have two; a captured one's is its graph's."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(_GEMM_WS_BYTES, dtype=torch.uint8, device=dev)
-    key = dev, _stream(dev) if stream is None else stream
+    key = dev.index, _stream(dev) if stream is None else stream
     ws = _GEMM_WS.get(key)
     if ws is None:
         with torch.inference_mode(False):

@@ -119,7 +119,7 @@ class EdgeWeights:
 
     def __init__(self, attn):
         from .attention import Kept
-        own = Kept()
+        own = Kept(streams=False)
         lin0, lin2 = attn.edge_mlp[0], attn.edge_mlp[2]
         self.first, self.second = (
             (w, b, own if w.requires_grad or b.requires_grad else attn._copies) for w, b in ((lin0.weight, lin0.bias), (lin2.weight, lin2.bias)))

@@ -251,3 +251,32 @@ def test_one_frozen_layer_keeps_its_copies():
     m(x, attn_mask=tril(32))[0].float().sum().backward()
     m.edge_mlp.requires_grad_(True)
     assert same(m, x)
+
+
+@pytest.mark.parametrize("D,H,dtype,mode", [(192, 4, torch.bfloat16, "bf16"), (128, 4, torch.bfloat16, "split8"), (128, 4, torch.float32, "auto")])
+def test_copies_are_waited_for(D, H, dtype, mode):
+    """A forward on one stream lays the weights out behind other work; one on another stream, at once, waits for the copies,
+    and they stay until it has read them."""
+    m = module(D, H, dtype, seed=13)
+    m.generator_precision = mode
+    x, mask = torch.randn(1, 32, D, device=DEV).to(dtype), tril(32)
+    with torch.no_grad():
+        want = m(x, attn_mask=mask)[0]
+        one, two = torch.cuda.Stream(), torch.cuda.Stream()
+        for first, second in ((one, two), (two, one)):
+            m.weights_changed()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(first):
+                if mode != "split8":                              # (which reads a number on the host as it lays out)
+                    torch.cuda._sleep(50_000_000)
+                a = m(x, attn_mask=mask)[0]
+            with torch.cuda.stream(second):
+                torch.cuda._sleep(5_000_000)
+                b = m(x, attn_mask=mask)[0]
+            m.weights_changed()
+            with torch.cuda.stream(first):
+                junk = [torch.full((1 << 18,), 9.0, device=DEV) for _ in range(20)]
+            torch.cuda.synchronize()
+            assert torch.equal(a, want) and torch.equal(b, want)
+            del junk
+    ops.check_status()
