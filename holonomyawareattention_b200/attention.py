@@ -45,12 +45,10 @@ def _is_exact_tril(mask: Optional[torch.Tensor], L: int) -> bool:
     return bool(torch.equal(mask.bool(), tril))
 
 
-@contextlib.contextmanager
 def _laying_out():
-    """Copies of weights are made without gradients but outside inference mode, whatever mode the call that needs them has:
-    a later one may save them for its backward pass."""
-    with torch.inference_mode(False), torch.no_grad():
-        yield
+    """Copies of (detached) weights are made outside inference mode, whatever mode the call that needs them has: a later one
+    may save them for its backward pass."""
+    return torch.inference_mode(False) if torch.is_inference_mode_enabled() else contextlib.nullcontext()
 
 
 class Kept:
